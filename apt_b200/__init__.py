@@ -23,5 +23,6 @@ from .ops import (  # noqa: F401
     register_min_vids, relabel_csc, rows_gather, rows_scatter, sddmm_u_add_v, sddmm_u_mul_v, set_sampling,
     gat_edge_softmax_sum, gat_edge_softmax_sum_backward, GATEdgeSoftmaxSum, shuffle_seeds, sp_feat_shuffle, sp_sample_and_shuffle, sp_sample_shuffle_src, spmm_copy_e_sum, spmm_copy_u_sum, spmm_u_mul_e_sum, src_to_vir,
     srcdst_to_vir, unique_sorted,
+    Dropout, GroupNormAct, GroupedLinear, dropout, group_norm_act, group_norm_act_backward, grouped_linear, grouped_linear_backward,
 )
 from .sampler import Block, DPNeighborSampler, MPSampler, MixedNeighborSampler, SPGATSampler, SPVirtualSampler, create_block  # noqa: F401

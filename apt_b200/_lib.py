@@ -23,7 +23,9 @@ FLAG_ID_OUT_OF_RANGE, FLAG_FEAT_NOT_EXIST, FLAG_ZERO_DEGREE, FLAG_TABLE_FULL, FL
 FLAG_NOT_GROUPED = 32
 FLAG_SIZE_MISMATCH = 64
 FLAG_COPY_TIMEOUT = 128
+FLAG_BAD_OFFSETS = 256
 F32, BF16, F16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 IPC_HANDLE_BYTES = 64
 
 P = c_void_p
@@ -107,6 +109,15 @@ PROTOTYPES = {
     "apt_cached_access": (c_int, [P, c_int64, P, c_int64, P, P]),
     "apt_rows_gather": (c_int, [P, P, c_int64, c_int64, P, P]),
     "apt_rows_scatter": (c_int, [P, P, c_int64, c_int64, P, P]),
+    "apt_dropout": (c_int, [c_int, P, c_int64, c_double, c_uint64, c_uint32, P, P]),
+    "apt_group_norm_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int64, c_int]),
+    "apt_group_norm_forward": (c_int, [c_int, c_int, P, c_int64, c_int64, c_int, P, c_int64, c_double, c_int, P, P, c_double, c_uint64, c_uint32,
+                                       P, P, P, c_size_t, P, P]),
+    "apt_group_norm_backward": (c_int, [c_int, c_int, P, P, c_int64, c_int64, c_int, P, c_int64, c_double, c_int, P, P, c_double, c_uint64,
+                                        c_uint32, P, P, P, P, P, c_size_t, P, P]),
+    "apt_grouped_linear_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int64, c_int]),
+    "apt_grouped_linear_forward": (c_int, [c_int, P, c_int64, c_int64, P, P, c_int64, P, c_int64, P, P, c_size_t, P, P]),
+    "apt_grouped_linear_backward": (c_int, [c_int, P, c_int64, c_int64, P, c_int64, P, c_int64, P, P, P, P, P, c_size_t, P, P]),
     "apt_p2p_create": (c_int, [c_int, c_int, c_size_t, ctypes.POINTER(P), P]),
     "apt_p2p_attach": (c_int, [P, c_int, P]),
     "apt_p2p_attach_ptr": (c_int, [P, c_int, P]),

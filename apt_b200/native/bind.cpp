@@ -298,6 +298,221 @@ struct GatFunction : public torch::autograd::Function<GatFunction> {
   }
 };
 
+// ------------------------------------------------------------------------------- the dense half of a layer
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+Tensor given(const OptTensor& t) { return t && t->defined() ? *t : Tensor(); }
+const void* data_or_null(const Tensor& t) { return t.defined() ? data(t) : nullptr; }
+void* mut_or_null(const Tensor& t) { return t.defined() ? mut(t) : nullptr; }
+
+int float_code(const char* who, const Tensor& t) {
+  const int code = dtype_code(t.scalar_type());
+  if (code < 0) fail(std::string(who) + ": unsupported dtype " + dtype_name(t));
+  return code;
+}
+void probability(const char* who, double p) {
+  if (!(p >= 0.0 && p <= 1.0)) fail(std::string(who) + ": p = " + std::to_string(p) + " is no probability");
+}
+void same_device(const char* who, const Tensor& a, const Tensor& b, const char* name) {
+  if (b.defined() && b.device() != a.device()) fail(std::string(who) + ": " + name + " is on another device than the rows");
+}
+
+Tensor dropout(const Tensor& x_in, double p, int64_t key, int64_t call) {
+  const Tensor x = cuda(x_in, "x");
+  const int code = float_code("dropout", x);
+  probability("dropout", p);
+  Tensor out = at::empty(x.sizes(), x.options());
+  check(apt_dropout(code, data(x), x.numel(), p, (uint64_t)key, (uint32_t)call, mut(out), stream()));
+  return out;
+}
+struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, double p, int64_t key, int64_t call) {
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["key"] = key;
+    ctx->saved_data["call"] = call;
+    return dropout(x, p, key, call);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    return {dropout(grads[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["key"].toInt(), ctx->saved_data["call"].toInt()), Tensor(), Tensor(),
+            Tensor()};
+  }
+};
+
+// What a call of the group norm is beside its tensors.
+struct NormSettings {
+  int64_t groups, act;
+  double eps, p;
+  int64_t key, call;
+};
+struct NormProblem {
+  Tensor x, weight, bias, offsets;
+  int code, param_code;
+  int64_t rows, dim, segments;
+};
+
+NormProblem norm_problem(const Tensor& x_in, const Tensor& weight, const Tensor& bias, const Tensor& offsets, const NormSettings& s) {
+  NormProblem q;
+  q.x = cuda(x_in, "x");
+  q.code = q.param_code = float_code("group_norm_act", q.x);
+  if (q.x.dim() < 2) fail("group_norm_act: x must have rows and channels, got " + std::to_string(q.x.dim()) + " dimension(s)");
+  q.dim = q.x.size(-1);
+  if (q.dim == 0) fail("group_norm_act: x has no channels");
+  q.rows = q.x.numel() / q.dim;
+  if (s.groups < 1 || q.dim % s.groups)
+    fail("group_norm_act: " + std::to_string(q.dim) + " channels are no whole number of " + std::to_string(s.groups) + " groups");
+  probability("group_norm_act", s.p);
+  if (!(s.eps >= 0.0)) fail("group_norm_act: eps must not be negative");
+  q.segments = q.rows ? q.x.size(0) : 0;
+  if (offsets.defined()) {
+    if (q.x.dim() != 2) fail("group_norm_act: offsets go with rows in two dimensions, got " + std::to_string(q.x.dim()));
+    q.offsets = ids(offsets, "offsets");
+    if (q.offsets.dim() != 1 || q.offsets.numel() < 2) fail("group_norm_act: offsets must hold the ends of one group at least");
+    q.segments = q.offsets.numel() - 1;
+    same_device("group_norm_act", q.x, q.offsets, "offsets");
+  }
+  for (auto [from, to, name] : {std::tuple<const Tensor*, Tensor*, const char*>{&weight, &q.weight, "weight"}, {&bias, &q.bias, "bias"}}) {
+    if (!from->defined()) continue;
+    *to = cuda(*from, name);
+    if (to->dim() != 1 || to->numel() != q.dim) fail(std::string("group_norm_act: ") + name + " must have one value a channel");
+    if (to->scalar_type() != q.x.scalar_type() && to->scalar_type() != at::kFloat)
+      fail(std::string("group_norm_act: ") + name + " of " + dtype_name(*to) + " beside x of " + dtype_name(q.x));
+    same_device("group_norm_act", q.x, *to, name);
+    q.param_code = dtype_code(to->scalar_type());
+  }
+  if (q.weight.defined() && q.bias.defined() && q.weight.scalar_type() != q.bias.scalar_type())
+    fail("group_norm_act: weight and bias must have the same dtype");
+  return q;
+}
+
+// (out, stats)
+std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& offsets, const NormSettings& s,
+                                        const Tensor& words) {
+  const NormProblem q = norm_problem(x, weight, bias, offsets, s);
+  Tensor out = at::empty(q.x.sizes(), q.x.options()), stats = at::empty({q.segments, s.groups, 2}, q.x.options().dtype(at::kFloat));
+  const size_t bytes = apt_group_norm_workspace_bytes(q.rows, q.dim, (int)s.groups, q.segments, 0);
+  const Tensor ws = scratch(q.x, std::max<size_t>(bytes, 16));
+  check(apt_group_norm_forward(q.code, q.param_code, data(q.x), q.rows, q.dim, (int)s.groups, q.offsets.defined() ? ptr(q.offsets) : nullptr, q.segments,
+                               s.eps, (int)s.act, data_or_null(q.weight), data_or_null(q.bias), s.p, (uint64_t)s.key, (uint32_t)s.call, mut(out),
+                               (float*)mut(stats), ws.mutable_data_ptr(), ws.numel(), status_word(words), stream()));
+  return {out, stats};
+}
+
+// Gradients of x, weight and bias (undefined where that is).
+std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& offsets, const Tensor& stats_in,
+                                                 const Tensor& grad_in, const NormSettings& s, bool want_weight, bool want_bias, const Tensor& words) {
+  const NormProblem q = norm_problem(x, weight, bias, offsets, s);
+  const Tensor grad = cuda(grad_in, "grad_out"), stats = cuda(stats_in, "stats", at::kFloat, "torch.float32");
+  if (grad.scalar_type() != q.x.scalar_type() || grad.sizes() != q.x.sizes())
+    fail("group_norm_act_backward: grad_out must be like x");
+  if (stats.numel() != q.segments * s.groups * 2) fail("group_norm_act_backward: stats are not those of this call");
+  Tensor grad_x = at::empty(q.x.sizes(), q.x.options()), grad_weight, grad_bias;
+  if (q.weight.defined() && want_weight) grad_weight = at::empty({q.dim}, q.weight.options());
+  if (q.bias.defined() && want_bias) grad_bias = at::empty({q.dim}, q.bias.options());
+  const size_t bytes = apt_group_norm_workspace_bytes(q.rows, q.dim, (int)s.groups, q.segments, 1);
+  const Tensor ws = scratch(q.x, std::max<size_t>(bytes, 16));
+  check(apt_group_norm_backward(q.code, q.param_code, data(q.x), data(grad), q.rows, q.dim, (int)s.groups, q.offsets.defined() ? ptr(q.offsets) : nullptr,
+                                q.segments, s.eps, (int)s.act, data_or_null(q.weight), data_or_null(q.bias), s.p, (uint64_t)s.key, (uint32_t)s.call,
+                                (const float*)data(stats), mut(grad_x), mut_or_null(grad_weight), mut_or_null(grad_bias), ws.mutable_data_ptr(),
+                                ws.numel(), status_word(words), stream()));
+  return {grad_x, grad_weight, grad_bias};
+}
+
+struct NormFunction : public torch::autograd::Function<NormFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& weight_in, const OptTensor& bias_in,
+                        const OptTensor& offsets_in, int64_t groups, int64_t act, double eps, double p, int64_t key, int64_t call, const Tensor& words) {
+    const Tensor weight = given(weight_in), bias = given(bias_in), offsets = given(offsets_in);
+    auto [out, stats] = norm_forward(x, weight, bias, offsets, {groups, act, eps, p, key, call}, words);
+    ctx->save_for_backward({x, weight, bias, offsets, stats});
+    ctx->saved_data["settings"] = std::vector<int64_t>{groups, act, key, call};
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["words"] = words;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    const auto s = ctx->saved_data["settings"].toIntVector();
+    auto [gx, gw, gb] = norm_backward(v[0], v[1], v[2], v[3], v[4], grads[0],
+                                      {s[0], s[1], ctx->saved_data["eps"].toDouble(), ctx->saved_data["p"].toDouble(), s[2], s[3]},
+                                      wants_grad(v[1]), wants_grad(v[2]), ctx->saved_data["words"].toTensor());
+    torch::autograd::variable_list r(11);
+    r[0] = gx, r[1] = gw, r[2] = gb;
+    return r;
+  }
+};
+
+struct LinearProblem {
+  Tensor x, weight, bias, offsets;
+  int code;
+  int64_t rows, dim, out_dim, groups;
+};
+LinearProblem linear_problem(const char* who, const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& bias) {
+  LinearProblem q;
+  q.x = cuda(x, "x");
+  q.weight = cuda(weight, "weight");
+  q.offsets = ids(offsets, "offsets");
+  q.code = float_code(who, q.x);
+  if (q.x.dim() != 2 || q.weight.dim() != 3 || q.weight.size(2) != q.x.size(1))
+    fail(std::string(who) + ": x must be [rows, dim] and weight [groups, out, dim]");
+  if (q.weight.scalar_type() != q.x.scalar_type()) fail(std::string(who) + ": mixed dtypes " + dtype_name(q.x) + "/" + dtype_name(q.weight));
+  q.rows = q.x.size(0), q.dim = q.x.size(1), q.out_dim = q.weight.size(1), q.groups = q.weight.size(0);
+  if (q.offsets.dim() != 1 || q.offsets.numel() != q.groups + 1)
+    fail(std::string(who) + ": offsets must hold groups + 1 = " + std::to_string(q.groups + 1) + " ends, got " + std::to_string(q.offsets.numel()));
+  if (bias.defined()) {
+    q.bias = cuda(bias, "bias");
+    if (q.bias.dim() != 2 || q.bias.size(0) != q.groups || q.bias.size(1) != q.out_dim) fail(std::string(who) + ": bias must be [groups, out]");
+    if (q.bias.scalar_type() != q.x.scalar_type()) fail(std::string(who) + ": mixed dtypes " + dtype_name(q.x) + "/" + dtype_name(q.bias));
+  }
+  for (const auto& [t, name] : {std::pair<const Tensor*, const char*>{&q.weight, "weight"}, {&q.offsets, "offsets"}, {&q.bias, "bias"}})
+    same_device(who, q.x, *t, name);
+  return q;
+}
+
+Tensor linear_forward(const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& bias, const Tensor& words) {
+  const LinearProblem q = linear_problem("grouped_linear", x, weight, offsets, bias);
+  Tensor out = at::empty({q.rows, q.out_dim}, q.x.options()), ws;
+  const size_t bytes = apt_grouped_linear_workspace_bytes(q.code, q.rows, q.dim, q.out_dim, q.groups, 0);
+  if (bytes) ws = scratch(q.x, bytes);
+  check(apt_grouped_linear_forward(q.code, data(q.x), q.rows, q.dim, data(q.weight), data_or_null(q.bias), q.out_dim, ptr(q.offsets), q.groups, mut(out),
+                                   mut_or_null(ws), bytes, status_word(words), stream()));
+  return out;
+}
+
+// Gradients of x, weight and bias, undefined where not wanted.
+std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& grad_in, bool want_x,
+                                                   bool want_weight, bool want_bias, const Tensor& words) {
+  const LinearProblem q = linear_problem("grouped_linear_backward", x, weight, offsets, Tensor());
+  const Tensor grad = cuda(grad_in, "grad_out");
+  if (grad.scalar_type() != q.x.scalar_type() || grad.dim() != 2 || grad.size(0) != q.rows || grad.size(1) != q.out_dim)
+    fail("grouped_linear_backward: grad_out must be [rows, out] of x's dtype");
+  Tensor grad_x, grad_weight, grad_bias, ws;
+  if (want_x) grad_x = at::empty(q.x.sizes(), q.x.options());
+  if (want_weight) grad_weight = at::empty(q.weight.sizes(), q.weight.options());
+  if (want_bias) grad_bias = at::empty({q.groups, q.out_dim}, q.weight.options());
+  const size_t bytes = apt_grouped_linear_workspace_bytes(q.code, q.rows, q.dim, q.out_dim, q.groups, 1);
+  if (bytes) ws = scratch(q.x, bytes);
+  check(apt_grouped_linear_backward(q.code, data(q.x), q.rows, q.dim, data(q.weight), q.out_dim, ptr(q.offsets), q.groups, data(grad), mut_or_null(grad_x),
+                                    mut_or_null(grad_weight), mut_or_null(grad_bias), mut_or_null(ws), bytes, status_word(words), stream()));
+  return {grad_x, grad_weight, grad_bias};
+}
+
+struct LinearFunction : public torch::autograd::Function<LinearFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& offsets, const OptTensor& bias,
+                        const Tensor& words) {
+    const Tensor b = given(bias);
+    Tensor out = linear_forward(x, weight, offsets, b, words);
+    ctx->save_for_backward({x, weight, offsets});
+    ctx->saved_data["wants"] = std::vector<int64_t>{wants_grad(x), wants_grad(weight), wants_grad(b)};
+    ctx->saved_data["words"] = words;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    const auto wants = ctx->saved_data["wants"].toIntVector();
+    auto [gx, gw, gb] = linear_backward(v[0], v[1], v[2], grads[0], wants[0], wants[1], wants[2], ctx->saved_data["words"].toTensor());
+    return {gx, gw, Tensor(), gb, Tensor()};
+  }
+};
+
 // ------------------------------------------------------------------------------------------------ samplers
 // Page-locked words, also while some stream is being captured.
 Tensor pinned_words(int64_t count) {
@@ -699,5 +914,29 @@ PYBIND11_MODULE(_native, m) {
                         int64_t num_dst, double slope, const Tensor& words) {
     const bool backward = at::GradMode::is_enabled() && (ft.requires_grad() || el.requires_grad() || er.requires_grad());
     return GatFunction::apply(row, col, ft, el, er, num_dst, slope, words, backward);
+  });
+  m.def("dropout", &dropout);
+  m.def("dropout_apply", [](const Tensor& x, double p, int64_t key, int64_t call) { return DropoutFunction::apply(x, p, key, call); });
+  m.def("norm_forward", [](const Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& offsets, int64_t groups, int64_t act,
+                           double eps, double p, int64_t key, int64_t call, const Tensor& words) {
+    return norm_forward(x, given(weight), given(bias), given(offsets), {groups, act, eps, p, key, call}, words);
+  });
+  m.def("norm_backward", [](const Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& offsets, const Tensor& stats,
+                            const Tensor& grad, int64_t groups, int64_t act, double eps, double p, int64_t key, int64_t call, const Tensor& words) {
+    return norm_backward(x, given(weight), given(bias), given(offsets), stats, grad, {groups, act, eps, p, key, call}, true, true, words);
+  });
+  m.def("norm_apply", [](const Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& offsets, int64_t groups, int64_t act,
+                         double eps, double p, int64_t key, int64_t call, const Tensor& words) {
+    return NormFunction::apply(x, weight, bias, offsets, groups, act, eps, p, key, call, words);
+  });
+  m.def("linear_forward", [](const Tensor& x, const Tensor& weight, const Tensor& offsets, const OptTensor& bias, const Tensor& words) {
+    return linear_forward(x, weight, offsets, given(bias), words);
+  });
+  m.def("linear_backward", [](const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& grad, bool want_x, bool want_weight,
+                              bool want_bias, const Tensor& words) {
+    return linear_backward(x, weight, offsets, grad, want_x, want_weight, want_bias, words);
+  });
+  m.def("linear_apply", [](const Tensor& x, const Tensor& weight, const Tensor& offsets, const OptTensor& bias, const Tensor& words) {
+    return LinearFunction::apply(x, weight, offsets, bias, words);
   });
 }

@@ -272,6 +272,7 @@ def _flag_text(flags):
                                 "exchange refuses further use: call init() again on every rank, behind a barrier",
         _lib.FLAG_NOT_GROUPED: "edges of a block are not grouped by destination",
         _lib.FLAG_SIZE_MISMATCH: "a peer sent another number of rows than the reduction expects",
+        _lib.FLAG_BAD_OFFSETS: "ends of row groups do not ascend from 0 to at most the number of rows",
         _lib.FLAG_COPY_TIMEOUT: "input rows of a sum did not reach shared memory in time; some of its rows are zero",
     }
     return ", ".join(v for k, v in names.items() if flags & k)
@@ -1040,6 +1041,92 @@ class GATEdgeSoftmaxSum:
     @staticmethod
     def apply(coo_row, coo_col, ft, el, er, num_dst, negative_slope=0.2):
         return _native.gat_apply(coo_row, coo_col, ft, el, er, int(num_dst), float(negative_slope), STATE.words())
+
+
+# -------------------------------------------------------- the dense half of a layer
+# The reference's models leave it to PyTorch (python/npc/model/sage_model.py, gatconv.py). Rows may come in ragged groups (node
+# types, experts, graphs of a batch): group g has the rows [offsets[g], offsets[g + 1]) of CUDA int64 offsets, so that the host
+# never has to know how long the groups of a mini-batch are. Rows from offsets[-1] on belong to no group and give zeros. Offsets
+# that do not ascend from 0 to at most the number of rows raise at the next host read (check_status).
+_ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
+
+
+def _activation(act: str) -> int:
+    if act not in _ACTIVATIONS:
+        raise RuntimeError(f"group_norm_act: unknown activation {act!r} (one of {', '.join(_ACTIVATIONS)})")
+    return _ACTIVATIONS[act]
+
+
+def _stream_key(key: int, call_id: int) -> Tuple[int, int]:
+    """The two numbers of a generator's stream as the library takes them (64 and 32 bits)."""
+    key &= (1 << 64) - 1
+    return key - (1 << 64 if key >> 63 else 0), int(call_id) & 0xFFFFFFFF
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[r] = x[r] @ weight[g].T + bias[g] for the rows r of every group g: x [R, K], weight [G, N, K], bias [G, N] of one dtype
+    (float32, bfloat16 or float16), offsets [G + 1]; out [R, N]. Sums are in fp32 and rounded once."""
+    return _native.linear_forward(x, weight, offsets, bias, STATE.words())
+
+
+def grouped_linear_backward(x, weight, offsets, grad_out, want_x: bool = True, want_weight: bool = True, want_bias: bool = True):
+    """Gradients of grouped_linear for grad_out [R, N]: (grad_x, grad_weight, grad_bias), None where not wanted. A group without
+    rows has gradients of zero."""
+    return _native.linear_backward(x, weight, offsets, grad_out, bool(want_x), bool(want_weight), bool(want_bias), STATE.words())
+
+
+class GroupedLinear:
+    """grouped_linear with its backward: ``out = GroupedLinear.apply(x, weight, offsets, bias)`` (an autograd function on the C++ side)."""
+
+    @staticmethod
+    def apply(x, weight, offsets, bias=None):
+        return _native.linear_apply(x, weight, offsets, bias, STATE.words())
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                   offsets: Optional[torch.Tensor] = None, eps: float = 1e-5, act: str = "none", p: float = 0.0, key: int = 0,
+                   call_id: int = 0, return_stats: bool = False):
+    """dropout(act(group_norm(x) * weight + bias)), channels last: mean and biased variance over num_groups runs of neighbouring
+    channels and, for 2-D x [R, C], over each row by itself or with `offsets` over the rows of each ragged group; for x [B, ..., C]
+    over everything between the first and the last dimension. act: "none", "relu", "silu" or "gelu" (by the error function). weight
+    and bias [C] of x's dtype or float32. p > 0 drops elements of the result as dropout(..., p, key, call_id) does.
+    return_stats: also mean and 1 / sqrt(variance + eps), float32 [segments, num_groups, 2], which the backward takes."""
+    out, stats = _native.norm_forward(x, weight, bias, offsets, int(num_groups), _activation(act), float(eps), float(p),
+                                      *_stream_key(key, call_id), STATE.words())
+    return (out, stats) if return_stats else out
+
+
+def group_norm_act_backward(x, grad_out, stats, num_groups: int, weight=None, bias=None, offsets=None, eps: float = 1e-5, act: str = "none",
+                            p: float = 0.0, key: int = 0, call_id: int = 0):
+    """Gradients of group_norm_act for grad_out like x and the forward's stats: (grad_x, grad_weight, grad_bias), the latter two
+    None without their parameter."""
+    return _native.norm_backward(x, weight, bias, offsets, stats, grad_out, int(num_groups), _activation(act), float(eps), float(p),
+                                 *_stream_key(key, call_id), STATE.words())
+
+
+class GroupNormAct:
+    """group_norm_act with its backward: ``y = GroupNormAct.apply(x, num_groups, weight, bias, offsets, eps, act, p, key, call_id)``
+    (an autograd function on the C++ side; the mask of the dropout is made anew in the backward)."""
+
+    @staticmethod
+    def apply(x, num_groups, weight=None, bias=None, offsets=None, eps=1e-5, act="none", p=0.0, key=0, call_id=0):
+        return _native.norm_apply(x, weight, bias, offsets, int(num_groups), _activation(act), float(eps), float(p),
+                                  *_stream_key(key, call_id), STATE.words())
+
+
+def dropout(x: torch.Tensor, p: float, key: int, call_id: int = 0) -> torch.Tensor:
+    """x / (1 - p) where the element's random word is at least p 2^32, else 0. The words are the Philox4x32-10 stream (key, call_id):
+    element i, counted row by row, has word i % 4 of counter (i / 4 low, i / 4 high, call_id, 0x64726f70). Nothing is stored: the
+    gradient is dropout(grad, p, key, call_id). Another layer or step takes another call_id."""
+    return _native.dropout(x, float(p), *_stream_key(key, call_id))
+
+
+class Dropout:
+    """dropout with its backward: ``y = Dropout.apply(x, p, key, call_id)`` (an autograd function on the C++ side)."""
+
+    @staticmethod
+    def apply(x, p, key, call_id=0):
+        return _native.dropout_apply(x, float(p), *_stream_key(key, call_id))
 
 
 # ------------------------------------------------------------------ row movers

@@ -54,6 +54,7 @@ typedef enum apt_dtype { APT_F32 = 0, APT_BF16 = 1, APT_F16 = 2 } apt_dtype;
 #define APT_FLAG_PEER_TIMEOUT    16 /* a peer's flag did not arrive in time */
 #define APT_FLAG_NOT_GROUPED     32 /* a block operator got edges not grouped by destination */
 #define APT_FLAG_SIZE_MISMATCH   64 /* a peer sent another number of rows than the reduction expects */
+#define APT_FLAG_BAD_OFFSETS     256 /* ends of row groups that do not ascend from 0 to at most the number of rows */
 #define APT_FLAG_COPY_TIMEOUT    128 /* input rows did not reach shared memory in time: the sums of the warp that waited are zero */
 
 const char* apt_last_error(void);
@@ -800,6 +801,59 @@ int apt_p2p_alltoall_fused(apt_p2p* ctx, const void* src, const int64_t* src_ind
                            int64_t num_dst_rows, int64_t row_bytes, int chunks,
                            void* dst, int32_t* status_word, int64_t timeout_ns,
                            void* stream);
+
+/* ------------------------------------------------- the dense half of a layer
+ * What a layer does with the aggregated rows. Rows may come in ragged groups
+ * (node types, experts, graphs of a batch): group g has the rows
+ * [offsets[g], offsets[g + 1]) of int64_t offsets[groups + 1] in device memory,
+ * offsets[0] == 0. Rows from offsets[groups] on belong to no group: what is
+ * computed for them is zero. Offsets that do not ascend or pass the number of
+ * rows set APT_FLAG_BAD_OFFSETS; nothing outside the buffers is touched, and
+ * the results are unspecified. Sums are in fp32 and rounded once. No
+ * counterpart in the reference, whose models leave this to PyTorch
+ * (python/npc/model/sage_model.py). */
+
+/* out[i] = x[i] / (1 - p) where word i of the Philox4x32-10 stream (key, call_id)
+ * is at least floor(p 2^32), else 0 (whatever x[i] is): counter (i / 4 low, i / 4
+ * high, call_id, 0x64726f70), word i % 4. The gradient is the same map of the
+ * gradient. in and out do not overlap. */
+int apt_dropout(int dtype, const void* in, int64_t n, double p, uint64_t key, uint32_t call_id, void* out, void* stream);
+
+typedef enum apt_activation { APT_ACT_NONE = 0, APT_ACT_RELU = 1, APT_ACT_SILU = 2, APT_ACT_GELU = 3 } apt_activation;
+
+/* out = dropout(act(norm(x) * weight + bias)) of x[rows, dim]: mean and (biased)
+ * variance over the rows of a segment and the dim / groups neighbouring channels
+ * of a group. Segments are ragged groups, or with offsets NULL `segments` equal
+ * blocks of rows (as many as rows: every row by itself). weight and bias [dim]
+ * of param_dtype (dtype or APT_F32), or NULL. p == 0: no dropout; else as
+ * apt_dropout over the elements of out. stats [segments, groups, 2] receives mean
+ * and 1 / sqrt(variance + eps), which the backward starts from. It gives grad_x,
+ * and grad_weight and grad_bias [dim] of param_dtype unless NULL. */
+size_t apt_group_norm_workspace_bytes(int64_t rows, int64_t dim, int groups, int64_t segments, int backward);
+int apt_group_norm_forward(int dtype, int param_dtype, const void* x, int64_t rows, int64_t dim, int groups, const int64_t* offsets,
+                           int64_t segments, double eps, int act, const void* weight, const void* bias, double p,
+                           uint64_t key, uint32_t call_id, void* out, float* stats, void* workspace,
+                           size_t workspace_bytes, int32_t* status_word, void* stream);
+int apt_group_norm_backward(int dtype, int param_dtype, const void* x, const void* grad_out, int64_t rows, int64_t dim, int groups,
+                            const int64_t* offsets, int64_t segments, double eps, int act, const void* weight,
+                            const void* bias, double p, uint64_t key, uint32_t call_id, const float* stats,
+                            void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                            size_t workspace_bytes, int32_t* status_word, void* stream);
+
+/* out[r] = x[r] weight[g]^T + bias[g] for the rows of every group g: x [rows, dim],
+ * weight [groups, out_dim, dim], bias [groups, out_dim] or NULL, out [rows, out_dim].
+ * Backward: grad_x [rows, dim], grad_weight, grad_bias like their parameters;
+ * each unless NULL. */
+#define APT_GROUPED_LINEAR_MAX_GROUPS 4096
+#define APT_GROUPED_LINEAR_MAX_DIM 65536
+size_t apt_grouped_linear_workspace_bytes(int dtype, int64_t rows, int64_t dim, int64_t out_dim, int64_t groups, int backward);
+int apt_grouped_linear_forward(int dtype, const void* x, int64_t rows, int64_t dim, const void* weight, const void* bias,
+                               int64_t out_dim, const int64_t* offsets, int64_t groups, void* out, void* workspace,
+                               size_t workspace_bytes, int32_t* status_word, void* stream);
+int apt_grouped_linear_backward(int dtype, const void* x, int64_t rows, int64_t dim, const void* weight, int64_t out_dim,
+                                const int64_t* offsets, int64_t groups, const void* grad_out, void* grad_x,
+                                void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                                int32_t* status_word, void* stream);
 
 /* --------------------------------------------------------- setup utilities
  * Not on the timed path; they prepare the synthetic graphs of the benchmark

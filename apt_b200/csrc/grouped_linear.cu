@@ -1,109 +1,597 @@
-// Products of rows in ragged groups with the weights of their group.
+// Products of rows in ragged groups with the weights of their group, on the tensor cores.
 //
 //   out[r, n] = sum_k x[r, k] w[g, n, k] + b[g, n]      rows r of group g
 //   dx[r, k]  = sum_n dy[r, n] w[g, n, k]
 //   dw[g, n, k] = sum_{r in g} dy[r, n] x[r, k],   db[g, n] = sum_{r in g} dy[r, n]
 //
-// Where the groups end is on the device only: the grid is for the most tiles there can be, and a block finds its tile from the ends.
+// One persistent kernel for all three (k_grouped), a block an SM: a warp has boxes of both operands copied to a ring of stages in
+// shared memory, one thread issues the products of a stage into tensor memory, four warps bring finished tiles out. Where the groups
+// end is on the device only, so every block makes the list of tiles from the ends and its warps walk it.
+//
+// Operands stay as they are in memory, row by row; whether rows run along the contraction or across it is a bit of the product. A box
+// that reaches past a matrix is filled with zeros. Past the end of a group within a matrix it has the next group's rows: in out and dx those are
+// rows of the tile that are not written, in dw they are part of the sum and are overwritten with zeros first, in both operands.
+//
+// fp32: x = h + m + l exactly, each bf16 (the upper 8, the next 8 and the last 8 bits: cut off, so nothing overflows). Of the nine
+// products of two such sums the six of more than 2^-24 of the whole are made: h h in one sum, the five small ones in another, which loses
+// nothing to the large one's roundings. Eight warps take the stages apart. A result that is not finite (infinities fall apart into NaN)
+// is computed again from the operands.
+#include <algorithm>
+
 #include "dense.cuh"
+#include "umma.cuh"
+#include "widen.cuh"
 
 namespace apt {
 
-constexpr int kTile = 64, kStep = 16;
+enum GroupedMode { kOut = 0, kGradX = 1, kGradW = 2 };
 
-// The group and the first row of row tile `tile`, counted group by group; tiles behind the last group's are those of the rows that
-// belong to none (group == groups). False: there is no such tile.
-__device__ __forceinline__ bool find_tile(const int64_t* offsets, int groups, int64_t rows, int64_t tile, int* group, RowRange* range) {
-  for (int g = 0; g <= groups; ++g) {
-    RowRange r = {0, rows};
-    if (g < groups) r = group_rows(offsets, g, rows);
-    else r.begin = min(max(offsets[groups], (int64_t)0), rows);
-    const int64_t n = (r.end - r.begin + kTile - 1) / kTile;
-    if (tile < n) {
-      *group = g;
-      *range = {r.begin + tile * kTile, min(r.begin + (tile + 1) * kTile, r.end)};
+constexpr int kTileM = 128;                  // rows of a product
+constexpr int kStageBytes = 227 * 1024;      // shared memory of a block
+constexpr int kAccColumns = 256;             // tensor memory of a tile: two of them, or one and the sums of the bias
+constexpr int kMaxStages = 8;
+
+template <typename T, int MODE>
+struct GroupedTraits {
+  static constexpr bool kSplit = sizeof(T) == 4;
+  static constexpr bool kMnA = MODE == kGradW, kMnB = MODE != kOut;
+  static constexpr int kBlock = kSplit ? 32 : 64;              // of the contraction in a stage
+  static constexpr int kBox = 128 / (int)sizeof(T);            // elements of a box's row
+  static constexpr int kMostN = kSplit ? 128 : 256;            // columns of a tile
+  static constexpr int kThreads = kSplit ? 512 : 256;
+  static constexpr int kPieces = kSplit ? 3 : 1;
+  // bytes of a tile of n rows (or columns) in a stage as copied, and of one bf16 piece of it
+  static __host__ __device__ constexpr int copied(int n, bool mn) { return mn ? (n + kBox - 1) / kBox * kBlock * 128 : n * 128; }
+  static __host__ __device__ constexpr int piece(int n, bool mn) { return mn ? (n + 63) / 64 * kBlock * 128 : n * kBlock * 2; }
+};
+
+struct GroupedCall {
+  const int64_t* offsets;
+  int64_t rows;
+  int groups;
+  int num_m, num_n, num_k;      // num_m: rows of dw, num_k: contraction of out and dx
+  int tile_m, tile_n, tiles_m, tiles_n;
+  int copied_stages, piece_stages;
+  int64_t ranges;               // dw: into how many runs of stages the work is cut at most
+  const void *a, *b;            // the operands, as the copies read them
+  int64_t pitch_a, pitch_b;     // elements
+  const void* bias;
+  void *out, *grad_bias;
+  float *partial, *partial_bias;
+  int64_t* plan;                // dw: for k_join_weights
+  int32_t* status;
+};
+
+// ---- the list of tiles ------------------------------------------------------------
+struct GroupedItem {
+  int g;
+  int64_t row;                  // first row of x
+  int rows;                     // of the group from there on, in out and dx at most tile_m
+  int m0, n0, stages;
+  int64_t piece;                // dw: number of the partial sum, -1: all of the sum
+};
+
+// Runs of stages of dw: every run is as long as any other within one, whatever the groups are. A run has all stages of the tiles and
+// groups in its middle; two at most, at its ends, it has parts of.
+struct GroupedRuns {
+  int64_t units, runs;
+  __device__ __forceinline__ int64_t begin(int64_t v) const { return v * units / runs; }
+  __device__ __forceinline__ int64_t of(int64_t u) const { return ((u + 1) * runs - 1) / units; }
+};
+constexpr int kLeastRun = 4;
+__host__ __device__ __forceinline__ GroupedRuns grouped_runs(int64_t units, int64_t most) {
+  const int64_t r = units / kLeastRun;
+  return {units, r < 1 ? 1 : r < most ? r : most};
+}
+
+template <typename T, int MODE>
+struct GroupedWalk {
+  using Tr = GroupedTraits<T, MODE>;
+  const GroupedCall& c;
+  const int* prefix;            // tiles (stages in dw) of the groups before
+  int64_t next, end, step;
+  GroupedRuns runs;
+  __device__ GroupedWalk(const GroupedCall& call, const int* p) : c(call), prefix(p) {
+    if constexpr (MODE == kGradW) {
+      runs = grouped_runs((int64_t)prefix[c.groups] * c.tiles_m * c.tiles_n, c.ranges);
+      step = blockIdx.x;
+      next = end = 0;
+      if (runs.units && step < runs.runs) next = runs.begin(step), end = runs.begin(step + 1);
+    } else {
+      next = blockIdx.x, step = gridDim.x, end = (int64_t)prefix[c.groups + 1] * c.tiles_n;
+    }
+  }
+  __device__ __forceinline__ int group_of(int t, int n) const {
+    int lo = 0, hi = n;         // the last group whose prefix is at most t
+    while (hi - lo > 1) {
+      const int m = (lo + hi) / 2;
+      if (prefix[m] <= t) lo = m; else hi = m;
+    }
+    return lo;
+  }
+  __device__ bool take(GroupedItem* item) {
+    if constexpr (MODE == kGradW) {
+      while (next >= end) {
+        step += gridDim.x;
+        if (!runs.units || step >= runs.runs) return false;
+        next = runs.begin(step), end = runs.begin(step + 1);
+      }
+      const int total = prefix[c.groups];
+      const int tile = (int)(next / total), t = (int)(next % total);
+      const int g = group_of(t, c.groups);
+      const int64_t n = min(end - next, (int64_t)(prefix[g + 1] - t));
+      const RowRange r = group_rows(c.offsets, g, c.rows);
+      item->g = g;
+      item->row = r.begin + (int64_t)(t - prefix[g]) * Tr::kBlock;
+      item->rows = (int)min(n * Tr::kBlock, r.end - item->row);
+      item->stages = (int)n;
+      item->m0 = tile / c.tiles_n * kTileM;
+      item->n0 = tile % c.tiles_n * c.tile_n;
+      item->piece = n == prefix[g + 1] - prefix[g] ? -1 : 2 * step + (next != runs.begin(step));
+      next += n;
+      return true;
+    } else {
+      if (next >= end) return false;
+      const int t = (int)(next / c.tiles_n);
+      const int g = group_of(t, c.groups + 1);
+      RowRange r;
+      if (g < c.groups) r = group_rows(c.offsets, g, c.rows);
+      else r.begin = min(max(c.offsets[c.groups], (int64_t)0), c.rows), r.end = c.rows;
+      item->g = g;
+      item->row = r.begin + (int64_t)(t - prefix[g]) * c.tile_m;
+      item->rows = (int)min((int64_t)c.tile_m, r.end - item->row);
+      item->m0 = 0;
+      item->n0 = (int)(next % c.tiles_n) * c.tile_n;
+      item->stages = g < c.groups ? (c.num_k + Tr::kBlock - 1) / Tr::kBlock : 0;      // rows of no group: zeros
+      item->piece = -1;
+      next += step;
       return true;
     }
-    tile -= n;
   }
-  return false;
-}
+};
 
-// acc += A[m, k] B[n, k] over one tile; a thread has 4 x 4 of 64 x 64.
-template <typename T>
-__device__ __forceinline__ void tile_product(const T* a, int64_t am, int64_t ak, int64_t num_m, const T* b, int64_t bn, int64_t bk, int64_t num_n,
-                                             int64_t num_k, float (&acc)[4][4]) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-  for (int64_t k0 = 0; k0 < num_k; k0 += kStep) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-      // the contiguous one of the two indices moves fastest
-      const int m = ak == 1 ? i / kStep : i % kTile, k = ak == 1 ? i % kStep : i / kTile;
-      sa[k][m] = m < num_m && k0 + k < num_k ? Elem<T>::to_f(a[m * am + (k0 + k) * ak]) : 0.0f;
-      const int n = bk == 1 ? i / kStep : i % kTile, l = bk == 1 ? i % kStep : i / kTile;
-      sb[l][n] = n < num_n && k0 + l < num_k ? Elem<T>::to_f(b[n * bn + (k0 + l) * bk]) : 0.0f;
+// ---- taking fp32 apart --------------------------------------------------------------
+struct Pieces {
+  uint4 p[3];
+};
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
+__device__ __forceinline__ float below(float v) { return v - __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+__device__ __forceinline__ Pieces take_apart(float4 a, float4 b) {
+  Pieces r;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    r.p[k] = make_uint4(upper_halves(a.x, a.y), upper_halves(a.z, a.w), upper_halves(b.x, b.y), upper_halves(b.z, b.w));
+    a = make_float4(below(a.x), below(a.y), below(a.z), below(a.w));
+    b = make_float4(below(b.x), below(b.y), below(b.z), below(b.w));
+  }
+  return r;
+}
+// One operand's stage. Its rows (of 128 bytes as copied) run along the contraction, 8 elements of a row a thread, or across it in
+// boxes of 32: 8 elements of one k a thread. `valid`: k's from there on are zero.
+template <bool MN>
+__device__ __forceinline__ void take_stage_apart(const char* copied, char* pieces, int n, int piece_bytes, int valid, int thread) {
+  if constexpr (!MN) {
+    for (int i = thread; i < n * 4; i += 256) {
+      const int r = i >> 2, s = i & 3;
+      const char* const row = copied + r * 128;
+      const Pieces v = take_apart(*(const float4*)(row + (((2 * s) ^ (r & 7)) << 4)), *(const float4*)(row + (((2 * s + 1) ^ (r & 7)) << 4)));
+      char* const to = pieces + r * 64 + ((s ^ ((r >> 1) & 3)) << 4);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *(uint4*)(to + p * piece_bytes) = v.p[p];
     }
-    __syncthreads();
+  } else {
+    for (int i = thread; i < (n + 63) / 64 * 256; i += 256) {
+      const int s = i & 3, k = (i >> 2) & 31, half = (i >> 7) & 1, block = i >> 8;
+      const char* const row = copied + (block * 2 + half) * 4096 + k * 128;
+      float4 lo = make_float4(0.0f, 0.0f, 0.0f, 0.0f), hi = lo;
+      if (k < valid && block * 64 + half * 32 < (n + 31) / 32 * 32) {
+        lo = *(const float4*)(row + (((2 * s) ^ (k & 7)) << 4));
+        hi = *(const float4*)(row + (((2 * s + 1) ^ (k & 7)) << 4));
+      }
+      const Pieces v = take_apart(lo, hi);
+      char* const to = pieces + block * 4096 + k * 128 + (((half * 4 + s) ^ (k & 7)) << 4);
 #pragma unroll
-    for (int k = 0; k < kStep; ++k) {
-      float u[4], v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = sa[k][tm + 16 * i], v[i] = sb[k][tn + 16 * i];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(u[i], v[j], acc[i][j]);
+      for (int p = 0; p < 3; ++p) *(uint4*)(to + p * piece_bytes) = v.p[p];
     }
   }
 }
 
-// Rows against weights: out (w by its rows) or dx (w by its columns).
-template <typename T>
-__global__ void __launch_bounds__(256)
-k_rows_product(const T* __restrict__ in, int64_t rows, int64_t num_k, const T* __restrict__ w, int64_t wn, int64_t wk, int64_t num_n, const T* bias,
-               const int64_t* __restrict__ offsets, int groups, T* __restrict__ out, int32_t* status) {
-  wait_for_previous();
-  if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int g = threadIdx.x; g < groups; g += 256)
-      if (bad_group(offsets, g, rows)) atomicOr(status, APT_FLAG_BAD_OFFSETS);
-  int g;
-  RowRange r;
-  if (!find_tile(offsets, groups, rows, blockIdx.x, &g, &r)) return;
-  const int64_t n0 = (int64_t)blockIdx.y * kTile, here = min((int64_t)kTile, num_n - n0);
-  float acc[4][4] = {};
-  if (g < groups)
-    tile_product(in + r.begin * num_k, num_k, (int64_t)1, r.end - r.begin, w + (int64_t)g * num_n * num_k + n0 * wn, wn, wk, here, num_k, acc);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = r.begin + threadIdx.x / 16 + 16 * i, n = n0 + threadIdx.x % 16 + 16 * j;
-      if (m < r.end && n < num_n) out[m * num_n + n] = Elem<T>::from_f(acc[i][j] + (bias && g < groups ? Elem<T>::to_f(bias[g * num_n + n]) : 0.0f));
-    }
+// A sum that came out infinite or NaN, from the operands.
+template <int MODE>
+__device__ __noinline__ float sum_again(const GroupedCall& c, const GroupedItem& item, int m, int n) {
+  const float *a = (const float*)c.a, *b = (const float*)c.b;
+  int64_t step_a = 1, step_b = 1, count = c.num_k;
+  if (MODE == kGradW) {
+    a += item.row * c.pitch_a + item.m0 + m, b += item.row * c.pitch_b + item.n0 + n;
+    step_a = c.pitch_a, step_b = c.pitch_b, count = item.rows;
+  } else {
+    a += (item.row + m) * c.pitch_a;
+    b += (int64_t)item.g * (MODE == kOut ? c.num_n : c.num_k) * c.pitch_b;
+    if (MODE == kOut) b += (int64_t)(item.n0 + n) * c.pitch_b;
+    else b += item.n0 + n, step_b = c.pitch_b;
+  }
+  float sum = 0.0f;
+  for (int64_t k = 0; k < count && sum == sum; ++k) sum = fmaf(a[k * step_a], b[k * step_b], sum);
+  return sum;
+}
+__device__ __noinline__ float column_again(const GroupedCall& c, const GroupedItem& item, int m) {
+  float sum = 0.0f;
+  for (int k = 0; k < item.rows && sum == sum; ++k) sum += ((const float*)c.a)[(item.row + k) * c.pitch_a + item.m0 + m];
+  return sum;
 }
 
-// dw of one group and tile.
-template <typename T>
-__global__ void __launch_bounds__(256)
-k_weight_product(const T* __restrict__ x, int64_t rows, int64_t dim, const T* __restrict__ grad, int64_t out_dim, const int64_t* __restrict__ offsets,
-                 T* __restrict__ grad_weight) {
-  wait_for_previous();
-  const int g = blockIdx.z;
-  const RowRange r = group_rows(offsets, g, rows);
-  const int64_t n0 = (int64_t)blockIdx.x * kTile, k0 = (int64_t)blockIdx.y * kTile;
-  float acc[4][4] = {};
-  tile_product(grad + r.begin * out_dim + n0, (int64_t)1, out_dim, min((int64_t)kTile, out_dim - n0), x + r.begin * dim + k0, (int64_t)1, dim,
-               min((int64_t)kTile, dim - k0), r.end - r.begin, acc);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + threadIdx.x / 16 + 16 * i, k = k0 + threadIdx.x % 16 + 16 * j;
-      if (n < out_dim && k < dim) grad_weight[((int64_t)g * out_dim + n) * dim + k] = Elem<T>::from_f(acc[i][j]);
+// ---- bringing a tile out -------------------------------------------------------------
+// A warp's 32 rows, 128 bytes of each at a time, through shared memory, so that the stores are whole rows of 128 bytes.
+template <typename T, typename O, int MODE>
+__device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedItem& item, uint32_t acc, bool empty, char* staging, int lane, int warp,
+                                           O* out, int64_t ld, int rows, int columns, const T* bias) {
+  using Tr = GroupedTraits<T, MODE>;
+  constexpr int kWide = 128 / (int)sizeof(O);
+  const int m = warp * 32 + lane, here = min(32, rows - warp * 32);
+  const bool whole = (ld * (int64_t)sizeof(O)) % 16 == 0;
+  O* const first = out + (int64_t)warp * 32 * ld;
+  for (int c0 = 0; c0 < columns; c0 += kWide) {
+#pragma unroll
+    for (int h = 0; h < kWide / 32; ++h) {
+      const int at = c0 + 32 * h;
+      if (at >= columns) break;
+      float v[32];
+      uint32_t wild = 0;
+      if (empty) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = 0.0f;
+      } else {
+        tmem_load_32(acc + ((uint32_t)warp << 21) + at, v);
+        if constexpr (Tr::kSplit) {
+          float small[32];
+          tmem_load_32(acc + ((uint32_t)warp << 21) + Tr::kMostN + at, small);
+          tmem_wait_loads();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            v[k] += small[k];
+            wild |= isfinite(v[k]) ? 0u : 1u << k;
+          }
+        } else {
+          tmem_wait_loads();
+        }
+      }
+      if (bias)
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (at + k < columns) v[k] += Elem<T>::to_f(__ldg(bias + at + k));
+      constexpr int kSlices = 32 * (int)sizeof(O) / 16, kPer = 16 / (int)sizeof(O);
+#pragma unroll
+      for (int s = 0; s < kSlices; ++s) {
+        Pack<O, kPer> p;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) p.v[k] = Elem<O>::from_f(v[s * kPer + k]);
+        *(uint4*)(staging + lane * 128 + (((h * kSlices + s) ^ (lane & 7)) << 4)) = *(const uint4*)&p;
+      }
+      if constexpr (Tr::kSplit) {
+        if (lane < here)
+          for (; wild; wild &= wild - 1) {
+            const int k = __ffs(wild) - 1;
+            if (at + k < columns)
+              *(float*)(staging + lane * 128 + (((k >> 2) ^ (lane & 7)) << 4) + (k & 3) * 4) =
+                  sum_again<MODE>(c, item, m, at + k) + (bias ? Elem<T>::to_f(bias[at + k]) : 0.0f);
+          }
+      }
     }
+    __syncwarp();
+    if (whole) {
+      const int s = lane & 7, col = c0 + s * (16 / (int)sizeof(O));
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += 4) {
+        const int r = r0 + (lane >> 3);
+        if (r < here && col < columns) *(uint4*)(first + r * ld + col) = *(const uint4*)(staging + r * 128 + ((s ^ (r & 7)) << 4));
+      }
+    } else {
+      for (int r = 0; r < here; ++r)
+        for (int k = lane; k < kWide; k += 32) {
+          const int s = k * (int)sizeof(O) / 16, in = k * (int)sizeof(O) % 16;
+          if (c0 + k < columns) first[r * ld + c0 + k] = *(const O*)(staging + r * 128 + ((s ^ (r & 7)) << 4) + in);
+        }
+    }
+    __syncwarp();
+  }
 }
 
+// ---- the kernel ----------------------------------------------------------------------
+template <typename T, int MODE>
+__global__ void __launch_bounds__(GroupedTraits<T, MODE>::kThreads, 1)
+k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GroupedCall c) {
+  using Tr = GroupedTraits<T, MODE>;
+  constexpr int kBuffers = MODE == kGradW ? 1 : 2;
+  extern __shared__ char raw_shared[];
+  __shared__ uint64_t full[kMaxStages], free_[kMaxStages], ready[kMaxStages], used[kMaxStages], acc_full[2], acc_free[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int gave_up_word, scan[33];
+  volatile int* const gave_up = &gave_up_word;
+  char* const shared = (char*)(((uintptr_t)raw_shared + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  const int copied_a = Tr::copied(kTileM, Tr::kMnA), copied_bytes = copied_a + Tr::copied(c.tile_n, Tr::kMnB);
+  const int piece_a = Tr::piece(kTileM, Tr::kMnA), piece_b = Tr::piece(c.tile_n, Tr::kMnB);
+  const int piece_bytes = Tr::kSplit ? 3 * (piece_a + piece_b) : 0;
+  char* const copied = shared;
+  char* const pieces = copied + (size_t)c.copied_stages * copied_bytes;
+  char* const staging = pieces + (size_t)c.piece_stages * piece_bytes;
+  char* const ones = staging + 4 * 4096;
+  int* const prefix = (int*)(ones + (MODE == kGradW ? 2048 : 0));
+
+  if (warp == 1) tmem_alloc(shared_addr(&tmem_slot), 512);
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < kMaxStages; ++k) {
+      barrier_init(shared_addr(full + k), 1);
+      barrier_init(shared_addr(free_ + k), Tr::kSplit ? 8 : 1);
+      barrier_init(shared_addr(ready + k), 8);
+      barrier_init(shared_addr(used + k), 1);
+    }
+    for (int k = 0; k < 2; ++k) barrier_init(shared_addr(acc_full + k), 1), barrier_init(shared_addr(acc_free + k), 4);
+    barrier_init(shared_addr(&drained), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    gave_up_word = 0;
+  }
+  if constexpr (MODE == kGradW) {
+    for (int i = threadIdx.x; i < 512; i += Tr::kThreads) ((uint32_t*)ones)[i] = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+    fence_for_tensor_cores();
+  }
+  wait_for_previous();
+
+  // tiles (stages) of the groups before each; none at all where the ends are no ends
+  int before = 0, bad = 0;
+  for (int g = threadIdx.x; g < c.groups; g += Tr::kThreads) bad |= bad_group(c.offsets, g, c.rows);
+  bad = __syncthreads_or(bad);
+  if (bad && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
+  const int lists = MODE == kGradW ? c.groups : c.groups + 1, unit = MODE == kGradW ? Tr::kBlock : c.tile_m;
+  for (int g0 = 0; g0 < lists; g0 += Tr::kThreads) {
+    const int g = g0 + threadIdx.x;
+    int n = 0;
+    if (g < c.groups) {
+      const RowRange r = group_rows(c.offsets, g, c.rows);
+      n = bad ? 0 : (int)((r.end - r.begin + unit - 1) / unit);
+    } else if (g < lists) {
+      n = bad ? 0 : (int)((c.rows - min(max(c.offsets[c.groups], (int64_t)0), c.rows) + unit - 1) / unit);
+    }
+    int total;
+    const int at = before + block_exclusive_scan(n, scan, &total);
+    if (g < lists) prefix[g] = at;
+    before += total;
+  }
+  if (threadIdx.x == 0) prefix[lists] = before;
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_slot;
+  if constexpr (MODE == kGradW)
+    if (blockIdx.x == 0)
+      for (int g = threadIdx.x; g <= c.groups; g += Tr::kThreads) c.plan[g] = prefix[g];
+
+  GroupedWalk<T, MODE> walk(c, prefix);
+  GroupedItem item;
+  bool fine = true;
+  if (warp == 0) {
+    // ---- copies
+    if (lane == 0) {
+      int stage = 0, loaded = 0;
+      uint32_t phase = 0;
+      while (fine && walk.take(&item)) {
+        const int boxes_a = MODE == kGradW ? (min(kTileM, c.num_m - item.m0) + Tr::kBox - 1) / Tr::kBox : 1;
+        const int boxes_b = Tr::kMnB ? (min(c.tile_n, c.num_n - item.n0) + Tr::kBox - 1) / Tr::kBox : 1;
+        constexpr int kBoxBytes = Tr::kBlock * 128;
+        const uint32_t bytes = (MODE == kGradW ? boxes_a * kBoxBytes : c.tile_m * 128) + (Tr::kMnB ? boxes_b * kBoxBytes : c.tile_n * 128);
+        for (int k = 0; k < item.stages; ++k) {
+          if (!(fine = barrier_wait(shared_addr(free_ + stage), phase ^ 1, gave_up))) break;
+          const uint32_t bar = shared_addr(full + stage), a = shared_addr(copied + (size_t)stage * copied_bytes), b = a + copied_a;
+          barrier_expect(bar, bytes);
+          if constexpr (MODE == kGradW) {
+            const int row = (int)item.row + k * Tr::kBlock;
+            for (int i = 0; i < boxes_a; ++i) copy_box(a + i * kBoxBytes, &map_a, item.m0 + i * Tr::kBox, row, bar);
+            for (int i = 0; i < boxes_b; ++i) copy_box(b + i * kBoxBytes, &map_b, item.n0 + i * Tr::kBox, row, bar);
+          } else {
+            copy_box(a, &map_a, k * Tr::kBlock, (int)item.row, bar);
+            if constexpr (MODE == kOut) {
+              copy_box(b, &map_b, k * Tr::kBlock, item.n0, item.g, bar);
+            } else {
+              for (int i = 0; i < boxes_b; ++i) copy_box(b + i * kBoxBytes, &map_b, item.n0 + i * Tr::kBox, k * Tr::kBlock, item.g, bar);
+            }
+          }
+          ++loaded;
+          if (++stage == c.copied_stages) stage = 0, phase ^= 1;
+        }
+      }
+      // a wait was given up: copies on their way still land
+      if (*gave_up) {
+        int nobody = 0;
+        for (int k = max(0, loaded - c.copied_stages); k < loaded; ++k)
+          barrier_wait(shared_addr(full + k % c.copied_stages), (k / c.copied_stages) & 1, &nobody);
+      }
+    }
+  } else if (warp == 1) {
+    // ---- products
+    const int stages = Tr::kSplit ? c.piece_stages : c.copied_stages;
+    const uint32_t what = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, Tr::kMnB, kTileM, c.tile_n);
+    const uint32_t what_bias = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, false, kTileM, 16);
+    const uint64_t ones_tile = tile_descriptor(shared_addr(ones), 16, 1024, kSwizzle128);
+    int stage = 0, tiles = 0;
+    uint32_t phase = 0;
+    while (fine && walk.take(&item)) {
+      if (!item.stages) continue;
+      const int buffer = tiles % kBuffers;
+      fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_free + buffer), ((tiles / kBuffers) & 1) ^ 1, gave_up));
+      if (!fine) break;
+      tmem_fence_after();
+      const uint32_t acc = tmem + buffer * kAccColumns;
+      const bool sums = MODE == kGradW && c.grad_bias && item.n0 == 0;
+      for (int k = 0; k < item.stages; ++k) {
+        uint64_t* const in = Tr::kSplit ? ready : full;
+        if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(in + stage), phase, gave_up)))) break;
+        tmem_fence_after();
+        const int left = (MODE == kGradW ? item.rows : c.num_k) - k * Tr::kBlock, valid = min(left, Tr::kBlock), steps = (valid + 15) / 16;
+        char* const base = Tr::kSplit ? pieces + (size_t)stage * piece_bytes : copied + (size_t)stage * copied_bytes;
+        if constexpr (MODE == kGradW && !Tr::kSplit) {
+          // rows of the next group
+          if (valid % 16) {
+            const int slices = (steps * 16 - valid) * 8, blocks = copied_bytes / 8192;
+            for (int i = lane; i < slices * blocks; i += 32)
+              *(uint4*)(base + i / slices * 8192 + valid * 128 + i % slices * 16) = make_uint4(0u, 0u, 0u, 0u);
+            fence_for_tensor_cores();
+            __syncwarp();
+          }
+        }
+        if (lane == 0) {
+          const uint32_t a = shared_addr(base), b = a + (Tr::kSplit ? 3 * piece_a : copied_a);
+          const uint64_t tile_a = Tr::kMnA ? tile_descriptor(a, Tr::kBlock * 128, 1024, kSwizzle128)
+                                           : tile_descriptor(a, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
+          const uint64_t tile_b = Tr::kMnB ? tile_descriptor(b, Tr::kBlock * 128, 1024, kSwizzle128)
+                                           : tile_descriptor(b, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
+          for (int s = 0; s < steps; ++s) {
+            const uint64_t da = tile_a + s * ((Tr::kMnA ? 2048 : 32) >> 4), db = tile_b + s * ((Tr::kMnB ? 2048 : 32) >> 4);
+            const bool add = k > 0 || s > 0;
+            tile_product(acc, da, db, what, add);
+            if constexpr (Tr::kSplit) {
+              const uint64_t pa = piece_a >> 4, pb = piece_b >> 4;
+              const uint32_t small = acc + Tr::kMostN;
+              tile_product(small, da, db + pb, what, add);
+              tile_product(small, da + pa, db, what, true);
+              tile_product(small, da + pa, db + pb, what, true);
+              tile_product(small, da, db + 2 * pb, what, true);
+              tile_product(small, da + 2 * pa, db, what, true);
+            }
+            if (sums)
+              for (int p = 0; p < Tr::kPieces; ++p) tile_product(tmem + kAccColumns, da + p * (piece_a >> 4), ones_tile, what_bias, add || p > 0);
+          }
+          products_done(shared_addr((Tr::kSplit ? used : free_) + stage));
+          if (k == item.stages - 1) products_done(shared_addr(acc_full + buffer));
+        }
+        __syncwarp();
+        if (++stage == stages) stage = 0, phase ^= 1;
+      }
+      ++tiles;
+    }
+    if (*gave_up && lane == 0) {
+      int nobody = 0;
+      products_done(shared_addr(&drained));
+      barrier_wait(shared_addr(&drained), 0, &nobody);
+    }
+  } else if (warp >= 4 && warp < 8) {
+    // ---- finished tiles
+    const int w = warp - 4;
+    char* const mine = staging + w * 4096;
+    int tiles = 0;
+    while (fine && walk.take(&item)) {
+      const int buffer = tiles % kBuffers;
+      const bool empty = item.stages == 0;
+      if (!empty) {
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_full + buffer), (tiles / kBuffers) & 1, gave_up));
+        if (!fine) break;
+        tmem_fence_after();
+      }
+      const uint32_t acc = tmem + buffer * kAccColumns;
+      const int columns = min(c.tile_n, c.num_n - item.n0);
+      if constexpr (MODE == kGradW) {
+        const int rows = min(kTileM, c.num_m - item.m0), m = w * 32 + lane;
+        if (w * 32 < rows) {
+          if (item.piece < 0)
+            store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, w, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0, (int64_t)c.num_n, rows, columns,
+                                   (const T*)nullptr);
+          else
+            store_tile<T, float, MODE>(c, item, acc, empty, mine, lane, w, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows, columns, (const T*)nullptr);
+          if (c.grad_bias && item.n0 == 0) {
+            float v = tmem_load_1(tmem + kAccColumns + ((uint32_t)w << 21));
+            tmem_wait_loads();
+            if (m < rows) {
+              if constexpr (Tr::kSplit)
+                if (!isfinite(v)) v = column_again(c, item, m);
+              if (item.piece < 0) ((T*)c.grad_bias)[(int64_t)item.g * c.num_m + item.m0 + m] = Elem<T>::from_f(v);
+              else c.partial_bias[item.piece * kTileM + m] = v;
+            }
+          }
+        }
+      } else if (w * 32 < item.rows) {
+        store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, w, (T*)c.out + item.row * c.num_n + item.n0, (int64_t)c.num_n, item.rows, columns,
+                               c.bias && !empty ? (const T*)c.bias + (int64_t)item.g * c.num_n + item.n0 : (const T*)nullptr);
+      }
+      if (!empty) {
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(shared_addr(acc_free + buffer));
+        ++tiles;
+      }
+    }
+  } else if (Tr::kSplit && warp >= 8) {
+    // ---- fp32 taken apart
+    const int thread = threadIdx.x - 256;
+    int from = 0, to = 0;
+    uint32_t from_phase = 0, to_phase = 0;
+    while (fine && walk.take(&item)) {
+      for (int k = 0; k < item.stages; ++k) {
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up) &&
+                                           barrier_wait(shared_addr(used + to), to_phase ^ 1, gave_up));
+        if (!fine) break;
+        const char* const in = copied + (size_t)from * copied_bytes;
+        char* const out = pieces + (size_t)to * piece_bytes;
+        const int valid = MODE == kGradW ? item.rows - k * Tr::kBlock : Tr::kBlock;
+        take_stage_apart<Tr::kMnA>(in, out, kTileM, piece_a, valid, thread);
+        take_stage_apart<Tr::kMnB>(in + copied_a, out + 3 * piece_a, c.tile_n, piece_b, MODE == kGradW ? valid : Tr::kBlock, thread);
+        fence_for_tensor_cores();
+        __syncwarp();
+        if (lane == 0) {
+          barrier_arrive(shared_addr(free_ + from));
+          barrier_arrive(shared_addr(ready + to));
+        }
+        if (++from == c.copied_stages) from = 0, from_phase ^= 1;
+        if (++to == c.piece_stages) to = 0, to_phase ^= 1;
+      }
+    }
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_free(tmem, 512);
+  if (threadIdx.x == 0 && *gave_up) atomicOr(c.status, APT_FLAG_COPY_TIMEOUT);
+}
+
+// The partial sums of dw and db that make up one, in the order of the rows; zeros for groups without rows.
+template <typename T, int BLOCK>
+__global__ void __launch_bounds__(256)
+k_join_weights(const __grid_constant__ GroupedCall c) {
+  wait_for_previous();
+  const int total = (int)c.plan[c.groups];
+  const GroupedRuns runs = grouped_runs((int64_t)total * c.tiles_m * c.tiles_n, c.ranges);
+  const int64_t per_row = (c.num_n + 3) / 4, weights = (int64_t)c.groups * c.num_m * per_row, all = weights + (c.grad_bias ? (int64_t)c.groups * c.num_m : 0);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const bool weight = i < weights;
+    const int64_t gm = weight ? i / per_row : i - weights;
+    const int n = weight ? (int)(i % per_row) * 4 : 0, g = (int)(gm / c.num_m), m = (int)(gm % c.num_m);
+    const int tile = m / kTileM * c.tiles_n + n / c.tile_n;
+    const int64_t first = c.plan[g], last = c.plan[g + 1];
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (last > first) {
+      const int64_t base = (int64_t)tile * total, r0 = runs.of(base + first), r1 = runs.of(base + last - 1);
+      if (r0 == r1) continue;      // one sum, which is in its place
+      for (int64_t r = r0; r <= r1; ++r) {
+        const int64_t piece = 2 * r + (runs.begin(r) < base + first);
+        if (weight) {
+          const float4 v = *(const float4*)(c.partial + (piece * kTileM + m % kTileM) * c.tile_n + n % c.tile_n);
+          sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+        } else {
+          sum[0] += c.partial_bias[piece * kTileM + m % kTileM];
+        }
+      }
+    }
+    if (weight) {
+      for (int k = 0; k < 4; ++k)
+        if (n + k < c.num_n) ((T*)c.out)[gm * c.num_n + n + k] = Elem<T>::from_f(sum[k]);
+    } else {
+      ((T*)c.grad_bias)[gm] = Elem<T>::from_f(sum[0]);
+    }
+  }
+}
+
+// db without dw.
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_bias_sums(const T* __restrict__ grad, int64_t rows, int64_t out_dim, const int64_t* __restrict__ offsets, int groups, T* __restrict__ grad_bias,
-            int32_t* status) {
+k_bias_sums(const T* __restrict__ grad, int64_t rows, int64_t out_dim, const int64_t* __restrict__ offsets, T* __restrict__ grad_bias, int32_t* status) {
   wait_for_previous();
   __shared__ float part[8][33];
   const int g = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -121,72 +609,238 @@ k_bias_sums(const T* __restrict__ grad, int64_t rows, int64_t out_dim, const int
   }
 }
 
-template <typename T>
-static int linear_forward(const void* x, int64_t rows, int64_t dim, const void* weight, const void* bias, int64_t out_dim, const int64_t* offsets, int groups,
-                          void* out, int32_t* status, cudaStream_t s) {
-  const dim3 grid((unsigned)(ceil_div(rows, kTile) + groups + 1), (unsigned)ceil_div(out_dim, kTile));
-  APT_FOLLOW((k_rows_product<T>), grid, 256, 0, s, (const T*)x, rows, dim, (const T*)weight, dim, (int64_t)1, out_dim, (const T*)bias, offsets, groups,
-             (T*)out, status);
-  return APT_OK;
+// ---- host side -----------------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) p = nullptr;
+    return (EncodeTiled)p;
+  }();
+  return fn;
 }
-template <typename T>
-static int linear_backward(const void* x, int64_t rows, int64_t dim, const void* weight, int64_t out_dim, const int64_t* offsets, int groups,
-                           const void* grad, void* grad_x, void* grad_weight, void* grad_bias, int32_t* status, cudaStream_t s) {
-  if (grad_x && rows) {
-    const dim3 grid((unsigned)(ceil_div(rows, kTile) + groups + 1), (unsigned)ceil_div(dim, kTile));
-    APT_FOLLOW((k_rows_product<T>), grid, 256, 0, s, (const T*)grad, rows, out_dim, (const T*)weight, (int64_t)1, dim, dim, (const T*)nullptr, offsets, groups,
-               (T*)grad_x, status);
+
+// A matrix of `rows` rows as the copies read it: in whole 16-byte slices, `pitch` elements apart.
+struct Operand {
+  const void* data;
+  int64_t stack, rows, columns, pitch;
+};
+static int make_map(CUtensorMap* map, int dtype, const Operand& o, int box_columns, int box_rows) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) {
+    set_error("grouped_linear: the driver has no cuTensorMapEncodeTiled");
+    return APT_ERR_CUDA;
   }
-  if (grad_weight) {
-    const dim3 grid((unsigned)ceil_div(out_dim, kTile), (unsigned)ceil_div(dim, kTile), (unsigned)groups);
-    APT_FOLLOW((k_weight_product<T>), grid, 256, 0, s, (const T*)x, rows, dim, (const T*)grad, out_dim, offsets, (T*)grad_weight);
-  }
-  if (grad_bias) {
-    const dim3 grid((unsigned)ceil_div(out_dim, 32), (unsigned)groups);
-    APT_FOLLOW((k_bias_sums<T>), grid, 256, 0, s, (const T*)grad, rows, out_dim, offsets, groups, (T*)grad_bias, status);
+  const size_t size = dtype == APT_F32 ? 4 : 2;
+  const cuuint64_t dims[3] = {(cuuint64_t)o.columns, (cuuint64_t)o.rows, (cuuint64_t)o.stack};
+  const cuuint64_t strides[2] = {(cuuint64_t)(o.pitch * size), (cuuint64_t)(o.rows * o.pitch * size)};
+  const cuuint32_t box[3] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
+  const CUresult r = encode(map, dtype == APT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == APT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            o.stack ? 3 : 2, (void*)o.data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("grouped_linear: cuTensorMapEncodeTiled -> %d (%lld x %lld, pitch %lld)", (int)r, (long long)o.rows, (long long)o.columns, (long long)o.pitch);
+    return APT_ERR_CUDA;
   }
   return APT_OK;
 }
 
-static int linear_check(const char* who, int dtype, int64_t rows, int64_t dim, int64_t out_dim, int64_t groups) {
+static int64_t pitch_of(int64_t columns, size_t size) { return widened_dim(columns, size); }
+static size_t room_of(int64_t rows, int64_t columns, size_t size) {
+  const int64_t pitch = pitch_of(columns, size);
+  return pitch == columns ? 0 : align_up((size_t)rows * pitch * size, 256);
+}
+// The matrix, or a copy of it in whole slices in front of *room.
+static int laid_out(const void* data, int64_t stack, int64_t rows, int64_t columns, size_t size, char** room, Operand* o, cudaStream_t s) {
+  *o = {data, stack, rows, columns, pitch_of(columns, size)};
+  if (o->pitch == columns) return APT_OK;
+  const int64_t all = rows * std::max<int64_t>(stack, 1);
+  if (const int e = widen_rows(data, all, columns * size, *room, s)) return e;
+  o->data = *room;
+  *room += room_of(all, columns, size);
+  return APT_OK;
+}
+
+// Columns of a tile: as few tiles as can be, of the same width.
+static int tile_columns(int64_t n, int most) { return (int)(ceil_div(ceil_div(n, ceil_div(n, most)), 16) * 16); }
+
+// Runs of stages that dw is cut into at most, and partial sums that come of it: one for every block, or more where a run would have over
+// 1024 rows of fp32, whose sums the tensor cores cut rather than round.
+struct WeightPlan {
+  int tile_n, tiles_m, tiles_n;
+  int64_t ranges, pieces;
+};
+template <typename T>
+static WeightPlan weight_plan(int64_t rows, int64_t dim, int64_t out_dim, int64_t groups) {
+  using Tr = GroupedTraits<T, kGradW>;
+  WeightPlan p;
+  p.tile_n = tile_columns(dim, Tr::kMostN);
+  p.tiles_m = (int)ceil_div(out_dim, kTileM);
+  p.tiles_n = (int)ceil_div(dim, p.tile_n);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, most = (ceil_div(rows, Tr::kBlock) + groups) * tiles;
+  p.ranges = kNumSMs;
+  if (Tr::kSplit) p.ranges *= std::max<int64_t>(1, ceil_div(rows * tiles, (int64_t)kNumSMs * 1024));
+  p.ranges = grouped_runs(most, p.ranges).runs;
+  p.pieces = 2 * p.ranges;
+  return p;
+}
+
+template <typename T, int MODE>
+static int launch_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap& b, int64_t items, cudaStream_t s) {
+  using Tr = GroupedTraits<T, MODE>;
+  const int fixed = 1024 + 4 * 4096 + (MODE == kGradW ? 2048 : 0) + (int)align_up((size_t)(c.groups + 2) * 4, 16);
+  const int copied = Tr::copied(kTileM, Tr::kMnA) + Tr::copied(c.tile_n, Tr::kMnB);
+  const int pieces = Tr::kSplit ? 3 * (Tr::piece(kTileM, Tr::kMnA) + Tr::piece(c.tile_n, Tr::kMnB)) : 0;
+  const int room = kStageBytes - 1024 - fixed;      // 1 KB: barriers
+  if (Tr::kSplit) {
+    c.piece_stages = 2;
+    c.copied_stages = std::min(kMaxStages, (room - 2 * pieces) / copied);
+  } else {
+    c.piece_stages = 0;
+    c.copied_stages = std::min(kMaxStages, room / copied);
+  }
+  const int bytes = fixed + c.copied_stages * copied + c.piece_stages * pieces;
+  static const cudaError_t allowed = cudaFuncSetAttribute(k_grouped<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStageBytes - 1024);
+  APT_CUDA(allowed);
+  // over half of an SM's shared memory, so that no two blocks share one: each takes all of its tensor memory
+  APT_FOLLOW((k_grouped<T, MODE>), std::min<int64_t>(items, kNumSMs), Tr::kThreads, std::max(bytes, kStageBytes / 2 + 1024), s, a, b, c);
+  return APT_OK;
+}
+
+template <typename T>
+static int code_of() { return sizeof(T) == 4 ? APT_F32 : std::is_same<T, __half>::value ? APT_F16 : APT_BF16; }
+
+// Rows against weights: out (contraction along w's rows) or dx (across them).
+template <typename T, int MODE>
+static int rows_product(const Operand& rows, const Operand& weight, int64_t num_n, const void* bias, const int64_t* offsets, int groups, void* out,
+                        int32_t* status, cudaStream_t s) {
+  using Tr = GroupedTraits<T, MODE>;
+  GroupedCall c = {};
+  c.offsets = offsets, c.rows = rows.rows, c.groups = groups;
+  c.num_n = (int)num_n, c.num_k = (int)rows.columns;
+  c.tile_n = tile_columns(num_n, Tr::kMostN), c.tiles_n = (int)ceil_div(num_n, c.tile_n);
+  c.tile_m = kTileM;
+  c.a = rows.data, c.b = weight.data, c.pitch_a = rows.pitch, c.pitch_b = weight.pitch;
+  c.bias = bias, c.out = out, c.status = status;
+  CUtensorMap a, b;
+  if (const int e = make_map(&a, code_of<T>(), rows, Tr::kBox, c.tile_m)) return e;
+  if (const int e = make_map(&b, code_of<T>(), weight, Tr::kBox, MODE == kOut ? c.tile_n : Tr::kBlock)) return e;
+  return launch_grouped<T, MODE>(c, a, b, (ceil_div(rows.rows, c.tile_m) + groups + 1) * c.tiles_n, s);
+}
+
+template <typename T>
+static int linear_forward(const void* x, int64_t rows, int64_t dim, const void* weight, const void* bias, int64_t out_dim, const int64_t* offsets, int groups,
+                          void* out, char* room, int32_t* status, cudaStream_t s) {
+  Operand a, w;
+  if (const int e = laid_out(x, 0, rows, dim, sizeof(T), &room, &a, s)) return e;
+  if (const int e = laid_out(weight, groups, out_dim, dim, sizeof(T), &room, &w, s)) return e;
+  return rows_product<T, kOut>(a, w, out_dim, bias, offsets, groups, out, status, s);
+}
+
+template <typename T>
+static size_t linear_room(int64_t rows, int64_t dim, int64_t out_dim, int64_t groups, bool backward) {
+  size_t bytes = room_of(rows, dim, sizeof(T)) + room_of(groups * out_dim, dim, sizeof(T));
+  if (backward) {
+    const WeightPlan p = weight_plan<T>(rows, dim, out_dim, groups);
+    bytes += room_of(rows, out_dim, sizeof(T)) + align_up((size_t)(groups + 1) * 8, 256) + (size_t)p.pieces * kTileM * (p.tile_n + 1) * 4;
+  }
+  return bytes;
+}
+
+template <typename T>
+static int linear_backward(const void* x, int64_t rows, int64_t dim, const void* weight, int64_t out_dim, const int64_t* offsets, int groups,
+                           const void* grad, void* grad_x, void* grad_weight, void* grad_bias, char* room, int32_t* status, cudaStream_t s) {
+  if (grad_bias && !grad_weight) {
+    const dim3 grid((unsigned)ceil_div(out_dim, 32), (unsigned)groups);
+    APT_FOLLOW((k_bias_sums<T>), grid, 256, 0, s, (const T*)grad, rows, out_dim, offsets, (T*)grad_bias, status);
+  }
+  if (rows == 0) {
+    if (grad_weight) APT_CUDA(cudaMemsetAsync(grad_weight, 0, (size_t)groups * out_dim * dim * sizeof(T), s));
+    if (grad_weight && grad_bias) APT_CUDA(cudaMemsetAsync(grad_bias, 0, (size_t)groups * out_dim * sizeof(T), s));
+    return APT_OK;
+  }
+  if (!grad_x && !grad_weight) return APT_OK;
+  Operand dy;
+  if (const int e = laid_out(grad, 0, rows, out_dim, sizeof(T), &room, &dy, s)) return e;
+  if (grad_x) {
+    Operand w;
+    if (const int e = laid_out(weight, groups, out_dim, dim, sizeof(T), &room, &w, s)) return e;
+    if (const int e = rows_product<T, kGradX>(dy, w, dim, nullptr, offsets, groups, grad_x, status, s)) return e;
+  }
+  if (grad_weight) {
+    using Tr = GroupedTraits<T, kGradW>;
+    Operand in;
+    if (const int e = laid_out(x, 0, rows, dim, sizeof(T), &room, &in, s)) return e;
+    const WeightPlan p = weight_plan<T>(rows, dim, out_dim, groups);
+    GroupedCall c = {};
+    c.offsets = offsets, c.rows = rows, c.groups = groups;
+    c.num_m = (int)out_dim, c.num_n = (int)dim;
+    c.tile_n = p.tile_n, c.tiles_m = p.tiles_m, c.tiles_n = p.tiles_n, c.ranges = p.ranges;
+    c.a = dy.data, c.b = in.data, c.pitch_a = dy.pitch, c.pitch_b = in.pitch;
+    c.out = grad_weight, c.grad_bias = grad_bias, c.status = status;
+    c.plan = (int64_t*)room;
+    c.partial = (float*)(room + align_up((size_t)(groups + 1) * 8, 256));
+    c.partial_bias = c.partial + (size_t)p.pieces * kTileM * p.tile_n;
+    CUtensorMap a, b;
+    if (const int e = make_map(&a, code_of<T>(), dy, Tr::kBox, Tr::kBlock)) return e;
+    if (const int e = make_map(&b, code_of<T>(), in, Tr::kBox, Tr::kBlock)) return e;
+    if (const int e = launch_grouped<T, kGradW>(c, a, b, p.ranges, s)) return e;
+    const int64_t threads = (int64_t)groups * out_dim * (ceil_div(dim, 4) + (grad_bias ? 1 : 0));
+    APT_FOLLOW((k_join_weights<T, Tr::kBlock>), wave_grid(ceil_div(threads, 256), 8), 256, 0, s, c);
+  }
+  return APT_OK;
+}
+
+static int linear_check(const char* who, int dtype, int64_t rows, int64_t dim, int64_t out_dim, int64_t groups, const void* workspace, size_t workspace_bytes,
+                        int backward) {
   APT_CHECK_ARG(dtype == APT_F32 || dtype == APT_BF16 || dtype == APT_F16, "%s: unsupported dtype %d", who, dtype);
   APT_CHECK_ARG(rows >= 0 && rows < (1ll << 31) - (1 << 20) && dim > 0 && out_dim > 0 && dim <= APT_GROUPED_LINEAR_MAX_DIM && out_dim <= APT_GROUPED_LINEAR_MAX_DIM,
-                "%s: %lld rows of %lld by %lld", who, (long long)rows, (long long)dim, (long long)out_dim);
+                "%s: %lld rows of %lld by %lld (1 to %d are possible)", who, (long long)rows, (long long)dim, (long long)out_dim, APT_GROUPED_LINEAR_MAX_DIM);
   APT_CHECK_ARG(groups > 0 && groups <= APT_GROUPED_LINEAR_MAX_GROUPS, "%s: %lld groups (1 to %d are possible)", who, (long long)groups,
                 APT_GROUPED_LINEAR_MAX_GROUPS);
+  APT_CHECK_ARG(rows == 0 || workspace_bytes >= apt_grouped_linear_workspace_bytes(dtype, rows, dim, out_dim, groups, backward), "%s: workspace too small", who);
+  APT_CHECK_ARG((uintptr_t)workspace % 16 == 0, "%s: workspace not aligned to 16 bytes", who);
   return APT_OK;
 }
 
 }  // namespace apt
 
 extern "C" size_t apt_grouped_linear_workspace_bytes(int dtype, int64_t rows, int64_t dim, int64_t out_dim, int64_t groups, int backward) {
-  return 0;
+  if (rows <= 0 || dim <= 0 || out_dim <= 0 || groups <= 0) return 0;
+  return dtype == APT_F32 ? apt::linear_room<float>(rows, dim, out_dim, groups, backward) : apt::linear_room<__half>(rows, dim, out_dim, groups, backward);
 }
 
 extern "C" int apt_grouped_linear_forward(int dtype, const void* x, int64_t rows, int64_t dim, const void* weight, const void* bias, int64_t out_dim,
                                           const int64_t* offsets, int64_t groups, void* out, void* workspace, size_t workspace_bytes,
                                           int32_t* status_word, void* stream) {
   using namespace apt;
-  if (const int e = linear_check("apt_grouped_linear_forward", dtype, rows, dim, out_dim, groups)) return e;
+  if (const int e = linear_check("apt_grouped_linear_forward", dtype, rows, dim, out_dim, groups, workspace, workspace_bytes, 0)) return e;
   if (rows == 0) return APT_OK;
   APT_CHECK_ARG(x && weight && offsets && out && status_word, "apt_grouped_linear_forward: null buffer");
+  APT_CHECK_ARG(((uintptr_t)x | (uintptr_t)weight | (uintptr_t)out) % 16 == 0, "apt_grouped_linear_forward: buffers not aligned to 16 bytes");
   const cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == APT_F32) return linear_forward<float>(x, rows, dim, weight, bias, out_dim, offsets, (int)groups, out, status_word, s);
-  if (dtype == APT_BF16) return linear_forward<__nv_bfloat16>(x, rows, dim, weight, bias, out_dim, offsets, (int)groups, out, status_word, s);
-  return linear_forward<__half>(x, rows, dim, weight, bias, out_dim, offsets, (int)groups, out, status_word, s);
+  char* const room = (char*)workspace;
+  if (dtype == APT_F32) return linear_forward<float>(x, rows, dim, weight, bias, out_dim, offsets, (int)groups, out, room, status_word, s);
+  if (dtype == APT_BF16) return linear_forward<__nv_bfloat16>(x, rows, dim, weight, bias, out_dim, offsets, (int)groups, out, room, status_word, s);
+  return linear_forward<__half>(x, rows, dim, weight, bias, out_dim, offsets, (int)groups, out, room, status_word, s);
 }
 
 extern "C" int apt_grouped_linear_backward(int dtype, const void* x, int64_t rows, int64_t dim, const void* weight, int64_t out_dim,
                                            const int64_t* offsets, int64_t groups, const void* grad_out, void* grad_x, void* grad_weight,
                                            void* grad_bias, void* workspace, size_t workspace_bytes, int32_t* status_word, void* stream) {
   using namespace apt;
-  if (const int e = linear_check("apt_grouped_linear_backward", dtype, rows, dim, out_dim, groups)) return e;
+  if (const int e = linear_check("apt_grouped_linear_backward", dtype, rows, dim, out_dim, groups, workspace, workspace_bytes, 1)) return e;
   APT_CHECK_ARG(offsets && status_word && (rows == 0 || grad_out) && (!grad_x || rows == 0 || weight) && (!grad_weight || rows == 0 || x),
                 "apt_grouped_linear_backward: null buffer");
+  APT_CHECK_ARG(((uintptr_t)x | (uintptr_t)weight | (uintptr_t)grad_out | (uintptr_t)grad_x | (uintptr_t)grad_weight) % 16 == 0,
+                "apt_grouped_linear_backward: buffers not aligned to 16 bytes");
   const cudaStream_t s = (cudaStream_t)stream;
   const int g = (int)groups;
-  if (dtype == APT_F32) return linear_backward<float>(x, rows, dim, weight, out_dim, offsets, g, grad_out, grad_x, grad_weight, grad_bias, status_word, s);
+  char* const room = (char*)workspace;
+  if (dtype == APT_F32) return linear_backward<float>(x, rows, dim, weight, out_dim, offsets, g, grad_out, grad_x, grad_weight, grad_bias, room, status_word, s);
   if (dtype == APT_BF16)
-    return linear_backward<__nv_bfloat16>(x, rows, dim, weight, out_dim, offsets, g, grad_out, grad_x, grad_weight, grad_bias, status_word, s);
-  return linear_backward<__half>(x, rows, dim, weight, out_dim, offsets, g, grad_out, grad_x, grad_weight, grad_bias, status_word, s);
+    return linear_backward<__nv_bfloat16>(x, rows, dim, weight, out_dim, offsets, g, grad_out, grad_x, grad_weight, grad_bias, room, status_word, s);
+  return linear_backward<__half>(x, rows, dim, weight, out_dim, offsets, g, grad_out, grad_x, grad_weight, grad_bias, room, status_word, s);
 }

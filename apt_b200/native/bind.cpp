@@ -440,6 +440,8 @@ struct NormFunction : public torch::autograd::Function<NormFunction> {
   }
 };
 
+Tensor aligned(const Tensor& t) { return (uintptr_t)data(t) % 16 ? t.clone() : t; }
+
 struct LinearProblem {
   Tensor x, weight, bias, offsets;
   int code;
@@ -464,6 +466,8 @@ LinearProblem linear_problem(const char* who, const Tensor& x, const Tensor& wei
   }
   for (const auto& [t, name] : {std::pair<const Tensor*, const char*>{&q.weight, "weight"}, {&q.offsets, "offsets"}, {&q.bias, "bias"}})
     same_device(who, q.x, *t, name);
+  // a view may begin anywhere
+  for (Tensor* t : {&q.x, &q.weight}) *t = aligned(*t);
   return q;
 }
 
@@ -481,7 +485,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const Tensor& offse
 std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& grad_in, bool want_x,
                                                    bool want_weight, bool want_bias, const Tensor& words) {
   const LinearProblem q = linear_problem("grouped_linear_backward", x, weight, offsets, Tensor());
-  const Tensor grad = cuda(grad_in, "grad_out");
+  const Tensor grad = aligned(cuda(grad_in, "grad_out"));
   if (grad.scalar_type() != q.x.scalar_type() || grad.dim() != 2 || grad.size(0) != q.rows || grad.size(1) != q.out_dim)
     fail("grouped_linear_backward: grad_out must be [rows, out] of x's dtype");
   Tensor grad_x, grad_weight, grad_bias, ws;

@@ -845,7 +845,7 @@ int apt_group_norm_backward(int dtype, int param_dtype, const void* x, const voi
  * Backward: grad_x [rows, dim], grad_weight, grad_bias like their parameters;
  * each unless NULL. */
 #define APT_GROUPED_LINEAR_MAX_GROUPS 4096
-#define APT_GROUPED_LINEAR_MAX_DIM 65536
+#define APT_GROUPED_LINEAR_MAX_DIM 8192
 size_t apt_grouped_linear_workspace_bytes(int dtype, int64_t rows, int64_t dim, int64_t out_dim, int64_t groups, int backward);
 int apt_grouped_linear_forward(int dtype, const void* x, int64_t rows, int64_t dim, const void* weight, const void* bias,
                                int64_t out_dim, const int64_t* offsets, int64_t groups, void* out, void* workspace,

@@ -110,7 +110,7 @@ PROTOTYPES = {
     "apt_rows_gather": (c_int, [P, P, c_int64, c_int64, P, P]),
     "apt_rows_scatter": (c_int, [P, P, c_int64, c_int64, P, P]),
     "apt_dropout": (c_int, [c_int, P, c_int64, c_double, c_uint64, c_uint32, P, P]),
-    "apt_group_norm_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int64, c_int]),
+    "apt_group_norm_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int, P, c_int64, c_int]),
     "apt_group_norm_forward": (c_int, [c_int, c_int, P, c_int64, c_int64, c_int, P, c_int64, c_double, c_int, P, P, c_double, c_uint64, c_uint32,
                                        P, P, P, c_size_t, P, P]),
     "apt_group_norm_backward": (c_int, [c_int, c_int, P, P, c_int64, c_int64, c_int, P, c_int64, c_double, c_int, P, P, c_double, c_uint64,

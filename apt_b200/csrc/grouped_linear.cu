@@ -246,6 +246,8 @@ __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedIt
           float small[32];
           tmem_load_32(acc + ((uint32_t)warp << 21) + Tr::kMostN + at, small);
           tmem_wait_loads();
+          settled(v);
+          settled(small);
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             v[k] += small[k];
@@ -253,6 +255,7 @@ __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedIt
           }
         } else {
           tmem_wait_loads();
+          settled(v);
         }
       }
       if (bias)
@@ -459,7 +462,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               tile_product(small, da + 2 * pa, db, what, true);
             }
             if (sums)
-              for (int p = 0; p < Tr::kPieces; ++p) tile_product(tmem + kAccColumns, da + p * (piece_a >> 4), ones_tile, what_bias, add || p > 0);
+              for (int p = 0; p < Tr::kPieces; ++p)
+                tile_product(tmem + kAccColumns + (p ? 16 : 0), da + p * (piece_a >> 4), ones_tile, what_bias, add || p > 1);
           }
           products_done(shared_addr((Tr::kSplit ? used : free_) + stage));
           if (k == item.stages - 1) products_done(shared_addr(acc_full + buffer));
@@ -498,8 +502,12 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           else
             store_tile<T, float, MODE>(c, item, acc, empty, mine, lane, w, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows, columns, (const T*)nullptr);
           if (c.grad_bias && item.n0 == 0) {
-            float v = tmem_load_1(tmem + kAccColumns + ((uint32_t)w << 21));
+            const uint32_t at = tmem + kAccColumns + ((uint32_t)w << 21);
+            float v = tmem_load_1(at), small = Tr::kSplit ? tmem_load_1(at + 16) : 0.0f;
             tmem_wait_loads();
+            settled(v);
+            settled(small);
+            v += small;
             if (m < rows) {
               if constexpr (Tr::kSplit)
                 if (!isfinite(v)) v = column_again(c, item, m);

@@ -78,7 +78,15 @@ __device__ __forceinline__ float tmem_load_1(uint32_t at) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(at));
   return __uint_as_float(r);
 }
+// Until the loads so far are done; what was loaded is used behind settled() of it only (the registers are written when the load is done, which the
+// compiler does not know).
 __device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void settled(float& v) { asm volatile("" : "+f"(v)); }
+template <int N>
+__device__ __forceinline__ void settled(float (&v)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) settled(v[k]);
+}
 
 // ---- products ----------------------------------------------------------------------
 // A tile in shared memory, its 16-byte slices swizzled within rows of 128 or 64 bytes as the copies leave them. Along the

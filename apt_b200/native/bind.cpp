@@ -383,16 +383,22 @@ NormProblem norm_problem(const Tensor& x_in, const Tensor& weight, const Tensor&
   return q;
 }
 
-// (out, stats)
+// Rows by themselves have their statistics made again in the backward.
+bool norm_keeps_stats(const NormProblem& q, const NormSettings& s) {
+  return q.offsets.defined() || q.segments != q.rows || q.dim / s.groups > APT_GROUP_NORM_ROW_CHANNELS;
+}
+
+// (out, stats); without `want_stats` only those that the backward needs.
 std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& offsets, const NormSettings& s,
-                                        const Tensor& words) {
+                                        bool want_stats, const Tensor& words) {
   const NormProblem q = norm_problem(x, weight, bias, offsets, s);
-  Tensor out = at::empty(q.x.sizes(), q.x.options()), stats = at::empty({q.segments, s.groups, 2}, q.x.options().dtype(at::kFloat));
-  const size_t bytes = apt_group_norm_workspace_bytes(q.rows, q.dim, (int)s.groups, q.segments, 0);
-  const Tensor ws = scratch(q.x, std::max<size_t>(bytes, 16));
+  Tensor out = at::empty(q.x.sizes(), q.x.options()), stats;
+  if (want_stats || norm_keeps_stats(q, s)) stats = at::empty({q.segments, s.groups, 2}, q.x.options().dtype(at::kFloat));
+  const size_t bytes = apt_group_norm_workspace_bytes(q.code, q.rows, q.dim, (int)s.groups, q.offsets.defined() ? ptr(q.offsets) : nullptr, q.segments, 0);
+  const Tensor ws = bytes ? scratch(q.x, bytes) : Tensor();
   check(apt_group_norm_forward(q.code, q.param_code, data(q.x), q.rows, q.dim, (int)s.groups, q.offsets.defined() ? ptr(q.offsets) : nullptr, q.segments,
                                s.eps, (int)s.act, data_or_null(q.weight), data_or_null(q.bias), s.p, (uint64_t)s.key, (uint32_t)s.call, mut(out),
-                               (float*)mut(stats), ws.mutable_data_ptr(), ws.numel(), status_word(words), stream()));
+                               (float*)mut_or_null(stats), mut_or_null(ws), bytes, status_word(words), stream()));
   return {out, stats};
 }
 
@@ -400,19 +406,19 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& weight, c
 std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& offsets, const Tensor& stats_in,
                                                  const Tensor& grad_in, const NormSettings& s, bool want_weight, bool want_bias, const Tensor& words) {
   const NormProblem q = norm_problem(x, weight, bias, offsets, s);
-  const Tensor grad = cuda(grad_in, "grad_out"), stats = cuda(stats_in, "stats", at::kFloat, "torch.float32");
+  const Tensor grad = cuda(grad_in, "grad_out"), stats = stats_in.defined() ? cuda(stats_in, "stats", at::kFloat, "torch.float32") : stats_in;
   if (grad.scalar_type() != q.x.scalar_type() || grad.sizes() != q.x.sizes())
     fail("group_norm_act_backward: grad_out must be like x");
-  if (stats.numel() != q.segments * s.groups * 2) fail("group_norm_act_backward: stats are not those of this call");
+  if (stats.defined() ? stats.numel() != q.segments * s.groups * 2 : norm_keeps_stats(q, s)) fail("group_norm_act_backward: stats are not those of this call");
   Tensor grad_x = at::empty(q.x.sizes(), q.x.options()), grad_weight, grad_bias;
   if (q.weight.defined() && want_weight) grad_weight = at::empty({q.dim}, q.weight.options());
   if (q.bias.defined() && want_bias) grad_bias = at::empty({q.dim}, q.bias.options());
-  const size_t bytes = apt_group_norm_workspace_bytes(q.rows, q.dim, (int)s.groups, q.segments, 1);
-  const Tensor ws = scratch(q.x, std::max<size_t>(bytes, 16));
+  const size_t bytes = apt_group_norm_workspace_bytes(q.code, q.rows, q.dim, (int)s.groups, q.offsets.defined() ? ptr(q.offsets) : nullptr, q.segments, 1);
+  const Tensor ws = bytes ? scratch(q.x, bytes) : Tensor();
   check(apt_group_norm_backward(q.code, q.param_code, data(q.x), data(grad), q.rows, q.dim, (int)s.groups, q.offsets.defined() ? ptr(q.offsets) : nullptr,
                                 q.segments, s.eps, (int)s.act, data_or_null(q.weight), data_or_null(q.bias), s.p, (uint64_t)s.key, (uint32_t)s.call,
-                                (const float*)data(stats), mut(grad_x), mut_or_null(grad_weight), mut_or_null(grad_bias), ws.mutable_data_ptr(),
-                                ws.numel(), status_word(words), stream()));
+                                (const float*)data_or_null(stats), mut(grad_x), mut_or_null(grad_weight), mut_or_null(grad_bias), mut_or_null(ws), bytes,
+                                status_word(words), stream()));
   return {grad_x, grad_weight, grad_bias};
 }
 
@@ -420,7 +426,7 @@ struct NormFunction : public torch::autograd::Function<NormFunction> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& weight_in, const OptTensor& bias_in,
                         const OptTensor& offsets_in, int64_t groups, int64_t act, double eps, double p, int64_t key, int64_t call, const Tensor& words) {
     const Tensor weight = given(weight_in), bias = given(bias_in), offsets = given(offsets_in);
-    auto [out, stats] = norm_forward(x, weight, bias, offsets, {groups, act, eps, p, key, call}, words);
+    auto [out, stats] = norm_forward(x, weight, bias, offsets, {groups, act, eps, p, key, call}, false, words);
     ctx->save_for_backward({x, weight, bias, offsets, stats});
     ctx->saved_data["settings"] = std::vector<int64_t>{groups, act, key, call};
     ctx->saved_data["eps"] = eps;
@@ -922,12 +928,12 @@ PYBIND11_MODULE(_native, m) {
   m.def("dropout", &dropout);
   m.def("dropout_apply", [](const Tensor& x, double p, int64_t key, int64_t call) { return DropoutFunction::apply(x, p, key, call); });
   m.def("norm_forward", [](const Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& offsets, int64_t groups, int64_t act,
-                           double eps, double p, int64_t key, int64_t call, const Tensor& words) {
-    return norm_forward(x, given(weight), given(bias), given(offsets), {groups, act, eps, p, key, call}, words);
+                           double eps, double p, int64_t key, int64_t call, bool want_stats, const Tensor& words) {
+    return norm_forward(x, given(weight), given(bias), given(offsets), {groups, act, eps, p, key, call}, want_stats, words);
   });
-  m.def("norm_backward", [](const Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& offsets, const Tensor& stats,
+  m.def("norm_backward", [](const Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& offsets, const OptTensor& stats,
                             const Tensor& grad, int64_t groups, int64_t act, double eps, double p, int64_t key, int64_t call, const Tensor& words) {
-    return norm_backward(x, given(weight), given(bias), given(offsets), stats, grad, {groups, act, eps, p, key, call}, true, true, words);
+    return norm_backward(x, given(weight), given(bias), given(offsets), given(stats), grad, {groups, act, eps, p, key, call}, true, true, words);
   });
   m.def("norm_apply", [](const Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& offsets, int64_t groups, int64_t act,
                          double eps, double p, int64_t key, int64_t call, const Tensor& words) {

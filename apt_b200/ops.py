@@ -1092,14 +1092,14 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     and bias [C] of x's dtype or float32. p > 0 drops elements of the result as dropout(..., p, key, call_id) does.
     return_stats: also mean and 1 / sqrt(variance + eps), float32 [segments, num_groups, 2], which the backward takes."""
     out, stats = _native.norm_forward(x, weight, bias, offsets, int(num_groups), _activation(act), float(eps), float(p),
-                                      *_stream_key(key, call_id), STATE.words())
+                                      *_stream_key(key, call_id), bool(return_stats), STATE.words())
     return (out, stats) if return_stats else out
 
 
 def group_norm_act_backward(x, grad_out, stats, num_groups: int, weight=None, bias=None, offsets=None, eps: float = 1e-5, act: str = "none",
                             p: float = 0.0, key: int = 0, call_id: int = 0):
-    """Gradients of group_norm_act for grad_out like x and the forward's stats: (grad_x, grad_weight, grad_bias), the latter two
-    None without their parameter."""
+    """Gradients of group_norm_act for grad_out like x and the forward's stats (None will do where every row is normalised by itself
+    in groups of at most 1024 channels): (grad_x, grad_weight, grad_bias), the latter two None without their parameter."""
     return _native.norm_backward(x, weight, bias, offsets, stats, grad_out, int(num_groups), _activation(act), float(eps), float(p),
                                  *_stream_key(key, call_id), STATE.words())
 

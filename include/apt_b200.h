@@ -827,9 +827,13 @@ typedef enum apt_activation { APT_ACT_NONE = 0, APT_ACT_RELU = 1, APT_ACT_SILU =
  * blocks of rows (as many as rows: every row by itself). weight and bias [dim]
  * of param_dtype (dtype or APT_F32), or NULL. p == 0: no dropout; else as
  * apt_dropout over the elements of out. stats [segments, groups, 2] receives mean
- * and 1 / sqrt(variance + eps), which the backward starts from. It gives grad_x,
- * and grad_weight and grad_bias [dim] of param_dtype unless NULL. */
-size_t apt_group_norm_workspace_bytes(int64_t rows, int64_t dim, int groups, int64_t segments, int backward);
+ * and 1 / sqrt(variance + eps), which the backward starts from (zeros for a
+ * segment without rows); where every row is a segment and a group has at most
+ * APT_GROUP_NORM_ROW_CHANNELS channels it may be NULL in both. The backward gives
+ * grad_x, and grad_weight and grad_bias [dim] of param_dtype unless NULL. */
+#define APT_GROUP_NORM_ROW_CHANNELS 1024
+size_t apt_group_norm_workspace_bytes(int dtype, int64_t rows, int64_t dim, int groups, const int64_t* offsets,
+                                      int64_t segments, int backward);
 int apt_group_norm_forward(int dtype, int param_dtype, const void* x, int64_t rows, int64_t dim, int groups, const int64_t* offsets,
                            int64_t segments, double eps, int act, const void* weight, const void* bias, double p,
                            uint64_t key, uint32_t call_id, void* out, float* stats, void* workspace,

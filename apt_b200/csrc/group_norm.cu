@@ -53,28 +53,37 @@ static NormPlan norm_plan(const NormShape& s, size_t size, uintptr_t addresses, 
   NormTiles& t = p.tiles;
   t.chunk = chunk;
   p.chunks = ceil_div(s.groups, chunk);
-  // Short segments by warps where there are enough to fill the chip and a warp holds a row; by blocks where there are fewer. Where the mean
-  // is well above what those do whole, nothing is looked for and all segments are long.
-  p.held = slices <= 256 ? 1 : 8 / p.slice;
-  p.warps = p.chunks == 1 && slices <= 32 * (8 / p.slice) && s.segments >= kNumSMs * 8;
-  if (p.warps) p.held = slices <= 32 ? 1 : 8 / p.slice;
+  p.warps = p.chunks == 1 && slices <= 32 * (8 / p.slice);
+  const int team = p.warps ? 32 : 256;
+  p.held = slices <= team ? 1 : 8 / p.slice;
   t.slots = (int)ceil_div(slices, p.held);
-  t.lines = t.slots <= 32 ? 8 * (32 / t.slots) : 256 / t.slots;
-  const int rows = held_rows(back, p.held);
-  t.cap = p.warps ? rows * (t.lines / 8) * kWarpChunks : rows * t.lines;
-  if (s.rows / s.segments > 4 * (int64_t)t.cap) t.cap = 0;
-  t.short_blocks = t.cap ? (int)std::min<int64_t>(p.warps ? ceil_div(s.segments, 8) : s.segments, kNumSMs * 4) : 0;
-  // one round of blocks, of eight rounds of rows at least
-  const int64_t blocks = ceil_div(kNumSMs * (t.cap || back ? 2 : 4), p.chunks);
-  t.tile = std::max<int64_t>(8 * t.lines, ceil_div(ceil_div(s.rows, blocks), t.lines) * t.lines);
-  t.tiles = ceil_div(s.rows, t.tile);
-  p.blocks = t.tiles + t.short_blocks;
+  t.lines = team / t.slots;
+  // a round of blocks each, two or three an SM (registers), of four rounds of rows at least
+  const auto tiles_of = [&](int per_sm, int64_t* rows, int64_t* tiles) {
+    const int64_t teams = ceil_div(kNumSMs * per_sm, p.chunks) * (256 / team);
+    *rows = std::max<int64_t>(4 * t.lines, ceil_div(ceil_div(s.rows, teams), t.lines) * t.lines);
+    *tiles = ceil_div(s.rows, *rows);
+  };
+  tiles_of(back ? 2 : 3, &t.sum_rows, &t.sum_tiles);
+  tiles_of(p.held > 1 || s.per % p.slice ? 2 : 3, &t.apply_rows, &t.apply_tiles);
+  // threads for all pieces of a mean segment, or a number of them
+  t.join_groups = 1;
+  while (t.join_groups < 64 && t.join_groups < s.groups && 256 / (2 * t.join_groups) >= t.sum_tiles / s.segments + 1) t.join_groups *= 2;
+  t.join_groups = std::max(t.join_groups, std::min(4, s.groups));
+  p.blocks = ceil_div(t.sum_tiles, 256 / team);
   return p;
 }
 
-static size_t norm_room(const NormShape& s, const NormPlan& p, bool back) {
-  const size_t columns = back && p.kind != kNormWide ? align_up((size_t)p.blocks * 2 * s.dim * 4, 256) : 0;
-  return columns + (p.kind == kNormTiles ? (size_t)(p.tiles.tiles + s.segments) * s.groups * 8 : 0);
+// Sums for dgamma and dbeta, sums of pieces, means of segments, what stays.
+struct NormRoom {
+  size_t columns, parts, means, mask;
+  size_t all() const { return columns + parts + means + mask; }
+};
+static NormRoom norm_room(const NormShape& s, const NormPlan& p, bool back) {
+  const bool tiles = p.kind == kNormTiles;
+  return {back && p.kind != kNormWide ? align_up((size_t)p.blocks * 2 * s.dim * 4, 256) : 0,
+          tiles ? align_up((size_t)(p.tiles.sum_tiles + s.segments) * s.groups * 8, 256) : 0,
+          back && tiles ? align_up((size_t)s.segments * s.groups * 8, 256) : 0, back && tiles && p.slice % 4 == 0 ? (size_t)(s.rows * s.dim) / p.slice : 0};
 }
 
 template <bool BACK>
@@ -108,7 +117,7 @@ extern "C" size_t apt_group_norm_workspace_bytes(int dtype, int64_t rows, int64_
   // buffers that begin anywhere may take narrower accesses
   const NormShape s = norm_shape(rows, dim, groups, offsets, segments);
   size_t most = 0;
-  for (const uintptr_t addresses : {0, 4, 2}) most = std::max(most, norm_room(s, norm_plan(s, dtype == APT_F32 ? 4 : 2, addresses, backward), backward));
+  for (const uintptr_t addresses : {0, 4, 2}) most = std::max(most, norm_room(s, norm_plan(s, dtype == APT_F32 ? 4 : 2, addresses, backward), backward).all());
   return most;
 }
 
@@ -124,7 +133,7 @@ extern "C" int apt_group_norm_forward(int dtype, int param_dtype, const void* x,
   APT_CHECK_ARG(workspace_bytes >= apt_group_norm_workspace_bytes(dtype, rows, dim, groups, offsets, segments, 0), "apt_group_norm_forward: workspace too small");
   const NormPlan plan = norm_plan(s, dtype == APT_F32 ? 4 : 2, (uintptr_t)x | (uintptr_t)out, false);
   const NormCall c{x, nullptr, weight, bias, out, nullptr, nullptr, (float2*)stats, (float)eps, act, param_dtype == APT_F32, p > 0.0,
-                   make_drop(p, key, call_id), status_word, nullptr, (float2*)workspace};
+                   make_drop(p, key, call_id), status_word, nullptr, (float2*)workspace, nullptr, nullptr};
   return norm_typed<false>(dtype, s, c, plan, (cudaStream_t)stream);
 }
 
@@ -146,8 +155,10 @@ extern "C" int apt_group_norm_backward(int dtype, int param_dtype, const void* x
   const NormShape s = norm_shape(rows, dim, groups, offsets, segments);
   const NormPlan plan = norm_plan(s, dtype == APT_F32 ? 4 : 2, (uintptr_t)x | (uintptr_t)grad_out | (uintptr_t)grad_x, true);
   const bool params = grad_weight || grad_bias;
-  const size_t columns = plan.kind != kNormWide ? align_up((size_t)plan.blocks * 2 * dim * 4, 256) : 0;
+  const NormRoom room = norm_room(s, plan, true);
+  char* const ws = (char*)workspace;
   const NormCall c{x, grad_out, weight, bias, grad_x, grad_weight, grad_bias, (float2*)stats, (float)eps, act, param_dtype == APT_F32, p > 0.0,
-                   make_drop(p, key, call_id), status_word, params ? (float*)workspace : nullptr, (float2*)((char*)workspace + columns)};
+                   make_drop(p, key, call_id), status_word, params ? (float*)ws : nullptr, (float2*)(ws + room.columns),
+                   (float2*)(ws + room.columns + room.parts), (uint8_t*)(ws + room.columns + room.parts + room.means)};
   return norm_typed<true>(dtype, s, c, plan, st);
 }

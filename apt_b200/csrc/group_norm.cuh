@@ -8,9 +8,9 @@
 //
 // Rows by themselves (k_norm_rows): a group of a row is a run of numbers that a few lanes hold; read once, written once, forwards and
 // backwards (statistics are made again rather than kept).
-// Segments: one whose rows a block's registers can hold is done by one block in one go (k_norm_first); of longer ones that kernel
-// makes the sums of tiles of rows, and k_norm_second joins them and does the rest. Which segments are which only the device knows, so
-// both kernels run always and look.
+// Segments: tiles of rows are summed up, piece by piece of the segments they have rows of (k_norm_sums), the pieces are joined
+// (k_norm_join) and the rows walked again (k_norm_apply), so that a segment's length matters to nobody: a batch of small graphs and a few
+// long node types are the same work. The second walk finds in L2 what fits there.
 // Groups too wide for either: k_norm_wide_*, a block a segment and group, by walks over memory.
 #pragma once
 
@@ -35,7 +35,8 @@ struct NormCall {
   Drop d;
   int32_t* status;
   float* columns;                                // [blocks][2][dim] sums for dgamma and dbeta
-  float2* parts;                                 // of the pieces of segments
+  float2 *parts, *means;                         // sums of the pieces of segments, the backward's two means of each
+  uint8_t* mask;                                 // backward of long segments, slices of whole quads: what stays
 };
 
 __device__ __forceinline__ RowRange segment_rows(const NormShape& s, int64_t k) {
@@ -126,6 +127,25 @@ __device__ __forceinline__ void store_all(T* p, const float (&v)[N]) {
   store_pack<T, N>(p, r);
 }
 
+// Which of the elements from e on stay, a bit each.
+template <int N>
+__device__ __forceinline__ uint32_t kept(const Drop& d, int64_t e) {
+  static_assert(N % 4 == 0, "whole quads");
+  uint32_t bits = 0;
+#pragma unroll
+  for (int q = 0; q < N / 4; ++q) {
+    const Philox4 w = drop_words(d, (e >> 2) + q);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) bits |= w.w[k] >= d.threshold && d.scale != 0.0f ? 1u << (4 * q + k) : 0u;
+  }
+  return bits;
+}
+template <int N>
+__device__ __forceinline__ void drop_by(const Drop& d, uint32_t bits, float (&v)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = bits >> k & 1 ? v[k] * d.scale : 0.0f;
+}
+
 // y of normalised elements, in place.
 template <int N>
 __device__ __forceinline__ void finish_forward(const NormCall& c, int64_t e, float (&v)[N], const float (&gamma)[N], const float (&beta)[N]) {
@@ -134,14 +154,25 @@ __device__ __forceinline__ void finish_forward(const NormCall& c, int64_t e, flo
   act_all(c.act, v);
   if (c.drop) drop_all(c.d, e, v);
 }
-// dz of normalised elements and gradients, into the gradients.
-template <int N>
+// dz of normalised elements and gradients, into the gradients. Where a call meets its elements twice, the first time leaves what stays in
+// c.mask, a byte a slice of whole quads, and the second takes it from there: making it anew is half of such a pass.
+enum MaskUse { kMaskMade, kMaskLeft, kMaskTaken };
+template <int USE, int N>
 __device__ __forceinline__ void begin_backward(const NormCall& c, int64_t e, const float (&xh)[N], float (&grad)[N], const float (&gamma)[N], const float (&beta)[N]) {
   float z[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) z[k] = fmaf(xh[k], gamma[k], beta[k]);
   slope_all(c.act, z);
-  if (c.drop) drop_all(c.d, e, grad);
+  if (c.drop) {
+    if constexpr (USE == kMaskMade || N % 4) {
+      drop_all(c.d, e, grad);
+    } else {
+      uint8_t* const at = c.mask + e / N;
+      const uint32_t bits = USE == kMaskTaken ? *at : kept<N>(c.d, e);
+      if (USE == kMaskLeft) *at = (uint8_t)bits;
+      drop_by(c.d, bits, grad);
+    }
+  }
 #pragma unroll
   for (int k = 0; k < N; ++k) grad[k] *= z[k];
 }
@@ -271,7 +302,7 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
           float xh[VE];
 #pragma unroll
           for (int k = 0; k < VE; ++k) xh[k] = (rx[u][j].get(k) - mean[u]) * rstd[u], dz[u][j][k] = rg[u][j].get(k);
-          begin_backward(c, row[u] * s.dim + at[j], xh, dz[u][j], gamma[j], beta[j]);
+          begin_backward<kMaskMade>(c, row[u] * s.dim + at[j], xh, dz[u][j], gamma[j], beta[j]);
           if (!in[j] || row[u] >= s.rows) continue;
 #pragma unroll
           for (int k = 0; k < VE; ++k) {
@@ -360,13 +391,14 @@ __global__ void __launch_bounds__(256) k_norm_columns(const __grid_constant__ No
 constexpr int kMostColumns = 2048;      // of a block: 8 a thread
 constexpr int kMostGroups = 512;        // of a block
 
-// A thread has NC slices of VE neighbouring channels of every `lines`-th row. Up to 32 threads side by side are lanes of one warp.
+// The rows are cut into tiles for teams of threads, a warp each where its lanes hold a row, else a block. A thread has NC slices of VE
+// neighbouring channels of every `lines`-th row of its tile.
 struct NormTiles {
-  int64_t tile, tiles;      // rows of a tile, how many
-  int short_blocks;         // behind the tiles' blocks: whole segments
-  int chunk;                // groups of a block
-  int slots, lines;         // threads side by side in a row, rows side by side
-  int cap;                  // rows of the segments that are done whole
+  int64_t sum_rows, sum_tiles;        // of k_norm_sums, whose tiles the pieces are of
+  int64_t apply_rows, apply_tiles;    // of k_norm_apply
+  int chunk;                          // groups of a team
+  int slots, lines;                   // threads side by side in a row, rows side by side
+  int join_groups;                    // groups of a block of k_norm_join
 };
 
 // GN: groups that a slice may have channels of (1 where a group is whole slices).
@@ -376,16 +408,10 @@ struct NormThread {
   bool mine;
   bool in[NC];
   int col[NC];
-  uint16_t group[NC][GN];        // within the block's
-  __device__ __forceinline__ NormThread(const NormShape& s, const NormTiles& t) {
-    if (t.slots <= 32) {
-      const int lane = threadIdx.x % 32, per_warp = 32 / t.slots;
-      slot = lane % t.slots, line = threadIdx.x / 32 * per_warp + lane / t.slots;
-      mine = lane < per_warp * t.slots;
-    } else {
-      slot = threadIdx.x % t.slots, line = threadIdx.x / t.slots;
-      mine = line < t.lines;
-    }
+  uint16_t group[NC][GN];        // within the team's
+  __device__ __forceinline__ NormThread(const NormShape& s, const NormTiles& t, int thread) {
+    slot = thread % t.slots, line = thread / t.slots;
+    mine = line < t.lines;
     group0 = blockIdx.y * t.chunk, groups = min(t.chunk, s.groups - group0), per = s.per, col0 = group0 * s.per;
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
@@ -401,7 +427,7 @@ struct NormThread {
 // Sums of K numbers over the rows and each group from per-thread sums a channel, into result[group][k]; by all threads of a block, or of
 // a warp with shared memory of its own.
 template <int VE, int NC, int GN, int K, bool WARP>
-__device__ __forceinline__ void sum_groups(const float (&v)[K][NC][VE], float* room, float* result, const NormThread<VE, NC, GN>& me, int slots, int lines, int line) {
+__device__ __forceinline__ void sum_groups(const float (&v)[K][NC][VE], float* room, float* result, const NormThread<VE, NC, GN>& me, int slots, int lines) {
   // a slice of one group is one number
   constexpr int kOwn = GN == 1 ? 1 : VE;
   const int columns = slots * NC * kOwn, pitch = columns + 1, per = GN == 1 ? me.per / VE : me.per, lane = threadIdx.x % 32;
@@ -418,10 +444,10 @@ __device__ __forceinline__ void sum_groups(const float (&v)[K][NC][VE], float* r
           float sum = 0.0f;
 #pragma unroll
           for (int i = 0; i < VE; ++i) sum += v[k][j][i];
-          room[line * pitch + me.slot + j * slots] = sum;
+          room[me.line * pitch + me.slot + j * slots] = sum;
         } else {
 #pragma unroll
-          for (int i = 0; i < VE; ++i) room[line * pitch + (me.slot + j * slots) * VE + i] = v[k][j][i];
+          for (int i = 0; i < VE; ++i) room[me.line * pitch + (me.slot + j * slots) * VE + i] = v[k][j][i];
         }
       }
     sync();
@@ -476,15 +502,15 @@ __device__ __forceinline__ void load_params(const NormCall& c, const NormThread<
     }
 }
 template <int VE, int NC, int GN>
-__device__ __forceinline__ void load_stats(const NormShape& s, const NormCall& c, const NormThread<VE, NC, GN>& me, int64_t seg, float2 (&st)[NC][GN]) {
+__device__ __forceinline__ void load_stats(const NormShape& s, const float2* stats, const NormThread<VE, NC, GN>& me, int64_t seg, float2 (&st)[NC][GN]) {
 #pragma unroll
   for (int j = 0; j < NC; ++j)
 #pragma unroll
-    for (int i = 0; i < GN; ++i) st[j][i] = c.stats[seg * s.groups + me.group0 + me.group[j][i]];
+    for (int i = 0; i < GN; ++i) st[j][i] = stats[seg * s.groups + me.group0 + me.group[j][i]];
 }
 
 // A block's sums of dgamma and dbeta to its line of c.columns.
-template <int VE, int NC, int GN>
+template <bool WARP, int VE, int NC, int GN>
 __device__ __forceinline__ void put_columns(const NormShape& s, const NormCall& c, const NormTiles& t, const NormThread<VE, NC, GN>& me, float* room,
                                             const float (&dgamma)[NC][VE], const float (&dbeta)[NC][VE]) {
   const int pitch = t.slots * NC * VE;
@@ -495,21 +521,28 @@ __device__ __forceinline__ void put_columns(const NormShape& s, const NormCall& 
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) room[me.line * pitch + (me.slot + j * t.slots) * VE + i] = which ? dbeta[j][i] : dgamma[j][i];
+        for (int i = 0; i < VE; ++i) room[(WARP ? threadIdx.x / 32 * t.lines + me.line : me.line) * pitch + (me.slot + j * t.slots) * VE + i] = which ? dbeta[j][i] : dgamma[j][i];
     __syncthreads();
     for (int k = threadIdx.x; k < me.groups * me.per; k += 256) {
       float v = 0.0f;
-      for (int l = 0; l < t.lines; ++l) v += room[l * pitch + k];
+      for (int l = 0; l < (WARP ? 8 : 1) * t.lines; ++l) v += room[l * pitch + k];
       c.columns[((int64_t)blockIdx.x * 2 + which) * s.dim + me.col0 + k] = v;
     }
   }
 }
 
-// Sums of a tile's rows of long segments, piece by piece: piece number tile + segment, which no other has. Forwards mean and squares around
-// it, backwards the sums of dxh and dxh xh. Bound by HBM: 151552 x 256 bf16 in 8 segments, 8 groups of channels a slice.
-template <typename T, int VE, int NC, int GN, bool BACK>
-__device__ __forceinline__ void tile_sums(const NormShape& s, const NormCall& c, const NormTiles& t, float* room, float* result) {
-  const NormThread<VE, NC, GN> me(s, t);
+// Sums of each tile's rows, piece by piece (the rows a tile has of a segment): piece number tile + segment, which no other has. Forwards the mean
+// and the squares around it, backwards the sums of dxh and dxh xh.
+// 151552 x 256 bf16 in 8 segments, us: forwards FWD_SUMS (HBM: 12), backwards BWD_SUMS (24), where the dropout's generator binds.
+template <typename T, int VE, int NC, int GN, bool BACK, bool WARP>
+__global__ void __launch_bounds__(256, BACK ? 2 : 3)
+k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t) {
+  wait_for_previous();
+  constexpr int kRoom = (WARP ? 32 : 256) * (NC * VE + 1), kGroups = WARP ? 256 : kMostGroups;
+  __shared__ float rooms[(WARP ? 8 : 1) * kRoom], results[(WARP ? 8 : 1) * kGroups * 2];
+  const int team = WARP ? threadIdx.x / 32 : 0, thread = WARP ? threadIdx.x % 32 : threadIdx.x, size = WARP ? 32 : 256;
+  float *const room = rooms + team * kRoom, *const result = results + team * kGroups * 2;
+  const NormThread<VE, NC, GN> me(s, t, thread);
   const T* const x = (const T*)c.x;
   const T* const grad = (const T*)c.grad;
   float gamma[BACK ? NC : 1][VE], beta[BACK ? NC : 1][VE], dgamma[BACK ? NC : 1][VE], dbeta[BACK ? NC : 1][VE];
@@ -520,13 +553,15 @@ __device__ __forceinline__ void tile_sums(const NormShape& s, const NormCall& c,
 #pragma unroll
       for (int i = 0; i < VE; ++i) dgamma[j][i] = dbeta[j][i] = 0.0f;
   }
-  const int64_t row0 = blockIdx.x * t.tile, row1 = min(row0 + t.tile, s.rows);
-  for (int64_t seg = segment_at(s, row0); seg < s.segments; ++seg) {
+  const int64_t tile = (int64_t)blockIdx.x * (WARP ? 8 : 1) + team, row0 = tile * t.sum_rows, row1 = min(row0 + t.sum_rows, s.rows), step = t.lines * s.dim;
+  for (int64_t seg = row0 < row1 ? segment_at(s, row0) : s.segments; seg < s.segments; ++seg) {
     const RowRange whole = segment_rows(s, seg);
     if (whole.begin >= row1) break;
     const int64_t b = max(whole.begin, row0), e = min(whole.end, row1);
-    if (whole.end - whole.begin <= t.cap || e <= b) continue;
-    float2* const parts = c.parts + (blockIdx.x + seg) * s.groups + me.group0;
+    if (e <= b) continue;
+    float2* const parts = c.parts + (tile + seg) * s.groups + me.group0;
+    int left = (int)(e - b) - me.line;      // rows from the thread's next one on
+    int64_t at = (b + me.line) * s.dim;
     if constexpr (!BACK) {
       float v[1][NC][VE], q[NC][VE];
 #pragma unroll
@@ -534,16 +569,16 @@ __device__ __forceinline__ void tile_sums(const NormShape& s, const NormCall& c,
 #pragma unroll
         for (int i = 0; i < VE; ++i) v[0][j][i] = q[j][i] = 0.0f;
       float n = 0.0f;
-      for (int64_t r0 = b + me.line; r0 < e; r0 += 4 * t.lines) {
+      for (; left > 0; left -= 4 * t.lines, at += 4 * step) {
         Raw<T, VE> raw[4][NC];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
           for (int j = 0; j < NC; ++j)
-            if (me.in[j] && r0 + u * t.lines < e) raw[u][j] = load_raw<T, VE>(x + (r0 + u * t.lines) * s.dim + me.col[j]);
+            if (me.in[j] && left > u * t.lines) raw[u][j] = load_raw<T, VE>(x + at + u * step + me.col[j]);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          if (!me.mine || r0 + u * t.lines >= e) break;
+          if (!me.mine || left <= u * t.lines) break;
           n += 1.0f;
           const float share = __fdividef(1.0f, n);
 #pragma unroll
@@ -563,38 +598,38 @@ __device__ __forceinline__ void tile_sums(const NormShape& s, const NormCall& c,
       for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int i = 0; i < VE; ++i) own[0][j][i] = me.in[j] ? v[0][j][i] * n : 0.0f;
-      sum_groups<VE, NC, GN, 1, false>(own, room, result, me, t.slots, t.lines, me.line);
-      const float count = (float)(e - b) * (float)me.per;
+      sum_groups<VE, NC, GN, 1, WARP>(own, room, result, me, t.slots, t.lines);
+      const float share = 1.0f / ((float)(e - b) * (float)me.per);
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-          const float d = v[0][j][i] - result[me.group[j][i % GN]] / count;
+          const float d = v[0][j][i] - result[me.group[j][i % GN]] * share;
           own[0][j][i] = me.in[j] ? fmaf(n * d, d, q[j][i]) : 0.0f;
         }
-      sum_groups<VE, NC, GN, 1, false>(own, room, result + kMostGroups, me, t.slots, t.lines, me.line);
-      for (int g = threadIdx.x; g < me.groups; g += 256) parts[g] = make_float2(result[g] / count, result[kMostGroups + g]);
+      sum_groups<VE, NC, GN, 1, WARP>(own, room, result + kGroups, me, t.slots, t.lines);
+      for (int g = thread; g < me.groups; g += size) parts[g] = make_float2(result[g] * share, result[kGroups + g]);
     } else {
       float2 st[NC][GN];
-      load_stats(s, c, me, seg, st);
+      load_stats(s, c.stats, me, seg, st);
       float ab[2][NC][VE];
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int i = 0; i < VE; ++i) ab[0][j][i] = ab[1][j][i] = 0.0f;
-      for (int64_t r0 = b + me.line; r0 < e; r0 += 2 * t.lines) {
+      for (; left > 0; left -= 2 * t.lines, at += 2 * step) {
         Raw<T, VE> rx[2][NC], rg[2][NC];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int j = 0; j < NC; ++j)
-            if (me.in[j] && r0 + u * t.lines < e) {
-              rx[u][j] = load_raw<T, VE>(x + (r0 + u * t.lines) * s.dim + me.col[j]);
-              rg[u][j] = load_raw<T, VE>(grad + (r0 + u * t.lines) * s.dim + me.col[j]);
+            if (me.in[j] && left > u * t.lines) {
+              rx[u][j] = load_raw<T, VE>(x + at + u * step + me.col[j]);
+              rg[u][j] = load_raw<T, VE>(grad + at + u * step + me.col[j]);
             }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          if (r0 + u * t.lines >= e) break;
+          if (left <= u * t.lines) break;
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
             if (!me.in[j]) continue;
@@ -602,7 +637,7 @@ __device__ __forceinline__ void tile_sums(const NormShape& s, const NormCall& c,
 #pragma unroll
             for (int i = 0; i < VE; ++i) xh[i] = rx[u][j].get(i), dz[i] = rg[u][j].get(i);
             normalise(xh, st[j]);
-            begin_backward(c, (r0 + u * t.lines) * s.dim + me.col[j], xh, dz, gamma[j], beta[j]);
+            begin_backward<kMaskLeft>(c, at + u * step + me.col[j], xh, dz, gamma[j], beta[j]);
 #pragma unroll
             for (int i = 0; i < VE; ++i) ab[0][j][i] += dz[i], ab[1][j][i] = fmaf(dz[i], xh[i], ab[1][j][i]);
           }
@@ -613,319 +648,150 @@ __device__ __forceinline__ void tile_sums(const NormShape& s, const NormCall& c,
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
           dbeta[j][i] += ab[0][j][i], dgamma[j][i] += ab[1][j][i];
-          ab[0][j][i] *= gamma[j][i], ab[1][j][i] *= gamma[j][i];
+          // one rounding, as of a single row's
+          ab[0][j][i] = __fmul_rn(ab[0][j][i], gamma[j][i]), ab[1][j][i] *= gamma[j][i];
         }
-      sum_groups<VE, NC, GN, 2, false>(ab, room, result, me, t.slots, t.lines, me.line);
-      for (int g = threadIdx.x; g < me.groups; g += 256) parts[g] = make_float2(result[2 * g], result[2 * g + 1]);
+      sum_groups<VE, NC, GN, 2, WARP>(ab, room, result, me, t.slots, t.lines);
+      for (int g = thread; g < me.groups; g += size) parts[g] = make_float2(result[2 * g], result[2 * g + 1]);
     }
-    __syncthreads();      // `result` is the next piece's
+    if (WARP) __syncwarp(); else __syncthreads();      // `result` is the next piece's
   }
-  if constexpr (BACK)
-    if (c.columns) put_columns(s, c, t, me, room, dgamma, dbeta);
-}
-
-// Whole segments, each by a block or a warp: rows in registers, in chunks where they are more (which are read again then, from L1).
-// A warp has eight chunks at most: 55001 x 64 f16 in 2048 segments, whose blocks of 256 threads were 86 us of latency backwards.
-constexpr int kWarpChunks = 8;
-constexpr int held_rows(bool back, int nc) { return (back ? 2 : 8) / nc > 0 ? (back ? 2 : 8) / nc : 1; }
-template <typename T, int VE, int NC, int GN, bool BACK, bool WARP>
-__device__ __forceinline__ void short_segments(const NormShape& s, const NormCall& c, const NormTiles& t, float* room, float* result) {
-  constexpr int kHeld = held_rows(BACK, NC), kTeams = WARP ? 8 : 1;
-  const NormThread<VE, NC, GN> me(s, t);
-  const int lines = t.lines / kTeams, line = me.line % lines, warp = threadIdx.x / 32, tid = WARP ? threadIdx.x % 32 : threadIdx.x, team = WARP ? 32 : 256;
-  float* const my_room = WARP ? room + warp * (32 * NC * VE + 32) : room;
-  float* const sums = WARP ? result + warp * 512 : result;      // 256 columns are 256 groups at most
-  float* const squares = WARP ? sums + 256 : sums + kMostGroups;
-  const T* const x = (const T*)c.x;
-  const T* const grad = (const T*)c.grad;
-  T* const out = (T*)c.out;
-  float gamma[NC][VE], beta[NC][VE], dgamma[NC][VE], dbeta[NC][VE];
-  load_params<T>(c, me, gamma, beta);
-#pragma unroll
-  for (int j = 0; j < NC; ++j)
-#pragma unroll
-    for (int i = 0; i < VE; ++i) dgamma[j][i] = dbeta[j][i] = 0.0f;
-  const int64_t first = (int64_t)(blockIdx.x - t.tiles) * kTeams + (WARP ? warp : 0);
-  for (int64_t seg = first; seg < s.segments; seg += (int64_t)t.short_blocks * kTeams) {
-    const RowRange r = segment_rows(s, seg);
-    const int rows = (int)min(r.end - r.begin, (int64_t)t.cap + 1);
-    if (rows > t.cap || rows == 0) continue;
-    const int chunks = (rows + kHeld * lines - 1) / (kHeld * lines);
-    const float inv = 1.0f / ((float)rows * (float)me.per);
-    Raw<T, VE> rx[kHeld][NC], rg[BACK ? kHeld : 1][NC];
-    const auto row_of = [&](int chunk, int u) { return (chunk * kHeld + u) * lines + line; };
-    const auto load = [&](int chunk, bool both) {
-#pragma unroll
-      for (int u = 0; u < kHeld; ++u)
-#pragma unroll
-        for (int j = 0; j < NC; ++j)
-          if (me.in[j] && row_of(chunk, u) < rows) {
-            rx[u][j] = load_raw<T, VE>(x + (r.begin + row_of(chunk, u)) * s.dim + me.col[j]);
-            if constexpr (BACK) rg[u][j] = load_raw<T, VE>(grad + (r.begin + row_of(chunk, u)) * s.dim + me.col[j]);
-          }
-    };
-    load(0, BACK);
-    float2 st[NC][GN];
-    if constexpr (!BACK) {
-      float own[1][NC][VE];
-#pragma unroll
-      for (int j = 0; j < NC; ++j)
-#pragma unroll
-        for (int i = 0; i < VE; ++i) own[0][j][i] = 0.0f;
-      for (int k = 0; k < chunks; ++k) {
-        if (k) load(k, false);
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-#pragma unroll
-          for (int j = 0; j < NC; ++j)
-            if (me.in[j] && row_of(k, u) < rows)
-#pragma unroll
-              for (int i = 0; i < VE; ++i) own[0][j][i] += rx[u][j].get(i);
-      }
-      sum_groups<VE, NC, GN, 1, WARP>(own, my_room, sums, me, t.slots, lines, line);
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-#pragma unroll
-        for (int i = 0; i < GN; ++i) st[j][i].x = sums[me.group[j][i]] * inv;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) own[0][j][i] = 0.0f;
-      }
-      for (int k = 0; k < chunks; ++k) {
-        if (chunks > 1) load(k, false);
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-#pragma unroll
-          for (int j = 0; j < NC; ++j)
-            if (me.in[j] && row_of(k, u) < rows)
-#pragma unroll
-              for (int i = 0; i < VE; ++i) {
-                const float d = rx[u][j].get(i) - st[j][i % GN].x;
-                own[0][j][i] = fmaf(d, d, own[0][j][i]);
-              }
-      }
-      sum_groups<VE, NC, GN, 1, WARP>(own, my_room, squares, me, t.slots, lines, line);
-#pragma unroll
-      for (int j = 0; j < NC; ++j)
-#pragma unroll
-        for (int i = 0; i < GN; ++i) st[j][i].y = rsqrtf(squares[me.group[j][i]] * inv + c.eps);
-      for (int g = tid; g < me.groups; g += team) c.stats[seg * s.groups + me.group0 + g] = make_float2(sums[g] * inv, rsqrtf(squares[g] * inv + c.eps));
-      for (int k = 0; k < chunks; ++k) {
-        if (chunks > 1) load(k, false);
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-#pragma unroll
-          for (int j = 0; j < NC; ++j)
-            if (me.in[j] && row_of(k, u) < rows) {
-              float v[VE];
-#pragma unroll
-              for (int i = 0; i < VE; ++i) v[i] = rx[u][j].get(i);
-              normalise(v, st[j]);
-              const int64_t e = (r.begin + row_of(k, u)) * s.dim + me.col[j];
-              finish_forward(c, e, v, gamma[j], beta[j]);
-              store_all<T, VE>(out + e, v);
-            }
-      }
-    } else {
-      load_stats(s, c, me, seg, st);
-      float ab[2][NC][VE], dz[kHeld][NC][VE];
-#pragma unroll
-      for (int j = 0; j < NC; ++j)
-#pragma unroll
-        for (int i = 0; i < VE; ++i) ab[0][j][i] = ab[1][j][i] = 0.0f;
-      const auto begin = [&](int k) {
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-#pragma unroll
-          for (int j = 0; j < NC; ++j)
-            if (me.in[j] && row_of(k, u) < rows) {
-              float xh[VE];
-#pragma unroll
-              for (int i = 0; i < VE; ++i) xh[i] = rx[u][j].get(i), dz[u][j][i] = rg[u][j].get(i);
-              normalise(xh, st[j]);
-              begin_backward(c, (r.begin + row_of(k, u)) * s.dim + me.col[j], xh, dz[u][j], gamma[j], beta[j]);
-            }
-      };
-      for (int k = 0; k < chunks; ++k) {
-        if (k) load(k, true);
-        begin(k);
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-#pragma unroll
-          for (int j = 0; j < NC; ++j)
-            if (me.in[j] && row_of(k, u) < rows)
-#pragma unroll
-              for (int i = 0; i < VE; ++i) {
-                const float v = dz[u][j][i], xh = (rx[u][j].get(i) - st[j][i % GN].x) * st[j][i % GN].y, dxh = __fmul_rn(v, gamma[j][i]);
-                dbeta[j][i] += v, dgamma[j][i] = fmaf(v, xh, dgamma[j][i]);
-                ab[0][j][i] += dxh, ab[1][j][i] = fmaf(dxh, xh, ab[1][j][i]);
-              }
-      }
-      sum_groups<VE, NC, GN, 2, WARP>(ab, my_room, sums, me, t.slots, lines, line);
-      float2 means[NC][GN];
-#pragma unroll
-      for (int j = 0; j < NC; ++j)
-#pragma unroll
-        for (int i = 0; i < GN; ++i) means[j][i] = make_float2(sums[2 * me.group[j][i]] * inv, sums[2 * me.group[j][i] + 1] * inv);
-      for (int k = 0; k < chunks; ++k) {
-        if (chunks > 1) {
-          load(k, true);
-          begin(k);
-        }
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-#pragma unroll
-          for (int j = 0; j < NC; ++j)
-            if (me.in[j] && row_of(k, u) < rows) {
-              float v[VE], dxh[VE];
-#pragma unroll
-              for (int i = 0; i < VE; ++i) v[i] = rx[u][j].get(i), dxh[i] = __fmul_rn(dz[u][j][i], gamma[j][i]);
-              normalise(v, st[j]);
-              finish_backward(v, dxh, st[j], means[j]);
-              store_all<T, VE>(out + (r.begin + row_of(k, u)) * s.dim + me.col[j], v);
-            }
-      }
-    }
-    if (WARP) __syncwarp(); else __syncthreads();      // `sums` are the next segment's
-  }
-  if constexpr (BACK)
-    if (c.columns) put_columns(s, c, t, me, room, dgamma, dbeta);
-}
-
-// Offsets that are none are flagged, and segments without rows have statistics of zero.
-__device__ __forceinline__ void look_at_segments(const NormShape& s, const NormCall& c) {
-  for (int64_t seg = threadIdx.x; seg < s.segments; seg += blockDim.x) {
-    const RowRange r = group_rows(s.offsets, (int)seg, s.rows);
-    if (bad_group(s.offsets, (int)seg, s.rows)) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
-    if (r.end <= r.begin)
-      for (int g = 0; g < s.groups; ++g) c.stats[seg * s.groups + g] = make_float2(0.0f, 0.0f);
+  if constexpr (BACK) {
+    if (!c.columns) return;
+    __syncthreads();
+    put_columns<WARP>(s, c, t, me, rooms, dgamma, dbeta);
   }
 }
 
-// Sums alone, where segments are long.
-template <typename T, int VE, int NC, int GN, bool BACK>
-__global__ void __launch_bounds__(256, BACK ? 2 : 4)
-k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t) {
-  wait_for_previous();
-  __shared__ float room[256 * NC * VE + 256], result[2 * kMostGroups];
-  if (!BACK && s.offsets && blockIdx.x == 0 && blockIdx.y == 0) look_at_segments(s, c);
-  tile_sums<T, VE, NC, GN, BACK>(s, c, t, room, result);
-}
-// Sums of long segments and all of short ones.
-template <typename T, int VE, int NC, int GN, bool BACK, bool WARP>
-__global__ void __launch_bounds__(256, 2)
-k_norm_first(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t) {
-  wait_for_previous();
-  __shared__ float room[256 * NC * VE + 256], result[WARP ? 8 * 512 : 2 * kMostGroups];
-  if (!BACK && s.offsets && blockIdx.x == 0 && blockIdx.y == 0) look_at_segments(s, c);
-  if (blockIdx.x < t.tiles) tile_sums<T, VE, NC, GN, BACK>(s, c, t, room, result);
-  else short_segments<T, VE, NC, GN, BACK, WARP>(s, c, t, room, result);
-}
-
-// Rows of long segments, and rows of none. Tiles from the last to the first: what was read last is still in L2.
-template <typename T, int VE, int NC, int GN, bool BACK>
-__global__ void __launch_bounds__(256, GN > 1 || NC > 1 ? 2 : BACK ? 3 : 4)
-k_norm_second(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t, int joins) {
+// The pieces of each segment joined, a block for some groups of a segment: forwards mean and 1 / deviation (zeros for a segment without rows),
+// backwards the two means. The first `joins` blocks join the columns' sums for dgamma and dbeta. Offsets that are none are flagged here.
+template <typename T, bool BACK>
+__global__ void __launch_bounds__(256)
+k_norm_join(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t, int joins, int64_t lines) {
   wait_for_previous();
   if (BACK && (int)blockIdx.x < joins) {
-    if (blockIdx.y == 0) join_columns<T>(s, c, blockIdx.x, t.tiles + t.short_blocks);
+    if (blockIdx.y == 0) join_columns<T>(s, c, blockIdx.x, lines);
     return;
   }
-  __shared__ float2 table[kMostGroups];
-  const NormThread<VE, NC, GN> me(s, t);
+  __shared__ float2 part[256];
+  const int64_t seg = blockIdx.x - joins;
+  const RowRange r = segment_rows(s, seg);
+  if (!BACK && s.offsets && blockIdx.y == 0 && threadIdx.x == 0 && bad_group(s.offsets, (int)seg, s.rows)) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
+  const int width = t.join_groups, g = blockIdx.y * width + threadIdx.x % width, lane = threadIdx.x / width, lanes = 256 / width;
+  const bool mine = g < s.groups && lane < lanes;
+  float2* const to = BACK ? c.means : c.stats;
+  if (r.end <= r.begin) {
+    if (mine && lane == 0) to[seg * s.groups + g] = make_float2(0.0f, 0.0f);
+    return;
+  }
+  const int64_t first = r.begin / t.sum_rows, last = (r.end - 1) / t.sum_rows;
+  const float2* const parts = c.parts + seg * s.groups + g;
+  const float inv = 1.0f / ((float)(r.end - r.begin) * (float)s.per);
+  const auto count = [&](int64_t i) { return (float)(min((i + 1) * t.sum_rows, r.end) - max(i * t.sum_rows, r.begin)) * (float)s.per; };
+  const auto together = [&](float2 v) {
+    __syncthreads();
+    if (mine) part[threadIdx.x] = v;
+    __syncthreads();
+    v = make_float2(0.0f, 0.0f);
+    if (mine)
+      for (int k = 0; k < lanes; ++k) v.x += part[k * width + threadIdx.x % width].x, v.y += part[k * width + threadIdx.x % width].y;
+    return v;
+  };
+  float2 v = make_float2(0.0f, 0.0f);
+  if (mine)
+#pragma unroll 4
+    for (int64_t i = first + lane; i <= last; i += lanes) {
+      const float2 p = parts[i * s.groups];
+      if constexpr (BACK) v.x += p.x, v.y += p.y;
+      else v.x = fmaf(p.x, count(i), v.x);
+    }
+  v = together(v);
+  const float mean = v.x * inv;
+  if constexpr (!BACK) {
+    v = make_float2(0.0f, 0.0f);
+    if (mine)
+#pragma unroll 4
+      for (int64_t i = first + lane; i <= last; i += lanes) {
+        const float2 p = parts[i * s.groups];
+        v.y += fmaf(count(i) * (p.x - mean), p.x - mean, p.y);
+      }
+    v = together(v);
+  }
+  if (mine && lane == 0) to[seg * s.groups + g] = make_float2(mean, BACK ? v.y * inv : rsqrtf(v.y * inv + c.eps));
+}
+
+// The rows themselves, and zeros for rows of no segment. Tiles from the last to the first: what k_norm_sums read last is still in L2.
+template <typename T, int VE, int NC, int GN, bool BACK, bool WARP>
+__global__ void __launch_bounds__(256, GN > 1 || NC > 1 ? 2 : 3)
+k_norm_apply(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t) {
+  wait_for_previous();
+  const NormThread<VE, NC, GN> me(s, t, WARP ? threadIdx.x % 32 : threadIdx.x);
   const T* const x = (const T*)c.x;
   const T* const grad = (const T*)c.grad;
   T* const out = (T*)c.out;
-  const int64_t tile = t.tiles - 1 - (blockIdx.x - joins), row0 = tile * t.tile, row1 = min(row0 + t.tile, s.rows);
+  const int64_t tile = t.apply_tiles - 1 - ((int64_t)blockIdx.x * (WARP ? 8 : 1) + (WARP ? threadIdx.x / 32 : 0));
+  if (tile < 0 || !me.mine) return;
+  const int64_t row0 = tile * t.apply_rows, row1 = min(row0 + t.apply_rows, s.rows), step = t.lines * s.dim;
   float gamma[NC][VE], beta[NC][VE];
-  bool loaded = false;
+  load_params<T>(c, me, gamma, beta);
   int64_t done = row0;      // rows up to here are of segments
   for (int64_t seg = segment_at(s, row0); seg < s.segments; ++seg) {
     const RowRange whole = segment_rows(s, seg);
     if (whole.begin >= row1) break;
     const int64_t b = max(whole.begin, row0), e = min(whole.end, row1);
+    if (e <= b) continue;
     if (e > done) done = e;
-    if (whole.end - whole.begin <= t.cap || e <= b) continue;
-    if (!loaded) load_params<T>(c, me, gamma, beta);
-    loaded = true;
-    // the segment's pieces, a warp a group
-    const int64_t first = whole.begin / t.tile, last = (whole.end - 1) / t.tile;
-    const float inv = 1.0f / ((float)(whole.end - whole.begin) * (float)me.per);
-    __syncthreads();
-    for (int g = threadIdx.x / 32; g < me.groups; g += 8) {
-      const float2* const parts = c.parts + me.group0 + g;
-      const auto rows_of = [&](int64_t i) { return (float)(min((i + 1) * t.tile, whole.end) - max(i * t.tile, whole.begin)); };
-      float a = 0.0f, q = 0.0f;
-      for (int64_t i = first + threadIdx.x % 32; i <= last; i += 32) {
-        const float2 p = parts[(i + seg) * s.groups];
-        if constexpr (BACK) a += p.x, q += p.y;
-        else a = fmaf(p.x, rows_of(i) * (float)me.per, a);
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        if constexpr (BACK) q += __shfl_xor_sync(0xffffffffu, q, o);
-      }
-      a *= inv;
-      if constexpr (!BACK) {
-        for (int64_t i = first + threadIdx.x % 32; i <= last; i += 32) {
-          const float2 p = parts[(i + seg) * s.groups];
-          q += fmaf(rows_of(i) * (float)me.per * (p.x - a), p.x - a, p.y);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-      }
-      if (threadIdx.x % 32 == 0) {
-        const float2 r = make_float2(a, BACK ? q * inv : rsqrtf(q * inv + c.eps));
-        table[g] = r;
-        if (!BACK && tile == first) c.stats[seg * s.groups + me.group0 + g] = r;
-      }
-    }
-    __syncthreads();
     float2 st[NC][GN], ab[BACK ? NC : 1][GN];
-    if constexpr (BACK) load_stats(s, c, me, seg, st);
+    load_stats(s, c.stats, me, seg, st);
+    if constexpr (BACK) load_stats(s, c.means, me, seg, ab);
+    // forwards (x - mean) (gamma / deviation) + beta
+    float scale[BACK ? 1 : NC][VE];
+    if constexpr (!BACK)
 #pragma unroll
-    for (int j = 0; j < NC; ++j)
+      for (int j = 0; j < NC; ++j)
 #pragma unroll
-      for (int i = 0; i < GN; ++i) (BACK ? ab : st)[j][i] = table[me.group[j][i]];
+        for (int i = 0; i < VE; ++i) scale[j][i] = gamma[j][i] * st[j][i % GN].y;
     constexpr int U = BACK ? 2 : 4;
-    for (int64_t r0 = b + me.line; r0 < e; r0 += U * t.lines) {
+    int left = (int)(e - b) - me.line;
+    for (int64_t at0 = (b + me.line) * s.dim; left > 0; left -= U * t.lines, at0 += U * step) {
       Raw<T, VE> rx[U][NC], rg[BACK ? U : 1][NC];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < NC; ++j)
-          if (me.in[j] && r0 + u * t.lines < e) {
-            rx[u][j] = load_raw<T, VE>(x + (r0 + u * t.lines) * s.dim + me.col[j]);
-            if constexpr (BACK) rg[u][j] = load_raw<T, VE>(grad + (r0 + u * t.lines) * s.dim + me.col[j]);
+          if (me.in[j] && left > u * t.lines) {
+            rx[u][j] = load_raw<T, VE>(x + at0 + u * step + me.col[j]);
+            if constexpr (BACK) rg[u][j] = load_raw<T, VE>(grad + at0 + u * step + me.col[j]);
           }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (r0 + u * t.lines >= e) break;
+        if (left <= u * t.lines) break;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
           if (!me.in[j]) continue;
-          const int64_t at = (r0 + u * t.lines) * s.dim + me.col[j];
+          const int64_t at = at0 + u * step + me.col[j];
           float v[VE];
-#pragma unroll
-          for (int i = 0; i < VE; ++i) v[i] = rx[u][j].get(i);
-          normalise(v, st[j]);
           if constexpr (BACK) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) v[i] = rx[u][j].get(i);
+            normalise(v, st[j]);
             float dz[VE];
 #pragma unroll
             for (int i = 0; i < VE; ++i) dz[i] = rg[u][j].get(i);
-            begin_backward(c, at, v, dz, gamma[j], beta[j]);
+            begin_backward<kMaskTaken>(c, at, v, dz, gamma[j], beta[j]);
 #pragma unroll
             for (int i = 0; i < VE; ++i) dz[i] = __fmul_rn(dz[i], gamma[j][i]);
             finish_backward(v, dz, st[j], ab[j]);
           } else {
-            finish_forward(c, at, v, gamma[j], beta[j]);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) v[i] = rx[u][j].get(i) - st[j][i % GN].x;
+            finish_forward(c, at, v, scale[j], beta[j]);
           }
           store_all<T, VE>(out + at, v);
         }
       }
     }
   }
-  // rows of no segment
   const float zeros[VE] = {};
   for (int64_t r = done + me.line; r < row1; r += t.lines)
 #pragma unroll
@@ -949,7 +815,7 @@ __device__ __forceinline__ float2 wide_xh_dz(const NormCall& c, int64_t e, int64
   const float g = *gamma = param<T>(c.weight, c.wide_params, col, 1.0f);
   float xh[1] = {(Elem<T>::to_f(((const T*)c.x)[e]) - st.x) * st.y}, dz[1] = {Elem<T>::to_f(((const T*)c.grad)[e])};
   const float gs[1] = {g}, bs[1] = {param<T>(c.bias, c.wide_params, col, 0.0f)};
-  begin_backward(c, e, xh, dz, gs, bs);
+  begin_backward<kMaskMade>(c, e, xh, dz, gs, bs);
   return make_float2(xh[0], dz[0]);
 }
 template <typename T, bool BACK>
@@ -1032,7 +898,7 @@ struct NormPlan {
   int held;               // slices a lane (thread) has of a row
   int64_t blocks, chunks; // grid of the first kernel
   NormTiles tiles;
-  bool warps;             // short segments by warps
+  bool warps;             // tiles by warps
 };
 
 template <typename T, int VE, bool BACK>
@@ -1049,22 +915,22 @@ static int norm_rows(const NormShape& s, const NormCall& c, const NormPlan& p, c
   if (BACK && c.columns) APT_FOLLOW((k_norm_columns<T>), ceil_div(2 * s.dim, 32), 256, 0, st, s, c, p.blocks);
   return APT_OK;
 }
-template <typename T, int VE, int NC, int GN, bool BACK>
+template <typename T, int VE, int NC, int GN, bool BACK, bool WARP>
 static int norm_tiles(const NormShape& s, const NormCall& c, const NormPlan& p, cudaStream_t st) {
-  const dim3 first((unsigned)p.blocks, (unsigned)p.chunks);
-  if (!p.tiles.short_blocks) APT_FOLLOW((k_norm_sums<T, VE, NC, GN, BACK>), first, 256, 0, st, s, c, p.tiles);
-  else if (p.warps) APT_FOLLOW((k_norm_first<T, VE, NC, GN, BACK, true>), first, 256, 0, st, s, c, p.tiles);
-  else APT_FOLLOW((k_norm_first<T, VE, NC, GN, BACK, false>), first, 256, 0, st, s, c, p.tiles);
+  const NormTiles& t = p.tiles;
+  const dim3 sums((unsigned)p.blocks, (unsigned)p.chunks), apply((unsigned)ceil_div(t.apply_tiles, WARP ? 8 : 1), (unsigned)p.chunks);
+  APT_FOLLOW((k_norm_sums<T, VE, NC, GN, BACK, WARP>), sums, 256, 0, st, s, c, t);
   const int joins = BACK && c.columns ? (int)ceil_div(2 * s.dim, 32) : 0;
-  const dim3 second((unsigned)(p.tiles.tiles + joins), (unsigned)p.chunks);
-  APT_FOLLOW((k_norm_second<T, VE, NC, GN, BACK>), second, 256, 0, st, s, c, p.tiles, joins);
+  const dim3 join((unsigned)(joins + s.segments), (unsigned)ceil_div(s.groups, t.join_groups));
+  APT_FOLLOW((k_norm_join<T, BACK>), join, 256, 0, st, s, c, t, joins, p.blocks);
+  APT_FOLLOW((k_norm_apply<T, VE, NC, GN, BACK, WARP>), apply, 256, 0, st, s, c, t);
   return APT_OK;
 }
 template <typename T, int VE, int NC, bool BACK>
 static int norm_held(const NormShape& s, const NormCall& c, const NormPlan& p, cudaStream_t st) {
   if constexpr (VE > 1)
-    if (s.per % VE) return norm_tiles<T, VE, NC, VE, BACK>(s, c, p, st);
-  return norm_tiles<T, VE, NC, 1, BACK>(s, c, p, st);
+    if (s.per % VE) return p.warps ? norm_tiles<T, VE, NC, VE, BACK, true>(s, c, p, st) : norm_tiles<T, VE, NC, VE, BACK, false>(s, c, p, st);
+  return p.warps ? norm_tiles<T, VE, NC, 1, BACK, true>(s, c, p, st) : norm_tiles<T, VE, NC, 1, BACK, false>(s, c, p, st);
 }
 template <typename T, int VE, bool BACK>
 static int norm_slices(const NormShape& s, const NormCall& c, const NormPlan& p, cudaStream_t st) {

@@ -95,6 +95,15 @@ __device__ __forceinline__ float act_slope(float z) {
   return 1.0f;
 }
 
+// N neighbouring elements, rounded.
+template <typename T, int N>
+__device__ __forceinline__ void store_all(T* p, const float (&v)[N]) {
+  Pack<T, N> r;
+#pragma unroll
+  for (int k = 0; k < N; ++k) r.v[k] = Elem<T>::from_f(v[k]);
+  store_pack<T, N>(p, r);
+}
+
 // ---- ragged groups --------------------------------------------------------------
 // Group g has the rows [offsets[g], offsets[g + 1]). Ends that do not ascend, begin elsewhere than at 0 or lie beyond the rows are
 // flagged, and whatever they are no row outside [0, rows) is touched.

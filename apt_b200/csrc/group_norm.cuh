@@ -43,13 +43,20 @@ __device__ __forceinline__ RowRange segment_rows(const NormShape& s, int64_t k) 
   if (s.offsets) return group_rows(s.offsets, (int)k, s.rows);
   return {k * s.per_segment, (k + 1) * s.per_segment};
 }
-// The first segment that ends behind the row.
+// The first segment that ends behind the row, by all lanes of a warp: 32 ends are looked at in a round.
 __device__ __forceinline__ int64_t segment_at(const NormShape& s, int64_t row) {
   if (!s.offsets) return row / s.per_segment;
   int64_t lo = 0, hi = s.segments;
   while (lo < hi) {
-    const int64_t m = (lo + hi) / 2;
-    if (s.offsets[m + 1] <= row) lo = m + 1; else hi = m;
+    const int64_t step = (hi - lo + 31) / 32, at = lo + (threadIdx.x % 32) * step;
+    const uint32_t behind = __ballot_sync(0xffffffffu, at < hi && s.offsets[at + 1] > row);
+    if (behind) {
+      const int first = __ffs(behind) - 1;
+      hi = lo + first * step;
+      if (first) lo = hi - step + 1;
+    } else {
+      lo += (hi - 1 - lo) / step * step + 1;
+    }
   }
   return lo;
 }
@@ -119,14 +126,6 @@ __device__ __forceinline__ void drop_all(const Drop& d, int64_t e, float (&v)[N]
     for (int k = 0; k < N; ++k) v[k] = dropped(d, at + k == 0 ? w.w[0] : at + k == 1 ? w.w[1] : at + k == 2 ? w.w[2] : w.w[3], v[k]);
   }
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_all(T* p, const float (&v)[N]) {
-  Pack<T, N> r;
-#pragma unroll
-  for (int k = 0; k < N; ++k) r.v[k] = Elem<T>::from_f(v[k]);
-  store_pack<T, N>(p, r);
-}
-
 // Which of the elements from e on stay, a bit each.
 template <int N>
 __device__ __forceinline__ uint32_t kept(const Drop& d, int64_t e) {
@@ -730,12 +729,13 @@ k_norm_apply(const __grid_constant__ NormShape s, const __grid_constant__ NormCa
   const T* const grad = (const T*)c.grad;
   T* const out = (T*)c.out;
   const int64_t tile = t.apply_tiles - 1 - ((int64_t)blockIdx.x * (WARP ? 8 : 1) + (WARP ? threadIdx.x / 32 : 0));
-  if (tile < 0 || !me.mine) return;
+  if (tile < 0) return;
   const int64_t row0 = tile * t.apply_rows, row1 = min(row0 + t.apply_rows, s.rows), step = t.lines * s.dim;
   float gamma[NC][VE], beta[NC][VE];
   load_params<T>(c, me, gamma, beta);
-  int64_t done = row0;      // rows up to here are of segments
-  for (int64_t seg = segment_at(s, row0); seg < s.segments; ++seg) {
+  int64_t done = row0, seg = segment_at(s, row0);      // rows up to here are of segments
+  if (!me.mine) return;
+  for (; seg < s.segments; ++seg) {
     const RowRange whole = segment_rows(s, seg);
     if (whole.begin >= row1) break;
     const int64_t b = max(whole.begin, row0), e = min(whole.end, row1);

@@ -27,9 +27,9 @@ namespace apt {
 enum GroupedMode { kOut = 0, kGradX = 1, kGradW = 2 };
 
 constexpr int kTileM = 128;                  // rows of a product
-constexpr int kStageBytes = 227 * 1024;      // shared memory of a block
+constexpr int kMostShared = 227 * 1024 - 640;      // shared memory of a block but for the barriers' and the scan's
 constexpr int kAccColumns = 256;             // tensor memory of a tile: two of them, or one and the sums of the bias
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 12;
 
 template <typename T, int MODE>
 struct GroupedTraits {
@@ -38,7 +38,9 @@ struct GroupedTraits {
   static constexpr int kBlock = kSplit ? 32 : 64;              // of the contraction in a stage
   static constexpr int kBox = 128 / (int)sizeof(T);            // elements of a box's row
   static constexpr int kMostN = kSplit ? 128 : 256;            // columns of a tile
-  static constexpr int kThreads = kSplit ? 512 : 256;
+  // warps that bring tiles out: two for each quarter of tensor memory's lanes, or one beside the eight that take fp32 apart
+  static constexpr int kOutWarps = kSplit ? 4 : 8;
+  static constexpr int kThreads = kSplit ? 512 : 384;
   static constexpr int kPieces = kSplit ? 3 : 1;
   // bytes of a tile of n rows (or columns) in a stage as copied, and of one bf16 piece of it
   static __host__ __device__ constexpr int copied(int n, bool mn) { return mn ? (n + kBox - 1) / kBox * kBlock * 128 : n * 128; }
@@ -58,7 +60,7 @@ struct GroupedCall {
   const void* bias;
   void *out, *grad_bias;
   float *partial, *partial_bias;
-  int64_t* plan;                // dw: for k_join_weights
+  int64_t* plan;                // dw, for k_join_weights: units, runs, and of each run the first piece's tile and group, first and last unit
   int32_t* status;
 };
 
@@ -69,6 +71,8 @@ struct GroupedItem {
   int rows;                     // of the group from there on, in out and dx at most tile_m
   int m0, n0, stages;
   int64_t piece;                // dw: number of the partial sum, -1: all of the sum
+  int64_t first, last;          // dw: units of all of the sum
+  int64_t run;                  // dw: the run that begins here, -1: none
 };
 
 // Runs of stages of dw: every run is as long as any other within one, whatever the groups are. A run has all stages of the tiles and
@@ -128,6 +132,8 @@ struct GroupedWalk {
       item->m0 = tile / c.tiles_n * kTileM;
       item->n0 = tile % c.tiles_n * c.tile_n;
       item->piece = n == prefix[g + 1] - prefix[g] ? -1 : 2 * step + (next != runs.begin(step));
+      item->run = next == runs.begin(step) ? step : -1;
+      item->first = (int64_t)tile * total + prefix[g], item->last = (int64_t)tile * total + prefix[g + 1];
       next += n;
       return true;
     } else {
@@ -143,7 +149,7 @@ struct GroupedWalk {
       item->m0 = 0;
       item->n0 = (int)(next % c.tiles_n) * c.tile_n;
       item->stages = g < c.groups ? (c.num_k + Tr::kBlock - 1) / Tr::kBlock : 0;      // rows of no group: zeros
-      item->piece = -1;
+      item->piece = -1, item->run = -1, item->first = item->last = 0;
       next += step;
       return true;
     }
@@ -221,72 +227,77 @@ __device__ __noinline__ float column_again(const GroupedCall& c, const GroupedIt
 }
 
 // ---- bringing a tile out -------------------------------------------------------------
-// A warp's 32 rows, 128 bytes of each at a time, through shared memory, so that the stores are whole rows of 128 bytes.
+// A warp's 32 rows, 128 bytes of each at a time, through shared memory, so that the stores are whole rows of 128 bytes. Warps that share
+// rows take turns.
 template <typename T, typename O, int MODE>
-__device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedItem& item, uint32_t acc, bool empty, char* staging, int lane, int warp,
-                                           O* out, int64_t ld, int rows, int columns, const T* bias) {
+__device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedItem& item, uint32_t acc, bool empty, char* staging, int lane, int quarter, int turn,
+                                           int turns, O* out, int64_t ld, int rows, int columns, const float* bias) {
   using Tr = GroupedTraits<T, MODE>;
-  constexpr int kWide = 128 / (int)sizeof(O);
-  const int m = warp * 32 + lane, here = min(32, rows - warp * 32);
+  constexpr int kWide = 128 / (int)sizeof(O), kPer = 16 / (int)sizeof(O);
+  const int m = quarter * 32 + lane, here = min(32, rows - quarter * 32);
   const bool whole = (ld * (int64_t)sizeof(O)) % 16 == 0;
-  O* const first = out + (int64_t)warp * 32 * ld;
-  for (int c0 = 0; c0 < columns; c0 += kWide) {
+  O* const first = out + (int64_t)quarter * 32 * ld;
+  acc += (uint32_t)quarter << 21;
+  for (int c0 = turn * kWide; c0 < columns; c0 += turns * kWide) {
+    float v[kWide / 32][32];
+    uint32_t wild = 0;
+    if (empty) {
 #pragma unroll
-    for (int h = 0; h < kWide / 32; ++h) {
-      const int at = c0 + 32 * h;
-      if (at >= columns) break;
-      float v[32];
-      uint32_t wild = 0;
-      if (empty) {
+      for (int h = 0; h < kWide / 32; ++h)
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = 0.0f;
-      } else {
-        tmem_load_32(acc + ((uint32_t)warp << 21) + at, v);
-        if constexpr (Tr::kSplit) {
-          float small[32];
-          tmem_load_32(acc + ((uint32_t)warp << 21) + Tr::kMostN + at, small);
-          tmem_wait_loads();
-          settled(v);
-          settled(small);
+        for (int k = 0; k < 32; ++k) v[h][k] = 0.0f;
+    } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            v[k] += small[k];
-            wild |= isfinite(v[k]) ? 0u : 1u << k;
-          }
-        } else {
-          tmem_wait_loads();
-          settled(v);
-        }
-      }
-      if (bias)
-#pragma unroll
-        for (int k = 0; k < 32; ++k)
-          if (at + k < columns) v[k] += Elem<T>::to_f(__ldg(bias + at + k));
-      constexpr int kSlices = 32 * (int)sizeof(O) / 16, kPer = 16 / (int)sizeof(O);
-#pragma unroll
-      for (int s = 0; s < kSlices; ++s) {
-        Pack<O, kPer> p;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) p.v[k] = Elem<O>::from_f(v[s * kPer + k]);
-        *(uint4*)(staging + lane * 128 + (((h * kSlices + s) ^ (lane & 7)) << 4)) = *(const uint4*)&p;
-      }
+      for (int h = 0; h < kWide / 32; ++h) tmem_load_32(acc + c0 + 32 * h, v[h]);
       if constexpr (Tr::kSplit) {
-        if (lane < here)
-          for (; wild; wild &= wild - 1) {
-            const int k = __ffs(wild) - 1;
-            if (at + k < columns)
-              *(float*)(staging + lane * 128 + (((k >> 2) ^ (lane & 7)) << 4) + (k & 3) * 4) =
-                  sum_again<MODE>(c, item, m, at + k) + (bias ? Elem<T>::to_f(bias[at + k]) : 0.0f);
-          }
+        float small[32];
+        tmem_load_32(acc + Tr::kMostN + c0, small);
+        tmem_wait_loads();
+        settled(small);
+        settled(v[0]);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          v[0][k] += small[k];
+          wild |= isfinite(v[0][k]) ? 0u : 1u << k;
+        }
+      } else {
+        tmem_wait_loads();
+#pragma unroll
+        for (int h = 0; h < kWide / 32; ++h) settled(v[h]);
       }
+    }
+    if (bias)
+#pragma unroll
+      for (int h = 0; h < kWide / 32; ++h)
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 b = *(const float4*)(bias + c0 + 32 * h + k);
+          v[h][k] += b.x, v[h][k + 1] += b.y, v[h][k + 2] += b.z, v[h][k + 3] += b.w;
+        }
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      Pack<O, kPer> p;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) p.v[k] = Elem<O>::from_f(v[s * kPer / 32][(s * kPer + k) % 32]);
+      *(uint4*)(staging + lane * 128 + ((s ^ (lane & 7)) << 4)) = *(const uint4*)&p;
+    }
+    if constexpr (Tr::kSplit) {
+      if (lane < here)
+        for (; wild; wild &= wild - 1) {
+          const int k = __ffs(wild) - 1;
+          if (c0 + k < columns)
+            *(float*)(staging + lane * 128 + (((k >> 2) ^ (lane & 7)) << 4) + (k & 3) * 4) = sum_again<MODE>(c, item, m, c0 + k) + (bias ? bias[c0 + k] : 0.0f);
+        }
     }
     __syncwarp();
     if (whole) {
-      const int s = lane & 7, col = c0 + s * (16 / (int)sizeof(O));
+      const int s = lane & 7, r1 = lane >> 3, col = c0 + s * kPer;
+      O* to = first + (int64_t)r1 * ld + col;
+      const char* from = staging + r1 * 128;
+      if (col < columns) {
 #pragma unroll
-      for (int r0 = 0; r0 < 32; r0 += 4) {
-        const int r = r0 + (lane >> 3);
-        if (r < here && col < columns) *(uint4*)(first + r * ld + col) = *(const uint4*)(staging + r * 128 + ((s ^ (r & 7)) << 4));
+        for (int r0 = 0; r0 < 32; r0 += 4, to += 4 * ld)
+          if (r0 + r1 < here) *(uint4*)to = *(const uint4*)(from + r0 * 128 + ((s ^ ((r0 + r1) & 7)) << 4));
       }
     } else {
       for (int r = 0; r < here; ++r)
@@ -319,8 +330,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   char* const copied = shared;
   char* const pieces = copied + (size_t)c.copied_stages * copied_bytes;
   char* const staging = pieces + (size_t)c.piece_stages * piece_bytes;
-  char* const ones = staging + 4 * 4096;
-  int* const prefix = (int*)(ones + (MODE == kGradW ? 2048 : 0));
+  char* const ones = staging + Tr::kOutWarps * 4096;      // (the bias of a tile in out)
+  int* const prefix = (int*)(ones + (MODE == kGradW ? 512 : 1024));
 
   if (warp == 1) tmem_alloc(shared_addr(&tmem_slot), 512);
   if (threadIdx.x == 0) {
@@ -330,13 +341,13 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       barrier_init(shared_addr(ready + k), 8);
       barrier_init(shared_addr(used + k), 1);
     }
-    for (int k = 0; k < 2; ++k) barrier_init(shared_addr(acc_full + k), 1), barrier_init(shared_addr(acc_free + k), 4);
+    for (int k = 0; k < 2; ++k) barrier_init(shared_addr(acc_full + k), 1), barrier_init(shared_addr(acc_free + k), Tr::kOutWarps);
     barrier_init(shared_addr(&drained), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     gave_up_word = 0;
   }
   if constexpr (MODE == kGradW) {
-    for (int i = threadIdx.x; i < 512; i += Tr::kThreads) ((uint32_t*)ones)[i] = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+    for (int i = threadIdx.x; i < 128; i += Tr::kThreads) ((uint32_t*)ones)[i] = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
     fence_for_tensor_cores();
   }
   wait_for_previous();
@@ -366,11 +377,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
-  if constexpr (MODE == kGradW)
-    if (blockIdx.x == 0)
-      for (int g = threadIdx.x; g <= c.groups; g += Tr::kThreads) c.plan[g] = prefix[g];
-
   GroupedWalk<T, MODE> walk(c, prefix);
+  if (MODE == kGradW && blockIdx.x == 0 && threadIdx.x == 0) c.plan[0] = walk.runs.units, c.plan[1] = walk.runs.runs;
   GroupedItem item;
   bool fine = true;
   if (warp == 0) {
@@ -415,7 +423,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const int stages = Tr::kSplit ? c.piece_stages : c.copied_stages;
     const uint32_t what = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, Tr::kMnB, kTileM, c.tile_n);
     const uint32_t what_bias = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, false, kTileM, 16);
-    const uint64_t ones_tile = tile_descriptor(shared_addr(ones), 16, 1024, kSwizzle128);
+    const uint64_t ones_tile = tile_descriptor(shared_addr(ones), 128, 256, 0);      // 16 x 16 in core matrices of 8 x 16 bytes
     int stage = 0, tiles = 0;
     uint32_t phase = 0;
     while (fine && walk.take(&item)) {
@@ -478,14 +486,23 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       products_done(shared_addr(&drained));
       barrier_wait(shared_addr(&drained), 0, &nobody);
     }
-  } else if (warp >= 4 && warp < 8) {
+  } else if (warp >= 4 && warp < 4 + Tr::kOutWarps) {
     // ---- finished tiles
-    const int w = warp - 4;
-    char* const mine = staging + w * 4096;
-    int tiles = 0;
+    const int quarter = warp % 4, turn = (warp - 4) / 4;
+    constexpr int kTurns = Tr::kOutWarps / 4;
+    char* const mine = staging + (warp - 4) * 4096;
+    float* const bias = (float*)ones;
+    int tiles = 0, bias_g = -1, bias_n = -1;
     while (fine && walk.take(&item)) {
       const int buffer = tiles % kBuffers;
       const bool empty = item.stages == 0;
+      if (MODE == kOut && c.bias && !empty && (item.g != bias_g || item.n0 != bias_n)) {
+        bias_g = item.g, bias_n = item.n0;
+        asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");      // the tile before is out
+        for (int k = threadIdx.x - 128; k < 256; k += Tr::kOutWarps * 32)
+          bias[k] = bias_n + k < c.num_n ? Elem<T>::to_f(((const T*)c.bias)[(int64_t)bias_g * c.num_n + bias_n + k]) : 0.0f;
+        asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");
+      }
       if (!empty) {
         fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_full + buffer), (tiles / kBuffers) & 1, gave_up));
         if (!fine) break;
@@ -494,15 +511,20 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       const uint32_t acc = tmem + buffer * kAccColumns;
       const int columns = min(c.tile_n, c.num_n - item.n0);
       if constexpr (MODE == kGradW) {
-        const int rows = min(kTileM, c.num_m - item.m0), m = w * 32 + lane;
-        if (w * 32 < rows) {
+        const int rows = min(kTileM, c.num_m - item.m0), m = quarter * 32 + lane;
+        if (threadIdx.x == 128 && item.run >= 0) {
+          int64_t* const to = c.plan + 2 + 3 * item.run;
+          to[0] = (int64_t)(item.m0 / kTileM * c.tiles_n + item.n0 / c.tile_n) * c.groups + item.g, to[1] = item.first, to[2] = item.last;
+        }
+        if (quarter * 32 < rows) {
           if (item.piece < 0)
-            store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, w, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0, (int64_t)c.num_n, rows, columns,
-                                   (const T*)nullptr);
+            store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0,
+                                   (int64_t)c.num_n, rows, columns, nullptr);
           else
-            store_tile<T, float, MODE>(c, item, acc, empty, mine, lane, w, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows, columns, (const T*)nullptr);
-          if (c.grad_bias && item.n0 == 0) {
-            const uint32_t at = tmem + kAccColumns + ((uint32_t)w << 21);
+            store_tile<T, float, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows,
+                                       columns, nullptr);
+          if (c.grad_bias && item.n0 == 0 && turn == 0) {
+            const uint32_t at = tmem + kAccColumns + ((uint32_t)quarter << 21);
             float v = tmem_load_1(at), small = Tr::kSplit ? tmem_load_1(at + 16) : 0.0f;
             tmem_wait_loads();
             settled(v);
@@ -516,9 +538,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             }
           }
         }
-      } else if (w * 32 < item.rows) {
-        store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, w, (T*)c.out + item.row * c.num_n + item.n0, (int64_t)c.num_n, item.rows, columns,
-                               c.bias && !empty ? (const T*)c.bias + (int64_t)item.g * c.num_n + item.n0 : (const T*)nullptr);
+      } else if (quarter * 32 < item.rows) {
+        store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + item.row * c.num_n + item.n0, (int64_t)c.num_n, item.rows, columns,
+                               MODE == kOut && c.bias && !empty ? bias : nullptr);
       }
       if (!empty) {
         tmem_fence_before();
@@ -526,6 +548,21 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if (lane == 0) barrier_arrive(shared_addr(acc_free + buffer));
         ++tiles;
       }
+    }
+  } else if (MODE == kGradW && warp < 4) {
+    // ---- groups without rows
+    const int64_t per = (int64_t)c.num_m * c.num_n;
+    const bool slices = per * sizeof(T) % 16 == 0;
+    const int64_t from = (int64_t)blockIdx.x * 64 + threadIdx.x - 64, by = (int64_t)gridDim.x * 64;
+    for (int g = 0; g < c.groups; ++g) {
+      if (prefix[g + 1] > prefix[g]) continue;
+      T* const out = (T*)c.out + g * per;
+      if (slices)
+        for (int64_t i = from; i < per * (int64_t)sizeof(T) / 16; i += by) *((uint4*)out + i) = make_uint4(0u, 0u, 0u, 0u);
+      else
+        for (int64_t i = from; i < per; i += by) out[i] = Elem<T>::from_f(0.0f);
+      if (c.grad_bias)
+        for (int64_t i = from; i < c.num_m; i += by) ((T*)c.grad_bias)[(int64_t)g * c.num_m + i] = Elem<T>::from_f(0.0f);
     }
   } else if (Tr::kSplit && warp >= 8) {
     // ---- fp32 taken apart
@@ -540,7 +577,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const char* const in = copied + (size_t)from * copied_bytes;
         char* const out = pieces + (size_t)to * piece_bytes;
         const int valid = MODE == kGradW ? item.rows - k * Tr::kBlock : Tr::kBlock;
-        take_stage_apart<Tr::kMnA>(in, out, kTileM, piece_a, valid, thread);
+        take_stage_apart<Tr::kMnA>(in, out, MODE == kGradW ? kTileM : c.tile_m, piece_a, valid, thread);
         take_stage_apart<Tr::kMnB>(in + copied_a, out + 3 * piece_a, c.tile_n, piece_b, MODE == kGradW ? valid : Tr::kBlock, thread);
         fence_for_tensor_cores();
         __syncwarp();
@@ -559,40 +596,42 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   if (threadIdx.x == 0 && *gave_up) atomicOr(c.status, APT_FLAG_COPY_TIMEOUT);
 }
 
-// The partial sums of dw and db that make up one, in the order of the rows; zeros for groups without rows.
-template <typename T, int BLOCK>
+// The partial sums of dw and db that make up one, in the order of the rows. A run that begins within a sum says so in the plan; the first
+// such run of a sum has it joined: blocks (part of the tile, run).
+template <typename T>
 __global__ void __launch_bounds__(256)
 k_join_weights(const __grid_constant__ GroupedCall c) {
   wait_for_previous();
-  const int total = (int)c.plan[c.groups];
-  const GroupedRuns runs = grouped_runs((int64_t)total * c.tiles_m * c.tiles_n, c.ranges);
-  const int64_t per_row = (c.num_n + 3) / 4, weights = (int64_t)c.groups * c.num_m * per_row, all = weights + (c.grad_bias ? (int64_t)c.groups * c.num_m : 0);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const bool weight = i < weights;
-    const int64_t gm = weight ? i / per_row : i - weights;
-    const int n = weight ? (int)(i % per_row) * 4 : 0, g = (int)(gm / c.num_m), m = (int)(gm % c.num_m);
-    const int tile = m / kTileM * c.tiles_n + n / c.tile_n;
-    const int64_t first = c.plan[g], last = c.plan[g + 1];
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (last > first) {
-      const int64_t base = (int64_t)tile * total, r0 = runs.of(base + first), r1 = runs.of(base + last - 1);
-      if (r0 == r1) continue;      // one sum, which is in its place
-      for (int64_t r = r0; r <= r1; ++r) {
-        const int64_t piece = 2 * r + (runs.begin(r) < base + first);
-        if (weight) {
-          const float4 v = *(const float4*)(c.partial + (piece * kTileM + m % kTileM) * c.tile_n + n % c.tile_n);
-          sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
-        } else {
-          sum[0] += c.partial_bias[piece * kTileM + m % kTileM];
-        }
-      }
+  const GroupedRuns runs{c.plan[0], c.plan[1]};
+  const int64_t v = blockIdx.y + 1;
+  if (v >= runs.runs) return;
+  const int64_t *const from = c.plan + 2 + 3 * v, first = from[1], last = from[2], here = runs.begin(v);
+  if (here <= first || runs.begin(v - 1) > first) return;
+  const int64_t tile = from[0] / c.groups, r1 = runs.of(last - 1);
+  const int g = (int)(from[0] % c.groups), m0 = (int)(tile / c.tiles_n) * kTileM, n0 = (int)(tile % c.tiles_n) * c.tile_n;
+  const int64_t piece = 2 * (v - 1) + (runs.begin(v - 1) < first);
+  const int slices = c.tile_n / 4, i = blockIdx.x * 256 + threadIdx.x, m = i / slices, n = i % slices * 4;
+  if (m < kTileM && m0 + m < c.num_m && n0 + n < c.num_n) {
+    const int64_t size = (int64_t)kTileM * c.tile_n, at = (int64_t)m * c.tile_n + n;
+    float4 sum = *(const float4*)(c.partial + piece * size + at);
+#pragma unroll 4
+    for (int64_t r = v; r <= r1; ++r) {
+      const float4 p = *(const float4*)(c.partial + 2 * r * size + at);
+      sum.x += p.x, sum.y += p.y, sum.z += p.z, sum.w += p.w;
     }
-    if (weight) {
-      for (int k = 0; k < 4; ++k)
-        if (n + k < c.num_n) ((T*)c.out)[gm * c.num_n + n + k] = Elem<T>::from_f(sum[k]);
+    T* const to = (T*)c.out + ((int64_t)g * c.num_m + m0 + m) * c.num_n + n0 + n;
+    const float s[4] = {sum.x, sum.y, sum.z, sum.w};
+    if (c.num_n % 4 == 0) {
+      store_all<T, 4>(to, s);
     } else {
-      ((T*)c.grad_bias)[gm] = Elem<T>::from_f(sum[0]);
+      for (int k = 0; k < 4; ++k)
+        if (n0 + n + k < c.num_n) to[k] = Elem<T>::from_f(s[k]);
     }
+  }
+  if (c.grad_bias && n0 == 0 && i < kTileM && m0 + i < c.num_m) {
+    float sum = c.partial_bias[piece * kTileM + i];
+    for (int64_t r = v; r <= r1; ++r) sum += c.partial_bias[2 * r * kTileM + i];
+    ((T*)c.grad_bias)[(int64_t)g * c.num_m + m0 + i] = Elem<T>::from_f(sum);
   }
 }
 
@@ -698,10 +737,10 @@ static WeightPlan weight_plan(int64_t rows, int64_t dim, int64_t out_dim, int64_
 template <typename T, int MODE>
 static int launch_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap& b, int64_t items, cudaStream_t s) {
   using Tr = GroupedTraits<T, MODE>;
-  const int fixed = 1024 + 4 * 4096 + (MODE == kGradW ? 2048 : 0) + (int)align_up((size_t)(c.groups + 2) * 4, 16);
+  const int fixed = 1024 + Tr::kOutWarps * 4096 + (MODE == kGradW ? 512 : 1024) + (int)align_up((size_t)(c.groups + 2) * 4, 16);
   const int copied = Tr::copied(kTileM, Tr::kMnA) + Tr::copied(c.tile_n, Tr::kMnB);
   const int pieces = Tr::kSplit ? 3 * (Tr::piece(kTileM, Tr::kMnA) + Tr::piece(c.tile_n, Tr::kMnB)) : 0;
-  const int room = kStageBytes - 1024 - fixed;      // 1 KB: barriers
+  const int room = kMostShared - fixed;
   if (Tr::kSplit) {
     c.piece_stages = 2;
     c.copied_stages = std::min(kMaxStages, (room - 2 * pieces) / copied);
@@ -710,10 +749,10 @@ static int launch_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap
     c.copied_stages = std::min(kMaxStages, room / copied);
   }
   const int bytes = fixed + c.copied_stages * copied + c.piece_stages * pieces;
-  static const cudaError_t allowed = cudaFuncSetAttribute(k_grouped<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStageBytes - 1024);
+  static const cudaError_t allowed = cudaFuncSetAttribute(k_grouped<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
   APT_CUDA(allowed);
   // over half of an SM's shared memory, so that no two blocks share one: each takes all of its tensor memory
-  APT_FOLLOW((k_grouped<T, MODE>), std::min<int64_t>(items, kNumSMs), Tr::kThreads, std::max(bytes, kStageBytes / 2 + 1024), s, a, b, c);
+  APT_FOLLOW((k_grouped<T, MODE>), std::min<int64_t>(items, kNumSMs), Tr::kThreads, std::max(bytes, 116 * 1024), s, a, b, c);
   return APT_OK;
 }
 
@@ -728,8 +767,19 @@ static int rows_product(const Operand& rows, const Operand& weight, int64_t num_
   GroupedCall c = {};
   c.offsets = offsets, c.rows = rows.rows, c.groups = groups;
   c.num_n = (int)num_n, c.num_k = (int)rows.columns;
-  c.tile_n = tile_columns(num_n, Tr::kMostN), c.tiles_n = (int)ceil_div(num_n, c.tile_n);
+  // Tiles of 128 rows, or as many as a mean group has twice over, are made smaller until every SM has one (four where rows are few, whose
+  // time is that of reading the weights), down to 16 rows and 64 columns. The products are of 128 rows always: rows that are not copied are
+  // not written either, so that only copies and conversions get fewer.
+  int64_t most = Tr::kMostN;
+  const auto tiles = [&] { return (ceil_div(rows.rows, c.tile_m) + std::min<int64_t>(groups, rows.rows) / 2) * ceil_div(num_n, most); };
   c.tile_m = kTileM;
+  while (c.tile_m > 16 && c.tile_m >= 2 * ceil_div(rows.rows, groups)) c.tile_m /= 2;
+  const int64_t enough = c.tile_m < 64 ? 4 * kNumSMs : kNumSMs;
+  while (tiles() < enough && (most > 64 || c.tile_m > 16)) {
+    if (most > 64 && (most >= 2 * c.tile_m || c.tile_m == 16)) most /= 2;
+    else c.tile_m /= 2;
+  }
+  c.tile_n = tile_columns(num_n, (int)most), c.tiles_n = (int)ceil_div(num_n, c.tile_n);
   c.a = rows.data, c.b = weight.data, c.pitch_a = rows.pitch, c.pitch_b = weight.pitch;
   c.bias = bias, c.out = out, c.status = status;
   CUtensorMap a, b;
@@ -752,7 +802,7 @@ static size_t linear_room(int64_t rows, int64_t dim, int64_t out_dim, int64_t gr
   size_t bytes = room_of(rows, dim, sizeof(T)) + room_of(groups * out_dim, dim, sizeof(T));
   if (backward) {
     const WeightPlan p = weight_plan<T>(rows, dim, out_dim, groups);
-    bytes += room_of(rows, out_dim, sizeof(T)) + align_up((size_t)(groups + 1) * 8, 256) + (size_t)p.pieces * kTileM * (p.tile_n + 1) * 4;
+    bytes += room_of(rows, out_dim, sizeof(T)) + align_up((size_t)(2 + 3 * p.ranges) * 8, 256) + (size_t)p.pieces * kTileM * (p.tile_n + 1) * 4;
   }
   return bytes;
 }
@@ -789,14 +839,16 @@ static int linear_backward(const void* x, int64_t rows, int64_t dim, const void*
     c.a = dy.data, c.b = in.data, c.pitch_a = dy.pitch, c.pitch_b = in.pitch;
     c.out = grad_weight, c.grad_bias = grad_bias, c.status = status;
     c.plan = (int64_t*)room;
-    c.partial = (float*)(room + align_up((size_t)(groups + 1) * 8, 256));
+    c.partial = (float*)(room + align_up((size_t)(2 + 3 * p.ranges) * 8, 256));
     c.partial_bias = c.partial + (size_t)p.pieces * kTileM * p.tile_n;
     CUtensorMap a, b;
     if (const int e = make_map(&a, code_of<T>(), dy, Tr::kBox, Tr::kBlock)) return e;
     if (const int e = make_map(&b, code_of<T>(), in, Tr::kBox, Tr::kBlock)) return e;
     if (const int e = launch_grouped<T, kGradW>(c, a, b, p.ranges, s)) return e;
-    const int64_t threads = (int64_t)groups * out_dim * (ceil_div(dim, 4) + (grad_bias ? 1 : 0));
-    APT_FOLLOW((k_join_weights<T, Tr::kBlock>), wave_grid(ceil_div(threads, 256), 8), 256, 0, s, c);
+    if (p.ranges > 1) {
+      const dim3 grid((unsigned)ceil_div((int64_t)kTileM * c.tile_n / 4, 256), (unsigned)(p.ranges - 1));
+      APT_FOLLOW((k_join_weights<T>), grid, 256, 0, s, c);
+    }
   }
   return APT_OK;
 }

@@ -54,6 +54,7 @@ struct GroupedCall {
   int num_m, num_n, num_k;      // num_m: rows of dw, num_k: contraction of out and dx
   int tile_m, tile_n, tiles_m, tiles_n;
   int copied_stages, piece_stages;
+  int keep;                     // out and dx: a group's weights stay in shared memory while a block has tiles of it
   int64_t ranges;               // dw: into how many runs of stages the work is cut at most
   const void *a, *b;            // the operands, as the copies read them
   int64_t pitch_a, pitch_b;     // elements
@@ -92,19 +93,21 @@ template <typename T, int MODE>
 struct GroupedWalk {
   using Tr = GroupedTraits<T, MODE>;
   const GroupedCall& c;
-  const int* prefix;            // tiles (stages in dw) of the groups before
+  const int *prefix, *begin;    // of each group: tiles (stages in dw) of those before, first row
   int64_t next, end, step;
   GroupedRuns runs;
-  __device__ GroupedWalk(const GroupedCall& call, const int* p) : c(call), prefix(p) {
+  __device__ GroupedWalk(const GroupedCall& call, const int* p, const int* rows) : c(call), prefix(p), begin(rows) {
     if constexpr (MODE == kGradW) {
       runs = grouped_runs((int64_t)prefix[c.groups] * c.tiles_m * c.tiles_n, c.ranges);
       step = blockIdx.x;
       next = end = 0;
       if (runs.units && step < runs.runs) next = runs.begin(step), end = runs.begin(step + 1);
     } else {
-      next = blockIdx.x, step = gridDim.x, end = (int64_t)prefix[c.groups + 1] * c.tiles_n;
+      const int64_t all = (int64_t)prefix[c.groups + 1] * c.tiles_n;
+      next = c.keep ? blockIdx.x * all / gridDim.x : blockIdx.x, step = c.keep ? 1 : gridDim.x, end = c.keep ? (blockIdx.x + 1) * all / gridDim.x : all;
     }
   }
+  static __device__ __forceinline__ int64_t quotient(int64_t a, int b) { return a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }
   __device__ __forceinline__ int group_of(int t, int n) const {
     int lo = 0, hi = n;         // the last group whose prefix is at most t
     while (hi - lo > 1) {
@@ -121,13 +124,12 @@ struct GroupedWalk {
         next = runs.begin(step), end = runs.begin(step + 1);
       }
       const int total = prefix[c.groups];
-      const int tile = (int)(next / total), t = (int)(next % total);
+      const int tile = (int)quotient(next, total), t = (int)(next - (int64_t)tile * total);
       const int g = group_of(t, c.groups);
       const int64_t n = min(end - next, (int64_t)(prefix[g + 1] - t));
-      const RowRange r = group_rows(c.offsets, g, c.rows);
       item->g = g;
-      item->row = r.begin + (int64_t)(t - prefix[g]) * Tr::kBlock;
-      item->rows = (int)min(n * Tr::kBlock, r.end - item->row);
+      item->row = begin[g] + (int64_t)(t - prefix[g]) * Tr::kBlock;
+      item->rows = (int)min(n * Tr::kBlock, begin[g + 1] - item->row);
       item->stages = (int)n;
       item->m0 = tile / c.tiles_n * kTileM;
       item->n0 = tile % c.tiles_n * c.tile_n;
@@ -138,16 +140,19 @@ struct GroupedWalk {
       return true;
     } else {
       if (next >= end) return false;
-      const int t = (int)(next / c.tiles_n);
+      int t = (int)quotient(next, c.tiles_n);
       const int g = group_of(t, c.groups + 1);
-      RowRange r;
-      if (g < c.groups) r = group_rows(c.offsets, g, c.rows);
-      else r.begin = min(max(c.offsets[c.groups], (int64_t)0), c.rows), r.end = c.rows;
+      int n = (int)(next - (int64_t)t * c.tiles_n);
+      if (c.keep) {      // a group's tiles column by column, not row by row
+        const int here = prefix[g + 1] - prefix[g];
+        const int64_t at = next - (int64_t)prefix[g] * c.tiles_n;
+        n = (int)quotient(at, here), t = prefix[g] + (int)(at - (int64_t)n * here);
+      }
       item->g = g;
-      item->row = r.begin + (int64_t)(t - prefix[g]) * c.tile_m;
-      item->rows = (int)min((int64_t)c.tile_m, r.end - item->row);
+      item->row = begin[g] + (int64_t)(t - prefix[g]) * c.tile_m;
+      item->rows = (int)min((int64_t)c.tile_m, begin[g + 1] - item->row);
       item->m0 = 0;
-      item->n0 = (int)(next % c.tiles_n) * c.tile_n;
+      item->n0 = n * c.tile_n;
       item->stages = g < c.groups ? (c.num_k + Tr::kBlock - 1) / Tr::kBlock : 0;      // rows of no group: zeros
       item->piece = -1, item->run = -1, item->first = item->last = 0;
       next += step;
@@ -316,32 +321,38 @@ __global__ void __launch_bounds__(GroupedTraits<T, MODE>::kThreads, 1)
 k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GroupedCall c) {
   using Tr = GroupedTraits<T, MODE>;
   constexpr int kBuffers = MODE == kGradW ? 1 : 2;
+  constexpr bool kMends = MODE == kGradW && !Tr::kSplit;
   extern __shared__ char raw_shared[];
-  __shared__ uint64_t full[kMaxStages], free_[kMaxStages], ready[kMaxStages], used[kMaxStages], acc_full[2], acc_free[2], drained;
+  __shared__ uint64_t full[kMaxStages], free_[kMaxStages], ready[kMaxStages], used[kMaxStages], acc_full[2], acc_free[2], kept_full, kept_free, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up_word, scan[33];
   volatile int* const gave_up = &gave_up_word;
   char* const shared = (char*)(((uintptr_t)raw_shared + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-  const int copied_a = Tr::copied(kTileM, Tr::kMnA), copied_bytes = copied_a + Tr::copied(c.tile_n, Tr::kMnB);
+  const bool keep = MODE != kGradW && c.keep;
+  const int copied_a = Tr::copied(kTileM, Tr::kMnA), copied_b = Tr::copied(c.tile_n, Tr::kMnB), copied_bytes = copied_a + (keep ? 0 : copied_b);
   const int piece_a = Tr::piece(kTileM, Tr::kMnA), piece_b = Tr::piece(c.tile_n, Tr::kMnB);
-  const int piece_bytes = Tr::kSplit ? 3 * (piece_a + piece_b) : 0;
+  const int piece_bytes = Tr::kSplit ? 3 * (piece_a + (keep ? 0 : piece_b)) : 0;
+  const int kept_stages = keep ? (c.num_k + Tr::kBlock - 1) / Tr::kBlock : 0, kept_bytes = Tr::kSplit ? 3 * piece_b : copied_b;
   char* const copied = shared;
   char* const pieces = copied + (size_t)c.copied_stages * copied_bytes;
-  char* const staging = pieces + (size_t)c.piece_stages * piece_bytes;
+  char* const kept = pieces + (size_t)c.piece_stages * piece_bytes;
+  char* const staging = kept + (size_t)kept_stages * kept_bytes;
   char* const ones = staging + Tr::kOutWarps * 4096;      // (the bias of a tile in out)
-  int* const prefix = (int*)(ones + (MODE == kGradW ? 512 : 1024));
+  int *const prefix = (int*)(ones + (MODE == kGradW ? 512 : 1024)), *const begin = prefix + c.groups + 2;
 
   if (warp == 1) tmem_alloc(shared_addr(&tmem_slot), 512);
   if (threadIdx.x == 0) {
     for (int k = 0; k < kMaxStages; ++k) {
       barrier_init(shared_addr(full + k), 1);
       barrier_init(shared_addr(free_ + k), Tr::kSplit ? 8 : 1);
-      barrier_init(shared_addr(ready + k), 8);
+      barrier_init(shared_addr(ready + k), Tr::kSplit ? 8 : 1);
       barrier_init(shared_addr(used + k), 1);
     }
     for (int k = 0; k < 2; ++k) barrier_init(shared_addr(acc_full + k), 1), barrier_init(shared_addr(acc_free + k), Tr::kOutWarps);
+    barrier_init(shared_addr(&kept_full), Tr::kSplit ? 8 : 1);
+    barrier_init(shared_addr(&kept_free), 1);
     barrier_init(shared_addr(&drained), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     gave_up_word = 0;
@@ -369,28 +380,54 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     }
     int total;
     const int at = before + block_exclusive_scan(n, scan, &total);
-    if (g < lists) prefix[g] = at;
+    if (g < lists) prefix[g] = at, begin[g] = (int)min(max(c.offsets[g], (int64_t)0), c.rows);
     before += total;
   }
-  if (threadIdx.x == 0) prefix[lists] = before;
+  // (where the ends are ends, a group's rows end where the next one's begin)
+  if (threadIdx.x == 0) prefix[lists] = before, begin[lists] = MODE == kGradW ? (int)min(max(c.offsets[c.groups], (int64_t)0), c.rows) : (int)c.rows;
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
-  GroupedWalk<T, MODE> walk(c, prefix);
+  GroupedWalk<T, MODE> walk(c, prefix, begin);
   if (MODE == kGradW && blockIdx.x == 0 && threadIdx.x == 0) c.plan[0] = walk.runs.units, c.plan[1] = walk.runs.runs;
   GroupedItem item;
   bool fine = true;
   if (warp == 0) {
     // ---- copies
-    if (lane == 0) {
-      int stage = 0, loaded = 0;
+    if (one_of_warp()) {
+      int stage = 0, loaded = 0, kept_g = -1, kept_n = -1, kept_times = 0;
       uint32_t phase = 0;
       while (fine && walk.take(&item)) {
         const int boxes_a = MODE == kGradW ? (min(kTileM, c.num_m - item.m0) + Tr::kBox - 1) / Tr::kBox : 1;
         const int boxes_b = Tr::kMnB ? (min(c.tile_n, c.num_n - item.n0) + Tr::kBox - 1) / Tr::kBox : 1;
         constexpr int kBoxBytes = Tr::kBlock * 128;
-        const uint32_t bytes = (MODE == kGradW ? boxes_a * kBoxBytes : c.tile_m * 128) + (Tr::kMnB ? boxes_b * kBoxBytes : c.tile_n * 128);
+        const uint32_t bytes_b = Tr::kMnB ? boxes_b * kBoxBytes : c.tile_n * 128;
+        const uint32_t bytes = (MODE == kGradW ? boxes_a * kBoxBytes : c.tile_m * 128) + (keep ? 0 : bytes_b);
+        const auto copy_weights = [&](uint32_t b, int k, uint32_t bar) {
+          if constexpr (MODE == kOut) {
+            copy_box(b, &map_b, k * Tr::kBlock, item.n0, item.g, bar);
+          } else {
+            for (int i = 0; i < boxes_b; ++i) copy_box(b + i * kBoxBytes, &map_b, item.n0 + i * Tr::kBox, k * Tr::kBlock, item.g, bar);
+          }
+        };
+        if (keep && item.stages && (item.g != kept_g || item.n0 != kept_n)) {
+          kept_g = item.g, kept_n = item.n0;
+          if constexpr (Tr::kSplit) {      // by the ring, to be taken apart
+            for (int k = 0; k < kept_stages; ++k) {
+              if (!(fine = barrier_wait(shared_addr(free_ + stage), phase ^ 1, gave_up))) break;
+              barrier_expect(shared_addr(full + stage), bytes_b);
+              copy_weights(shared_addr(copied + (size_t)stage * copied_bytes), k, shared_addr(full + stage));
+              ++loaded;
+              if (++stage == c.copied_stages) stage = 0, phase ^= 1;
+            }
+          } else if ((fine = barrier_wait(shared_addr(&kept_free), (kept_times & 1) ^ 1, gave_up))) {
+            barrier_expect(shared_addr(&kept_full), bytes_b * kept_stages);
+            for (int k = 0; k < kept_stages; ++k) copy_weights(shared_addr(kept + (size_t)k * kept_bytes), k, shared_addr(&kept_full));
+            ++kept_times;
+          }
+          if (!fine) break;
+        }
         for (int k = 0; k < item.stages; ++k) {
           if (!(fine = barrier_wait(shared_addr(free_ + stage), phase ^ 1, gave_up))) break;
           const uint32_t bar = shared_addr(full + stage), a = shared_addr(copied + (size_t)stage * copied_bytes), b = a + copied_a;
@@ -401,11 +438,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             for (int i = 0; i < boxes_b; ++i) copy_box(b + i * kBoxBytes, &map_b, item.n0 + i * Tr::kBox, row, bar);
           } else {
             copy_box(a, &map_a, k * Tr::kBlock, (int)item.row, bar);
-            if constexpr (MODE == kOut) {
-              copy_box(b, &map_b, k * Tr::kBlock, item.n0, item.g, bar);
-            } else {
-              for (int i = 0; i < boxes_b; ++i) copy_box(b + i * kBoxBytes, &map_b, item.n0 + i * Tr::kBox, k * Tr::kBlock, item.g, bar);
-            }
+            if (!keep) copy_weights(b, k, bar);
           }
           ++loaded;
           if (++stage == c.copied_stages) stage = 0, phase ^= 1;
@@ -416,47 +449,48 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         int nobody = 0;
         for (int k = max(0, loaded - c.copied_stages); k < loaded; ++k)
           barrier_wait(shared_addr(full + k % c.copied_stages), (k / c.copied_stages) & 1, &nobody);
+        if (kept_times) barrier_wait(shared_addr(&kept_full), (kept_times - 1) & 1, &nobody);
       }
     }
   } else if (warp == 1) {
     // ---- products
-    const int stages = Tr::kSplit ? c.piece_stages : c.copied_stages;
-    const uint32_t what = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, Tr::kMnB, kTileM, c.tile_n);
-    const uint32_t what_bias = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, false, kTileM, 16);
-    const uint64_t ones_tile = tile_descriptor(shared_addr(ones), 128, 256, 0);      // 16 x 16 in core matrices of 8 x 16 bytes
-    int stage = 0, tiles = 0;
-    uint32_t phase = 0;
-    while (fine && walk.take(&item)) {
-      if (!item.stages) continue;
-      const int buffer = tiles % kBuffers;
-      fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_free + buffer), ((tiles / kBuffers) & 1) ^ 1, gave_up));
-      if (!fine) break;
-      tmem_fence_after();
-      const uint32_t acc = tmem + buffer * kAccColumns;
-      const bool sums = MODE == kGradW && c.grad_bias && item.n0 == 0;
-      for (int k = 0; k < item.stages; ++k) {
-        uint64_t* const in = Tr::kSplit ? ready : full;
-        if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(in + stage), phase, gave_up)))) break;
-        tmem_fence_after();
-        const int left = (MODE == kGradW ? item.rows : c.num_k) - k * Tr::kBlock, valid = min(left, Tr::kBlock), steps = (valid + 15) / 16;
-        char* const base = Tr::kSplit ? pieces + (size_t)stage * piece_bytes : copied + (size_t)stage * copied_bytes;
-        if constexpr (MODE == kGradW && !Tr::kSplit) {
-          // rows of the next group
-          if (valid % 16) {
-            const int slices = (steps * 16 - valid) * 8, blocks = copied_bytes / 8192;
-            for (int i = lane; i < slices * blocks; i += 32)
-              *(uint4*)(base + i / slices * 8192 + valid * 128 + i % slices * 16) = make_uint4(0u, 0u, 0u, 0u);
-            fence_for_tensor_cores();
-            __syncwarp();
-          }
+    if (one_of_warp()) {
+      const int stages = Tr::kSplit ? c.piece_stages : c.copied_stages;
+      const uint32_t what = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, Tr::kMnB, kTileM, c.tile_n);
+      const uint32_t what_bias = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, false, kTileM, 16);
+      const uint64_t ones_tile = tile_descriptor(shared_addr(ones), 128, 256, 0);      // 16 x 16 in core matrices of 8 x 16 bytes
+      int stage = 0, tiles = 0, kept_g = -1, kept_n = -1, kept_times = 0;
+      uint32_t phase = 0, mended = 0;
+      while (fine && walk.take(&item)) {
+        if (!item.stages) continue;
+        const int buffer = tiles % kBuffers;
+        if (!(fine = barrier_wait(shared_addr(acc_free + buffer), ((tiles / kBuffers) & 1) ^ 1, gave_up))) break;
+        if (keep && (item.g != kept_g || item.n0 != kept_n)) {
+          kept_g = item.g, kept_n = item.n0;
+          if (kept_times) products_done(shared_addr(&kept_free));
+          if (!(fine = barrier_wait(shared_addr(&kept_full), kept_times & 1, gave_up))) break;
+          ++kept_times;
         }
-        if (lane == 0) {
-          const uint32_t a = shared_addr(base), b = a + (Tr::kSplit ? 3 * piece_a : copied_a);
+        const uint32_t acc = tmem + buffer * kAccColumns;
+        const bool sums = MODE == kGradW && c.grad_bias && item.n0 == 0;
+        for (int k = 0; k < item.stages; ++k) {
+          if (!(fine = barrier_wait(shared_addr((Tr::kSplit ? ready : full) + stage), phase, gave_up))) break;
+          const int left = (MODE == kGradW ? item.rows : c.num_k) - k * Tr::kBlock, steps = (min(left, Tr::kBlock) + 15) / 16;
+          if (kMends && left < Tr::kBlock && left % 16) {
+            barrier_arrive(shared_addr(ready));
+            if (!(fine = barrier_wait(shared_addr(ready + 1), mended, gave_up))) break;
+            mended ^= 1;
+          }
+          tmem_fence_after();
+          const uint32_t a = shared_addr(Tr::kSplit ? pieces + (size_t)stage * piece_bytes : copied + (size_t)stage * copied_bytes);
+          const uint32_t b = keep ? shared_addr(kept + (size_t)k * kept_bytes) : a + (Tr::kSplit ? 3 * piece_a : copied_a);
           const uint64_t tile_a = Tr::kMnA ? tile_descriptor(a, Tr::kBlock * 128, 1024, kSwizzle128)
                                            : tile_descriptor(a, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
           const uint64_t tile_b = Tr::kMnB ? tile_descriptor(b, Tr::kBlock * 128, 1024, kSwizzle128)
                                            : tile_descriptor(b, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
-          for (int s = 0; s < steps; ++s) {
+#pragma unroll
+          for (int s = 0; s < Tr::kBlock / 16; ++s) {
+            if (s >= steps) break;
             const uint64_t da = tile_a + s * ((Tr::kMnA ? 2048 : 32) >> 4), db = tile_b + s * ((Tr::kMnB ? 2048 : 32) >> 4);
             const bool add = k > 0 || s > 0;
             tile_product(acc, da, db, what, add);
@@ -470,21 +504,40 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               tile_product(small, da + 2 * pa, db, what, true);
             }
             if (sums)
+#pragma unroll
               for (int p = 0; p < Tr::kPieces; ++p)
                 tile_product(tmem + kAccColumns + (p ? 16 : 0), da + p * (piece_a >> 4), ones_tile, what_bias, add || p > 1);
           }
           products_done(shared_addr((Tr::kSplit ? used : free_) + stage));
           if (k == item.stages - 1) products_done(shared_addr(acc_full + buffer));
+          if (++stage == stages) stage = 0, phase ^= 1;
         }
-        __syncwarp();
-        if (++stage == stages) stage = 0, phase ^= 1;
+        ++tiles;
       }
-      ++tiles;
+      if (*gave_up) {
+        int nobody = 0;
+        products_done(shared_addr(&drained));
+        barrier_wait(shared_addr(&drained), 0, &nobody);
+      }
     }
-    if (*gave_up && lane == 0) {
-      int nobody = 0;
-      products_done(shared_addr(&drained));
-      barrier_wait(shared_addr(&drained), 0, &nobody);
+  } else if (kMends && warp == 2) {
+    // ---- rows of the next group in the last stage of a sum: zeros, in both operands, when the products get there and ask for it (ready[0], answered by
+    // ready[1]: both sides count the same stages)
+    int64_t before_item = 0;
+    uint32_t mended = 0;
+    while (fine && walk.take(&item)) {
+      const int64_t last = before_item + item.stages - 1;
+      before_item += item.stages;
+      if (item.rows % 16 == 0) continue;
+      const int stage = (int)(last % c.copied_stages), valid = item.rows - (item.stages - 1) * Tr::kBlock;
+      if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(ready), mended, gave_up)))) break;
+      mended ^= 1;
+      char* const base = copied + (size_t)stage * copied_bytes;
+      const int slices = ((valid + 15) / 16 * 16 - valid) * 8, blocks = copied_bytes / 8192;
+      for (int i = lane; i < slices * blocks; i += 32) *(uint4*)(base + i / slices * 8192 + valid * 128 + i % slices * 16) = make_uint4(0u, 0u, 0u, 0u);
+      fence_for_tensor_cores();
+      __syncwarp();
+      if (lane == 0) barrier_arrive(shared_addr(ready + 1));
     }
   } else if (warp >= 4 && warp < 4 + Tr::kOutWarps) {
     // ---- finished tiles
@@ -549,11 +602,11 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         ++tiles;
       }
     }
-  } else if (MODE == kGradW && warp < 4) {
+  } else if (MODE == kGradW && warp == 3) {
     // ---- groups without rows
     const int64_t per = (int64_t)c.num_m * c.num_n;
     const bool slices = per * sizeof(T) % 16 == 0;
-    const int64_t from = (int64_t)blockIdx.x * 64 + threadIdx.x - 64, by = (int64_t)gridDim.x * 64;
+    const int64_t from = (int64_t)blockIdx.x * 32 + lane, by = (int64_t)gridDim.x * 32;
     for (int g = 0; g < c.groups; ++g) {
       if (prefix[g + 1] > prefix[g]) continue;
       T* const out = (T*)c.out + g * per;
@@ -567,18 +620,33 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   } else if (Tr::kSplit && warp >= 8) {
     // ---- fp32 taken apart
     const int thread = threadIdx.x - 256;
-    int from = 0, to = 0;
+    int from = 0, to = 0, kept_g = -1, kept_n = -1, kept_times = 0;
     uint32_t from_phase = 0, to_phase = 0;
     while (fine && walk.take(&item)) {
+      if (keep && item.stages && (item.g != kept_g || item.n0 != kept_n)) {
+        kept_g = item.g, kept_n = item.n0;
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(&kept_free), (kept_times & 1) ^ 1, gave_up));
+        ++kept_times;
+        for (int k = 0; fine && k < kept_stages; ++k) {
+          if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up)))) break;
+          take_stage_apart<Tr::kMnB>(copied + (size_t)from * copied_bytes, kept + (size_t)k * kept_bytes, c.tile_n, piece_b, Tr::kBlock, thread);
+          __syncwarp();
+          if (lane == 0) barrier_arrive(shared_addr(free_ + from));
+          if (++from == c.copied_stages) from = 0, from_phase ^= 1;
+        }
+        if (!fine) break;
+        fence_for_tensor_cores();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(shared_addr(&kept_full));
+      }
       for (int k = 0; k < item.stages; ++k) {
-        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up) &&
-                                           barrier_wait(shared_addr(used + to), to_phase ^ 1, gave_up));
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up) && barrier_wait(shared_addr(used + to), to_phase ^ 1, gave_up));
         if (!fine) break;
         const char* const in = copied + (size_t)from * copied_bytes;
         char* const out = pieces + (size_t)to * piece_bytes;
         const int valid = MODE == kGradW ? item.rows - k * Tr::kBlock : Tr::kBlock;
         take_stage_apart<Tr::kMnA>(in, out, MODE == kGradW ? kTileM : c.tile_m, piece_a, valid, thread);
-        take_stage_apart<Tr::kMnB>(in + copied_a, out + 3 * piece_a, c.tile_n, piece_b, MODE == kGradW ? valid : Tr::kBlock, thread);
+        if (!keep) take_stage_apart<Tr::kMnB>(in + copied_a, out + 3 * piece_a, c.tile_n, piece_b, MODE == kGradW ? valid : Tr::kBlock, thread);
         fence_for_tensor_cores();
         __syncwarp();
         if (lane == 0) {
@@ -737,18 +805,21 @@ static WeightPlan weight_plan(int64_t rows, int64_t dim, int64_t out_dim, int64_
 template <typename T, int MODE>
 static int launch_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap& b, int64_t items, cudaStream_t s) {
   using Tr = GroupedTraits<T, MODE>;
-  const int fixed = 1024 + Tr::kOutWarps * 4096 + (MODE == kGradW ? 512 : 1024) + (int)align_up((size_t)(c.groups + 2) * 4, 16);
-  const int copied = Tr::copied(kTileM, Tr::kMnA) + Tr::copied(c.tile_n, Tr::kMnB);
-  const int pieces = Tr::kSplit ? 3 * (Tr::piece(kTileM, Tr::kMnA) + Tr::piece(c.tile_n, Tr::kMnB)) : 0;
+  const int fixed = 1024 + Tr::kOutWarps * 4096 + (MODE == kGradW ? 512 : 1024) + (int)align_up((size_t)(c.groups + 2) * 8, 16);
   const int room = kMostShared - fixed;
-  if (Tr::kSplit) {
-    c.piece_stages = 2;
-    c.copied_stages = std::min(kMaxStages, (room - 2 * pieces) / copied);
-  } else {
-    c.piece_stages = 0;
-    c.copied_stages = std::min(kMaxStages, room / copied);
+  int copied = Tr::copied(kTileM, Tr::kMnA), pieces = Tr::kSplit ? 3 * Tr::piece(kTileM, Tr::kMnA) : 0, kept = 0;
+  const int copied_b = Tr::copied(c.tile_n, Tr::kMnB), pieces_b = Tr::kSplit ? 3 * Tr::piece(c.tile_n, Tr::kMnB) : 0;
+  // Weights are kept where they leave room for four stages of rows and a block has several tiles of them: what the copies bring from L2, which
+  // gives 10 to 12 TB/s, is then the rows alone.
+  if (MODE != kGradW) {
+    const int64_t bytes = ceil_div(c.num_k, Tr::kBlock) * (Tr::kSplit ? pieces_b : copied_b), least = Tr::kSplit ? 2 * pieces + 3 * copied : 4 * copied;
+    c.keep = bytes + least <= room && items >= 3 * kNumSMs && items >= 3 * (int64_t)c.groups * c.tiles_n;
+    if (c.keep) kept = (int)bytes;
   }
-  const int bytes = fixed + c.copied_stages * copied + c.piece_stages * pieces;
+  if (!c.keep) copied += copied_b, pieces += pieces_b;
+  c.piece_stages = Tr::kSplit ? 2 : 0;
+  c.copied_stages = std::min(kMaxStages, (room - kept - c.piece_stages * pieces) / copied);
+  const int bytes = fixed + kept + c.copied_stages * copied + c.piece_stages * pieces;
   static const cudaError_t allowed = cudaFuncSetAttribute(k_grouped<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
   APT_CUDA(allowed);
   // over half of an SM's shared memory, so that no two blocks share one: each takes all of its tensor memory

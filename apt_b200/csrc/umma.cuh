@@ -37,6 +37,22 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
   return false;
 }
 
+// The same for a warp, by its first lane: every poll is an operation on shared memory of each lane that makes it, and warps that
+// wait for a tile would slow down those that work on it.
+__device__ __forceinline__ bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+  int fine = 1;
+  if (threadIdx.x % 32 == 0) fine = barrier_wait(bar, parity, gave_up);
+  return __shfl_sync(0xffffffffu, fine, 0);
+}
+
+// True for one lane of a converged warp, which the compiler knows to be one: products and copies, which take their operands in uniform
+// registers, are issued as they are then. Under a condition on the lane's number a product took 140 cycles to issue.
+__device__ __forceinline__ bool one_of_warp() {
+  uint32_t is;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(is));
+  return is;
+}
+
 // Boxes of a row-major matrix, or of a stack of them, on their way to shared memory; `bar` counts their bytes.
 __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),

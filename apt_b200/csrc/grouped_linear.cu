@@ -95,6 +95,7 @@ struct GroupedWalk {
   const GroupedCall& c;
   const int *prefix, *begin;    // of each group: tiles (stages in dw) of those before, first row
   int64_t next, end, step;
+  int last_g = 0, last_n = 0, last_t = -2;      // of the tile before
   GroupedRuns runs;
   __device__ GroupedWalk(const GroupedCall& call, const int* p, const int* rows) : c(call), prefix(p), begin(rows) {
     if constexpr (MODE == kGradW) {
@@ -140,14 +141,20 @@ struct GroupedWalk {
       return true;
     } else {
       if (next >= end) return false;
-      int t = (int)quotient(next, c.tiles_n);
-      const int g = group_of(t, c.groups + 1);
-      int n = (int)(next - (int64_t)t * c.tiles_n);
-      if (c.keep) {      // a group's tiles column by column, not row by row
-        const int here = prefix[g + 1] - prefix[g];
-        const int64_t at = next - (int64_t)prefix[g] * c.tiles_n;
-        n = (int)quotient(at, here), t = prefix[g] + (int)(at - (int64_t)n * here);
+      int t, n, g;
+      if (c.keep && last_t >= 0 && last_t + 1 < prefix[last_g + 1]) {      // the next rows of the same weights
+        t = last_t + 1, n = last_n, g = last_g;
+      } else {
+        t = c.tiles_n == 1 ? (int)next : (int)quotient(next, c.tiles_n);
+        g = t < prefix[last_g + 1] && !c.keep ? last_g : group_of(t, c.groups + 1);
+        n = (int)(next - (int64_t)t * c.tiles_n);
+        if (c.keep) {      // a group's tiles column by column, not row by row
+          const int here = prefix[g + 1] - prefix[g];
+          const int64_t at = next - (int64_t)prefix[g] * c.tiles_n;
+          n = (int)quotient(at, here), t = prefix[g] + (int)(at - (int64_t)n * here);
+        }
       }
+      last_t = t, last_n = n, last_g = g;
       item->g = g;
       item->row = begin[g] + (int64_t)(t - prefix[g]) * c.tile_m;
       item->rows = (int)min((int64_t)c.tile_m, begin[g + 1] - item->row);
@@ -177,30 +184,43 @@ __device__ __forceinline__ Pieces take_apart(float4 a, float4 b) {
   }
   return r;
 }
-// One operand's stage. Its rows (of 128 bytes as copied) run along the contraction, 8 elements of a row a thread, or across it in
-// boxes of 32: 8 elements of one k a thread. `valid`: k's from there on are zero.
+// One operand's stage by a team of 128 threads. Its rows (of 128 bytes as copied) run along the contraction, 8 elements of a row a thread, or
+// across it in boxes of 32: 8 elements of one k a thread. `valid`: k's from there on are zero. Four at a time are read before any is written.
+constexpr int kApartTeam = 128;
 template <bool MN>
 __device__ __forceinline__ void take_stage_apart(const char* copied, char* pieces, int n, int piece_bytes, int valid, int thread) {
-  if constexpr (!MN) {
-    for (int i = thread; i < n * 4; i += 256) {
-      const int r = i >> 2, s = i & 3;
-      const char* const row = copied + r * 128;
-      const Pieces v = take_apart(*(const float4*)(row + (((2 * s) ^ (r & 7)) << 4)), *(const float4*)(row + (((2 * s + 1) ^ (r & 7)) << 4)));
-      char* const to = pieces + r * 64 + ((s ^ ((r >> 1) & 3)) << 4);
+  const int all = MN ? (n + 63) / 64 * 256 : n * 4;
+  for (int i0 = thread; i0 < all; i0 += 4 * kApartTeam) {
+    float4 lo[4], hi[4];
 #pragma unroll
-      for (int p = 0; p < 3; ++p) *(uint4*)(to + p * piece_bytes) = v.p[p];
-    }
-  } else {
-    for (int i = thread; i < (n + 63) / 64 * 256; i += 256) {
-      const int s = i & 3, k = (i >> 2) & 31, half = (i >> 7) & 1, block = i >> 8;
-      const char* const row = copied + (block * 2 + half) * 4096 + k * 128;
-      float4 lo = make_float4(0.0f, 0.0f, 0.0f, 0.0f), hi = lo;
-      if (k < valid && block * 64 + half * 32 < (n + 31) / 32 * 32) {
-        lo = *(const float4*)(row + (((2 * s) ^ (k & 7)) << 4));
-        hi = *(const float4*)(row + (((2 * s + 1) ^ (k & 7)) << 4));
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * kApartTeam;
+      lo[u] = hi[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i >= all) continue;
+      if constexpr (!MN) {
+        const int r = i >> 2, s = i & 3;
+        const char* const row = copied + r * 128;
+        lo[u] = *(const float4*)(row + (((2 * s) ^ (r & 7)) << 4)), hi[u] = *(const float4*)(row + (((2 * s + 1) ^ (r & 7)) << 4));
+      } else {
+        const int s = i & 3, k = (i >> 2) & 31, half = (i >> 7) & 1, block = i >> 8;
+        const char* const row = copied + (block * 2 + half) * 4096 + k * 128;
+        if (k < valid && block * 64 + half * 32 < (n + 31) / 32 * 32)
+          lo[u] = *(const float4*)(row + (((2 * s) ^ (k & 7)) << 4)), hi[u] = *(const float4*)(row + (((2 * s + 1) ^ (k & 7)) << 4));
       }
-      const Pieces v = take_apart(lo, hi);
-      char* const to = pieces + block * 4096 + k * 128 + (((half * 4 + s) ^ (k & 7)) << 4);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * kApartTeam;
+      if (i >= all) break;
+      const Pieces v = take_apart(lo[u], hi[u]);
+      char* to;
+      if constexpr (!MN) {
+        const int r = i >> 2, s = i & 3;
+        to = pieces + r * 64 + ((s ^ ((r >> 1) & 3)) << 4);
+      } else {
+        const int s = i & 3, k = (i >> 2) & 31, half = (i >> 7) & 1, block = i >> 8;
+        to = pieces + block * 4096 + k * 128 + (((half * 4 + s) ^ (k & 7)) << 4);
+      }
 #pragma unroll
       for (int p = 0; p < 3; ++p) *(uint4*)(to + p * piece_bytes) = v.p[p];
     }
@@ -236,7 +256,7 @@ __device__ __noinline__ float column_again(const GroupedCall& c, const GroupedIt
 // rows take turns.
 template <typename T, typename O, int MODE>
 __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedItem& item, uint32_t acc, bool empty, char* staging, int lane, int quarter, int turn,
-                                           int turns, O* out, int64_t ld, int rows, int columns, const float* bias) {
+                                           int turns, O* out, int64_t ld, int rows, int columns, const float* bias, uint32_t acc_free) {
   using Tr = GroupedTraits<T, MODE>;
   constexpr int kWide = 128 / (int)sizeof(O), kPer = 16 / (int)sizeof(O);
   const int m = quarter * 32 + lane, here = min(32, rows - quarter * 32);
@@ -269,6 +289,11 @@ __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedIt
         tmem_wait_loads();
 #pragma unroll
         for (int h = 0; h < kWide / 32; ++h) settled(v[h]);
+      }
+      if (acc_free && c0 + turns * kWide >= columns) {      // the tile's sums are read
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(acc_free);
       }
     }
     if (bias)
@@ -346,8 +371,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   if (threadIdx.x == 0) {
     for (int k = 0; k < kMaxStages; ++k) {
       barrier_init(shared_addr(full + k), 1);
-      barrier_init(shared_addr(free_ + k), Tr::kSplit ? 8 : 1);
-      barrier_init(shared_addr(ready + k), Tr::kSplit ? 8 : 1);
+      barrier_init(shared_addr(free_ + k), Tr::kSplit ? 4 : 1);
+      barrier_init(shared_addr(ready + k), Tr::kSplit ? 4 : 1);
       barrier_init(shared_addr(used + k), 1);
     }
     for (int k = 0; k < 2; ++k) barrier_init(shared_addr(acc_full + k), 1), barrier_init(shared_addr(acc_free + k), Tr::kOutWarps);
@@ -572,10 +597,10 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if (quarter * 32 < rows) {
           if (item.piece < 0)
             store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0,
-                                   (int64_t)c.num_n, rows, columns, nullptr);
+                                   (int64_t)c.num_n, rows, columns, nullptr, 0u);
           else
             store_tile<T, float, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows,
-                                       columns, nullptr);
+                                       columns, nullptr, 0u);
           if (c.grad_bias && item.n0 == 0 && turn == 0) {
             const uint32_t at = tmem + kAccColumns + ((uint32_t)quarter << 21);
             float v = tmem_load_1(at), small = Tr::kSplit ? tmem_load_1(at + 16) : 0.0f;
@@ -591,14 +616,17 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             }
           }
         }
-      } else if (quarter * 32 < item.rows) {
-        store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + item.row * c.num_n + item.n0, (int64_t)c.num_n, item.rows, columns,
-                               MODE == kOut && c.bias && !empty ? bias : nullptr);
       }
+      const bool stores = MODE != kGradW && quarter * 32 < item.rows && turn * (128 / (int)sizeof(T)) < columns;
+      if (stores)
+        store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + item.row * c.num_n + item.n0, (int64_t)c.num_n, item.rows, columns,
+                               MODE == kOut && c.bias && !empty ? bias : nullptr, shared_addr(acc_free + buffer));
       if (!empty) {
-        tmem_fence_before();
-        __syncwarp();
-        if (lane == 0) barrier_arrive(shared_addr(acc_free + buffer));
+        if (!stores) {
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) barrier_arrive(shared_addr(acc_free + buffer));
+        }
         ++tiles;
       }
     }
@@ -618,32 +646,36 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         for (int64_t i = from; i < c.num_m; i += by) ((T*)c.grad_bias)[(int64_t)g * c.num_m + i] = Elem<T>::from_f(0.0f);
     }
   } else if (Tr::kSplit && warp >= 8) {
-    // ---- fp32 taken apart
-    const int thread = threadIdx.x - 256;
-    int from = 0, to = 0, kept_g = -1, kept_n = -1, kept_times = 0;
+    // ---- fp32 taken apart, by two teams in turn: one's waits and fence are the other's work
+    const int team = (warp - 8) / 4, thread = (threadIdx.x - 256) % kApartTeam;
+    int from = 0, kept_g = -1, kept_n = -1, kept_times = 0, turn = 0;
     uint32_t from_phase = 0, to_phase = 0;
+    const auto next_from = [&] {
+      if (++from == c.copied_stages) from = 0, from_phase ^= 1;
+    };
     while (fine && walk.take(&item)) {
       if (keep && item.stages && (item.g != kept_g || item.n0 != kept_n)) {
         kept_g = item.g, kept_n = item.n0;
         fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(&kept_free), (kept_times & 1) ^ 1, gave_up));
         ++kept_times;
-        for (int k = 0; fine && k < kept_stages; ++k) {
+        for (int k = 0; fine && k < kept_stages; ++k, next_from()) {
+          if ((k & 1) != team) continue;
           if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up)))) break;
           take_stage_apart<Tr::kMnB>(copied + (size_t)from * copied_bytes, kept + (size_t)k * kept_bytes, c.tile_n, piece_b, Tr::kBlock, thread);
           __syncwarp();
           if (lane == 0) barrier_arrive(shared_addr(free_ + from));
-          if (++from == c.copied_stages) from = 0, from_phase ^= 1;
         }
         if (!fine) break;
         fence_for_tensor_cores();
         __syncwarp();
         if (lane == 0) barrier_arrive(shared_addr(&kept_full));
       }
-      for (int k = 0; k < item.stages; ++k) {
-        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up) && barrier_wait(shared_addr(used + to), to_phase ^ 1, gave_up));
+      for (int k = 0; k < item.stages; ++k, turn ^= 1, next_from()) {
+        if (turn != team) continue;      // each team has a stage of pieces of its own
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up) && barrier_wait(shared_addr(used + team), to_phase ^ 1, gave_up));
         if (!fine) break;
         const char* const in = copied + (size_t)from * copied_bytes;
-        char* const out = pieces + (size_t)to * piece_bytes;
+        char* const out = pieces + (size_t)team * piece_bytes;
         const int valid = MODE == kGradW ? item.rows - k * Tr::kBlock : Tr::kBlock;
         take_stage_apart<Tr::kMnA>(in, out, MODE == kGradW ? kTileM : c.tile_m, piece_a, valid, thread);
         if (!keep) take_stage_apart<Tr::kMnB>(in + copied_a, out + 3 * piece_a, c.tile_n, piece_b, MODE == kGradW ? valid : Tr::kBlock, thread);
@@ -651,10 +683,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         __syncwarp();
         if (lane == 0) {
           barrier_arrive(shared_addr(free_ + from));
-          barrier_arrive(shared_addr(ready + to));
+          barrier_arrive(shared_addr(ready + team));
         }
-        if (++from == c.copied_stages) from = 0, from_phase ^= 1;
-        if (++to == c.piece_stages) to = 0, to_phase ^= 1;
+        to_phase ^= 1;
       }
     }
   }

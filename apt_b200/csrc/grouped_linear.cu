@@ -44,7 +44,7 @@ struct GroupedTraits {
   static constexpr int kPieces = kSplit ? 3 : 1;
   // bytes of a tile of n rows (or columns) in a stage as copied, and of one bf16 piece of it
   static __host__ __device__ constexpr int copied(int n, bool mn) { return mn ? (n + kBox - 1) / kBox * kBlock * 128 : n * 128; }
-  static __host__ __device__ constexpr int piece(int n, bool mn) { return mn ? (n + 63) / 64 * kBlock * 128 : n * kBlock * 2; }
+  static __host__ __device__ constexpr int piece(int n, bool mn) { return mn ? (n + 63) / 64 * kBlock * 128 : (n + 31) / 32 * 32 * kBlock * 2; }
 };
 
 struct GroupedCall {
@@ -185,45 +185,38 @@ __device__ __forceinline__ Pieces take_apart(float4 a, float4 b) {
   return r;
 }
 // One operand's stage by a team of 128 threads. Its rows (of 128 bytes as copied) run along the contraction, 8 elements of a row a thread, or
-// across it in boxes of 32: 8 elements of one k a thread. `valid`: k's from there on are zero. Four at a time are read before any is written.
+// across it in boxes of 32: 8 elements of one k a thread. Everything is a constant of the thread away from the stage's beginning, and
+// nothing is compared: with few warps at work, a stage's time is the latency of its instructions. What lies beyond the operand's rows is taken
+// apart with them (the pieces have room for whole rounds) and never used. `valid`: k's from there on are zero.
 constexpr int kApartTeam = 128;
-template <bool MN>
-__device__ __forceinline__ void take_stage_apart(const char* copied, char* pieces, int n, int piece_bytes, int valid, int thread) {
-  const int all = MN ? (n + 63) / 64 * 256 : n * 4;
-  for (int i0 = thread; i0 < all; i0 += 4 * kApartTeam) {
-    float4 lo[4], hi[4];
+template <bool MN, int U, bool CUT>
+__device__ __forceinline__ void take_rounds_apart(const char* from, char* to, int piece_bytes, bool zero) {
+  float4 lo[U], hi[U];
+  const int thread = threadIdx.x % kApartTeam, s = thread & 3, line = thread >> 2;      // a row, or a k
+  const int at = line * 128, lo_at = at + (((2 * s) ^ (line & 7)) << 4), hi_at = at + (((2 * s + 1) ^ (line & 7)) << 4);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u * kApartTeam;
-      lo[u] = hi[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (i >= all) continue;
-      if constexpr (!MN) {
-        const int r = i >> 2, s = i & 3;
-        const char* const row = copied + r * 128;
-        lo[u] = *(const float4*)(row + (((2 * s) ^ (r & 7)) << 4)), hi[u] = *(const float4*)(row + (((2 * s + 1) ^ (r & 7)) << 4));
-      } else {
-        const int s = i & 3, k = (i >> 2) & 31, half = (i >> 7) & 1, block = i >> 8;
-        const char* const row = copied + (block * 2 + half) * 4096 + k * 128;
-        if (k < valid && block * 64 + half * 32 < (n + 31) / 32 * 32)
-          lo[u] = *(const float4*)(row + (((2 * s) ^ (k & 7)) << 4)), hi[u] = *(const float4*)(row + (((2 * s + 1) ^ (k & 7)) << 4));
-      }
-    }
+  for (int u = 0; u < U; ++u) lo[u] = *(const float4*)(from + lo_at + u * 4096), hi[u] = *(const float4*)(from + hi_at + u * 4096);
+  const int to_at = MN ? line * 128 + ((s ^ (line & 7)) << 4) : line * 64 + ((s ^ ((line >> 1) & 3)) << 4);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u * kApartTeam;
-      if (i >= all) break;
-      const Pieces v = take_apart(lo[u], hi[u]);
-      char* to;
-      if constexpr (!MN) {
-        const int r = i >> 2, s = i & 3;
-        to = pieces + r * 64 + ((s ^ ((r >> 1) & 3)) << 4);
-      } else {
-        const int s = i & 3, k = (i >> 2) & 31, half = (i >> 7) & 1, block = i >> 8;
-        to = pieces + block * 4096 + k * 128 + (((half * 4 + s) ^ (k & 7)) << 4);
-      }
+  for (int u = 0; u < U; ++u) {
+    if (CUT && zero) lo[u] = hi[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const Pieces v = take_apart(lo[u], hi[u]);
+    // two rounds make a block of 64 across: the second has the other half of its slices
+    char* const p = to + (MN ? (to_at ^ (u & 1) << 6) + (u >> 1) * 4096 : to_at + u * 2048);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) *(uint4*)(to + p * piece_bytes) = v.p[p];
-    }
+    for (int k = 0; k < 3; ++k) *(uint4*)(p + k * piece_bytes) = v.p[k];
+  }
+}
+template <bool MN, bool CUT>
+__device__ __forceinline__ void take_stage_apart(const char* copied, char* pieces, int n, int piece_bytes, int valid) {
+  const bool zero = CUT && (int)(threadIdx.x % kApartTeam >> 2) >= valid;
+  const int rounds = MN ? (n + 63) / 64 * 2 : (n + 31) / 32;
+  if (rounds == 4) {
+    take_rounds_apart<MN, 4, CUT>(copied, pieces, piece_bytes, zero);
+  } else if (MN) {
+    take_rounds_apart<MN, 2, CUT>(copied, pieces, piece_bytes, zero);
+  } else {
+    for (int u = 0; u < rounds; ++u) take_rounds_apart<MN, 1, CUT>(copied + u * 4096, pieces + u * 2048, piece_bytes, zero);
   }
 }
 
@@ -484,6 +477,12 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       const uint32_t what = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, Tr::kMnB, kTileM, c.tile_n);
       const uint32_t what_bias = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, false, kTileM, 16);
       const uint64_t ones_tile = tile_descriptor(shared_addr(ones), 128, 256, 0);      // 16 x 16 in core matrices of 8 x 16 bytes
+      const uint32_t start = shared_addr(Tr::kSplit ? pieces : copied), start_b = keep ? shared_addr(kept) : start + (Tr::kSplit ? 3 * piece_a : copied_a);
+      const uint32_t stage_units = (Tr::kSplit ? piece_bytes : copied_bytes) >> 4;
+      const uint64_t first_a = Tr::kMnA ? tile_descriptor(start, Tr::kBlock * 128, 1024, kSwizzle128)
+                                        : tile_descriptor(start, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
+      const uint64_t first_b = Tr::kMnB ? tile_descriptor(start_b, Tr::kBlock * 128, 1024, kSwizzle128)
+                                        : tile_descriptor(start_b, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
       int stage = 0, tiles = 0, kept_g = -1, kept_n = -1, kept_times = 0;
       uint32_t phase = 0, mended = 0;
       while (fine && walk.take(&item)) {
@@ -507,15 +506,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             mended ^= 1;
           }
           tmem_fence_after();
-          const uint32_t a = shared_addr(Tr::kSplit ? pieces + (size_t)stage * piece_bytes : copied + (size_t)stage * copied_bytes);
-          const uint32_t b = keep ? shared_addr(kept + (size_t)k * kept_bytes) : a + (Tr::kSplit ? 3 * piece_a : copied_a);
-          const uint64_t tile_a = Tr::kMnA ? tile_descriptor(a, Tr::kBlock * 128, 1024, kSwizzle128)
-                                           : tile_descriptor(a, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
-          const uint64_t tile_b = Tr::kMnB ? tile_descriptor(b, Tr::kBlock * 128, 1024, kSwizzle128)
-                                           : tile_descriptor(b, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
-#pragma unroll
-          for (int s = 0; s < Tr::kBlock / 16; ++s) {
-            if (s >= steps) break;
+          const uint64_t tile_a = first_a + (uint32_t)stage * stage_units, tile_b = keep ? first_b + (uint32_t)k * (uint32_t)(kept_bytes >> 4) : first_b + (uint32_t)stage * stage_units;
+          const auto step = [&](int s) {
             const uint64_t da = tile_a + s * ((Tr::kMnA ? 2048 : 32) >> 4), db = tile_b + s * ((Tr::kMnB ? 2048 : 32) >> 4);
             const bool add = k > 0 || s > 0;
             tile_product(acc, da, db, what, add);
@@ -528,10 +520,16 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               tile_product(small, da, db + 2 * pb, what, true);
               tile_product(small, da + 2 * pa, db, what, true);
             }
-            if (sums)
+            if (MODE == kGradW && sums)
 #pragma unroll
               for (int p = 0; p < Tr::kPieces; ++p)
                 tile_product(tmem + kAccColumns + (p ? 16 : 0), da + p * (piece_a >> 4), ones_tile, what_bias, add || p > 1);
+          };
+          if (steps == Tr::kBlock / 16) {
+#pragma unroll
+            for (int s = 0; s < Tr::kBlock / 16; ++s) step(s);
+          } else {
+            for (int s = 0; s < steps; ++s) step(s);
           }
           products_done(shared_addr((Tr::kSplit ? used : free_) + stage));
           if (k == item.stages - 1) products_done(shared_addr(acc_full + buffer));
@@ -647,7 +645,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     }
   } else if (Tr::kSplit && warp >= 8) {
     // ---- fp32 taken apart, by two teams in turn: one's waits and fence are the other's work
-    const int team = (warp - 8) / 4, thread = (threadIdx.x - 256) % kApartTeam;
+    const int team = (warp - 8) / 4;
     int from = 0, kept_g = -1, kept_n = -1, kept_times = 0, turn = 0;
     uint32_t from_phase = 0, to_phase = 0;
     const auto next_from = [&] {
@@ -661,7 +659,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         for (int k = 0; fine && k < kept_stages; ++k, next_from()) {
           if ((k & 1) != team) continue;
           if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up)))) break;
-          take_stage_apart<Tr::kMnB>(copied + (size_t)from * copied_bytes, kept + (size_t)k * kept_bytes, c.tile_n, piece_b, Tr::kBlock, thread);
+          take_stage_apart<Tr::kMnB, false>(copied + (size_t)from * copied_bytes, kept + (size_t)k * kept_bytes, c.tile_n, piece_b, Tr::kBlock);
           __syncwarp();
           if (lane == 0) barrier_arrive(shared_addr(free_ + from));
         }
@@ -677,8 +675,13 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const char* const in = copied + (size_t)from * copied_bytes;
         char* const out = pieces + (size_t)team * piece_bytes;
         const int valid = MODE == kGradW ? item.rows - k * Tr::kBlock : Tr::kBlock;
-        take_stage_apart<Tr::kMnA>(in, out, MODE == kGradW ? kTileM : c.tile_m, piece_a, valid, thread);
-        if (!keep) take_stage_apart<Tr::kMnB>(in + copied_a, out + 3 * piece_a, c.tile_n, piece_b, MODE == kGradW ? valid : Tr::kBlock, thread);
+        if (MODE == kGradW && valid < Tr::kBlock) {
+          take_stage_apart<Tr::kMnA, true>(in, out, kTileM, piece_a, valid);
+          take_stage_apart<Tr::kMnB, true>(in + copied_a, out + 3 * piece_a, c.tile_n, piece_b, valid);
+        } else {
+          take_stage_apart<Tr::kMnA, false>(in, out, MODE == kGradW ? kTileM : c.tile_m, piece_a, valid);
+          if (!keep) take_stage_apart<Tr::kMnB, false>(in + copied_a, out + 3 * piece_a, c.tile_n, piece_b, valid);
+        }
         fence_for_tensor_cores();
         __syncwarp();
         if (lane == 0) {

@@ -95,13 +95,34 @@ __device__ __forceinline__ float act_slope(float z) {
   return 1.0f;
 }
 
+// Two 16-bit elements, rounded by one instruction.
+template <typename T>
+__device__ __forceinline__ uint32_t rounded_pair(float a, float b) {
+  if constexpr (Elem<T>::kIsBf16) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&r;
+  } else {
+    const __half2 r = __floats2half2_rn(a, b);
+    return *(const uint32_t*)&r;
+  }
+}
+// A 16-byte slice of elements from v on, rounded.
+template <typename T>
+__device__ __forceinline__ uint4 rounded_slice(const float* v) {
+  if constexpr (sizeof(T) == 4) return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  else return make_uint4(rounded_pair<T>(v[0], v[1]), rounded_pair<T>(v[2], v[3]), rounded_pair<T>(v[4], v[5]), rounded_pair<T>(v[6], v[7]));
+}
 // N neighbouring elements, rounded.
 template <typename T, int N>
 __device__ __forceinline__ void store_all(T* p, const float (&v)[N]) {
-  Pack<T, N> r;
+  if constexpr (N * sizeof(T) == 16) {
+    *(uint4*)p = rounded_slice<T>(v);
+  } else {
+    Pack<T, N> r;
 #pragma unroll
-  for (int k = 0; k < N; ++k) r.v[k] = Elem<T>::from_f(v[k]);
-  store_pack<T, N>(p, r);
+    for (int k = 0; k < N; ++k) r.v[k] = Elem<T>::from_f(v[k]);
+    store_pack<T, N>(p, r);
+  }
 }
 
 // ---- ragged groups --------------------------------------------------------------

@@ -14,14 +14,14 @@ __global__ void __launch_bounds__(256) k_dropout(const T* __restrict__ in, int64
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VE; i < n; i += (int64_t)gridDim.x * 256 * VE) {
     if (VEC && i + VE <= n) {
       const Raw<T, VE> v = load_raw<T, VE>(in + i);
-      Pack<T, VE> r;
+      float r[VE];
 #pragma unroll
       for (int q = 0; q < VE / 4; ++q) {
         const Philox4 w = drop_words(d, (i >> 2) + q);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) r.v[4 * q + k] = Elem<T>::from_f(dropped(d, w.w[k], v.get(4 * q + k)));
+        for (int k = 0; k < 4; ++k) r[4 * q + k] = dropped(d, w.w[k], v.get(4 * q + k));
       }
-      store_pack<T, VE>(out + i, r);
+      store_all<T, VE>(out + i, r);
     } else {
       for (int q = 0; q < VE / 4; ++q) {
         const Philox4 w = drop_words(d, (i >> 2) + q);

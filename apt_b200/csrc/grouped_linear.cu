@@ -28,8 +28,11 @@ enum GroupedMode { kOut = 0, kGradX = 1, kGradW = 2 };
 
 constexpr int kTileM = 128;                  // rows of a product
 constexpr int kMostShared = 227 * 1024 - 640;      // shared memory of a block but for the barriers' and the scan's
-constexpr int kAccColumns = 256;             // tensor memory of a tile: two of them, or one and the sums of the bias
+constexpr int kAccColumns = 256;             // tensor memory of a tile: there is room for two
 constexpr int kMaxStages = 12;
+constexpr int kPlanWords = 5;                // of a run
+constexpr int kJoinParts = 16;               // blocks for a sum of dw
+constexpr int kKeepChange = 2;               // tiles that changing kept weights takes the time of (5 us to 2.4 a tile of bf16, 8 to 4 of fp32)
 
 template <typename T, int MODE>
 struct GroupedTraits {
@@ -41,7 +44,6 @@ struct GroupedTraits {
   // warps that bring tiles out: two for each quarter of tensor memory's lanes, or one beside the eight that take fp32 apart
   static constexpr int kOutWarps = kSplit ? 4 : 8;
   static constexpr int kThreads = kSplit ? 512 : 384;
-  static constexpr int kPieces = kSplit ? 3 : 1;
   // bytes of a tile of n rows (or columns) in a stage as copied, and of one bf16 piece of it
   static __host__ __device__ constexpr int copied(int n, bool mn) { return mn ? (n + kBox - 1) / kBox * kBlock * 128 : n * 128; }
   static __host__ __device__ constexpr int piece(int n, bool mn) { return mn ? (n + 63) / 64 * kBlock * 128 : (n + 31) / 32 * 32 * kBlock * 2; }
@@ -55,13 +57,16 @@ struct GroupedCall {
   int tile_m, tile_n, tiles_m, tiles_n;
   int copied_stages, piece_stages;
   int keep;                     // out and dx: a group's weights stay in shared memory while a block has tiles of it
+  int halves;                   // out and dx: tiles of 128 rows that share a stage's weights
+  int deep;                     // out and dx: blocks of the contraction in a stage
   int64_t ranges;               // dw: into how many runs of stages the work is cut at most
   const void *a, *b;            // the operands, as the copies read them
   int64_t pitch_a, pitch_b;     // elements
   const void* bias;
   void *out, *grad_bias;
   float *partial, *partial_bias;
-  int64_t* plan;                // dw, for k_join_weights: units, runs, and of each run the first piece's tile and group, first and last unit
+  int64_t* plan;                // dw, for k_join_weights: units, runs, and of each run its first piece's tile and group and the sum's first unit, the run's
+                                // beginning and that of the run before, the sum's last run
   int32_t* status;
 };
 
@@ -69,7 +74,7 @@ struct GroupedCall {
 struct GroupedItem {
   int g;
   int64_t row;                  // first row of x
-  int rows;                     // of the group from there on, in out and dx at most tile_m
+  int rows;                     // of the group from there on, in out and dx at most halves tile_m
   int m0, n0, stages;
   int64_t piece;                // dw: number of the partial sum, -1: all of the sum
   int64_t first, last;          // dw: units of all of the sum
@@ -148,19 +153,24 @@ struct GroupedWalk {
         t = c.tiles_n == 1 ? (int)next : (int)quotient(next, c.tiles_n);
         g = t < prefix[last_g + 1] && !c.keep ? last_g : group_of(t, c.groups + 1);
         n = (int)(next - (int64_t)t * c.tiles_n);
-        if (c.keep) {      // a group's tiles column by column, not row by row
+        if (c.keep) {      // a group's tiles column by column, not row by row; the first of each column stand for the change of weights
           const int here = prefix[g + 1] - prefix[g];
           const int64_t at = next - (int64_t)prefix[g] * c.tiles_n;
-          n = (int)quotient(at, here), t = prefix[g] + (int)(at - (int64_t)n * here);
+          n = (int)quotient(at, here), t = (int)(at - (int64_t)n * here);
+          if (t < kKeepChange) {
+            next += kKeepChange - t, t = kKeepChange;
+            if (next >= end) return false;
+          }
+          t += prefix[g];
         }
       }
       last_t = t, last_n = n, last_g = g;
       item->g = g;
-      item->row = begin[g] + (int64_t)(t - prefix[g]) * c.tile_m;
-      item->rows = (int)min((int64_t)c.tile_m, begin[g + 1] - item->row);
+      item->row = begin[g] + (int64_t)(t - prefix[g] - (c.keep ? kKeepChange : 0)) * (c.tile_m * c.halves);
+      item->rows = (int)min((int64_t)(c.tile_m * c.halves), begin[g + 1] - item->row);
       item->m0 = 0;
       item->n0 = n * c.tile_n;
-      item->stages = g < c.groups ? (c.num_k + Tr::kBlock - 1) / Tr::kBlock : 0;      // rows of no group: zeros
+      item->stages = g < c.groups ? (c.num_k + Tr::kBlock * c.deep - 1) / (Tr::kBlock * c.deep) : 0;      // rows of no group: zeros
       item->piece = -1, item->run = -1, item->first = item->last = 0;
       next += step;
       return true;
@@ -238,10 +248,37 @@ __device__ __noinline__ float sum_again(const GroupedCall& c, const GroupedItem&
   for (int64_t k = 0; k < count && sum == sum; ++k) sum = fmaf(a[k * step_a], b[k * step_b], sum);
   return sum;
 }
-__device__ __noinline__ float column_again(const GroupedCall& c, const GroupedItem& item, int m) {
-  float sum = 0.0f;
-  for (int k = 0; k < item.rows && sum == sum; ++k) sum += ((const float*)c.a)[(item.row + k) * c.pitch_a + item.m0 + m];
-  return sum;
+// Sums over the rows of a stage of dy as copied: of a column (fp32, 128 threads), or over a quarter of the rows of a pair of columns.
+template <typename T>
+__device__ __forceinline__ void add_columns(const char* stage, int valid, int thread, float (&sum)[2]) {
+  constexpr bool kWide = sizeof(T) == 4;
+  const int word = kWide ? thread : thread & 63, k0 = kWide ? 0 : (thread >> 6) * 16;
+  const char* const from = stage + (word >> 5) * ((kWide ? 32 : 64) * 128) + k0 * 128 + (word & 3) * 4;
+  const int slice = (word & 31) >> 2, rows = min(valid - k0, kWide ? 32 : 16);
+  const auto add = [](uint32_t v, float& a, float& b) {
+    if constexpr (kWide) {
+      a += __uint_as_float(v);
+    } else if constexpr (Elem<T>::kIsBf16) {
+      a += __uint_as_float(v << 16), b += __uint_as_float(v & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*(const __half2*)&v);
+      a += f.x, b += f.y;
+    }
+  };
+  if (rows == (kWide ? 32 : 16)) {
+    float a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k0 = 0; k0 < (kWide ? 32 : 16); k0 += 16) {
+      uint32_t v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = *(const uint32_t*)(from + (k0 + k) * 128 + ((slice ^ (k & 7)) << 4));
+#pragma unroll
+      for (int k = 0; k < 16; ++k) add(v[k], a[k % 4], b[k % 4]);
+    }
+    sum[0] += (a[0] + a[1]) + (a[2] + a[3]), sum[1] += (b[0] + b[1]) + (b[2] + b[3]);
+  } else {
+    for (int k = 0; k < rows; ++k) add(*(const uint32_t*)(from + k * 128 + ((slice ^ (k & 7)) << 4)), sum[0], sum[1]);
+  }
 }
 
 // ---- bringing a tile out -------------------------------------------------------------
@@ -298,12 +335,7 @@ __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedIt
           v[h][k] += b.x, v[h][k + 1] += b.y, v[h][k + 2] += b.z, v[h][k + 3] += b.w;
         }
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      Pack<O, kPer> p;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) p.v[k] = Elem<O>::from_f(v[s * kPer / 32][(s * kPer + k) % 32]);
-      *(uint4*)(staging + lane * 128 + ((s ^ (lane & 7)) << 4)) = *(const uint4*)&p;
-    }
+    for (int s = 0; s < 8; ++s) *(uint4*)(staging + lane * 128 + ((s ^ (lane & 7)) << 4)) = rounded_slice<O>(&v[s * kPer / 32][s * kPer % 32]);
     if constexpr (Tr::kSplit) {
       if (lane < here)
         for (; wild; wild &= wild - 1) {
@@ -317,11 +349,14 @@ __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedIt
       const int s = lane & 7, r1 = lane >> 3, col = c0 + s * kPer;
       O* to = first + (int64_t)r1 * ld + col;
       const char* from = staging + r1 * 128;
-      if (col < columns) {
+      // all of them are read before any is stored: the compiler does not know that the stores go elsewhere
+      uint4 slice[8];
 #pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += 4, to += 4 * ld)
-          if (r0 + r1 < here) *(uint4*)to = *(const uint4*)(from + r0 * 128 + ((s ^ ((r0 + r1) & 7)) << 4));
-      }
+      for (int k = 0; k < 8; ++k) slice[k] = *(const uint4*)(from + k * 512 + ((s ^ ((4 * k + r1) & 7)) << 4));
+      const int rows_left = col < columns ? here - r1 : 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k, to += 4 * ld)
+        if (4 * k < rows_left) *(uint4*)to = slice[k];
     } else {
       for (int r = 0; r < here; ++r)
         for (int k = lane; k < kWide; k += 32) {
@@ -338,7 +373,7 @@ template <typename T, int MODE>
 __global__ void __launch_bounds__(GroupedTraits<T, MODE>::kThreads, 1)
 k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GroupedCall c) {
   using Tr = GroupedTraits<T, MODE>;
-  constexpr int kBuffers = MODE == kGradW ? 1 : 2;
+  constexpr int kBuffers = 2;
   constexpr bool kMends = MODE == kGradW && !Tr::kSplit;
   extern __shared__ char raw_shared[];
   __shared__ uint64_t full[kMaxStages], free_[kMaxStages], ready[kMaxStages], used[kMaxStages], acc_full[2], acc_free[2], kept_full, kept_free, drained;
@@ -349,7 +384,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   const bool keep = MODE != kGradW && c.keep;
-  const int copied_a = Tr::copied(kTileM, Tr::kMnA), copied_b = Tr::copied(c.tile_n, Tr::kMnB), copied_bytes = copied_a + (keep ? 0 : copied_b);
+  // (products read 128 rows of a smaller tile too: what lies behind it in shared memory)
+  const int copied_a = MODE == kGradW || Tr::kSplit ? Tr::copied(kTileM, Tr::kMnA) : c.halves * c.tile_m * 128, copied_b = Tr::copied(c.tile_n, Tr::kMnB);
+  const int block_bytes = copied_a + (keep ? 0 : copied_b), copied_bytes = c.deep * block_bytes;
   const int piece_a = Tr::piece(kTileM, Tr::kMnA), piece_b = Tr::piece(c.tile_n, Tr::kMnB);
   const int piece_bytes = Tr::kSplit ? 3 * (piece_a + (keep ? 0 : piece_b)) : 0;
   const int kept_stages = keep ? (c.num_k + Tr::kBlock - 1) / Tr::kBlock : 0, kept_bytes = Tr::kSplit ? 3 * piece_b : copied_b;
@@ -357,14 +394,14 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   char* const pieces = copied + (size_t)c.copied_stages * copied_bytes;
   char* const kept = pieces + (size_t)c.piece_stages * piece_bytes;
   char* const staging = kept + (size_t)kept_stages * kept_bytes;
-  char* const ones = staging + Tr::kOutWarps * 4096;      // (the bias of a tile in out)
-  int *const prefix = (int*)(ones + (MODE == kGradW ? 512 : 1024)), *const begin = prefix + c.groups + 2;
+  float* const bias = (float*)(staging + Tr::kOutWarps * 4096);      // of a tile in out; in dw the sums of db that several threads have
+  int *const prefix = (int*)(bias + (MODE == kGradW ? 512 : 256)), *const begin = prefix + c.groups + 2;
 
   if (warp == 1) tmem_alloc(shared_addr(&tmem_slot), 512);
   if (threadIdx.x == 0) {
     for (int k = 0; k < kMaxStages; ++k) {
       barrier_init(shared_addr(full + k), 1);
-      barrier_init(shared_addr(free_ + k), Tr::kSplit ? 4 : 1);
+      barrier_init(shared_addr(free_ + k), (Tr::kSplit ? 4 : 1) + (MODE == kGradW && c.grad_bias ? Tr::kOutWarps : 0));
       barrier_init(shared_addr(ready + k), Tr::kSplit ? 4 : 1);
       barrier_init(shared_addr(used + k), 1);
     }
@@ -375,34 +412,44 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     gave_up_word = 0;
   }
-  if constexpr (MODE == kGradW) {
-    for (int i = threadIdx.x; i < 128; i += Tr::kThreads) ((uint32_t*)ones)[i] = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
-    fence_for_tensor_cores();
-  }
   wait_for_previous();
 
-  // tiles (stages) of the groups before each; none at all where the ends are no ends
-  int before = 0, bad = 0;
-  for (int g = threadIdx.x; g < c.groups; g += Tr::kThreads) bad |= bad_group(c.offsets, g, c.rows);
+  // The groups' first rows, and the tiles (stages) of the groups before each; none at all where the ends are no ends.
+  int bad = 0;
+  for (int g = threadIdx.x; g <= c.groups; g += Tr::kThreads) {
+    const int64_t v = c.offsets[g];
+    bad |= v < 0 || v > c.rows || (g == 0 && v != 0);
+    begin[g] = (int)min(max(v, (int64_t)0), c.rows);
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < c.groups; g += Tr::kThreads) bad |= begin[g + 1] < begin[g];
   bad = __syncthreads_or(bad);
   if (bad && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
-  const int lists = MODE == kGradW ? c.groups : c.groups + 1, unit = MODE == kGradW ? Tr::kBlock : c.tile_m;
+  const int lists = MODE == kGradW ? c.groups : c.groups + 1, unit = MODE == kGradW ? Tr::kBlock : c.tile_m * c.halves;      // (the last one: rows of no group)
+  int before = 0;
   for (int g0 = 0; g0 < lists; g0 += Tr::kThreads) {
     const int g = g0 + threadIdx.x;
-    int n = 0;
-    if (g < c.groups) {
-      const RowRange r = group_rows(c.offsets, g, c.rows);
-      n = bad ? 0 : (int)((r.end - r.begin + unit - 1) / unit);
-    } else if (g < lists) {
-      n = bad ? 0 : (int)((c.rows - min(max(c.offsets[c.groups], (int64_t)0), c.rows) + unit - 1) / unit);
+    int total, n = 0;
+    if (g < lists && !bad) n = ((g < c.groups ? begin[g + 1] : (int)c.rows) - begin[g] + unit - 1) / unit;
+    if (MODE != kGradW && c.keep && n) n += kKeepChange;
+    if (lists <= 32) {      // one warp's
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      if (g < lists) prefix[g + 1] = sum;
+    } else {
+      const int at = before + block_exclusive_scan(n, scan, &total);
+      if (g < lists) prefix[g + 1] = at + n;
+      before += total;
     }
-    int total;
-    const int at = before + block_exclusive_scan(n, scan, &total);
-    if (g < lists) prefix[g] = at, begin[g] = (int)min(max(c.offsets[g], (int64_t)0), c.rows);
-    before += total;
   }
-  // (where the ends are ends, a group's rows end where the next one's begin)
-  if (threadIdx.x == 0) prefix[lists] = before, begin[lists] = MODE == kGradW ? (int)min(max(c.offsets[c.groups], (int64_t)0), c.rows) : (int)c.rows;
+  if (threadIdx.x == 0) {
+    prefix[0] = 0;
+    if (MODE != kGradW) begin[lists] = (int)c.rows;
+  }
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -421,7 +468,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const int boxes_b = Tr::kMnB ? (min(c.tile_n, c.num_n - item.n0) + Tr::kBox - 1) / Tr::kBox : 1;
         constexpr int kBoxBytes = Tr::kBlock * 128;
         const uint32_t bytes_b = Tr::kMnB ? boxes_b * kBoxBytes : c.tile_n * 128;
-        const uint32_t bytes = (MODE == kGradW ? boxes_a * kBoxBytes : c.tile_m * 128) + (keep ? 0 : bytes_b);
+        const int halves = MODE != kGradW && item.rows > c.tile_m ? 2 : 1, blocks = MODE == kGradW ? 0 : (c.num_k + Tr::kBlock - 1) / Tr::kBlock;
+        const uint32_t bytes = (MODE == kGradW ? boxes_a * kBoxBytes : halves * c.tile_m * 128) + (keep ? 0 : bytes_b);
         const auto copy_weights = [&](uint32_t b, int k, uint32_t bar) {
           if constexpr (MODE == kOut) {
             copy_box(b, &map_b, k * Tr::kBlock, item.n0, item.g, bar);
@@ -448,15 +496,21 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         for (int k = 0; k < item.stages; ++k) {
           if (!(fine = barrier_wait(shared_addr(free_ + stage), phase ^ 1, gave_up))) break;
-          const uint32_t bar = shared_addr(full + stage), a = shared_addr(copied + (size_t)stage * copied_bytes), b = a + copied_a;
-          barrier_expect(bar, bytes);
+          const uint32_t bar = shared_addr(full + stage);
+          uint32_t a = shared_addr(copied + (size_t)stage * copied_bytes), b = a + copied_a;
           if constexpr (MODE == kGradW) {
+            barrier_expect(bar, bytes);
             const int row = (int)item.row + k * Tr::kBlock;
             for (int i = 0; i < boxes_a; ++i) copy_box(a + i * kBoxBytes, &map_a, item.m0 + i * Tr::kBox, row, bar);
             for (int i = 0; i < boxes_b; ++i) copy_box(b + i * kBoxBytes, &map_b, item.n0 + i * Tr::kBox, row, bar);
           } else {
-            copy_box(a, &map_a, k * Tr::kBlock, (int)item.row, bar);
-            if (!keep) copy_weights(b, k, bar);
+            const int first = k * c.deep, last = min(first + c.deep, blocks);
+            barrier_expect(bar, bytes * (last - first));
+            for (int l = first; l < last; ++l, a += block_bytes, b += block_bytes) {
+              copy_box(a, &map_a, l * Tr::kBlock, (int)item.row, bar);
+              if (halves == 2) copy_box(a + kTileM * 128, &map_a, l * Tr::kBlock, (int)item.row + kTileM, bar);
+              if (!keep) copy_weights(b, l, bar);
+            }
           }
           ++loaded;
           if (++stage == c.copied_stages) stage = 0, phase ^= 1;
@@ -475,20 +529,21 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (one_of_warp()) {
       const int stages = Tr::kSplit ? c.piece_stages : c.copied_stages;
       const uint32_t what = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, Tr::kMnB, kTileM, c.tile_n);
-      const uint32_t what_bias = product_descriptor(!std::is_same<T, __half>::value, Tr::kMnA, false, kTileM, 16);
-      const uint64_t ones_tile = tile_descriptor(shared_addr(ones), 128, 256, 0);      // 16 x 16 in core matrices of 8 x 16 bytes
       const uint32_t start = shared_addr(Tr::kSplit ? pieces : copied), start_b = keep ? shared_addr(kept) : start + (Tr::kSplit ? 3 * piece_a : copied_a);
       const uint32_t stage_units = (Tr::kSplit ? piece_bytes : copied_bytes) >> 4;
       const uint64_t first_a = Tr::kMnA ? tile_descriptor(start, Tr::kBlock * 128, 1024, kSwizzle128)
                                         : tile_descriptor(start, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
       const uint64_t first_b = Tr::kMnB ? tile_descriptor(start_b, Tr::kBlock * 128, 1024, kSwizzle128)
                                         : tile_descriptor(start_b, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
-      int stage = 0, tiles = 0, kept_g = -1, kept_n = -1, kept_times = 0;
-      uint32_t phase = 0, mended = 0;
+      int stage = 0, kept_g = -1, kept_n = -1, kept_times = 0, buffer = kBuffers - 1;
+      uint32_t phase = 0, mended = 0, turns = 0;      // turns: parity of each buffer's uses
       while (fine && walk.take(&item)) {
         if (!item.stages) continue;
-        const int buffer = tiles % kBuffers;
-        if (!(fine = barrier_wait(shared_addr(acc_free + buffer), ((tiles / kBuffers) & 1) ^ 1, gave_up))) break;
+        const int halves = MODE != kGradW && item.rows > c.tile_m ? 2 : 1;
+        buffer = c.halves == 2 || buffer == kBuffers - 1 ? 0 : buffer + 1;
+        if (!(fine = barrier_wait(shared_addr(acc_free + buffer), turns >> buffer & 1 ^ 1, gave_up))) break;
+        if (halves == 2 && !(fine = barrier_wait(shared_addr(acc_free + 1), turns >> 1 & 1 ^ 1, gave_up))) break;
+        turns ^= halves == 2 ? 3 : 1 << buffer;
         if (keep && (item.g != kept_g || item.n0 != kept_n)) {
           kept_g = item.g, kept_n = item.n0;
           if (kept_times) products_done(shared_addr(&kept_free));
@@ -496,10 +551,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           ++kept_times;
         }
         const uint32_t acc = tmem + buffer * kAccColumns;
-        const bool sums = MODE == kGradW && c.grad_bias && item.n0 == 0;
         for (int k = 0; k < item.stages; ++k) {
           if (!(fine = barrier_wait(shared_addr((Tr::kSplit ? ready : full) + stage), phase, gave_up))) break;
-          const int left = (MODE == kGradW ? item.rows : c.num_k) - k * Tr::kBlock, steps = (min(left, Tr::kBlock) + 15) / 16;
+          const int left = (MODE == kGradW ? item.rows : c.num_k) - k * Tr::kBlock * c.deep, steps = (min(left, Tr::kBlock * c.deep) + 15) / 16;
           if (kMends && left < Tr::kBlock && left % 16) {
             barrier_arrive(shared_addr(ready));
             if (!(fine = barrier_wait(shared_addr(ready + 1), mended, gave_up))) break;
@@ -507,10 +561,10 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           }
           tmem_fence_after();
           const uint64_t tile_a = first_a + (uint32_t)stage * stage_units, tile_b = keep ? first_b + (uint32_t)k * (uint32_t)(kept_bytes >> 4) : first_b + (uint32_t)stage * stage_units;
-          const auto step = [&](int s) {
+          const auto step = [&](uint64_t tile_a, uint64_t tile_b, int s, bool add) {
             const uint64_t da = tile_a + s * ((Tr::kMnA ? 2048 : 32) >> 4), db = tile_b + s * ((Tr::kMnB ? 2048 : 32) >> 4);
-            const bool add = k > 0 || s > 0;
             tile_product(acc, da, db, what, add);
+            if (!Tr::kSplit && MODE != kGradW && halves == 2) tile_product(acc + kAccColumns, da + (kTileM * 128 >> 4), db, what, add);
             if constexpr (Tr::kSplit) {
               const uint64_t pa = piece_a >> 4, pb = piece_b >> 4;
               const uint32_t small = acc + Tr::kMostN;
@@ -520,22 +574,24 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               tile_product(small, da, db + 2 * pb, what, true);
               tile_product(small, da + 2 * pa, db, what, true);
             }
-            if (MODE == kGradW && sums)
-#pragma unroll
-              for (int p = 0; p < Tr::kPieces; ++p)
-                tile_product(tmem + kAccColumns + (p ? 16 : 0), da + p * (piece_a >> 4), ones_tile, what_bias, add || p > 1);
           };
-          if (steps == Tr::kBlock / 16) {
+          constexpr int kSteps = Tr::kBlock / 16;
+          for (int l = 0; l < (Tr::kSplit || MODE == kGradW ? 1 : c.deep) && l * kSteps < steps; ++l) {
+            const uint64_t at_a = tile_a + (uint32_t)l * (uint32_t)(block_bytes >> 4), at_b = tile_b + (uint32_t)l * (uint32_t)(block_bytes >> 4);
+            if (steps >= (l + 1) * kSteps) {
 #pragma unroll
-            for (int s = 0; s < Tr::kBlock / 16; ++s) step(s);
-          } else {
-            for (int s = 0; s < steps; ++s) step(s);
+              for (int s = 0; s < kSteps; ++s) step(at_a, at_b, s, k > 0 || l > 0 || s > 0);
+            } else {
+              for (int s = 0; s < steps - l * kSteps; ++s) step(at_a, at_b, s, k > 0 || l > 0 || s > 0);
+            }
           }
           products_done(shared_addr((Tr::kSplit ? used : free_) + stage));
-          if (k == item.stages - 1) products_done(shared_addr(acc_full + buffer));
+          if (k == item.stages - 1) {
+            products_done(shared_addr(acc_full + buffer));
+            if (halves == 2) products_done(shared_addr(acc_full + 1));
+          }
           if (++stage == stages) stage = 0, phase ^= 1;
         }
-        ++tiles;
       }
       if (*gave_up) {
         int nobody = 0;
@@ -562,70 +618,93 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       __syncwarp();
       if (lane == 0) barrier_arrive(shared_addr(ready + 1));
     }
-  } else if (warp >= 4 && warp < 4 + Tr::kOutWarps) {
+  } else if (warp >= 4 && (warp < 8 || !Tr::kSplit)) {
     // ---- finished tiles
-    const int quarter = warp % 4, turn = (warp - 4) / 4;
+    const int quarter = warp % 4, turn = warp >= 8, thread = turn * 128 + threadIdx.x % 128;
     constexpr int kTurns = Tr::kOutWarps / 4;
-    char* const mine = staging + (warp - 4) * 4096;
-    float* const bias = (float*)ones;
-    int tiles = 0, bias_g = -1, bias_n = -1;
+    char* const mine = staging + (turn * 4 + quarter) * 4096;
+    int summed = 0;
+    uint32_t summed_phase = 0;
+    int bias_g = -1, bias_n = -1, buffer = kBuffers - 1;
+    uint32_t turns = 0;
     while (fine && walk.take(&item)) {
-      const int buffer = tiles % kBuffers;
       const bool empty = item.stages == 0;
+      const int columns = min(c.tile_n, c.num_n - item.n0);
       if (MODE == kOut && c.bias && !empty && (item.g != bias_g || item.n0 != bias_n)) {
         bias_g = item.g, bias_n = item.n0;
         asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");      // the tile before is out
-        for (int k = threadIdx.x - 128; k < 256; k += Tr::kOutWarps * 32)
+        for (int k = thread; k < 256; k += Tr::kOutWarps * 32)
           bias[k] = bias_n + k < c.num_n ? Elem<T>::to_f(((const T*)c.bias)[(int64_t)bias_g * c.num_n + bias_n + k]) : 0.0f;
         asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");
       }
-      if (!empty) {
-        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_full + buffer), (tiles / kBuffers) & 1, gave_up));
-        if (!fine) break;
-        tmem_fence_after();
-      }
-      const uint32_t acc = tmem + buffer * kAccColumns;
-      const int columns = min(c.tile_n, c.num_n - item.n0);
+      float column = 0.0f;      // of db
       if constexpr (MODE == kGradW) {
-        const int rows = min(kTileM, c.num_m - item.m0), m = quarter * 32 + lane;
-        if (threadIdx.x == 128 && item.run >= 0) {
-          int64_t* const to = c.plan + 2 + 3 * item.run;
-          to[0] = (int64_t)(item.m0 / kTileM * c.tiles_n + item.n0 / c.tile_n) * c.groups + item.g, to[1] = item.first, to[2] = item.last;
-        }
-        if (quarter * 32 < rows) {
-          if (item.piece < 0)
-            store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0,
-                                   (int64_t)c.num_n, rows, columns, nullptr, 0u);
-          else
-            store_tile<T, float, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows,
-                                       columns, nullptr, 0u);
-          if (c.grad_bias && item.n0 == 0 && turn == 0) {
-            const uint32_t at = tmem + kAccColumns + ((uint32_t)quarter << 21);
-            float v = tmem_load_1(at), small = Tr::kSplit ? tmem_load_1(at + 16) : 0.0f;
-            tmem_wait_loads();
-            settled(v);
-            settled(small);
-            v += small;
-            if (m < rows) {
-              if constexpr (Tr::kSplit)
-                if (!isfinite(v)) v = column_again(c, item, m);
-              if (item.piece < 0) ((T*)c.grad_bias)[(int64_t)item.g * c.num_m + item.m0 + m] = Elem<T>::from_f(v);
-              else c.partial_bias[item.piece * kTileM + m] = v;
+        if (c.grad_bias) {
+          // the columns of dy, while the products are made of them: as products with ones they took a third of the time of a stage
+          float sum[2] = {0.0f, 0.0f};
+          for (int k = 0; k < item.stages; ++k) {
+            if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + summed), summed_phase, gave_up)))) break;
+            const int valid = item.rows - k * Tr::kBlock;
+            if (item.n0 == 0) add_columns<T>(copied + (size_t)summed * copied_bytes, valid, thread, sum);
+            __syncwarp();
+            if (lane == 0) barrier_arrive(shared_addr(free_ + summed));
+            if (++summed == c.copied_stages) summed = 0, summed_phase ^= 1;
+          }
+          if (!fine) break;
+          column = sum[0];
+          if constexpr (!Tr::kSplit) {      // four threads have a pair of columns
+            if (item.n0 == 0) {
+              asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");
+              *(float2*)(bias + (thread >> 6) * 128 + (thread & 63) * 2) = make_float2(sum[0], sum[1]);
+              asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");
+              const int m = thread & 127;
+              column = (bias[m] + bias[128 + m]) + (bias[256 + m] + bias[384 + m]);
             }
           }
         }
       }
-      const bool stores = MODE != kGradW && quarter * 32 < item.rows && turn * (128 / (int)sizeof(T)) < columns;
-      if (stores)
-        store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + item.row * c.num_n + item.n0, (int64_t)c.num_n, item.rows, columns,
-                               MODE == kOut && c.bias && !empty ? bias : nullptr, shared_addr(acc_free + buffer));
-      if (!empty) {
-        if (!stores) {
+      const int halves = MODE != kGradW && item.rows > c.tile_m ? 2 : 1;
+      for (int half = 0; half < halves; ++half) {
+        if (!empty) {
+          buffer = c.halves == 2 ? half : buffer == kBuffers - 1 ? 0 : buffer + 1;
+          fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_full + buffer), turns >> buffer & 1, gave_up));
+          if (!fine) break;
+          turns ^= 1u << buffer;
+          tmem_fence_after();
+        }
+        const uint32_t acc = tmem + buffer * kAccColumns;
+        if constexpr (MODE == kGradW) {
+          const int rows = min(kTileM, c.num_m - item.m0), m = quarter * 32 + lane;
+          if (thread == 0 && item.run >= 0) {
+            int64_t* const to = c.plan + 2 + kPlanWords * item.run;
+            to[0] = (int64_t)(item.m0 / kTileM * c.tiles_n + item.n0 / c.tile_n) * c.groups + item.g, to[1] = item.first;
+            to[2] = walk.runs.begin(item.run), to[3] = item.run ? walk.runs.begin(item.run - 1) : 0, to[4] = walk.runs.of(item.last - 1);
+          }
+          if (quarter * 32 < rows) {
+            if (item.piece < 0)
+              store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0,
+                                     (int64_t)c.num_n, rows, columns, nullptr, 0u);
+            else
+              store_tile<T, float, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows,
+                                         columns, nullptr, 0u);
+            if (c.grad_bias && item.n0 == 0 && turn == 0) {
+              if (m < rows) {
+                if (item.piece < 0) ((T*)c.grad_bias)[(int64_t)item.g * c.num_m + item.m0 + m] = Elem<T>::from_f(column);
+                else c.partial_bias[item.piece * kTileM + m] = column;
+              }
+            }
+          }
+        }
+        const int rows = item.rows - half * kTileM;
+        const bool stores = MODE != kGradW && quarter * 32 < min(rows, c.tile_m) && turn * (128 / (int)sizeof(T)) < columns;
+        if (stores)
+          store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + (item.row + half * kTileM) * c.num_n + item.n0, (int64_t)c.num_n,
+                                 min(rows, c.tile_m), columns, MODE == kOut && c.bias && !empty ? bias : nullptr, shared_addr(acc_free + buffer));
+        if (!empty && !stores) {
           tmem_fence_before();
           __syncwarp();
           if (lane == 0) barrier_arrive(shared_addr(acc_free + buffer));
         }
-        ++tiles;
       }
     }
   } else if (MODE == kGradW && warp == 3) {
@@ -647,7 +726,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     // ---- fp32 taken apart, by two teams in turn: one's waits and fence are the other's work
     const int team = (warp - 8) / 4;
     int from = 0, kept_g = -1, kept_n = -1, kept_times = 0, turn = 0;
-    uint32_t from_phase = 0, to_phase = 0;
+    uint32_t from_phase = 0, uses = 0;      // uses: parity of the team's stage of pieces
     const auto next_from = [&] {
       if (++from == c.copied_stages) from = 0, from_phase ^= 1;
     };
@@ -670,7 +749,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       }
       for (int k = 0; k < item.stages; ++k, turn ^= 1, next_from()) {
         if (turn != team) continue;      // each team has a stage of pieces of its own
-        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up) && barrier_wait(shared_addr(used + team), to_phase ^ 1, gave_up));
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up) && barrier_wait(shared_addr(used + team), uses ^ 1, gave_up));
         if (!fine) break;
         const char* const in = copied + (size_t)from * copied_bytes;
         char* const out = pieces + (size_t)team * piece_bytes;
@@ -688,7 +767,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           barrier_arrive(shared_addr(free_ + from));
           barrier_arrive(shared_addr(ready + team));
         }
-        to_phase ^= 1;
+        uses ^= 1;
       }
     }
   }
@@ -704,33 +783,46 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 k_join_weights(const __grid_constant__ GroupedCall c) {
   wait_for_previous();
-  const GroupedRuns runs{c.plan[0], c.plan[1]};
   const int64_t v = blockIdx.y + 1;
-  if (v >= runs.runs) return;
-  const int64_t *const from = c.plan + 2 + 3 * v, first = from[1], last = from[2], here = runs.begin(v);
-  if (here <= first || runs.begin(v - 1) > first) return;
-  const int64_t tile = from[0] / c.groups, r1 = runs.of(last - 1);
-  const int g = (int)(from[0] % c.groups), m0 = (int)(tile / c.tiles_n) * kTileM, n0 = (int)(tile % c.tiles_n) * c.tile_n;
-  const int64_t piece = 2 * (v - 1) + (runs.begin(v - 1) < first);
-  const int slices = c.tile_n / 4, i = blockIdx.x * 256 + threadIdx.x, m = i / slices, n = i % slices * 4;
-  if (m < kTileM && m0 + m < c.num_m && n0 + n < c.num_n) {
-    const int64_t size = (int64_t)kTileM * c.tile_n, at = (int64_t)m * c.tile_n + n;
-    float4 sum = *(const float4*)(c.partial + piece * size + at);
-#pragma unroll 4
+  if (v >= c.plan[1]) return;
+  const int64_t *const from = c.plan + 2 + kPlanWords * v, what = from[0], first = from[1], here = from[2], before = from[3], r1 = from[4];
+  // a run that begins with a sum has nothing to join it to; an earlier run that begins within this sum does it
+  if (here <= first || before > first) return;
+  const int tile = (int)(what / c.groups), g = (int)(what - (int64_t)tile * c.groups), m0 = tile / c.tiles_n * kTileM, n0 = tile % c.tiles_n * c.tile_n;
+  const int64_t piece = 2 * (v - 1) + (before < first);
+  const int slices = c.tile_n / 4;
+  const int64_t size = (int64_t)kTileM * c.tile_n;
+  // a sixteenth of the rows, four slices a thread at once
+  const int i1 = (blockIdx.x + 1) * (kTileM / kJoinParts) * slices;
+  for (int i0 = blockIdx.x * (kTileM / kJoinParts) * slices + threadIdx.x; i0 < i1; i0 += 4 * 256) {
+    float4 sum[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i0 + u * 256 < i1) sum[u] = *(const float4*)(c.partial + piece * size + (int64_t)(i0 + u * 256) * 4);
     for (int64_t r = v; r <= r1; ++r) {
-      const float4 p = *(const float4*)(c.partial + 2 * r * size + at);
-      sum.x += p.x, sum.y += p.y, sum.z += p.z, sum.w += p.w;
+      float4 p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i0 + u * 256 < i1) p[u] = *(const float4*)(c.partial + 2 * r * size + (int64_t)(i0 + u * 256) * 4);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sum[u].x += p[u].x, sum[u].y += p[u].y, sum[u].z += p[u].z, sum[u].w += p[u].w;
     }
-    T* const to = (T*)c.out + ((int64_t)g * c.num_m + m0 + m) * c.num_n + n0 + n;
-    const float s[4] = {sum.x, sum.y, sum.z, sum.w};
-    if (c.num_n % 4 == 0) {
-      store_all<T, 4>(to, s);
-    } else {
-      for (int k = 0; k < 4; ++k)
-        if (n0 + n + k < c.num_n) to[k] = Elem<T>::from_f(s[k]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * 256, m = i / slices, n = i % slices * 4;
+      if (i >= i1 || m0 + m >= c.num_m || n0 + n >= c.num_n) continue;
+      T* const to = (T*)c.out + ((int64_t)g * c.num_m + m0 + m) * c.num_n + n0 + n;
+      const float s[4] = {sum[u].x, sum[u].y, sum[u].z, sum[u].w};
+      if (c.num_n % 4 == 0) {
+        store_all<T, 4>(to, s);
+      } else {
+        for (int k = 0; k < 4; ++k)
+          if (n0 + n + k < c.num_n) to[k] = Elem<T>::from_f(s[k]);
+      }
     }
   }
-  if (c.grad_bias && n0 == 0 && i < kTileM && m0 + i < c.num_m) {
+  const int i = threadIdx.x;
+  if (c.grad_bias && n0 == 0 && blockIdx.x == 0 && i < kTileM && m0 + i < c.num_m) {
     float sum = c.partial_bias[piece * kTileM + i];
     for (int64_t r = v; r <= r1; ++r) sum += c.partial_bias[2 * r * kTileM + i];
     ((T*)c.grad_bias)[(int64_t)g * c.num_m + m0 + i] = Elem<T>::from_f(sum);
@@ -839,9 +931,9 @@ static WeightPlan weight_plan(int64_t rows, int64_t dim, int64_t out_dim, int64_
 template <typename T, int MODE>
 static int launch_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap& b, int64_t items, cudaStream_t s) {
   using Tr = GroupedTraits<T, MODE>;
-  const int fixed = 1024 + Tr::kOutWarps * 4096 + (MODE == kGradW ? 512 : 1024) + (int)align_up((size_t)(c.groups + 2) * 8, 16);
-  const int room = kMostShared - fixed;
-  int copied = Tr::copied(kTileM, Tr::kMnA), pieces = Tr::kSplit ? 3 * Tr::piece(kTileM, Tr::kMnA) : 0, kept = 0;
+  const int lists = 1024 + (MODE == kGradW ? 2048 : 1024) + (int)align_up((size_t)(c.groups + 2) * 8, 16);
+  const int room = kMostShared - lists - Tr::kOutWarps * 4096;
+  int copied = MODE == kGradW || Tr::kSplit ? Tr::copied(kTileM, Tr::kMnA) : c.tile_m * 128, pieces = Tr::kSplit ? 3 * Tr::piece(kTileM, Tr::kMnA) : 0, kept = 0;
   const int copied_b = Tr::copied(c.tile_n, Tr::kMnB), pieces_b = Tr::kSplit ? 3 * Tr::piece(c.tile_n, Tr::kMnB) : 0;
   // Weights are kept where they leave room for four stages of rows and a block has several tiles of them: what the copies bring from L2, which
   // gives 10 to 12 TB/s, is then the rows alone.
@@ -850,10 +942,20 @@ static int launch_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap
     c.keep = bytes + least <= room && items >= 3 * kNumSMs && items >= 3 * (int64_t)c.groups * c.tiles_n;
     if (c.keep) kept = (int)bytes;
   }
+  c.halves = c.deep = 1;
+  if (MODE != kGradW && !Tr::kSplit && !c.keep) {
+    // Two tiles of rows share the weights of a stage where groups are long and the contraction is: the weights come half as often, and bringing
+    // tiles out beside the products, which both halves of tensor memory are taken from, is what a long contraction needs least.
+    if (c.tile_m == kTileM && c.num_k >= 512 && c.rows >= (int64_t)c.groups * 4 * kTileM && items >= 4 * kNumSMs) c.halves = 2, items /= 2;
+    // Small stages are two blocks of the contraction deep: a stage costs its waits whatever it holds.
+    else if (c.num_k > Tr::kBlock && 2 * (copied + copied_b) <= 48 * 1024) c.deep = 2;
+  }
   if (!c.keep) copied += copied_b, pieces += pieces_b;
+  if (c.halves == 2) copied += kTileM * 128;
+  copied *= c.deep;
   c.piece_stages = Tr::kSplit ? 2 : 0;
   c.copied_stages = std::min(kMaxStages, (room - kept - c.piece_stages * pieces) / copied);
-  const int bytes = fixed + kept + c.copied_stages * copied + c.piece_stages * pieces;
+  const int bytes = lists + Tr::kOutWarps * 4096 + kept + c.copied_stages * copied + c.piece_stages * pieces;
   static const cudaError_t allowed = cudaFuncSetAttribute(k_grouped<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
   APT_CUDA(allowed);
   // over half of an SM's shared memory, so that no two blocks share one: each takes all of its tensor memory
@@ -872,17 +974,19 @@ static int rows_product(const Operand& rows, const Operand& weight, int64_t num_
   GroupedCall c = {};
   c.offsets = offsets, c.rows = rows.rows, c.groups = groups;
   c.num_n = (int)num_n, c.num_k = (int)rows.columns;
-  // Tiles of 128 rows, or as many as a mean group has twice over, are made smaller until every SM has one (four where rows are few, whose
-  // time is that of reading the weights), down to 16 rows and 64 columns. The products are of 128 rows always: rows that are not copied are
-  // not written either, so that only copies and conversions get fewer.
+  // Tiles of 128 rows, or as many as a mean group has twice over, are made smaller, down to 16 rows and 64 columns, while every tile is still
+  // another SM's (or two of them are one's, where rows are few and the time is that of reading the weights). The products are of 128 rows
+  // always: rows that are not copied are not written either, so that only copies and conversions get fewer.
   int64_t most = Tr::kMostN;
-  const auto tiles = [&] { return (ceil_div(rows.rows, c.tile_m) + std::min<int64_t>(groups, rows.rows) / 2) * ceil_div(num_n, most); };
+  const auto tiles = [&](int64_t m, int64_t n) { return (ceil_div(rows.rows, m) + std::min<int64_t>(groups, rows.rows) / 2) * ceil_div(num_n, n); };
   c.tile_m = kTileM;
   while (c.tile_m > 16 && c.tile_m >= 2 * ceil_div(rows.rows, groups)) c.tile_m /= 2;
-  const int64_t enough = c.tile_m < 64 ? 4 * kNumSMs : kNumSMs;
-  while (tiles() < enough && (most > 64 || c.tile_m > 16)) {
-    if (most > 64 && (most >= 2 * c.tile_m || c.tile_m == 16)) most /= 2;
-    else c.tile_m /= 2;
+  const int64_t enough = c.tile_m < 64 ? 2 * kNumSMs : kNumSMs;
+  for (;;) {
+    const bool columns = most > 64 && (most >= 2 * c.tile_m || c.tile_m == 16);
+    const int64_t m = columns ? c.tile_m : c.tile_m / 2, n = columns ? most / 2 : most;
+    if (m < 16 || tiles(m, n) > enough) break;
+    c.tile_m = (int)m, most = n;
   }
   c.tile_n = tile_columns(num_n, (int)most), c.tiles_n = (int)ceil_div(num_n, c.tile_n);
   c.a = rows.data, c.b = weight.data, c.pitch_a = rows.pitch, c.pitch_b = weight.pitch;
@@ -907,7 +1011,7 @@ static size_t linear_room(int64_t rows, int64_t dim, int64_t out_dim, int64_t gr
   size_t bytes = room_of(rows, dim, sizeof(T)) + room_of(groups * out_dim, dim, sizeof(T));
   if (backward) {
     const WeightPlan p = weight_plan<T>(rows, dim, out_dim, groups);
-    bytes += room_of(rows, out_dim, sizeof(T)) + align_up((size_t)(2 + 3 * p.ranges) * 8, 256) + (size_t)p.pieces * kTileM * (p.tile_n + 1) * 4;
+    bytes += room_of(rows, out_dim, sizeof(T)) + align_up((size_t)(2 + kPlanWords * p.ranges) * 8, 256) + (size_t)p.pieces * kTileM * (p.tile_n + 1) * 4;
   }
   return bytes;
 }
@@ -944,14 +1048,14 @@ static int linear_backward(const void* x, int64_t rows, int64_t dim, const void*
     c.a = dy.data, c.b = in.data, c.pitch_a = dy.pitch, c.pitch_b = in.pitch;
     c.out = grad_weight, c.grad_bias = grad_bias, c.status = status;
     c.plan = (int64_t*)room;
-    c.partial = (float*)(room + align_up((size_t)(2 + 3 * p.ranges) * 8, 256));
+    c.partial = (float*)(room + align_up((size_t)(2 + kPlanWords * p.ranges) * 8, 256));
     c.partial_bias = c.partial + (size_t)p.pieces * kTileM * p.tile_n;
     CUtensorMap a, b;
     if (const int e = make_map(&a, code_of<T>(), dy, Tr::kBox, Tr::kBlock)) return e;
     if (const int e = make_map(&b, code_of<T>(), in, Tr::kBox, Tr::kBlock)) return e;
     if (const int e = launch_grouped<T, kGradW>(c, a, b, p.ranges, s)) return e;
     if (p.ranges > 1) {
-      const dim3 grid((unsigned)ceil_div((int64_t)kTileM * c.tile_n / 4, 256), (unsigned)(p.ranges - 1));
+      const dim3 grid(kJoinParts, (unsigned)(p.ranges - 1));
       APT_FOLLOW((k_join_weights<T>), grid, 256, 0, s, c);
     }
   }

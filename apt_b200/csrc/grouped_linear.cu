@@ -205,14 +205,18 @@ __device__ __forceinline__ void take_rounds_apart(const char* from, char* to, in
   const int thread = threadIdx.x % kApartTeam, s = thread & 3, line = thread >> 2;      // a row, or a k
   const int at = line * 128, lo_at = at + (((2 * s) ^ (line & 7)) << 4), hi_at = at + (((2 * s + 1) ^ (line & 7)) << 4);
 #pragma unroll
-  for (int u = 0; u < U; ++u) lo[u] = *(const float4*)(from + lo_at + u * 4096), hi[u] = *(const float4*)(from + hi_at + u * 4096);
+  for (int u = 0; u < U; ++u) {
+    const int box = MN ? (u ^ (line & 1)) * 4096 : u * 4096;
+    lo[u] = *(const float4*)(from + lo_at + box), hi[u] = *(const float4*)(from + hi_at + box);
+  }
   const int to_at = MN ? line * 128 + ((s ^ (line & 7)) << 4) : line * 64 + ((s ^ ((line >> 1) & 3)) << 4);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (CUT && zero) lo[u] = hi[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const Pieces v = take_apart(lo[u], hi[u]);
-    // two rounds make a block of 64 across: the second has the other half of its slices
-    char* const p = to + (MN ? (to_at ^ (u & 1) << 6) + (u >> 1) * 4096 : to_at + u * 2048);
+    // two rounds make a block of 64 across, of two boxes: of neighbouring k's one is at the first box and one at the second, so that eight lanes
+    // read, and write, all banks of a row between them
+    char* const p = to + (MN ? (to_at ^ ((u ^ line) & 1) << 6) + (u >> 1) * 4096 : to_at + u * 2048);
 #pragma unroll
     for (int k = 0; k < 3; ++k) *(uint4*)(p + k * piece_bytes) = v.p[k];
   }
@@ -878,9 +882,18 @@ static int make_map(CUtensorMap* map, int dtype, const Operand& o, int box_colum
   const cuuint64_t dims[3] = {(cuuint64_t)o.columns, (cuuint64_t)o.rows, (cuuint64_t)o.stack};
   const cuuint64_t strides[2] = {(cuuint64_t)(o.pitch * size), (cuuint64_t)(o.rows * o.pitch * size)};
   const cuuint32_t box[3] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
-  const CUresult r = encode(map, dtype == APT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == APT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                            o.stack ? 3 : 2, (void*)o.data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const auto made = [&] {
+    return encode(map, dtype == APT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == APT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  o.stack ? 3 : 2, (void*)o.data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = made();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {      // a thread (the autograd engine's, say) that has not called the runtime yet
+    int device;
+    APT_CUDA(cudaGetDevice(&device));
+    APT_CUDA(cudaSetDevice(device));
+    r = made();
+  }
   if (r != CUDA_SUCCESS) {
     set_error("grouped_linear: cuTensorMapEncodeTiled -> %d (%lld x %lld, pitch %lld)", (int)r, (long long)o.rows, (long long)o.columns, (long long)o.pitch);
     return APT_ERR_CUDA;

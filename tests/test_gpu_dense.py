@@ -411,6 +411,27 @@ def test_another_stream_and_a_captured_graph():
     ops.check_status()
 
 
+def test_a_thread_that_has_not_used_the_gpu():
+    """The autograd engine's threads, or a caller's: nothing has bound them to the device's context yet."""
+    import threading
+
+    x, weight, offsets = torch.randn((64, 32), device="cuda"), torch.randn((1, 32, 32), device="cuda"), torch.tensor([0, 64], device="cuda")
+    want = apt_b200.grouped_linear(x, weight, offsets)
+    got = []
+
+    def call():
+        try:
+            got.append(apt_b200.grouped_linear(x, weight, offsets))
+        except RuntimeError as e:
+            got.append(e)
+
+    thread = threading.Thread(target=call)
+    thread.start()
+    thread.join()
+    assert torch.is_tensor(got[0]), got[0]
+    assert torch.equal(got[0], want)
+
+
 @pytest.mark.parametrize("ends", [[1, 5, 20], [0, 9, 5], [0, 5, 21], [-1, 5, 20], [0, -5, 2 ** 60]])
 def test_bad_offsets_are_reported(ends):
     offsets = torch.tensor(ends, device="cuda")

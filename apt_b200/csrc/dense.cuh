@@ -75,12 +75,21 @@ __device__ __forceinline__ float logistic(float z) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_short(-1.4426950408889634f * z)));
   return r;
 }
+// The normal distribution's mass below z, given q = exp(-z z / 2), which the density needs too: the upper tail is q / 2 times a polynomial in
+// 1 / (1 + 0.3275911 |z| / sqrt 2) (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: the error function to 1.5e-7).
+// 12 instructions where the library's error function takes 30 and a branch.
+__device__ __forceinline__ float normal_below(float z, float q) {
+  float t;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.23164189f, fabsf(z), 1.0f)));
+  const float tail = 0.5f * q * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  return z < 0.0f ? tail : 1.0f - tail;
+}
 // A NaN stays one, in relu too.
 template <int ACT>
 __device__ __forceinline__ float act_of(float z) {
   if constexpr (ACT == APT_ACT_RELU) return z < 0.0f ? 0.0f : z;
   if constexpr (ACT == APT_ACT_SILU) return z * logistic(z);
-  if constexpr (ACT == APT_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == APT_ACT_GELU) return z * normal_below(z, exp2_short(-0.72134752044448170f * z * z));
   return z;
 }
 template <int ACT>
@@ -90,8 +99,10 @@ __device__ __forceinline__ float act_slope(float z) {
     const float s = logistic(z);
     return fmaf(s * z, 1.0f - s, s);
   }
-  if constexpr (ACT == APT_ACT_GELU)
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * exp2_short(-0.72134752044448170f * z * z) * 0.39894228040143268f;
+  if constexpr (ACT == APT_ACT_GELU) {
+    const float q = exp2_short(-0.72134752044448170f * z * z);
+    return fmaf(0.39894228040143268f * z, q, normal_below(z, q));
+  }
   return 1.0f;
 }
 

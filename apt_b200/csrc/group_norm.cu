@@ -70,6 +70,7 @@ static NormPlan norm_plan(const NormShape& s, size_t size, uintptr_t addresses, 
   t.join_groups = 1;
   while (t.join_groups < 64 && t.join_groups < s.groups && 256 / (2 * t.join_groups) >= t.sum_tiles / s.segments + 1) t.join_groups *= 2;
   t.join_groups = std::max(t.join_groups, std::min(4, s.groups));
+  t.join_segments = s.segments >= kNumSMs * 8 ? 8 : 1;
   p.blocks = ceil_div(t.sum_tiles, 256 / team);
   return p;
 }

@@ -397,39 +397,80 @@ struct NormTiles {
   int64_t apply_rows, apply_tiles;    // of k_norm_apply
   int chunk;                          // groups of a team
   int slots, lines;                   // threads side by side in a row, rows side by side
-  int join_groups;                    // groups of a block of k_norm_join
+  int join_groups, join_segments;     // of a block of k_norm_join
 };
 
 // GN: groups that a slice may have channels of (1 where a group is whole slices).
 template <int VE, int NC, int GN>
 struct NormThread {
   int slot, line, group0, groups, per, col0;
-  bool mine;
+  bool mine, even;      // even: sum_groups
   bool in[NC];
   int col[NC];
   uint16_t group[NC][GN];        // within the team's
+  uint32_t heads;                // channels that are their group's first
   __device__ __forceinline__ NormThread(const NormShape& s, const NormTiles& t, int thread) {
     slot = thread % t.slots, line = thread / t.slots;
     mine = line < t.lines;
     group0 = blockIdx.y * t.chunk, groups = min(t.chunk, s.groups - group0), per = s.per, col0 = group0 * s.per;
+    const int slices = per / VE;
+    heads = 0;
+    even = 32 % t.slots == 0 && (GN == 1 ? (slices & (slices - 1)) == 0 && slices <= t.slots : per == 1);
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
       const int k = (slot + j * t.slots) * VE;
       in[j] = mine && k < groups * per;
       col[j] = col0 + k;
 #pragma unroll
-      for (int i = 0; i < GN; ++i) group[j][i] = in[j] ? (uint16_t)((k + i) / per) : 0;
+      for (int i = 0; i < GN; ++i) {
+        group[j][i] = in[j] ? (uint16_t)((k + i) / per) : 0;
+        if (in[j] && (k + i) % per == 0) heads |= 1u << (j * GN + i);
+      }
     }
   }
 };
 
-// Sums of K numbers over the rows and each group from per-thread sums a channel, into result[group][k]; by all threads of a block, or of
-// a warp with shared memory of its own.
+// Sums of K numbers over the rows and each group from per-thread sums a channel, by all threads of a block, or of a warp: got[k] of the groups that
+// a thread has channels of. Between lanes directly where a warp's rows and a group's slices are powers of two (`even`); else through
+// shared memory (`room`, `result`: a team's own).
 template <int VE, int NC, int GN, int K, bool WARP>
-__device__ __forceinline__ void sum_groups(const float (&v)[K][NC][VE], float* room, float* result, const NormThread<VE, NC, GN>& me, int slots, int lines) {
+__device__ __forceinline__ void sum_groups(const float (&v)[K][NC][VE], float (&got)[K][NC][GN], float* room, float* result, const NormThread<VE, NC, GN>& me, int slots,
+                                           int lines) {
   // a slice of one group is one number
   constexpr int kOwn = GN == 1 ? 1 : VE;
   const int columns = slots * NC * kOwn, pitch = columns + 1, per = GN == 1 ? me.per / VE : me.per, lane = threadIdx.x % 32;
+  float own[K][NC][kOwn];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      if constexpr (kOwn == 1) {
+        own[k][j][0] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) own[k][j][0] += v[k][j][i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) own[k][j][i] = v[k][j][i];
+      }
+    }
+  if (WARP && me.even) {
+    for (int o = 16; o; o >>= 1) {
+      if (o < slots && (GN > 1 || o >= per)) continue;      // between rows, or within a group
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+          for (int i = 0; i < kOwn; ++i) own[k][j][i] += __shfl_xor_sync(0xffffffffu, own[k][j][i], o);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int i = 0; i < GN; ++i) got[k][j][i] = own[k][j][i];
+    return;
+  }
   const auto sync = [] {
     if (WARP) __syncwarp(); else __syncthreads();
   };
@@ -438,24 +479,16 @@ __device__ __forceinline__ void sum_groups(const float (&v)[K][NC][VE], float* r
     sync();
     if (me.mine)
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        if constexpr (kOwn == 1) {
-          float sum = 0.0f;
+      for (int j = 0; j < NC; ++j)
 #pragma unroll
-          for (int i = 0; i < VE; ++i) sum += v[k][j][i];
-          room[me.line * pitch + me.slot + j * slots] = sum;
-        } else {
-#pragma unroll
-          for (int i = 0; i < VE; ++i) room[me.line * pitch + (me.slot + j * slots) * VE + i] = v[k][j][i];
-        }
-      }
+        for (int i = 0; i < kOwn; ++i) room[me.line * pitch + (me.slot + j * slots) * kOwn + i] = own[k][j][i];
     sync();
     if (WARP && me.groups > 8) {
       for (int g = lane; g < me.groups; g += 32) {
         float sum = 0.0f;
         for (int r = 0; r < lines; ++r)
           for (int i = 0; i < per; ++i) sum += room[r * pitch + g * per + i];
-        result[g * K + k] = sum;
+        result[g] = sum;
       }
     } else {
       for (int g = WARP ? 0 : threadIdx.x / 32; g < me.groups; g += WARP ? 1 : 8) {
@@ -470,11 +503,25 @@ __device__ __forceinline__ void sum_groups(const float (&v)[K][NC][VE], float* r
           for (int i = lane; i < lines * per; i += 32) sum += room[i / per * pitch + g * per + i % per];
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) result[g * K + k] = sum;
+        if (lane == 0) result[g] = sum;
       }
     }
+    sync();
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int i = 0; i < GN; ++i) got[k][j][i] = result[me.group[j][i]];
   }
-  sync();
+}
+// Two numbers of each group to `to`, by the thread that has a group's first channel in the first row.
+template <int VE, int NC, int GN>
+__device__ __forceinline__ void put_groups(float2* to, const float (&a)[NC][GN], const float (&b)[NC][GN], const NormThread<VE, NC, GN>& me) {
+  if (me.line) return;
+#pragma unroll
+  for (int j = 0; j < NC; ++j)
+#pragma unroll
+    for (int i = 0; i < GN; ++i)
+      if (me.heads >> (j * GN + i) & 1) to[me.group[j][i]] = make_float2(a[j][i], b[j][i]);
 }
 
 // (v - mean) / deviation of a slice.
@@ -538,9 +585,9 @@ __global__ void __launch_bounds__(256, BACK ? 2 : 3)
 k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t) {
   wait_for_previous();
   constexpr int kRoom = (WARP ? 32 : 256) * (NC * VE + 1), kGroups = WARP ? 256 : kMostGroups;
-  __shared__ float rooms[(WARP ? 8 : 1) * kRoom], results[(WARP ? 8 : 1) * kGroups * 2];
-  const int team = WARP ? threadIdx.x / 32 : 0, thread = WARP ? threadIdx.x % 32 : threadIdx.x, size = WARP ? 32 : 256;
-  float *const room = rooms + team * kRoom, *const result = results + team * kGroups * 2;
+  __shared__ float rooms[(WARP ? 8 : 1) * kRoom], results[(WARP ? 8 : 1) * kGroups];
+  const int team = WARP ? threadIdx.x / 32 : 0, thread = WARP ? threadIdx.x % 32 : threadIdx.x;
+  float *const room = rooms + team * kRoom, *const result = results + team * kGroups;
   const NormThread<VE, NC, GN> me(s, t, thread);
   const T* const x = (const T*)c.x;
   const T* const grad = (const T*)c.grad;
@@ -597,17 +644,22 @@ k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
       for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int i = 0; i < VE; ++i) own[0][j][i] = me.in[j] ? v[0][j][i] * n : 0.0f;
-      sum_groups<VE, NC, GN, 1, WARP>(own, room, result, me, t.slots, t.lines);
-      const float share = 1.0f / ((float)(e - b) * (float)me.per);
+      float sums[1][NC][GN], squares[1][NC][GN];
+      sum_groups<VE, NC, GN, 1, WARP>(own, sums, room, result, me, t.slots, t.lines);
+      const float share = __fdividef(1.0f, (float)(e - b) * (float)me.per);
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int i = 0; i < GN; ++i) sums[0][j][i] *= share;
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-          const float d = v[0][j][i] - result[me.group[j][i % GN]] * share;
+          const float d = v[0][j][i] - sums[0][j][i % GN];
           own[0][j][i] = me.in[j] ? fmaf(n * d, d, q[j][i]) : 0.0f;
         }
-      sum_groups<VE, NC, GN, 1, WARP>(own, room, result + kGroups, me, t.slots, t.lines);
-      for (int g = thread; g < me.groups; g += size) parts[g] = make_float2(result[g] * share, result[kGroups + g]);
+      sum_groups<VE, NC, GN, 1, WARP>(own, squares, room, result, me, t.slots, t.lines);
+      put_groups(parts, sums[0], squares[0], me);
     } else {
       float2 st[NC][GN];
       load_stats(s, c.stats, me, seg, st);
@@ -650,10 +702,10 @@ k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
           // one rounding, as of a single row's
           ab[0][j][i] = __fmul_rn(ab[0][j][i], gamma[j][i]), ab[1][j][i] *= gamma[j][i];
         }
-      sum_groups<VE, NC, GN, 2, WARP>(ab, room, result, me, t.slots, t.lines);
-      for (int g = thread; g < me.groups; g += size) parts[g] = make_float2(result[2 * g], result[2 * g + 1]);
+      float sums[2][NC][GN];
+      sum_groups<VE, NC, GN, 2, WARP>(ab, sums, room, result, me, t.slots, t.lines);
+      put_groups(parts, sums[0], sums[1], me);
     }
-    if (WARP) __syncwarp(); else __syncthreads();      // `result` is the next piece's
   }
   if constexpr (BACK) {
     if (!c.columns) return;
@@ -662,8 +714,41 @@ k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
   }
 }
 
-// The pieces of each segment joined, a block for some groups of a segment: forwards mean and 1 / deviation (zeros for a segment without rows),
-// backwards the two means. The first `joins` blocks join the columns' sums for dgamma and dbeta. Offsets that are none are flagged here.
+// The pieces of each segment joined: forwards mean and 1 / deviation (zeros for a segment without rows), backwards the two means. A block has
+// some groups of a segment; or, where there are many segments, eight of them, a warp each, and all of its threads those that turn out to
+// be long. The first `joins` blocks join the columns' sums for dgamma and dbeta. Offsets that are none are flagged here.
+struct NormPieces {
+  const float2* parts;
+  int64_t first, last, tile, pitch;
+  RowRange rows;
+  float per, inv;
+  __device__ __forceinline__ NormPieces(const NormShape& s, const NormCall& c, const NormTiles& t, int64_t seg, const RowRange& r)
+      : parts(c.parts + seg * s.groups), first(r.begin / t.sum_rows), last((r.end - 1) / t.sum_rows), tile(t.sum_rows), pitch(s.groups), rows(r),
+        per((float)s.per), inv(1.0f / ((float)(r.end - r.begin) * (float)s.per)) {}
+  __device__ __forceinline__ float count(int64_t i) const { return (float)(min((i + 1) * tile, rows.end) - max(i * tile, rows.begin)) * per; }
+  // of every step-th piece: the backward's sums, or the sum of the means
+  template <bool BACK>
+  __device__ __forceinline__ float2 sums(int g, int64_t from, int64_t step) const {
+    float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for (int64_t i = from; i <= last; i += step) {
+      const float2 p = parts[i * pitch + g];
+      if constexpr (BACK) v.x += p.x, v.y += p.y;
+      else v.x = fmaf(p.x, count(i), v.x);
+    }
+    return v;
+  }
+  __device__ __forceinline__ float squares(int g, int64_t from, int64_t step, float mean) const {
+    float q = 0.0f;
+#pragma unroll 4
+    for (int64_t i = from; i <= last; i += step) {
+      const float2 p = parts[i * pitch + g];
+      q += fmaf(count(i) * (p.x - mean), p.x - mean, p.y);
+    }
+    return q;
+  }
+};
+constexpr int kFewPieces = 16;
 template <typename T, bool BACK>
 __global__ void __launch_bounds__(256)
 k_norm_join(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t, int joins, int64_t lines) {
@@ -673,50 +758,70 @@ k_norm_join(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
     return;
   }
   __shared__ float2 part[256];
-  const int64_t seg = blockIdx.x - joins;
-  const RowRange r = segment_rows(s, seg);
-  if (!BACK && s.offsets && blockIdx.y == 0 && threadIdx.x == 0 && bad_group(s.offsets, (int)seg, s.rows)) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
-  const int width = t.join_groups, g = blockIdx.y * width + threadIdx.x % width, lane = threadIdx.x / width, lanes = 256 / width;
-  const bool mine = g < s.groups && lane < lanes;
   float2* const to = BACK ? c.means : c.stats;
-  if (r.end <= r.begin) {
-    if (mine && lane == 0) to[seg * s.groups + g] = make_float2(0.0f, 0.0f);
-    return;
-  }
-  const int64_t first = r.begin / t.sum_rows, last = (r.end - 1) / t.sum_rows;
-  const float2* const parts = c.parts + seg * s.groups + g;
-  const float inv = 1.0f / ((float)(r.end - r.begin) * (float)s.per);
-  const auto count = [&](int64_t i) { return (float)(min((i + 1) * t.sum_rows, r.end) - max(i * t.sum_rows, r.begin)) * (float)s.per; };
-  const auto together = [&](float2 v) {
-    __syncthreads();
-    if (mine) part[threadIdx.x] = v;
-    __syncthreads();
-    v = make_float2(0.0f, 0.0f);
-    if (mine)
-      for (int k = 0; k < lanes; ++k) v.x += part[k * width + threadIdx.x % width].x, v.y += part[k * width + threadIdx.x % width].y;
-    return v;
+  const auto put = [&](int64_t seg, int g, float a, float b, float inv) {
+    to[seg * s.groups + g] = make_float2(a, BACK ? b * inv : rsqrtf(b * inv + c.eps));
   };
-  float2 v = make_float2(0.0f, 0.0f);
-  if (mine)
-#pragma unroll 4
-    for (int64_t i = first + lane; i <= last; i += lanes) {
-      const float2 p = parts[i * s.groups];
-      if constexpr (BACK) v.x += p.x, v.y += p.y;
-      else v.x = fmaf(p.x, count(i), v.x);
+  const int64_t block = blockIdx.x - joins;
+  uint32_t rest = 1;      // of the block's segments, for all its threads
+  if (t.join_segments > 1) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int64_t seg = block * t.join_segments + warp;
+    int many = 0;
+    if (seg < s.segments) {
+      const RowRange r = segment_rows(s, seg);
+      if (!BACK && s.offsets && lane == 0 && bad_group(s.offsets, (int)seg, s.rows)) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
+      const NormPieces p(s, c, t, seg, r);
+      many = r.end > r.begin && p.last - p.first >= kFewPieces;
+      if (!many)
+        for (int g = lane; g < s.groups; g += 32) {
+          if (r.end <= r.begin) {
+            to[seg * s.groups + g] = make_float2(0.0f, 0.0f);
+            continue;
+          }
+          const float2 v = p.sums<BACK>(g, p.first, 1);
+          const float mean = v.x * p.inv;
+          put(seg, g, mean, BACK ? v.y : p.squares(g, p.first, 1, mean), p.inv);
+        }
     }
-  v = together(v);
-  const float mean = v.x * inv;
-  if constexpr (!BACK) {
-    v = make_float2(0.0f, 0.0f);
-    if (mine)
-#pragma unroll 4
-      for (int64_t i = first + lane; i <= last; i += lanes) {
-        const float2 p = parts[i * s.groups];
-        v.y += fmaf(count(i) * (p.x - mean), p.x - mean, p.y);
-      }
-    v = together(v);
+    if (!__syncthreads_or(many)) return;
+    __shared__ uint32_t long_ones;
+    if (threadIdx.x == 0) long_ones = 0;
+    __syncthreads();
+    if (many && lane == 0) atomicOr(&long_ones, 1u << warp);
+    __syncthreads();
+    rest = long_ones;
   }
-  if (mine && lane == 0) to[seg * s.groups + g] = make_float2(mean, BACK ? v.y * inv : rsqrtf(v.y * inv + c.eps));
+  for (; rest; rest &= rest - 1) {
+    const int64_t seg = block * t.join_segments + __ffs(rest) - 1;
+    const RowRange r = segment_rows(s, seg);
+    if (!BACK && t.join_segments == 1 && s.offsets && blockIdx.y == 0 && threadIdx.x == 0 && bad_group(s.offsets, (int)seg, s.rows))
+      atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
+    const NormPieces p(s, c, t, seg, r);
+    const int width = t.join_groups, lane = threadIdx.x / width, lanes = 256 / width;
+    for (int g0 = blockIdx.y * width; g0 < s.groups; g0 += gridDim.y * width) {
+      const int g = g0 + threadIdx.x % width;
+      const bool mine = g < s.groups && lane < lanes;
+      if (r.end <= r.begin) {
+        if (mine && lane == 0) to[seg * s.groups + g] = make_float2(0.0f, 0.0f);
+        continue;
+      }
+      const auto together = [&](float2 v) {
+        __syncthreads();
+        if (mine) part[threadIdx.x] = v;
+        __syncthreads();
+        v = make_float2(0.0f, 0.0f);
+        if (mine)
+          for (int k = 0; k < lanes; ++k) v.x += part[k * width + threadIdx.x % width].x, v.y += part[k * width + threadIdx.x % width].y;
+        return v;
+      };
+      const float2 v = together(mine ? p.sums<BACK>(g, p.first + lane, lanes) : make_float2(0.0f, 0.0f));
+      const float mean = v.x * p.inv;
+      float q = v.y;
+      if constexpr (!BACK) q = together(make_float2(0.0f, mine ? p.squares(g, p.first + lane, lanes, mean) : 0.0f)).y;
+      if (mine && lane == 0) put(seg, g, mean, q, p.inv);
+    }
+  }
 }
 
 // The rows themselves, and zeros for rows of no segment. Tiles from the last to the first: what k_norm_sums read last is still in L2.
@@ -921,7 +1026,7 @@ static int norm_tiles(const NormShape& s, const NormCall& c, const NormPlan& p, 
   const dim3 sums((unsigned)p.blocks, (unsigned)p.chunks), apply((unsigned)ceil_div(t.apply_tiles, WARP ? 8 : 1), (unsigned)p.chunks);
   APT_FOLLOW((k_norm_sums<T, VE, NC, GN, BACK, WARP>), sums, 256, 0, st, s, c, t);
   const int joins = BACK && c.columns ? (int)ceil_div(2 * s.dim, 32) : 0;
-  const dim3 join((unsigned)(joins + s.segments), (unsigned)ceil_div(s.groups, t.join_groups));
+  const dim3 join((unsigned)(joins + ceil_div(s.segments, t.join_segments)), t.join_segments > 1 ? 1u : (unsigned)ceil_div(s.groups, t.join_groups));
   APT_FOLLOW((k_norm_join<T, BACK>), join, 256, 0, st, s, c, t, joins, p.blocks);
   APT_FOLLOW((k_norm_apply<T, VE, NC, GN, BACK, WARP>), apply, 256, 0, st, s, c, t);
   return APT_OK;

@@ -12,6 +12,17 @@ pytestmark = pytest.mark.gpu
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
 
 
+@pytest.fixture(autouse=True)
+def _state_as_before():
+    """The graph and the feature table that a test installs go with it: other tests' samplers look rows up in whatever is installed."""
+    state = ops.STATE
+    before = state.feat, state.graph
+    state.feat, state.graph = ops.FeatStorage(), ops.GraphStorage()
+    yield
+    state.feat, state.graph = before
+    state.generation += 1
+
+
 def test_a_layer_and_its_gradients():
     import typed_sage
 

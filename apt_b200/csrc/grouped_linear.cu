@@ -740,8 +740,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(&kept_free), (kept_times & 1) ^ 1, gave_up));
         ++kept_times;
         for (int k = 0; fine && k < kept_stages; ++k, next_from()) {
-          if ((k & 1) != team) continue;
+          // the other team's stages too: a wait for a phase is one only where the phase before is known to be over
           if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up)))) break;
+          if ((k & 1) != team) continue;
           take_stage_apart<Tr::kMnB, false>(copied + (size_t)from * copied_bytes, kept + (size_t)k * kept_bytes, c.tile_n, piece_b, Tr::kBlock);
           __syncwarp();
           if (lane == 0) barrier_arrive(shared_addr(free_ + from));
@@ -753,7 +754,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       }
       for (int k = 0; k < item.stages; ++k, turn ^= 1, next_from()) {
         if (turn != team) continue;      // each team has a stage of pieces of its own
-        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up) && barrier_wait(shared_addr(used + team), uses ^ 1, gave_up));
+        // first the products of the team's stage before: they came behind those of all earlier ones, so that what the ring's place held before
+        // has arrived, and the wait for its next phase is one
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(used + team), uses ^ 1, gave_up) && barrier_wait(shared_addr(full + from), from_phase, gave_up));
         if (!fine) break;
         const char* const in = copied + (size_t)from * copied_bytes;
         char* const out = pieces + (size_t)team * piece_bytes;

@@ -411,6 +411,25 @@ def test_another_stream_and_a_captured_graph():
     ops.check_status()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_again_and_again(dtype):
+    """The same bits every time, from the first call on and with the cache full of something else: nothing is read before it is there."""
+    gen = _gen(17)
+    offsets, rows = _offsets([7000, 0, 9000, 4001])
+    make = lambda *shape: torch.randn(shape, device="cuda", generator=gen).to(dtype)
+    x, weight, bias, grad = make(rows, 328), make(4, 88, 328), make(4, 88), make(rows, 88)
+    other = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    first = None
+    for k in range(60):
+        if k % 2:
+            other.fill_(k)
+        got = (apt_b200.grouped_linear(x, weight, offsets, bias),) + apt_b200.grouped_linear_backward(x, weight, offsets, grad)
+        first = first or got
+        for a, b in zip(got, first):
+            assert torch.equal(a, b), k
+    ops.check_status()
+
+
 def test_a_thread_that_has_not_used_the_gpu():
     """The autograd engine's threads, or a caller's: nothing has bound them to the device's context yet."""
     import threading

@@ -58,10 +58,10 @@ static NormPlan norm_plan(const NormShape& s, size_t size, uintptr_t addresses, 
   p.held = slices <= team ? 1 : 8 / p.slice;
   t.slots = (int)ceil_div(slices, p.held);
   t.lines = team / t.slots;
-  // a round of blocks each, two or three an SM (registers), of four rounds of rows at least
+  // a round of blocks each, two or three an SM (registers)
   const auto tiles_of = [&](int per_sm, int64_t* rows, int64_t* tiles) {
     const int64_t teams = ceil_div(kNumSMs * per_sm, p.chunks) * (256 / team);
-    *rows = std::max<int64_t>(4 * t.lines, ceil_div(ceil_div(s.rows, teams), t.lines) * t.lines);
+    *rows = ceil_div(ceil_div(s.rows, teams), t.lines) * t.lines;
     *tiles = ceil_div(s.rows, *rows);
   };
   tiles_of(back ? 2 : 3, &t.sum_rows, &t.sum_tiles);

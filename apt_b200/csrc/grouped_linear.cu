@@ -286,6 +286,32 @@ __device__ __forceinline__ void add_columns(const char* stage, int valid, int th
 }
 
 // ---- bringing a tile out -------------------------------------------------------------
+// 32 rows of 128 bytes from shared memory to `to`, `rows` of them and of each the first `columns` elements, where rows are no whole 16-byte
+// slices: in words as wide as rows are aligned to. Eight words a lane are read before any is stored: the compiler does not know that the
+// stores go elsewhere. Not inlined, nor unrolled further: it would take the registers of every tile.
+template <typename O, typename W>
+__device__ __noinline__ void put_narrow_rows(const char* staging, int lane, O* to, int64_t ld, int rows, int columns) {
+  constexpr int kLanes = 128 / sizeof(W) < 32 ? 128 / (int)sizeof(W) : 32, kSide = 32 / kLanes;      // lanes of a row, rows at once
+  const int r0 = lane / kLanes;
+#pragma unroll 1
+  for (int at = lane % kLanes * (int)sizeof(W); at < 128; at += kLanes * (int)sizeof(W)) {
+    const int col = at / (int)sizeof(O);
+    if (col >= columns) break;
+    O* p = to + r0 * ld + col;
+#pragma unroll 1
+    for (int k0 = r0; k0 < rows; k0 += 8 * kSide) {
+      W word[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int r = k0 + k * kSide;
+        word[k] = *(const W*)(staging + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15));
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k, p += kSide * ld)
+        if (k0 + k * kSide < rows) *(W*)p = word[k];
+    }
+  }
+}
 // A warp's 32 rows, 128 bytes of each at a time, through shared memory, so that the stores are whole rows of 128 bytes. Warps that share
 // rows take turns.
 template <typename T, typename O, int MODE>
@@ -361,12 +387,12 @@ __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedIt
 #pragma unroll
       for (int k = 0; k < 8; ++k, to += 4 * ld)
         if (4 * k < rows_left) *(uint4*)to = slice[k];
-    } else {
-      for (int r = 0; r < here; ++r)
-        for (int k = lane; k < kWide; k += 32) {
-          const int s = k * (int)sizeof(O) / 16, in = k * (int)sizeof(O) % 16;
-          if (c0 + k < columns) first[r * ld + c0 + k] = *(const O*)(staging + r * 128 + ((s ^ (r & 7)) << 4) + in);
-        }
+    } else if (ld * (int64_t)sizeof(O) % 8 == 0) {
+      put_narrow_rows<O, uint2>(staging, lane, first + c0, ld, here, columns - c0);
+    } else if (ld * (int64_t)sizeof(O) % 4 == 0) {
+      put_narrow_rows<O, uint32_t>(staging, lane, first + c0, ld, here, columns - c0);
+    } else if constexpr (sizeof(O) == 2) {
+      put_narrow_rows<O, uint16_t>(staging, lane, first + c0, ld, here, columns - c0);
     }
     __syncwarp();
   }

@@ -13,7 +13,8 @@ namespace apt {
 //
 // What the first two rounds make of the numbers that are the same for all elements (the call, the tag, and the upper word of the quad's
 // number while it is 0) is worked out on the host, and so are the rounds' keys: 18 products and 19 logical operations a quad instead of 20,
-// 20 and 20 additions. The products go at half the rate of others and every one counts: 151552 x 256 bf16, both ways, 81 -> 59 us.
+// 20 and 20 additions (151552 x 256 bf16, both ways: 81 -> 79 us). A product of 32 by 32 bits takes its pipe for four cycles a warp, so that the
+// words alone of that matrix are 29 us, as long as reading and writing it; the upper half from a product in 64-bit floating point took 33.
 struct Drop {
   uint32_t k0[10], k1[10];      // the rounds' keys
   uint32_t a0, a1, a2;          // behind the first round: the first word but for the quad's upper one, the second, part of the third

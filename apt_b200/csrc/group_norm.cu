@@ -10,9 +10,9 @@ extern template int norm<__nv_bfloat16, true>(const NormShape&, const NormCall&,
 extern template int norm<__half, false>(const NormShape&, const NormCall&, const NormPlan&, cudaStream_t);
 extern template int norm<__half, true>(const NormShape&, const NormCall&, const NormPlan&, cudaStream_t);
 
-// Elements of an access that `run` elements from any of the addresses on are a whole number of: 16 or 4 bytes, or one.
+// Elements of an access that `run` elements from any of the addresses on are a whole number of: 16, 8 or 4 bytes, or one.
 static int slice_of(int64_t run, size_t size, uintptr_t addresses) {
-  for (const int bytes : {16, 4})
+  for (const int bytes : {16, 8, 4})
     if (bytes > (int)size && (run * (int64_t)size) % bytes == 0 && addresses % bytes == 0) return bytes / (int)size;
   return 1;
 }
@@ -37,22 +37,30 @@ static NormPlan norm_plan(const NormShape& s, size_t size, uintptr_t addresses, 
       return p;
     }
   }
+  NormTiles& t = p.tiles;
   p.slice = slice_of(s.dim, size, addresses);
-  // a block has whole groups, a chunk of them that begins on an access
-  int chunk = s.groups;
-  if (s.dim > kMostColumns || s.groups > kMostColumns / 4) {
-    chunk = std::min<int>(kMostColumns / s.per, kMostColumns / 4);
-    while (chunk > 0 && (int64_t)chunk * s.per % p.slice) --chunk;
+  // a group wider than a block's columns is cut into equal parts; rows by themselves that come here stay a block's, walk by walk
+  t.fold = 1;
+  if (s.per > kMostColumns && (s.offsets || s.per_segment > 1)) {
+    t.fold = (int)ceil_div(s.per, kMostColumns);
+    while (s.per / t.fold >= 64 && s.per % (t.fold * p.slice)) ++t.fold;
   }
-  const int64_t slices = chunk > 0 ? ceil_div((int64_t)std::min(chunk, s.groups) * s.per, p.slice) : 0;
-  if (chunk <= 0 || slices > 256 * (8 / p.slice) || s.segments == 0) {
+  const int per = s.per / t.fold, groups = s.groups * t.fold;
+  // a block has whole groups (or parts), a chunk of them that begins on an access
+  int chunk = groups;
+  if (s.dim > kMostColumns || groups > kMostColumns / 4) {
+    chunk = std::min<int>(kMostColumns / per, kMostColumns / 4);
+    while (chunk > 0 && (int64_t)chunk * per % p.slice) --chunk;
+  }
+  const int64_t slices = chunk > 0 ? ceil_div((int64_t)std::min(chunk, groups) * per, p.slice) : 0;
+  if (chunk <= 0 || per * t.fold != s.per || slices > 256 * (8 / p.slice) || s.segments == 0) {
     p.kind = kNormWide;
+    p.blocks = std::max<int64_t>(1, std::min<int64_t>(ceil_div(s.rows, 32), kNumSMs * 8 / ceil_div(s.dim, 256)));
     return p;
   }
   p.kind = kNormTiles;
-  NormTiles& t = p.tiles;
   t.chunk = chunk;
-  p.chunks = ceil_div(s.groups, chunk);
+  p.chunks = ceil_div(groups, chunk);
   p.warps = p.chunks == 1 && slices <= 32 * (8 / p.slice);
   const int team = p.warps ? 32 : 256;
   p.held = slices <= team ? 1 : 8 / p.slice;
@@ -65,7 +73,7 @@ static NormPlan norm_plan(const NormShape& s, size_t size, uintptr_t addresses, 
     *tiles = ceil_div(s.rows, *rows);
   };
   tiles_of(back ? 2 : 3, &t.sum_rows, &t.sum_tiles);
-  tiles_of(p.held > 1 || s.per % p.slice ? 2 : 3, &t.apply_rows, &t.apply_tiles);
+  tiles_of(p.held > 1 || per % p.slice ? 2 : 3, &t.apply_rows, &t.apply_tiles);
   // threads for all pieces of a mean segment, or a number of them
   t.join_groups = 1;
   while (t.join_groups < 64 && t.join_groups < s.groups && 256 / (2 * t.join_groups) >= t.sum_tiles / s.segments + 1) t.join_groups *= 2;
@@ -82,8 +90,8 @@ struct NormRoom {
 };
 static NormRoom norm_room(const NormShape& s, const NormPlan& p, bool back) {
   const bool tiles = p.kind == kNormTiles;
-  return {back && p.kind != kNormWide ? align_up((size_t)p.blocks * 2 * s.dim * 4, 256) : 0,
-          tiles ? align_up((size_t)(p.tiles.sum_tiles + s.segments) * s.groups * 8, 256) : 0,
+  return {back ? align_up((size_t)p.blocks * 2 * s.dim * 4, 256) : 0,
+          tiles ? align_up((size_t)(p.tiles.sum_tiles + s.segments) * s.groups * p.tiles.fold * 8, 256) : 0,
           back && tiles ? align_up((size_t)s.segments * s.groups * 8, 256) : 0, back && tiles && p.slice % 4 == 0 ? (size_t)(s.rows * s.dim) / p.slice : 0};
 }
 
@@ -118,7 +126,7 @@ extern "C" size_t apt_group_norm_workspace_bytes(int dtype, int64_t rows, int64_
   // buffers that begin anywhere may take narrower accesses
   const NormShape s = norm_shape(rows, dim, groups, offsets, segments);
   size_t most = 0;
-  for (const uintptr_t addresses : {0, 4, 2}) most = std::max(most, norm_room(s, norm_plan(s, dtype == APT_F32 ? 4 : 2, addresses, backward), backward).all());
+  for (const uintptr_t addresses : {0, 8, 4, 2}) most = std::max(most, norm_room(s, norm_plan(s, dtype == APT_F32 ? 4 : 2, addresses, backward), backward).all());
   return most;
 }
 

@@ -395,6 +395,7 @@ constexpr int kMostGroups = 512;        // of a block
 struct NormTiles {
   int64_t sum_rows, sum_tiles;        // of k_norm_sums, whose tiles the pieces are of
   int64_t apply_rows, apply_tiles;    // of k_norm_apply
+  int fold;                           // parts of a group that the kernels take for groups (those that are wider than a block's columns)
   int chunk;                          // groups of a team
   int slots, lines;                   // threads side by side in a row, rows side by side
   int join_groups, join_segments;     // of a block of k_norm_join
@@ -548,7 +549,15 @@ __device__ __forceinline__ void load_params(const NormCall& c, const NormThread<
     }
 }
 template <int VE, int NC, int GN>
-__device__ __forceinline__ void load_stats(const NormShape& s, const float2* stats, const NormThread<VE, NC, GN>& me, int64_t seg, float2 (&st)[NC][GN]) {
+__device__ __forceinline__ void load_stats(const NormShape& s, const NormTiles& t, const float2* stats, const NormThread<VE, NC, GN>& me, int64_t seg,
+                                           float2 (&st)[NC][GN]) {
+  if (t.fold > 1) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int i = 0; i < GN; ++i) st[j][i] = stats[seg * (s.groups / t.fold) + (me.group0 + me.group[j][i]) / t.fold];
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < NC; ++j)
 #pragma unroll
@@ -579,7 +588,7 @@ __device__ __forceinline__ void put_columns(const NormShape& s, const NormCall& 
 
 // Sums of each tile's rows, piece by piece (the rows a tile has of a segment): piece number tile + segment, which no other has. Forwards the mean
 // and the squares around it, backwards the sums of dxh and dxh xh.
-// 151552 x 256 bf16 in 8 segments, us: forwards FWD_SUMS (HBM: 12), backwards BWD_SUMS (24), where the dropout's generator binds.
+// 151552 x 256 bf16 in 8 segments, us: forwards 23 (HBM: 12), backwards 84 (24), where silu and the dropout's generator bind.
 template <typename T, int VE, int NC, int GN, bool BACK, bool WARP>
 __global__ void __launch_bounds__(256, BACK ? 2 : 3)
 k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t) {
@@ -662,7 +671,7 @@ k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
       put_groups(parts, sums[0], squares[0], me);
     } else {
       float2 st[NC][GN];
-      load_stats(s, c.stats, me, seg, st);
+      load_stats(s, t, c.stats, me, seg, st);
       float ab[2][NC][VE];
 #pragma unroll
       for (int j = 0; j < NC; ++j)
@@ -720,31 +729,34 @@ k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
 struct NormPieces {
   const float2* parts;
   int64_t first, last, tile, pitch;
+  int fold;
   RowRange rows;
   float per, inv;
   __device__ __forceinline__ NormPieces(const NormShape& s, const NormCall& c, const NormTiles& t, int64_t seg, const RowRange& r)
-      : parts(c.parts + seg * s.groups), first(r.begin / t.sum_rows), last((r.end - 1) / t.sum_rows), tile(t.sum_rows), pitch(s.groups), rows(r),
-        per((float)s.per), inv(1.0f / ((float)(r.end - r.begin) * (float)s.per)) {}
+      : parts(c.parts + seg * s.groups), first(r.begin / t.sum_rows), last((r.end - 1) / t.sum_rows), tile(t.sum_rows), pitch(s.groups), fold(t.fold), rows(r),
+        per((float)s.per), inv(1.0f / ((float)(r.end - r.begin) * (float)s.per * (float)t.fold)) {}
   __device__ __forceinline__ float count(int64_t i) const { return (float)(min((i + 1) * tile, rows.end) - max(i * tile, rows.begin)) * per; }
   // of every step-th piece: the backward's sums, or the sum of the means
   template <bool BACK>
   __device__ __forceinline__ float2 sums(int g, int64_t from, int64_t step) const {
     float2 v = make_float2(0.0f, 0.0f);
+    for (int f = g * fold; f < (g + 1) * fold; ++f)
 #pragma unroll 4
-    for (int64_t i = from; i <= last; i += step) {
-      const float2 p = parts[i * pitch + g];
-      if constexpr (BACK) v.x += p.x, v.y += p.y;
-      else v.x = fmaf(p.x, count(i), v.x);
-    }
+      for (int64_t i = from; i <= last; i += step) {
+        const float2 p = parts[i * pitch + f];
+        if constexpr (BACK) v.x += p.x, v.y += p.y;
+        else v.x = fmaf(p.x, count(i), v.x);
+      }
     return v;
   }
   __device__ __forceinline__ float squares(int g, int64_t from, int64_t step, float mean) const {
     float q = 0.0f;
+    for (int f = g * fold; f < (g + 1) * fold; ++f)
 #pragma unroll 4
-    for (int64_t i = from; i <= last; i += step) {
-      const float2 p = parts[i * pitch + g];
-      q += fmaf(count(i) * (p.x - mean), p.x - mean, p.y);
-    }
+      for (int64_t i = from; i <= last; i += step) {
+        const float2 p = parts[i * pitch + f];
+        q += fmaf(count(i) * (p.x - mean), p.x - mean, p.y);
+      }
     return q;
   }
 };
@@ -759,8 +771,9 @@ k_norm_join(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
   }
   __shared__ float2 part[256];
   float2* const to = BACK ? c.means : c.stats;
+  const int groups = s.groups / t.fold;
   const auto put = [&](int64_t seg, int g, float a, float b, float inv) {
-    to[seg * s.groups + g] = make_float2(a, BACK ? b * inv : rsqrtf(b * inv + c.eps));
+    to[seg * groups + g] = make_float2(a, BACK ? b * inv : rsqrtf(b * inv + c.eps));
   };
   const int64_t block = blockIdx.x - joins;
   uint32_t rest = 1;      // of the block's segments, for all its threads
@@ -774,9 +787,9 @@ k_norm_join(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
       const NormPieces p(s, c, t, seg, r);
       many = r.end > r.begin && p.last - p.first >= kFewPieces;
       if (!many)
-        for (int g = lane; g < s.groups; g += 32) {
+        for (int g = lane; g < groups; g += 32) {
           if (r.end <= r.begin) {
-            to[seg * s.groups + g] = make_float2(0.0f, 0.0f);
+            to[seg * groups + g] = make_float2(0.0f, 0.0f);
             continue;
           }
           const float2 v = p.sums<BACK>(g, p.first, 1);
@@ -799,11 +812,11 @@ k_norm_join(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
       atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
     const NormPieces p(s, c, t, seg, r);
     const int width = t.join_groups, lane = threadIdx.x / width, lanes = 256 / width;
-    for (int g0 = blockIdx.y * width; g0 < s.groups; g0 += gridDim.y * width) {
+    for (int g0 = blockIdx.y * width; g0 < groups; g0 += gridDim.y * width) {
       const int g = g0 + threadIdx.x % width;
-      const bool mine = g < s.groups && lane < lanes;
+      const bool mine = g < groups && lane < lanes;
       if (r.end <= r.begin) {
-        if (mine && lane == 0) to[seg * s.groups + g] = make_float2(0.0f, 0.0f);
+        if (mine && lane == 0) to[seg * groups + g] = make_float2(0.0f, 0.0f);
         continue;
       }
       const auto together = [&](float2 v) {
@@ -847,8 +860,8 @@ k_norm_apply(const __grid_constant__ NormShape s, const __grid_constant__ NormCa
     if (e <= b) continue;
     if (e > done) done = e;
     float2 st[NC][GN], ab[BACK ? NC : 1][GN];
-    load_stats(s, c.stats, me, seg, st);
-    if constexpr (BACK) load_stats(s, c.means, me, seg, ab);
+    load_stats(s, t, c.stats, me, seg, st);
+    if constexpr (BACK) load_stats(s, t, c.means, me, seg, ab);
     // forwards (x - mean) (gamma / deviation) + beta
     float scale[BACK ? 1 : NC][VE];
     if constexpr (!BACK)
@@ -974,24 +987,29 @@ __global__ void __launch_bounds__(256) k_norm_wide(const __grid_constant__ NormS
     for (int64_t row = min(max(s.offsets[s.segments], (int64_t)0), s.rows) + blockIdx.x; row < s.rows; row += gridDim.x)
       for (int64_t k = threadIdx.x; k < s.dim; k += 256) out[row * s.dim + k] = Elem<T>::from_f(0.0f);
 }
-// dgamma and dbeta, a channel a thread.
+// Sums for dgamma and dbeta of some rows, a channel a thread.
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_wide_params(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c) {
+__global__ void __launch_bounds__(256) k_norm_wide_columns(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c) {
   wait_for_previous();
-  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x, some = (s.rows + gridDim.y - 1) / gridDim.y;
+  const int64_t row0 = blockIdx.y * some, row1 = min(row0 + some, s.rows);
+  int64_t seg = row0 < row1 ? segment_at(s, row0) : s.segments;
   if (col >= s.dim) return;
   float dgamma = 0.0f, dbeta = 0.0f, gamma;
-  for (int64_t seg = 0; seg < s.segments; ++seg) {
+  for (; seg < s.segments; ++seg) {
     const RowRange r = segment_rows(s, seg);
+    if (r.begin >= row1) break;
     float a = 0.0f, b = 0.0f;
-    for (int64_t row = r.begin; row < r.end; ++row) {
-      const float2 v = wide_xh_dz<T>(c, row * s.dim + col, col, c.stats[seg * s.groups + col / s.per], &gamma);
+    const float2 st = r.end > r.begin ? c.stats[seg * s.groups + col / s.per] : make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for (int64_t row = max(r.begin, row0); row < min(r.end, row1); ++row) {
+      const float2 v = wide_xh_dz<T>(c, row * s.dim + col, col, st, &gamma);
       a = fmaf(v.x, v.y, a), b += v.y;
     }
     dgamma += a, dbeta += b;
   }
-  put_param<T>(c.grad_weight, c.wide_params, col, dgamma);
-  put_param<T>(c.grad_bias, c.wide_params, col, dbeta);
+  c.columns[(int64_t)blockIdx.y * 2 * s.dim + col] = dgamma;
+  c.columns[((int64_t)blockIdx.y * 2 + 1) * s.dim + col] = dbeta;
 }
 
 // ------------------------------------------------------------------------------------------------- host side
@@ -1024,17 +1042,19 @@ template <typename T, int VE, int NC, int GN, bool BACK, bool WARP>
 static int norm_tiles(const NormShape& s, const NormCall& c, const NormPlan& p, cudaStream_t st) {
   const NormTiles& t = p.tiles;
   const dim3 sums((unsigned)p.blocks, (unsigned)p.chunks), apply((unsigned)ceil_div(t.apply_tiles, WARP ? 8 : 1), (unsigned)p.chunks);
-  APT_FOLLOW((k_norm_sums<T, VE, NC, GN, BACK, WARP>), sums, 256, 0, st, s, c, t);
+  NormShape parts = s;
+  parts.groups *= t.fold, parts.per /= t.fold;
+  APT_FOLLOW((k_norm_sums<T, VE, NC, GN, BACK, WARP>), sums, 256, 0, st, parts, c, t);
   const int joins = BACK && c.columns ? (int)ceil_div(2 * s.dim, 32) : 0;
   const dim3 join((unsigned)(joins + ceil_div(s.segments, t.join_segments)), t.join_segments > 1 ? 1u : (unsigned)ceil_div(s.groups, t.join_groups));
-  APT_FOLLOW((k_norm_join<T, BACK>), join, 256, 0, st, s, c, t, joins, p.blocks);
-  APT_FOLLOW((k_norm_apply<T, VE, NC, GN, BACK, WARP>), apply, 256, 0, st, s, c, t);
+  APT_FOLLOW((k_norm_join<T, BACK>), join, 256, 0, st, parts, c, t, joins, p.blocks);
+  APT_FOLLOW((k_norm_apply<T, VE, NC, GN, BACK, WARP>), apply, 256, 0, st, parts, c, t);
   return APT_OK;
 }
 template <typename T, int VE, int NC, bool BACK>
 static int norm_held(const NormShape& s, const NormCall& c, const NormPlan& p, cudaStream_t st) {
   if constexpr (VE > 1)
-    if (s.per % VE) return p.warps ? norm_tiles<T, VE, NC, VE, BACK, true>(s, c, p, st) : norm_tiles<T, VE, NC, VE, BACK, false>(s, c, p, st);
+    if (s.per / p.tiles.fold % VE) return p.warps ? norm_tiles<T, VE, NC, VE, BACK, true>(s, c, p, st) : norm_tiles<T, VE, NC, VE, BACK, false>(s, c, p, st);
   return p.warps ? norm_tiles<T, VE, NC, 1, BACK, true>(s, c, p, st) : norm_tiles<T, VE, NC, 1, BACK, false>(s, c, p, st);
 }
 template <typename T, int VE, bool BACK>
@@ -1048,10 +1068,14 @@ template <typename T, bool BACK>
 int norm(const NormShape& s, const NormCall& c, const NormPlan& p, cudaStream_t st) {
   if (p.kind == kNormWide) {
     if (s.rows) APT_FOLLOW((k_norm_wide<T, BACK>), wave_grid(s.segments * s.groups, 8), 256, 0, st, s, c);
-    if (BACK && (c.grad_weight || c.grad_bias)) APT_FOLLOW((k_norm_wide_params<T>), ceil_div(s.dim, 256), 256, 0, st, s, c);
+    if (BACK && c.columns) {
+      APT_FOLLOW((k_norm_wide_columns<T>), dim3((unsigned)ceil_div(s.dim, 256), (unsigned)p.blocks), 256, 0, st, s, c);
+      APT_FOLLOW((k_norm_columns<T>), ceil_div(2 * s.dim, 32), 256, 0, st, s, c, p.blocks);
+    }
     return APT_OK;
   }
   if (p.slice == 16 / (int)sizeof(T)) return norm_slices<T, 16 / (int)sizeof(T), BACK>(s, c, p, st);
+  if (p.slice == 8 / (int)sizeof(T)) return norm_slices<T, 8 / (int)sizeof(T), BACK>(s, c, p, st);
   if constexpr (sizeof(T) == 2)
     if (p.slice == 2) return norm_slices<T, 2, BACK>(s, c, p, st);
   return norm_slices<T, 1, BACK>(s, c, p, st);

@@ -37,14 +37,6 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
   return false;
 }
 
-// The same for a warp, by its first lane: every poll is an operation on shared memory of each lane that makes it, and warps that
-// wait for a tile would slow down those that work on it.
-__device__ __forceinline__ bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-  int fine = 1;
-  if (threadIdx.x % 32 == 0) fine = barrier_wait(bar, parity, gave_up);
-  return __shfl_sync(0xffffffffu, fine, 0);
-}
-
 // True for one lane of a converged warp, which the compiler knows to be one: products and copies, which take their operands in uniform
 // registers, are issued as they are then. Under a condition on the lane's number a product took 140 cycles to issue.
 __device__ __forceinline__ bool one_of_warp() {
@@ -88,11 +80,6 @@ __device__ __forceinline__ void tmem_load_32(uint32_t at, float (&v)[32]) {
         "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
         "=r"(r[31])
       : "r"(at));
-}
-__device__ __forceinline__ float tmem_load_1(uint32_t at) {
-  uint32_t r;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(at));
-  return __uint_as_float(r);
 }
 // Until the loads so far are done; what was loaded is used behind settled() of it only (the registers are written when the load is done, which the
 // compiler does not know).

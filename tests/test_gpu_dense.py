@@ -174,6 +174,28 @@ def test_norm_of_ragged_segments(sizes, tail, dim, groups, dtype):
     _check_norm(x, groups, offsets, act="silu" if dim % 8 else "gelu", p=0.25 if groups > 8 else 0.0, params="f32" if groups != 4 else "own")
 
 
+# groups wider than a block's columns: cut into parts of whole slices, or (2053 is a prime) walked over by a block
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,tail", [([90, 0, 1, 400], 7), ([3] * 70, 0)])
+@pytest.mark.parametrize("dim,groups", [(8192, 1), (6000, 2), (2053, 1), (4106, 1), (2068, 1)])
+def test_norm_of_wide_groups(sizes, tail, dim, groups, dtype):
+    offsets, rows = _offsets(sizes, tail)
+    x = (torch.randn((rows, dim), device="cuda", generator=_gen(rows + dim)) * 0.7 - 0.2).to(dtype)
+    _check_norm(x, groups, offsets, act="gelu", p=0.1)
+    if dim == 8192:
+        _check_norm(x[: rows // 6 * 6].view(-1, 3, dim), groups, act="none", p=0.0)
+
+
+# rows whose groups are slices of 8 bytes, rows of 1433
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,groups", [(100, 1), (36, 3), (42, 3), (138, 1), (316, 1), (1433, 1), (2060, 1)])
+def test_norm_of_rows_of_narrow_slices(dim, groups, dtype):
+    x = (torch.randn((301, dim), device="cuda", generator=_gen(dim)) * 1.5 + 0.3).to(dtype)
+    _check_norm(x, groups, act="silu", p=0.5)
+    offsets, _ = _offsets([200, 1, 0, 70], 30)
+    _check_norm(x, groups, offsets, act="gelu", p=0.5)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape,groups", [((2, 5, 7, 32), 4), ((1, 3000, 16), 16), ((3, 1, 48), 6), ((40, 9, 64), 1), ((2, 2, 2, 2, 10), 5)])
 def test_norm_channels_last(shape, groups, dtype):

@@ -178,27 +178,31 @@ __device__ __forceinline__ void begin_backward(const NormCall& c, int64_t e, con
 
 // ------------------------------------------------------------------------------------------ rows by themselves
 struct NormLanes {
-  int width;              // lanes of a row's group: a power of two up to 32, or 256
+  int width;              // lanes of a row's group: a power of two up to 256; BLOCK: above 32
   int groups, rows;       // a block has side by side
 };
 
-// A sum over the lanes of each group, of U rows at once.
+// A sum over the lanes of each group, of U rows at once. `shared`: not that of the sum before, whose readers this one's barrier waits for.
 template <bool BLOCK, int U>
 __device__ __forceinline__ void sum_lanes(float (&v)[U], int width, float (*shared)[U]) {
 #pragma unroll
   for (int u = 0; u < U; ++u)
     for (int o = (BLOCK ? 32 : width) / 2; o; o >>= 1) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
   if constexpr (BLOCK) {
-    __syncthreads();
     if (threadIdx.x % 32 == 0)
 #pragma unroll
       for (int u = 0; u < U; ++u) shared[threadIdx.x / 32][u] = v[u];
     __syncthreads();
+    const int warps = width / 32, first = threadIdx.x / width * warps;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      v[u] = 0.0f;
+      float sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[u] += shared[k][u];
+      for (int k = 0; k < 4; ++k) sum += shared[first + k][u];
+      if (warps > 4)
+#pragma unroll
+        for (int k = 4; k < 8; ++k) sum += shared[first + k][u];
+      v[u] = sum;
     }
   }
 }
@@ -208,9 +212,9 @@ template <typename T, int VE, int NV, int U, bool BLOCK, bool BACK>
 __global__ void __launch_bounds__(256)
 k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormLanes l) {
   wait_for_previous();
-  __shared__ float shared[8][U];
+  __shared__ float shared[2][8][U];
   __shared__ float sums[BACK ? 256 * VE : 1];
-  const int width = BLOCK ? 256 : l.width;
+  const int width = l.width;
   const int lane = threadIdx.x % width, slot = threadIdx.x / width % l.groups, line = threadIdx.x / (width * l.groups), g = blockIdx.y * l.groups + slot;
   const bool mine = line < l.rows && g < s.groups;
   const T* const x = (const T*)c.x;
@@ -259,7 +263,7 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
 #pragma unroll
         for (int k = 0; k < VE; ++k) mean[u] += rx[u][j].get(k);
     }
-    sum_lanes<BLOCK, U>(mean, width, shared);
+    sum_lanes<BLOCK, U>(mean, width, shared[0]);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       mean[u] *= inv;
@@ -272,7 +276,7 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
           rstd[u] += in[j] ? d * d : 0.0f;
         }
     }
-    sum_lanes<BLOCK, U>(rstd, width, shared);
+    sum_lanes<BLOCK, U>(rstd, width, shared[1]);
 #pragma unroll
     for (int u = 0; u < U; ++u) rstd[u] = rsqrtf(rstd[u] * inv + c.eps);
     if constexpr (!BACK) {
@@ -314,8 +318,8 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
           }
         }
       }
-      sum_lanes<BLOCK, U>(a, width, shared);
-      sum_lanes<BLOCK, U>(b, width, shared);
+      sum_lanes<BLOCK, U>(a, width, shared[0]);
+      sum_lanes<BLOCK, U>(b, width, shared[1]);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (row[u] >= s.rows) continue;
@@ -1027,7 +1031,7 @@ struct NormPlan {
 template <typename T, int VE, bool BACK>
 static int norm_rows(const NormShape& s, const NormCall& c, const NormPlan& p, cudaStream_t st) {
   const dim3 grid((unsigned)p.blocks, (unsigned)p.chunks);
-  if (p.lanes.width == 256) {
+  if (p.lanes.width > 32) {
     if (p.held == 1) APT_FOLLOW((k_norm_rows<T, VE, 1, BACK ? 1 : 2, true, BACK>), grid, 256, 0, st, s, c, p.lanes);
     else if (p.held == 2) APT_FOLLOW((k_norm_rows<T, VE, 2, 1, true, BACK>), grid, 256, 0, st, s, c, p.lanes);
     else APT_FOLLOW((k_norm_rows<T, VE, 4, 1, true, BACK>), grid, 256, 0, st, s, c, p.lanes);

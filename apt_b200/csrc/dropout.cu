@@ -1,7 +1,8 @@
 // Dropout whose mask is made anew wherever it is needed.
 //
 // y = x / (1 - p) where the element's word is at least p 2^32, else 0; the gradient is the same map. Nothing but x is read and nothing
-// but y is written.
+// but y is written. 151552 x 256 bf16: 41 us (155 MB; a copy takes 24 to 28), bound by the generator's integer products and logic, 29 us of them:
+// 63 per cent of the issue slots and 60 of the integer pipes' cycles.
 #include "dense.cuh"
 
 namespace apt {

@@ -4,9 +4,11 @@
 //   dx[r, k]  = sum_n dy[r, n] w[g, n, k]
 //   dw[g, n, k] = sum_{r in g} dy[r, n] x[r, k],   db[g, n] = sum_{r in g} dy[r, n]
 //
-// One persistent kernel for all three (k_grouped), a block an SM: a warp has boxes of both operands copied to a ring of stages in
-// shared memory, one thread issues the products of a stage into tensor memory, four warps bring finished tiles out. Where the groups
-// end is on the device only, so every block makes the list of tiles from the ends and its warps walk it.
+// One persistent kernel for all three (k_grouped), a block an SM: a thread has boxes of both operands copied to a ring of stages in
+// shared memory, one issues the products of a stage into tensor memory, eight warps (fp32: four) bring finished tiles out, from one half of
+// tensor memory while the products of the next go to the other. Where the groups end is on the device only, so every block makes the list of
+// tiles from the ends and its warps walk it. In dw a run of stages, as long for every block, may begin and end within a sum: it leaves
+// partial sums, which k_join_weights adds up.
 //
 // Operands stay as they are in memory, row by row; whether rows run along the contraction or across it is a bit of the product. A box
 // that reaches past a matrix is filled with zeros. Past the end of a group within a matrix it has the next group's rows: in out and dx those are
@@ -14,8 +16,8 @@
 //
 // fp32: x = h + m + l exactly, each bf16 (the upper 8, the next 8 and the last 8 bits: cut off, so nothing overflows). Of the nine
 // products of two such sums the six of more than 2^-24 of the whole are made: h h in one sum, the five small ones in another, which loses
-// nothing to the large one's roundings. Eight warps take the stages apart. A result that is not finite (infinities fall apart into NaN)
-// is computed again from the operands.
+// nothing to the large one's roundings. Two teams of four warps take the stages apart in turn. A result that is not finite (infinities fall
+// apart into NaN) is computed again from the operands.
 #include <algorithm>
 
 #include "dense.cuh"
@@ -399,6 +401,11 @@ __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedIt
 }
 
 // ---- the kernel ----------------------------------------------------------------------
+// 151552 x 256 -> 256 bf16 in 16 groups, us: out 34, dx 35 (HBM: 24; products: 12), dw and db 45 (24; 12) and their join 11.5. Eight tiles a block,
+// of which the first waits for the list and the weights and the last is brought out beside nothing: a third of the tensor cores' cycles and 36 to 45 per
+// cent of the DRAM's are in use. 495616 x 1024 -> 256 f16 in 4 groups: 260 (194; 159), at 1.05 to 1.3 GHz under the power cap. 67584 x 128 -> 256 fp32 in
+// 8 groups: 45, 45, 52 and 13.5 (HBM: 16, 16, 16; products: 16 each): six products of pieces read 208 KB of shared memory a stage, which bounds it.
+// 61 rows in 64 groups, 1024 -> 1024 bf16: 25, the weights of the groups that have rows (13).
 template <typename T, int MODE>
 __global__ void __launch_bounds__(GroupedTraits<T, MODE>::kThreads, 1)
 k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GroupedCall c) {
@@ -811,7 +818,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 }
 
 // The partial sums of dw and db that make up one, in the order of the rows. A run that begins within a sum says so in the plan; the first
-// such run of a sum has it joined: blocks (part of the tile, run).
+// such run of a sum has it joined: blocks (part of the tile, run). 147 runs of 256 x 256: 11.5 us for 38 MB out of L2, of which half is the launch
+// and the look at the plan.
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_join_weights(const __grid_constant__ GroupedCall c) {
@@ -862,23 +870,29 @@ k_join_weights(const __grid_constant__ GroupedCall c) {
   }
 }
 
-// db without dw.
+// db without dw: 32 columns of a group a block. 151552 x 256 bf16 in 16 groups 20 us (HBM: 12), 32 warps with eight rows each
+// on their way; eight with one each took 97.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 k_bias_sums(const T* __restrict__ grad, int64_t rows, int64_t out_dim, const int64_t* __restrict__ offsets, T* __restrict__ grad_bias, int32_t* status) {
   wait_for_previous();
-  __shared__ float part[8][33];
+  __shared__ float part[32][33];
   const int g = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   if (threadIdx.x == 0 && blockIdx.x == 0 && bad_group(offsets, g, rows)) atomicOr(status, APT_FLAG_BAD_OFFSETS);
   const RowRange r = group_rows(offsets, g, rows);
   const int64_t n = (int64_t)blockIdx.x * 32 + lane;
   float sum = 0.0f;
   if (n < out_dim)
-    for (int64_t row = r.begin + warp; row < r.end; row += 8) sum += Elem<T>::to_f(grad[row * out_dim + n]);
+    for (int64_t row = r.begin + warp; row < r.end; row += 8 * 32) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = row + 32 * k < r.end ? Elem<T>::to_f(grad[(row + 32 * k) * out_dim + n]) : 0.0f;
+      sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
   part[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && n < out_dim) {
-    for (int k = 1; k < 8; ++k) sum += part[k][lane];
+    for (int k = 1; k < 32; ++k) sum += part[k][lane];
     grad_bias[g * out_dim + n] = Elem<T>::from_f(sum);
   }
 }
@@ -1063,7 +1077,7 @@ static int linear_backward(const void* x, int64_t rows, int64_t dim, const void*
                            const void* grad, void* grad_x, void* grad_weight, void* grad_bias, char* room, int32_t* status, cudaStream_t s) {
   if (grad_bias && !grad_weight) {
     const dim3 grid((unsigned)ceil_div(out_dim, 32), (unsigned)groups);
-    APT_FOLLOW((k_bias_sums<T>), grid, 256, 0, s, (const T*)grad, rows, out_dim, offsets, (T*)grad_bias, status);
+    APT_FOLLOW((k_bias_sums<T>), grid, 1024, 0, s, (const T*)grad, rows, out_dim, offsets, (T*)grad_bias, status);
   }
   if (rows == 0) {
     if (grad_weight) APT_CUDA(cudaMemsetAsync(grad_weight, 0, (size_t)groups * out_dim * dim * sizeof(T), s));

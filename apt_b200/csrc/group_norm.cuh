@@ -184,24 +184,24 @@ struct NormLanes {
 
 // A sum over the lanes of each group, of U rows at once. `shared`: not that of the sum before, whose readers this one's barrier waits for.
 template <bool BLOCK, int U>
-__device__ __forceinline__ void sum_lanes(float (&v)[U], int width, float (*shared)[U]) {
+__device__ __forceinline__ void sum_lanes(float (&v)[U], int width, float* shared) {
 #pragma unroll
   for (int u = 0; u < U; ++u)
     for (int o = (BLOCK ? 32 : width) / 2; o; o >>= 1) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
   if constexpr (BLOCK) {
     if (threadIdx.x % 32 == 0)
 #pragma unroll
-      for (int u = 0; u < U; ++u) shared[threadIdx.x / 32][u] = v[u];
+      for (int u = 0; u < U; ++u) shared[threadIdx.x / 32 * U + u] = v[u];
     __syncthreads();
     const int warps = width / 32, first = threadIdx.x / width * warps;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum += shared[first + k][u];
+      for (int k = 0; k < 4; ++k) sum += shared[(first + k) * U + u];
       if (warps > 4)
 #pragma unroll
-        for (int k = 4; k < 8; ++k) sum += shared[first + k][u];
+        for (int k = 4; k < 8; ++k) sum += shared[(first + k) * U + u];
       v[u] = sum;
     }
   }
@@ -214,7 +214,7 @@ template <typename T, int VE, int NV, int U, bool BLOCK, bool BACK>
 __global__ void __launch_bounds__(256)
 k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormLanes l) {
   wait_for_previous();
-  __shared__ float shared[2][8][U];
+  __shared__ float shared[3][16 * U];
   __shared__ float sums[BACK ? 256 * VE : 1];
   const int width = l.width;
   const int lane = threadIdx.x % width, slot = threadIdx.x / width % l.groups, line = threadIdx.x / (width * l.groups), g = blockIdx.y * l.groups + slot;
@@ -239,23 +239,39 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
   }
   const float inv = 1.0f / (float)s.per;
   const int64_t step = (int64_t)l.rows * U;
-  for (int64_t base = blockIdx.x * step; base < s.rows; base += gridDim.x * step) {
-    Raw<T, VE> rx[U][NV], rg[BACK ? U : 1][NV];
-    int64_t row[U];
+  constexpr bool kAhead = BLOCK && NV == 1;      // the next rows are loaded in front of the sums of these
+  Raw<T, VE> rx[U][NV], rg[BACK ? U : 1][NV], next_x[kAhead ? U : 1][NV], next_g[kAhead && BACK ? U : 1][NV];
+  const auto load = [&](int64_t base, auto& to_x, auto& to_g) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      row[u] = base + u * l.rows + line;
+      const int64_t row = base + u * l.rows + line;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (in[j] && row[u] < s.rows) {
-          rx[u][j] = load_raw<T, VE>(x + row[u] * s.dim + at[j]);
-          if constexpr (BACK) rg[u][j] = load_raw<T, VE>(grad + row[u] * s.dim + at[j]);
+        if (in[j] && row < s.rows) {
+          to_x[u][j] = load_raw<T, VE>(x + row * s.dim + at[j]);
+          if constexpr (BACK) to_g[u][j] = load_raw<T, VE>(grad + row * s.dim + at[j]);
         } else {
-          rx[u][j] = Raw<T, VE>{};
-          if constexpr (BACK) rg[u][j] = Raw<T, VE>{};
+          to_x[u][j] = Raw<T, VE>{};
+          if constexpr (BACK) to_g[u][j] = Raw<T, VE>{};
         }
       }
     }
+  };
+  if constexpr (kAhead) load(blockIdx.x * step, next_x, next_g);
+  for (int64_t base = blockIdx.x * step; base < s.rows; base += gridDim.x * step) {
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        rx[u][0] = next_x[u][0];
+        if constexpr (BACK) rg[u][0] = next_g[u][0];
+      }
+      load(base + gridDim.x * step, next_x, next_g);
+    } else {
+      load(base, rx, rg);
+    }
+    int64_t row[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) row[u] = base + u * l.rows + line;
     float mean[U], rstd[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -298,10 +314,10 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
         }
       }
     } else {
-      float a[U], b[U], dz[U][NV][VE];
+      float ab[2 * U], dz[U][NV][VE];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        a[u] = b[u] = 0.0f;
+        ab[u] = ab[U + u] = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           float xh[VE];
@@ -315,23 +331,22 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
             dgamma[j][k] = fmaf(v, xh[k], dgamma[j][k]);
             dbeta[j][k] += v;
             dz[u][j][k] = dxh;
-            a[u] += dxh;
-            b[u] = fmaf(dxh, xh[k], b[u]);
+            ab[u] += dxh;
+            ab[U + u] = fmaf(dxh, xh[k], ab[U + u]);
           }
         }
       }
-      sum_lanes<BLOCK, U>(a, width, shared[0]);
-      sum_lanes<BLOCK, U>(b, width, shared[1]);
+      sum_lanes<BLOCK, 2 * U>(ab, width, shared[2]);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (row[u] >= s.rows) continue;
-        a[u] *= inv, b[u] *= inv;
+        const float a = ab[u] * inv, b = ab[U + u] * inv;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           if (!in[j]) continue;
           float v[VE];
 #pragma unroll
-          for (int k = 0; k < VE; ++k) v[k] = rstd[u] * (dz[u][j][k] - a[u] - (rx[u][j].get(k) - mean[u]) * rstd[u] * b[u]);
+          for (int k = 0; k < VE; ++k) v[k] = rstd[u] * (dz[u][j][k] - a - (rx[u][j].get(k) - mean[u]) * rstd[u] * b);
           store_all<T, VE>(out + row[u] * s.dim + at[j], v);
         }
       }

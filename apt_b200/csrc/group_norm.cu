@@ -26,10 +26,11 @@ static NormPlan norm_plan(const NormShape& s, size_t size, uintptr_t addresses, 
       p.kind = kNormRows;
       int w = 1;
       while (w < 32 && w < slices) w *= 2;
-      // Rows of more than two slices a lane of a warp are several warps', as few as will do: 128 lanes against 256 for 128 slices, backwards (forwards),
-      // 131072 x 512 fp32 221 us (124) against 398 (198), 65536 x 1024 bf16 215 (88) against 399 (127). Slices of one or two elements, four a lane,
-      // up to 512: 187980 x 357 bf16 430 (257) with 128 lanes, 609 (385) with 256; wider ones spill then.
-      if (slices > 64)
+      // Rows of more slices than a warp's lanes are several warps', as few as will do: us backwards (forwards), 131072 x 512 bf16 with 64 lanes
+      // 149 (82), a warp with two slices a lane 236 (100); 65536 x 1024 bf16 with 128 lanes 215 (88), with 256 399 (127). Slices of one or two
+      // elements are little work for the barriers: two a lane of a warp (657930 x 102 fp32 291 (182), with 64 lanes 336 (188)), then four a lane of 128
+      // up to 512 (187980 x 357 bf16 430 (257), with 256 lanes 609 (385)).
+      if (slices > (p.slice <= 2 ? 64 : 32))
         while (w < (p.slice <= 2 && slices <= 512 ? 128 : 256) && w < slices) w *= 2;
       p.held = (int)ceil_div(slices, w);
       if (p.held == 3) p.held = 4;

@@ -198,7 +198,10 @@ __device__ __forceinline__ void sum_lanes(float (&v)[U], int width, float* share
     for (int u = 0; u < U; ++u) {
       float sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum += shared[(first + k) * U + u];
+      for (int k = 0; k < 2; ++k) sum += shared[(first + k) * U + u];
+      if (warps > 2)
+#pragma unroll
+        for (int k = 2; k < 4; ++k) sum += shared[(first + k) * U + u];
       if (warps > 4)
 #pragma unroll
         for (int k = 4; k < 8; ++k) sum += shared[(first + k) * U + u];
@@ -208,8 +211,8 @@ __device__ __forceinline__ void sum_lanes(float (&v)[U], int width, float* share
 }
 
 // NV slices of VE elements a lane, U rows on their way. 67584 x 256 fp32 in 8 groups, silu and dropout: forwards 43 us (HBM: 21), backwards 61 (32),
-// the instructions of the generator and of silu. 65536 x 1024 bf16, gelu: 88 (41) and 215 (62), where a row's sums follow one another (four
-// barriers backwards) and registers (64 and 80) leave room for few rows at a time.
+// the instructions of the generator and of silu. 65536 x 1024 bf16, gelu: 83 (41) and 152 (62), where a row's sums follow one another (three
+// barriers backwards) and registers leave room for few rows at a time.
 template <typename T, int VE, int NV, int U, bool BLOCK, bool BACK>
 __global__ void __launch_bounds__(256)
 k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormLanes l) {
@@ -239,7 +242,7 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
   }
   const float inv = 1.0f / (float)s.per;
   const int64_t step = (int64_t)l.rows * U;
-  constexpr bool kAhead = BLOCK && NV == 1;      // the next rows are loaded in front of the sums of these
+  constexpr bool kAhead = BLOCK && NV <= 2;      // the next rows are loaded in front of the sums of these
   Raw<T, VE> rx[U][NV], rg[BACK ? U : 1][NV], next_x[kAhead ? U : 1][NV], next_g[kAhead && BACK ? U : 1][NV];
   const auto load = [&](int64_t base, auto& to_x, auto& to_g) {
 #pragma unroll
@@ -262,8 +265,11 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
     if constexpr (kAhead) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        rx[u][0] = next_x[u][0];
-        if constexpr (BACK) rg[u][0] = next_g[u][0];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          rx[u][j] = next_x[u][j];
+          if constexpr (BACK) rg[u][j] = next_g[u][j];
+        }
       }
       load(base + gridDim.x * step, next_x, next_g);
     } else {
@@ -1058,8 +1064,9 @@ static int norm_rows(const NormShape& s, const NormCall& c, const NormPlan& p, c
     else if (p.held == 2) APT_FOLLOW((k_norm_rows<T, VE, 2, 1, true, BACK>), grid, 256, 0, st, s, c, p.lanes);
     else APT_FOLLOW((k_norm_rows<T, VE, 4, 1, true, BACK>), grid, 256, 0, st, s, c, p.lanes);
   } else {
+    if constexpr (VE <= 2)
+      if (p.held == 2) APT_FOLLOW((k_norm_rows<T, VE, 2, BACK ? 1 : 2, false, BACK>), grid, 256, 0, st, s, c, p.lanes);
     if (p.held == 1) APT_FOLLOW((k_norm_rows<T, VE, 1, BACK ? 2 : 4, false, BACK>), grid, 256, 0, st, s, c, p.lanes);
-    else APT_FOLLOW((k_norm_rows<T, VE, 2, BACK ? 1 : 2, false, BACK>), grid, 256, 0, st, s, c, p.lanes);
   }
   if (BACK && c.columns) APT_FOLLOW((k_norm_columns<T>), ceil_div(2 * s.dim, 32), 256, 0, st, s, c, p.blocks);
   return APT_OK;

@@ -28,9 +28,9 @@ def _offsets(sizes, tail=0):
 
 
 # --------------------------------------------------------------------------------------------------------- dropout
-def _words(n, key, call_id):
-    """The generator's words by the CPU oracle's Philox."""
-    quads = np.arange((n + 3) // 4, dtype=np.uint64)
+def _words(n, key, call_id, first=0):
+    """The generator's words by the CPU oracle's Philox, from element `first` (of a whole quad) on."""
+    quads = np.arange((n + 3) // 4, dtype=np.uint64) + np.uint64(first // 4)
     low, high = (quads & np.uint64(0xFFFFFFFF)).astype(np.uint32), (quads >> np.uint64(32)).astype(np.uint32)
     w = orc.philox4x32_10(low, high, np.full_like(low, call_id & 0xFFFFFFFF), np.full_like(low, 0x64726F70),
                           np.uint32(key & 0xFFFFFFFF), np.uint32(key >> 32 & 0xFFFFFFFF))
@@ -523,4 +523,38 @@ def test_no_rows(dtype):
     assert y.shape == (0, 16)
     gx, gw, gb = apt_b200.group_norm_act_backward(x, x, stats, 2, x.new_ones(16), x.new_ones(16), offsets)
     assert gx.shape == (0, 16) and not gw.any() and not gb.any()
+    ops.check_status()
+
+
+def test_more_than_31_bits_of_elements():
+    rows, dim, n = 8_400_000, 256, 1000
+    x = torch.randn((rows, dim), device="cuda", generator=_gen(5), dtype=torch.bfloat16)
+    assert x.numel() > 2 ** 31
+    tail = x[-n:].clone()
+    ends = torch.tensor([0, 10, rows - n, rows], device="cuda")
+    one = torch.tensor([0, n], device="cuda")
+    # rows by themselves: what they are alone
+    y = apt_b200.group_norm_act(x, 4, act="silu")
+    assert torch.equal(y[-n:], apt_b200.group_norm_act(tail, 4, act="silu"))
+    # the last segment, alone in other tiles: roundings of its statistics
+    y, stats = apt_b200.group_norm_act(x, 4, None, None, ends, 1e-5, "silu", return_stats=True)
+    alone, alone_stats = apt_b200.group_norm_act(tail, 4, None, None, one, 1e-5, "silu", return_stats=True)
+    _close(y[-n:], alone, UNIT[x.dtype])
+    _close(stats[2], alone_stats[0], 1e-5)
+    grad = apt_b200.group_norm_act_backward(x, y, stats, 4, None, None, ends, 1e-5, "silu")[0]
+    _close(grad[-n:], apt_b200.group_norm_act_backward(tail, y[-n:].clone(), alone_stats, 4, None, None, one, 1e-5, "silu")[0], UNIT[x.dtype])
+    del y, grad
+    # dropout: words by the element's number
+    first = rows * dim - 4096
+    keep = torch.from_numpy(_words(4096, 7, 2, first) >= 2 ** 31).cuda()
+    out = apt_b200.dropout(x, 0.5, 7, 2)
+    assert torch.equal(out.view(-1)[first:], torch.where(keep, x.view(-1)[first:] * 2, 0.0))
+    del out
+    weight = (torch.randn((3, dim, dim), device="cuda", generator=_gen(6)) / 16).bfloat16()
+    out = apt_b200.grouped_linear(x, weight, ends)
+    _close(out[-n:], tail.double() @ weight[2].double().T, 4e-6 + UNIT[x.dtype])
+    _close(out[10:1010], x[10:1010].double() @ weight[1].double().T, 4e-6 + UNIT[x.dtype])
+    grad_x, grad_weight, _ = apt_b200.grouped_linear_backward(x, weight, ends, out)
+    _close(grad_x[-n:], out[-n:].double() @ weight[2].double(), 4e-6 + UNIT[x.dtype])
+    _close(grad_weight[2], out[-n:].double().T @ tail.double(), 4e-6 + UNIT[x.dtype])
     ops.check_status()

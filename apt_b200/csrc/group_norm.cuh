@@ -677,7 +677,7 @@ k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
     float2* const parts = c.parts + (tile + seg) * s.groups + me.group0;
     int left = (int)(e - b) - me.line;      // rows from the thread's next one on
     int64_t at = (b + me.line) * s.dim;
-    constexpr int U = (BACK ? 2 : 4) / (NC > 2 ? 2 : 1);
+    constexpr int U = BACK || NC > 4 ? 2 : 4;
     if constexpr (!BACK) {
       float v[1][NC][VE], q[NC][VE];
 #pragma unroll
@@ -933,8 +933,9 @@ k_norm_apply(const __grid_constant__ NormShape s, const __grid_constant__ NormCa
       for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int i = 0; i < VE; ++i) scale[j][i] = gamma[j][i] * st[j][i % GN].y;
-    // of narrow slices half as many rows at once, for each slice and row has code of its own: 18305 x 319 bf16 in 1651 segments 34 us, with four rows 47
-    constexpr int U = (BACK ? 2 : 4) / (NC > 2 ? 2 : 1);
+    // two rows of single elements at once, for each slice and row has code of its own: 18305 x 319 bf16 in 1651 segments 34 us, with four rows 47; in 8
+    // segments, 150000 rows, 127 and 134. One row at a time backwards: 38 for 41, but 165 for 148.
+    constexpr int U = BACK || NC > 4 ? 2 : 4;
     int left = (int)(e - b) - me.line;
     for (int64_t at0 = (b + me.line) * s.dim; left > 0; left -= U * t.lines, at0 += U * step) {
       Raw<T, VE> rx[U][NC], rg[BACK ? U : 1][NC];

@@ -83,7 +83,8 @@ inline dim3 as_grid(dim3 grid) { return grid; }
   } while (0)
 
 void set_relabel_small(bool on);   // relabel.cu: one-block shared-memory path for small layers
-void set_bulk_wait_polls(int polls);   // spmm.cu: bound of k_spmm_stream's waits
+void set_bulk_wait_polls(int polls);   // spmm.cu: bound of the waits of k_spmm_stream and k_grouped
+int bulk_wait_polls();
 
 // The tag of a sequence number (Tagged). A plain value's upper half is all zeros or all ones: no tag is, whatever the number, so that
 // words which were read already are never taken for an answer. Numbers 2^30 apart share one.

@@ -61,6 +61,7 @@ struct GroupedCall {
   int keep;                     // out and dx: a group's weights stay in shared memory while a block has tiles of it
   int halves;                   // out and dx: tiles of 128 rows that share a stage's weights
   int deep;                     // out and dx: blocks of the contraction in a stage
+  int polls;                    // of a wait
   int64_t ranges;               // dw: into how many runs of stages the work is cut at most
   const void *a, *b;            // the operands, as the copies read them
   int64_t pitch_a, pitch_b;     // elements
@@ -413,7 +414,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   constexpr int kBuffers = 2;
   constexpr bool kMends = MODE == kGradW && !Tr::kSplit;
   extern __shared__ char raw_shared[];
-  __shared__ uint64_t full[kMaxStages], free_[kMaxStages], ready[kMaxStages], used[kMaxStages], acc_full[2], acc_free[2], kept_full, kept_free, drained;
+  __shared__ uint64_t full[kMaxStages], free_[kMaxStages], ready[kMaxStages], used[kMaxStages], acc_full[2], acc_free[2], kept_full, kept_free, drained, met;
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up_word, scan[33];
   volatile int* const gave_up = &gave_up_word;
@@ -446,6 +447,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     barrier_init(shared_addr(&kept_full), Tr::kSplit ? 8 : 1);
     barrier_init(shared_addr(&kept_free), 1);
     barrier_init(shared_addr(&drained), 1);
+    barrier_init(shared_addr(&met), Tr::kOutWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     gave_up_word = 0;
   }
@@ -518,13 +520,13 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           kept_g = item.g, kept_n = item.n0;
           if constexpr (Tr::kSplit) {      // by the ring, to be taken apart
             for (int k = 0; k < kept_stages; ++k) {
-              if (!(fine = barrier_wait(shared_addr(free_ + stage), phase ^ 1, gave_up))) break;
+              if (!(fine = barrier_wait(shared_addr(free_ + stage), phase ^ 1, gave_up, c.polls))) break;
               barrier_expect(shared_addr(full + stage), bytes_b);
               copy_weights(shared_addr(copied + (size_t)stage * copied_bytes), k, shared_addr(full + stage));
               ++loaded;
               if (++stage == c.copied_stages) stage = 0, phase ^= 1;
             }
-          } else if ((fine = barrier_wait(shared_addr(&kept_free), (kept_times & 1) ^ 1, gave_up))) {
+          } else if ((fine = barrier_wait(shared_addr(&kept_free), (kept_times & 1) ^ 1, gave_up, c.polls))) {
             barrier_expect(shared_addr(&kept_full), bytes_b * kept_stages);
             for (int k = 0; k < kept_stages; ++k) copy_weights(shared_addr(kept + (size_t)k * kept_bytes), k, shared_addr(&kept_full));
             ++kept_times;
@@ -532,7 +534,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           if (!fine) break;
         }
         for (int k = 0; k < item.stages; ++k) {
-          if (!(fine = barrier_wait(shared_addr(free_ + stage), phase ^ 1, gave_up))) break;
+          if (!(fine = barrier_wait(shared_addr(free_ + stage), phase ^ 1, gave_up, c.polls))) break;
           const uint32_t bar = shared_addr(full + stage);
           uint32_t a = shared_addr(copied + (size_t)stage * copied_bytes), b = a + copied_a;
           if constexpr (MODE == kGradW) {
@@ -553,13 +555,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           if (++stage == c.copied_stages) stage = 0, phase ^= 1;
         }
       }
-      // a wait was given up: copies on their way still land
-      if (*gave_up) {
-        int nobody = 0;
-        for (int k = max(0, loaded - c.copied_stages); k < loaded; ++k)
-          barrier_wait(shared_addr(full + k % c.copied_stages), (k / c.copied_stages) & 1, &nobody);
-        if (kept_times) barrier_wait(shared_addr(&kept_full), (kept_times - 1) & 1, &nobody);
-      }
+      // copies on their way land before the block ends, also where somebody has given up, or will behind the last copy
+      for (int k = max(0, loaded - c.copied_stages); k < loaded; ++k) barrier_settle(shared_addr(full + k % c.copied_stages), (k / c.copied_stages) & 1);
+      if (kept_times) barrier_settle(shared_addr(&kept_full), (kept_times - 1) & 1);
     }
   } else if (warp == 1) {
     // ---- products
@@ -578,22 +576,22 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if (!item.stages) continue;
         const int halves = MODE != kGradW && item.rows > c.tile_m ? 2 : 1;
         buffer = c.halves == 2 || buffer == kBuffers - 1 ? 0 : buffer + 1;
-        if (!(fine = barrier_wait(shared_addr(acc_free + buffer), turns >> buffer & 1 ^ 1, gave_up))) break;
-        if (halves == 2 && !(fine = barrier_wait(shared_addr(acc_free + 1), turns >> 1 & 1 ^ 1, gave_up))) break;
+        if (!(fine = barrier_wait(shared_addr(acc_free + buffer), turns >> buffer & 1 ^ 1, gave_up, c.polls))) break;
+        if (halves == 2 && !(fine = barrier_wait(shared_addr(acc_free + 1), turns >> 1 & 1 ^ 1, gave_up, c.polls))) break;
         turns ^= halves == 2 ? 3 : 1 << buffer;
         if (keep && (item.g != kept_g || item.n0 != kept_n)) {
           kept_g = item.g, kept_n = item.n0;
           if (kept_times) products_done(shared_addr(&kept_free));
-          if (!(fine = barrier_wait(shared_addr(&kept_full), kept_times & 1, gave_up))) break;
+          if (!(fine = barrier_wait(shared_addr(&kept_full), kept_times & 1, gave_up, c.polls))) break;
           ++kept_times;
         }
         const uint32_t acc = tmem + buffer * kAccColumns;
         for (int k = 0; k < item.stages; ++k) {
-          if (!(fine = barrier_wait(shared_addr((Tr::kSplit ? ready : full) + stage), phase, gave_up))) break;
+          if (!(fine = barrier_wait(shared_addr((Tr::kSplit ? ready : full) + stage), phase, gave_up, c.polls))) break;
           const int left = (MODE == kGradW ? item.rows : c.num_k) - k * Tr::kBlock * c.deep, steps = (min(left, Tr::kBlock * c.deep) + 15) / 16;
           if (kMends && left < Tr::kBlock && left % 16) {
             barrier_arrive(shared_addr(ready));
-            if (!(fine = barrier_wait(shared_addr(ready + 1), mended, gave_up))) break;
+            if (!(fine = barrier_wait(shared_addr(ready + 1), mended, gave_up, c.polls))) break;
             mended ^= 1;
           }
           tmem_fence_after();
@@ -630,11 +628,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           if (++stage == stages) stage = 0, phase ^= 1;
         }
       }
-      if (*gave_up) {
-        int nobody = 0;
-        products_done(shared_addr(&drained));
-        barrier_wait(shared_addr(&drained), 0, &nobody);
-      }
+      products_done(shared_addr(&drained));      // (as the copies)
+      barrier_settle(shared_addr(&drained), 0);
     }
   } else if (kMends && warp == 2) {
     // ---- rows of the next group in the last stage of a sum: zeros, in both operands, when the products get there and ask for it (ready[0], answered by
@@ -646,7 +641,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       before_item += item.stages;
       if (item.rows % 16 == 0) continue;
       const int stage = (int)(last % c.copied_stages), valid = item.rows - (item.stages - 1) * Tr::kBlock;
-      if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(ready), mended, gave_up)))) break;
+      if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(ready), mended, gave_up, c.polls)))) break;
       mended ^= 1;
       char* const base = copied + (size_t)stage * copied_bytes;
       const int slices = ((valid + 15) / 16 * 16 - valid) * 8, blocks = copied_bytes / 8192;
@@ -663,16 +658,23 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     int summed = 0;
     uint32_t summed_phase = 0;
     int bias_g = -1, bias_n = -1, buffer = kBuffers - 1;
-    uint32_t turns = 0;
+    uint32_t turns = 0, meetings = 0;
+    const auto meet = [&] {      // of the warps here; false: somebody has given up
+      __syncwarp();
+      if (lane == 0) barrier_arrive(shared_addr(&met));
+      const bool all = __all_sync(0xffffffffu, barrier_wait(shared_addr(&met), meetings, gave_up, c.polls));
+      meetings ^= 1;
+      return all;
+    };
     while (fine && walk.take(&item)) {
       const bool empty = item.stages == 0;
       const int columns = min(c.tile_n, c.num_n - item.n0);
       if (MODE == kOut && c.bias && !empty && (item.g != bias_g || item.n0 != bias_n)) {
         bias_g = item.g, bias_n = item.n0;
-        asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");      // the tile before is out
+        if (!(fine = meet())) break;      // the tile before is out
         for (int k = thread; k < 256; k += Tr::kOutWarps * 32)
           bias[k] = bias_n + k < c.num_n ? Elem<T>::to_f(((const T*)c.bias)[(int64_t)bias_g * c.num_n + bias_n + k]) : 0.0f;
-        asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");
+        if (!(fine = meet())) break;
       }
       float column = 0.0f;      // of db
       if constexpr (MODE == kGradW) {
@@ -680,7 +682,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           // the columns of dy, while the products are made of them: as products with ones they took a third of the time of a stage
           float sum[2] = {0.0f, 0.0f};
           for (int k = 0; k < item.stages; ++k) {
-            if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + summed), summed_phase, gave_up)))) break;
+            if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + summed), summed_phase, gave_up, c.polls)))) break;
             const int valid = item.rows - k * Tr::kBlock;
             if (item.n0 == 0) add_columns<T>(copied + (size_t)summed * copied_bytes, valid, thread, sum);
             __syncwarp();
@@ -691,9 +693,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           column = sum[0];
           if constexpr (!Tr::kSplit) {      // four threads have a pair of columns
             if (item.n0 == 0) {
-              asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");
+              if (!(fine = meet())) break;
               *(float2*)(bias + (thread >> 6) * 128 + (thread & 63) * 2) = make_float2(sum[0], sum[1]);
-              asm volatile("bar.sync 1, %0;" ::"n"(Tr::kOutWarps * 32) : "memory");
+              if (!(fine = meet())) break;
               const int m = thread & 127;
               column = (bias[m] + bias[128 + m]) + (bias[256 + m] + bias[384 + m]);
             }
@@ -704,7 +706,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       for (int half = 0; half < halves; ++half) {
         if (!empty) {
           buffer = c.halves == 2 ? half : buffer == kBuffers - 1 ? 0 : buffer + 1;
-          fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_full + buffer), turns >> buffer & 1, gave_up));
+          fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_full + buffer), turns >> buffer & 1, gave_up, c.polls));
           if (!fine) break;
           turns ^= 1u << buffer;
           tmem_fence_after();
@@ -770,11 +772,11 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     while (fine && walk.take(&item)) {
       if (keep && item.stages && (item.g != kept_g || item.n0 != kept_n)) {
         kept_g = item.g, kept_n = item.n0;
-        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(&kept_free), (kept_times & 1) ^ 1, gave_up));
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(&kept_free), (kept_times & 1) ^ 1, gave_up, c.polls));
         ++kept_times;
         for (int k = 0; fine && k < kept_stages; ++k, next_from()) {
           // the other team's stages too: a wait for a phase is one only where the phase before is known to be over
-          if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up)))) break;
+          if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + from), from_phase, gave_up, c.polls)))) break;
           if ((k & 1) != team) continue;
           take_stage_apart<Tr::kMnB, false>(copied + (size_t)from * copied_bytes, kept + (size_t)k * kept_bytes, c.tile_n, piece_b, Tr::kBlock);
           __syncwarp();
@@ -789,7 +791,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if (turn != team) continue;      // each team has a stage of pieces of its own
         // first the products of the team's stage before: they came behind those of all earlier ones, so that what the ring's place held before
         // has arrived, and the wait for its next phase is one
-        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(used + team), uses ^ 1, gave_up) && barrier_wait(shared_addr(full + from), from_phase, gave_up));
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(used + team), uses ^ 1, gave_up, c.polls) && barrier_wait(shared_addr(full + from), from_phase, gave_up, c.polls));
         if (!fine) break;
         const char* const in = copied + (size_t)from * copied_bytes;
         char* const out = pieces + (size_t)team * piece_bytes;
@@ -998,7 +1000,7 @@ static int launch_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap
     c.keep = bytes + least <= room && items >= 3 * kNumSMs && items >= 3 * (int64_t)c.groups * c.tiles_n;
     if (c.keep) kept = (int)bytes;
   }
-  c.halves = c.deep = 1;
+  c.halves = c.deep = 1, c.polls = bulk_wait_polls();
   if (MODE != kGradW && !Tr::kSplit && !c.keep) {
     // Two tiles of rows share the weights of a stage where groups are long and the contraction is: the weights come half as often, and bringing
     // tiles out beside the products, which both halves of tensor memory are taken from, is what a long contraction needs least.

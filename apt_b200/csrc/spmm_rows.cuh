@@ -679,7 +679,6 @@ int launch_spmm_rows(int op, const RowArgs<T>& a, cudaStream_t s);
 
 // ---- shared by spmm.cu and gat.cu -----------------------------------------------------
 constexpr int kStreamWaitPolls = 1 << 20;      // of an mbarrier, each of which may suspend for a while itself
-int bulk_wait_polls();
 int pending_word(int32_t** word);            // for flags of calls without a status word: see spmm.cu
 // slot_bytes: of order[] (OrderKind).
 size_t spmm_layout(int64_t num_rows, int64_t num_edges, char* base, SpmmWs* ws, int slot_bytes = 8);

@@ -19,12 +19,10 @@ __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void barrier_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Polls of a barrier, each of which may suspend for a while itself, after which a wait is given up.
-constexpr int kBarrierPolls = 1 << 20;
-// Until the barrier's phase of this parity is over. False: somebody has given up (*gave_up); nothing may be used then but what
-// ends the kernel.
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-  for (int i = 0; i < kBarrierPolls; ++i) {
+// Until the barrier's phase of this parity is over, or for that many polls, each of which may suspend for a while itself. False: somebody
+// has given up (*gave_up); nothing may be used then but what ends the kernel.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int polls) {
+  for (int i = 0; i < polls; ++i) {
     uint32_t done;
     asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
                  : "=r"(done)
@@ -35,6 +33,12 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
   }
   *gave_up = 1;
   return false;
+}
+// For what is in flight and has to land before a block ends, whoever has given up.
+constexpr int kLastPolls = 1 << 20;
+__device__ __forceinline__ void barrier_settle(uint32_t bar, uint32_t parity) {
+  int nobody = 0;
+  barrier_wait(bar, parity, &nobody, kLastPolls);
 }
 
 // True for one lane of a converged warp, which the compiler knows to be one: products and copies, which take their operands in uniform

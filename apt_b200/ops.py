@@ -273,7 +273,8 @@ def _flag_text(flags):
         _lib.FLAG_NOT_GROUPED: "edges of a block are not grouped by destination",
         _lib.FLAG_SIZE_MISMATCH: "a peer sent another number of rows than the reduction expects",
         _lib.FLAG_BAD_OFFSETS: "ends of row groups do not ascend from 0 to at most the number of rows",
-        _lib.FLAG_COPY_TIMEOUT: "input rows of a sum did not reach shared memory in time; some of its rows are zero",
+        _lib.FLAG_COPY_TIMEOUT: "input rows did not reach shared memory in time; some rows of a sum are zero, or the results of a grouped "
+                                "product are unspecified",
     }
     return ", ".join(v for k, v in names.items() if flags & k)
 

@@ -55,7 +55,8 @@ typedef enum apt_dtype { APT_F32 = 0, APT_BF16 = 1, APT_F16 = 2 } apt_dtype;
 #define APT_FLAG_NOT_GROUPED     32 /* a block operator got edges not grouped by destination */
 #define APT_FLAG_SIZE_MISMATCH   64 /* a peer sent another number of rows than the reduction expects */
 #define APT_FLAG_BAD_OFFSETS     256 /* ends of row groups that do not ascend from 0 to at most the number of rows */
-#define APT_FLAG_COPY_TIMEOUT    128 /* input rows did not reach shared memory in time: the sums of the warp that waited are zero */
+#define APT_FLAG_COPY_TIMEOUT    128 /* input rows did not reach shared memory in time: the sums of the warp that waited are zero, the
+                                       results of a grouped product unspecified */
 
 const char* apt_last_error(void);
 int apt_version(void);
@@ -113,7 +114,8 @@ int apt_profile_read(const char* tag, double* total_ms, int64_t* launches);
  *   gather_miss_mode, gather_miss_blocks, gather_miss_kb_per_block, gather_hit_mode, gather_hit_waves
  *                      accepted, without effect and reported on stderr (they chose between forms of the gather that
  *                      are gone)
- *   bulk_wait_polls    polls after which a wait for rows on their way to shared memory is given up, 0 to 1048576 (default)
+ *   bulk_wait_polls    polls after which a wait for rows on their way to shared memory (in a grouped product any wait
+ *                      within a block) is given up, 0 to 1048576 (default)
  *   relabel_small      1 (default): layers of up to 8192 items are relabelled by one block with
  *                      the hash table in shared memory; 0: always the multi-block path */
 int apt_set_tunable(const char* name, int64_t value);

@@ -1,0 +1,62 @@
+"""The operators of a layer's dense half where they end: waits that run out, sizes at the ends of what a call takes, numbers that a mean error
+would hide."""
+import numpy as np
+import pytest
+import torch
+
+import apt_b200
+from apt_b200 import ops
+from apt_b200._lib import check, lib
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+UNIT = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _ends(*sizes):
+    return torch.tensor(np.concatenate([[0], np.cumsum(sizes)]), device="cuda")
+
+
+# ------------------------------------------------------------------------------------------------- grouped products
+def _given_up(call, polls):
+    """The call's results with so few polls a wait, and whether one of them ran out."""
+    check(lib.apt_set_tunable(b"bulk_wait_polls", polls))
+    try:
+        got = call()
+        torch.cuda.synchronize()
+    finally:
+        check(lib.apt_set_tunable(b"bulk_wait_polls", 1 << 20))
+    try:
+        ops.check_status()
+    except RuntimeError as e:
+        assert "did not reach shared memory" in str(e)
+        return got, True
+    return got, False
+
+
+def _right_or_flagged(call, polls):
+    want = call()
+    ops.check_status()
+    got, flagged = _given_up(call, polls)
+    assert flagged or all(torch.equal(a, b) for a, b in zip(got, want))
+    assert flagged or polls > 0
+    for a, b in zip(call(), want):
+        assert torch.equal(a, b)
+    ops.check_status()
+
+
+# weights that stay in shared memory, tiles in pairs, two blocks a stage, few rows a group
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,dim,out_dim", [([60000, 1], 128, 256), ([40000, 40000], 1024, 264), ([300, 0, 5], 256, 40), ([3] * 64, 1024, 512)])
+@pytest.mark.parametrize("polls", [0, 1, 6, 50])
+def test_products_of_rows_end_when_a_wait_runs_out(sizes, dim, out_dim, dtype, polls):
+    gen = _gen(1)
+    make = lambda *shape: torch.randn(shape, device="cuda", generator=gen).to(dtype)
+    offsets, rows = _ends(*sizes), sum(sizes)
+    x, weight, bias, grad = make(rows, dim), make(len(sizes), out_dim, dim), make(len(sizes), out_dim), make(rows, out_dim)
+    _right_or_flagged(lambda: (apt_b200.grouped_linear(x, weight, offsets, bias),
+                               apt_b200.grouped_linear_backward(x, weight, offsets, grad, want_weight=False, want_bias=False)[0]), polls)

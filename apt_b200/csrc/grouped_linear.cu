@@ -714,11 +714,6 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const uint32_t acc = tmem + buffer * kAccColumns;
         if constexpr (MODE == kGradW) {
           const int rows = min(kTileM, c.num_m - item.m0), m = quarter * 32 + lane;
-          if (thread == 0 && item.run >= 0) {
-            int64_t* const to = c.plan + 2 + kPlanWords * item.run;
-            to[0] = (int64_t)(item.m0 / kTileM * c.tiles_n + item.n0 / c.tile_n) * c.groups + item.g, to[1] = item.first;
-            to[2] = walk.runs.begin(item.run), to[3] = item.run ? walk.runs.begin(item.run - 1) : 0, to[4] = walk.runs.of(item.last - 1);
-          }
           if (quarter * 32 < rows) {
             if (item.piece < 0)
               store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0,
@@ -747,6 +742,14 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       }
     }
   } else if (MODE == kGradW && warp == 3) {
+    // ---- the plan of the block's runs, which follows from the walk and waits for nothing: k_join_weights reads it whoever gives up
+    if (lane == 0)
+      while (walk.take(&item)) {
+        if (item.run < 0) continue;
+        int64_t* const to = c.plan + 2 + kPlanWords * item.run;
+        to[0] = (int64_t)(item.m0 / kTileM * c.tiles_n + item.n0 / c.tile_n) * c.groups + item.g, to[1] = item.first;
+        to[2] = walk.runs.begin(item.run), to[3] = item.run ? walk.runs.begin(item.run - 1) : 0, to[4] = walk.runs.of(item.last - 1);
+      }
     // ---- groups without rows
     const int64_t per = (int64_t)c.num_m * c.num_n;
     const bool slices = per * sizeof(T) % 16 == 0;

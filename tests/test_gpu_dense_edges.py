@@ -60,3 +60,16 @@ def test_products_of_rows_end_when_a_wait_runs_out(sizes, dim, out_dim, dtype, p
     x, weight, bias, grad = make(rows, dim), make(len(sizes), out_dim, dim), make(len(sizes), out_dim), make(rows, out_dim)
     _right_or_flagged(lambda: (apt_b200.grouped_linear(x, weight, offsets, bias),
                                apt_b200.grouped_linear_backward(x, weight, offsets, grad, want_weight=False, want_bias=False)[0]), polls)
+
+
+# sums within a run and across runs, groups without rows, an end within a stage
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,dim,out_dim", [([60000, 1], 128, 256), ([4000, 0, 777], 264, 136), ([3] * 64, 256, 512), ([17], 16, 8)])
+@pytest.mark.parametrize("polls", [0, 1, 6, 50])
+def test_weight_gradients_end_when_a_wait_runs_out(sizes, dim, out_dim, dtype, polls):
+    """The partial sums that a run did not make are not there; which of them belong together the join knows all the same."""
+    gen = _gen(2)
+    make = lambda *shape: torch.randn(shape, device="cuda", generator=gen).to(dtype)
+    offsets, rows = _ends(*sizes), sum(sizes)
+    x, weight, grad = make(rows, dim), make(len(sizes), out_dim, dim), make(rows, out_dim)
+    _right_or_flagged(lambda: apt_b200.grouped_linear_backward(x, weight, offsets, grad, want_x=False)[1:], polls)

@@ -16,8 +16,8 @@
 //
 // fp32: x = h + m + l exactly, each bf16 (the upper 8, the next 8 and the last 8 bits: cut off, so nothing overflows). Of the nine
 // products of two such sums the six of more than 2^-24 of the whole are made: h h in one sum, the five small ones in another, which loses
-// nothing to the large one's roundings. Two teams of four warps take the stages apart in turn. A result that is not finite (infinities fall
-// apart into NaN) is computed again from the operands.
+// nothing to the large one's roundings. Two teams of four warps take the stages apart in turn. Infinities are their own upper bits, and NaN below
+// them: where the two sums make a NaN the large one, which has everything that is not finite in its upper bits, is the result.
 #include <algorithm>
 
 #include "dense.cuh"
@@ -189,6 +189,8 @@ __device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __
 __device__ __forceinline__ float below(float v) { return v - __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 __device__ __forceinline__ Pieces take_apart(float4 a, float4 b) {
   Pieces r;
+  // a sum has a NaN's upper bits set, which an operand may have in its lower ones alone
+  a = make_float4(a.x + 0.0f, a.y + 0.0f, a.z + 0.0f, a.w + 0.0f), b = make_float4(b.x + 0.0f, b.y + 0.0f, b.z + 0.0f, b.w + 0.0f);
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     r.p[k] = make_uint4(upper_halves(a.x, a.y), upper_halves(a.z, a.w), upper_halves(b.x, b.y), upper_halves(b.z, b.w));
@@ -237,24 +239,6 @@ __device__ __forceinline__ void take_stage_apart(const char* copied, char* piece
   }
 }
 
-// A sum that came out infinite or NaN, from the operands.
-template <int MODE>
-__device__ __noinline__ float sum_again(const GroupedCall& c, const GroupedItem& item, int m, int n) {
-  const float *a = (const float*)c.a, *b = (const float*)c.b;
-  int64_t step_a = 1, step_b = 1, count = c.num_k;
-  if (MODE == kGradW) {
-    a += item.row * c.pitch_a + item.m0 + m, b += item.row * c.pitch_b + item.n0 + n;
-    step_a = c.pitch_a, step_b = c.pitch_b, count = item.rows;
-  } else {
-    a += (item.row + m) * c.pitch_a;
-    b += (int64_t)item.g * (MODE == kOut ? c.num_n : c.num_k) * c.pitch_b;
-    if (MODE == kOut) b += (int64_t)(item.n0 + n) * c.pitch_b;
-    else b += item.n0 + n, step_b = c.pitch_b;
-  }
-  float sum = 0.0f;
-  for (int64_t k = 0; k < count && sum == sum; ++k) sum = fmaf(a[k * step_a], b[k * step_b], sum);
-  return sum;
-}
 // Sums over the rows of a stage of dy as copied: of a column (fp32, 128 threads), or over a quarter of the rows of a pair of columns.
 template <typename T>
 __device__ __forceinline__ void add_columns(const char* stage, int valid, int thread, float (&sum)[2]) {
@@ -318,17 +302,16 @@ __device__ __noinline__ void put_narrow_rows(const char* staging, int lane, O* t
 // A warp's 32 rows, 128 bytes of each at a time, through shared memory, so that the stores are whole rows of 128 bytes. Warps that share
 // rows take turns.
 template <typename T, typename O, int MODE>
-__device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedItem& item, uint32_t acc, bool empty, char* staging, int lane, int quarter, int turn,
-                                           int turns, O* out, int64_t ld, int rows, int columns, const float* bias, uint32_t acc_free) {
+__device__ __forceinline__ void store_tile(uint32_t acc, bool empty, char* staging, int lane, int quarter, int turn, int turns, O* out, int64_t ld, int rows,
+                                           int columns, const float* bias, uint32_t acc_free) {
   using Tr = GroupedTraits<T, MODE>;
   constexpr int kWide = 128 / (int)sizeof(O), kPer = 16 / (int)sizeof(O);
-  const int m = quarter * 32 + lane, here = min(32, rows - quarter * 32);
+  const int here = min(32, rows - quarter * 32);
   const bool whole = (ld * (int64_t)sizeof(O)) % 16 == 0;
   O* const first = out + (int64_t)quarter * 32 * ld;
   acc += (uint32_t)quarter << 21;
   for (int c0 = turn * kWide; c0 < columns; c0 += turns * kWide) {
     float v[kWide / 32][32];
-    uint32_t wild = 0;
     if (empty) {
 #pragma unroll
       for (int h = 0; h < kWide / 32; ++h)
@@ -345,8 +328,8 @@ __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedIt
         settled(v[0]);
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
-          v[0][k] += small[k];
-          wild |= isfinite(v[0][k]) ? 0u : 1u << k;
+          const float sum = v[0][k] + small[k];
+          v[0][k] = sum == sum ? sum : v[0][k];      // infinite, see above
         }
       } else {
         tmem_wait_loads();
@@ -369,14 +352,6 @@ __device__ __forceinline__ void store_tile(const GroupedCall& c, const GroupedIt
         }
 #pragma unroll
     for (int s = 0; s < 8; ++s) *(uint4*)(staging + lane * 128 + ((s ^ (lane & 7)) << 4)) = rounded_slice<O>(&v[s * kPer / 32][s * kPer % 32]);
-    if constexpr (Tr::kSplit) {
-      if (lane < here)
-        for (; wild; wild &= wild - 1) {
-          const int k = __ffs(wild) - 1;
-          if (c0 + k < columns)
-            *(float*)(staging + lane * 128 + (((k >> 2) ^ (lane & 7)) << 4) + (k & 3) * 4) = sum_again<MODE>(c, item, m, c0 + k) + (bias ? bias[c0 + k] : 0.0f);
-        }
-    }
     __syncwarp();
     if (whole) {
       const int s = lane & 7, r1 = lane >> 3, col = c0 + s * kPer;
@@ -716,10 +691,10 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           const int rows = min(kTileM, c.num_m - item.m0), m = quarter * 32 + lane;
           if (quarter * 32 < rows) {
             if (item.piece < 0)
-              store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0,
+              store_tile<T, T, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0,
                                      (int64_t)c.num_n, rows, columns, nullptr, 0u);
             else
-              store_tile<T, float, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows,
+              store_tile<T, float, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows,
                                          columns, nullptr, 0u);
             if (c.grad_bias && item.n0 == 0 && turn == 0) {
               if (m < rows) {
@@ -732,7 +707,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const int rows = item.rows - half * kTileM;
         const bool stores = MODE != kGradW && quarter * 32 < min(rows, c.tile_m) && turn * (128 / (int)sizeof(T)) < columns;
         if (stores)
-          store_tile<T, T, MODE>(c, item, acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + (item.row + half * kTileM) * c.num_n + item.n0, (int64_t)c.num_n,
+          store_tile<T, T, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + (item.row + half * kTileM) * c.num_n + item.n0, (int64_t)c.num_n,
                                  min(rows, c.tile_m), columns, MODE == kOut && c.bias && !empty ? bias : nullptr, shared_addr(acc_free + buffer));
         if (!empty && !stores) {
           tmem_fence_before();

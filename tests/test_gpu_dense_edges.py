@@ -73,3 +73,54 @@ def test_weight_gradients_end_when_a_wait_runs_out(sizes, dim, out_dim, dtype, p
     offsets, rows = _ends(*sizes), sum(sizes)
     x, weight, grad = make(rows, dim), make(len(sizes), out_dim, dim), make(rows, out_dim)
     _right_or_flagged(lambda: apt_b200.grouped_linear_backward(x, weight, offsets, grad, want_x=False)[1:], polls)
+
+
+def test_infinite_results_take_no_longer():
+    """Rows that are infinite all over, long contractions: right, and without a wait that runs out."""
+    gen = _gen(3)
+    rows, dim, n = 2000, 4096, 512
+    offsets = _ends(1500, 300, 200)
+    x, weight = torch.randn((rows, dim), device="cuda", generator=gen), torch.randn((3, n, dim), device="cuda", generator=gen)
+    grad = torch.randn((rows, n), device="cuda", generator=gen)
+    calm = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    wild = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+
+    def both(events):
+        for k in range(2):
+            events[0].record()
+            got = (apt_b200.grouped_linear(x, weight, offsets),) + apt_b200.grouped_linear_backward(x, weight, offsets, grad)
+            events[1].record()
+        torch.cuda.synchronize()
+        return got
+
+    both(calm)
+    x[:, 17] = float("inf")
+    grad[:, 5] = float("-inf")
+    out, gx, gw, gb = both(wild)
+    ops.check_status()
+    for g, (b, e) in enumerate(((0, 1500), (1500, 1800), (1800, 2000))):
+        assert torch.equal(out[b:e], torch.copysign(torch.full((e - b, n), float("inf"), device="cuda"), weight[g, :, 17].expand(e - b, n)))
+        assert torch.equal(gx[b:e], torch.copysign(torch.full((e - b, dim), float("inf"), device="cuda"), -weight[g, 5].expand(e - b, dim)))
+        # infinite terms of either sign in one sum, but where an infinite factor meets the other
+        nan = torch.zeros((n, dim), dtype=torch.bool, device="cuda")
+        nan[:, 17] = nan[5] = True
+        nan[5, 17] = False
+        assert torch.equal(torch.isnan(gw[g]), nan) and float(gw[g, 5, 17]) == float("-inf") == float(gb[g, 5])
+    assert wild[0].elapsed_time(wild[1]) < 4 * calm[0].elapsed_time(calm[1])
+
+
+@pytest.mark.parametrize("bits", [0x7FC00000, 0x7F800001, -1, 0xFF800001 - 2 ** 32])
+def test_a_nan_is_one_whatever_its_bits(bits):
+    gen = _gen(4)
+    x, weight = torch.randn((200, 64), device="cuda", generator=gen), torch.randn((1, 48, 64), device="cuda", generator=gen)
+    x[77].view(torch.int32)[9] = bits
+    weight[0, 30].view(torch.int32)[3] = bits
+    offsets = _ends(200)
+    out = apt_b200.grouped_linear(x, weight, offsets)
+    nan = torch.zeros((200, 48), dtype=torch.bool, device="cuda")
+    nan[77], nan[:, 30] = True, True
+    assert torch.equal(torch.isnan(out), nan) and torch.isfinite(out[~nan]).all()
+    grad = torch.randn((200, 48), device="cuda", generator=gen)
+    gx, gw, _ = apt_b200.grouped_linear_backward(x, weight, offsets, grad)
+    assert torch.isnan(gx[:, 3]).all() and torch.isfinite(gx[:, :3]).all() and torch.isnan(gw[0, :, 9]).all() and torch.isfinite(gw[0, :, :9]).all()
+    ops.check_status()

@@ -10,6 +10,8 @@
 // tiles from the ends and its warps walk it. In dw a run of stages, as long for every block, may begin and end within a sum: it leaves
 // partial sums, which k_join_weights adds up.
 //
+// In fp32 a sum of dw is brought out every 1024 rows and added up by rounding, for the tensor cores cut their sums off instead.
+//
 // Operands stay as they are in memory, row by row; whether rows run along the contraction or across it is a bit of the product. A box
 // that reaches past a matrix is filled with zeros. Past the end of a group within a matrix it has the next group's rows: in out and dx those are
 // rows of the tile that are not written, in dw they are part of the sum and are overwritten with zeros first, in both operands.
@@ -46,6 +48,9 @@ struct GroupedTraits {
   // warps that bring tiles out: two for each quarter of tensor memory's lanes, or one beside the eight that take fp32 apart
   static constexpr int kOutWarps = kSplit ? 4 : 8;
   static constexpr int kThreads = kSplit ? 512 : 384;
+  // a sum in tensor memory has so many stages at most: 1024 rows
+  static constexpr bool kCuts = kSplit && MODE == kGradW;
+  static constexpr int kCut = 32;
   // bytes of a tile of n rows (or columns) in a stage as copied, and of one bf16 piece of it
   static __host__ __device__ constexpr int copied(int n, bool mn) { return mn ? (n + kBox - 1) / kBox * kBlock * 128 : n * 128; }
   static __host__ __device__ constexpr int piece(int n, bool mn) { return mn ? (n + 63) / 64 * kBlock * 128 : (n + 31) / 32 * 32 * kBlock * 2; }
@@ -62,12 +67,13 @@ struct GroupedCall {
   int halves;                   // out and dx: tiles of 128 rows that share a stage's weights
   int deep;                     // out and dx: blocks of the contraction in a stage
   int polls;                    // of a wait
-  int64_t ranges;               // dw: into how many runs of stages the work is cut at most
+  int64_t ranges;               // dw: into how many runs of stages the work is cut at most, each a block's
   const void *a, *b;            // the operands, as the copies read them
   int64_t pitch_a, pitch_b;     // elements
   const void* bias;
   void *out, *grad_bias;
   float *partial, *partial_bias;
+  float* carry;                 // a tile a block: the parts so far of a sum that is brought out in parts
   int64_t* plan;                // dw, for k_join_weights: units, runs, and of each run its first piece's tile and group and the sum's first unit, the run's
                                 // beginning and that of the run before, the sum's last run
   int32_t* status;
@@ -79,9 +85,9 @@ struct GroupedItem {
   int64_t row;                  // first row of x
   int rows;                     // of the group from there on, in out and dx at most halves tile_m
   int m0, n0, stages;
+  int before = 0, after = 0;    // stages of the same sum (in dw, of the run's piece of it) in parts before this one, and behind it
   int64_t piece;                // dw: number of the partial sum, -1: all of the sum
   int64_t first, last;          // dw: units of all of the sum
-  int64_t run;                  // dw: the run that begins here, -1: none
 };
 
 // Runs of stages of dw: every run is as long as any other within one, whatever the groups are. A run has all stages of the tiles and
@@ -108,9 +114,8 @@ struct GroupedWalk {
   __device__ GroupedWalk(const GroupedCall& call, const int* p, const int* rows) : c(call), prefix(p), begin(rows) {
     if constexpr (MODE == kGradW) {
       runs = grouped_runs((int64_t)prefix[c.groups] * c.tiles_m * c.tiles_n, c.ranges);
-      step = blockIdx.x;
       next = end = 0;
-      if (runs.units && step < runs.runs) next = runs.begin(step), end = runs.begin(step + 1);
+      if (runs.units && blockIdx.x < runs.runs) next = runs.begin(blockIdx.x), end = runs.begin(blockIdx.x + 1);
     } else {
       const int64_t all = (int64_t)prefix[c.groups + 1] * c.tiles_n;
       next = c.keep ? blockIdx.x * all / gridDim.x : blockIdx.x, step = c.keep ? 1 : gridDim.x, end = c.keep ? (blockIdx.x + 1) * all / gridDim.x : all;
@@ -125,25 +130,33 @@ struct GroupedWalk {
     }
     return lo;
   }
+  // The first part of n stages.
+  __device__ __forceinline__ void take_part(GroupedItem* item, int n) const {
+    item->stages = Tr::kCuts ? min(n, Tr::kCut) : n;
+    item->after = n - item->stages;
+  }
   __device__ bool take(GroupedItem* item) {
+    if (Tr::kCuts && item->after) {
+      item->before += item->stages;
+      if constexpr (MODE == kGradW) item->row += (int64_t)item->stages * Tr::kBlock;
+      take_part(item, item->after);
+      if constexpr (MODE == kGradW) item->rows = (int)min((int64_t)item->stages * Tr::kBlock, begin[item->g + 1] - item->row);
+      return true;
+    }
+    item->before = 0;
     if constexpr (MODE == kGradW) {
-      while (next >= end) {
-        step += gridDim.x;
-        if (!runs.units || step >= runs.runs) return false;
-        next = runs.begin(step), end = runs.begin(step + 1);
-      }
+      if (next >= end) return false;
       const int total = prefix[c.groups];
       const int tile = (int)quotient(next, total), t = (int)(next - (int64_t)tile * total);
       const int g = group_of(t, c.groups);
       const int64_t n = min(end - next, (int64_t)(prefix[g + 1] - t));
       item->g = g;
       item->row = begin[g] + (int64_t)(t - prefix[g]) * Tr::kBlock;
-      item->rows = (int)min(n * Tr::kBlock, begin[g + 1] - item->row);
-      item->stages = (int)n;
+      take_part(item, (int)n);
+      item->rows = (int)min((int64_t)item->stages * Tr::kBlock, begin[g + 1] - item->row);
       item->m0 = tile / c.tiles_n * kTileM;
       item->n0 = tile % c.tiles_n * c.tile_n;
-      item->piece = n == prefix[g + 1] - prefix[g] ? -1 : 2 * step + (next != runs.begin(step));
-      item->run = next == runs.begin(step) ? step : -1;
+      item->piece = n == prefix[g + 1] - prefix[g] ? -1 : 2 * (int64_t)blockIdx.x + (next != runs.begin(blockIdx.x));
       item->first = (int64_t)tile * total + prefix[g], item->last = (int64_t)tile * total + prefix[g + 1];
       next += n;
       return true;
@@ -173,8 +186,8 @@ struct GroupedWalk {
       item->rows = (int)min((int64_t)(c.tile_m * c.halves), begin[g + 1] - item->row);
       item->m0 = 0;
       item->n0 = n * c.tile_n;
-      item->stages = g < c.groups ? (c.num_k + Tr::kBlock * c.deep - 1) / (Tr::kBlock * c.deep) : 0;      // rows of no group: zeros
-      item->piece = -1, item->run = -1, item->first = item->last = 0;
+      take_part(item, g < c.groups ? (c.num_k + Tr::kBlock * c.deep - 1) / (Tr::kBlock * c.deep) : 0);      // rows of no group: zeros
+      item->piece = -1, item->first = item->last = 0;
       next += step;
       return true;
     }
@@ -300,10 +313,11 @@ __device__ __noinline__ void put_narrow_rows(const char* staging, int lane, O* t
   }
 }
 // A warp's 32 rows, 128 bytes of each at a time, through shared memory, so that the stores are whole rows of 128 bytes. Warps that share
-// rows take turns.
+// rows take turns. Parts of a sum `before` this one are in carry, where this one is added to them while more come `after`: 128 columns of 16 slices a lane,
+// its own.
 template <typename T, typename O, int MODE>
 __device__ __forceinline__ void store_tile(uint32_t acc, bool empty, char* staging, int lane, int quarter, int turn, int turns, O* out, int64_t ld, int rows,
-                                           int columns, const float* bias, uint32_t acc_free) {
+                                           int columns, const float* bias, uint32_t acc_free, float* carry, int before, int after) {
   using Tr = GroupedTraits<T, MODE>;
   constexpr int kWide = 128 / (int)sizeof(O), kPer = 16 / (int)sizeof(O);
   const int here = min(32, rows - quarter * 32);
@@ -340,6 +354,24 @@ __device__ __forceinline__ void store_tile(uint32_t acc, bool empty, char* stagi
         tmem_fence_before();
         __syncwarp();
         if (lane == 0) barrier_arrive(acc_free);
+      }
+      if constexpr (Tr::kCuts) {
+        float* const at = carry + c0 * 32;
+        if (before)
+#pragma unroll
+          for (int h = 0; h < kWide / 32; ++h)
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              const float4 p = *(const float4*)(at + (32 * h + k) * 32);
+              v[h][k] += p.x, v[h][k + 1] += p.y, v[h][k + 2] += p.z, v[h][k + 3] += p.w;
+            }
+        if (after) {
+#pragma unroll
+          for (int h = 0; h < kWide / 32; ++h)
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) *(float4*)(at + (32 * h + k) * 32) = make_float4(v[h][k], v[h][k + 1], v[h][k + 2], v[h][k + 3]);
+          continue;
+        }
       }
     }
     if (bias)
@@ -518,7 +550,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             for (int i = 0; i < boxes_a; ++i) copy_box(a + i * kBoxBytes, &map_a, item.m0 + i * Tr::kBox, row, bar);
             for (int i = 0; i < boxes_b; ++i) copy_box(b + i * kBoxBytes, &map_b, item.n0 + i * Tr::kBox, row, bar);
           } else {
-            const int first = k * c.deep, last = min(first + c.deep, blocks);
+            const int first = (item.before + k) * c.deep, last = min(first + c.deep, blocks);
             barrier_expect(bar, bytes * (last - first));
             for (int l = first; l < last; ++l, a += block_bytes, b += block_bytes) {
               copy_box(a, &map_a, l * Tr::kBlock, (int)item.row, bar);
@@ -563,7 +595,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const uint32_t acc = tmem + buffer * kAccColumns;
         for (int k = 0; k < item.stages; ++k) {
           if (!(fine = barrier_wait(shared_addr((Tr::kSplit ? ready : full) + stage), phase, gave_up, c.polls))) break;
-          const int left = (MODE == kGradW ? item.rows : c.num_k) - k * Tr::kBlock * c.deep, steps = (min(left, Tr::kBlock * c.deep) + 15) / 16;
+          const int left = MODE == kGradW ? item.rows - k * Tr::kBlock : c.num_k - (item.before + k) * Tr::kBlock * c.deep, steps = (min(left, Tr::kBlock * c.deep) + 15) / 16;
           if (kMends && left < Tr::kBlock && left % 16) {
             barrier_arrive(shared_addr(ready));
             if (!(fine = barrier_wait(shared_addr(ready + 1), mended, gave_up, c.polls))) break;
@@ -634,6 +666,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     uint32_t summed_phase = 0;
     int bias_g = -1, bias_n = -1, buffer = kBuffers - 1;
     uint32_t turns = 0, meetings = 0;
+    float sum[2] = {0.0f, 0.0f};      // of columns of dy
+    float* const carry = Tr::kCuts ? c.carry + ((int64_t)blockIdx.x * 4 + quarter) * 32 * Tr::kMostN + lane * 4 : nullptr;
     const auto meet = [&] {      // of the warps here; false: somebody has given up
       __syncwarp();
       if (lane == 0) barrier_arrive(shared_addr(&met));
@@ -655,7 +689,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       if constexpr (MODE == kGradW) {
         if (c.grad_bias) {
           // the columns of dy, while the products are made of them: as products with ones they took a third of the time of a stage
-          float sum[2] = {0.0f, 0.0f};
+          if (!item.before) sum[0] = sum[1] = 0.0f;
           for (int k = 0; k < item.stages; ++k) {
             if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + summed), summed_phase, gave_up, c.polls)))) break;
             const int valid = item.rows - k * Tr::kBlock;
@@ -667,7 +701,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           if (!fine) break;
           column = sum[0];
           if constexpr (!Tr::kSplit) {      // four threads have a pair of columns
-            if (item.n0 == 0) {
+            if (item.n0 == 0 && !item.after) {
               if (!(fine = meet())) break;
               *(float2*)(bias + (thread >> 6) * 128 + (thread & 63) * 2) = make_float2(sum[0], sum[1]);
               if (!(fine = meet())) break;
@@ -690,13 +724,13 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if constexpr (MODE == kGradW) {
           const int rows = min(kTileM, c.num_m - item.m0), m = quarter * 32 + lane;
           if (quarter * 32 < rows) {
-            if (item.piece < 0)
+            if (item.piece < 0 || item.after)
               store_tile<T, T, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0,
-                                     (int64_t)c.num_n, rows, columns, nullptr, 0u);
+                                     (int64_t)c.num_n, rows, columns, nullptr, 0u, carry, item.before, item.after);
             else
               store_tile<T, float, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows,
-                                         columns, nullptr, 0u);
-            if (c.grad_bias && item.n0 == 0 && turn == 0) {
+                                         columns, nullptr, 0u, carry, item.before, item.after);
+            if (c.grad_bias && item.n0 == 0 && turn == 0 && !item.after) {
               if (m < rows) {
                 if (item.piece < 0) ((T*)c.grad_bias)[(int64_t)item.g * c.num_m + item.m0 + m] = Elem<T>::from_f(column);
                 else c.partial_bias[item.piece * kTileM + m] = column;
@@ -708,7 +742,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const bool stores = MODE != kGradW && quarter * 32 < min(rows, c.tile_m) && turn * (128 / (int)sizeof(T)) < columns;
         if (stores)
           store_tile<T, T, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + (item.row + half * kTileM) * c.num_n + item.n0, (int64_t)c.num_n,
-                                 min(rows, c.tile_m), columns, MODE == kOut && c.bias && !empty ? bias : nullptr, shared_addr(acc_free + buffer));
+                                 min(rows, c.tile_m), columns, MODE == kOut && c.bias && !empty ? bias : nullptr, shared_addr(acc_free + buffer), carry, item.before, item.after);
         if (!empty && !stores) {
           tmem_fence_before();
           __syncwarp();
@@ -717,14 +751,13 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       }
     }
   } else if (MODE == kGradW && warp == 3) {
-    // ---- the plan of the block's runs, which follows from the walk and waits for nothing: k_join_weights reads it whoever gives up
-    if (lane == 0)
-      while (walk.take(&item)) {
-        if (item.run < 0) continue;
-        int64_t* const to = c.plan + 2 + kPlanWords * item.run;
-        to[0] = (int64_t)(item.m0 / kTileM * c.tiles_n + item.n0 / c.tile_n) * c.groups + item.g, to[1] = item.first;
-        to[2] = walk.runs.begin(item.run), to[3] = item.run ? walk.runs.begin(item.run - 1) : 0, to[4] = walk.runs.of(item.last - 1);
-      }
+    // ---- the plan of the block's run, which follows from the walk and waits for nothing: k_join_weights reads it whoever gives up
+    if (lane == 0 && walk.take(&item)) {
+      const int64_t run = blockIdx.x;
+      int64_t* const to = c.plan + 2 + kPlanWords * run;
+      to[0] = (int64_t)(item.m0 / kTileM * c.tiles_n + item.n0 / c.tile_n) * c.groups + item.g, to[1] = item.first;
+      to[2] = walk.runs.begin(run), to[3] = run ? walk.runs.begin(run - 1) : 0, to[4] = walk.runs.of(item.last - 1);
+    }
     // ---- groups without rows
     const int64_t per = (int64_t)c.num_m * c.num_n;
     const bool slices = per * sizeof(T) % 16 == 0;
@@ -943,8 +976,7 @@ static int laid_out(const void* data, int64_t stack, int64_t rows, int64_t colum
 // Columns of a tile: as few tiles as can be, of the same width.
 static int tile_columns(int64_t n, int most) { return (int)(ceil_div(ceil_div(n, ceil_div(n, most)), 16) * 16); }
 
-// Runs of stages that dw is cut into at most, and partial sums that come of it: one for every block, or more where a run would have over
-// 1024 rows of fp32, whose sums the tensor cores cut rather than round.
+// Runs of stages that dw is cut into at most, one for every block, and partial sums that come of it.
 struct WeightPlan {
   int tile_n, tiles_m, tiles_n;
   int64_t ranges, pieces;
@@ -957,11 +989,16 @@ static WeightPlan weight_plan(int64_t rows, int64_t dim, int64_t out_dim, int64_
   p.tiles_m = (int)ceil_div(out_dim, kTileM);
   p.tiles_n = (int)ceil_div(dim, p.tile_n);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, most = (ceil_div(rows, Tr::kBlock) + groups) * tiles;
-  p.ranges = kNumSMs;
-  if (Tr::kSplit) p.ranges *= std::max<int64_t>(1, ceil_div(rows * tiles, (int64_t)kNumSMs * 1024));
-  p.ranges = grouped_runs(most, p.ranges).runs;
+  p.ranges = grouped_runs(most, kNumSMs).runs;
   p.pieces = 2 * p.ranges;
   return p;
+}
+
+// The blocks' tiles of sums that are brought out in parts.
+template <typename T>
+static size_t carry_room(int64_t rows, bool backward) {
+  using Tr = GroupedTraits<T, kGradW>;
+  return Tr::kCuts && backward && rows > Tr::kCut * Tr::kBlock ? (size_t)kNumSMs * kTileM * Tr::kMostN * 4 : 0;
 }
 
 template <typename T, int MODE>
@@ -1005,7 +1042,7 @@ static int code_of() { return sizeof(T) == 4 ? APT_F32 : std::is_same<T, __half>
 // Rows against weights: out (contraction along w's rows) or dx (across them).
 template <typename T, int MODE>
 static int rows_product(const Operand& rows, const Operand& weight, int64_t num_n, const void* bias, const int64_t* offsets, int groups, void* out,
-                        int32_t* status, cudaStream_t s) {
+                        char* carry, int32_t* status, cudaStream_t s) {
   using Tr = GroupedTraits<T, MODE>;
   GroupedCall c = {};
   c.offsets = offsets, c.rows = rows.rows, c.groups = groups;
@@ -1026,7 +1063,7 @@ static int rows_product(const Operand& rows, const Operand& weight, int64_t num_
   }
   c.tile_n = tile_columns(num_n, (int)most), c.tiles_n = (int)ceil_div(num_n, c.tile_n);
   c.a = rows.data, c.b = weight.data, c.pitch_a = rows.pitch, c.pitch_b = weight.pitch;
-  c.bias = bias, c.out = out, c.status = status;
+  c.bias = bias, c.out = out, c.carry = (float*)carry, c.status = status;
   CUtensorMap a, b;
   if (const int e = make_map(&a, code_of<T>(), rows, Tr::kBox, c.tile_m)) return e;
   if (const int e = make_map(&b, code_of<T>(), weight, Tr::kBox, MODE == kOut ? c.tile_n : Tr::kBlock)) return e;
@@ -1036,15 +1073,17 @@ static int rows_product(const Operand& rows, const Operand& weight, int64_t num_
 template <typename T>
 static int linear_forward(const void* x, int64_t rows, int64_t dim, const void* weight, const void* bias, int64_t out_dim, const int64_t* offsets, int groups,
                           void* out, char* room, int32_t* status, cudaStream_t s) {
+  char* const carry = room;
+  room += carry_room<T>(rows, false);
   Operand a, w;
   if (const int e = laid_out(x, 0, rows, dim, sizeof(T), &room, &a, s)) return e;
   if (const int e = laid_out(weight, groups, out_dim, dim, sizeof(T), &room, &w, s)) return e;
-  return rows_product<T, kOut>(a, w, out_dim, bias, offsets, groups, out, status, s);
+  return rows_product<T, kOut>(a, w, out_dim, bias, offsets, groups, out, carry, status, s);
 }
 
 template <typename T>
 static size_t linear_room(int64_t rows, int64_t dim, int64_t out_dim, int64_t groups, bool backward) {
-  size_t bytes = room_of(rows, dim, sizeof(T)) + room_of(groups * out_dim, dim, sizeof(T));
+  size_t bytes = carry_room<T>(rows, backward) + room_of(rows, dim, sizeof(T)) + room_of(groups * out_dim, dim, sizeof(T));
   if (backward) {
     const WeightPlan p = weight_plan<T>(rows, dim, out_dim, groups);
     bytes += room_of(rows, out_dim, sizeof(T)) + align_up((size_t)(2 + kPlanWords * p.ranges) * 8, 256) + (size_t)p.pieces * kTileM * (p.tile_n + 1) * 4;
@@ -1065,12 +1104,14 @@ static int linear_backward(const void* x, int64_t rows, int64_t dim, const void*
     return APT_OK;
   }
   if (!grad_x && !grad_weight) return APT_OK;
+  char* const carry = room;
+  room += carry_room<T>(rows, true);
   Operand dy;
   if (const int e = laid_out(grad, 0, rows, out_dim, sizeof(T), &room, &dy, s)) return e;
   if (grad_x) {
     Operand w;
     if (const int e = laid_out(weight, groups, out_dim, dim, sizeof(T), &room, &w, s)) return e;
-    if (const int e = rows_product<T, kGradX>(dy, w, dim, nullptr, offsets, groups, grad_x, status, s)) return e;
+    if (const int e = rows_product<T, kGradX>(dy, w, dim, nullptr, offsets, groups, grad_x, carry, status, s)) return e;
   }
   if (grad_weight) {
     using Tr = GroupedTraits<T, kGradW>;
@@ -1082,7 +1123,7 @@ static int linear_backward(const void* x, int64_t rows, int64_t dim, const void*
     c.num_m = (int)out_dim, c.num_n = (int)dim;
     c.tile_n = p.tile_n, c.tiles_m = p.tiles_m, c.tiles_n = p.tiles_n, c.ranges = p.ranges;
     c.a = dy.data, c.b = in.data, c.pitch_a = dy.pitch, c.pitch_b = in.pitch;
-    c.out = grad_weight, c.grad_bias = grad_bias, c.status = status;
+    c.out = grad_weight, c.grad_bias = grad_bias, c.carry = (float*)carry, c.status = status;
     c.plan = (int64_t*)room;
     c.partial = (float*)(room + align_up((size_t)(2 + kPlanWords * p.ranges) * 8, 256));
     c.partial_bias = c.partial + (size_t)p.pieces * kTileM * p.tile_n;

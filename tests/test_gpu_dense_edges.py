@@ -124,3 +124,17 @@ def test_a_nan_is_one_whatever_its_bits(bits):
     gx, gw, _ = apt_b200.grouped_linear_backward(x, weight, offsets, grad)
     assert torch.isnan(gx[:, 3]).all() and torch.isfinite(gx[:, :3]).all() and torch.isnan(gw[0, :, 9]).all() and torch.isfinite(gw[0, :, :9]).all()
     ops.check_status()
+
+
+def test_weight_gradients_of_very_many_tiles():
+    """4096 tiles of 16500 rows: as many runs as there are blocks, and no more."""
+    rows, dim = 16500, 8192
+    x, grad = torch.randn((rows, dim), device="cuda", generator=_gen(12)), torch.randn((rows, dim), device="cuda", generator=_gen(13))
+    weight = torch.zeros((2, dim, dim), device="cuda")
+    gw = apt_b200.grouped_linear_backward(x, weight, _ends(16000, 500), grad, want_x=False)[1]
+    ops.check_status()
+    for g, (b, e) in enumerate(((0, 16000), (16000, 16500))):
+        for some in (slice(0, 64), slice(4000, 4064), slice(8128, 8192)):
+            want = grad[b:e, some].double().T @ x[b:e].double()
+            size = grad[b:e, some].double().abs().T @ x[b:e].double().abs()
+            assert ((gw[g, some].double() - want).abs() <= 80 * 2.0 ** -23 * size).all()

@@ -10,7 +10,10 @@
 // tiles from the ends and its warps walk it. In dw a run of stages, as long for every block, may begin and end within a sum: it leaves
 // partial sums, which k_join_weights adds up.
 //
-// In fp32 a sum of dw is brought out every 1024 rows and added up by rounding, for the tensor cores cut their sums off instead.
+// The tensor cores cut their sums off instead of rounding them: sums of one sign lose half a unit of the 24th bit with every 16 terms (8192 terms in one
+// sum: 2.6e-5; 262144 rows in dw: 1.1e-3, twice the rounding of f16). So a sum is brought out in parts (GroupedTraits::kCut), which are added up in
+// fp32, rounded to nearest: 3e-6 in fp32, 3e-5 in dw of 16 bits, where the rounding of f16 is 4.9e-4. A contraction of out or dx in 16 bits has 8192 terms at
+// most and is not cut.
 //
 // Operands stay as they are in memory, row by row; whether rows run along the contraction or across it is a bit of the product. A box
 // that reaches past a matrix is filled with zeros. Past the end of a group within a matrix it has the next group's rows: in out and dx those are
@@ -48,9 +51,10 @@ struct GroupedTraits {
   // warps that bring tiles out: two for each quarter of tensor memory's lanes, or one beside the eight that take fp32 apart
   static constexpr int kOutWarps = kSplit ? 4 : 8;
   static constexpr int kThreads = kSplit ? 512 : 384;
-  // a sum in tensor memory has so many stages at most: 1024 rows
-  static constexpr bool kCuts = kSplit && MODE == kGradW;
-  static constexpr int kCut = 32;
+  // a sum in tensor memory has so many stages at most: 1024 terms of fp32, 8192 rows of 16 bits (with 4096, 65536 x 1024 -> 1024 bf16, dw and db 182 -> 205 us:
+  // the warps that bring parts out are those that add up db, for which the stages wait)
+  static constexpr bool kCuts = kSplit || MODE == kGradW;
+  static constexpr int kCut = kSplit ? 32 : 128;
   // bytes of a tile of n rows (or columns) in a stage as copied, and of one bf16 piece of it
   static __host__ __device__ constexpr int copied(int n, bool mn) { return mn ? (n + kBox - 1) / kBox * kBlock * 128 : n * 128; }
   static __host__ __device__ constexpr int piece(int n, bool mn) { return mn ? (n + 63) / 64 * kBlock * 128 : (n + 31) / 32 * 32 * kBlock * 2; }
@@ -996,9 +1000,11 @@ static WeightPlan weight_plan(int64_t rows, int64_t dim, int64_t out_dim, int64_
 
 // The blocks' tiles of sums that are brought out in parts.
 template <typename T>
-static size_t carry_room(int64_t rows, bool backward) {
+static size_t carry_room(int64_t rows, int64_t dim, int64_t out_dim, bool backward) {
   using Tr = GroupedTraits<T, kGradW>;
-  return Tr::kCuts && backward && rows > Tr::kCut * Tr::kBlock ? (size_t)kNumSMs * kTileM * Tr::kMostN * 4 : 0;
+  const int64_t terms = (int64_t)Tr::kCut * Tr::kBlock;
+  const bool cut = backward ? rows > terms || (Tr::kSplit && out_dim > terms) : Tr::kSplit && dim > terms;
+  return cut ? (size_t)kNumSMs * kTileM * Tr::kMostN * 4 : 0;
 }
 
 template <typename T, int MODE>
@@ -1074,7 +1080,7 @@ template <typename T>
 static int linear_forward(const void* x, int64_t rows, int64_t dim, const void* weight, const void* bias, int64_t out_dim, const int64_t* offsets, int groups,
                           void* out, char* room, int32_t* status, cudaStream_t s) {
   char* const carry = room;
-  room += carry_room<T>(rows, false);
+  room += carry_room<T>(rows, dim, out_dim, false);
   Operand a, w;
   if (const int e = laid_out(x, 0, rows, dim, sizeof(T), &room, &a, s)) return e;
   if (const int e = laid_out(weight, groups, out_dim, dim, sizeof(T), &room, &w, s)) return e;
@@ -1083,7 +1089,7 @@ static int linear_forward(const void* x, int64_t rows, int64_t dim, const void* 
 
 template <typename T>
 static size_t linear_room(int64_t rows, int64_t dim, int64_t out_dim, int64_t groups, bool backward) {
-  size_t bytes = carry_room<T>(rows, backward) + room_of(rows, dim, sizeof(T)) + room_of(groups * out_dim, dim, sizeof(T));
+  size_t bytes = carry_room<T>(rows, dim, out_dim, backward) + room_of(rows, dim, sizeof(T)) + room_of(groups * out_dim, dim, sizeof(T));
   if (backward) {
     const WeightPlan p = weight_plan<T>(rows, dim, out_dim, groups);
     bytes += room_of(rows, out_dim, sizeof(T)) + align_up((size_t)(2 + kPlanWords * p.ranges) * 8, 256) + (size_t)p.pieces * kTileM * (p.tile_n + 1) * 4;
@@ -1105,7 +1111,7 @@ static int linear_backward(const void* x, int64_t rows, int64_t dim, const void*
   }
   if (!grad_x && !grad_weight) return APT_OK;
   char* const carry = room;
-  room += carry_room<T>(rows, true);
+  room += carry_room<T>(rows, dim, out_dim, true);
   Operand dy;
   if (const int e = laid_out(grad, 0, rows, out_dim, sizeof(T), &room, &dy, s)) return e;
   if (grad_x) {

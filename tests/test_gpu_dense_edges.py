@@ -126,6 +126,54 @@ def test_a_nan_is_one_whatever_its_bits(bits):
     ops.check_status()
 
 
+def _one_sign(*shape, seed, dtype=torch.float32, scale=1.0):
+    """Numbers of 0.5 to 1.5, and columns of factors of 1 to 2, so that roundings of their sums are of either sign."""
+    gen = _gen(seed)
+    return ((torch.rand(shape, device="cuda", generator=gen) + 0.5) * (torch.rand(shape[-1], device="cuda", generator=gen) + 1.0) * scale).to(dtype)
+
+
+# A part of a sum has at most 64 steps of 16 terms, each of which loses less than a unit of 2^-23 of it; eight parts are rounded as they are added up,
+# and operands taken apart lose 2^-22: 74 units, whatever the number of terms. In one sum 8192 terms lose 216 units.
+@pytest.mark.parametrize("dim,n", [(1024, 130), (1040, 64), (2049, 47), (8192, 200), (8190, 130)])
+def test_long_contractions_of_one_sign(dim, n):
+    offsets = _ends(200, 0, 101)
+    for rows_of, out_dim in ((dim, n), (n, dim)):
+        x, weight = _one_sign(310, rows_of, seed=6), _one_sign(3, out_dim, rows_of, seed=7)
+        bias, grad = _one_sign(3, out_dim, seed=8), _one_sign(310, out_dim, seed=9)
+        out = apt_b200.grouped_linear(x, weight, offsets, bias)
+        gx = apt_b200.grouped_linear_backward(x, weight, offsets, grad, want_weight=False, want_bias=False)[0]
+        for g, (b, e) in enumerate(((0, 200), (200, 200), (200, 301))):
+            for got, want in ((out, x[b:e].double() @ weight[g].double().T + bias[g].double()), (gx, grad[b:e].double() @ weight[g].double())):
+                assert ((got[b:e].double() - want).abs() <= 74 * 2.0 ** -23 * want).all()
+        assert not out[301:].any() and not gx[301:].any()
+    ops.check_status()
+
+
+# Parts of 8192 rows (fp32: 1024) have 512 (64) steps, and are added up one by one with errors of either sign, m of them: sqrt(m) / 2 units at three
+# deviations. The mean over what is looked at has the roundings of the results, uniform in half a unit of theirs, as noise besides, at five deviations.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,dim,n", [([262144], 512, 264), ([131072], 1100, 1000), ([70000, 3, 60007], 130, 70)])
+def test_weight_gradients_of_long_groups_of_one_sign(sizes, dim, n, dtype):
+    rows = sum(sizes)
+    x, grad = _one_sign(rows, dim, seed=10, dtype=dtype, scale=1 / 64), _one_sign(rows, n, seed=11, dtype=dtype, scale=1 / 64)
+    weight = torch.zeros((len(sizes), n, dim), device="cuda", dtype=dtype)
+    _, gw, gb = apt_b200.grouped_linear_backward(x, weight, _ends(*sizes), grad, want_x=False)
+    ops.check_status()
+    steps, unit = (64, 0.0) if dtype == torch.float32 else (512, UNIT[dtype])
+    end = 0
+    for g, size in enumerate(sizes):
+        b, end = end, end + size
+        for columns in (slice(0, 40), slice(n - 40, n)):
+            want = grad[b:end, columns].double().T @ x[b:end].double()
+            off = (gw[g, columns].double() - want) / want
+            parts = size / (16 * steps) + 1
+            loss = (steps + 3 * parts ** 0.5 / 2 + 4) * 2.0 ** -23
+            assert float(off.abs().max()) <= loss + unit
+            assert abs(float(off.mean())) <= loss + 5 * unit / (3 * off.numel()) ** 0.5
+        want = grad[b:end].double().sum(0)
+        assert (((gb[g].double() - want) / want).abs() <= 2e-6 + unit).all()
+
+
 def test_weight_gradients_of_very_many_tiles():
     """4096 tiles of 16500 rows: as many runs as there are blocks, and no more."""
     rows, dim = 16500, 8192

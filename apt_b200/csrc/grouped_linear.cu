@@ -1035,8 +1035,13 @@ static int launch_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap
   c.piece_stages = Tr::kSplit ? 2 : 0;
   c.copied_stages = std::min(kMaxStages, (room - kept - c.piece_stages * pieces) / copied);
   const int bytes = lists + Tr::kOutWarps * 4096 + kept + c.copied_stages * copied + c.piece_stages * pieces;
-  static const cudaError_t allowed = cudaFuncSetAttribute(k_grouped<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
-  APT_CUDA(allowed);
+  static bool sized[64] = {};
+  int dev = 0;
+  APT_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !sized[dev]) {
+    APT_CUDA(cudaFuncSetAttribute(k_grouped<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+    if (dev < 64) sized[dev] = true;
+  }
   // over half of an SM's shared memory, so that no two blocks share one: each takes all of its tensor memory
   APT_FOLLOW((k_grouped<T, MODE>), std::min<int64_t>(items, kNumSMs), Tr::kThreads, std::max(bytes, 116 * 1024), s, a, b, c);
   return APT_OK;

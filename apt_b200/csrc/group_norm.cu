@@ -141,7 +141,10 @@ extern "C" int apt_group_norm_forward(int dtype, int param_dtype, const void* x,
                                       void* stream) {
   using namespace apt;
   if (const int e = norm_check("apt_group_norm_forward", dtype, param_dtype, rows, dim, groups, offsets, segments, eps, act, p)) return e;
-  if (rows == 0) return APT_OK;
+  if (rows == 0) {
+    if (stats) APT_CUDA(cudaMemsetAsync(stats, 0, (size_t)segments * groups * 8, (cudaStream_t)stream));
+    return APT_OK;
+  }
   const NormShape s = norm_shape(rows, dim, groups, offsets, segments);
   APT_CHECK_ARG(x && out && status_word && (stats || (!offsets && segments == rows && dim / groups <= APT_GROUP_NORM_ROW_CHANNELS)), "apt_group_norm_forward: null buffer");
   APT_CHECK_ARG(workspace_bytes >= apt_group_norm_workspace_bytes(dtype, rows, dim, groups, offsets, segments, 0), "apt_group_norm_forward: workspace too small");

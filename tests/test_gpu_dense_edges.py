@@ -186,3 +186,14 @@ def test_weight_gradients_of_very_many_tiles():
             want = grad[b:e, some].double().T @ x[b:e].double()
             size = grad[b:e, some].double().abs().T @ x[b:e].double().abs()
             assert ((gw[g, some].double() - want).abs() <= 80 * 2.0 ** -23 * size).all()
+
+
+# ------------------------------------------------------------------------------------------------------ group norm
+def test_statistics_of_segments_without_rows_are_zeros():
+    for rows in (0, 7):
+        filled = torch.full((4, 3, 2), 7.0, device="cuda")
+        del filled      # what the statistics are written to held something else before
+        offsets = torch.tensor([0, 0, rows, rows, rows], device="cuda")
+        _, stats = apt_b200.group_norm_act(torch.randn((rows, 12), device="cuda"), 3, offsets=offsets, return_stats=True)
+        assert stats.shape == (4, 3, 2) and not stats[[0, 2, 3]].any() and bool(stats[1].all()) == (rows > 0)
+    ops.check_status()

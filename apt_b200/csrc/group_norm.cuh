@@ -845,7 +845,7 @@ k_norm_join(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
     int many = 0;
     if (seg < s.segments) {
       const RowRange r = segment_rows(s, seg);
-      if (!BACK && s.offsets && lane == 0 && bad_group(s.offsets, (int)seg, s.rows)) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
+      if (s.offsets && lane == 0 && bad_group(s.offsets, (int)seg, s.rows)) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
       const NormPieces p(s, c, t, seg, r);
       many = r.end > r.begin && p.last - p.first >= kFewPieces;
       if (!many)
@@ -870,7 +870,7 @@ k_norm_join(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
   for (; rest; rest &= rest - 1) {
     const int64_t seg = block * t.join_segments + __ffs(rest) - 1;
     const RowRange r = segment_rows(s, seg);
-    if (!BACK && t.join_segments == 1 && s.offsets && blockIdx.y == 0 && threadIdx.x == 0 && bad_group(s.offsets, (int)seg, s.rows))
+    if (t.join_segments == 1 && s.offsets && blockIdx.y == 0 && threadIdx.x == 0 && bad_group(s.offsets, (int)seg, s.rows))
       atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
     const NormPieces p(s, c, t, seg, r);
     const int width = t.join_groups, lane = threadIdx.x / width, lanes = 256 / width;
@@ -1013,7 +1013,7 @@ __global__ void __launch_bounds__(256) k_norm_wide(const __grid_constant__ NormS
   for (int64_t item = blockIdx.x; item < s.segments * s.groups; item += gridDim.x) {
     const int64_t seg = item / s.groups, c0 = item % s.groups * s.per;
     const RowRange r = segment_rows(s, seg);
-    if (!BACK && s.offsets && c0 == 0 && threadIdx.x == 0 && bad_group(s.offsets, (int)seg, s.rows)) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
+    if (s.offsets && c0 == 0 && threadIdx.x == 0 && bad_group(s.offsets, (int)seg, s.rows)) atomicOr(c.status, APT_FLAG_BAD_OFFSETS);
     const float inv = 1.0f / ((float)(r.end - r.begin) * (float)s.per);
     const auto walk = [&](auto&& f) {
       for (int64_t row = r.begin; row < r.end; ++row)

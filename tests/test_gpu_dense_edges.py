@@ -197,3 +197,22 @@ def test_statistics_of_segments_without_rows_are_zeros():
         _, stats = apt_b200.group_norm_act(torch.randn((rows, 12), device="cuda"), 3, offsets=offsets, return_stats=True)
         assert stats.shape == (4, 3, 2) and not stats[[0, 2, 3]].any() and bool(stats[1].all()) == (rows > 0)
     ops.check_status()
+
+
+# tiles of segments, many segments (joined eight a block), groups that a block walks over
+@pytest.mark.parametrize("dim,segments", [(64, 2), (64, 1500), (4106, 2)])
+def test_the_backward_looks_at_the_ends_too(dim, segments):
+    x = torch.randn((2000, dim), device="cuda", generator=_gen(14))
+    good = torch.arange(segments + 1, device="cuda")
+    good[-1] = 2000
+    _, stats = apt_b200.group_norm_act(x, 2, offsets=good, return_stats=True)
+    ops.check_status()
+    for place, end in ((0, 1), (1, 1999), (-1, 2001), (1, -5)):
+        bad = good.clone()
+        bad[place] = end
+        if segments == 1500 or not (bad.diff() >= 0).all() or place != 1:
+            apt_b200.group_norm_act_backward(x, x, stats, 2, offsets=bad)
+            with pytest.raises(RuntimeError, match="row groups"):
+                ops.check_status()
+    apt_b200.group_norm_act_backward(x, x, stats, 2, offsets=good)
+    ops.check_status()

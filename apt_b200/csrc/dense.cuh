@@ -150,5 +150,7 @@ __device__ __forceinline__ RowRange group_rows(const int64_t* offsets, int g, in
 __device__ __forceinline__ bool bad_group(const int64_t* offsets, int g, int64_t rows) {
   return offsets[g + 1] < offsets[g] || offsets[g + 1] > rows || (g == 0 && offsets[0] != 0);
 }
+// The same of all groups, where there are no rows and so no kernel that looks at them (group_norm.cu).
+int look_at_ends(const int64_t* offsets, int64_t groups, int64_t rows, int32_t* status, cudaStream_t s);
 
 }  // namespace apt

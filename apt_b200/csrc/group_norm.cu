@@ -10,6 +10,16 @@ extern template int norm<__nv_bfloat16, true>(const NormShape&, const NormCall&,
 extern template int norm<__half, false>(const NormShape&, const NormCall&, const NormPlan&, cudaStream_t);
 extern template int norm<__half, true>(const NormShape&, const NormCall&, const NormPlan&, cudaStream_t);
 
+__global__ void __launch_bounds__(256) k_look_at_ends(const int64_t* __restrict__ offsets, int groups, int64_t rows, int32_t* status) {
+  wait_for_previous();
+  const int g = blockIdx.x * 256 + threadIdx.x;
+  if (g < groups && bad_group(offsets, g, rows)) atomicOr(status, APT_FLAG_BAD_OFFSETS);
+}
+int look_at_ends(const int64_t* offsets, int64_t groups, int64_t rows, int32_t* status, cudaStream_t s) {
+  if (offsets && groups > 0 && status) APT_FOLLOW(k_look_at_ends, ceil_div(groups, 256), 256, 0, s, offsets, (int)groups, rows, status);
+  return APT_OK;
+}
+
 // Elements of an access that `run` elements from any of the addresses on are a whole number of: 16, 8 or 4 bytes, or one.
 static int slice_of(int64_t run, size_t size, uintptr_t addresses) {
   for (const int bytes : {16, 8, 4})
@@ -143,7 +153,7 @@ extern "C" int apt_group_norm_forward(int dtype, int param_dtype, const void* x,
   if (const int e = norm_check("apt_group_norm_forward", dtype, param_dtype, rows, dim, groups, offsets, segments, eps, act, p)) return e;
   if (rows == 0) {
     if (stats) APT_CUDA(cudaMemsetAsync(stats, 0, (size_t)segments * groups * 8, (cudaStream_t)stream));
-    return APT_OK;
+    return look_at_ends(offsets, segments, 0, status_word, (cudaStream_t)stream);
   }
   const NormShape s = norm_shape(rows, dim, groups, offsets, segments);
   APT_CHECK_ARG(x && out && status_word && (stats || (!offsets && segments == rows && dim / groups <= APT_GROUP_NORM_ROW_CHANNELS)), "apt_group_norm_forward: null buffer");
@@ -165,7 +175,7 @@ extern "C" int apt_group_norm_backward(int dtype, int param_dtype, const void* x
     const size_t bytes = (size_t)dim * (param_dtype == APT_F32 ? 4 : 2);
     if (grad_weight) APT_CUDA(cudaMemsetAsync(grad_weight, 0, bytes, st));
     if (grad_bias) APT_CUDA(cudaMemsetAsync(grad_bias, 0, bytes, st));
-    return APT_OK;
+    return look_at_ends(offsets, segments, 0, status_word, st);
   }
   APT_CHECK_ARG(x && grad_out && grad_x && status_word && (stats || (!offsets && segments == rows && dim / groups <= APT_GROUP_NORM_ROW_CHANNELS)), "apt_group_norm_backward: null buffer");
   APT_CHECK_ARG(workspace_bytes >= apt_group_norm_workspace_bytes(dtype, rows, dim, groups, offsets, segments, 1), "apt_group_norm_backward: workspace too small");

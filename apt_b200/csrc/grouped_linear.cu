@@ -1112,7 +1112,7 @@ static int linear_backward(const void* x, int64_t rows, int64_t dim, const void*
   if (rows == 0) {
     if (grad_weight) APT_CUDA(cudaMemsetAsync(grad_weight, 0, (size_t)groups * out_dim * dim * sizeof(T), s));
     if (grad_weight && grad_bias) APT_CUDA(cudaMemsetAsync(grad_bias, 0, (size_t)groups * out_dim * sizeof(T), s));
-    return APT_OK;
+    return look_at_ends(offsets, groups, 0, status, s);
   }
   if (!grad_x && !grad_weight) return APT_OK;
   char* const carry = room;
@@ -1174,7 +1174,7 @@ extern "C" int apt_grouped_linear_forward(int dtype, const void* x, int64_t rows
                                           int32_t* status_word, void* stream) {
   using namespace apt;
   if (const int e = linear_check("apt_grouped_linear_forward", dtype, rows, dim, out_dim, groups, workspace, workspace_bytes, 0)) return e;
-  if (rows == 0) return APT_OK;
+  if (rows == 0) return look_at_ends(offsets, groups, 0, status_word, (cudaStream_t)stream);
   APT_CHECK_ARG(x && weight && offsets && out && status_word, "apt_grouped_linear_forward: null buffer");
   APT_CHECK_ARG(((uintptr_t)x | (uintptr_t)weight | (uintptr_t)out) % 16 == 0, "apt_grouped_linear_forward: buffers not aligned to 16 bytes");
   const cudaStream_t s = (cudaStream_t)stream;

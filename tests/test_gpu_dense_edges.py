@@ -216,3 +216,17 @@ def test_the_backward_looks_at_the_ends_too(dim, segments):
                 ops.check_status()
     apt_b200.group_norm_act_backward(x, x, stats, 2, offsets=good)
     ops.check_status()
+
+
+def test_ends_of_calls_without_rows_are_looked_at():
+    x, weight = torch.zeros((0, 16), device="cuda"), torch.ones((2, 4, 16), device="cuda")
+    grad, stats = torch.zeros((0, 4), device="cuda"), torch.zeros((2, 2, 2), device="cuda")
+    for ends in ([0, 0, 0], [0, 0, 5], [1, 1, 1], [0, 3, 0]):
+        offsets = torch.tensor(ends, device="cuda")
+        for call in (lambda: apt_b200.grouped_linear(x, weight, offsets), lambda: apt_b200.grouped_linear_backward(x, weight, offsets, grad),
+                     lambda: apt_b200.group_norm_act(x, 2, offsets=offsets), lambda: apt_b200.group_norm_act_backward(x, x, stats, 2, offsets=offsets)):
+            call()
+            if any(ends):
+                with pytest.raises(RuntimeError, match="row groups"):
+                    ops.check_status()
+            ops.check_status()

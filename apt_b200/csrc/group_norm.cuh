@@ -996,6 +996,17 @@ __device__ __forceinline__ float block_sum(float v, float* shared) {
   for (int k = 0; k < 8; ++k) v += shared[k];
   return v;
 }
+// A sum of however many numbers: what each addition loses is kept beside it (Knuth's two-sum). One thread may have a 256th of all of a long segment's, whose
+// running mean stands still, and whose squares, of few different values in 16 bits, are rounded the same way every time (1e-4 of 20000 x 2053).
+struct LongSum {
+  float sum = 0.0f, lost = 0.0f;
+  __device__ __forceinline__ void add(float v) {
+    const float all = sum + v, added = all - sum;
+    lost += (sum - (all - added)) + (v - added);
+    sum = all;
+  }
+  __device__ __forceinline__ float get() const { return sum + lost; }
+};
 template <typename T>
 __device__ __forceinline__ float2 wide_xh_dz(const NormCall& c, int64_t e, int64_t col, float2 st, float* gamma) {
   const float g = *gamma = param<T>(c.weight, c.wide_params, col, 1.0f);
@@ -1020,15 +1031,14 @@ __global__ void __launch_bounds__(256) k_norm_wide(const __grid_constant__ NormS
         for (int k = threadIdx.x; k < s.per; k += 256) f(row * s.dim + c0 + k, c0 + k);
     };
     if constexpr (!BACK) {
-      float sum = 0.0f;
-      walk([&](int64_t e, int64_t) { sum += Elem<T>::to_f(x[e]); });
-      const float mean = block_sum(sum, shared) * inv;
-      sum = 0.0f;
+      LongSum all, squares;
+      walk([&](int64_t e, int64_t) { all.add(Elem<T>::to_f(x[e])); });
+      const float mean = block_sum(all.get(), shared) * inv;
       walk([&](int64_t e, int64_t) {
         const float d = Elem<T>::to_f(x[e]) - mean;
-        sum = fmaf(d, d, sum);
+        squares.add(d * d);
       });
-      const float rstd = rsqrtf(block_sum(sum, shared) * inv + c.eps);
+      const float rstd = rsqrtf(block_sum(squares.get(), shared) * inv + c.eps);
       if (threadIdx.x == 0) c.stats[item] = r.end > r.begin ? make_float2(mean, rstd) : make_float2(0.0f, 0.0f);
       walk([&](int64_t e, int64_t col) {
         float v[1] = {(Elem<T>::to_f(x[e]) - mean) * rstd};
@@ -1038,13 +1048,14 @@ __global__ void __launch_bounds__(256) k_norm_wide(const __grid_constant__ NormS
       });
     } else {
       const float2 st = c.stats[item];
-      float a = 0.0f, b = 0.0f, gamma;
+      LongSum dxhs, dxh_xhs;
+      float gamma;
       walk([&](int64_t e, int64_t col) {
         const float2 v = wide_xh_dz<T>(c, e, col, st, &gamma);
         const float dxh = __fmul_rn(v.y, gamma);
-        a += dxh, b = fmaf(dxh, v.x, b);
+        dxhs.add(dxh), dxh_xhs.add(dxh * v.x);
       });
-      a = block_sum(a, shared) * inv, b = block_sum(b, shared) * inv;
+      const float a = block_sum(dxhs.get(), shared) * inv, b = block_sum(dxh_xhs.get(), shared) * inv;
       walk([&](int64_t e, int64_t col) {
         const float2 v = wide_xh_dz<T>(c, e, col, st, &gamma);
         out[e] = Elem<T>::from_f(st.y * (__fmul_rn(v.y, gamma) - a - v.x * b));

@@ -230,3 +230,33 @@ def test_ends_of_calls_without_rows_are_looked_at():
                 with pytest.raises(RuntimeError, match="row groups"):
                     ops.check_status()
             ops.check_status()
+
+
+def _statistics(x, groups, ends):
+    """Mean and 1 / deviation of each segment that has rows, in 64 bits."""
+    v = [x[b:e].double().view(e - b, groups, -1) for b, e in zip(ends, ends[1:])]
+    return torch.stack([t.mean((0, 2)) for t in v]), torch.stack([1 / torch.sqrt(t.var((0, 2), unbiased=False) + 1e-5) for t in v])
+
+
+# 301 with a deviation of 0.3. A mean is a sum rounded eight times as it is joined: 16 units. The variance's terms are 0.3^2, off by 2^-22 of themselves
+# each way and by the square of the mean's error, (3e-4)^2: 2e-5 of it. A sum whose losses are lost had the mean off by 0.27 in 20000 rows of 2053.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,groups,sizes", [(2053, 1, [19000, 1000]), (70001, 1, [1, 2]), (4106, 2, [1, 3000])])
+def test_groups_that_a_block_walks_over_far_from_zero(dim, groups, sizes, dtype):
+    x = (torch.randn((sum(sizes), dim), device="cuda", generator=_gen(15)) * 0.3 + 301.0).to(dtype)
+    ends = _ends(*sizes)
+    _, stats = apt_b200.group_norm_act(x, groups, offsets=ends, return_stats=True)
+    mean, rstd = _statistics(x, groups, ends.tolist())
+    assert ((stats[..., 0].double() - mean).abs() <= 16 * 2.0 ** -24 * 302).all()
+    assert ((stats[..., 1].double() / rstd - 1).abs() <= 2e-5).all()
+
+
+def test_a_gradient_without_a_slope_over_a_long_segment():
+    """dxh is 0.9 everywhere, so dx is zero but for roundings of its three terms: 2^-22 of 0.9 and of |xh|'s share of the second mean, itself zero but for
+    the mean of xh (2e-5) and roundings."""
+    rows, dim = 40000, 2053
+    x = torch.randn((rows, dim), device="cuda", generator=_gen(16))
+    ends = _ends(rows)
+    _, stats = apt_b200.group_norm_act(x, 1, offsets=ends, return_stats=True)
+    grad = apt_b200.group_norm_act_backward(x, torch.full_like(x, 0.9), stats, 1, offsets=ends)[0]
+    assert float(grad.abs().max()) <= 0.9 * (2.0 ** -22 + 7 * 2e-5)

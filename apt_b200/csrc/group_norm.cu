@@ -53,22 +53,29 @@ static NormPlan norm_plan(const NormShape& s, size_t size, uintptr_t addresses, 
     }
   }
   NormTiles& t = p.tiles;
-  p.slice = slice_of(s.dim, size, addresses);
-  // a group wider than a block's columns is cut into equal parts; rows by themselves that come here stay a block's, walk by walk
-  t.fold = 1;
-  if (s.per > kMostColumns && (s.offsets || s.per_segment > 1)) {
-    t.fold = (int)ceil_div(s.per, kMostColumns);
-    while (s.per / t.fold >= 64 && s.per % (t.fold * p.slice)) ++t.fold;
+  // A group wider than a block's columns is cut into equal parts (rows by themselves that come here stay a block's, walk by walk), and a block has whole
+  // groups (or parts), a chunk of them that begins on an access. Where whole accesses leave no such chunk (eight groups of 513 channels of 16 bits: not even
+  // one of them is a number of 16-byte slices) accesses are narrower, down to single elements: 40000 x 4104 in 8 groups of 4 segments, bf16, gelu, 0.64 and 1.05 ms
+  // where a block that walks over a segment's group took 29 and 25.
+  int per, groups, chunk;
+  int64_t slices;
+  bool fits;
+  for (p.slice = slice_of(s.dim, size, addresses);; p.slice /= 2) {
+    t.fold = 1;
+    if (s.per > kMostColumns && (s.offsets || s.per_segment > 1)) {
+      t.fold = (int)ceil_div(s.per, kMostColumns);
+      while (s.per / t.fold >= 64 && s.per % (t.fold * p.slice)) ++t.fold;
+    }
+    per = s.per / t.fold, groups = s.groups * t.fold, chunk = groups;
+    if (s.dim > kMostColumns || groups > kMostColumns / 4) {
+      chunk = std::min<int>(kMostColumns / per, kMostColumns / 4);
+      while (chunk > 0 && (int64_t)chunk * per % p.slice) --chunk;
+    }
+    slices = chunk > 0 ? ceil_div((int64_t)std::min(chunk, groups) * per, p.slice) : 0;
+    fits = chunk > 0 && per * t.fold == s.per && slices <= 256 * (8 / p.slice) && s.segments > 0;
+    if (fits || p.slice == 1) break;
   }
-  const int per = s.per / t.fold, groups = s.groups * t.fold;
-  // a block has whole groups (or parts), a chunk of them that begins on an access
-  int chunk = groups;
-  if (s.dim > kMostColumns || groups > kMostColumns / 4) {
-    chunk = std::min<int>(kMostColumns / per, kMostColumns / 4);
-    while (chunk > 0 && (int64_t)chunk * per % p.slice) --chunk;
-  }
-  const int64_t slices = chunk > 0 ? ceil_div((int64_t)std::min(chunk, groups) * per, p.slice) : 0;
-  if (chunk <= 0 || per * t.fold != s.per || slices > 256 * (8 / p.slice) || s.segments == 0) {
+  if (!fits) {
     p.kind = kNormWide;
     p.blocks = std::max<int64_t>(1, std::min<int64_t>(ceil_div(s.rows, 32), kNumSMs * 8 / ceil_div(s.dim, 256)));
     return p;

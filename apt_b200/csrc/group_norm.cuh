@@ -984,8 +984,8 @@ k_norm_apply(const __grid_constant__ NormShape s, const __grid_constant__ NormCa
 }
 
 // --------------------------------------------------------------------------------------- groups of very many channels
-// Rows by themselves of more than 1024 slices, and groups of segments of more than 2048 channels that cannot be cut into parts of whole
-// slices. 4096 x 8192 fp32: forwards 87 us (HBM: 41), backwards 201 (62) and the columns 313: three walks and two, the later ones out of L2.
+// Rows by themselves of more than 1024 slices, and groups of segments of more than 2048 channels that cannot be cut into equal parts.
+// 4096 x 8192 fp32: forwards 87 us (HBM: 41), backwards 201 (62) and the columns 313: three walks and two, the later ones out of L2.
 __device__ __forceinline__ float block_sum(float v, float* shared) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

@@ -260,3 +260,35 @@ def test_a_gradient_without_a_slope_over_a_long_segment():
     _, stats = apt_b200.group_norm_act(x, 1, offsets=ends, return_stats=True)
     grad = apt_b200.group_norm_act_backward(x, torch.full_like(x, 0.9), stats, 1, offsets=ends)[0]
     assert float(grad.abs().max()) <= 0.9 * (2.0 ** -22 + 7 * 2e-5)
+
+
+def _time(call):
+    """The shorter of two calls behind a first one, in milliseconds."""
+    call()
+    times = []
+    for _ in range(2):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+# groups of which not one is a whole number of 16-byte slices, in rows that are, of more than a block's columns
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,groups", [(4104, 8), (4112, 16), (4120, 2), (2056, 8), (2570, 10)])
+def test_segments_of_groups_of_odd_widths(dim, groups, dtype):
+    sizes = [12000, 1, 0, 8000]
+    ends, rows = _ends(*sizes), sum(sizes)
+    x = (torch.randn((rows, dim), device="cuda", generator=_gen(17)) * 0.3 + 301.0).to(dtype)
+    call = lambda t, o: apt_b200.group_norm_act(t, groups, offsets=o, act="silu", return_stats=True)
+    _, stats = call(x, ends)
+    mean, rstd = _statistics(x, groups, [0, 12000, 12001, 20001])
+    some = [0, 1, 3]
+    assert ((stats[some, :, 0].double() - mean).abs() <= 16 * 2.0 ** -24 * 302).all()
+    assert ((stats[some, :, 1].double() / rstd - 1).abs() <= 2e-5).all() and not stats[2].any()
+    # single elements take six times as long as whole slices, one block for a long segment's group thirty times and more
+    even = torch.randn((rows, 2048), device="cuda", generator=_gen(18)).to(dtype)
+    assert _time(lambda: call(x, ends)) < 12 * (dim / 2048) * _time(lambda: apt_b200.group_norm_act(even, 8, offsets=ends, act="silu"))

@@ -49,6 +49,7 @@ static NormPlan norm_plan(const NormShape& s, size_t size, uintptr_t addresses, 
       p.lanes.rows = 256 / (w * p.lanes.groups);
       p.chunks = ceil_div(s.groups, p.lanes.groups);
       p.blocks = std::max<int64_t>(1, std::min<int64_t>(ceil_div(s.rows, p.lanes.rows * (back ? 2 : 4)), ceil_div(kNumSMs * (back ? 4 : 8), p.chunks)));
+      p.lanes.blocks = (int)p.blocks;
       return p;
     }
   }

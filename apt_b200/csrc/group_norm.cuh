@@ -180,6 +180,7 @@ __device__ __forceinline__ void begin_backward(const NormCall& c, int64_t e, con
 struct NormLanes {
   int width;              // lanes of a row's group: a power of two up to 256; BLOCK: above 32
   int groups, rows;       // a block has side by side
+  int blocks;             // for the rows of each such chunk of groups (all in one dimension of the grid: of chunks there may be over 65535)
 };
 
 // A sum over the lanes of each group, of U rows at once. `shared`: not that of the sum before, whose readers this one's barrier waits for.
@@ -220,7 +221,8 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
   __shared__ float shared[3][16 * U];
   __shared__ float sums[BACK ? 256 * VE : 1];
   const int width = l.width;
-  const int lane = threadIdx.x % width, slot = threadIdx.x / width % l.groups, line = threadIdx.x / (width * l.groups), g = blockIdx.y * l.groups + slot;
+  const int lane = threadIdx.x % width, slot = threadIdx.x / width % l.groups, line = threadIdx.x / (width * l.groups);
+  const int block = blockIdx.x % l.blocks, g = blockIdx.x / l.blocks * l.groups + slot;
   const bool mine = line < l.rows && g < s.groups;
   const T* const x = (const T*)c.x;
   const T* const grad = (const T*)c.grad;
@@ -260,8 +262,8 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
       }
     }
   };
-  if constexpr (kAhead) load(blockIdx.x * step, next_x, next_g);
-  for (int64_t base = blockIdx.x * step; base < s.rows; base += gridDim.x * step) {
+  if constexpr (kAhead) load(block * step, next_x, next_g);
+  for (int64_t base = block * step; base < s.rows; base += l.blocks * step) {
     if constexpr (kAhead) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -271,7 +273,7 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
           if constexpr (BACK) rg[u][j] = next_g[u][j];
         }
       }
-      load(base + gridDim.x * step, next_x, next_g);
+      load(base + l.blocks * step, next_x, next_g);
     } else {
       load(base, rx, rg);
     }
@@ -374,7 +376,7 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
           for (int k = 0; k < VE; ++k) {
             float v = 0.0f;
             for (int r = 0; r < l.rows; ++r) v += sums[(threadIdx.x + r * width * l.groups) * VE + k];
-            c.columns[((int64_t)blockIdx.x * 2 + which) * s.dim + at[j] + k] = v;
+            c.columns[((int64_t)block * 2 + which) * s.dim + at[j] + k] = v;
           }
         }
       }
@@ -1105,7 +1107,7 @@ struct NormPlan {
 
 template <typename T, int VE, bool BACK>
 static int norm_rows(const NormShape& s, const NormCall& c, const NormPlan& p, cudaStream_t st) {
-  const dim3 grid((unsigned)p.blocks, (unsigned)p.chunks);
+  const int64_t grid = p.blocks * p.chunks;
   if (p.lanes.width > 32) {
     if (p.held == 1) APT_FOLLOW((k_norm_rows<T, VE, 1, BACK ? 1 : 2, true, BACK>), grid, 256, 0, st, s, c, p.lanes);
     else if (p.held == 2) APT_FOLLOW((k_norm_rows<T, VE, 2, 1, true, BACK>), grid, 256, 0, st, s, c, p.lanes);
@@ -1126,7 +1128,7 @@ static int norm_tiles(const NormShape& s, const NormCall& c, const NormPlan& p, 
   parts.groups *= t.fold, parts.per /= t.fold;
   APT_FOLLOW((k_norm_sums<T, VE, NC, GN, BACK, WARP>), sums, 256, 0, st, parts, c, t);
   const int joins = BACK && c.columns ? (int)ceil_div(2 * s.dim, 32) : 0;
-  const dim3 join((unsigned)(joins + ceil_div(s.segments, t.join_segments)), t.join_segments > 1 ? 1u : (unsigned)ceil_div(s.groups, t.join_groups));
+  const dim3 join((unsigned)(joins + ceil_div(s.segments, t.join_segments)), t.join_segments > 1 ? 1u : (unsigned)std::min<int64_t>(65535, ceil_div(s.groups, t.join_groups)));
   APT_FOLLOW((k_norm_join<T, BACK>), join, 256, 0, st, parts, c, t, joins, p.blocks);
   APT_FOLLOW((k_norm_apply<T, VE, NC, GN, BACK, WARP>), apply, 256, 0, st, parts, c, t);
   return APT_OK;

@@ -292,3 +292,24 @@ def test_segments_of_groups_of_odd_widths(dim, groups, dtype):
     # single elements take six times as long as whole slices, one block for a long segment's group thirty times and more
     even = torch.randn((rows, 2048), device="cuda", generator=_gen(18)).to(dtype)
     assert _time(lambda: call(x, ends)) < 12 * (dim / 2048) * _time(lambda: apt_b200.group_norm_act(even, 8, offsets=ends, act="silu"))
+
+
+# more than 65535 times what a block has of them: of rows by themselves 8 groups, and 256 where a group is one channel; of segments 64 in the join
+@pytest.mark.parametrize("dim,groups,sizes", [(17 * 600_000, 600_000, None), (16_777_215, 16_777_215, None), (5_000_000, 5_000_000, [2])])
+def test_very_many_groups(dim, groups, sizes):
+    x = torch.randn((2, dim), device="cuda", generator=_gen(19))
+    ends = None if sizes is None else _ends(*sizes)
+    out, stats = apt_b200.group_norm_act(x, groups, offsets=ends, return_stats=True)
+    grad, _, _ = apt_b200.group_norm_act_backward(x, x, stats, groups, offsets=ends)
+    ops.check_status()
+    for part in (slice(0, 17 * 64), slice(dim - 17 * 64 if dim % 17 == 0 else dim - 64, dim)):
+        v = x[:, part].double()
+        v = v.view(2, -1, dim // groups) if sizes is None else v.t().reshape(1, -1, 2)
+        mean, var = v.mean(2, keepdim=True), v.var(2, unbiased=False, keepdim=True)
+        rstd = 1 / torch.sqrt(var + 1e-5)
+        xh = (v - mean) * rstd
+        dx = rstd * (v - mean - xh * (v * xh).mean(2, keepdim=True))
+        back = lambda t: t.reshape(2, -1) if sizes is None else t.view(-1, 2).t()
+        # ten roundings of numbers of at most |x| rstd, which the gradient multiplies by rstd: 316 each at most
+        assert ((out[:, part].double() - back(xh)).abs() <= 2e-6 * back(v.abs() * rstd + rstd * mean.abs()) + 1e-7).all()
+        assert ((grad[:, part].double() - back(dx)).abs() <= 2e-5 * back(rstd * (v.abs() + mean.abs()) * (1 + xh * xh)) + 1e-7).all()

@@ -72,37 +72,37 @@ __device__ __forceinline__ void put_param(void* p, int wide, int64_t c, float v)
   if (wide) ((float*)p)[c] = v; else ((T*)p)[c] = Elem<T>::from_f(v);
 }
 
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ void act_all(int act, float (&z)[N]) {
   switch (act) {
     case APT_ACT_RELU:
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = act_of<APT_ACT_RELU>(z[k]);
+      for (int k = 0; k < N; ++k) z[k] = act_of<T, APT_ACT_RELU>(z[k]);
       break;
     case APT_ACT_SILU:
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = act_of<APT_ACT_SILU>(z[k]);
+      for (int k = 0; k < N; ++k) z[k] = act_of<T, APT_ACT_SILU>(z[k]);
       break;
     case APT_ACT_GELU:
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = act_of<APT_ACT_GELU>(z[k]);
+      for (int k = 0; k < N; ++k) z[k] = act_of<T, APT_ACT_GELU>(z[k]);
       break;
   }
 }
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ void slope_all(int act, float (&z)[N]) {
   switch (act) {
     case APT_ACT_RELU:
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = act_slope<APT_ACT_RELU>(z[k]);
+      for (int k = 0; k < N; ++k) z[k] = act_slope<T, APT_ACT_RELU>(z[k]);
       break;
     case APT_ACT_SILU:
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = act_slope<APT_ACT_SILU>(z[k]);
+      for (int k = 0; k < N; ++k) z[k] = act_slope<T, APT_ACT_SILU>(z[k]);
       break;
     case APT_ACT_GELU:
 #pragma unroll
-      for (int k = 0; k < N; ++k) z[k] = act_slope<APT_ACT_GELU>(z[k]);
+      for (int k = 0; k < N; ++k) z[k] = act_slope<T, APT_ACT_GELU>(z[k]);
       break;
     default:
 #pragma unroll
@@ -146,22 +146,22 @@ __device__ __forceinline__ void drop_by(const Drop& d, uint32_t bits, float (&v)
 }
 
 // y of normalised elements, in place.
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ void finish_forward(const NormCall& c, int64_t e, float (&v)[N], const float (&gamma)[N], const float (&beta)[N]) {
 #pragma unroll
   for (int k = 0; k < N; ++k) v[k] = fmaf(v[k], gamma[k], beta[k]);
-  act_all(c.act, v);
+  act_all<T>(c.act, v);
   if (c.drop) drop_all(c.d, e, v);
 }
 // dz of normalised elements and gradients, into the gradients. Where a call meets its elements twice, the first time leaves what stays in
 // c.mask, a byte a slice of whole quads, and the second takes it from there: making it anew is half of such a pass.
 enum MaskUse { kMaskMade, kMaskLeft, kMaskTaken };
-template <int USE, int N>
+template <typename T, int USE, int N>
 __device__ __forceinline__ void begin_backward(const NormCall& c, int64_t e, const float (&xh)[N], float (&grad)[N], const float (&gamma)[N], const float (&beta)[N]) {
   float z[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) z[k] = fmaf(xh[k], gamma[k], beta[k]);
-  slope_all(c.act, z);
+  slope_all<T>(c.act, z);
   if (c.drop) {
     if constexpr (USE == kMaskMade || N % 4) {
       drop_all(c.d, e, grad);
@@ -317,7 +317,7 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
 #pragma unroll
           for (int k = 0; k < VE; ++k) v[k] = (rx[u][j].get(k) - mean[u]) * rstd[u];
           const int64_t e = row[u] * s.dim + at[j];
-          finish_forward(c, e, v, gamma[j], beta[j]);
+          finish_forward<T>(c, e, v, gamma[j], beta[j]);
           store_all<T, VE>(out + e, v);
         }
       }
@@ -331,7 +331,7 @@ k_norm_rows(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
           float xh[VE];
 #pragma unroll
           for (int k = 0; k < VE; ++k) xh[k] = (rx[u][j].get(k) - mean[u]) * rstd[u], dz[u][j][k] = rg[u][j].get(k);
-          begin_backward<kMaskMade>(c, row[u] * s.dim + at[j], xh, dz[u][j], gamma[j], beta[j]);
+          begin_backward<T, kMaskMade>(c, row[u] * s.dim + at[j], xh, dz[u][j], gamma[j], beta[j]);
           if (!in[j] || row[u] >= s.rows) continue;
 #pragma unroll
           for (int k = 0; k < VE; ++k) {
@@ -760,7 +760,7 @@ k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCal
 #pragma unroll
             for (int i = 0; i < VE; ++i) xh[i] = rx[u][j].get(i), dz[i] = rg[u][j].get(i);
             normalise(xh, st[j]);
-            begin_backward<kMaskLeft>(c, at + u * step + me.col[j], xh, dz, gamma[j], beta[j]);
+            begin_backward<T, kMaskLeft>(c, at + u * step + me.col[j], xh, dz, gamma[j], beta[j]);
 #pragma unroll
             for (int i = 0; i < VE; ++i) ab[0][j][i] += dz[i], ab[1][j][i] = fmaf(dz[i], xh[i], ab[1][j][i]);
           }
@@ -964,14 +964,14 @@ k_norm_apply(const __grid_constant__ NormShape s, const __grid_constant__ NormCa
             float dz[VE];
 #pragma unroll
             for (int i = 0; i < VE; ++i) dz[i] = rg[u][j].get(i);
-            begin_backward<kMaskTaken>(c, at, v, dz, gamma[j], beta[j]);
+            begin_backward<T, kMaskTaken>(c, at, v, dz, gamma[j], beta[j]);
 #pragma unroll
             for (int i = 0; i < VE; ++i) dz[i] = __fmul_rn(dz[i], gamma[j][i]);
             finish_backward(v, dz, st[j], ab[j]);
           } else {
 #pragma unroll
             for (int i = 0; i < VE; ++i) v[i] = rx[u][j].get(i) - st[j][i % GN].x;
-            finish_forward(c, at, v, scale[j], beta[j]);
+            finish_forward<T>(c, at, v, scale[j], beta[j]);
           }
           store_all<T, VE>(out + at, v);
         }
@@ -1014,7 +1014,7 @@ __device__ __forceinline__ float2 wide_xh_dz(const NormCall& c, int64_t e, int64
   const float g = *gamma = param<T>(c.weight, c.wide_params, col, 1.0f);
   float xh[1] = {(Elem<T>::to_f(((const T*)c.x)[e]) - st.x) * st.y}, dz[1] = {Elem<T>::to_f(((const T*)c.grad)[e])};
   const float gs[1] = {g}, bs[1] = {param<T>(c.bias, c.wide_params, col, 0.0f)};
-  begin_backward<kMaskMade>(c, e, xh, dz, gs, bs);
+  begin_backward<T, kMaskMade>(c, e, xh, dz, gs, bs);
   return make_float2(xh[0], dz[0]);
 }
 template <typename T, bool BACK>
@@ -1045,7 +1045,7 @@ __global__ void __launch_bounds__(256) k_norm_wide(const __grid_constant__ NormS
       walk([&](int64_t e, int64_t col) {
         float v[1] = {(Elem<T>::to_f(x[e]) - mean) * rstd};
         const float g[1] = {param<T>(c.weight, c.wide_params, col, 1.0f)}, b[1] = {param<T>(c.bias, c.wide_params, col, 0.0f)};
-        finish_forward(c, e, v, g, b);
+        finish_forward<T>(c, e, v, g, b);
         out[e] = Elem<T>::from_f(v[0]);
       });
     } else {

@@ -313,3 +313,23 @@ def test_very_many_groups(dim, groups, sizes):
         # ten roundings of numbers of at most |x| rstd, which the gradient multiplies by rstd: 316 each at most
         assert ((out[:, part].double() - back(xh)).abs() <= 2e-6 * back(v.abs() * rstd + rstd * mean.abs()) + 1e-7).all()
         assert ((grad[:, part].double() - back(dx)).abs() <= 2e-5 * back(rstd * (v.abs() + mean.abs()) * (1 + xh * xh)) + 1e-7).all()
+
+
+# Without a slope of its own (gamma 0) z is beta. q's exponent z^2 / 2 is a product of three numbers, rounded each: 1.5 z^2 units of 2^-24; the exponential, the
+# reciprocal, the polynomial (6; of 16 bits 20) and the products: 24 (38) units. Below -13 the exponential is smaller than a normal number, and f16 ends at
+# 2^-24, bf16's normal numbers at 2^-126.
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gelu_where_it_is_small(dtype):
+    z = torch.linspace(-13.0, 13.0, 4096, device="cuda")
+    x, gamma = torch.randn((1, 4096), device="cuda", generator=_gen(20)).to(dtype), torch.zeros(4096, device="cuda")
+    out, stats = apt_b200.group_norm_act(x, 1, gamma, z, act="gelu", return_stats=True)
+    slope = apt_b200.group_norm_act_backward(x, torch.ones_like(x), stats, 1, gamma, z, act="gelu")[2]
+    wide = z.double()
+    below = 0.5 * torch.erfc(-wide / 2 ** 0.5)
+    density = torch.exp(-wide * wide / 2) / (2 * np.pi) ** 0.5
+    share = (1.5 * wide * wide + (24 if dtype == torch.float32 else 38)) * 2.0 ** -24
+    least = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25}[dtype]
+    assert ((out[0].double() - wide * below).abs() <= (share + UNIT[dtype] * (1 + share)) * (wide * below).abs() + least).all()
+    assert ((slope.double() - (below + wide * density)).abs() <= share * (below + wide.abs() * density)).all()
+    low, high = (apt_b200.group_norm_act(x, 1, gamma, torch.full_like(z, end), act="gelu") for end in (-40.0, 40.0))
+    assert not low.any() and (high == 40.0).all()

@@ -188,6 +188,31 @@ def test_weight_gradients_of_very_many_tiles():
             assert ((gw[g, some].double() - want).abs() <= 80 * 2.0 ** -23 * size).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,out_dim", [([1, 0, 300, 5000, 31], 70), ([0], 1), ([33] * 200, 32), ([20000], 257)])
+def test_the_gradient_of_the_bias_alone(sizes, out_dim, dtype):
+    """Sums of a column: 256 rows' side by side, 8 of them and then 32 partial ones added up, in all 20000 / 256 + 40 roundings of either sign."""
+    rows, offsets = sum(sizes) + 9, _ends(*sizes)
+    grad = torch.randn((rows, out_dim), device="cuda", generator=_gen(5)).to(dtype)
+    grad[sum(sizes):] = float("nan")      # of no group
+    x, weight = torch.randn((rows, 8), device="cuda").to(dtype), torch.randn((len(sizes), out_dim, 8), device="cuda").to(dtype)
+    gx, gw, gb = apt_b200.grouped_linear_backward(x, weight, offsets, grad, want_x=False, want_weight=False)
+    assert gx is None and gw is None
+    ends = offsets.tolist()
+    for g, (b, e) in enumerate(zip(ends, ends[1:])):
+        want, size = grad[b:e].double().sum(0), grad[b:e].double().abs().sum(0)
+        assert ((gb[g].double() - want).abs() <= 32 * 2.0 ** -24 * size + UNIT[dtype] * want.abs()).all()
+    bias = torch.zeros((len(sizes), out_dim), device="cuda", dtype=dtype, requires_grad=True)
+    out = apt_b200.GroupedLinear.apply(x, weight, offsets, bias)
+    assert torch.equal(torch.autograd.grad(out, bias, grad)[0], gb)
+    # with the weight's, whose kernel makes it beside: another order
+    _, _, beside = apt_b200.grouped_linear_backward(x, weight, offsets, grad, want_x=False)
+    for g, (b, e) in enumerate(zip(ends, ends[1:])):
+        size = grad[b:e].double().abs().sum(0)
+        assert ((gb[g].double() - beside[g].double()).abs() <= 64 * 2.0 ** -24 * size + 2 * UNIT[dtype] * gb[g].double().abs()).all()
+    ops.check_status()
+
+
 # ------------------------------------------------------------------------------------------------------ group norm
 def test_statistics_of_segments_without_rows_are_zeros():
     for rows in (0, 7):

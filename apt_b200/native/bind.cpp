@@ -316,6 +316,27 @@ void same_device(const char* who, const Tensor& a, const Tensor& b, const char* 
   if (b.defined() && b.device() != a.device()) fail(std::string(who) + ": " + name + " is on another device than the rows");
 }
 
+// A gradient that is not differentiable itself. With create_graph it would be a constant, and a second derivative silently too small; one that is
+// asked for, along any of the tensors that the gradient is made of, raises.
+struct OnceFunction : public torch::autograd::Function<OnceFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& gradient, const Tensor&, const OptTensor&, const OptTensor&, const Tensor&,
+                        const std::string& who) {
+    ctx->saved_data["who"] = who;
+    return gradient.detach();
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list) {
+    fail(ctx->saved_data["who"].toStringRef() + " has no second derivatives");
+  }
+};
+torch::autograd::variable_list only_once(const std::string& who, torch::autograd::variable_list gradients, const Tensor& x, const Tensor& weight, const Tensor& bias,
+                                         const Tensor& grad) {
+  if (at::GradMode::is_enabled())
+    for (Tensor& t : gradients)
+      if (t.defined())
+        t = OnceFunction::apply(t, x, weight.defined() ? OptTensor(weight) : OptTensor(), bias.defined() ? OptTensor(bias) : OptTensor(), grad, who);
+  return gradients;
+}
+
 Tensor dropout(const Tensor& x_in, double p, int64_t key, int64_t call) {
   const Tensor x = cuda(x_in, "x");
   const int code = float_code("dropout", x);
@@ -332,8 +353,10 @@ struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
     return dropout(x, p, key, call);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-    return {dropout(grads[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["key"].toInt(), ctx->saved_data["call"].toInt()), Tensor(), Tensor(),
-            Tensor()};
+    const double p = ctx->saved_data["p"].toDouble();
+    const int64_t key = ctx->saved_data["key"].toInt(), call = ctx->saved_data["call"].toInt();
+    // the same map, whose gradient is the same again
+    return {at::GradMode::is_enabled() ? apply(grads[0], p, key, call) : dropout(grads[0], p, key, call), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -442,7 +465,7 @@ struct NormFunction : public torch::autograd::Function<NormFunction> {
                                       wants_grad(v[1]), wants_grad(v[2]), ctx->saved_data["words"].toTensor());
     torch::autograd::variable_list r(11);
     r[0] = gx, r[1] = gw, r[2] = gb;
-    return r;
+    return only_once("group_norm_act", std::move(r), v[0], v[1], v[2], grads[0]);
   }
 };
 
@@ -519,7 +542,7 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
     const auto v = ctx->get_saved_variables();
     const auto wants = ctx->saved_data["wants"].toIntVector();
     auto [gx, gw, gb] = linear_backward(v[0], v[1], v[2], grads[0], wants[0], wants[1], wants[2], ctx->saved_data["words"].toTensor());
-    return {gx, gw, Tensor(), gb, Tensor()};
+    return only_once("grouped_linear", {gx, gw, Tensor(), gb, Tensor()}, v[0], v[1], Tensor(), grads[0]);
   }
 };
 

@@ -1077,7 +1077,8 @@ def grouped_linear_backward(x, weight, offsets, grad_out, want_x: bool = True, w
 
 
 class GroupedLinear:
-    """grouped_linear with its backward: ``out = GroupedLinear.apply(x, weight, offsets, bias)`` (an autograd function on the C++ side)."""
+    """grouped_linear with its backward: ``out = GroupedLinear.apply(x, weight, offsets, bias)`` (an autograd function on the C++ side;
+    second derivatives raise)."""
 
     @staticmethod
     def apply(x, weight, offsets, bias=None):
@@ -1107,7 +1108,7 @@ def group_norm_act_backward(x, grad_out, stats, num_groups: int, weight=None, bi
 
 class GroupNormAct:
     """group_norm_act with its backward: ``y = GroupNormAct.apply(x, num_groups, weight, bias, offsets, eps, act, p, key, call_id)``
-    (an autograd function on the C++ side; the mask of the dropout is made anew in the backward)."""
+    (an autograd function on the C++ side; the mask of the dropout is made anew in the backward; second derivatives raise)."""
 
     @staticmethod
     def apply(x, num_groups, weight=None, bias=None, offsets=None, eps=1e-5, act="none", p=0.0, key=0, call_id=0):

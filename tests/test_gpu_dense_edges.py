@@ -358,3 +358,21 @@ def test_gelu_where_it_is_small(dtype):
     assert ((slope.double() - (below + wide * density)).abs() <= share * (below + wide.abs() * density)).all()
     low, high = (apt_b200.group_norm_act(x, 1, gamma, torch.full_like(z, end), act="gelu") for end in (-40.0, 40.0))
     assert not low.any() and (high == 40.0).all()
+
+
+# ------------------------------------------------------------------------------------------------------ derivatives
+def test_second_derivatives_are_right_or_refused():
+    x = torch.randn((6, 8), device="cuda", generator=_gen(21), requires_grad=True)
+    weight = torch.randn((2, 4, 8), device="cuda", generator=_gen(22), requires_grad=True)
+    y = apt_b200.Dropout.apply(x, 0.5, 1)
+    g = torch.autograd.grad((y ** 3).sum(), x, create_graph=True)[0]
+    keep = 2.0 * (apt_b200.dropout(torch.ones_like(x), 0.5, 1) > 0)
+    assert torch.equal(g, 3 * (x * keep) ** 2 * keep)
+    assert torch.allclose(torch.autograd.grad(g.sum(), x)[0], 6 * x * keep ** 3, rtol=1e-6)
+    for name, y in (("grouped_linear", apt_b200.GroupedLinear.apply(x, weight, _ends(2, 4))),
+                    ("group_norm_act", apt_b200.GroupNormAct.apply(x, 2, None, None, None, 1e-5, "silu"))):
+        plain = torch.autograd.grad((y * y).sum(), x, retain_graph=True)[0]
+        g = torch.autograd.grad((y * y).sum(), x, create_graph=True)[0]
+        assert torch.equal(g, plain) and not plain.requires_grad
+        with pytest.raises(RuntimeError, match=f"{name} has no second derivatives"):
+            torch.autograd.grad((g * g).sum() + (x * x).sum(), x)

@@ -384,7 +384,7 @@ NormProblem norm_problem(const Tensor& x_in, const Tensor& weight, const Tensor&
     fail("group_norm_act: " + std::to_string(q.dim) + " channels are no whole number of " + std::to_string(s.groups) + " groups");
   probability("group_norm_act", s.p);
   if (!(s.eps >= 0.0)) fail("group_norm_act: eps must not be negative");
-  q.segments = q.rows ? q.x.size(0) : 0;
+  q.segments = q.x.size(0);
   if (offsets.defined()) {
     if (q.x.dim() != 2) fail("group_norm_act: offsets go with rows in two dimensions, got " + std::to_string(q.x.dim()));
     q.offsets = ids(offsets, "offsets");

@@ -224,6 +224,17 @@ def test_statistics_of_segments_without_rows_are_zeros():
     ops.check_status()
 
 
+def test_blocks_without_rows_are_segments():
+    x = torch.zeros((5, 0, 12), device="cuda")
+    weight = torch.ones(12, device="cuda")
+    y, stats = apt_b200.group_norm_act(x, 3, weight, return_stats=True)
+    assert y.shape == x.shape and stats.shape == (5, 3, 2) and not stats.any()
+    gx, gw, _ = apt_b200.group_norm_act_backward(x, x, stats, 3, weight)
+    assert gx.shape == x.shape and not gw.any()
+    for empty in (torch.zeros((0, 4, 12), device="cuda"), torch.zeros((0, 12), device="cuda")):
+        assert apt_b200.group_norm_act(empty, 3, return_stats=True)[1].shape == (0, 3, 2)
+
+
 # tiles of segments, many segments (joined eight a block), groups that a block walks over
 @pytest.mark.parametrize("dim,segments", [(64, 2), (64, 1500), (4106, 2)])
 def test_the_backward_looks_at_the_ends_too(dim, segments):

@@ -203,16 +203,21 @@ struct Pieces {
   uint4 p[3];
 };
 __device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
+// The same, cut off by the conversion, which leaves a NaN one that has its bits in its lower half.
+__device__ __forceinline__ uint32_t upper_numbers(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 __device__ __forceinline__ float below(float v) { return v - __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 __device__ __forceinline__ Pieces take_apart(float4 a, float4 b) {
   Pieces r;
-  // a sum has a NaN's upper bits set, which an operand may have in its lower ones alone
-  a = make_float4(a.x + 0.0f, a.y + 0.0f, a.z + 0.0f, a.w + 0.0f), b = make_float4(b.x + 0.0f, b.y + 0.0f, b.z + 0.0f, b.w + 0.0f);
+  r.p[0] = make_uint4(upper_numbers(a.x, a.y), upper_numbers(a.z, a.w), upper_numbers(b.x, b.y), upper_numbers(b.z, b.w));
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    r.p[k] = make_uint4(upper_halves(a.x, a.y), upper_halves(a.z, a.w), upper_halves(b.x, b.y), upper_halves(b.z, b.w));
+  for (int k = 1; k < 3; ++k) {
     a = make_float4(below(a.x), below(a.y), below(a.z), below(a.w));
     b = make_float4(below(b.x), below(b.y), below(b.z), below(b.w));
+    r.p[k] = make_uint4(upper_halves(a.x, a.y), upper_halves(a.z, a.w), upper_halves(b.x, b.y), upper_halves(b.z, b.w));
   }
   return r;
 }

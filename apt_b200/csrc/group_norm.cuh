@@ -999,10 +999,16 @@ __device__ __forceinline__ float block_sum(float v, float* shared) {
   return v;
 }
 // A sum of however many numbers: what each addition loses is kept beside it (Knuth's two-sum). One thread may have a 256th of all of a long segment's, whose
-// running mean stands still, and whose squares, of few different values in 16 bits, are rounded the same way every time (1e-4 of 20000 x 2053).
+// running mean stands still, and whose squares, of few different values in 16 bits, are rounded the same way every time (1e-4 of 20000 x 2053). A sum of
+// 32 (LONG false) loses nothing to speak of.
+template <bool LONG>
 struct LongSum {
   float sum = 0.0f, lost = 0.0f;
   __device__ __forceinline__ void add(float v) {
+    if (!LONG) {
+      sum += v;
+      return;
+    }
     const float all = sum + v, added = all - sum;
     lost += (sum - (all - added)) + (v - added);
     sum = all;
@@ -1017,7 +1023,7 @@ __device__ __forceinline__ float2 wide_xh_dz(const NormCall& c, int64_t e, int64
   begin_backward<T, kMaskMade>(c, e, xh, dz, gs, bs);
   return make_float2(xh[0], dz[0]);
 }
-template <typename T, bool BACK>
+template <typename T, bool BACK, bool LONG>
 __global__ void __launch_bounds__(256) k_norm_wide(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c) {
   wait_for_previous();
   __shared__ float shared[8];
@@ -1033,7 +1039,7 @@ __global__ void __launch_bounds__(256) k_norm_wide(const __grid_constant__ NormS
         for (int k = threadIdx.x; k < s.per; k += 256) f(row * s.dim + c0 + k, c0 + k);
     };
     if constexpr (!BACK) {
-      LongSum all, squares;
+      LongSum<LONG> all, squares;
       walk([&](int64_t e, int64_t) { all.add(Elem<T>::to_f(x[e])); });
       const float mean = block_sum(all.get(), shared) * inv;
       walk([&](int64_t e, int64_t) {
@@ -1050,7 +1056,7 @@ __global__ void __launch_bounds__(256) k_norm_wide(const __grid_constant__ NormS
       });
     } else {
       const float2 st = c.stats[item];
-      LongSum dxhs, dxh_xhs;
+      LongSum<LONG> dxhs, dxh_xhs;
       float gamma;
       walk([&](int64_t e, int64_t col) {
         const float2 v = wide_xh_dz<T>(c, e, col, st, &gamma);
@@ -1149,7 +1155,10 @@ static int norm_slices(const NormShape& s, const NormCall& c, const NormPlan& p,
 template <typename T, bool BACK>
 int norm(const NormShape& s, const NormCall& c, const NormPlan& p, cudaStream_t st) {
   if (p.kind == kNormWide) {
-    if (s.rows) APT_FOLLOW((k_norm_wide<T, BACK>), wave_grid(s.segments * s.groups, 8), 256, 0, st, s, c);
+    // a thread's share of a row of up to 8192 channels is a sum of 32: 4096 x 8192 fp32, forwards, gelu 86 us, 97 with what additions lose kept beside
+    const int64_t grid = wave_grid(s.segments * s.groups, 8);
+    if (s.rows && !s.offsets && s.per_segment == 1 && s.per <= 32 * 256) APT_FOLLOW((k_norm_wide<T, BACK, false>), grid, 256, 0, st, s, c);
+    else if (s.rows) APT_FOLLOW((k_norm_wide<T, BACK, true>), grid, 256, 0, st, s, c);
     if (BACK && c.columns) {
       APT_FOLLOW((k_norm_wide_columns<T>), dim3((unsigned)ceil_div(s.dim, 256), (unsigned)p.blocks), 256, 0, st, s, c);
       APT_FOLLOW((k_norm_columns<T>), ceil_div(2 * s.dim, 32), 256, 0, st, s, c, p.blocks);

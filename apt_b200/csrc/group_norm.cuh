@@ -211,8 +211,8 @@ __device__ __forceinline__ void sum_lanes(float (&v)[U], int width, float* share
   }
 }
 
-// NV slices of VE elements a lane, U rows on their way. 67584 x 256 fp32 in 8 groups, silu and dropout: forwards 43 us (HBM: 21), backwards 61 (32),
-// the instructions of the generator and of silu. 65536 x 1024 bf16, gelu: 83 (41) and 152 (62), where a row's sums follow one another (three
+// NV slices of VE elements a lane, U rows on their way. 67584 x 256 fp32 in 8 groups, silu and dropout: forwards 42 us (HBM: 21), backwards 65 (32),
+// of which no pipe is full: issue slots 60 per cent, integer 52 and 45, DRAM 25 and 33. 65536 x 1024 bf16, gelu: 85 (41) and 161 (62), where a row's sums follow one another (three
 // barriers backwards) and registers leave room for few rows at a time.
 template <typename T, int VE, int NV, int U, bool BLOCK, bool BACK>
 __global__ void __launch_bounds__(256)
@@ -650,7 +650,7 @@ __device__ __forceinline__ void put_columns(const NormShape& s, const NormCall& 
 
 // Sums of each tile's rows, piece by piece (the rows a tile has of a segment): piece number tile + segment, which no other has. Forwards the mean
 // and the squares around it, backwards the sums of dxh and dxh xh.
-// 151552 x 256 bf16 in 8 segments, us: forwards 23 (HBM: 12), backwards 84 (24), where silu and the dropout's generator bind.
+// 151552 x 256 bf16 in 8 segments, us: forwards 23 (HBM: 12), backwards 84 (24) with silu and the dropout's generator.
 template <typename T, int VE, int NC, int GN, bool BACK, bool WARP>
 __global__ void __launch_bounds__(256, BACK ? 2 : 3)
 k_norm_sums(const __grid_constant__ NormShape s, const __grid_constant__ NormCall c, const __grid_constant__ NormTiles t) {
@@ -987,7 +987,8 @@ k_norm_apply(const __grid_constant__ NormShape s, const __grid_constant__ NormCa
 
 // --------------------------------------------------------------------------------------- groups of very many channels
 // Rows by themselves of more than 1024 slices, and groups of segments of more than 2048 channels that cannot be cut into equal parts.
-// 4096 x 8192 fp32: forwards 87 us (HBM: 41), backwards 201 (62) and the columns 313: three walks and two, the later ones out of L2.
+// 4096 x 8192 fp32, gelu: forwards 86 us (HBM: 41), backwards 498 (62), of which the columns 300: three walks and two, the later ones out of L2. 20000 x 2053 bf16
+// in two segments 55 and 96 ms: two blocks.
 __device__ __forceinline__ float block_sum(float v, float* shared) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

@@ -421,7 +421,7 @@ __device__ __forceinline__ void store_tile(uint32_t acc, bool empty, char* stagi
 // 151552 x 256 -> 256 bf16 in 16 groups, us: out 34, dx 35 (HBM: 24; products: 12), dw and db 45 (24; 12) and their join 11.5. Eight tiles a block,
 // of which the first waits for the list and the weights and the last is brought out beside nothing: a third of the tensor cores' cycles and 36 to 45 per
 // cent of the DRAM's are in use. 495616 x 1024 -> 256 f16 in 4 groups: 260 (194; 159), at 1.05 to 1.3 GHz under the power cap. 67584 x 128 -> 256 fp32 in
-// 8 groups: 45, 45, 52 and 13.5 (HBM: 16, 16, 16; products: 16 each): six products of pieces read 208 KB of shared memory a stage, which bounds it.
+// 8 groups: out 40, dx 42, dw and db with their join 53 (HBM: 16, 16, 16; products: 16 each): six products of pieces read 208 KB of shared memory a stage, which bounds it.
 // 61 rows in 64 groups, 1024 -> 1024 bf16: 25, the weights of the groups that have rows (13).
 template <typename T, int MODE>
 __global__ void __launch_bounds__(GroupedTraits<T, MODE>::kThreads, 1)

@@ -1091,7 +1091,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     """dropout(act(group_norm(x) * weight + bias)), channels last: mean and biased variance over num_groups runs of neighbouring
     channels and, for 2-D x [R, C], over each row by itself or with `offsets` over the rows of each ragged group; for x [B, ..., C]
     over everything between the first and the last dimension. act: "none", "relu", "silu" or "gelu" (by the error function). weight
-    and bias [C] of x's dtype or float32. p > 0 drops elements of the result as dropout(..., p, key, call_id) does.
+    and bias [C] of x's dtype or float32. p > 0 drops elements of the result as dropout(..., p, key, call_id) does (in every replay of a
+    captured graph the same ones).
     return_stats: also mean and 1 / sqrt(variance + eps), float32 [segments, num_groups, 2], which the backward takes."""
     out, stats = _native.norm_forward(x, weight, bias, offsets, int(num_groups), _activation(act), float(eps), float(p),
                                       *_stream_key(key, call_id), bool(return_stats), STATE.words())
@@ -1119,7 +1120,8 @@ class GroupNormAct:
 def dropout(x: torch.Tensor, p: float, key: int, call_id: int = 0) -> torch.Tensor:
     """x / (1 - p) where the element's random word is at least p 2^32, else 0. The words are the Philox4x32-10 stream (key, call_id):
     element i, counted row by row, has word i % 4 of counter (i / 4 low, i / 4 high, call_id, 0x64726f70). Nothing is stored: the
-    gradient is dropout(grad, p, key, call_id). Another layer or step takes another call_id."""
+    gradient is dropout(grad, p, key, call_id). Another layer or step takes another call_id. Both numbers are the host's: a captured
+    graph has those of its capture, and the same mask in every replay."""
     return _native.dropout(x, float(p), *_stream_key(key, call_id))
 
 

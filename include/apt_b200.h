@@ -810,15 +810,17 @@ int apt_p2p_alltoall_fused(apt_p2p* ctx, const void* src, const int64_t* src_ind
  * [offsets[g], offsets[g + 1]) of int64_t offsets[groups + 1] in device memory,
  * offsets[0] == 0. Rows from offsets[groups] on belong to no group: what is
  * computed for them is zero. Offsets that do not ascend or pass the number of
- * rows set APT_FLAG_BAD_OFFSETS; nothing outside the buffers is touched, and
- * the results are unspecified. Sums are in fp32 and rounded once. No
+ * rows set APT_FLAG_BAD_OFFSETS, in calls without rows too; nothing outside the
+ * buffers is touched, and the results are unspecified. Sums are in fp32 and rounded
+ * to the type once. No
  * counterpart in the reference, whose models leave this to PyTorch
  * (python/npc/model/sage_model.py). */
 
 /* out[i] = x[i] / (1 - p) where word i of the Philox4x32-10 stream (key, call_id)
  * is at least floor(p 2^32), else 0 (whatever x[i] is): counter (i / 4 low, i / 4
  * high, call_id, 0x64726f70), word i % 4. The gradient is the same map of the
- * gradient. in and out do not overlap. */
+ * gradient. in and out do not overlap. key and call_id are the host's, here and in
+ * the norm: a captured graph drops the same elements in every replay. */
 int apt_dropout(int dtype, const void* in, int64_t n, double p, uint64_t key, uint32_t call_id, void* out, void* stream);
 
 typedef enum apt_activation { APT_ACT_NONE = 0, APT_ACT_RELU = 1, APT_ACT_SILU = 2, APT_ACT_GELU = 3 } apt_activation;

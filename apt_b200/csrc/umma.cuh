@@ -19,16 +19,21 @@ __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void barrier_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ bool barrier_over(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(done)
+               : "r"(bar), "r"(parity)
+               : "memory");
+  return done;
+}
 // Until the barrier's phase of this parity is over, or for that many polls, each of which may suspend for a while itself. False: somebody
-// has given up (*gave_up); nothing may be used then but what ends the kernel.
+// has given up (*gave_up); nothing may be used then but what ends the kernel. The first poll stands by itself: with the count in front of it, products of
+// 65536 x 1024 -> 1024 fp32 take 820 us, not 807.
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int polls) {
-  for (int i = 0; i < polls; ++i) {
-    uint32_t done;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(done)
-                 : "r"(bar), "r"(parity)
-                 : "memory");
-    if (done) return true;
+  if (polls && barrier_over(bar, parity)) return true;
+  for (int i = 1; i < polls; ++i) {
+    if (barrier_over(bar, parity)) return true;
     if ((i & 63) == 63 && *gave_up) return false;
   }
   *gave_up = 1;

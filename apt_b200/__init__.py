@@ -24,5 +24,7 @@ from .ops import (  # noqa: F401
     gat_edge_softmax_sum, gat_edge_softmax_sum_backward, GATEdgeSoftmaxSum, shuffle_seeds, sp_feat_shuffle, sp_sample_and_shuffle, sp_sample_shuffle_src, spmm_copy_e_sum, spmm_copy_u_sum, spmm_u_mul_e_sum, src_to_vir,
     srcdst_to_vir, unique_sorted,
     Dropout, GroupNormAct, GroupedLinear, dropout, group_norm_act, group_norm_act_backward, grouped_linear, grouped_linear_backward,
+    ExpertRows, ExpertSum, RouteExperts, expert_rows, expert_rows_backward, expert_sum, expert_sum_backward, route_experts,
+    route_experts_backward,
 )
 from .sampler import Block, DPNeighborSampler, MPSampler, MixedNeighborSampler, SPGATSampler, SPVirtualSampler, create_block  # noqa: F401

@@ -26,6 +26,7 @@ FLAG_COPY_TIMEOUT = 128
 FLAG_BAD_OFFSETS = 256
 F32, BF16, F16 = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 IPC_HANDLE_BYTES = 64
 
 P = c_void_p
@@ -118,6 +119,12 @@ PROTOTYPES = {
     "apt_grouped_linear_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int64, c_int]),
     "apt_grouped_linear_forward": (c_int, [c_int, P, c_int64, c_int64, P, P, c_int64, P, c_int64, P, P, c_size_t, P, P]),
     "apt_grouped_linear_backward": (c_int, [c_int, P, c_int64, c_int64, P, c_int64, P, c_int64, P, P, P, P, P, c_size_t, P, P]),
+    "apt_route_experts": (c_int, [c_int, P, c_int64, c_int64, c_int64, c_int, P, c_int64, c_int64, c_int, c_int, c_float, P, P, P]),
+    "apt_route_experts_backward": (c_int, [c_int, P, c_int64, c_int64, c_int64, c_int, c_int, c_float, P, P, P, P]),
+    "apt_expert_rows_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "apt_expert_rows": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, P, P, P, P, c_size_t, P, P]),
+    "apt_expert_sum": (c_int, [c_int, P, c_int64, c_int64, c_int64, P, P, P, P, P]),
+    "apt_expert_sum_backward": (c_int, [c_int, P, c_int64, c_int64, c_int64, P, P, P, P, P, P, P]),
     "apt_p2p_create": (c_int, [c_int, c_int, c_size_t, ctypes.POINTER(P), P]),
     "apt_p2p_attach": (c_int, [P, c_int, P]),
     "apt_p2p_attach_ptr": (c_int, [P, c_int, P]),

@@ -546,6 +546,171 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
   }
 };
 
+// -------------------------------------------------------------------------------------- a layer of experts
+void on_current_device(const char* who, const Tensor& t) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || t.device().index() != device)
+    fail(std::string(who) + ": the tensors are on another device than the current one (cuda:" + std::to_string(device) + ")");
+}
+void same_shape(const char* who, const Tensor& a, const Tensor& b, const char* text) {
+  if (a.sizes() != b.sizes()) fail(std::string(who) + ": " + text);
+}
+
+// What a call of the router is beside its tensors.
+struct RouteSettings {
+  int64_t k, score, groups, top_groups, best;
+  bool renormalize;
+  double scale;
+};
+Tensor route_logits(const char* who, const Tensor& given) {
+  const Tensor logits = cuda(given, "logits");
+  float_code(who, logits);
+  if (logits.dim() != 2 || logits.size(1) == 0) fail(std::string(who) + ": logits must be [rows, experts]");
+  on_current_device(who, logits);
+  return logits;
+}
+std::tuple<Tensor, Tensor> route_forward(const Tensor& logits_in, const Tensor& bias_in, const RouteSettings& s) {
+  const Tensor logits = route_logits("route_experts", logits_in);
+  Tensor bias;
+  if (bias_in.defined()) {
+    bias = cuda(bias_in, "bias", at::kFloat, "torch.float32");
+    if (bias.dim() != 1 || bias.size(0) != logits.size(1)) fail("route_experts: bias must have one value an expert");
+    same_device("route_experts", logits, bias, "bias");
+  }
+  if (s.k < 1) fail("route_experts: k must be at least 1");
+  const int64_t rows = logits.size(0);
+  Tensor chosen = at::empty({rows, s.k}, logits.options().dtype(at::kLong)), weights = at::empty({rows, s.k}, logits.options().dtype(at::kFloat));
+  check(apt_route_experts(dtype_code(logits.scalar_type()), data(logits), rows, logits.size(1), s.k, (int)s.score, (const float*)data_or_null(bias), s.groups,
+                          s.top_groups, (int)s.best, s.renormalize, (float)s.scale, (int64_t*)mut(chosen), (float*)mut(weights), stream()));
+  return {chosen, weights};
+}
+Tensor route_backward(const Tensor& logits_in, const Tensor& chosen_in, const Tensor& grad_in, int64_t score, bool renormalize, double scale) {
+  const char* const who = "route_experts_backward";
+  const Tensor logits = route_logits(who, logits_in), chosen = ids(chosen_in, "experts"), grad = cuda(grad_in, "grad_weights", at::kFloat, "torch.float32");
+  if (chosen.dim() != 2 || chosen.size(0) != logits.size(0)) fail(std::string(who) + ": experts must be [rows, k]");
+  same_shape(who, chosen, grad, "grad_weights must be like experts");
+  same_device(who, logits, chosen, "experts");
+  same_device(who, logits, grad, "grad_weights");
+  Tensor out = at::empty(logits.sizes(), logits.options());
+  check(apt_route_experts_backward(dtype_code(logits.scalar_type()), data(logits), logits.size(0), logits.size(1), chosen.size(1), (int)score, renormalize,
+                                   (float)scale, ptr(chosen), (const float*)data(grad), mut(out), stream()));
+  return out;
+}
+struct RouteFunction : public torch::autograd::Function<RouteFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const OptTensor& bias, int64_t k, int64_t score,
+                                                int64_t groups, int64_t top_groups, int64_t best, bool renormalize, double scale) {
+    auto [chosen, weights] = route_forward(logits, given(bias), {k, score, groups, top_groups, best, renormalize, scale});
+    ctx->save_for_backward({logits, chosen});
+    ctx->mark_non_differentiable({chosen});
+    ctx->saved_data["score"] = score;
+    ctx->saved_data["renormalize"] = renormalize;
+    ctx->saved_data["scale"] = scale;
+    return {chosen, weights};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    torch::autograd::variable_list r(9);
+    r[0] = route_backward(v[0], v[1], grads[1], ctx->saved_data["score"].toInt(), ctx->saved_data["renormalize"].toBool(), ctx->saved_data["scale"].toDouble());
+    return only_once("route_experts", std::move(r), v[0], Tensor(), Tensor(), grads[1]);
+  }
+};
+
+// (rows, offsets, place)
+std::tuple<Tensor, Tensor, Tensor> expert_rows(const Tensor& x_in, const Tensor& experts_in, int64_t num_experts, const Tensor& words) {
+  const Tensor x = cuda(x_in, "x"), experts = ids(experts_in, "experts");
+  float_code("expert_rows", x);
+  if (x.dim() != 2 || x.size(1) == 0) fail("expert_rows: x must be [rows, dim]");
+  if (experts.dim() < 1 || experts.dim() > 2 || experts.size(0) != x.size(0)) fail("expert_rows: experts must be [rows, k] or [rows]");
+  on_current_device("expert_rows", x);
+  same_device("expert_rows", x, experts, "experts");
+  if (num_experts < 1) fail("expert_rows: num_experts must be at least 1");
+  const int64_t rows = x.size(0), k = experts.dim() == 2 ? experts.size(1) : 1;
+  if (k < 1) fail("expert_rows: experts must name one expert a row at least");
+  Tensor out = at::empty({rows * k, x.size(1)}, x.options()), offsets = at::empty({num_experts + 1}, experts.options()), place = at::empty(experts.sizes(), experts.options()), ws;
+  const size_t bytes = apt_expert_rows_workspace_bytes(rows * k, num_experts);
+  if (bytes) ws = scratch(x, bytes);
+  check(apt_expert_rows(data(x), rows, x.size(1) * x.element_size(), ptr(experts), k, num_experts, mut(out), (int64_t*)mut(offsets), (int64_t*)mut(place),
+                        mut_or_null(ws), bytes, status_word(words), stream()));
+  return {out, offsets, place};
+}
+
+struct SumProblem {
+  Tensor y, weights, place;
+  int64_t rows, dim, k;
+};
+SumProblem sum_problem(const char* who, const Tensor& y, const char* y_name, const Tensor& weights, const Tensor& place) {
+  SumProblem q;
+  q.y = cuda(y, y_name);
+  q.place = ids(place, "place");
+  float_code(who, q.y);
+  if (q.place.dim() < 1 || q.place.dim() > 2) fail(std::string(who) + ": place must be [rows, k] or [rows]");
+  q.rows = q.place.size(0), q.k = q.place.dim() == 2 ? q.place.size(1) : 1;
+  if (q.k < 1 || q.y.dim() != 2 || q.y.size(1) == 0 || q.y.size(0) != q.place.numel())
+    fail(std::string(who) + ": " + y_name + " must have a row for each of the " + std::to_string(q.place.numel()) + " places");
+  q.dim = q.y.size(1);
+  on_current_device(who, q.y);
+  same_device(who, q.y, q.place, "place");
+  if (weights.defined()) {
+    q.weights = cuda(weights, "weights", at::kFloat, "torch.float32");
+    same_shape(who, q.weights, q.place, "weights must be like place");
+    same_device(who, q.y, q.weights, "weights");
+  }
+  return q;
+}
+// Without weights: the gradient of expert_rows.
+Tensor expert_sum(const char* who, const Tensor& y, const char* y_name, const Tensor& weights, const Tensor& place, const Tensor& words) {
+  const SumProblem q = sum_problem(who, y, y_name, weights, place);
+  Tensor out = at::empty({q.rows, q.dim}, q.y.options());
+  check(apt_expert_sum(dtype_code(q.y.scalar_type()), data(q.y), q.rows, q.dim, q.k, (const float*)data_or_null(q.weights), ptr(q.place), mut(out), status_word(words),
+                       stream()));
+  return out;
+}
+std::tuple<Tensor, Tensor> expert_sum_backward(const Tensor& y, const Tensor& weights, const Tensor& place, const Tensor& grad_in, bool want_y, bool want_weights,
+                                               const Tensor& words) {
+  const char* const who = "expert_sum_backward";
+  const SumProblem q = sum_problem(who, y, "y", weights, place);
+  const Tensor grad = cuda(grad_in, "grad_out");
+  if (grad.scalar_type() != q.y.scalar_type() || grad.dim() != 2 || grad.size(0) != q.rows || grad.size(1) != q.dim)
+    fail(std::string(who) + ": grad_out must be [rows, dim] of y's dtype");
+  same_device(who, q.y, grad, "grad_out");
+  Tensor grad_y, grad_weights;
+  if (want_y) grad_y = at::empty(q.y.sizes(), q.y.options());
+  if (want_weights) grad_weights = at::empty(q.weights.sizes(), q.weights.options());
+  check(apt_expert_sum_backward(dtype_code(q.y.scalar_type()), data(q.y), q.rows, q.dim, q.k, (const float*)data(q.weights), ptr(q.place), data(grad),
+                                mut_or_null(grad_y), (float*)mut_or_null(grad_weights), status_word(words), stream()));
+  return {grad_y, grad_weights};
+}
+
+struct ExpertRowsFunction : public torch::autograd::Function<ExpertRowsFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& experts, int64_t num_experts, const Tensor& words) {
+    auto [rows, offsets, place] = expert_rows(x, experts, num_experts, words);
+    ctx->save_for_backward({place});
+    ctx->mark_non_differentiable({offsets, place});
+    ctx->saved_data["words"] = words;
+    return {rows, offsets, place};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    Tensor gx = expert_sum("expert_rows_backward", grads[0], "grad_rows", Tensor(), v[0], ctx->saved_data["words"].toTensor());
+    return only_once("expert_rows", {gx, Tensor(), Tensor(), Tensor()}, grads[0], Tensor(), Tensor(), grads[0]);
+  }
+};
+struct ExpertSumFunction : public torch::autograd::Function<ExpertSumFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& y, const Tensor& weights, const Tensor& place, const Tensor& words) {
+    Tensor out = expert_sum("expert_sum", y, "y", weights, place, words);
+    ctx->save_for_backward({y, weights, place});
+    ctx->saved_data["wants"] = std::vector<int64_t>{wants_grad(y), wants_grad(weights)};
+    ctx->saved_data["words"] = words;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    const auto wants = ctx->saved_data["wants"].toIntVector();
+    auto [gy, gw] = expert_sum_backward(v[0], v[1], v[2], grads[0], wants[0], wants[1], ctx->saved_data["words"].toTensor());
+    return only_once("expert_sum", {gy, gw, Tensor(), Tensor()}, v[0], v[1], Tensor(), grads[0]);
+  }
+};
+
 // ------------------------------------------------------------------------------------------------ samplers
 // Page-locked words, also while some stream is being captured.
 Tensor pinned_words(int64_t count) {
@@ -971,5 +1136,28 @@ PYBIND11_MODULE(_native, m) {
   });
   m.def("linear_apply", [](const Tensor& x, const Tensor& weight, const Tensor& offsets, const OptTensor& bias, const Tensor& words) {
     return LinearFunction::apply(x, weight, offsets, bias, words);
+  });
+  m.def("route_forward", [](const Tensor& logits, const OptTensor& bias, int64_t k, int64_t score, int64_t groups, int64_t top_groups, int64_t best,
+                            bool renormalize, double scale) { return route_forward(logits, given(bias), {k, score, groups, top_groups, best, renormalize, scale}); });
+  m.def("route_backward", &route_backward);
+  m.def("route_apply", [](const Tensor& logits, const OptTensor& bias, int64_t k, int64_t score, int64_t groups, int64_t top_groups, int64_t best,
+                          bool renormalize, double scale) {
+    auto r = RouteFunction::apply(logits, bias, k, score, groups, top_groups, best, renormalize, scale);
+    return std::make_tuple(r[0], r[1]);
+  });
+  m.def("expert_rows", &expert_rows);
+  m.def("expert_rows_backward", [](const Tensor& grad, const Tensor& place, const Tensor& words) {
+    return expert_sum("expert_rows_backward", grad, "grad_rows", Tensor(), place, words);
+  });
+  m.def("expert_rows_apply", [](const Tensor& x, const Tensor& experts, int64_t num_experts, const Tensor& words) {
+    auto r = ExpertRowsFunction::apply(x, experts, num_experts, words);
+    return std::make_tuple(r[0], r[1], r[2]);
+  });
+  m.def("expert_sum", [](const Tensor& y, const Tensor& weights, const Tensor& place, const Tensor& words) {
+    return expert_sum("expert_sum", y, "y", weights, place, words);
+  });
+  m.def("expert_sum_backward", &expert_sum_backward);
+  m.def("expert_sum_apply", [](const Tensor& y, const Tensor& weights, const Tensor& place, const Tensor& words) {
+    return ExpertSumFunction::apply(y, weights, place, words);
   });
 }

@@ -1133,6 +1133,88 @@ class Dropout:
         return _native.dropout_apply(x, float(p), *_stream_key(key, call_id))
 
 
+# ----------------------------------------------------------------- a layer of experts
+# rows -> route_experts(logits) -> expert_rows -> grouped_linear and what else there is of ragged groups -> expert_sum. The experts of a
+# row are its router's, -1 for none; how many rows an expert has only the device knows.
+_SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+
+
+def _score(score: str) -> int:
+    if score not in _SCORES:
+        raise RuntimeError(f"route_experts: unknown score {score!r} (one of {', '.join(_SCORES)})")
+    return _SCORES[score]
+
+
+def route_experts(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optional[torch.Tensor] = None, num_groups: int = 1, top_groups: int = 1,
+                  group_best: int = 1, renormalize: bool = True, scale: float = 1.0):
+    """The k experts that every row goes to, and their weights: (experts int64 [R, k], weights float32 [R, k]) of logits [R, E] (at most 1024).
+
+    s = softmax(logits) or sigmoid(logits). The k largest of s + bias are chosen (bias float32 [E], for the balance of the experts' load;
+    without one the largest logits), largest first, ties to the lowest index. num_groups > 1: the experts are that many equal runs, and only
+    those of the top_groups groups count whose best (group_best=2: best two, added up) of s + bias, or of s, are largest. weights = scale s,
+    divided by the sum of the row's chosen s with renormalize. An expert with a logit (or s + bias) of -inf is never chosen; where fewer than
+    k are left, the others are -1 with weight 0."""
+    return _native.route_forward(logits, bias, int(k), _score(score), int(num_groups), int(top_groups), int(group_best), bool(renormalize), float(scale))
+
+
+def route_experts_backward(logits, experts, grad_weights, score: str = "softmax", renormalize: bool = True, scale: float = 1.0):
+    """Gradient of route_experts' weights with respect to the logits, for the experts that it gave and grad_weights float32 [R, k]. The
+    choice and the bias have none."""
+    return _native.route_backward(logits, experts, grad_weights, _score(score), bool(renormalize), float(scale))
+
+
+class RouteExperts:
+    """route_experts with its backward: ``experts, weights = RouteExperts.apply(logits, k, score, bias, num_groups, top_groups, group_best,
+    renormalize, scale)`` (an autograd function on the C++ side; second derivatives raise)."""
+
+    @staticmethod
+    def apply(logits, k, score="softmax", bias=None, num_groups=1, top_groups=1, group_best=1, renormalize=True, scale=1.0):
+        return _native.route_apply(logits, bias, int(k), _score(score), int(num_groups), int(top_groups), int(group_best), bool(renormalize), float(scale))
+
+
+def expert_rows(x: torch.Tensor, experts: torch.Tensor, num_experts: int):
+    """A copy of every row of x [R, D] for each of its experts (int64 [R, k], or [R]), ordered by expert and within one as they come:
+    (rows [R k, D], offsets [num_experts + 1] as grouped_linear and group_norm_act take them, place like experts). rows[place[r, j]] is
+    x[r]; a pair whose expert is -1 lies behind the last group, as a row of zeros, and its place is -1 - the position. Other experts outside
+    [0, num_experts) count as -1 and raise at the next host read (check_status)."""
+    return _native.expert_rows(x, experts, int(num_experts), STATE.words())
+
+
+def expert_rows_backward(grad_rows, place):
+    """Gradient of expert_rows' rows with respect to x: the sum over each row's places."""
+    return _native.expert_rows_backward(grad_rows, place, STATE.words())
+
+
+class ExpertRows:
+    """expert_rows with its backward: ``rows, offsets, place = ExpertRows.apply(x, experts, num_experts)`` (an autograd function on the
+    C++ side; second derivatives raise)."""
+
+    @staticmethod
+    def apply(x, experts, num_experts):
+        return _native.expert_rows_apply(x, experts, int(num_experts), STATE.words())
+
+
+def expert_sum(y: torch.Tensor, weights: torch.Tensor, place: torch.Tensor) -> torch.Tensor:
+    """out[r] = sum_j weights[r, j] y[place[r, j]] over the pairs that have an expert: y [R k, D], weights float32 [R, k] (or [R]), place as
+    expert_rows gave it; out [R, D]. Sums are in fp32 and rounded once."""
+    return _native.expert_sum(y, weights, place, STATE.words())
+
+
+def expert_sum_backward(y, weights, place, grad_out, want_y: bool = True, want_weights: bool = True):
+    """Gradients of expert_sum for grad_out [R, D]: (grad_y, grad_weights), None where not wanted. Rows of pairs without an expert have
+    gradients of zero."""
+    return _native.expert_sum_backward(y, weights, place, grad_out, bool(want_y), bool(want_weights), STATE.words())
+
+
+class ExpertSum:
+    """expert_sum with its backward: ``out = ExpertSum.apply(y, weights, place)`` (an autograd function on the C++ side; second derivatives
+    raise)."""
+
+    @staticmethod
+    def apply(y, weights, place):
+        return _native.expert_sum_apply(y, weights, place, STATE.words())
+
+
 # ------------------------------------------------------------------ row movers
 def rows_gather(inp: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
     """out[i] = inp[index[i]] for 2-D inp (the model's h[inverse_idx],

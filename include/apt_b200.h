@@ -863,6 +863,48 @@ int apt_grouped_linear_backward(int dtype, const void* x, int64_t rows, int64_t 
                                 void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
                                 int32_t* status_word, void* stream);
 
+/* Which experts a row goes to. With s = softmax(logits) or 1 / (1 + exp(-logits))
+ * over the row's `experts` logits, the k largest of s + bias (bias NULL: of the
+ * logits) are chosen, ties to the lowest index, largest first; with groups > 1
+ * equal runs of experts, only out of the top_groups groups whose best (or whose
+ * best two, added up) of s + bias (NULL: of s) are largest. Ranks are those of the
+ * exact scores. chosen [rows, k], weights [rows, k] = scale s, divided by the
+ * sum of the row's chosen s where renormalize is not 0. An expert whose logit or
+ * s + bias is -inf is never chosen; where fewer than k are left the others are -1
+ * with weight 0. Rows with a NaN: any experts, NaN weights.
+ * Backward: grad_logits [rows, experts] of grad_weights, for `chosen` as it came (the
+ * choice itself and the bias have no gradient). */
+typedef enum apt_score { APT_SCORE_SOFTMAX = 0, APT_SCORE_SIGMOID = 1 } apt_score;
+#define APT_ROUTE_MAX_EXPERTS 1024
+#define APT_ROUTE_MAX_CHOSEN 64
+int apt_route_experts(int dtype, const void* logits, int64_t rows, int64_t experts, int64_t k, int score, const float* bias, int64_t groups,
+                      int64_t top_groups, int group_best, int renormalize, float scale, int64_t* chosen,
+                      float* weights, void* stream);
+int apt_route_experts_backward(int dtype, const void* logits, int64_t rows, int64_t experts, int64_t k, int score, int renormalize,
+                               float scale, const int64_t* chosen, const float* grad_weights, void* grad_logits,
+                               void* stream);
+
+/* A copy of every row for each of its k experts, ordered by expert and within one
+ * as they come: rows [rows k, row_bytes], offsets [num_experts + 1] as the
+ * operators of ragged groups take them, place [rows, k] where pair (r, j) went. A
+ * pair whose expert is -1 goes behind the last group, its row is zeros and its place
+ * -1 - the position. Experts beyond those set APT_FLAG_ID_OUT_OF_RANGE and
+ * count as -1. num_experts at most APT_GROUPED_LINEAR_MAX_GROUPS. */
+size_t apt_expert_rows_workspace_bytes(int64_t pairs, int64_t num_experts);
+int apt_expert_rows(const void* x, int64_t rows, int64_t row_bytes, const int64_t* experts, int64_t k, int64_t num_experts,
+                    void* out, int64_t* offsets, int64_t* place, void* workspace, size_t workspace_bytes,
+                    int32_t* status_word, void* stream);
+
+/* out[r] = sum_j weights[r, j] y[place[r, j]] over the pairs with an expert: y
+ * [rows k, dim], weights [rows, k] or NULL (ones: the gradient of apt_expert_rows),
+ * place as apt_expert_rows gave it (places beyond y set APT_FLAG_ID_OUT_OF_RANGE and
+ * count for nothing). Backward: grad_y [rows k, dim], zeros for the pairs without
+ * an expert, and grad_weights [rows, k]; each unless NULL. */
+int apt_expert_sum(int dtype, const void* y, int64_t rows, int64_t dim, int64_t k, const float* weights, const int64_t* place,
+                   void* out, int32_t* status_word, void* stream);
+int apt_expert_sum_backward(int dtype, const void* y, int64_t rows, int64_t dim, int64_t k, const float* weights, const int64_t* place,
+                            const void* grad_out, void* grad_y, float* grad_weights, int32_t* status_word, void* stream);
+
 /* --------------------------------------------------------- setup utilities
  * Not on the timed path; they prepare the synthetic graphs of the benchmark
  * on the GPU so that a 1.6 G-edge graph is built in seconds. */

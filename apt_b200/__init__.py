@@ -26,5 +26,6 @@ from .ops import (  # noqa: F401
     Dropout, GroupNormAct, GroupedLinear, dropout, group_norm_act, group_norm_act_backward, grouped_linear, grouped_linear_backward,
     ExpertRows, ExpertSum, RouteExperts, expert_rows, expert_rows_backward, expert_sum, expert_sum_backward, route_experts,
     route_experts_backward,
+    LinearCrossEntropy, linear_cross_entropy, linear_cross_entropy_backward,
 )
 from .sampler import Block, DPNeighborSampler, MPSampler, MixedNeighborSampler, SPGATSampler, SPVirtualSampler, create_block  # noqa: F401

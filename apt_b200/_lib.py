@@ -27,6 +27,7 @@ FLAG_BAD_OFFSETS = 256
 F32, BF16, F16 = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+LOSS_NONE, LOSS_SUM, LOSS_MEAN = 0, 1, 2
 IPC_HANDLE_BYTES = 64
 
 P = c_void_p
@@ -125,6 +126,9 @@ PROTOTYPES = {
     "apt_expert_rows": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, P, P, P, P, c_size_t, P, P]),
     "apt_expert_sum": (c_int, [c_int, P, c_int64, c_int64, c_int64, P, P, P, P, P]),
     "apt_expert_sum_backward": (c_int, [c_int, P, c_int64, c_int64, c_int64, P, P, P, P, P, P, P]),
+    "apt_linear_cross_entropy_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int]),
+    "apt_linear_cross_entropy_forward": (c_int, [c_int, P, c_int64, c_int64, P, P, c_int64, P, c_int64, c_int, P, P, P, c_size_t, P, P]),
+    "apt_linear_cross_entropy_backward": (c_int, [c_int, P, c_int64, c_int64, P, P, c_int64, P, c_int, P, P, P, P, P, P, c_size_t, P, P]),
     "apt_p2p_create": (c_int, [c_int, c_int, c_size_t, ctypes.POINTER(P), P]),
     "apt_p2p_attach": (c_int, [P, c_int, P]),
     "apt_p2p_attach_ptr": (c_int, [P, c_int, P]),

@@ -17,7 +17,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libapt_b200.so")
 NATIVE = os.path.join(PKG_DIR, "native")
 NATIVE_PATH = os.path.join(PKG_DIR, "_native.so")
 SOURCES = ["core.cu", "sample.cu", "relabel.cu", "bucket.cu", "gather.cu", "spmm.cu", "widen.cu", "spmm_f32.cu", "spmm_bf16.cu",
-           "spmm_f16.cu", "gat.cu", "virt.cu", "hotness.cu", "p2p.cu", "util.cu", "dropout.cu", "group_norm.cu", "group_norm_f32.cu", "group_norm_bf16.cu", "group_norm_f16.cu", "grouped_linear.cu", "route.cu", "experts.cu"]
+           "spmm_f16.cu", "gat.cu", "virt.cu", "hotness.cu", "p2p.cu", "util.cu", "dropout.cu", "group_norm.cu", "group_norm_f32.cu", "group_norm_bf16.cu", "group_norm_f16.cu", "grouped_linear.cu", "route.cu", "experts.cu", "loss.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",

@@ -711,6 +711,82 @@ struct ExpertSumFunction : public torch::autograd::Function<ExpertSumFunction> {
   }
 };
 
+// ------------------------------------------------------------------------------------------------ the loss
+struct LossProblem {
+  Tensor x, weight, bias, labels;
+  int code;
+  int64_t rows, dim, classes;
+};
+LossProblem loss_problem(const char* who, const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& labels) {
+  LossProblem q;
+  q.x = cuda(x, "x");
+  q.code = float_code(who, q.x);
+  on_current_device(who, q.x);
+  q.weight = cuda(weight, "weight");
+  q.labels = ids(labels, "labels");
+  if (q.x.dim() != 2 || q.weight.dim() != 2 || q.weight.size(1) != q.x.size(1)) fail(std::string(who) + ": x must be [rows, dim] and weight [classes, dim]");
+  if (q.weight.scalar_type() != q.x.scalar_type()) fail(std::string(who) + ": mixed dtypes " + dtype_name(q.x) + "/" + dtype_name(q.weight));
+  q.rows = q.x.size(0), q.dim = q.x.size(1), q.classes = q.weight.size(0);
+  if (q.labels.dim() != 1 || q.labels.size(0) != q.rows) fail(std::string(who) + ": labels must be [rows]");
+  if (bias.defined()) {
+    q.bias = cuda(bias, "bias");
+    if (q.bias.dim() != 1 || q.bias.size(0) != q.classes) fail(std::string(who) + ": bias must be [classes]");
+    if (q.bias.scalar_type() != q.x.scalar_type()) fail(std::string(who) + ": mixed dtypes " + dtype_name(q.x) + "/" + dtype_name(q.bias));
+  }
+  for (const auto& [t, name] : {std::pair<const Tensor*, const char*>{&q.weight, "weight"}, {&q.labels, "labels"}, {&q.bias, "bias"}}) same_device(who, q.x, *t, name);
+  for (Tensor* t : {&q.x, &q.weight}) *t = aligned(*t);
+  return q;
+}
+// (loss, what the backward needs)
+std::tuple<Tensor, Tensor> loss_forward(const Tensor& x, const Tensor& weight, const Tensor& labels, const Tensor& bias, int64_t reduction, int64_t ignore,
+                                        const Tensor& words) {
+  const LossProblem q = loss_problem("linear_cross_entropy", x, weight, bias, labels);
+  const auto floats = q.x.options().dtype(at::kFloat);
+  Tensor loss = reduction == APT_LOSS_NONE ? at::empty({q.rows}, floats) : at::empty({}, floats), saved = at::empty({2 * q.rows + 1}, floats), ws;
+  const size_t bytes = apt_linear_cross_entropy_workspace_bytes(q.code, q.rows, q.dim, q.classes, 0);
+  if (bytes) ws = scratch(q.x, bytes);
+  check(apt_linear_cross_entropy_forward(q.code, data(q.x), q.rows, q.dim, data(q.weight), data_or_null(q.bias), q.classes, ptr(q.labels), ignore, (int)reduction,
+                                         (float*)mut(loss), (float*)mut(saved), mut_or_null(ws), bytes, status_word(words), stream()));
+  return {loss, saved};
+}
+std::tuple<Tensor, Tensor, Tensor> loss_backward(const Tensor& x, const Tensor& weight, const Tensor& labels, const Tensor& bias, const Tensor& saved_in,
+                                                 const Tensor& grad_in, int64_t reduction, bool want_x, bool want_weight, bool want_bias, const Tensor& words) {
+  const char* const who = "linear_cross_entropy_backward";
+  const LossProblem q = loss_problem(who, x, weight, bias, labels);
+  const Tensor saved = cuda(saved_in, "saved", at::kFloat, "torch.float32"), grad = cuda(grad_in, "grad_loss", at::kFloat, "torch.float32");
+  if (saved.numel() != 2 * q.rows + 1) fail(std::string(who) + ": saved is not that of this call");
+  if (grad.numel() != (reduction == APT_LOSS_NONE ? q.rows : 1)) fail(std::string(who) + ": grad_loss must be like the loss");
+  same_device(who, q.x, saved, "saved");
+  same_device(who, q.x, grad, "grad_loss");
+  Tensor grad_x, grad_weight, grad_bias, ws;
+  if (want_x) grad_x = at::empty(q.x.sizes(), q.x.options());
+  if (want_weight) grad_weight = at::empty(q.weight.sizes(), q.weight.options());
+  if (want_bias && q.bias.defined()) grad_bias = at::empty({q.classes}, q.weight.options());
+  const size_t bytes = apt_linear_cross_entropy_workspace_bytes(q.code, q.rows, q.dim, q.classes, 1);
+  if (bytes) ws = scratch(q.x, bytes);
+  check(apt_linear_cross_entropy_backward(q.code, data(q.x), q.rows, q.dim, data(q.weight), data_or_null(q.bias), q.classes, ptr(q.labels), (int)reduction,
+                                          (const float*)data(saved), (const float*)data(grad), mut_or_null(grad_x), mut_or_null(grad_weight), mut_or_null(grad_bias),
+                                          mut_or_null(ws), bytes, status_word(words), stream()));
+  return {grad_x, grad_weight, grad_bias};
+}
+struct LossFunction : public torch::autograd::Function<LossFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& labels, const OptTensor& bias_in, int64_t reduction,
+                        int64_t ignore, const Tensor& words) {
+    const Tensor bias = given(bias_in);
+    auto [loss, saved] = loss_forward(x, weight, labels, bias, reduction, ignore, words);
+    ctx->save_for_backward({x, weight, labels, bias, saved});
+    ctx->saved_data["settings"] = std::vector<int64_t>{reduction, wants_grad(x), wants_grad(weight), wants_grad(bias)};
+    ctx->saved_data["words"] = words;
+    return loss;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    const auto s = ctx->saved_data["settings"].toIntVector();
+    auto [gx, gw, gb] = loss_backward(v[0], v[1], v[2], v[3], v[4], grads[0], s[0], s[1], s[2], s[3], ctx->saved_data["words"].toTensor());
+    return only_once("linear_cross_entropy", {gx, gw, Tensor(), gb, Tensor(), Tensor(), Tensor()}, v[0], v[1], v[3], grads[0]);
+  }
+};
+
 // ------------------------------------------------------------------------------------------------ samplers
 // Page-locked words, also while some stream is being captured.
 Tensor pinned_words(int64_t count) {
@@ -1136,6 +1212,16 @@ PYBIND11_MODULE(_native, m) {
   });
   m.def("linear_apply", [](const Tensor& x, const Tensor& weight, const Tensor& offsets, const OptTensor& bias, const Tensor& words) {
     return LinearFunction::apply(x, weight, offsets, bias, words);
+  });
+  m.def("loss_forward", [](const Tensor& x, const Tensor& weight, const Tensor& labels, const OptTensor& bias, int64_t reduction, int64_t ignore, const Tensor& words) {
+    return loss_forward(x, weight, labels, given(bias), reduction, ignore, words);
+  });
+  m.def("loss_backward", [](const Tensor& x, const Tensor& weight, const Tensor& labels, const OptTensor& bias, const Tensor& saved, const Tensor& grad,
+                            int64_t reduction, bool want_x, bool want_weight, bool want_bias, const Tensor& words) {
+    return loss_backward(x, weight, labels, given(bias), saved, grad, reduction, want_x, want_weight, want_bias, words);
+  });
+  m.def("loss_apply", [](const Tensor& x, const Tensor& weight, const Tensor& labels, const OptTensor& bias, int64_t reduction, int64_t ignore, const Tensor& words) {
+    return LossFunction::apply(x, weight, labels, bias, reduction, ignore, words);
   });
   m.def("route_forward", [](const Tensor& logits, const OptTensor& bias, int64_t k, int64_t score, int64_t groups, int64_t top_groups, int64_t best,
                             bool renormalize, double scale) { return route_forward(logits, given(bias), {k, score, groups, top_groups, best, renormalize, scale}); });

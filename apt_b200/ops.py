@@ -1215,6 +1215,43 @@ class ExpertSum:
         return _native.expert_sum_apply(y, weights, place, STATE.words())
 
 
+# -------------------------------------------------------------------------- the loss
+_REDUCTIONS = {"none": _lib.LOSS_NONE, "sum": _lib.LOSS_SUM, "mean": _lib.LOSS_MEAN}
+
+
+def _reduction(reduction: str) -> int:
+    if reduction not in _REDUCTIONS:
+        raise RuntimeError(f"linear_cross_entropy: unknown reduction {reduction!r} (one of {', '.join(_REDUCTIONS)})")
+    return _REDUCTIONS[reduction]
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, bias: Optional[torch.Tensor] = None, reduction: str = "mean",
+                         ignore_index: int = -100, return_saved: bool = False):
+    """Softmax cross entropy of the logits x @ weight.T + bias, which are never kept: x [R, K], weight [V, K] and bias [V] of one dtype
+    (float32, bfloat16 or float16), labels int64 [R]. float32: "none" [R], "sum", or "mean" over the rows whose label is not ignore_index
+    (0 where there are none; rows that are ignored have a loss of 0). Other labels outside [0, V) are left out and raise at the next host
+    read (check_status). return_saved: also what the backward takes."""
+    loss, saved = _native.loss_forward(x, weight, labels, bias, _reduction(reduction), int(ignore_index), STATE.words())
+    return (loss, saved) if return_saved else loss
+
+
+def linear_cross_entropy_backward(x, weight, labels, saved, grad_loss, bias=None, reduction: str = "mean", want_x: bool = True, want_weight: bool = True,
+                                  want_bias: bool = True):
+    """Gradients of linear_cross_entropy for grad_loss (float32, like the loss) and what the forward saved: (grad_x, grad_weight,
+    grad_bias), None where not wanted or without a bias. The logits are made once more, some classes at a time."""
+    return _native.loss_backward(x, weight, labels, bias, saved, grad_loss, _reduction(reduction), bool(want_x), bool(want_weight), bool(want_bias),
+                                 STATE.words())
+
+
+class LinearCrossEntropy:
+    """linear_cross_entropy with its backward: ``loss = LinearCrossEntropy.apply(x, weight, labels, bias, reduction, ignore_index)`` (an
+    autograd function on the C++ side; second derivatives raise)."""
+
+    @staticmethod
+    def apply(x, weight, labels, bias=None, reduction="mean", ignore_index=-100):
+        return _native.loss_apply(x, weight, labels, bias, _reduction(reduction), int(ignore_index), STATE.words())
+
+
 # ------------------------------------------------------------------ row movers
 def rows_gather(inp: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
     """out[i] = inp[index[i]] for 2-D inp (the model's h[inverse_idx],

@@ -905,6 +905,26 @@ int apt_expert_sum(int dtype, const void* y, int64_t rows, int64_t dim, int64_t 
 int apt_expert_sum_backward(int dtype, const void* y, int64_t rows, int64_t dim, int64_t k, const float* weights, const int64_t* place,
                             const void* grad_out, void* grad_y, float* grad_weights, int32_t* status_word, void* stream);
 
+/* Softmax cross entropy of z = x weight^T + bias against labels, the logits z never
+ * kept: x [rows, dim], weight [classes, dim], bias [classes] or NULL, of dtype; labels
+ * [rows], of which `ignore` takes the row out of the loss. Other labels outside [0,
+ * classes) set APT_FLAG_ID_OUT_OF_RANGE and take it out too. loss: float [rows]
+ * (0 for rows that are out), their sum, or their mean over the rows that count (0
+ * where none does). saved [2 rows + 1] is for the backward, which gives grad_x,
+ * grad_weight and grad_bias (each unless NULL) for grad_loss [rows] or [1]. Both are
+ * NaN where a row that counts has a logit that is NaN or +inf. dim at most
+ * APT_GROUPED_LINEAR_MAX_DIM. The workspace is aligned to 256 bytes. */
+typedef enum apt_loss_reduction { APT_LOSS_NONE = 0, APT_LOSS_SUM = 1, APT_LOSS_MEAN = 2 } apt_loss_reduction;
+size_t apt_linear_cross_entropy_workspace_bytes(int dtype, int64_t rows, int64_t dim, int64_t classes, int backward);
+int apt_linear_cross_entropy_forward(int dtype, const void* x, int64_t rows, int64_t dim, const void* weight, const void* bias,
+                                     int64_t classes, const int64_t* labels, int64_t ignore, int reduction, float* loss,
+                                     float* saved, void* workspace, size_t workspace_bytes, int32_t* status_word,
+                                     void* stream);
+int apt_linear_cross_entropy_backward(int dtype, const void* x, int64_t rows, int64_t dim, const void* weight, const void* bias,
+                                      int64_t classes, const int64_t* labels, int reduction, const float* saved,
+                                      const float* grad_loss, void* grad_x, void* grad_weight, void* grad_bias,
+                                      void* workspace, size_t workspace_bytes, int32_t* status_word, void* stream);
+
 /* --------------------------------------------------------- setup utilities
  * Not on the timed path; they prepare the synthetic graphs of the benchmark
  * on the GPU so that a 1.6 G-edge graph is built in seconds. */

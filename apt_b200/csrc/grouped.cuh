@@ -55,8 +55,13 @@ struct GroupedTraits {
   static constexpr int kBox = 128 / (int)sizeof(T);            // elements of a box's row
   static constexpr int kMostN = kSplit ? 128 : 256;            // columns of a tile
   // warps that bring tiles out: two for each quarter of tensor memory's lanes, or one beside the eight that take fp32 apart
-  static constexpr int kOutWarps = kSplit ? 4 : 8;
-  static constexpr int kThreads = kSplit ? 512 : 384;
+  // (logits in 16 bits: two gangs of eight, each with every other tile. The exponentials of a tile take as long as its products of 256 terms, and a
+  // tile's way through a warp, with its waits for tensor memory and for what is known of its rows, is longer than that)
+  static constexpr int kOutWarps = kSplit ? 4 : kClasses ? 16 : 8, kGangs = kClasses && !kSplit ? 2 : 1, kTurns = kOutWarps / kGangs / 4;
+  static constexpr int kThreads = kSplit ? 512 : 128 + 32 * kOutWarps;
+  // shared memory of one of those warps, in which 32 rows lie on their way out (or their statistics on the way to the warp that joins them)
+  static constexpr int kStaging = MODE == kStats ? (kTurns - 1) * 32 * 8 : MODE == kSumX ? 0 : MODE == kSlopes && !kSplit ? 2048 : 4096;
+  static constexpr int kBiasFloats = kOverRows ? 512 : 256 * kGangs;
   // a sum in tensor memory has so many stages at most: 1024 terms of fp32, 8192 rows of 16 bits (with 4096, 65536 x 1024 -> 1024 bf16, dw and db 182 -> 205 us:
   // the warps that bring parts out are those that add up db, for which the stages wait)
   static constexpr bool kCuts = kSplit || kOverRows || MODE == kSumX;
@@ -72,7 +77,7 @@ struct LossCall {
   const int64_t* labels;
   int64_t class0, ignore;       // the classes' first, the label of rows that do not count
   int64_t pitch;                // of the parts and of the slopes
-  float2* parts;                // [tiles of classes x warps that share one's rows][pitch]
+  float2* parts;                // [tiles of classes][pitch]
   float* picked;                // the logit of the row's label
   const float2* stats;
   const float* grad;            // of the rows' losses; null: all the same
@@ -151,7 +156,7 @@ struct GroupedWalk {
       next = c.keep ? blockIdx.x * all / gridDim.x : blockIdx.x, step = c.keep ? 1 : gridDim.x, end = c.keep ? (blockIdx.x + 1) * all / gridDim.x : all;
     }
   }
-  static __device__ __forceinline__ int64_t quotient(int64_t a, int b) { return a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }
+  static __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }
   __device__ __forceinline__ int group_of(int t, int n) const {
     int lo = 0, hi = n;         // the last group whose prefix is at most t
     while (hi - lo > 1) {
@@ -167,16 +172,19 @@ struct GroupedWalk {
   }
   // Rows against classes: bands of rows that stay in L2 while the classes go by, each once for all of the band; within a band the rows of a tile of
   // classes one behind the other. dx: all of one part of the contraction before the next one, columns of the same rows beside one another.
-  __device__ __forceinline__ void take_listed(GroupedItem* item) const {
+  __device__ __forceinline__ void take_listed(GroupedItem* item) {
     int t, n, part = 0;
     if constexpr (MODE == kSumX) {
       const int64_t rest = quotient(next, c.tiles_n);
       n = (int)(next - rest * c.tiles_n), part = (int)quotient(rest, c.tiles_m), t = (int)(rest - (int64_t)part * c.tiles_m);
+    } else if (c.keep && last_t >= 0 && last_t + 1 < c.tiles_m) {      // (one band)
+      t = last_t + 1, n = last_n;
     } else {
-      const int64_t whole = (int64_t)c.band * c.tiles_n, b = next / whole, at = next - b * whole;
+      const int64_t whole = (int64_t)c.band * c.tiles_n, b = quotient(next, whole), at = next - b * whole;
       const int here = min(c.band, c.tiles_m - (int)b * c.band);
       n = (int)quotient(at, here), t = (int)(b * c.band + (at - (int64_t)n * here));
     }
+    last_t = t, last_n = n;
     const int all = (c.num_k + Tr::kBlock * c.deep - 1) / (Tr::kBlock * c.deep);
     item->g = 0, item->m0 = t, item->n0 = n * c.tile_n;
     item->row = (int64_t)t * (c.tile_m * c.halves);
@@ -514,8 +522,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Of a row: the largest of its logits in these columns, in units of log2(e), and the sum of 2^(what the others are below it). The exponent is one
 // multiply-add of the logit, whose rounding the sum does not see: it refers to the number that was subtracted.
 template <typename T, int MODE>
-__device__ __forceinline__ void tile_statistics(uint32_t acc, int turn, int turns, int columns, const float* bias, int label, float* carry, int before, int after,
-                                                float2* part, float* picked, bool row) {
+__device__ __forceinline__ float2 tile_statistics(uint32_t acc, int turn, int turns, int columns, const float* bias, int label, float* carry, int before, int after,
+                                                  float* picked) {
   using Tr = GroupedTraits<T, MODE>;
   float top = -INFINITY, sum = 0.0f;
   for (int c0 = turn * 32; c0 < columns; c0 += turns * 32) {
@@ -562,7 +570,17 @@ __device__ __forceinline__ void tile_statistics(uint32_t acc, int turn, int turn
     for (int k = 0; k < 32; ++k) s[k % 4] += exp2_short(fmaf(v[k], kLog2e, -ref));
     sum += (s[0] + s[1]) + (s[2] + s[3]);
   }
-  if (row && !(Tr::kCuts && after)) *part = make_float2(top, sum);
+  return make_float2(top, sum);
+}
+// Statistics of other columns of the same row.
+__device__ __forceinline__ void join_statistics(float2* a, float2 b) {
+  if (b.x == -INFINITY) {
+    a->y += b.y;      // nothing, or NaN
+  } else if (b.x > a->x) {
+    a->y = a->y * exp2_short(a->x - b.x) + b.y, a->x = b.x;
+  } else {
+    a->y += b.y * exp2_short(b.x - a->x);
+  }
 }
 
 // The loss's slope along a row's logits: probabilities less one at the label, times the row's factor.
@@ -601,6 +619,37 @@ __device__ __forceinline__ Slopes row_slopes(const LossCall& l, int64_t row, boo
   return s;
 }
 
+// Slopes of 16 bits: 32 columns of a warp's 32 rows at a time, 64 bytes of each through shared memory. `rows` of them are there, `columns` of the tile;
+// to: whole 16-byte slices.
+template <typename T, int MODE>
+__device__ __forceinline__ void store_slopes(uint32_t acc, char* staging, int lane, int turn, int turns, T* to, int64_t ld, int rows, int columns, const float* bias,
+                                             const Slopes& slopes) {
+  for (int c0 = turn * 32; c0 < columns; c0 += turns * 32) {
+    float v[1][32];
+    load_sums<T, MODE>(acc + c0, v[0]);
+    if (bias)
+#pragma unroll
+      for (int k = 0; k < 32; k += 4) {
+        const float4 b = *(const float4*)(bias + c0 + k);
+        v[0][k] += b.x, v[0][k + 1] += b.y, v[0][k + 2] += b.z, v[0][k + 3] += b.w;
+      }
+    slopes(v, c0);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) *(uint4*)(staging + lane * 64 + ((s ^ ((lane >> 1) & 3)) << 4)) = rounded_slice<T>(&v[0][8 * s]);
+    __syncwarp();
+    const int s = lane & 3, r1 = lane >> 2;
+    uint4 slice[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) slice[k] = *(const uint4*)(staging + (8 * k + r1) * 64 + ((s ^ (((8 * k + r1) >> 1) & 3)) << 4));
+    T* p = to + (int64_t)r1 * ld + c0 + 8 * s;
+    const int left = c0 + 8 * s < columns ? rows - r1 : 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k, p += 8 * ld)
+      if (8 * k < left) *(uint4*)p = slice[k];
+    __syncwarp();
+  }
+}
+
 // dx: a part's sums, 16 slices of a row a lane, to where they are added up.
 template <typename T, int MODE>
 __device__ __forceinline__ void tile_to_slot(uint32_t acc, int turn, int turns, int columns, float* slot, bool add) {
@@ -630,9 +679,10 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   constexpr int kBuffers = 2;
   constexpr bool kMends = Tr::kOverRows && !Tr::kSplit;
   extern __shared__ char raw_shared[];
-  __shared__ uint64_t full[kMaxStages], free_[kMaxStages], ready[kMaxStages], used[kMaxStages], acc_full[2], acc_free[2], kept_full, kept_free, drained, met;
+  __shared__ uint64_t full[kMaxStages], free_[kMaxStages], ready[kMaxStages], used[kMaxStages], acc_full[2], acc_free[2], kept_full, kept_free, drained, met[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up_word, scan[33];
+  constexpr bool kJoins = MODE == kStats && Tr::kTurns > 1;      // several warps have parts of a row: `used` counts them, which only fp32 has a use for else
   volatile int* const gave_up = &gave_up_word;
   char* const shared = (char*)(((uintptr_t)raw_shared + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -648,8 +698,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   char* const pieces = copied + (size_t)c.copied_stages * copied_bytes;
   char* const kept = pieces + (size_t)c.piece_stages * piece_bytes;
   char* const staging = kept + (size_t)kept_stages * kept_bytes;
-  float* const bias = (float*)(staging + Tr::kOutWarps * 4096);      // of a tile in out; in dw the sums of db that several threads have
-  int *const prefix = (int*)(bias + (Tr::kOverRows ? 512 : 256)), *const begin = prefix + c.groups + 2;
+  float* const all_bias = (float*)(staging + Tr::kOutWarps * Tr::kStaging);      // of a tile in out; in dw the sums of db that several threads have
+  int *const prefix = (int*)(all_bias + Tr::kBiasFloats), *const begin = prefix + c.groups + 2;
 
   if (warp == 1) tmem_alloc(shared_addr(&tmem_slot), 512);
   if (threadIdx.x == 0) {
@@ -657,13 +707,12 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       barrier_init(shared_addr(full + k), 1);
       barrier_init(shared_addr(free_ + k), (Tr::kSplit ? 4 : 1) + (Tr::kOverRows && c.grad_bias ? Tr::kOutWarps : 0));
       barrier_init(shared_addr(ready + k), Tr::kSplit ? 4 : 1);
-      barrier_init(shared_addr(used + k), 1);
+      barrier_init(shared_addr(used + k), kJoins ? Tr::kTurns - 1 : 1);
     }
-    for (int k = 0; k < 2; ++k) barrier_init(shared_addr(acc_full + k), 1), barrier_init(shared_addr(acc_free + k), Tr::kOutWarps);
+    for (int k = 0; k < 2; ++k) barrier_init(shared_addr(acc_full + k), 1), barrier_init(shared_addr(acc_free + k), Tr::kOutWarps / Tr::kGangs), barrier_init(shared_addr(met + k), Tr::kOutWarps / Tr::kGangs);
     barrier_init(shared_addr(&kept_full), Tr::kSplit ? 8 : 1);
     barrier_init(shared_addr(&kept_free), 1);
     barrier_init(shared_addr(&drained), 1);
-    barrier_init(shared_addr(&met), Tr::kOutWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     gave_up_word = 0;
   }
@@ -868,9 +917,10 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     }
   } else if (warp >= 4 && (warp < 8 || !Tr::kSplit)) {
     // ---- finished tiles
-    const int quarter = warp % 4, turn = warp >= 8, thread = turn * 128 + threadIdx.x % 128;
-    constexpr int kTurns = Tr::kOutWarps / 4;
-    char* const mine = staging + (turn * 4 + quarter) * 4096;
+    constexpr int kTurns = Tr::kTurns;
+    const int quarter = warp % 4, gang = (warp - 4) / (4 * kTurns), turn = (warp - 4) / 4 % kTurns, thread = turn * 128 + threadIdx.x % 128;
+    char* const mine = staging + (warp - 4) * Tr::kStaging;
+    float* const bias = all_bias + gang * 256;
     int summed = 0;
     uint32_t summed_phase = 0;
     int bias_g = -1, bias_n = -1, buffer = kBuffers - 1;
@@ -882,18 +932,22 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if constexpr (MODE == kSumW) finish.by = factor;
     const auto meet = [&] {      // of the warps here; false: somebody has given up
       __syncwarp();
-      if (lane == 0) barrier_arrive(shared_addr(&met));
-      const bool all = __all_sync(0xffffffffu, barrier_wait(shared_addr(&met), meetings, gave_up, c.polls));
+      if (lane == 0) barrier_arrive(shared_addr(met + gang));
+      const bool all = __all_sync(0xffffffffu, barrier_wait(shared_addr(met + gang), meetings, gave_up, c.polls));
       meetings ^= 1;
       return all;
     };
     while (fine && walk.take(&item)) {
       const bool empty = item.stages == 0;
+      if (Tr::kGangs > 1 && c.halves == 1 && (buffer == kBuffers - 1 ? 0 : buffer + 1) != gang) {      // the other gang's
+        buffer = buffer == kBuffers - 1 ? 0 : buffer + 1;
+        continue;
+      }
       const int columns = min(c.tile_n, c.num_n - item.n0);
       if (Tr::kHasBias && c.bias && !empty && (item.g != bias_g || item.n0 != bias_n)) {
         bias_g = item.g, bias_n = item.n0;
         if (!(fine = meet())) break;      // the tile before is out
-        for (int k = thread; k < 256; k += Tr::kOutWarps * 32)
+        for (int k = thread; k < 256; k += kTurns * 128)
           bias[k] = bias_n + k < c.num_n ? Elem<T>::to_f(((const T*)c.bias)[(int64_t)bias_g * c.num_n + bias_n + k]) : 0.0f;
         if (!(fine = meet())) break;
       }
@@ -925,6 +979,12 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       }
       const int halves = !Tr::kOverRows && item.rows > c.tile_m ? 2 : 1;
       for (int half = 0; half < halves; ++half) {
+        if (Tr::kGangs > 1 && c.halves == 2 && half != gang) continue;
+        const int64_t row = item.row + half * kTileM + quarter * 32 + lane;      // (in out, dx and logits)
+        const bool there = row < item.row + item.rows;
+        int64_t label = -1;
+        if (MODE == kStats && there) label = c.loss.labels[row] - c.loss.class0 - item.n0;
+        if constexpr (MODE == kSlopes) finish = row_slopes(c.loss, row, there, item.n0);
         if (!empty) {
           buffer = c.halves == 2 ? half : buffer == kBuffers - 1 ? 0 : buffer + 1;
           fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_full + buffer), turns >> buffer & 1, gave_up, c.polls));
@@ -934,12 +994,26 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         const uint32_t acc = tmem + buffer * kAccColumns;
         if constexpr (MODE == kStats || MODE == kSumX) {
-          const int64_t row = item.row + half * kTileM + quarter * 32 + lane;
           const uint32_t sums = acc + ((uint32_t)quarter << 21);
           if constexpr (MODE == kStats) {
-            const int64_t label = row < item.row + item.rows ? c.loss.labels[row] - c.loss.class0 - item.n0 : -1;
-            tile_statistics<T, MODE>(sums, turn, kTurns, columns, c.bias ? bias : nullptr, label >= 0 && label < columns ? (int)label : -1, carry, item.before, item.after,
-                                     c.loss.parts + ((int64_t)(item.n0 / c.tile_n) * kTurns + turn) * c.loss.pitch + row, c.loss.picked + row, row < item.row + item.rows);
+            float2 s = tile_statistics<T, MODE>(sums, turn, kTurns, columns, c.bias ? bias : nullptr, label >= 0 && label < columns ? (int)label : -1, carry, item.before,
+                                                item.after, c.loss.picked + row);
+            if constexpr (kJoins) {
+              // the first of the warps that share the rows puts their statistics together. Their places are another tile's when this one's sums have been
+              // given back by all
+              float2* const place = (float2*)staging + (buffer * 4 + quarter) * (kTurns - 1) * 32 + lane;
+              const uint32_t bar = shared_addr(used + buffer * 4 + quarter);
+              if (turn) {
+                place[(turn - 1) * 32] = s;
+                __syncwarp();
+                if (lane == 0) barrier_arrive(bar);
+              } else {
+                if (!(fine = __all_sync(0xffffffffu, barrier_wait(bar, turns >> buffer & 1 ^ 1, gave_up, c.polls)))) break;
+#pragma unroll
+                for (int w = 0; w < kTurns - 1; ++w) join_statistics(&s, place[w * 32]);
+              }
+            }
+            if (turn == 0 && there && !(Tr::kCuts && item.after)) c.loss.parts[(int64_t)(item.n0 / c.tile_n) * c.loss.pitch + row] = s;
           } else {
             tile_to_slot<T, MODE>(sums, turn, kTurns, columns, c.carry + ((item.piece * c.halves + half) * 4 + quarter) * 32 * Tr::kMostN + lane * 4, c.loss.more || item.first);
           }
@@ -966,9 +1040,15 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           }
         }
         const int rows = item.rows - half * kTileM;
-        if constexpr (MODE == kSlopes) {
-          const int r = quarter * 32 + lane;
-          finish = row_slopes(c.loss, item.row + half * kTileM + r, r < min(rows, c.tile_m), item.n0);
+        if constexpr (MODE == kSlopes && !Tr::kSplit) {
+          const int mine_rows = min(rows, c.tile_m) - quarter * 32;
+          if (mine_rows > 0)
+            store_slopes<T, MODE>(acc + ((uint32_t)quarter << 21), mine, lane, turn, kTurns, (T*)c.out + (item.row + half * kTileM + quarter * 32) * c.loss.pitch + item.n0,
+                                  c.loss.pitch, mine_rows, columns, c.bias ? bias : nullptr, finish);
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) barrier_arrive(shared_addr(acc_free + buffer));
+          continue;
         }
         const bool stores = !Tr::kOverRows && quarter * 32 < min(rows, c.tile_m) && turn * (128 / (int)sizeof(T)) < columns;
         const int64_t ld = MODE == kSlopes ? c.loss.pitch : (int64_t)c.num_n;
@@ -1238,14 +1318,14 @@ static size_t carry_room(int64_t rows, int64_t dim, int64_t out_dim, bool backwa
 
 // Shared memory of the lists of groups, and of what lies in front of them.
 template <typename T, int MODE>
-static int grouped_lists(int groups) { return 1024 + (GroupedTraits<T, MODE>::kOverRows ? 2048 : 1024) + (int)align_up((size_t)(groups + 2) * 8, 16); }
+static int grouped_lists(int groups) { return 1024 + GroupedTraits<T, MODE>::kBiasFloats * 4 + (int)align_up((size_t)(groups + 2) * 8, 16); }
 
 // With what is kept, how many tiles share a stage and how deep it is: as many stages as there is room for.
 template <typename T, int MODE>
 static int run_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap& b, int64_t items, cudaStream_t s) {
   using Tr = GroupedTraits<T, MODE>;
   const int lists = grouped_lists<T, MODE>(c.groups);
-  const int room = kMostShared - lists - Tr::kOutWarps * 4096;
+  const int room = kMostShared - lists - Tr::kOutWarps * Tr::kStaging;
   int copied = Tr::kOverRows || Tr::kSplit ? Tr::copied(kTileM, Tr::kMnA) : c.tile_m * 128, pieces = Tr::kSplit ? 3 * Tr::piece(kTileM, Tr::kMnA) : 0;
   const int copied_b = Tr::copied(c.tile_n, Tr::kMnB), pieces_b = Tr::kSplit ? 3 * Tr::piece(c.tile_n, Tr::kMnB) : 0;
   const int kept = c.keep ? (int)(ceil_div(c.num_k, Tr::kBlock) * (Tr::kSplit ? pieces_b : copied_b)) : 0;
@@ -1255,7 +1335,7 @@ static int run_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap& b
   copied *= c.deep;
   c.piece_stages = Tr::kSplit ? 2 : 0;
   c.copied_stages = std::min(kMaxStages, (room - kept - c.piece_stages * pieces) / copied);
-  const int bytes = lists + Tr::kOutWarps * 4096 + kept + c.copied_stages * copied + c.piece_stages * pieces;
+  const int bytes = lists + Tr::kOutWarps * Tr::kStaging + kept + c.copied_stages * copied + c.piece_stages * pieces;
   static bool sized[64] = {};
   int dev = 0;
   APT_CUDA(cudaGetDevice(&dev));
@@ -1271,7 +1351,7 @@ static int run_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap& b
 template <typename T, int MODE>
 static int launch_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap& b, int64_t items, cudaStream_t s) {
   using Tr = GroupedTraits<T, MODE>;
-  const int room = kMostShared - grouped_lists<T, MODE>(c.groups) - Tr::kOutWarps * 4096;
+  const int room = kMostShared - grouped_lists<T, MODE>(c.groups) - Tr::kOutWarps * Tr::kStaging;
   const int copied = Tr::kOverRows || Tr::kSplit ? Tr::copied(kTileM, Tr::kMnA) : c.tile_m * 128, pieces = Tr::kSplit ? 3 * Tr::piece(kTileM, Tr::kMnA) : 0;
   const int copied_b = Tr::copied(c.tile_n, Tr::kMnB), pieces_b = Tr::kSplit ? 3 * Tr::piece(c.tile_n, Tr::kMnB) : 0;
   // Weights are kept where they leave room for four stages of rows and a block has several tiles of them: what the copies bring from L2, which

@@ -34,17 +34,6 @@ struct RowsCall {
   int32_t* status;
 };
 
-// Statistics of other columns of the same row.
-__device__ __forceinline__ void join_statistics(float2* a, float2 b) {
-  if (b.x == -INFINITY) {
-    a->y += b.y;      // nothing, or NaN
-  } else if (b.x > a->x) {
-    a->y = a->y * exp2_short(a->x - b.x) + b.y, a->x = b.x;
-  } else {
-    a->y += b.y * exp2_short(b.x - a->x);
-  }
-}
-
 // 32 rows a block, eight warps that have every eighth part.
 __global__ void __launch_bounds__(256) k_loss_rows(const __grid_constant__ RowsCall c) {
   wait_for_previous();
@@ -136,38 +125,51 @@ __global__ void __launch_bounds__(1024) k_loss_scale(const float* __restrict__ g
   }
 }
 
-// dx from its parts: 32 rows and 64 columns a block.
-template <typename T>
+// dx from its parts: 32 rows and 64 columns a block. WHOLE: rows are whole slices of 8 elements.
+template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256) k_loss_grad_rows(const __grid_constant__ GroupedCall c, T* out, int splits) {
   wait_for_previous();
   constexpr int kMostN = GroupedTraits<T, kSumX>::kMostN;
-  __shared__ float tile[32][65];
+  __shared__ float tile[32][68];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int64_t row0 = (int64_t)blockIdx.x * 32;
   const int col0 = blockIdx.y * 64;
   const float scale = c.loss.scale[1];
   const int tall = c.tile_m * c.halves;
-  // (tiles of fewer rows than 32 have their rows at the same lanes as taller ones)
   const int64_t row = row0 + lane;
   const int t = (int)(row / tall), in = (int)(row - (int64_t)t * tall), half = in / kTileM, quarter = in % kTileM / 32;
+  const int64_t apart = (int64_t)c.tiles_m * c.tiles_n * c.halves * kTileM * kMostN;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int col = col0 + (warp + 8 * u) * 4, n = col / c.tile_n;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (row < c.rows && col < c.num_n)
+    if (row < c.rows && col < c.num_n) {
+      const float* const from = c.carry + ((((int64_t)t * c.tiles_n + n) * c.halves + half) * 4 + quarter) * 32 * kMostN + (col - n * c.tile_n) * 32 + in % 32 * 4;
+#pragma unroll 4
       for (int s = 0; s < splits; ++s) {
-        const int64_t piece = ((int64_t)s * c.tiles_m + t) * c.tiles_n + n;
-        const float4 p = *(const float4*)(c.carry + ((piece * c.halves + half) * 4 + quarter) * 32 * kMostN + (col - n * c.tile_n) * 32 + in % 32 * 4);
+        const float4 p = *(const float4*)(from + s * apart);
         sum.x += p.x, sum.y += p.y, sum.z += p.z, sum.w += p.w;
       }
-    float* const to = &tile[lane][(warp + 8 * u) * 4];
-    to[0] = sum.x * scale, to[1] = sum.y * scale, to[2] = sum.z * scale, to[3] = sum.w * scale;
+    }
+    *(float4*)&tile[lane][(warp + 8 * u) * 4] = make_float4(sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 32 * 64; i += 256) {
-    const int64_t r = row0 + i / 64;
-    const int col = col0 + i % 64;
-    if (r < c.rows && col < c.num_n) out[r * c.num_n + col] = Elem<T>::from_f(tile[i / 64][i % 64]);
+  if constexpr (WHOLE) {
+    const int r = threadIdx.x / 8, col = threadIdx.x % 8 * 8;
+    if (row0 + r < c.rows && col0 + col < c.num_n) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = tile[r][col + q];
+      T* const to = out + (row0 + r) * c.num_n + col0 + col;
+      if constexpr (sizeof(T) == 2) *(uint4*)to = rounded_slice<T>(v);
+      else *(uint4*)to = rounded_slice<T>(v), *(uint4*)(to + 4) = rounded_slice<T>(v + 4);
+    }
+  } else {
+    for (int i = threadIdx.x; i < 32 * 64; i += 256) {
+      const int64_t r = row0 + i / 64;
+      const int col = col0 + i % 64;
+      if (r < c.rows && col < c.num_n) out[r * c.num_n + col] = Elem<T>::from_f(tile[i / 64][i % 64]);
+    }
   }
 }
 
@@ -219,11 +221,11 @@ static GroupedCall listed_call(int64_t rows, int64_t n, int64_t k) {
   if (Tr::kClasses)
     while (most > 64 && tiles_m * ceil_div(n, most) < kNumSMs) most /= 2;
   c.tile_n = tile_columns(n, (int)most), c.tiles_n = (int)ceil_div(n, c.tile_n);
-  const int room = kMostShared - grouped_lists<T, MODE>(1) - Tr::kOutWarps * 4096;
+  const int room = kMostShared - grouped_lists<T, MODE>(1) - Tr::kOutWarps * Tr::kStaging;
   const int copied = Tr::kSplit ? Tr::copied(kTileM, Tr::kMnA) : c.tile_m * 128, pieces = Tr::kSplit ? 3 * Tr::piece(kTileM, Tr::kMnA) : 0;
   const int copied_b = Tr::copied(c.tile_n, Tr::kMnB), pieces_b = Tr::kSplit ? 3 * Tr::piece(c.tile_n, Tr::kMnB) : 0;
   if (Tr::kClasses) {
-    const int64_t bytes = ceil_div(k, Tr::kBlock) * (Tr::kSplit ? pieces_b : copied_b), least = Tr::kSplit ? 2 * pieces + 3 * copied : 4 * copied;
+    const int64_t bytes = ceil_div(k, Tr::kBlock) * (Tr::kSplit ? pieces_b : copied_b), least = (Tr::kSplit ? 2 * pieces : 0) + 3 * copied;
     c.keep = bytes + least <= room && tiles_m >= 3 && tiles_m * c.tiles_n >= 3 * kNumSMs;
   }
   if (!Tr::kSplit && !c.keep) {
@@ -235,11 +237,12 @@ static GroupedCall listed_call(int64_t rows, int64_t n, int64_t k) {
   // a band's rows: a quarter of L2
   c.band = c.keep ? c.tiles_m : (int)std::max<int64_t>(1, std::min<int64_t>(tiles_m, (32ll << 20) / ((int64_t)c.tile_m * c.halves * k * (int64_t)sizeof(T))));
   if (MODE == kSumX) {
-    // Few tiles share the contraction among as many blocks as make the longest one's work least, with six stages' time for bringing a tile out.
-    const int64_t stages = ceil_div(k, Tr::kBlock * c.deep), tiles = tiles_m * c.tiles_n;
+    // Few tiles share the contraction among as many blocks as make it shortest: the longest one's stages, six stages' time for bringing a part
+    // out, and a part's way to memory and back (a stage's time for 256 KB).
+    const int64_t stages = ceil_div(k, Tr::kBlock * c.deep), tiles = tiles_m * c.tiles_n, bytes = (int64_t)c.halves * kTileM * c.tile_n * 4;
     int64_t best = 0, cost = 0;
     for (int64_t s = 1; s <= std::max<int64_t>(1, std::min(stages / 4, 4 * kNumSMs / tiles)); ++s) {
-      const int64_t here = ceil_div(tiles * s, kNumSMs) * (ceil_div(stages, s) + 6);
+      const int64_t here = ceil_div(tiles * s, kNumSMs) * (ceil_div(stages, s) + 6) + 2 * tiles * s * bytes / (1 << 20);
       if (!best || here < cost) best = s, cost = here;
     }
     c.split_stages = (int)ceil_div(stages, best), c.splits = (int)ceil_div(stages, c.split_stages);
@@ -284,15 +287,14 @@ static float* carry_of(Arena* a, int64_t terms) {
 template <typename T>
 static int loss_forward(const LossProblem& q, float* loss, float* saved, Arena* arena, bool run, cudaStream_t s) {
   using Tr = GroupedTraits<T, kStats>;
-  constexpr int kTurns = Tr::kOutWarps / 4;
   bool copy_x, copy_w;
   const Operand x = in_arena(arena, q.x, 0, q.rows, q.dim, sizeof(T), &copy_x), w = in_arena(arena, q.weight, 1, q.classes, q.dim, sizeof(T), &copy_w);
   const int64_t pitch = align_up(q.rows, 32), blocks = ceil_div(q.rows, 32);
   // (tiles of 64 columns at the least; in narrower ones than the widest there are few)
-  const int64_t piece = piece_of(q.classes, (double)pitch * 8 * kTurns / Tr::kMostN, kMostParts);
+  const int64_t piece = piece_of(q.classes, (double)pitch * 8 / Tr::kMostN, kMostParts);
   int64_t most_parts = 0;
   for (const int64_t n : {std::min(piece, q.classes), q.classes - (ceil_div(q.classes, piece) - 1) * piece})
-    most_parts = std::max<int64_t>(most_parts, listed_call<T, kStats>(q.rows, n, q.dim).tiles_n * (int64_t)kTurns);
+    most_parts = std::max<int64_t>(most_parts, listed_call<T, kStats>(q.rows, n, q.dim).tiles_n);
   float2* const parts = arena->take<float2>(most_parts * pitch);
   float* const picked = arena->take<float>(q.rows);
   float2* const sums = arena->take<float2>(blocks);
@@ -309,7 +311,7 @@ static int loss_forward(const LossProblem& q, float* loss, float* saved, Arena* 
     c.loss.labels = q.labels, c.loss.class0 = v0, c.loss.pitch = pitch, c.loss.parts = parts, c.loss.picked = picked;
     if (const int e = run_listed<T, kStats>(c, x, some_rows(w, v0, n, sizeof(T)), s)) return e;
     RowsCall r = {};
-    r.parts = parts, r.num_parts = c.tiles_n * kTurns, r.pitch = pitch, r.stats = (float2*)saved, r.picked = picked, r.labels = q.labels;
+    r.parts = parts, r.num_parts = c.tiles_n, r.pitch = pitch, r.stats = (float2*)saved, r.picked = picked, r.labels = q.labels;
     r.rows = q.rows, r.classes = q.classes, r.ignore = q.ignore, r.first = v0 == 0, r.last = v0 + n == q.classes;
     r.losses = q.reduction == APT_LOSS_NONE ? loss : nullptr, r.sums = sums, r.status = q.status;
     APT_FOLLOW(k_loss_rows, blocks, 256, 0, s, r);
@@ -383,7 +385,8 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
   if (grad_x) {
     sum_x.loss.scale = scale;
     const dim3 grid((unsigned)ceil_div(q.rows, 32), (unsigned)ceil_div(q.dim, 64));
-    APT_FOLLOW((k_loss_grad_rows<T>), grid, 256, 0, s, sum_x, (T*)grad_x, splits);
+    if (q.dim % 8 == 0) APT_FOLLOW((k_loss_grad_rows<T, true>), grid, 256, 0, s, sum_x, (T*)grad_x, splits);
+    else APT_FOLLOW((k_loss_grad_rows<T, false>), grid, 256, 0, s, sum_x, (T*)grad_x, splits);
   }
   return APT_OK;
 }

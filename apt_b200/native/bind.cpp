@@ -602,6 +602,7 @@ struct RouteFunction : public torch::autograd::Function<RouteFunction> {
     auto [chosen, weights] = route_forward(logits, given(bias), {k, score, groups, top_groups, best, renormalize, scale});
     ctx->save_for_backward({logits, chosen});
     ctx->mark_non_differentiable({chosen});
+    ctx->set_materialize_grads(false);
     ctx->saved_data["score"] = score;
     ctx->saved_data["renormalize"] = renormalize;
     ctx->saved_data["scale"] = scale;
@@ -610,6 +611,7 @@ struct RouteFunction : public torch::autograd::Function<RouteFunction> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto v = ctx->get_saved_variables();
     torch::autograd::variable_list r(9);
+    if (!grads[1].defined()) return r;
     r[0] = route_backward(v[0], v[1], grads[1], ctx->saved_data["score"].toInt(), ctx->saved_data["renormalize"].toBool(), ctx->saved_data["scale"].toDouble());
     return only_once("route_experts", std::move(r), v[0], Tensor(), Tensor(), grads[1]);
   }
@@ -686,11 +688,13 @@ struct ExpertRowsFunction : public torch::autograd::Function<ExpertRowsFunction>
     auto [rows, offsets, place] = expert_rows(x, experts, num_experts, words);
     ctx->save_for_backward({place});
     ctx->mark_non_differentiable({offsets, place});
+    ctx->set_materialize_grads(false);
     ctx->saved_data["words"] = words;
     return {rows, offsets, place};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto v = ctx->get_saved_variables();
+    if (!grads[0].defined()) return torch::autograd::variable_list(4);
     Tensor gx = expert_sum("expert_rows_backward", grads[0], "grad_rows", Tensor(), v[0], ctx->saved_data["words"].toTensor());
     return only_once("expert_rows", {gx, Tensor(), Tensor(), Tensor()}, grads[0], Tensor(), Tensor(), grads[0]);
   }

@@ -60,7 +60,7 @@ struct GroupedTraits {
   static constexpr int kOutWarps = kSplit ? 4 : kClasses ? 16 : 8, kGangs = kClasses && !kSplit ? 2 : 1, kTurns = kOutWarps / kGangs / 4;
   static constexpr int kThreads = kSplit ? 512 : 128 + 32 * kOutWarps;
   // shared memory of one of those warps, in which 32 rows lie on their way out (or their statistics on the way to the warp that joins them)
-  static constexpr int kStaging = MODE == kStats ? (kTurns - 1) * 32 * 8 : MODE == kSumX ? 0 : MODE == kSlopes && !kSplit ? 2048 : 4096;
+  static constexpr int kStaging = MODE == kStats ? 2 * 4 * (kTurns - 1) * 32 * 8 / kOutWarps : MODE == kSumX ? 0 : MODE == kSlopes && !kSplit ? 2048 : 4096;
   static constexpr int kBiasFloats = kOverRows ? 512 : 256 * kGangs;
   // a sum in tensor memory has so many stages at most: 1024 terms of fp32, 8192 rows of 16 bits (with 4096, 65536 x 1024 -> 1024 bf16, dw and db 182 -> 205 us:
   // the warps that bring parts out are those that add up db, for which the stages wait)
@@ -837,6 +837,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                                         : tile_descriptor(start_b, 16, Tr::kBlock * 16, Tr::kSplit ? kSwizzle64 : kSwizzle128);
       int stage = 0, kept_g = -1, kept_n = -1, kept_times = 0, buffer = kBuffers - 1;
       uint32_t phase = 0, mended = 0, turns = 0;      // turns: parity of each buffer's uses
+      bool there = false;                             // the stage, as far as is known
       while (fine && walk.take(&item)) {
         if (!item.stages) continue;
         const int halves = !Tr::kOverRows && item.rows > c.tile_m ? 2 : 1;
@@ -852,7 +853,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         const uint32_t acc = tmem + buffer * kAccColumns;
         for (int k = 0; k < item.stages; ++k) {
-          if (!(fine = barrier_wait(shared_addr((Tr::kSplit ? ready : full) + stage), phase, gave_up, c.polls))) break;
+          if (!((!Tr::kSplit && there) || (fine = barrier_wait(shared_addr((Tr::kSplit ? ready : full) + stage), phase, gave_up, c.polls)))) break;
           const int left = Tr::kOverRows ? item.rows - k * Tr::kBlock : c.num_k - (item.before + k) * Tr::kBlock * c.deep, steps = (min(left, Tr::kBlock * c.deep) + 15) / 16;
           if (kMends && left < Tr::kBlock && left % 16) {
             barrier_arrive(shared_addr(ready));
@@ -861,10 +862,10 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           }
           tmem_fence_after();
           const uint64_t tile_a = first_a + (uint32_t)stage * stage_units, tile_b = keep ? first_b + (uint32_t)k * (uint32_t)(kept_bytes >> 4) : first_b + (uint32_t)stage * stage_units;
-          const auto step = [&](uint64_t tile_a, uint64_t tile_b, int s, bool add) {
+          const auto step = [&](auto two, uint64_t tile_a, uint64_t tile_b, int s, bool add) {
             const uint64_t da = tile_a + s * ((Tr::kMnA ? 2048 : 32) >> 4), db = tile_b + s * ((Tr::kMnB ? 2048 : 32) >> 4);
             tile_product(acc, da, db, what, add);
-            if (!Tr::kSplit && !Tr::kOverRows && halves == 2) tile_product(acc + kAccColumns, da + (kTileM * 128 >> 4), db, what, add);
+            if constexpr (decltype(two)::value) tile_product(acc + kAccColumns, da + (kTileM * 128 >> 4), db, what, add);
             if constexpr (Tr::kSplit) {
               const uint64_t pa = piece_a >> 4, pb = piece_b >> 4;
               const uint32_t small = acc + Tr::kMostN;
@@ -875,16 +876,28 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               tile_product(small, da + 2 * pa, db, what, true);
             }
           };
-          constexpr int kSteps = Tr::kBlock / 16;
-          for (int l = 0; l < (Tr::kSplit || Tr::kOverRows ? 1 : c.deep) && l * kSteps < steps; ++l) {
-            const uint64_t at_a = tile_a + (uint32_t)l * (uint32_t)(block_bytes >> 4), at_b = tile_b + (uint32_t)l * (uint32_t)(block_bytes >> 4);
-            if (steps >= (l + 1) * kSteps) {
-#pragma unroll
-              for (int s = 0; s < kSteps; ++s) step(at_a, at_b, s, k > 0 || l > 0 || s > 0);
-            } else {
-              for (int s = 0; s < steps - l * kSteps; ++s) step(at_a, at_b, s, k > 0 || l > 0 || s > 0);
-            }
+          // whether the next stage is there is asked in front of this one's products: the answer takes 130 cycles
+          // (fp32's six products a step hide it)
+          if constexpr (!Tr::kSplit) {
+            const bool wraps = stage + 1 == stages;
+            there = barrier_is_over(shared_addr(full + (wraps ? 0 : stage + 1)), phase ^ (uint32_t)wraps);
           }
+          // Nothing is asked between the products of a block: with a branch behind each they had their operands in one set of uniform registers, and
+          // every product waited for the one before to have read it (211 cycles for 128 x 256 x 16, not 128).
+          const auto products = [&](auto two) {
+            constexpr int kSteps = Tr::kBlock / 16;
+            for (int l = 0; l < (Tr::kSplit || Tr::kOverRows ? 1 : c.deep) && l * kSteps < steps; ++l) {
+              const uint64_t at_a = tile_a + (uint32_t)l * (uint32_t)(block_bytes >> 4), at_b = tile_b + (uint32_t)l * (uint32_t)(block_bytes >> 4);
+              if (steps >= (l + 1) * kSteps) {
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) step(two, at_a, at_b, s, k > 0 || l > 0 || s > 0);
+              } else {
+                for (int s = 0; s < steps - l * kSteps; ++s) step(two, at_a, at_b, s, k > 0 || l > 0 || s > 0);
+              }
+            }
+          };
+          if (!Tr::kSplit && !Tr::kOverRows && halves == 2) products(std::true_type{});
+          else products(std::false_type{});
           products_done(shared_addr((Tr::kSplit ? used : free_) + stage));
           if (k == item.stages - 1) {
             products_done(shared_addr(acc_full + buffer));

@@ -7,18 +7,24 @@
 //   backward, g = scale dL/dw:  s_e (g_e - sum_j g_j s_j) for softmax (g_e = 0 where e is not chosen), g_e s_e (1 - s_e) for the logistic;
 //   divided by the sum, p = w / scale:  p_e (g_e - sum_j g_j p_j), times (1 - s_e) for the logistic; 0 where e is not chosen
 //
-// A team of lanes has a row, NV neighbouring experts a lane, in registers; lanes and slots ascend with the experts, so that of equal
-// values the first lane's first slot is the lowest. k rounds take the largest key each. An expert whose logit is -inf is never chosen:
-// where fewer are left than k, the others are -1 with weight 0.
+// A team of lanes has a row, NV neighbouring experts a lane, in registers; lanes and slots ascend with the experts. The k-th largest of the
+// lanes' own largest is a bound below which nothing is chosen: what is not below it (of rows over 256 experts some ten) goes to shared memory, where
+// every candidate finds its place by counting those in front of it. An expert whose logit is -inf is never chosen: where fewer are left than k, the
+// others are -1 with weight 0.
 //
-// Ranks are those of the exact scores. Without a bias logits are compared as they are. Scores in 32 bits are off by less than 2^-18 of the
-// row's largest (the argument's rounding, exp, the sum, the quotient: 1e-6) and their sum with the bias by 2^-23 of itself: where two that were
-// taken one behind the other, or the last one and the next, are nearer than twice that, the row is done again in 64 bits.
+// Ranks are those of the exact scores. Without a bias logits are compared as they are. Scores in 32 bits are off by less than 2^-19 of the
+// row's largest: the argument's rounding, 2^-23 of |z| exp(-|z|), exp, reciprocal and quotient by two units in the last place each, a sum of 1024 in ten
+// steps and eight. Their sum with the bias is off by 2^-24 of itself. Where two that were taken one behind the other, or the last one and the
+// next, are nearer than both errors, the row is done again in 64 bits, by a warp for itself (route_again); of rows over 256 experts one in a
+// hundred.
+//
+#include <algorithm>
+
 #include "dense.cuh"
 
 namespace apt {
 
-constexpr int kRouteThreads = 128;
+constexpr int kRouteThreads = 128, kRouteFound = 64;
 
 struct RouteCall {
   const void* logits;
@@ -26,7 +32,9 @@ struct RouteCall {
   int64_t rows;
   int experts, k, groups, per, top_groups, best;      // per: experts of a group
   int group_lanes, team_lanes;                        // logarithms
-  int sigmoid, renorm, whole;                         // whole: a lane's experts are there, all or none, and may be read in slices
+  int sigmoid, renorm;
+  int whole;                                          // a lane's experts are there, all or none, and may be read in slices
+  int found;                                          // places for candidates
   float scale;
   int64_t* chosen;
   float* weights;
@@ -34,32 +42,28 @@ struct RouteCall {
   void* grad_logits;
 };
 
-// Numbers as unsigned ones of the same order; 0: not to be had.
+// Numbers as unsigned ones of the same order; 0: not to be had. NaN is above all others.
 __device__ __forceinline__ uint32_t rank_of(float v) {
   const uint32_t u = __float_as_uint(v + 0.0f);      // -0 is 0
-  return v != v ? 0xffffffffu : v == -INFINITY ? 0u : u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
-}
-__device__ __forceinline__ uint64_t rank_of(double v) {
-  const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
-  return v != v ? ~0ull : v == -INFINITY ? 0ull : u ^ ((int64_t)u < 0 ? ~0ull : 1ull << 63);
+  return v != v ? 0xffffffffu : v == -INFINITY ? 0u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float number_of(uint32_t r) { return __uint_as_float(r ^ (r >> 31 ? 0x80000000u : 0xffffffffu)); }
-template <typename F> struct RankOf { using type = uint32_t; };
-template <> struct RankOf<double> { using type = unsigned long long; };
 
-template <typename V>
-__device__ __forceinline__ V team_max(V v, int lanes) {
-  for (int o = 0; o < lanes; ++o) {
-    const V w = __shfl_xor_sync(0xffffffffu, v, 1 << o);
-    v = v < w ? w : v;
-  }
-  return v;
-}
 template <typename V>
 __device__ __forceinline__ V team_sum(V v, int lanes) {
   for (int o = 0; o < lanes; ++o) v += __shfl_xor_sync(0xffffffffu, v, 1 << o);
   return v;
 }
+__device__ __forceinline__ float team_most(float v, int lanes) {
+  for (int o = 0; o < lanes; ++o) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1 << o));
+  return v;
+}
+__device__ __forceinline__ uint32_t team_most(uint32_t v, int lanes) {
+  if (lanes == 5) return __reduce_max_sync(0xffffffffu, v);
+  for (int o = 0; o < lanes; ++o) v = max(v, __shfl_xor_sync(0xffffffffu, v, 1 << o));
+  return v;
+}
+__device__ __forceinline__ uint32_t team_least(uint32_t v, int lanes) { return ~team_most(~v, lanes); }
 
 struct Team {
   int lane, first, lanes;      // within the team, the team's first in the warp, logarithm of their number
@@ -69,82 +73,102 @@ struct Team {
   }
 };
 
+// exp(z), off by two units in the last place and |z| more for its rounded argument; quotients: two units.
+__device__ __forceinline__ float exp_short(float z) { return exp2_short(1.4426950408889634f * z); }
 // log(1 / (1 + exp(-z)))
 __device__ __forceinline__ float log_logistic(float z) { return fminf(z, 0.0f) - log1pf(expf(-fabsf(z))); }
+__device__ __forceinline__ bool too_near(float a, float b, float slack) { return !(a - b >= slack + 0x1p-22f * fabsf(a)); }
 
-// The rounds. c: what experts are ranked by, v: what groups are by. Leaves the team's picks; true where two values were too near one another for 32
-// bits: `slack`, and a share of the values themselves. (v is looked at closely only where two of them are added up.)
-template <typename F, int NV>
-__device__ __forceinline__ bool choose(const RouteCall& r, const Team& team, const F (&c)[NV], const F (&v)[NV], F slack, int* picks, bool write) {
-  using K = typename RankOf<F>::type;
-  constexpr bool kShort = sizeof(F) == 4;
-  const int group = team.lane >> r.group_lanes, base = group * r.per + (team.lane & ((1 << r.group_lanes) - 1)) * NV;
-  const auto too_near = [](F a, F b, F slack) { return !(a - b >= slack + (F)0x1p-22 * (a < 0 ? -a : a)); };
-  bool near = false, kept = true;
-  if (r.groups > 1) {
-    K one = 0, two = 0;
-    F first = 0, second = 0;
+// Whether the lane's group is one of those that stay: of all groups' values, the same in all lanes of a group. near: the last that stays and the
+// first that does not are too near one another for 32 bits.
+template <int NV>
+__device__ __forceinline__ bool group_stays(const RouteCall& r, const Team& team, const float (&v)[NV], float slack, bool* near) {
+  const int group = team.lane >> r.group_lanes;
+  uint32_t one = 0, two = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const K k = rank_of(v[i]);
-      if (k > one) two = one, second = first, one = k, first = v[i];
-      else if (k > two) two = k, second = v[i];
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t k = rank_of(v[i]);
+    two = max(two, min(one, k)), one = max(one, k);
+  }
+  for (int o = 0; o < r.group_lanes; ++o) {
+    const uint32_t a = __shfl_xor_sync(0xffffffffu, one, 1 << o), b = __shfl_xor_sync(0xffffffffu, two, 1 << o);
+    two = max(min(one, a), max(two, b)), one = max(one, a);
+  }
+  const uint32_t key = group >= r.groups ? 0 : r.best == 2 && two ? rank_of(number_of(one) + number_of(two)) : one;
+  int above = 0;
+  for (int g = 0; g < r.groups; ++g) {
+    const uint32_t other = __shfl_sync(0xffffffffu, key, team.first + (g << r.group_lanes));
+    above += other > key || (other == key && g < group);
+  }
+  const bool stays = above < r.top_groups;
+  if (r.best == 2) {
+    const uint32_t last = team_least(stays && group < r.groups ? key : 0xffffffffu, r.team_lanes), next = team_most(stays ? 0u : key, r.team_lanes);
+    *near = next && too_near(number_of(last), number_of(next), 2.0f * slack);
+  }
+  return stays;
+}
+
+// The largest keys, largest first and of equal ones the lowest expert's, to best[0 .. wanted): (key, complement of the expert), 0 where there is none.
+// False: very many that are equal, or more wanted than there are lanes, and so more candidates than there are places.
+template <int NV>
+__device__ __forceinline__ bool take_best(const RouteCall& r, const Team& team, uint32_t (&key)[NV], uint64_t* found, uint64_t* best, int wanted) {
+  const int base = (team.lane >> r.group_lanes) * r.per + (team.lane & ((1 << r.group_lanes) - 1)) * NV, lanes = 1 << r.team_lanes;
+  const auto entry = [&](int i) { return (uint64_t)key[i] << 32 | (uint32_t)~(base + i); };
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) mine = max(mine, key[i]);
+  uint32_t bound = 0;
+  if (r.team_lanes == 5) {      // (equal ones go together: the bound is lower then, and holds as well)
+    for (int j = 0; j < wanted; ++j) {
+      bound = __reduce_max_sync(0xffffffffu, mine);
+      if (mine == bound) mine = 0;
     }
-    for (int o = 0; o < r.group_lanes; ++o) {
-      const K a = __shfl_xor_sync(0xffffffffu, one, 1 << o), b = __shfl_xor_sync(0xffffffffu, two, 1 << o);
-      const F x = __shfl_xor_sync(0xffffffffu, first, 1 << o), y = __shfl_xor_sync(0xffffffffu, second, 1 << o);
-      if (a > one) {
-        const bool mine = one > b;
-        two = mine ? one : b, second = mine ? first : y, one = a, first = x;
-      } else if (a > two) {
-        two = a, second = x;
+  } else if (wanted <= lanes) {
+    int above = 0;
+    for (int l = 0; l < lanes; ++l) {
+      const uint32_t other = __shfl_sync(0xffffffffu, mine, team.first + l);
+      above += other > mine || (other == mine && l < team.lane);
+    }
+    bound = __shfl_sync(0xffffffffu, mine, team.first + __ffs(team.votes(above == wanted - 1)) - 1);
+  }
+  bound = max(bound, 1u);
+  // where a lane's candidates go: the lanes' numbers of them, bit by bit
+  uint32_t which = 0;
+#pragma unroll
+  for (int i = 0; i < NV && i < 32; ++i) which |= (uint32_t)(key[i] >= bound) << i;
+  int own = __popc(which);
+  if constexpr (NV > 32) {
+#pragma unroll
+    for (int i = 32; i < NV; ++i) own += key[i] >= bound;
+  }
+  int at = 0, count = 0;
+  constexpr int kBits = NV == 8 ? 4 : NV == 16 ? 5 : NV == 32 ? 6 : 7;
+#pragma unroll
+  for (int b = 0; b < kBits; ++b) {
+    const unsigned all = team.votes(own >> b & 1);
+    at += __popc(all & ((1u << team.lane) - 1)) << b, count += __popc(all) << b;
+  }
+  if (own && count <= kRouteFound) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (key[i] >= bound) found[at++] = entry(i);
+  }
+  for (int j = team.lane; j < wanted; j += lanes) best[j] = 0;
+  if (team.lane == 0 && count <= kRouteFound) found[count] = 0;      // two are read at once
+  __syncwarp();
+  if (count <= kRouteFound) {
+    for (int p = team.lane; p < count; p += lanes) {
+      const uint64_t me = found[p];
+      int place = 0;
+      for (int q = 0; q < count; q += 2) {
+        const ulonglong2 two = *(const ulonglong2*)(found + q);
+        place += (two.x > me) + (two.y > me);
       }
-    }
-    const F value = r.best == 2 && two ? first + second : first;
-    K key = group < r.groups && one ? rank_of(value) : 0;
-    F last = 0;
-    kept = false;
-    for (int t = 0; t < r.top_groups; ++t) {
-      const K top = team_max(key, r.team_lanes);
-      const unsigned who = team.votes(key == top && top);
-      const int owner = who ? __ffs(who) - 1 : 0;
-      last = __shfl_sync(0xffffffffu, value, team.first + owner);
-      if (who && owner >> r.group_lanes == group) kept = true, key = 0;
-    }
-    if (kShort && r.best == 2) {
-      const K top = team_max(key, r.team_lanes);
-      const unsigned who = team.votes(key == top && top);
-      const F next = __shfl_sync(0xffffffffu, value, team.first + (who ? __ffs(who) - 1 : 0));
-      near = who && too_near(last, next, 2 * slack);
+      if (place < wanted) best[place] = me;
     }
   }
-  K key[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) key[i] = kept ? rank_of(c[i]) : 0;
-  F last = 0;
-  const int rounds = r.k + (kShort && r.bias ? 1 : 0);      // one more for what the last pick is compared with
-  for (int j = 0; j < rounds; ++j) {
-    K best = 0;
-    int slot = 0;
-    F value = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (key[i] > best) best = key[i], slot = i, value = c[i];
-    const K top = team_max(best, r.team_lanes);
-    const unsigned who = team.votes(best == top && top);
-    const int owner = who ? __ffs(who) - 1 : 0;
-    const int expert = __shfl_sync(0xffffffffu, base + slot, team.first + owner);
-    if (kShort && r.bias) {
-      value = __shfl_sync(0xffffffffu, value, team.first + owner);
-      if (j && who) near |= too_near(last, value, slack);
-      last = value;
-    }
-    if (j < r.k && write && team.lane == 0) picks[j] = who ? expert : -1;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (who && team.lane == owner && i == slot) key[i] = 0;
-  }
-  return near;
+  __syncwarp();
+  return count <= kRouteFound;
 }
 
 // The logits of a lane's experts; -inf for those that are not there.
@@ -178,207 +202,324 @@ __device__ __forceinline__ void row_softmax(const float (&z)[NV], int lanes, flo
   m = m == -INFINITY ? 0.0f : m;
   float s = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) s += expf(z[i] - m);
+  for (int i = 0; i < NV; ++i) s += exp_short(z[i] - m);
   *top = m, *sum = team_sum(s, lanes);
 }
 
-template <typename T, int NV>
+// A row's picks in 64 bits, by a warp: what experts are ranked by lies in shared memory, 32 neighbours at a time. Nothing is unrolled: few rows come
+// here, and the instructions would be in every row's way.
+template <typename T>
+__device__ __noinline__ void route_again(const RouteCall& r, const T* row, double* c, uint64_t* picks) {
+  const int lane = threadIdx.x % 32;
+  const bool scores = r.bias || r.groups > 1;
+  double total = 1.0, top = 0.0;
+  if (!r.sigmoid && scores) {
+    float m = -INFINITY;
+    for (int e = lane; e < r.experts; e += 32) m = fmaxf(m, Elem<T>::to_f(row[e]));
+    m = team_most(m, 5);
+    top = m == -INFINITY ? 0.0 : (double)m, total = 0.0;
+    for (int e = lane; e < r.experts; e += 32) total += exp((double)Elem<T>::to_f(row[e]) - top);
+    total = team_sum(total, 5);
+  }
+  for (int e = lane; e < r.experts; e += 32) {
+    const double z = (double)Elem<T>::to_f(row[e]);
+    double v = z;
+    if (scores && z != -INFINITY && (r.bias || r.best == 2)) {
+      v = r.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - top) / total;
+      if (r.bias) v += r.bias[e];
+    }
+    c[e] = v;
+  }
+  __syncwarp();
+  // (a, its place) is in front of (b, its place)
+  const auto before = [](double a, int i, double b, int j) { return b != b ? a != a && i < j : a != a || a > b || (a == b && i < j); };
+  if (r.groups > 1) {
+    double value = -INFINITY;
+    if (lane < r.groups) {
+      double second = -INFINITY;
+      for (int e = lane * r.per; e < (lane + 1) * r.per; ++e) {
+        const double v = c[e];
+        if (before(v, 0, value, 1)) second = value, value = v;
+        else if (before(v, 0, second, 1)) second = v;
+      }
+      if (r.best == 2 && second != -INFINITY) value += second;
+    }
+    int above = 0;
+    for (int g = 0; g < r.groups; ++g) above += before(__shfl_sync(0xffffffffu, value, g), g, value, lane);
+    const unsigned stay = __ballot_sync(0xffffffffu, lane < r.groups && above < r.top_groups);
+    for (int e = lane; e < r.experts; e += 32) c[e] = !(stay >> e / r.per & 1) ? -INFINITY : r.bias ? c[e] : (double)Elem<T>::to_f(row[e]);
+    __syncwarp();
+  }
+  for (int j = 0; j < r.k; ++j) {
+    double best = -INFINITY;
+    int at = r.experts;
+    for (int e = lane; e < r.experts; e += 32)
+      if (c[e] != -INFINITY && before(c[e], e, best, at)) best = c[e], at = e;
+#pragma unroll 1
+    for (int o = 16; o; o >>= 1) {
+      const double b = __shfl_xor_sync(0xffffffffu, best, o);
+      const int i = __shfl_xor_sync(0xffffffffu, at, o);
+      if (i < r.experts && (at == r.experts || before(b, i, best, at))) best = b, at = i;
+    }
+    if (lane == 0) {
+      picks[j] = at < r.experts ? (uint64_t)rank_of(Elem<T>::to_f(row[at])) << 32 | (uint32_t)~at : 0;
+      if (at < r.experts) c[at] = -INFINITY;
+    }
+    __syncwarp();
+  }
+}
+
+// Renormalised weights of a row whose chosen scores are all next to nothing in 32 bits, by their logarithms. One thread.
+template <typename T>
+__device__ __noinline__ void weights_by_logarithms(const RouteCall& r, const T* row, const uint64_t* best, float* to) {
+  const auto value = [&](int j) {
+    const float v = Elem<T>::to_f(row[~(uint32_t)best[j]]);
+    return r.sigmoid ? log_logistic(v) : v;
+  };
+  float m = -INFINITY, total = 0.0f;
+  for (int j = 0; j < r.k && best[j]; ++j) m = fmaxf(m, value(j));
+  for (int j = 0; j < r.k && best[j]; ++j) total += expf(value(j) - m);
+  for (int j = 0; j < r.k; ++j) to[j] = best[j] ? r.scale * (expf(value(j) - m) / total) : 0.0f;
+}
+
+// 67584 rows over 256 experts in eight groups, logistic with a bias, fp32: 104 us (reading 69 MB: 11), without groups and bias 42; 151552 over 64, softmax,
+// bf16: 39 (6). Instructions bound it, 80 per cent of the issue slots: 1230 a row of the first, 560 of the second. EXACT: ranks are those of scores, not of
+// the logits.
+template <typename T, int NV, bool GROUPS, bool EXACT>
 __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__ RouteCall r) {
   wait_for_previous();
-  extern __shared__ int picks_of_all[];
+  extern __shared__ __align__(16) uint64_t room[];
   Team team;
   team.lanes = r.team_lanes, team.lane = threadIdx.x & ((1 << r.team_lanes) - 1), team.first = (threadIdx.x & 31) - team.lane;
-  const int number = threadIdx.x >> r.team_lanes;
-  const int64_t row = (int64_t)blockIdx.x * (kRouteThreads >> r.team_lanes) + number;
+  const int number = threadIdx.x >> r.team_lanes, teams = kRouteThreads >> r.team_lanes, lanes = 1 << r.team_lanes;
+  const int64_t row = (int64_t)blockIdx.x * teams + number;
   const bool alive = row < r.rows;
-  int* const picks = picks_of_all + number * r.k;
+  // candidates and the best of them of all teams, and a row in 64 bits a warp
+  uint64_t *const found = room + number * r.found, *const best = room + teams * r.found + number * (r.k + 1);
   const T* const from = (const T*)r.logits + (alive ? row : 0) * r.experts;
-  const int group = team.lane >> r.group_lanes, base = group * r.per + (team.lane & ((1 << r.group_lanes) - 1)) * NV;
+  const int group = GROUPS ? team.lane >> r.group_lanes : 0, base = GROUPS ? group * r.per + (team.lane & ((1 << r.group_lanes) - 1)) * NV : team.lane * NV;
   const int end = alive && group < r.groups ? (group + 1) * r.per : 0;
 
   float z[NV], top = 0.0f, sum = 1.0f;
   load_logits<T, NV>(from, base, end, r.whole, z);
-  if (!r.sigmoid && (r.bias || !r.renorm || (r.groups > 1 && r.best == 2))) row_softmax(z, r.team_lanes, &top, &sum);
-  bool near;
-  if (r.bias || (r.groups > 1 && r.best == 2)) {
-    float s[NV], c[NV];
+  if (!r.sigmoid && (EXACT || !r.renorm)) row_softmax(z, r.team_lanes, &top, &sum);
+  uint32_t key[NV];
+  bool again = false, stays = true;
+  float slack = 0.0f;
+  if constexpr (EXACT) {
+    float s[NV];
+    const float by = r.sigmoid ? 1.0f : 1.0f / sum;      // the largest score there can be
+    slack = 0x1p-18f * by;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const bool there = z[i] != -INFINITY;
-      s[i] = there ? (r.sigmoid ? 1.0f / (1.0f + expf(-z[i])) : expf(z[i] - top) / sum) : -INFINITY;
+      s[i] = there ? (r.sigmoid ? logistic(z[i]) : exp_short(z[i] - top) * by) : -INFINITY;
       if (r.bias && there) s[i] += r.bias[base + i];
-      c[i] = r.bias ? s[i] : z[i];
     }
-    // no score is larger than one, and none of a softmax than that of the largest logit
-    near = choose<float, NV>(r, team, c, s, 0x1p-17f * (r.sigmoid ? 1.0f : 1.0f / sum), picks, true);
+    if constexpr (GROUPS) stays = group_stays<NV>(r, team, s, slack, &again);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) key[i] = stays ? rank_of(r.bias ? s[i] : z[i]) : 0;
   } else {
-    near = choose<float, NV>(r, team, z, z, 0.0f, picks, true);
-  }
-  if (__any_sync(0xffffffffu, near)) {
-    double s[NV], c[NV], total = 1.0;
-    if (!r.sigmoid) {
-      total = 0.0;
+    if constexpr (GROUPS) stays = group_stays<NV>(r, team, z, 0.0f, &again);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) total += exp((double)z[i] - top);
-      total = team_sum(total, r.team_lanes);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const bool there = z[i] != -INFINITY;
-      s[i] = there ? (r.sigmoid ? 1.0 / (1.0 + exp(-(double)z[i])) : exp((double)z[i] - top) / total) : -INFINITY;
-      if (r.bias && there) s[i] += r.bias[base + i];
-      c[i] = r.bias ? s[i] : (double)z[i];
-    }
-    choose<double, NV>(r, team, c, s, 0.0, picks, near);
+    for (int i = 0; i < NV; ++i) key[i] = stays ? rank_of(z[i]) : 0;
   }
+  // (one more for what the last one is compared with)
+  again |= !take_best<NV>(r, team, key, found, best, r.k + (EXACT ? 1 : 0));
+  if (EXACT && r.bias)
+    for (int j = team.lane; j < r.k; j += lanes) {
+      const uint32_t mine = (uint32_t)(best[j] >> 32), next = (uint32_t)(best[j + 1] >> 32);
+      again |= next && too_near(number_of(mine), number_of(next), slack);
+    }
+  const unsigned who = __ballot_sync(0xffffffffu, again && alive);
+  if (who)
+    for (int first = 0; first < 32; first += lanes)
+      if (who >> first & (lanes == 32 ? ~0u : (1u << lanes) - 1)) {
+        const int n = (threadIdx.x / 32 * 32 + first) >> r.team_lanes;
+        route_again<T>(r, (const T*)r.logits + ((int64_t)blockIdx.x * teams + n) * r.experts, (double*)(room + teams * (r.found + r.k + 1)) + threadIdx.x / 32 * r.experts,
+                       room + teams * r.found + n * (r.k + 1));
+      }
   __syncwarp();
 
-  // weights: of the picks' own logits, so that a sum of scores that are all too small for 32 bits is none of zero
-  float m = -INFINITY, total = 0.0f;
-  const int lanes = 1 << r.team_lanes;
-  const auto logit = [&](int e) { return e >= 0 ? Elem<T>::to_f(from[e]) : -INFINITY; };
+  // Weights: of the picks' own logits, which without a bias are what they were ranked by, the first the largest of them.
+  const auto logit = [&](uint64_t pick) { return r.bias ? Elem<T>::to_f(from[~(uint32_t)pick]) : number_of((uint32_t)(pick >> 32)); };
+  const float m = r.bias || !r.renorm ? top : best[0] ? logit(best[0]) : 0.0f;
+  const auto score = [&](uint64_t pick) { return !pick ? 0.0f : r.sigmoid ? logistic(logit(pick)) : exp_short(logit(pick) - m); };
+  float total = sum;
   if (r.renorm) {
-    for (int j = team.lane; j < r.k; j += lanes) {
-      const float v = logit(picks[j]);
-      m = fmaxf(m, r.sigmoid ? log_logistic(v) : v);
-    }
-    for (int o = 0; o < r.team_lanes; ++o) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1 << o));
-    for (int j = team.lane; j < r.k; j += lanes) {
-      const float v = logit(picks[j]);
-      if (picks[j] >= 0) total += expf((r.sigmoid ? log_logistic(v) : v) - m);
-    }
+    total = 0.0f;
+    for (int j = team.lane; j < r.k; j += lanes) total += score(best[j]);
     total = team_sum(total, r.team_lanes) + (sum - sum);      // a row's scores that are NaN (a bias ranked them then) stay so
   }
+  if (!alive) return;
+  const float by = r.renorm || !r.sigmoid ? __fdividef(r.scale, total) : r.scale;
   for (int j = team.lane; j < r.k; j += lanes) {
-    const int e = picks[j];
-    const float v = logit(e);
-    float w = 0.0f;
-    if (e >= 0) {
-      if (r.renorm) w = expf((r.sigmoid ? log_logistic(v) : v) - m) / total;
-      else w = r.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - top) / sum;
-    }
-    if (alive) r.chosen[row * r.k + j] = e, r.weights[row * r.k + j] = r.scale * w;
+    const uint64_t pick = best[j];
+    r.chosen[row * r.k + j] = pick ? (int)~(uint32_t)pick : -1;
+    r.weights[row * r.k + j] = pick ? score(pick) * by : 0.0f;
   }
+  if (r.renorm && total < 1e-30f && team.lane == 0) weights_by_logarithms<T>(r, from, best, r.weights + row * r.k);
 }
 
-template <typename T, int NV>
+// A team of lanes has a row, which lies in shared memory: gradients of the row's picks are found by a lane each, put to their experts, and leave as
+// whole rows. With softmax scores that are not renormalised every expert has a gradient, and the logits are there beside them. The same rows as
+// above: 24 us (writing 69 MB: 11) and 33 (39 MB: 6).
+template <typename T>
 __global__ void __launch_bounds__(kRouteThreads) k_route_backward(const __grid_constant__ RouteCall r) {
   wait_for_previous();
-  extern __shared__ int shared[];
-  const int lane = threadIdx.x & ((1 << r.team_lanes) - 1), lanes = 1 << r.team_lanes, number = threadIdx.x >> r.team_lanes, teams = kRouteThreads >> r.team_lanes;
+  extern __shared__ float rows_of_all[];
+  const int lanes = 1 << r.team_lanes, lane = threadIdx.x & (lanes - 1), number = threadIdx.x >> r.team_lanes, teams = kRouteThreads >> r.team_lanes;
   const int64_t row = (int64_t)blockIdx.x * teams + number;
-  const bool alive = row < r.rows;
-  int* const pick = shared + number * r.k;
-  float* const part = (float*)shared + teams * r.k + number * r.k;            // p (or s) of a pick, then its gradient
-  float* const slots = (float*)shared + 2 * teams * r.k + threadIdx.x;        // this lane's experts, kRouteThreads apart
+  const bool alive = row < r.rows, dense = !r.sigmoid && !r.renorm;
+  const int width = (r.experts + 3) / 4 * 4;
+  float* const g = rows_of_all + number * width;
+  float* const zs = rows_of_all + (teams + number) * width;                    // dense only
+  float* const part = rows_of_all + (dense ? 2 : 1) * teams * width + number * r.k;      // p (or s) of a pick, then its gradient
+  int* const pick = (int*)(rows_of_all + (dense ? 2 : 1) * teams * width + teams * r.k) + number * r.k;
   const T* const from = (const T*)r.logits + (alive ? row : 0) * r.experts;
-  const bool dense = !r.sigmoid && !r.renorm;      // gradients for experts that were not chosen too
-  float z[NV], top = 0.0f, sum = 1.0f;
-  if (dense) {
-    load_logits<T, NV>(from, lane * NV, alive ? r.experts : 0, r.whole, z);
-    row_softmax(z, r.team_lanes, &top, &sum);
-  }
-  const auto grad = [&](int j) { return r.scale * r.grad[row * r.k + j]; };
+  constexpr int VE = 16 / (int)sizeof(T) < 4 ? 16 / (int)sizeof(T) : 4;
+
+  // what the picks need is asked for in front of all that is waited for
   float m = -INFINITY;
   for (int j = lane; j < r.k; j += lanes) {
     const int64_t given = alive ? r.chosen[row * r.k + j] : -1;
     const int e = given >= 0 && given < r.experts ? (int)given : -1;
-    const float v = e >= 0 ? Elem<T>::to_f(from[e]) : -INFINITY, t = r.sigmoid ? log_logistic(v) : v;
-    pick[j] = e;
-    part[j] = r.renorm ? t : r.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - top) / sum;
-    if (e >= 0) m = fmaxf(m, t);
+    const float v = e >= 0 ? Elem<T>::to_f(from[e]) : -INFINITY;
+    pick[j] = e, part[j] = v;
+    if (e >= 0) m = fmaxf(m, r.sigmoid ? log_logistic(v) : v);
   }
-  float dot = 0.0f;
-  if (r.renorm) {
-    for (int o = 0; o < r.team_lanes; ++o) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1 << o));
-    float total = 0.0f;
-    for (int j = lane; j < r.k; j += lanes) total += part[j] = pick[j] >= 0 ? expf(part[j] - m) : 0.0f;
-    total = team_sum(total, r.team_lanes);
-    for (int j = lane; j < r.k; j += lanes)
-      if (pick[j] >= 0) part[j] /= total, dot += part[j] * grad(j);
-  } else if (dense) {
-    for (int j = lane; j < r.k; j += lanes)
-      if (pick[j] >= 0) dot += part[j] * grad(j);
-  }
-  dot = team_sum(dot, r.team_lanes);
-  for (int j = lane; j < r.k; j += lanes) {
-    if (pick[j] < 0) continue;
-    const float g = grad(j);
-    if (dense) {
-      part[j] = g;
+  float top = 0.0f, sum = 1.0f;
+  if (dense) {
+    float most = -INFINITY;
+    if (r.whole) {
+      for (int e = lane * VE; e < r.experts; e += lanes * VE) {
+        const Raw<T, VE> v = load_raw<T, VE>(from + e);
+#pragma unroll
+        for (int q = 0; q < VE; ++q) most = fmaxf(most, v.get(q)), zs[e + q] = v.get(q), g[e + q] = 0.0f;
+      }
     } else {
-      // 1 - s without a difference of two near ones
-      const float rest = r.sigmoid ? 1.0f / (1.0f + expf(Elem<T>::to_f(from[pick[j]]))) : 1.0f;
-      part[j] = part[j] * rest * (r.renorm ? g - dot : g);
-    }
-  }
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < NV; ++i) slots[i * kRouteThreads] = 0.0f;
-  for (int j = 0; j < r.k; ++j) {
-    const int e = pick[j];
-    if (e >= 0 && e / NV == lane) slots[e % NV * kRouteThreads] += part[j];
-  }
-  if (!alive) return;
-  T* const to = (T*)r.grad_logits + row * r.experts + lane * NV;
-  float out[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    out[i] = slots[i * kRouteThreads];
-    if (dense) out[i] = z[i] == -INFINITY ? 0.0f : expf(z[i] - top) / sum * (out[i] - dot);
-  }
-  if (r.whole) {
-    constexpr int VE = 16 / (int)sizeof(T) < NV ? 16 / (int)sizeof(T) : NV;
-    if (lane * NV < r.experts) {
-#pragma unroll
-      for (int i = 0; i < NV; i += VE) {
-        float v[VE];
-#pragma unroll
-        for (int q = 0; q < VE; ++q) v[q] = out[i + q];
-        store_all<T, VE>(to + i, v);
+      for (int e = lane; e < r.experts; e += lanes) {
+        const float v = Elem<T>::to_f(from[e]);
+        most = fmaxf(most, v), zs[e] = v, g[e] = 0.0f;
       }
     }
+    most = team_most(most, r.team_lanes);
+    top = most == -INFINITY ? 0.0f : most, sum = 0.0f;
+    __syncwarp();
+    for (int e = lane; e < r.experts; e += lanes) {
+      const float s = exp_short(zs[e] - top);
+      zs[e] = s, sum += s;
+    }
+    sum = team_sum(sum, r.team_lanes);
   } else {
+    for (int e = lane; e < width; e += lanes) g[e] = 0.0f;
+  }
+  const auto grad = [&](int j) { return r.scale * r.grad[row * r.k + j]; };
+  float dot = 0.0f, total = 0.0f;
+  if (r.renorm) {
+    m = team_most(m, r.team_lanes);
+    for (int j = lane; j < r.k; j += lanes) total += pick[j] >= 0 ? exp_short((r.sigmoid ? log_logistic(part[j]) : part[j]) - m) : 0.0f;
+    total = team_sum(total, r.team_lanes);
+  }
+  const auto share = [&](int j) {
+    const float v = part[j];
+    return r.renorm ? __fdividef(exp_short((r.sigmoid ? log_logistic(v) : v) - m), total) : r.sigmoid ? logistic(v) : __fdividef(exp_short(v - top), sum);
+  };
+  if (r.renorm || dense) {
+    for (int j = lane; j < r.k; j += lanes)
+      if (pick[j] >= 0) dot += share(j) * grad(j);
+    dot = team_sum(dot, r.team_lanes);
+  }
+  for (int j = lane; j < r.k; j += lanes) {
+    if (pick[j] < 0) continue;
+    // 1 - s without a difference of two near ones
+    const float rest = r.sigmoid ? logistic(-part[j]) : 1.0f;
+    part[j] = dense ? grad(j) : share(j) * rest * (r.renorm ? grad(j) - dot : grad(j));
+  }
+  __syncwarp();
+  // one lane an expert, in the picks' order: an expert that is named twice has the sum
+  for (int j = 0; j < r.k; ++j) {
+    const int e = pick[j];
+    if (e >= 0 && (e & (lanes - 1)) == lane) g[e] += part[j];
+  }
+  __syncwarp();
+  if (!alive) return;
+  T* const to = (T*)r.grad_logits + row * r.experts;
+  const float by = dense ? 1.0f / sum : 0.0f;
+  const auto out = [&](float s, float g) { return !dense ? g : s == 0.0f ? 0.0f : s * by * (g - dot); };
+  if (r.whole) {
+    constexpr int W = 16 / (int)sizeof(T);
+    for (int e = lane * W; e < r.experts; e += lanes * W) {
+      float v[W];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (lane * NV + i < r.experts) to[i] = Elem<T>::from_f(out[i]);
+      for (int q = 0; q < W; q += 4) {
+        const float4 d = *(const float4*)(g + e + q), s = dense ? *(const float4*)(zs + e + q) : d;
+        v[q] = out(s.x, d.x), v[q + 1] = out(s.y, d.y), v[q + 2] = out(s.z, d.z), v[q + 3] = out(s.w, d.w);
+      }
+      store_all<T, W>(to + e, v);
+    }
+  } else {
+    for (int e = lane; e < r.experts; e += lanes) to[e] = Elem<T>::from_f(out(dense ? zs[e] : 0.0f, g[e]));
   }
 }
 
 // ---- host side -----------------------------------------------------------------------
-// Experts a lane and lanes: the fewest experts with which the groups, each in lanes of its own, a power of two of them, fit a warp. Eight
-// at least: a round costs the team its exchanges, whatever a lane holds.
+// Experts a lane and lanes. What a row costs whatever it holds (bound, places, weights: some 400 instructions) several rows share in a warp that has
+// more experts a lane; but the bound comes of twice as many lanes as are chosen, or it is too low and there are too many candidates. So 16 experts a
+// lane where that leaves lanes enough, of the groups that stay, else eight; or the fewest with which the groups, each in lanes of its own, a power of two
+// of them, fit a warp.
 static int route_plan(RouteCall* r) {
-  int nv = 8;
-  for (;; nv *= 2) {
+  const auto lay_out = [r](int nv) {
     r->group_lanes = 0;
     while ((nv << r->group_lanes) < r->per) ++r->group_lanes;
     r->team_lanes = r->group_lanes;
     while ((1 << (r->team_lanes - r->group_lanes)) < r->groups) ++r->team_lanes;
-    if (r->team_lanes <= 5) return nv;
-  }
+    return r->team_lanes <= 5;
+  };
+  if (r->experts > 64 && lay_out(16) && (r->top_groups << r->group_lanes) >= 2 * r->k) return 16;
+  int nv = 8;
+  while (!lay_out(nv)) nv *= 2;
+  return nv;
 }
 
 template <typename T, int NV>
-static int launch_route(RouteCall r, bool backward, cudaStream_t s) {
+static int launch_route(const RouteCall& r, cudaStream_t s) {
   const int teams = kRouteThreads >> r.team_lanes;
   const int64_t blocks = ceil_div(r.rows, teams);
   APT_CHECK_ARG(blocks < 1ll << 31, "route_experts: %lld rows are too many", (long long)r.rows);
-  const size_t picks = (size_t)teams * r.k * 4;
-  if (backward)
-    APT_FOLLOW((k_route_backward<T, NV>), blocks, kRouteThreads, 2 * picks + NV * kRouteThreads * 4, s, r);
-  else
-    APT_FOLLOW((k_route<T, NV>), blocks, kRouteThreads, picks, s, r);
+  const size_t bytes = ((size_t)teams * (r.found + r.k + 1) + kRouteThreads / 32 * r.experts) * 8;
+  const bool exact = r.bias || (r.groups > 1 && r.best == 2);
+  if (r.groups > 1) {
+    if (exact) APT_FOLLOW((k_route<T, NV, true, true>), blocks, kRouteThreads, bytes, s, r);
+    else APT_FOLLOW((k_route<T, NV, true, false>), blocks, kRouteThreads, bytes, s, r);
+  } else if constexpr (NV < 64) {
+    if (exact) APT_FOLLOW((k_route<T, NV, false, true>), blocks, kRouteThreads, bytes, s, r);
+    else APT_FOLLOW((k_route<T, NV, false, false>), blocks, kRouteThreads, bytes, s, r);
+  }
   return APT_OK;
 }
 template <typename T>
-static int route(RouteCall r, bool backward, cudaStream_t s) {
+static int route(RouteCall r, cudaStream_t s) {
   const int nv = route_plan(&r);
-  r.whole = r.per % nv == 0 && r.experts * sizeof(T) % 16 == 0 && ((uintptr_t)r.logits | (uintptr_t)r.grad_logits) % 16 == 0;
-  if (nv == 8) return launch_route<T, 8>(r, backward, s);
-  if (nv == 16) return launch_route<T, 16>(r, backward, s);
-  if (nv == 32) return launch_route<T, 32>(r, backward, s);
-  return launch_route<T, 64>(r, backward, s);
+  r.found = (std::min(r.experts, kRouteFound) + 2) / 2 * 2;
+  r.whole = r.per % nv == 0 && r.experts * sizeof(T) % 16 == 0 && (uintptr_t)r.logits % 16 == 0;
+  if (nv == 8) return launch_route<T, 8>(r, s);
+  if (nv == 16) return launch_route<T, 16>(r, s);
+  if (nv == 32) return launch_route<T, 32>(r, s);
+  return launch_route<T, 64>(r, s);
+}
+// Lanes for a row's picks, and for 64 of its experts each at the most: few, so that many rows are on their way at once.
+template <typename T>
+static int route_backward(RouteCall r, cudaStream_t s) {
+  const bool dense = !r.sigmoid && !r.renorm;
+  r.team_lanes = 2;
+  while (r.team_lanes < 5 && ((1 << r.team_lanes) < r.k || (1 << r.team_lanes) * (dense ? 8 : 64) < r.experts)) ++r.team_lanes;
+  r.whole = r.experts * sizeof(T) % 16 == 0 && ((uintptr_t)r.logits | (uintptr_t)r.grad_logits) % 16 == 0;
+  const int teams = kRouteThreads >> r.team_lanes;
+  const int64_t blocks = ceil_div(r.rows, teams);
+  APT_CHECK_ARG(blocks < 1ll << 31, "route_experts_backward: %lld rows are too many", (long long)r.rows);
+  APT_FOLLOW((k_route_backward<T>), blocks, kRouteThreads, (size_t)teams * ((dense ? 2 : 1) * align_up(r.experts, 4) + 2 * r.k) * 4, s, r);
+  return APT_OK;
 }
 static int route_check(const char* who, int dtype, int64_t rows, int64_t experts, int64_t k, int score) {
   APT_CHECK_ARG(dtype == APT_F32 || dtype == APT_BF16 || dtype == APT_F16, "%s: unsupported dtype %d", who, dtype);
@@ -407,12 +548,12 @@ extern "C" int apt_route_experts(int dtype, const void* logits, int64_t rows, in
   r.logits = logits, r.bias = bias, r.rows = rows, r.experts = (int)experts, r.k = (int)k;
   // groups that all stay are none
   const bool grouped = groups > 1 && top_groups < groups;
-  r.groups = grouped ? (int)groups : 1, r.per = grouped ? (int)(experts / groups) : (int)experts, r.top_groups = (int)top_groups, r.best = group_best;
+  r.groups = grouped ? (int)groups : 1, r.per = grouped ? (int)(experts / groups) : (int)experts, r.top_groups = grouped ? (int)top_groups : 1, r.best = group_best;
   r.sigmoid = score == APT_SCORE_SIGMOID, r.renorm = renormalize != 0, r.scale = scale, r.chosen = chosen, r.weights = weights;
   const cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == APT_F32) return route<float>(r, false, s);
-  if (dtype == APT_BF16) return route<__nv_bfloat16>(r, false, s);
-  return route<__half>(r, false, s);
+  if (dtype == APT_F32) return route<float>(r, s);
+  if (dtype == APT_BF16) return route<__nv_bfloat16>(r, s);
+  return route<__half>(r, s);
 }
 
 extern "C" int apt_route_experts_backward(int dtype, const void* logits, int64_t rows, int64_t experts, int64_t k, int score, int renormalize, float scale,
@@ -426,7 +567,7 @@ extern "C" int apt_route_experts_backward(int dtype, const void* logits, int64_t
   r.sigmoid = score == APT_SCORE_SIGMOID, r.renorm = renormalize != 0, r.scale = scale;
   r.chosen = (int64_t*)chosen, r.grad = grad_weights, r.grad_logits = grad_logits;
   const cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == APT_F32) return route<float>(r, true, s);
-  if (dtype == APT_BF16) return route<__nv_bfloat16>(r, true, s);
-  return route<__half>(r, true, s);
+  if (dtype == APT_F32) return route_backward<float>(r, s);
+  if (dtype == APT_BF16) return route_backward<__nv_bfloat16>(r, s);
+  return route_backward<__half>(r, s);
 }

@@ -27,6 +27,12 @@ __device__ __forceinline__ bool barrier_over(uint32_t bar, uint32_t parity) {
                : "memory");
   return done;
 }
+// The same at once, without a wait.
+__device__ __forceinline__ bool barrier_is_over(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done;
+}
 // Until the barrier's phase of this parity is over, or for that many polls, each of which may suspend for a while itself. False: somebody
 // has given up (*gave_up); nothing may be used then but what ends the kernel. The first poll stands by itself: with the count in front of it, products of
 // 65536 x 1024 -> 1024 fp32 take 820 us, not 807.

@@ -23,15 +23,15 @@ def test_other_arguments_are_refused():
     assert lib.apt_route_experts(_lib.F32, None, 4, 8, 2, 0, None, 1, 1, 1, 1, 1.0, P, P, None) == _lib.APT_ERR_BAD_ARG
     assert lib.apt_route_experts_backward(_lib.F32, P, 4, 8, 2, 0, 1, 1.0, P, None, P, None) == _lib.APT_ERR_BAD_ARG
     assert lib.apt_expert_rows(P, 2 ** 30, 64, P, 2, 8, P, P, P, None, 0, P, None) == _lib.APT_ERR_BAD_ARG
-    assert lib.apt_expert_rows(P, 4000, 64, P, 2, 8, P, P, P, None, 0, P, None) == _lib.APT_ERR_BAD_ARG and b"workspace" in lib.apt_last_error()
+    assert lib.apt_expert_rows(P, 8000, 64, P, 2, 8, P, P, P, None, 0, P, None) == _lib.APT_ERR_BAD_ARG and b"workspace" in lib.apt_last_error()
     assert lib.apt_expert_rows(P, 4, 63, P, 2, 8, P, P, P, None, 0, P, None) == _lib.APT_ERR_BAD_ARG
     assert lib.apt_expert_sum(_lib.F32, P, 2 ** 30, 8, 2, P, P, P, P, None) == _lib.APT_ERR_BAD_ARG
     assert lib.apt_expert_sum_backward(_lib.F32, P, 4, 8, 2, None, P, P, P, P, P, None) == _lib.APT_ERR_BAD_ARG
 
 
 def test_few_pairs_take_no_workspace():
-    assert lib.apt_expert_rows_workspace_bytes(1024, 4096) == 0
-    for pairs, experts in ((1025, 1), (10 ** 6, 64), (10 ** 8, 4096)):
+    assert lib.apt_expert_rows_workspace_bytes(4096, 1024) == 0
+    for pairs, experts in ((4097, 1), (1, 1025), (10 ** 6, 64), (10 ** 8, 4096)):
         assert lib.apt_expert_rows_workspace_bytes(pairs, experts) == (experts + 1) * (-(-pairs // 1024) + 1) * 4
 
 

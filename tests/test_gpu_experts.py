@@ -239,7 +239,8 @@ def _experts(rows, k, num_experts, seed, none=0.1):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,k,num_experts,dim", [(1, 1, 1, 1), (1, 6, 64, 256), (3, 2, 2, 7), (31, 3, 5, 8), (129, 8, 512, 33), (512, 2, 16, 100), (513, 2, 16, 4),
-                                                    (1024, 1, 3, 64), (2500, 3, 47, 119), (1500, 7, 4096, 16), (3000, 5, 700, 258)])
+                                                    (1024, 1, 3, 64), (2500, 3, 47, 119), (1500, 7, 4096, 16), (3000, 5, 700, 258), (2048, 2, 1024, 6), (4097, 1, 1024, 6), (1, 1, 1025, 5),
+                                                    (2, 2, 4096, 3)])
 def test_rows_by_expert(rows, k, num_experts, dim, dtype):
     x = torch.randn((rows, dim), device="cuda", generator=_gen(dim)).to(dtype)
     _check_rows(x, _experts(rows, k, num_experts, rows), num_experts)

@@ -33,8 +33,8 @@
 
 namespace apt {
 
-// The last four are linear_cross_entropy's (loss.cuh), whose rows are one group.
-enum GroupedMode { kOut = 0, kGradX = 1, kGradW = 2, kStats = 3, kSlopes = 4, kSumX = 5, kSumW = 6 };
+// The last five are linear_cross_entropy's (loss.cu), whose rows are one group. kTallW: dW in whole sums, two tiles of classes that share a stage's rows.
+enum GroupedMode { kOut = 0, kGradX = 1, kGradW = 2, kStats = 3, kSlopes = 4, kSumX = 5, kSumW = 6, kTallW = 7 };
 
 constexpr int kTileM = 128;                  // rows of a product
 constexpr int kMostShared = 227 * 1024 - 640;      // shared memory of a block but for the barriers' and the scan's
@@ -47,9 +47,11 @@ constexpr int kKeepChange = 2;               // tiles that changing kept weights
 template <typename T, int MODE>
 struct GroupedTraits {
   static constexpr bool kSplit = sizeof(T) == 4;
-  static constexpr bool kOverRows = MODE == kGradW || MODE == kSumW;                // the contraction is over the rows
+  static constexpr bool kTall = MODE == kTallW, kOverRows = MODE == kGradW || MODE == kSumW || kTall;      // the contraction is over the rows
+  static constexpr bool kScaled = MODE == kSumW || kTall;
+  static constexpr int kTileA = kTall ? 2 * kTileM : kTileM;      // of rows that are copied
   static constexpr bool kClasses = MODE == kStats || MODE == kSlopes, kLists = kClasses || MODE == kSumX;
-  static constexpr bool kOneGroup = kLists || MODE == kSumW, kHasBias = MODE == kOut || kClasses;
+  static constexpr bool kOneGroup = kLists || kScaled, kHasBias = MODE == kOut || kClasses;
   static constexpr bool kMnA = kOverRows, kMnB = !(MODE == kOut || kClasses);
   static constexpr int kBlock = kSplit ? 32 : 64;              // of the contraction in a stage
   static constexpr int kBox = 128 / (int)sizeof(T);            // elements of a box's row
@@ -61,7 +63,7 @@ struct GroupedTraits {
   static constexpr int kThreads = kSplit ? 512 : 128 + 32 * kOutWarps;
   // shared memory of one of those warps, in which 32 rows lie on their way out (or their statistics on the way to the warp that joins them)
   static constexpr int kStaging = MODE == kStats ? 2 * 4 * (kTurns - 1) * 32 * 8 / kOutWarps : MODE == kSumX ? 0 : MODE == kSlopes && !kSplit ? 2048 : 4096;
-  static constexpr int kBiasFloats = kOverRows ? 512 : 256 * kGangs;
+  static constexpr int kBiasFloats = kTall ? 0 : kOverRows ? 512 : 256 * kGangs;      // (tall tiles: where rows lie on their way out)
   // a sum in tensor memory has so many stages at most: 1024 terms of fp32, 8192 rows of 16 bits (with 4096, 65536 x 1024 -> 1024 bf16, dw and db 182 -> 205 us:
   // the warps that bring parts out are those that add up db, for which the stages wait)
   static constexpr bool kCuts = kSplit || kOverRows || MODE == kSumX;
@@ -147,6 +149,8 @@ struct GroupedWalk {
     if constexpr (Tr::kLists) {
       const int64_t all = (int64_t)c.tiles_m * c.tiles_n * c.splits;
       next = c.keep ? blockIdx.x * all / gridDim.x : blockIdx.x, step = c.keep ? 1 : gridDim.x, end = c.keep ? (blockIdx.x + 1) * all / gridDim.x : all;
+    } else if constexpr (Tr::kTall) {
+      next = blockIdx.x, step = gridDim.x, end = (int64_t)c.tiles_m * c.tiles_n;
     } else if constexpr (Tr::kOverRows) {
       runs = grouped_runs((int64_t)prefix[c.groups] * c.tiles_m * c.tiles_n, c.ranges);
       next = end = 0;
@@ -207,6 +211,15 @@ struct GroupedWalk {
     if constexpr (Tr::kLists) {
       if (next >= end) return false;
       take_listed(item);
+      next += step;
+      return true;
+    } else if constexpr (Tr::kTall) {
+      if (next >= end) return false;
+      const int m = (int)quotient(next, c.tiles_n);
+      item->g = 0, item->row = 0, item->m0 = m * Tr::kTileA, item->n0 = (int)(next - (int64_t)m * c.tiles_n) * c.tile_n;
+      take_part(item, (int)((c.rows + Tr::kBlock - 1) / Tr::kBlock));
+      item->rows = (int)min((int64_t)item->stages * Tr::kBlock, c.rows);
+      item->piece = -1, item->first = item->last = 0;
       next += step;
       return true;
     } else if constexpr (Tr::kOverRows) {
@@ -689,7 +702,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 
   const bool keep = !Tr::kOverRows && c.keep;
   // (products read 128 rows of a smaller tile too: what lies behind it in shared memory)
-  const int copied_a = Tr::kOverRows || Tr::kSplit ? Tr::copied(kTileM, Tr::kMnA) : c.halves * c.tile_m * 128, copied_b = Tr::copied(c.tile_n, Tr::kMnB);
+  const int copied_a = Tr::kOverRows || Tr::kSplit ? Tr::copied(Tr::kTileA, Tr::kMnA) : c.halves * c.tile_m * 128, copied_b = Tr::copied(c.tile_n, Tr::kMnB);
   const int block_bytes = copied_a + (keep ? 0 : copied_b), copied_bytes = c.deep * block_bytes;
   const int piece_a = Tr::piece(kTileM, Tr::kMnA), piece_b = Tr::piece(c.tile_n, Tr::kMnB);
   const int piece_bytes = Tr::kSplit ? 3 * (piece_a + (keep ? 0 : piece_b)) : 0;
@@ -759,7 +772,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
   GroupedWalk<T, MODE> walk(c, prefix, begin);
-  if (Tr::kOverRows && blockIdx.x == 0 && threadIdx.x == 0) c.plan[0] = walk.runs.units, c.plan[1] = walk.runs.runs;
+  if (Tr::kOverRows && !Tr::kTall && blockIdx.x == 0 && threadIdx.x == 0) c.plan[0] = walk.runs.units, c.plan[1] = walk.runs.runs;
   GroupedItem item;
   bool fine = true;
   if (warp == 0) {
@@ -768,7 +781,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       int stage = 0, loaded = 0, kept_g = -1, kept_n = -1, kept_times = 0;
       uint32_t phase = 0;
       while (fine && walk.take(&item)) {
-        const int boxes_a = Tr::kOverRows ? (min(kTileM, c.num_m - item.m0) + Tr::kBox - 1) / Tr::kBox : 1;
+        const int boxes_a = Tr::kOverRows ? (min(Tr::kTileA, c.num_m - item.m0) + Tr::kBox - 1) / Tr::kBox : 1;
         const int boxes_b = Tr::kMnB ? (min(c.tile_n, c.num_n - item.n0) + Tr::kBox - 1) / Tr::kBox : 1;
         constexpr int kBoxBytes = Tr::kBlock * 128;
         const uint32_t bytes_b = Tr::kMnB ? boxes_b * kBoxBytes : c.tile_n * 128;
@@ -840,7 +853,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       bool there = false;                             // the stage, as far as is known
       while (fine && walk.take(&item)) {
         if (!item.stages) continue;
-        const int halves = !Tr::kOverRows && item.rows > c.tile_m ? 2 : 1;
+        const int halves = (Tr::kTall ? c.num_m - item.m0 > kTileM : !Tr::kOverRows && item.rows > c.tile_m) ? 2 : 1;
         buffer = c.halves == 2 || buffer == kBuffers - 1 ? 0 : buffer + 1;
         if (!(fine = barrier_wait(shared_addr(acc_free + buffer), turns >> buffer & 1 ^ 1, gave_up, c.polls))) break;
         if (halves == 2 && !(fine = barrier_wait(shared_addr(acc_free + 1), turns >> 1 & 1 ^ 1, gave_up, c.polls))) break;
@@ -896,7 +909,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               }
             }
           };
-          if (!Tr::kSplit && !Tr::kOverRows && halves == 2) products(std::true_type{});
+          if ((Tr::kTall || (!Tr::kSplit && !Tr::kOverRows)) && halves == 2) products(std::true_type{});
           else products(std::false_type{});
           products_done(shared_addr((Tr::kSplit ? used : free_) + stage));
           if (k == item.stages - 1) {
@@ -933,16 +946,17 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     constexpr int kTurns = Tr::kTurns;
     const int quarter = warp % 4, gang = (warp - 4) / (4 * kTurns), turn = (warp - 4) / 4 % kTurns, thread = turn * 128 + threadIdx.x % 128;
     char* const mine = staging + (warp - 4) * Tr::kStaging;
-    float* const bias = all_bias + gang * 256;
+    float* const bias = Tr::kTall ? (float*)staging : all_bias + gang * 256;
     int summed = 0;
     uint32_t summed_phase = 0;
     int bias_g = -1, bias_n = -1, buffer = kBuffers - 1;
     uint32_t turns = 0, meetings = 0;
-    float sum[2] = {0.0f, 0.0f};      // of columns of dy
-    float* const carry = Tr::kCuts ? c.carry + ((int64_t)blockIdx.x * 4 + quarter) * 32 * Tr::kMostN + lane * 4 : nullptr;
-    const float factor = MODE == kSumW ? c.loss.scale[1] : 1.0f;
-    std::conditional_t<MODE == kSlopes, Slopes, std::conditional_t<MODE == kSumW, Multiplied, AsTheyAre>> finish;
-    if constexpr (MODE == kSumW) finish.by = factor;
+    constexpr int kHalves = Tr::kTileA / kTileM;      // of tiles of dw
+    float sum[kHalves][2] = {};      // of columns of dy
+    float* const all_carry = Tr::kCuts ? c.carry + ((int64_t)blockIdx.x * kHalves * 4 + quarter) * 32 * Tr::kMostN + lane * 4 : nullptr;
+    const float factor = Tr::kScaled ? c.loss.scale[1] : 1.0f;
+    std::conditional_t<MODE == kSlopes, Slopes, std::conditional_t<Tr::kScaled, Multiplied, AsTheyAre>> finish;
+    if constexpr (Tr::kScaled) finish.by = factor;
     const auto meet = [&] {      // of the warps here; false: somebody has given up
       __syncwarp();
       if (lane == 0) barrier_arrive(shared_addr(met + gang));
@@ -964,33 +978,43 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           bias[k] = bias_n + k < c.num_n ? Elem<T>::to_f(((const T*)c.bias)[(int64_t)bias_g * c.num_n + bias_n + k]) : 0.0f;
         if (!(fine = meet())) break;
       }
-      float column = 0.0f;      // of db
+      const int halves = (Tr::kTall ? c.num_m - item.m0 > kTileM : !Tr::kOverRows && item.rows > c.tile_m) ? 2 : 1;
+      float column[kHalves] = {};      // of db
       if constexpr (Tr::kOverRows) {
         if (c.grad_bias) {
           // the columns of dy, while the products are made of them: as products with ones they took a third of the time of a stage
-          if (!item.before) sum[0] = sum[1] = 0.0f;
+          if (!item.before)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) sum[h][0] = sum[h][1] = 0.0f;
           for (int k = 0; k < item.stages; ++k) {
             if (!(fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(full + summed), summed_phase, gave_up, c.polls)))) break;
             const int valid = item.rows - k * Tr::kBlock;
-            if (item.n0 == 0) add_columns<T>(copied + (size_t)summed * copied_bytes, valid, thread, sum);
+            if (item.n0 == 0)
+#pragma unroll
+              for (int h = 0; h < kHalves; ++h)
+                if (h < halves) add_columns<T>(copied + (size_t)summed * copied_bytes + h * kTileM * 128, valid, thread, sum[h]);
             __syncwarp();
             if (lane == 0) barrier_arrive(shared_addr(free_ + summed));
             if (++summed == c.copied_stages) summed = 0, summed_phase ^= 1;
           }
           if (!fine) break;
-          column = sum[0];
-          if constexpr (!Tr::kSplit) {      // four threads have a pair of columns
-            if (item.n0 == 0 && !item.after) {
-              if (!(fine = meet())) break;
-              *(float2*)(bias + (thread >> 6) * 128 + (thread & 63) * 2) = make_float2(sum[0], sum[1]);
-              if (!(fine = meet())) break;
-              const int m = thread & 127;
-              column = (bias[m] + bias[128 + m]) + (bias[256 + m] + bias[384 + m]);
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            column[h] = sum[h][0];
+            if constexpr (!Tr::kSplit) {      // four threads have a pair of columns
+              if (item.n0 == 0 && !item.after) {
+                if (!(fine = meet())) break;
+                *(float2*)(bias + (thread >> 6) * 128 + (thread & 63) * 2) = make_float2(sum[h][0], sum[h][1]);
+                if (!(fine = meet())) break;
+                const int m = thread & 127;
+                column[h] = (bias[m] + bias[128 + m]) + (bias[256 + m] + bias[384 + m]);
+              }
             }
           }
+          if (Tr::kTall && fine && item.n0 == 0 && !item.after) fine = meet();      // it is read before rows lie there
+          if (!fine) break;
         }
       }
-      const int halves = !Tr::kOverRows && item.rows > c.tile_m ? 2 : 1;
       for (int half = 0; half < halves; ++half) {
         if (Tr::kGangs > 1 && c.halves == 2 && half != gang) continue;
         const int64_t row = item.row + half * kTileM + quarter * 32 + lane;      // (in out, dx and logits)
@@ -1006,6 +1030,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           tmem_fence_after();
         }
         const uint32_t acc = tmem + buffer * kAccColumns;
+        float* const carry = Tr::kCuts ? all_carry + (Tr::kTall ? half * 4 * 32 * Tr::kMostN : 0) : nullptr;
         if constexpr (MODE == kStats || MODE == kSumX) {
           const uint32_t sums = acc + ((uint32_t)quarter << 21);
           if constexpr (MODE == kStats) {
@@ -1036,18 +1061,18 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           continue;
         }
         if constexpr (Tr::kOverRows) {
-          const int rows = min(kTileM, c.num_m - item.m0), m = quarter * 32 + lane;
+          const int m0 = item.m0 + (Tr::kTall ? half * kTileM : 0), rows = min(kTileM, c.num_m - m0), m = quarter * 32 + lane;
           if (quarter * 32 < rows) {
             if (item.piece < 0 || item.after)
-              store_tile<T, T, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + item.m0) * c.num_n + item.n0,
+              store_tile<T, T, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + ((int64_t)item.g * c.num_m + m0) * c.num_n + item.n0,
                                      (int64_t)c.num_n, rows, columns, nullptr, 0u, carry, item.before, item.after, finish);
             else
               store_tile<T, float, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, c.partial + item.piece * kTileM * c.tile_n, (int64_t)c.tile_n, rows,
                                          columns, nullptr, 0u, carry, item.before, item.after, AsTheyAre{});
             if (c.grad_bias && item.n0 == 0 && turn == 0 && !item.after) {
               if (m < rows) {
-                if (item.piece < 0) ((T*)c.grad_bias)[(int64_t)item.g * c.num_m + item.m0 + m] = Elem<T>::from_f(MODE == kSumW ? column * factor : column);
-                else c.partial_bias[item.piece * kTileM + m] = column;
+                if (item.piece < 0) ((T*)c.grad_bias)[(int64_t)item.g * c.num_m + m0 + m] = Elem<T>::from_f(Tr::kScaled ? column[Tr::kTall ? half : 0] * factor : column[0]);
+                else c.partial_bias[item.piece * kTileM + m] = column[0];
               }
             }
           }
@@ -1075,7 +1100,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
       }
     }
-  } else if (Tr::kOverRows && warp == 3) {
+  } else if (Tr::kOverRows && !Tr::kTall && warp == 3) {
     // ---- the plan of the block's run, which follows from the walk and waits for nothing: k_join_weights reads it whoever gives up
     if (lane == 0 && walk.take(&item)) {
       const int64_t run = blockIdx.x;
@@ -1339,12 +1364,12 @@ static int run_grouped(GroupedCall c, const CUtensorMap& a, const CUtensorMap& b
   using Tr = GroupedTraits<T, MODE>;
   const int lists = grouped_lists<T, MODE>(c.groups);
   const int room = kMostShared - lists - Tr::kOutWarps * Tr::kStaging;
-  int copied = Tr::kOverRows || Tr::kSplit ? Tr::copied(kTileM, Tr::kMnA) : c.tile_m * 128, pieces = Tr::kSplit ? 3 * Tr::piece(kTileM, Tr::kMnA) : 0;
+  int copied = Tr::kOverRows || Tr::kSplit ? Tr::copied(Tr::kTileA, Tr::kMnA) : c.tile_m * 128, pieces = Tr::kSplit ? 3 * Tr::piece(kTileM, Tr::kMnA) : 0;
   const int copied_b = Tr::copied(c.tile_n, Tr::kMnB), pieces_b = Tr::kSplit ? 3 * Tr::piece(c.tile_n, Tr::kMnB) : 0;
   const int kept = c.keep ? (int)(ceil_div(c.num_k, Tr::kBlock) * (Tr::kSplit ? pieces_b : copied_b)) : 0;
   c.polls = bulk_wait_polls();
   if (!c.keep) copied += copied_b, pieces += pieces_b;
-  if (c.halves == 2) copied += kTileM * 128;
+  if (c.halves == 2 && !Tr::kTall) copied += kTileM * 128;
   copied *= c.deep;
   c.piece_stages = Tr::kSplit ? 2 : 0;
   c.copied_stages = std::min(kMaxStages, (room - kept - c.piece_stages * pieces) / copied);

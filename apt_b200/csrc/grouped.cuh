@@ -41,6 +41,7 @@ constexpr int kMostShared = 227 * 1024 - 640;      // shared memory of a block b
 constexpr int kAccColumns = 256;             // tensor memory of a tile: there is room for two
 constexpr int kMaxStages = 12;
 constexpr int kPlanWords = 5;                // of a run
+constexpr int kJoinSlots = 3;                // tiles whose statistics are on the way
 constexpr int kJoinParts = 16;               // blocks for a sum of dw
 constexpr int kKeepChange = 2;               // tiles that changing kept weights takes the time of (5 us to 2.4 a tile of bf16, 8 to 4 of fp32)
 
@@ -57,12 +58,12 @@ struct GroupedTraits {
   static constexpr int kBox = 128 / (int)sizeof(T);            // elements of a box's row
   static constexpr int kMostN = kSplit ? 128 : 256;            // columns of a tile
   // warps that bring tiles out: two for each quarter of tensor memory's lanes, or one beside the eight that take fp32 apart
-  // (logits in 16 bits: two gangs of eight, each with every other tile. The exponentials of a tile take as long as its products of 256 terms, and a
-  // tile's way through a warp, with its waits for tensor memory and for what is known of its rows, is longer than that)
+  // (logits in 16 bits: sixteen, whose exponentials take as long as the products of 256 terms: two gangs of eight, each with every other tile, so that one's
+  // waits and stores are beside the other's exponentials)
   static constexpr int kOutWarps = kSplit ? 4 : kClasses ? 16 : 8, kGangs = kClasses && !kSplit ? 2 : 1, kTurns = kOutWarps / kGangs / 4;
   static constexpr int kThreads = kSplit ? 512 : 128 + 32 * kOutWarps;
-  // shared memory of one of those warps, in which 32 rows lie on their way out (or their statistics on the way to the warp that joins them)
-  static constexpr int kStaging = MODE == kStats ? 2 * 4 * (kTurns - 1) * 32 * 8 / kOutWarps : MODE == kSumX ? 0 : MODE == kSlopes && !kSplit ? 2048 : 4096;
+  // shared memory of one of those warps, in which 32 rows lie on their way out (or statistics of three tiles of a gang on the way to the warps that join them)
+  static constexpr int kStaging = MODE == kStats ? (kSplit ? 0 : kGangs * kJoinSlots * 4 * kTurns * 32 * 8 / kOutWarps) : MODE == kSlopes && !kSplit ? 2048 : 4096;
   static constexpr int kBiasFloats = kTall ? 0 : kOverRows ? 512 : 256 * kGangs;      // (tall tiles: where rows lie on their way out)
   // a sum in tensor memory has so many stages at most: 1024 terms of fp32, 8192 rows of 16 bits (with 4096, 65536 x 1024 -> 1024 bf16, dw and db 182 -> 205 us:
   // the warps that bring parts out are those that add up db, for which the stages wait)
@@ -144,9 +145,11 @@ struct GroupedWalk {
   const int *prefix, *begin;    // of each group: tiles (stages in dw) of those before, first row
   int64_t next, end, step;
   int last_g = 0, last_n = 0, last_t = -2;      // of the tile before
+  int all_stages = 0;                           // of a tile, without groups
   GroupedRuns runs;
   __device__ GroupedWalk(const GroupedCall& call, const int* p, const int* rows) : c(call), prefix(p), begin(rows) {
     if constexpr (Tr::kLists) {
+      all_stages = (c.num_k + Tr::kBlock * c.deep - 1) / (Tr::kBlock * c.deep);
       const int64_t all = (int64_t)c.tiles_m * c.tiles_n * c.splits;
       next = c.keep ? blockIdx.x * all / gridDim.x : blockIdx.x, step = c.keep ? 1 : gridDim.x, end = c.keep ? (blockIdx.x + 1) * all / gridDim.x : all;
     } else if constexpr (Tr::kTall) {
@@ -189,14 +192,17 @@ struct GroupedWalk {
       n = (int)quotient(at, here), t = (int)(b * c.band + (at - (int64_t)n * here));
     }
     last_t = t, last_n = n;
-    const int all = (c.num_k + Tr::kBlock * c.deep - 1) / (Tr::kBlock * c.deep);
-    item->g = 0, item->m0 = t, item->n0 = n * c.tile_n;
-    item->row = (int64_t)t * (c.tile_m * c.halves);
-    item->rows = (int)min((int64_t)(c.tile_m * c.halves), c.rows - item->row);
-    item->first = 0, item->last = 0;
-    item->piece = ((int64_t)part * c.tiles_m + t) * c.tiles_n + n;
-    if constexpr (MODE == kSumX) item->before = part * c.split_stages;
-    take_part(item, MODE == kSumX ? min(all - item->before, c.split_stages) : all);
+    const int row = t * (c.tile_m * c.halves);
+    item->g = 0, item->m0 = n, item->n0 = n * c.tile_n;      // (m0: which tile of columns)
+    item->row = row, item->rows = min(c.tile_m * c.halves, (int)c.rows - row);
+    item->first = 0;
+    if constexpr (MODE == kSumX) {
+      item->piece = ((int64_t)part * c.tiles_m + t) * c.tiles_n + n;
+      item->before = part * c.split_stages;
+      take_part(item, min(all_stages - item->before, c.split_stages));
+    } else {
+      take_part(item, all_stages);
+    }
   }
   __device__ bool take(GroupedItem* item) {
     if (Tr::kCuts && item->after) {
@@ -578,10 +584,17 @@ __device__ __forceinline__ float2 tile_statistics(uint32_t acc, int turn, int tu
     const float here = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * kLog2e;
     if (here > top) sum *= exp2_short(top - here), top = here;
     const float ref = top == -INFINITY ? 0.0f : top;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const F2 by = f2_pack(kLog2e, kLog2e), less = f2_pack(-ref, -ref);
+    F2 s[2] = {0ull, 0ull};
 #pragma unroll
-    for (int k = 0; k < 32; ++k) s[k % 4] += exp2_short(fmaf(v[k], kLog2e, -ref));
-    sum += (s[0] + s[1]) + (s[2] + s[3]);
+    for (int k = 0; k < 32; k += 2) {
+      float x, y;
+      f2_unpack(f2_fma(f2_pack(v[k], v[k + 1]), by, less), x, y);
+      s[k / 2 % 2] = f2_add(s[k / 2 % 2], f2_pack(exp2_short(x), exp2_short(y)));
+    }
+    float x, y;
+    f2_unpack(f2_add(s[0], s[1]), x, y);
+    sum += x + y;
   }
   return make_float2(top, sum);
 }
@@ -596,16 +609,26 @@ __device__ __forceinline__ void join_statistics(float2* a, float2 b) {
   }
 }
 
-// The loss's slope along a row's logits: probabilities less one at the label, times the row's factor.
+// The loss's slope along a row's logits: probabilities less one at the label, times the row's factor. 16 bits have the factor over the sum in the
+// exponent, 2^-23 of some twenty; fp32 multiplies. Rows whose factor is not above zero are minus those of its magnitude, or zeros.
 struct Slopes {
-  float top, share, factor;
+  float less, share, factor;
   int label;
   template <int H>
   __device__ __forceinline__ void operator()(float (&v)[H][32], int c0) const {
+    const F2 by = f2_pack(kLog2e, kLog2e), under = f2_pack(-less, -less);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k) v[h][k] = exp2_short(fmaf(v[h][k], kLog2e, -top)) * share;
+      for (int k = 0; k < 32; k += 2) {
+        float x, y;
+        f2_unpack(f2_fma(f2_pack(v[h][k], v[h][k + 1]), by, under), x, y);
+        v[h][k] = exp2_short(x), v[h][k + 1] = exp2_short(y);
+      }
+      if (__any_sync(0xffffffffu, share != 1.0f)) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[h][k] *= share;
+      }
       const int mine = label - c0 - 32 * h;
       if (__any_sync(0xffffffffu, (unsigned)mine < 32u)) {
 #pragma unroll
@@ -619,15 +642,29 @@ struct Slopes {
     }
   }
 };
-__device__ __forceinline__ Slopes row_slopes(const LossCall& l, int64_t row, bool there, int64_t n0) {
-  Slopes s = {0.0f, 0.0f, 0.0f, -1};
-  if (!there) return s;
-  const int64_t label = l.labels[row];
-  const float2 t = l.stats[row];
-  if (t.y < 0.0f) return s;      // does not count
-  s.factor = (l.grad ? l.grad[row] : 1.0f) * l.scale[0];
-  s.top = t.x, s.share = s.factor / t.y;
-  const int64_t at = label - l.class0 - n0;
+// What a row's slopes are made of, as it is in memory.
+struct RowFacts {
+  int64_t label;
+  float2 stats;
+  float grad;
+};
+__device__ __forceinline__ RowFacts ask_row(const LossCall& l, int64_t row, bool there) {
+  RowFacts f = {-1, make_float2(0.0f, -1.0f), 1.0f};
+  if (there) {
+    f.label = l.labels[row];
+    if (l.stats) f.stats = l.stats[row];
+    if (l.grad) f.grad = l.grad[row];
+  }
+  return f;
+}
+template <bool SHORT>
+__device__ __forceinline__ Slopes row_slopes(const LossCall& l, const RowFacts& f, int64_t n0) {
+  Slopes s = {0.0f, 1.0f, 0.0f, -1};
+  if (f.stats.y < 0.0f) return s;      // does not count, or is not there
+  s.factor = f.grad * l.scale[0];
+  s.less = f.stats.x, s.share = s.factor / f.stats.y;
+  if (SHORT && fabsf(s.factor) < INFINITY) s.less -= log2f(fabsf(s.factor) / f.stats.y), s.share = s.factor < 0.0f ? -1.0f : 1.0f;
+  const int64_t at = f.label - l.class0 - n0;
   s.label = at >= 0 && at < 256 ? (int)at : -1;
   return s;
 }
@@ -695,7 +732,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   __shared__ uint64_t full[kMaxStages], free_[kMaxStages], ready[kMaxStages], used[kMaxStages], acc_full[2], acc_free[2], kept_full, kept_free, drained, met[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up_word, scan[33];
-  constexpr bool kJoins = MODE == kStats && Tr::kTurns > 1;      // several warps have parts of a row: `used` counts them, which only fp32 has a use for else
+  constexpr bool kLogits = Tr::kClasses && !Tr::kSplit, kJoins = kLogits && MODE == kStats;      // several warps have parts of a row
   volatile int* const gave_up = &gave_up_word;
   char* const shared = (char*)(((uintptr_t)raw_shared + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -719,8 +756,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     for (int k = 0; k < kMaxStages; ++k) {
       barrier_init(shared_addr(full + k), 1);
       barrier_init(shared_addr(free_ + k), (Tr::kSplit ? 4 : 1) + (Tr::kOverRows && c.grad_bias ? Tr::kOutWarps : 0));
-      barrier_init(shared_addr(ready + k), Tr::kSplit ? 4 : 1);
-      barrier_init(shared_addr(used + k), kJoins ? Tr::kTurns - 1 : 1);
+      barrier_init(shared_addr(ready + k), Tr::kSplit ? 4 : kJoins ? Tr::kTurns : 1);
+      barrier_init(shared_addr(used + k), kJoins ? Tr::kTurns : 1);
     }
     for (int k = 0; k < 2; ++k) barrier_init(shared_addr(acc_full + k), 1), barrier_init(shared_addr(acc_free + k), Tr::kOutWarps / Tr::kGangs), barrier_init(shared_addr(met + k), Tr::kOutWarps / Tr::kGangs);
     barrier_init(shared_addr(&kept_full), Tr::kSplit ? 8 : 1);
@@ -941,12 +978,113 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       __syncwarp();
       if (lane == 0) barrier_arrive(shared_addr(ready + 1));
     }
-  } else if (warp >= 4 && (warp < 8 || !Tr::kSplit)) {
+  } else if (kLogits && warp >= 4) {
+    // ---- logits of 16 bits. What is known of a tile's rows is asked for a tile ahead: its way from memory is as long as half of a tile's exponentials
+    if constexpr (kLogits) {
+      constexpr int kTurns = Tr::kTurns;
+      const int quarter = warp % 4, gang = (warp - 4) / (4 * kTurns), turn = (warp - 4) / 4 % kTurns, thread = turn * 128 + threadIdx.x % 128;
+      char* const mine = staging + (warp - 4) * Tr::kStaging;
+      float* const bias = all_bias + gang * 256;
+      int bias_n = -1, tiles = 0;
+      uint32_t turns = 0, meetings = 0;
+      // the tiles as GroupedWalk has them, with no more of them kept than is needed (t: of rows, n: of classes)
+      const int64_t all = (int64_t)c.tiles_m * c.tiles_n;
+      int at = c.keep ? (int)(blockIdx.x * all / gridDim.x) : (int)blockIdx.x, left = c.keep ? (int)((blockIdx.x + 1) * all / gridDim.x) - at : ((int)all - at + gridDim.x - 1) / (int)gridDim.x;
+      int n = at / c.tiles_m, t = at % c.tiles_m - 1, buffer = kBuffers - 1, half = 0, halves = 0;
+      // the lane's row, how many of the warp's 32 there are, the tile's columns, their number
+      int row = 0, rows = 0, n0 = 0, part = 0, ahead_row = 0, ahead_rows = 0, ahead_n = 0;
+      RowFacts ahead = {};
+      const auto meet = [&] {
+        __syncwarp();
+        if (lane == 0) barrier_arrive(shared_addr(met + gang));
+        const bool all = __all_sync(0xffffffffu, barrier_wait(shared_addr(met + gang), meetings, gave_up, c.polls));
+        meetings ^= 1;
+        return all;
+      };
+      const auto look_ahead = [&] {
+        do {
+          if (half + 1 < halves) {
+            ++half;
+          } else {
+            if (left-- <= 0) return false;
+            if (c.keep) {
+              if (++t == c.tiles_m) t = 0, ++n;
+            } else {
+              const int whole = c.band * c.tiles_n, b = at / whole, in = at - b * whole, here = min(c.band, c.tiles_m - b * c.band);
+              n = in / here, t = b * c.band + in - n * here;
+              at += gridDim.x;
+            }
+            half = 0, halves = c.halves == 2 && (int)c.rows - t * 2 * kTileM > kTileM ? 2 : 1;
+          }
+          buffer = c.halves == 2 ? half : buffer == kBuffers - 1 ? 0 : buffer + 1;
+        } while (buffer != gang);
+        const int first = t * (c.tile_m * c.halves) + half * kTileM;
+        ahead_rows = min((int)c.rows - first, c.tile_m) - quarter * 32, ahead_row = first + quarter * 32 + lane, ahead_n = n;
+        ahead = ask_row(c.loss, ahead_row, lane < ahead_rows);
+        return true;
+      };
+      // Statistics: the warps that share rows leave theirs in shared memory, and one of them, in turn, puts a tile's together when it has given the next one's
+      // sums back. A place is another tile's three of the gang's tiles later: by then all have given back the sums of the one before that, behind this.
+      float2* part_of_last = nullptr;
+      const auto place_of = [&](int i) { return (float2*)staging + ((gang * kJoinSlots + i % kJoinSlots) * 4 + quarter) * kTurns * 32 + lane; };
+      const auto barrier_of = [&](int i) {
+        const int k = (gang * kJoinSlots + i % kJoinSlots) * 4 + quarter;
+        return shared_addr(k < kMaxStages ? used + k : ready + k - kMaxStages);
+      };
+      const auto put_together = [&](int i) {
+        if (!__all_sync(0xffffffffu, barrier_wait(barrier_of(i), i / kJoinSlots & 1, gave_up, c.polls))) return false;
+        const float2* const place = place_of(i);
+        float2 s = place[0];
+#pragma unroll
+        for (int w = 1; w < kTurns; ++w) join_statistics(&s, place[w * 32]);
+        if (part_of_last) *part_of_last = s;
+        return true;
+      };
+      bool more = look_ahead();
+      while (more) {
+        row = ahead_row, rows = ahead_rows, part = ahead_n, n0 = part * c.tile_n;
+        const int columns = min(c.tile_n, c.num_n - n0);
+        const int64_t label = ahead.label - c.loss.class0 - n0;
+        Slopes slopes;
+        if constexpr (MODE == kSlopes) slopes = row_slopes<true>(c.loss, ahead, n0);
+        more = look_ahead();
+        if (c.bias && n0 != bias_n) {
+          bias_n = n0;
+          if (!(fine = meet())) break;      // the tile before is out
+          for (int k = thread; k < 256; k += kTurns * 128) bias[k] = bias_n + k < c.num_n ? Elem<T>::to_f(((const T*)c.bias)[bias_n + k]) : 0.0f;
+          if (!(fine = meet())) break;
+        }
+        fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_full + gang), turns, gave_up, c.polls));
+        if (!fine) break;
+        turns ^= 1;
+        tmem_fence_after();
+        const uint32_t acc = tmem + gang * kAccColumns + ((uint32_t)quarter << 21);
+        const float* const add = c.bias ? bias : nullptr;
+        if constexpr (MODE == kStats)
+          place_of(tiles)[turn * 32] = tile_statistics<T, MODE>(acc, turn, kTurns, columns, add, label >= 0 && label < columns ? (int)label : -1, nullptr, 0, 0, c.loss.picked + row);
+        else if (rows > 0)
+          store_slopes<T, MODE>(acc, mine, lane, turn, kTurns, (T*)c.out + (int64_t)(row - lane) * c.loss.pitch + n0, c.loss.pitch, rows, columns, add, slopes);
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          barrier_arrive(shared_addr(acc_free + gang));
+          if (kJoins) barrier_arrive(barrier_of(tiles));
+        }
+        if constexpr (kJoins) {
+          if (tiles && (tiles - 1) % kTurns == turn && !(fine = put_together(tiles - 1))) break;
+          part_of_last = lane < rows ? c.loss.parts + part * c.loss.pitch + row : nullptr;
+          ++tiles;
+        }
+      }
+      if constexpr (kJoins)
+        if (fine && tiles && (tiles - 1) % kTurns == turn) put_together(tiles - 1);
+    }
+  } else if (!kLogits && warp >= 4 && (warp < 8 || !Tr::kSplit)) {
     // ---- finished tiles
     constexpr int kTurns = Tr::kTurns;
-    const int quarter = warp % 4, gang = (warp - 4) / (4 * kTurns), turn = (warp - 4) / 4 % kTurns, thread = turn * 128 + threadIdx.x % 128;
+    const int quarter = warp % 4, turn = (warp - 4) / 4, thread = turn * 128 + threadIdx.x % 128;
     char* const mine = staging + (warp - 4) * Tr::kStaging;
-    float* const bias = Tr::kTall ? (float*)staging : all_bias + gang * 256;
+    float* const bias = Tr::kTall ? (float*)staging : all_bias;
     int summed = 0;
     uint32_t summed_phase = 0;
     int bias_g = -1, bias_n = -1, buffer = kBuffers - 1;
@@ -959,17 +1097,13 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if constexpr (Tr::kScaled) finish.by = factor;
     const auto meet = [&] {      // of the warps here; false: somebody has given up
       __syncwarp();
-      if (lane == 0) barrier_arrive(shared_addr(met + gang));
-      const bool all = __all_sync(0xffffffffu, barrier_wait(shared_addr(met + gang), meetings, gave_up, c.polls));
+      if (lane == 0) barrier_arrive(shared_addr(met));
+      const bool all = __all_sync(0xffffffffu, barrier_wait(shared_addr(met), meetings, gave_up, c.polls));
       meetings ^= 1;
       return all;
     };
     while (fine && walk.take(&item)) {
       const bool empty = item.stages == 0;
-      if (Tr::kGangs > 1 && c.halves == 1 && (buffer == kBuffers - 1 ? 0 : buffer + 1) != gang) {      // the other gang's
-        buffer = buffer == kBuffers - 1 ? 0 : buffer + 1;
-        continue;
-      }
       const int columns = min(c.tile_n, c.num_n - item.n0);
       if (Tr::kHasBias && c.bias && !empty && (item.g != bias_g || item.n0 != bias_n)) {
         bias_g = item.g, bias_n = item.n0;
@@ -1016,12 +1150,11 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
       }
       for (int half = 0; half < halves; ++half) {
-        if (Tr::kGangs > 1 && c.halves == 2 && half != gang) continue;
         const int64_t row = item.row + half * kTileM + quarter * 32 + lane;      // (in out, dx and logits)
         const bool there = row < item.row + item.rows;
         int64_t label = -1;
         if (MODE == kStats && there) label = c.loss.labels[row] - c.loss.class0 - item.n0;
-        if constexpr (MODE == kSlopes) finish = row_slopes(c.loss, row, there, item.n0);
+        if constexpr (MODE == kSlopes) finish = row_slopes<false>(c.loss, ask_row(c.loss, row, there), item.n0);
         if (!empty) {
           buffer = c.halves == 2 ? half : buffer == kBuffers - 1 ? 0 : buffer + 1;
           fine = __all_sync(0xffffffffu, barrier_wait(shared_addr(acc_full + buffer), turns >> buffer & 1, gave_up, c.polls));
@@ -1036,24 +1169,15 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           if constexpr (MODE == kStats) {
             float2 s = tile_statistics<T, MODE>(sums, turn, kTurns, columns, c.bias ? bias : nullptr, label >= 0 && label < columns ? (int)label : -1, carry, item.before,
                                                 item.after, c.loss.picked + row);
-            if constexpr (kJoins) {
-              // the first of the warps that share the rows puts their statistics together. Their places are another tile's when this one's sums have been
-              // given back by all
-              float2* const place = (float2*)staging + (buffer * 4 + quarter) * (kTurns - 1) * 32 + lane;
-              const uint32_t bar = shared_addr(used + buffer * 4 + quarter);
-              if (turn) {
-                place[(turn - 1) * 32] = s;
-                __syncwarp();
-                if (lane == 0) barrier_arrive(bar);
-              } else {
-                if (!(fine = __all_sync(0xffffffffu, barrier_wait(bar, turns >> buffer & 1 ^ 1, gave_up, c.polls)))) break;
-#pragma unroll
-                for (int w = 0; w < kTurns - 1; ++w) join_statistics(&s, place[w * 32]);
-              }
-            }
-            if (turn == 0 && there && !(Tr::kCuts && item.after)) c.loss.parts[(int64_t)(item.n0 / c.tile_n) * c.loss.pitch + row] = s;
+            if (there && !(Tr::kCuts && item.after)) c.loss.parts[item.m0 * c.loss.pitch + row] = s;
           } else {
-            tile_to_slot<T, MODE>(sums, turn, kTurns, columns, c.carry + ((item.piece * c.halves + half) * 4 + quarter) * 32 * Tr::kMostN + lane * 4, c.loss.more || item.first);
+            if (c.out) {      // whole sums
+              if (quarter * 32 < item.rows - half * kTileM)
+                store_tile<T, T, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + (item.row + half * kTileM) * c.num_n + item.n0, (int64_t)c.num_n,
+                                       min(item.rows - half * kTileM, c.tile_m), columns, nullptr, 0u, carry, 0, 0, Multiplied{c.loss.scale[1]});
+            } else {
+              tile_to_slot<T, MODE>(sums, turn, kTurns, columns, c.carry + ((item.piece * c.halves + half) * 4 + quarter) * 32 * Tr::kMostN + lane * 4, c.loss.more || item.first);
+            }
           }
           tmem_fence_before();
           __syncwarp();
@@ -1078,16 +1202,6 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           }
         }
         const int rows = item.rows - half * kTileM;
-        if constexpr (MODE == kSlopes && !Tr::kSplit) {
-          const int mine_rows = min(rows, c.tile_m) - quarter * 32;
-          if (mine_rows > 0)
-            store_slopes<T, MODE>(acc + ((uint32_t)quarter << 21), mine, lane, turn, kTurns, (T*)c.out + (item.row + half * kTileM + quarter * 32) * c.loss.pitch + item.n0,
-                                  c.loss.pitch, mine_rows, columns, c.bias ? bias : nullptr, finish);
-          tmem_fence_before();
-          __syncwarp();
-          if (lane == 0) barrier_arrive(shared_addr(acc_free + buffer));
-          continue;
-        }
         const bool stores = !Tr::kOverRows && quarter * 32 < min(rows, c.tile_m) && turn * (128 / (int)sizeof(T)) < columns;
         const int64_t ld = MODE == kSlopes ? c.loss.pitch : (int64_t)c.num_n;
         if (stores)

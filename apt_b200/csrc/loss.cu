@@ -341,7 +341,9 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
   float* const carry = carry_of<T>(arena, q.dim);
   GroupedCall sum_x = listed_call<T, kSumX>(q.rows, q.dim, most);
   const int splits = sum_x.splits;
-  sum_x.carry = arena->take<float>((size_t)splits * sum_x.tiles_m * sum_x.tiles_n * sum_x.halves * kTileM * GroupedTraits<T, kSumX>::kMostN);
+  // dx in whole sums: all classes at once, in one part of the contraction
+  const bool whole_x = splits == 1 && most == q.classes && most <= (int64_t)GroupedTraits<T, kSumX>::kCut * GroupedTraits<T, kSumX>::kBlock;
+  if (!whole_x) sum_x.carry = arena->take<float>((size_t)splits * sum_x.tiles_m * sum_x.tiles_n * sum_x.halves * kTileM * GroupedTraits<T, kSumX>::kMostN);
   const WeightPlan p = weight_plan<T>(q.rows, q.dim, most, 1);
   int64_t* const plan = arena->take<int64_t>(2 + kPlanWords * p.ranges);
   float* const partial = arena->take<float>((size_t)p.pieces * kTileM * p.tile_n);
@@ -368,7 +370,7 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
     if (grad_x) {
       GroupedCall d = sum_x;
       d.num_k = (int)n, d.splits = (int)ceil_div(ceil_div(n, GroupedTraits<T, kSumX>::kBlock * d.deep), d.split_stages);
-      d.status = q.status, d.loss.more = v0 > 0;
+      d.status = q.status, d.loss.more = v0 > 0, d.loss.scale = scale, d.out = whole_x ? grad_x : nullptr;
       if (const int e = run_listed<T, kSumX>(d, dz, some, s)) return e;
     }
     if (grad_weight && tall_weights<T>(q.dim, most)) {
@@ -404,7 +406,7 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
       APT_FOLLOW((k_loss_grad_bias<T>), ceil_div(n, 32), 1024, 0, s, (const T*)slopes, q.rows, pitch, (int)n, (const float*)scale, (T*)grad_bias + v0);
     }
   }
-  if (grad_x) {
+  if (grad_x && !whole_x) {
     sum_x.loss.scale = scale;
     const dim3 grid((unsigned)ceil_div(q.rows, 32), (unsigned)ceil_div(q.dim, 64));
     if (q.dim % 8 == 0) APT_FOLLOW((k_loss_grad_rows<T, true>), grid, 256, 0, s, sum_x, (T*)grad_x, splits);

@@ -91,7 +91,7 @@ def test_loss_and_gradients(rows, dim, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,dim,classes", [(3000, 256, 20_000), (20_000, 64, 700), (700, 1024, 9000), (9000, 512, 1500), (4, 128, 60_001)])
+@pytest.mark.parametrize("rows,dim,classes", [(3000, 256, 20_000), (20_000, 64, 700), (700, 1024, 9000), (9000, 512, 1500), (4, 128, 60_001), (2000, 72, 30_011), (9000, 300, 30_000)])
 def test_larger(rows, dim, classes, dtype):
     x, w, b, labels = _inputs(rows, dim, classes, dtype)
     _check(x, w, b, labels, "mean")

@@ -84,9 +84,17 @@ struct LossCall {
   float* picked;                // the logit of the row's label
   const float2* stats;
   const float* grad;            // of the rows' losses; null: all the same
-  const float* scale;           // [2]: what the rows' gradients are multiplied by, what dx and dw are
+  const float* scale;           // [2]: what the rows' gradients are multiplied by, what dx and dw are; null: range and common over it
+  const float *common, *count;  // the gradient that all rows have, and what it is divided by (or null)
+  float range;
+  int* turn;                    // statistics: set to 0 for the kernel behind
   int more;                     // dx: there are sums of earlier classes
 };
+
+__device__ __forceinline__ float slope_scale(const LossCall& l) { return l.scale ? l.scale[0] : l.range; }
+__device__ __forceinline__ float sum_scale(const LossCall& l) {
+  return l.scale ? l.scale[1] : l.common ? *l.common / (l.count ? fmaxf(*l.count, 1.0f) : 1.0f) / l.range : 1.0f;
+}
 
 struct GroupedCall {
   const int64_t* offsets;
@@ -661,7 +669,7 @@ template <bool SHORT>
 __device__ __forceinline__ Slopes row_slopes(const LossCall& l, const RowFacts& f, int64_t n0) {
   Slopes s = {0.0f, 1.0f, 0.0f, -1};
   if (f.stats.y < 0.0f) return s;      // does not count, or is not there
-  s.factor = f.grad * l.scale[0];
+  s.factor = f.grad * slope_scale(l);
   s.less = f.stats.x, s.share = s.factor / f.stats.y;
   if (SHORT && fabsf(s.factor) < INFINITY) s.less -= log2f(fabsf(s.factor) / f.stats.y), s.share = s.factor < 0.0f ? -1.0f : 1.0f;
   const int64_t at = f.label - l.class0 - n0;
@@ -809,6 +817,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
   GroupedWalk<T, MODE> walk(c, prefix, begin);
+  if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *c.loss.turn = 0;
   if (Tr::kOverRows && !Tr::kTall && blockIdx.x == 0 && threadIdx.x == 0) c.plan[0] = walk.runs.units, c.plan[1] = walk.runs.runs;
   GroupedItem item;
   bool fine = true;
@@ -1092,7 +1101,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     constexpr int kHalves = Tr::kTileA / kTileM;      // of tiles of dw
     float sum[kHalves][2] = {};      // of columns of dy
     float* const all_carry = Tr::kCuts ? c.carry + ((int64_t)blockIdx.x * kHalves * 4 + quarter) * 32 * Tr::kMostN + lane * 4 : nullptr;
-    const float factor = Tr::kScaled ? c.loss.scale[1] : 1.0f;
+    const float factor = Tr::kScaled ? sum_scale(c.loss) : 1.0f;
     std::conditional_t<MODE == kSlopes, Slopes, std::conditional_t<Tr::kScaled, Multiplied, AsTheyAre>> finish;
     if constexpr (Tr::kScaled) finish.by = factor;
     const auto meet = [&] {      // of the warps here; false: somebody has given up
@@ -1174,7 +1183,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             if (c.out) {      // whole sums
               if (quarter * 32 < item.rows - half * kTileM)
                 store_tile<T, T, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + (item.row + half * kTileM) * c.num_n + item.n0, (int64_t)c.num_n,
-                                       min(item.rows - half * kTileM, c.tile_m), columns, nullptr, 0u, carry, 0, 0, Multiplied{c.loss.scale[1]});
+                                       min(item.rows - half * kTileM, c.tile_m), columns, nullptr, 0u, carry, 0, 0, Multiplied{sum_scale(c.loss)});
             } else {
               tile_to_slot<T, MODE>(sums, turn, kTurns, columns, c.carry + ((item.piece * c.halves + half) * 4 + quarter) * 32 * Tr::kMostN + lane * 4, c.loss.more || item.first);
             }
@@ -1308,7 +1317,7 @@ k_join_weights(const __grid_constant__ GroupedCall c) {
   if (here <= first || before > first) return;
   const int tile = (int)(what / c.groups), g = (int)(what - (int64_t)tile * c.groups), m0 = tile / c.tiles_n * kTileM, n0 = tile % c.tiles_n * c.tile_n;
   const int64_t piece = 2 * (v - 1) + (before < first);
-  const float factor = c.loss.scale ? c.loss.scale[1] : 1.0f;
+  const float factor = sum_scale(c.loss);
   const int slices = c.tile_n / 4;
   const int64_t size = (int64_t)kTileM * c.tile_n;
   // a sixteenth of the rows, four slices a thread at once

@@ -31,6 +31,9 @@ struct RowsCall {
   int first, last;
   float* losses;                // null: not wanted row by row
   float2* sums;                 // [blocks]: losses and rows that count
+  int* turn;                    // blocks that have theirs there
+  int mean;
+  float *loss, *count;          // of all rows; loss null: not wanted
   int32_t* status;
 };
 
@@ -38,6 +41,8 @@ struct RowsCall {
 __global__ void __launch_bounds__(256) k_loss_rows(const __grid_constant__ RowsCall c) {
   wait_for_previous();
   __shared__ float2 shared[8][32];
+  __shared__ double total[2][8];
+  __shared__ int is_last;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int64_t row = (int64_t)blockIdx.x * 32 + lane;
   const bool there = row < c.rows;
@@ -57,125 +62,116 @@ __global__ void __launch_bounds__(256) k_loss_rows(const __grid_constant__ RowsC
   }
   shared[warp][lane] = s;
   __syncthreads();
-  if (warp) return;
+  if (warp == 0) {
 #pragma unroll
-  for (int w = 1; w < 8; ++w) join_statistics(&s, shared[w][lane]);
-  if (!c.last) {
-    if (there) c.stats[row] = s;
-    return;
-  }
-  float loss = 0.0f, counts = 0.0f;
-  if (there) {
-    const int64_t label = c.labels[row];
-    const bool known = label >= 0 && label < c.classes;
-    if (label != c.ignore && !known) atomicOr(c.status, APT_FLAG_ID_OUT_OF_RANGE);
-    if (label != c.ignore && known) {
-      // against the same number that the sum's exponents refer to, so that a row that is all but sure of its label keeps its digits
-      loss = (log2f(s.y) - fmaf(c.picked[row], kLog2e, -s.x)) * kLn2, counts = 1.0f;
-    } else {
-      s.y = -1.0f;
+    for (int w = 1; w < 8; ++w) join_statistics(&s, shared[w][lane]);
+    float loss = 0.0f, counts = 0.0f;
+    if (there && c.last) {
+      const int64_t label = c.labels[row];
+      const bool known = label >= 0 && label < c.classes;
+      if (label != c.ignore && !known) atomicOr(c.status, APT_FLAG_ID_OUT_OF_RANGE);
+      if (label != c.ignore && known) {
+        // against the same number that the sum's exponents refer to, so that a row that is all but sure of its label keeps its digits
+        loss = (log2f(s.y) - fmaf(c.picked[row], kLog2e, -s.x)) * kLn2, counts = 1.0f;
+      } else {
+        s.y = -1.0f;
+      }
+      if (c.losses) c.losses[row] = loss;
     }
-    c.stats[row] = s;
-    if (c.losses) c.losses[row] = loss;
-  }
+    if (there) c.stats[row] = s;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o), counts += __shfl_xor_sync(0xffffffffu, counts, o);
-  if (lane == 0) c.sums[blockIdx.x] = make_float2(loss, counts);
-}
-
-// All losses' sum, or mean over the rows that count (0 where none does), and their number. One block.
-__global__ void __launch_bounds__(1024) k_loss_total(const float2* __restrict__ sums, int64_t blocks, int mean, float* loss, float* count) {
-  wait_for_previous();
-  __shared__ double part[2][32];
+    for (int o = 16; o; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o), counts += __shfl_xor_sync(0xffffffffu, counts, o);
+    if (lane == 0 && c.last) {
+      c.sums[blockIdx.x] = make_float2(loss, counts);
+      __threadfence();
+      is_last = atomicAdd(c.turn, 1) == (int)gridDim.x - 1;
+    }
+  }
+  if (!c.last) return;
+  __syncthreads();
+  if (!is_last) return;
+  // The last block adds up what all have left, in their order: the sum, or the mean over the rows that count (0 where none does), and their number.
+  __threadfence();
   double a = 0.0, b = 0.0;
-  for (int64_t i = threadIdx.x; i < blocks; i += 1024) a += sums[i].x, b += sums[i].y;
+  const volatile float2* const sums = c.sums;
+  for (int64_t i = threadIdx.x; i < gridDim.x; i += 256) a += sums[i].x, b += sums[i].y;
 #pragma unroll
   for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o), b += __shfl_xor_sync(0xffffffffu, b, o);
-  if (threadIdx.x % 32 == 0) part[0][threadIdx.x / 32] = a, part[1][threadIdx.x / 32] = b;
+  if (lane == 0) total[0][warp] = a, total[1][warp] = b;
   __syncthreads();
   if (threadIdx.x) return;
-  a = b = 0.0;
-  for (int w = 0; w < 32; ++w) a += part[0][w], b += part[1][w];
-  *count = (float)b;
-  if (loss) *loss = (float)(mean ? a / fmax(b, 1.0) : a);
+  for (int w = 1; w < 8; ++w) a += total[0][w], b += total[1][w];
+  *c.count = (float)b;
+  if (c.loss) *c.loss = (float)(c.mean ? a / fmax(b, 1.0) : a);
 }
 
-// scale[0]: what a row's gradient is multiplied by in its slopes, scale[1]: what the sums over slopes are. A row's own gradients go into the
-// slopes, less the largest of them. One block.
-__global__ void __launch_bounds__(1024) k_loss_scale(const float* __restrict__ grad, int64_t grads, const float2* __restrict__ stats, const float* __restrict__ count,
-                                                     int mean, float range, float* scale) {
+// Rows' own gradients go into their slopes, less the largest of them. scale[0]: what they are multiplied by there, scale[1]: what the sums over slopes
+// are. One block.
+__global__ void __launch_bounds__(1024) k_loss_scale(const float* __restrict__ grad, int64_t rows, const float2* __restrict__ stats, float range, float* scale) {
   wait_for_previous();
   __shared__ float part[32];
   float m = 0.0f;
-  if (grads > 1) {
-    for (int64_t i = threadIdx.x; i < grads; i += 1024)
-      if (stats[i].y >= 0.0f || stats[i].y != stats[i].y) m = fmaxf(m, fabsf(grad[i]));
+  for (int64_t i = threadIdx.x; i < rows; i += 1024)
+    if (!(stats[i].y < 0.0f)) m = fmaxf(m, fabsf(grad[i]));
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
-    __syncthreads();
-    for (int w = 0; w < 32; ++w) m = fmaxf(m, part[w]);
-  }
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
+  __syncthreads();
   if (threadIdx.x) return;
-  if (grads > 1) {
-    m = m > 0.0f && m < INFINITY ? fmaxf(m, 1e-30f) : 1.0f;
-    scale[0] = range / m, scale[1] = m / range;
-  } else {
-    scale[0] = range, scale[1] = *grad / (mean ? fmaxf(*count, 1.0f) : 1.0f) / range;
-  }
+  for (int w = 0; w < 32; ++w) m = fmaxf(m, part[w]);
+  m = m > 0.0f && m < INFINITY ? fmaxf(m, 1e-30f) : 1.0f;
+  scale[0] = range / m, scale[1] = m / range;
 }
 
-// dx from its parts: 32 rows and 64 columns a block. WHOLE: rows are whole slices of 8 elements.
+// dx from its parts: 32 rows and 64 columns a block, 16 warps, or twice as many that have every other part. WHOLE: rows are whole slices of 8 elements.
 template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(256) k_loss_grad_rows(const __grid_constant__ GroupedCall c, T* out, int splits) {
+__global__ void __launch_bounds__(1024) k_loss_grad_rows(const __grid_constant__ GroupedCall c, T* out, int splits) {
   wait_for_previous();
   constexpr int kMostN = GroupedTraits<T, kSumX>::kMostN;
-  __shared__ float tile[32][68];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  __shared__ float tile[2][32][68];
+  const int lane = threadIdx.x % 32, quad = threadIdx.x / 32 % 16, team = threadIdx.x / 512, teams = blockDim.x / 512;
   const int64_t row0 = (int64_t)blockIdx.x * 32;
   const int col0 = blockIdx.y * 64;
-  const float scale = c.loss.scale[1];
+  const float scale = sum_scale(c.loss);
   const int tall = c.tile_m * c.halves;
   const int64_t row = row0 + lane;
   const int t = (int)(row / tall), in = (int)(row - (int64_t)t * tall), half = in / kTileM, quarter = in % kTileM / 32;
   const int64_t apart = (int64_t)c.tiles_m * c.tiles_n * c.halves * kTileM * kMostN;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int col = col0 + (warp + 8 * u) * 4, n = col / c.tile_n;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (row < c.rows && col < c.num_n) {
-      const float* const from = c.carry + ((((int64_t)t * c.tiles_n + n) * c.halves + half) * 4 + quarter) * 32 * kMostN + (col - n * c.tile_n) * 32 + in % 32 * 4;
-#pragma unroll 4
-      for (int s = 0; s < splits; ++s) {
-        const float4 p = *(const float4*)(from + s * apart);
-        sum.x += p.x, sum.y += p.y, sum.z += p.z, sum.w += p.w;
-      }
+  const int col = col0 + quad * 4, n = col / c.tile_n;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (row < c.rows && col < c.num_n) {
+    const float* const from = c.carry + ((((int64_t)t * c.tiles_n + n) * c.halves + half) * 4 + quarter) * 32 * kMostN + (col - n * c.tile_n) * 32 + in % 32 * 4;
+#pragma unroll 8
+    for (int s = team; s < splits; s += teams) {
+      const float4 p = *(const float4*)(from + s * apart);
+      sum.x += p.x, sum.y += p.y, sum.z += p.z, sum.w += p.w;
     }
-    *(float4*)&tile[lane][(warp + 8 * u) * 4] = make_float4(sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale);
   }
+  *(float4*)&tile[team][lane][quad * 4] = sum;
   __syncthreads();
   if constexpr (WHOLE) {
-    const int r = threadIdx.x / 8, col = threadIdx.x % 8 * 8;
-    if (row0 + r < c.rows && col0 + col < c.num_n) {
+    if (threadIdx.x >= 256) return;
+    const int r = threadIdx.x / 8, at = threadIdx.x % 8 * 8;
+    if (row0 + r < c.rows && col0 + at < c.num_n) {
       float v[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = tile[r][col + q];
-      T* const to = out + (row0 + r) * c.num_n + col0 + col;
+      for (int q = 0; q < 8; ++q) v[q] = (tile[0][r][at + q] + (teams > 1 ? tile[1][r][at + q] : 0.0f)) * scale;
+      T* const to = out + (row0 + r) * c.num_n + col0 + at;
       if constexpr (sizeof(T) == 2) *(uint4*)to = rounded_slice<T>(v);
       else *(uint4*)to = rounded_slice<T>(v), *(uint4*)(to + 4) = rounded_slice<T>(v + 4);
     }
   } else {
-    for (int i = threadIdx.x; i < 32 * 64; i += 256) {
+    for (int i = threadIdx.x; i < 32 * 64; i += blockDim.x) {
       const int64_t r = row0 + i / 64;
-      const int col = col0 + i % 64;
-      if (r < c.rows && col < c.num_n) out[r * c.num_n + col] = Elem<T>::from_f(tile[i / 64][i % 64]);
+      const int at = i % 64;
+      if (r < c.rows && col0 + at < c.num_n) out[r * c.num_n + col0 + at] = Elem<T>::from_f((tile[0][i / 64][at] + (teams > 1 ? tile[1][i / 64][at] : 0.0f)) * scale);
     }
   }
 }
 
 // db without dW.
 template <typename T>
-__global__ void __launch_bounds__(1024) k_loss_grad_bias(const T* __restrict__ slopes, int64_t rows, int64_t pitch, int classes, const float* __restrict__ scale, T* out) {
+__global__ void __launch_bounds__(1024) k_loss_grad_bias(const T* __restrict__ slopes, int64_t rows, int64_t pitch, int classes, const __grid_constant__ LossCall loss, T* out) {
   wait_for_previous();
   __shared__ float part[32][33];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, v = blockIdx.x * 32 + lane;
@@ -186,7 +182,7 @@ __global__ void __launch_bounds__(1024) k_loss_grad_bias(const T* __restrict__ s
   __syncthreads();
   if (warp == 0 && v < classes) {
     for (int k = 1; k < 32; ++k) sum += part[k][lane];
-    out[v] = Elem<T>::from_f(sum * scale[1]);
+    out[v] = Elem<T>::from_f(sum * sum_scale(loss));
   }
 }
 
@@ -217,9 +213,13 @@ static GroupedCall listed_call(int64_t rows, int64_t n, int64_t k) {
   c.rows = rows, c.groups = 1, c.num_n = (int)n, c.num_k = (int)k, c.halves = c.deep = c.splits = 1;
   c.tile_m = kTileM;
   while (c.tile_m > 16 && c.tile_m >= 2 * rows) c.tile_m /= 2;
-  int64_t tiles_m = ceil_div(rows, c.tile_m), most = Tr::kMostN;
-  if (Tr::kClasses)
-    while (most > 64 && tiles_m * ceil_div(n, most) < kNumSMs) most /= 2;
+  int64_t most = Tr::kMostN;
+  if (Tr::kClasses) {
+    // narrower tiles while there are blocks without one, or shorter ones (the products are of 128 rows always: copies and conversions get fewer)
+    while (most > 64 && ceil_div(rows, c.tile_m) * ceil_div(n, most) < kNumSMs) most /= 2;
+    while (c.tile_m > 16 && 2 * ceil_div(rows, c.tile_m) * ceil_div(n, most) <= kNumSMs) c.tile_m /= 2;
+  }
+  int64_t tiles_m = ceil_div(rows, c.tile_m);
   c.tile_n = tile_columns(n, (int)most), c.tiles_n = (int)ceil_div(n, c.tile_n);
   const int room = kMostShared - grouped_lists<T, MODE>(1) - Tr::kOutWarps * Tr::kStaging;
   const int copied = Tr::kSplit ? Tr::copied(kTileM, Tr::kMnA) : c.tile_m * 128, pieces = Tr::kSplit ? 3 * Tr::piece(kTileM, Tr::kMnA) : 0;
@@ -307,6 +307,7 @@ static int loss_forward(const LossProblem& q, float* loss, float* saved, Arena* 
   float2* const parts = arena->take<float2>(most_parts * pitch);
   float* const picked = arena->take<float>(q.rows);
   float2* const sums = arena->take<float2>(blocks);
+  int* const turn = arena->take<int>(1);
   float* const carry = carry_of<T>(arena, q.dim);
   if (!run) return APT_OK;
   if (copy_x)
@@ -317,15 +318,15 @@ static int loss_forward(const LossProblem& q, float* loss, float* saved, Arena* 
     const int64_t n = std::min(piece, q.classes - v0);
     GroupedCall c = listed_call<T, kStats>(q.rows, n, q.dim);
     c.bias = q.bias ? (const T*)q.bias + v0 : nullptr, c.carry = carry, c.status = q.status;
-    c.loss.labels = q.labels, c.loss.class0 = v0, c.loss.pitch = pitch, c.loss.parts = parts, c.loss.picked = picked;
+    c.loss.labels = q.labels, c.loss.class0 = v0, c.loss.pitch = pitch, c.loss.parts = parts, c.loss.picked = picked, c.loss.turn = turn;
     if (const int e = run_listed<T, kStats>(c, x, some_rows(w, v0, n, sizeof(T)), s)) return e;
     RowsCall r = {};
     r.parts = parts, r.num_parts = c.tiles_n, r.pitch = pitch, r.stats = (float2*)saved, r.picked = picked, r.labels = q.labels;
     r.rows = q.rows, r.classes = q.classes, r.ignore = q.ignore, r.first = v0 == 0, r.last = v0 + n == q.classes;
-    r.losses = q.reduction == APT_LOSS_NONE ? loss : nullptr, r.sums = sums, r.status = q.status;
+    r.losses = q.reduction == APT_LOSS_NONE ? loss : nullptr, r.sums = sums, r.turn = turn, r.status = q.status;
+    r.mean = q.reduction == APT_LOSS_MEAN, r.loss = q.reduction == APT_LOSS_NONE ? nullptr : loss, r.count = saved + 2 * q.rows;
     APT_FOLLOW(k_loss_rows, blocks, 256, 0, s, r);
   }
-  APT_FOLLOW(k_loss_total, 1, 1024, 0, s, sums, blocks, (int)(q.reduction == APT_LOSS_MEAN), q.reduction == APT_LOSS_NONE ? nullptr : loss, saved + 2 * q.rows);
   return APT_OK;
 }
 
@@ -357,20 +358,26 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
   const bool each = q.reduction == APT_LOSS_NONE;
   const float range = std::is_same<T, __half>::value ? 16384.0f : 1.0f;
   // a single row's own gradient is the common one
-  APT_FOLLOW(k_loss_scale, 1, 1024, 0, s, grad, each ? q.rows : 1, (const float2*)saved, saved + 2 * q.rows, (int)(q.reduction == APT_LOSS_MEAN), range, scale);
+  LossCall call = {};
+  call.labels = q.labels, call.pitch = pitch, call.stats = (const float2*)saved, call.range = range;
+  if (each && q.rows > 1) {
+    call.grad = grad, call.scale = scale;
+    APT_FOLLOW(k_loss_scale, 1, 1024, 0, s, grad, q.rows, (const float2*)saved, range, scale);
+  } else {
+    call.common = grad, call.count = q.reduction == APT_LOSS_MEAN ? saved + 2 * q.rows : nullptr;
+  }
   for (int64_t v0 = 0; v0 < q.classes; v0 += piece) {
     const int64_t n = std::min(piece, q.classes - v0);
     const Operand some = some_rows(w, v0, n, sizeof(T));
     GroupedCall c = listed_call<T, kSlopes>(q.rows, n, q.dim);
     c.bias = q.bias ? (const T*)q.bias + v0 : nullptr, c.carry = carry, c.out = slopes, c.status = q.status;
-    c.loss.labels = q.labels, c.loss.class0 = v0, c.loss.pitch = pitch, c.loss.stats = (const float2*)saved, c.loss.scale = scale;
-    c.loss.grad = each && q.rows > 1 ? grad : nullptr;
+    c.loss = call, c.loss.class0 = v0;
     if (const int e = run_listed<T, kSlopes>(c, x, some, s)) return e;
     const Operand dz = {slopes, 0, q.rows, n, pitch};
     if (grad_x) {
       GroupedCall d = sum_x;
       d.num_k = (int)n, d.splits = (int)ceil_div(ceil_div(n, GroupedTraits<T, kSumX>::kBlock * d.deep), d.split_stages);
-      d.status = q.status, d.loss.more = v0 > 0, d.loss.scale = scale, d.out = whole_x ? grad_x : nullptr;
+      d.status = q.status, d.loss = call, d.loss.more = v0 > 0, d.out = whole_x ? grad_x : nullptr;
       if (const int e = run_listed<T, kSumX>(d, dz, some, s)) return e;
     }
     if (grad_weight && tall_weights<T>(q.dim, most)) {
@@ -380,7 +387,7 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
         d.rows = q.rows, d.groups = 1, d.num_m = (int)n, d.num_n = (int)q.dim, d.halves = 2, d.deep = 1;
         d.tile_n = tile_columns(q.dim, Tr::kMostN), d.tiles_m = (int)ceil_div(n, 2 * kTileM), d.tiles_n = (int)ceil_div(q.dim, d.tile_n);
         d.out = (T*)grad_weight + v0 * q.dim, d.grad_bias = grad_bias ? (T*)grad_bias + v0 : nullptr, d.carry = weight_carry, d.status = q.status;
-        d.loss.scale = scale;
+        d.loss = call;
         CUtensorMap a, b;
         if (const int e = make_map(&a, code_of<T>(), dz, Tr::kBox, Tr::kBlock)) return e;
         if (const int e = make_map(&b, code_of<T>(), x, Tr::kBox, Tr::kBlock)) return e;
@@ -392,7 +399,7 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
       d.rows = q.rows, d.groups = 1, d.num_m = (int)n, d.num_n = (int)q.dim;
       d.tile_n = p.tile_n, d.tiles_m = p.tiles_m, d.tiles_n = p.tiles_n, d.ranges = p.ranges;
       d.out = (T*)grad_weight + v0 * q.dim, d.grad_bias = grad_bias ? (T*)grad_bias + v0 : nullptr, d.carry = weight_carry, d.status = q.status;
-      d.plan = plan, d.partial = partial, d.partial_bias = partial_bias, d.loss.scale = scale;
+      d.plan = plan, d.partial = partial, d.partial_bias = partial_bias, d.loss = call;
       using Tr = GroupedTraits<T, kSumW>;
       CUtensorMap a, b;
       if (const int e = make_map(&a, code_of<T>(), dz, Tr::kBox, Tr::kBlock)) return e;
@@ -403,14 +410,14 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
         APT_FOLLOW((k_join_weights<T>), grid, 256, 0, s, d);
       }
     } else if (grad_bias) {
-      APT_FOLLOW((k_loss_grad_bias<T>), ceil_div(n, 32), 1024, 0, s, (const T*)slopes, q.rows, pitch, (int)n, (const float*)scale, (T*)grad_bias + v0);
+      APT_FOLLOW((k_loss_grad_bias<T>), ceil_div(n, 32), 1024, 0, s, (const T*)slopes, q.rows, pitch, (int)n, call, (T*)grad_bias + v0);
     }
   }
   if (grad_x && !whole_x) {
-    sum_x.loss.scale = scale;
+    sum_x.loss = call;
     const dim3 grid((unsigned)ceil_div(q.rows, 32), (unsigned)ceil_div(q.dim, 64));
-    if (q.dim % 8 == 0) APT_FOLLOW((k_loss_grad_rows<T, true>), grid, 256, 0, s, sum_x, (T*)grad_x, splits);
-    else APT_FOLLOW((k_loss_grad_rows<T, false>), grid, 256, 0, s, sum_x, (T*)grad_x, splits);
+    if (q.dim % 8 == 0) APT_FOLLOW((k_loss_grad_rows<T, true>), grid, splits >= 16 ? 1024 : 512, 0, s, sum_x, (T*)grad_x, splits);
+    else APT_FOLLOW((k_loss_grad_rows<T, false>), grid, splits >= 16 ? 1024 : 512, 0, s, sum_x, (T*)grad_x, splits);
   }
   return APT_OK;
 }

@@ -87,7 +87,10 @@ struct LossCall {
   const float* scale;           // [2]: what the rows' gradients are multiplied by, what dx and dw are; null: range and common over it
   const float *common, *count;  // the gradient that all rows have, and what it is divided by (or null)
   float range;
-  int* turn;                    // statistics: set to 0 for the kernel behind
+  int *turn, *dirty;            // statistics: set to 0 for the kernel behind
+  // dW: a row that does not count has slopes of zero, and its own elements are no number: there is a copy of the rows with zeros for those
+  const int* unclean;
+  alignas(64) CUtensorMap clean;
   int more;                     // dx: there are sums of earlier classes
 };
 
@@ -817,7 +820,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
   GroupedWalk<T, MODE> walk(c, prefix, begin);
-  if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *c.loss.turn = 0;
+  if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *c.loss.turn = 0, *c.loss.dirty = 0;
   if (Tr::kOverRows && !Tr::kTall && blockIdx.x == 0 && threadIdx.x == 0) c.plan[0] = walk.runs.units, c.plan[1] = walk.runs.runs;
   GroupedItem item;
   bool fine = true;
@@ -826,6 +829,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (one_of_warp()) {
       int stage = 0, loaded = 0, kept_g = -1, kept_n = -1, kept_times = 0;
       uint32_t phase = 0;
+      const CUtensorMap* const from_b = Tr::kScaled && *c.loss.unclean ? &c.loss.clean : &map_b;
       while (fine && walk.take(&item)) {
         const int boxes_a = Tr::kOverRows ? (min(Tr::kTileA, c.num_m - item.m0) + Tr::kBox - 1) / Tr::kBox : 1;
         const int boxes_b = Tr::kMnB ? (min(c.tile_n, c.num_n - item.n0) + Tr::kBox - 1) / Tr::kBox : 1;
@@ -865,7 +869,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             barrier_expect(bar, bytes);
             const int row = (int)item.row + k * Tr::kBlock;
             for (int i = 0; i < boxes_a; ++i) copy_box(a + i * kBoxBytes, &map_a, item.m0 + i * Tr::kBox, row, bar);
-            for (int i = 0; i < boxes_b; ++i) copy_box(b + i * kBoxBytes, &map_b, item.n0 + i * Tr::kBox, row, bar);
+            for (int i = 0; i < boxes_b; ++i) copy_box(b + i * kBoxBytes, from_b, item.n0 + i * Tr::kBox, row, bar);
           } else {
             const int first = (item.before + k) * c.deep, last = min(first + c.deep, blocks);
             barrier_expect(bar, bytes * (last - first));

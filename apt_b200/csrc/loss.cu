@@ -31,7 +31,7 @@ struct RowsCall {
   int first, last;
   float* losses;                // null: not wanted row by row
   float2* sums;                 // [blocks]: losses and rows that count
-  int* turn;                    // blocks that have theirs there
+  int *turn, *dirty;            // blocks that have theirs there; 1: rows that do not count have logits that are no numbers
   int mean;
   float *loss, *count;          // of all rows; loss null: not wanted
   int32_t* status;
@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(256) k_loss_rows(const __grid_constant__ RowsC
         // against the same number that the sum's exponents refer to, so that a row that is all but sure of its label keeps its digits
         loss = (log2f(s.y) - fmaf(c.picked[row], kLog2e, -s.x)) * kLn2, counts = 1.0f;
       } else {
+        if (!(fabsf(s.x) < INFINITY && s.y < INFINITY)) *c.dirty = 1;
         s.y = -1.0f;
       }
       if (c.losses) c.losses[row] = loss;
@@ -167,6 +168,16 @@ __global__ void __launch_bounds__(1024) k_loss_grad_rows(const __grid_constant__
       if (r < c.rows && col0 + at < c.num_n) out[r * c.num_n + col0 + at] = Elem<T>::from_f((tile[0][i / 64][at] + (teams > 1 ? tile[1][i / 64][at] : 0.0f)) * scale);
     }
   }
+}
+
+// The rows for dW, zeros for those that do not count, where some of these hold what is no number (0 times it would be none either). Nothing is done where
+// none does. Rows of whole 16-byte slices.
+__global__ void __launch_bounds__(256) k_loss_clean(const uint4* __restrict__ x, int64_t rows, int slices, const float2* __restrict__ stats, const int* __restrict__ unclean,
+                                                    uint4* out) {
+  wait_for_previous();
+  if (!*unclean) return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * slices; i += (int64_t)gridDim.x * 256)
+    out[i] = stats[i / slices].y < 0.0f ? make_uint4(0u, 0u, 0u, 0u) : x[i];
 }
 
 // db without dW.
@@ -318,12 +329,12 @@ static int loss_forward(const LossProblem& q, float* loss, float* saved, Arena* 
     const int64_t n = std::min(piece, q.classes - v0);
     GroupedCall c = listed_call<T, kStats>(q.rows, n, q.dim);
     c.bias = q.bias ? (const T*)q.bias + v0 : nullptr, c.carry = carry, c.status = q.status;
-    c.loss.labels = q.labels, c.loss.class0 = v0, c.loss.pitch = pitch, c.loss.parts = parts, c.loss.picked = picked, c.loss.turn = turn;
+    c.loss.labels = q.labels, c.loss.class0 = v0, c.loss.pitch = pitch, c.loss.parts = parts, c.loss.picked = picked, c.loss.turn = turn, c.loss.dirty = (int*)saved + 2 * q.rows + 1;
     if (const int e = run_listed<T, kStats>(c, x, some_rows(w, v0, n, sizeof(T)), s)) return e;
     RowsCall r = {};
     r.parts = parts, r.num_parts = c.tiles_n, r.pitch = pitch, r.stats = (float2*)saved, r.picked = picked, r.labels = q.labels;
     r.rows = q.rows, r.classes = q.classes, r.ignore = q.ignore, r.first = v0 == 0, r.last = v0 + n == q.classes;
-    r.losses = q.reduction == APT_LOSS_NONE ? loss : nullptr, r.sums = sums, r.turn = turn, r.status = q.status;
+    r.losses = q.reduction == APT_LOSS_NONE ? loss : nullptr, r.sums = sums, r.turn = turn, r.dirty = (int*)saved + 2 * q.rows + 1, r.status = q.status;
     r.mean = q.reduction == APT_LOSS_MEAN, r.loss = q.reduction == APT_LOSS_NONE ? nullptr : loss, r.count = saved + 2 * q.rows;
     APT_FOLLOW(k_loss_rows, blocks, 256, 0, s, r);
   }
@@ -340,6 +351,7 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
   T* const slopes = arena->take<T>(q.rows * pitch);
   float* const scale = arena->take<float>(2);
   float* const carry = carry_of<T>(arena, q.dim);
+  void* const clean = arena->take<char>((size_t)q.rows * x.pitch * sizeof(T));
   GroupedCall sum_x = listed_call<T, kSumX>(q.rows, q.dim, most);
   const int splits = sum_x.splits;
   // dx in whole sums: all classes at once, in one part of the contraction
@@ -359,6 +371,15 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
   const float range = std::is_same<T, __half>::value ? 16384.0f : 1.0f;
   // a single row's own gradient is the common one
   LossCall call = {};
+  if (grad_weight) {
+    call.unclean = (const int*)saved + 2 * q.rows + 1;
+    const int slices = (int)(x.pitch * sizeof(T) / 16);
+    APT_FOLLOW(k_loss_clean, wave_grid(ceil_div(q.rows * slices, 256), 8, 1), 256, 0, s, (const uint4*)x.data, q.rows, slices, (const float2*)saved, call.unclean,
+               (uint4*)clean);
+    Operand o = x;
+    o.data = clean;
+    if (const int e = make_map(&call.clean, code_of<T>(), o, GroupedTraits<T, kSumW>::kBox, GroupedTraits<T, kSumW>::kBlock)) return e;
+  }
   call.labels = q.labels, call.pitch = pitch, call.stats = (const float2*)saved, call.range = range;
   if (each && q.rows > 1) {
     call.grad = grad, call.scale = scale;
@@ -457,7 +478,7 @@ extern "C" int apt_linear_cross_entropy_forward(int dtype, const void* x, int64_
   APT_CHECK_ARG((loss || (rows == 0 && reduction == APT_LOSS_NONE)) && saved, "%s: null buffer", who);
   const cudaStream_t s = (cudaStream_t)stream;
   if (rows == 0) {
-    APT_CUDA(cudaMemsetAsync(saved, 0, 4, s));
+    APT_CUDA(cudaMemsetAsync(saved, 0, 8, s));
     if (reduction != APT_LOSS_NONE) APT_CUDA(cudaMemsetAsync(loss, 0, 4, s));
     return APT_OK;
   }

@@ -746,7 +746,7 @@ std::tuple<Tensor, Tensor> loss_forward(const Tensor& x, const Tensor& weight, c
                                         const Tensor& words) {
   const LossProblem q = loss_problem("linear_cross_entropy", x, weight, bias, labels);
   const auto floats = q.x.options().dtype(at::kFloat);
-  Tensor loss = reduction == APT_LOSS_NONE ? at::empty({q.rows}, floats) : at::empty({}, floats), saved = at::empty({2 * q.rows + 1}, floats), ws;
+  Tensor loss = reduction == APT_LOSS_NONE ? at::empty({q.rows}, floats) : at::empty({}, floats), saved = at::empty({2 * q.rows + 2}, floats), ws;
   const size_t bytes = apt_linear_cross_entropy_workspace_bytes(q.code, q.rows, q.dim, q.classes, 0);
   if (bytes) ws = scratch(q.x, bytes);
   check(apt_linear_cross_entropy_forward(q.code, data(q.x), q.rows, q.dim, data(q.weight), data_or_null(q.bias), q.classes, ptr(q.labels), ignore, (int)reduction,
@@ -758,7 +758,7 @@ std::tuple<Tensor, Tensor, Tensor> loss_backward(const Tensor& x, const Tensor& 
   const char* const who = "linear_cross_entropy_backward";
   const LossProblem q = loss_problem(who, x, weight, bias, labels);
   const Tensor saved = cuda(saved_in, "saved", at::kFloat, "torch.float32"), grad = cuda(grad_in, "grad_loss", at::kFloat, "torch.float32");
-  if (saved.numel() != 2 * q.rows + 1) fail(std::string(who) + ": saved is not that of this call");
+  if (saved.numel() != 2 * q.rows + 2) fail(std::string(who) + ": saved is not that of this call");
   if (grad.numel() != (reduction == APT_LOSS_NONE ? q.rows : 1)) fail(std::string(who) + ": grad_loss must be like the loss");
   same_device(who, q.x, saved, "saved");
   same_device(who, q.x, grad, "grad_loss");

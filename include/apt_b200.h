@@ -910,9 +910,10 @@ int apt_expert_sum_backward(int dtype, const void* y, int64_t rows, int64_t dim,
  * [rows], of which `ignore` takes the row out of the loss. Other labels outside [0,
  * classes) set APT_FLAG_ID_OUT_OF_RANGE and take it out too. loss: float [rows]
  * (0 for rows that are out), their sum, or their mean over the rows that count (0
- * where none does). saved [2 rows + 1] is for the backward, which gives grad_x,
+ * where none does). saved [2 rows + 2] is for the backward, which gives grad_x,
  * grad_weight and grad_bias (each unless NULL) for grad_loss [rows] or [1]. Both are
- * NaN where a row that counts has a logit that is NaN or +inf. dim at most
+ * NaN where a row that counts has a logit that is NaN or +inf; rows that are out may
+ * hold anything. dim at most
  * APT_GROUPED_LINEAR_MAX_DIM. The workspace is aligned to 256 bytes. */
 typedef enum apt_loss_reduction { APT_LOSS_NONE = 0, APT_LOSS_SUM = 1, APT_LOSS_MEAN = 2 } apt_loss_reduction;
 size_t apt_linear_cross_entropy_workspace_bytes(int dtype, int64_t rows, int64_t dim, int64_t classes, int backward);

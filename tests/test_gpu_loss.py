@@ -12,6 +12,7 @@ import torch
 
 import apt_b200
 from apt_b200 import _lib, ops
+from apt_b200._lib import check
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -183,6 +184,57 @@ def test_wild_values_stay_in_their_rows(dtype):
     assert torch.equal(gx[fine], want[fine]) and torch.isnan(gx[3]).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim,classes", [(200, 64, 300), (333, 100, 47), (100, 40, 24_000)])
+def test_rows_that_do_not_count_may_hold_anything(rows, dim, classes, dtype):
+    x, w, b, labels = _inputs(rows, dim, classes, dtype)
+    out = labels == IGNORE
+    clean = torch.where(out.unsqueeze(1), 0.0, x.float()).to(dtype)
+
+    def step(x, reduction):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        loss = apt_b200.LinearCrossEntropy.apply(leaves[0], leaves[1], labels, leaves[2], reduction)
+        return (loss.detach(),) + torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+
+    for reduction in ("mean", "none"):
+        want = step(clean, reduction)
+        assert int(out.sum()) > 3 and all(torch.isfinite(t).all() for t in want)
+        for v in (float("nan"), float("inf"), -float("inf")):
+            wild = x.clone()
+            wild[out, 3:] = v
+            assert all(torch.equal(a, b) for a, b in zip(step(wild, reduction), want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("polls", [0, 1, 6, 50])
+@pytest.mark.parametrize("rows,dim,classes", [(300, 128, 700), (3000, 64, 1500), (700, 1024, 25_000)])
+def test_the_kernels_end_when_a_wait_runs_out(rows, dim, classes, dtype, polls):
+    x, w, b, labels = _inputs(rows, dim, classes, dtype)
+    saved = apt_b200.linear_cross_entropy(x, w, labels, b, return_saved=True)[1]
+    grad = torch.ones((), device="cuda")
+
+    def call():
+        return (apt_b200.linear_cross_entropy(x, w, labels, b),) + apt_b200.linear_cross_entropy_backward(x, w, labels, saved, grad, b)
+
+    want = call()
+    ops.check_status()
+    check(_lib.lib.apt_set_tunable(b"bulk_wait_polls", polls))
+    try:
+        got = call()
+        torch.cuda.synchronize()
+    finally:
+        check(_lib.lib.apt_set_tunable(b"bulk_wait_polls", 1 << 20))
+    flagged = False
+    try:
+        ops.check_status()
+    except RuntimeError as e:
+        assert "did not reach shared memory" in str(e)
+        flagged = True
+    assert flagged or (polls > 0 and all(torch.equal(a, b) for a, b in zip(got, want)))
+    assert all(torch.equal(a, b) for a, b in zip(call(), want))
+    ops.check_status()
+
+
 def test_small_gradients_of_f16_are_numbers():
     """A mean over many rows makes slopes of 1e-9, below f16's smallest number: they are held times the common factor."""
     x, w, b, labels = _inputs(4096, 32, 3000, torch.float16, scale=0.5, ignored=0.0)
@@ -319,6 +371,6 @@ def test_refusals():
             (lambda: apt_b200.linear_cross_entropy(x, w.cpu(), labels), "CUDA tensor"), (lambda: apt_b200.linear_cross_entropy(x, w[:0], labels), "0 classes"),
             (lambda: apt_b200.linear_cross_entropy(torch.zeros((2, 8200), device="cuda"), torch.zeros((3, 8200), device="cuda"), labels[:2]), "rows of 8200"),
             (lambda: apt_b200.linear_cross_entropy_backward(x, w, labels, torch.zeros(5, device="cuda"), torch.zeros((), device="cuda")), "saved"),
-            (lambda: apt_b200.linear_cross_entropy_backward(x, w, labels, torch.zeros(19, device="cuda"), torch.zeros(9, device="cuda")), "like the loss")]:
+            (lambda: apt_b200.linear_cross_entropy_backward(x, w, labels, torch.zeros(20, device="cuda"), torch.zeros(9, device="cuda")), "like the loss")]:
         with pytest.raises((RuntimeError, _lib.AptError), match=text):
             call()

@@ -209,6 +209,19 @@ __device__ __forceinline__ Pairs<U> load_pairs(const SumCall& c, int64_t r, int 
   return p;
 }
 
+// A slice that is read once: not kept in L1.
+template <typename T, int VE>
+__device__ __forceinline__ Raw<T, VE> load_once(const T* p) {
+  if constexpr (sizeof(T) * VE == 16) {
+    const uint4 u = ld_stream_16(p);
+    Raw<T, VE> r;
+    r.w[0] = u.x, r.w[1] = u.y, r.w[2] = u.z, r.w[3] = u.w;
+    return r;
+  } else {
+    return load_raw<T, VE>(p);
+  }
+}
+
 // 151552 rows of 256 bf16, two of 16 experts: 48 us with weights, 49 without (HBM: 36); four pairs at once of two rows 49 and 51, the next row's
 // places asked for a row ahead, which spilled, 78.
 template <typename T, int VE, int U>
@@ -233,7 +246,7 @@ __global__ void __launch_bounds__(256, U == 4 ? 5 : 6) k_expert_sum(const __grid
         for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int i = 0; i < D; ++i)
-            if (p.at[u] >= 0 && d0 + i * apart < c.dim) v[u][i] = load_raw<T, VE>(y + (int64_t)p.at[u] * c.dim + d0 + i * apart);
+            if (p.at[u] >= 0 && d0 + i * apart < c.dim) v[u][i] = load_once<T, VE>(y + (int64_t)p.at[u] * c.dim + d0 + i * apart);
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (p.at[u] >= 0)
@@ -273,7 +286,7 @@ __global__ void __launch_bounds__(256, U == 4 || VE == 1 ? 4 : 5) k_expert_sum_b
           for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < D; ++i)
-              if (p.at[u] >= 0 && y && d0 + i * apart < c.dim) v[u][i] = load_raw<T, VE>(y + (int64_t)p.at[u] * c.dim + d0 + i * apart);
+              if (p.at[u] >= 0 && y && d0 + i * apart < c.dim) v[u][i] = load_once<T, VE>(y + (int64_t)p.at[u] * c.dim + d0 + i * apart);
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             if (p.at[u] == kNowhere) continue;

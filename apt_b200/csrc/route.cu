@@ -8,7 +8,7 @@
 //   divided by the sum, p = w / scale:  p_e (g_e - sum_j g_j p_j), times (1 - s_e) for the logistic; 0 where e is not chosen
 //
 // A team of lanes has a row, NV neighbouring experts a lane, in registers; lanes and slots ascend with the experts. The k-th largest of the
-// lanes' own largest is a bound below which nothing is chosen: what is not below it (of rows over 256 experts some ten) goes to shared memory, where
+// lanes' own largest (of their two largest each, where lanes are few) is a bound below which nothing is chosen: what is not below it (some ten) goes to shared memory, where
 // every candidate finds its place by counting those in front of it. An expert whose logit is -inf is never chosen: where fewer are left than k, the
 // others are -1 with weight 0.
 //
@@ -33,6 +33,7 @@ struct RouteCall {
   int experts, k, groups, per, top_groups, best;      // per: experts of a group
   int group_lanes, team_lanes;                        // logarithms
   int sigmoid, renorm;
+  int whole_bias;
   int whole;                                          // a lane's experts are there, all or none, and may be read in slices
   int found;                                          // places for candidates
   float scale;
@@ -114,22 +115,31 @@ template <int NV>
 __device__ __forceinline__ bool take_best(const RouteCall& r, const Team& team, uint32_t (&key)[NV], uint64_t* found, uint64_t* best, int wanted) {
   const int base = (team.lane >> r.group_lanes) * r.per + (team.lane & ((1 << r.group_lanes) - 1)) * NV, lanes = 1 << r.team_lanes;
   const auto entry = [&](int i) { return (uint64_t)key[i] << 32 | (uint32_t)~(base + i); };
-  uint32_t mine = 0;
+  uint32_t one = 0, two = 0, bound = 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) mine = max(mine, key[i]);
-  uint32_t bound = 0;
+  for (int i = 0; i < NV; ++i) two = max(two, min(one, key[i])), one = max(one, key[i]);
   if (r.team_lanes == 5) {      // (equal ones go together: the bound is lower then, and holds as well)
     for (int j = 0; j < wanted; ++j) {
-      bound = __reduce_max_sync(0xffffffffu, mine);
-      if (mine == bound) mine = 0;
+      bound = __reduce_max_sync(0xffffffffu, one);
+      if (one == bound) one = 0;
     }
-  } else if (wanted <= lanes) {
+  } else if (r.team_lanes == 4 && wanted <= lanes) {
     int above = 0;
     for (int l = 0; l < lanes; ++l) {
-      const uint32_t other = __shfl_sync(0xffffffffu, mine, team.first + l);
-      above += other > mine || (other == mine && l < team.lane);
+      const uint32_t other = __shfl_sync(0xffffffffu, one, team.first + l);
+      above += other > one || (other == one && l < team.lane);
     }
-    bound = __shfl_sync(0xffffffffu, mine, team.first + __ffs(team.votes(above == wanted - 1)) - 1);
+    bound = __shfl_sync(0xffffffffu, one, team.first + __ffs(team.votes(above == wanted - 1)) - 1);
+  } else if (wanted <= 2 * lanes) {      // few lanes: by their two largest
+    int above_one = 0, above_two = 0;
+    for (int l = 0; l < lanes; ++l) {
+      const uint32_t a = __shfl_sync(0xffffffffu, one, team.first + l), b = __shfl_sync(0xffffffffu, two, team.first + l);
+      const bool before = l < team.lane;
+      above_one += (a > one || (a == one && before)) + (b > one || (b == one && before));
+      above_two += (a > two || (a == two && l <= team.lane)) + (b > two || (b == two && before));
+    }
+    const unsigned first = team.votes(above_one == wanted - 1), second = team.votes(above_two == wanted - 1);
+    bound = __shfl_sync(0xffffffffu, first ? one : two, team.first + __ffs(first ? first : second) - 1);
   }
   bound = max(bound, 1u);
   // where a lane's candidates go: the lanes' numbers of them, bit by bit
@@ -307,14 +317,25 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
   bool again = false, stays = true;
   float slack = 0.0f;
   if constexpr (EXACT) {
-    float s[NV];
+    float s[NV], b[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i += 4) {
+      if (!r.bias) {
+        b[i] = b[i + 1] = b[i + 2] = b[i + 3] = 0.0f;
+      } else if (r.whole_bias) {
+        const float4 v = base < end ? *(const float4*)(r.bias + base + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        b[i] = v.x, b[i + 1] = v.y, b[i + 2] = v.z, b[i + 3] = v.w;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) b[i + q] = base + i + q < end ? r.bias[base + i + q] : 0.0f;
+      }
+    }
     const float by = r.sigmoid ? 1.0f : 1.0f / sum;      // the largest score there can be
     slack = 0x1p-18f * by;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const bool there = z[i] != -INFINITY;
-      s[i] = there ? (r.sigmoid ? logistic(z[i]) : exp_short(z[i] - top) * by) : -INFINITY;
-      if (r.bias && there) s[i] += r.bias[base + i];
+      s[i] = there ? (r.sigmoid ? logistic(z[i]) : exp_short(z[i] - top) * by) + b[i] : -INFINITY;
     }
     if constexpr (GROUPS) stays = group_stays<NV>(r, team, s, slack, &again);
 #pragma unroll
@@ -465,9 +486,9 @@ __global__ void __launch_bounds__(kRouteThreads) k_route_backward(const __grid_c
 
 // ---- host side -----------------------------------------------------------------------
 // Experts a lane and lanes. What a row costs whatever it holds (bound, places, weights: some 400 instructions) several rows share in a warp that has
-// more experts a lane; but the bound comes of twice as many lanes as are chosen, or it is too low and there are too many candidates. So 16 experts a
-// lane where that leaves lanes enough, of the groups that stay, else eight; or the fewest with which the groups, each in lanes of its own, a power of two
-// of them, fit a warp.
+// more experts a lane; but a bound that comes of too few of the lanes' largest is too low, and there are too many candidates. So 16 experts a lane where
+// that leaves lanes enough, of the groups that stay, else eight; or the fewest with which the groups, each in lanes of its own, a power of two of them,
+// fit a warp.
 static int route_plan(RouteCall* r) {
   const auto lay_out = [r](int nv) {
     r->group_lanes = 0;
@@ -503,6 +524,7 @@ static int route(RouteCall r, cudaStream_t s) {
   const int nv = route_plan(&r);
   r.found = (std::min(r.experts, kRouteFound) + 2) / 2 * 2;
   r.whole = r.per % nv == 0 && r.experts * sizeof(T) % 16 == 0 && (uintptr_t)r.logits % 16 == 0;
+  r.whole_bias = r.per % nv == 0 && (uintptr_t)r.bias % 16 == 0;
   if (nv == 8) return launch_route<T, 8>(r, s);
   if (nv == 16) return launch_route<T, 16>(r, s);
   if (nv == 32) return launch_route<T, 32>(r, s);

@@ -12,12 +12,12 @@
 // every candidate finds its place by counting those in front of it. An expert whose logit is -inf is never chosen: where fewer are left than k, the
 // others are -1 with weight 0.
 //
-// Ranks are those of the exact scores. Without a bias logits are compared as they are. Scores in 32 bits are off by less than 2^-19 of the
-// row's largest: the argument's rounding, 2^-23 of |z| exp(-|z|), exp, reciprocal and quotient by two units in the last place each, a sum of 1024 in ten
-// steps and eight. Their sum with the bias is off by 2^-24 of itself. Where two that were taken one behind the other, or the last one and the
-// next, are nearer than both errors, the row is done again in 64 bits, by a warp for itself (route_again); of rows over 256 experts one in a
-// hundred.
-//
+// Ranks are those of the exact scores. Without a bias logits are compared as they are. In 32 bits two logistic scores differ by less than 2^-20.9 from
+// what they should: s (1 - s) (2^-24 |z| + 2^-22) for the rounded argument and the exponential, and three quarters of 2^-22 s for sum and reciprocal, twice. Two
+// of a softmax by less than 2^-18.4 of the row's largest: 2^-21.2 each (2^-23 |d| exp(-|d|) for the differences' rounding, 2^-22 and 2^-23 for exponential
+// and product), and the sum of up to 1024 exponentials, 2^-18.9, which all scores share. Their sum with the bias is off by 2^-24 of itself. Where
+// two that are taken one behind the other, or the last one and the next, are nearer than 2^-20 (2^-18 of the largest) and 2^-22 of their size, the row is
+// done again in 64 bits, by a warp for itself (route_again); of rows over 256 experts one in two hundred.
 #include <algorithm>
 
 #include "dense.cuh"
@@ -216,29 +216,32 @@ __device__ __forceinline__ void row_softmax(const float (&z)[NV], int lanes, flo
   *top = m, *sum = team_sum(s, lanes);
 }
 
-// A row's picks in 64 bits, by a warp: what experts are ranked by lies in shared memory, 32 neighbours at a time. Nothing is unrolled: few rows come
-// here, and the instructions would be in every row's way.
+// A row's picks in 64 bits, by a warp: what experts are ranked by lies in shared memory, 32 neighbours at a time. Few rows come here, and the
+// last of them is what a call waits for.
 template <typename T>
 __device__ __noinline__ void route_again(const RouteCall& r, const T* row, double* c, uint64_t* picks) {
   const int lane = threadIdx.x % 32;
   const bool scores = r.bias || r.groups > 1;
-  double total = 1.0, top = 0.0;
+  double top = 0.0;
   if (!r.sigmoid && scores) {
     float m = -INFINITY;
     for (int e = lane; e < r.experts; e += 32) m = fmaxf(m, Elem<T>::to_f(row[e]));
     m = team_most(m, 5);
-    top = m == -INFINITY ? 0.0 : (double)m, total = 0.0;
-    for (int e = lane; e < r.experts; e += 32) total += exp((double)Elem<T>::to_f(row[e]) - top);
-    total = team_sum(total, 5);
+    top = m == -INFINITY ? 0.0 : (double)m;
   }
-  for (int e = lane; e < r.experts; e += 32) {
-    const double z = (double)Elem<T>::to_f(row[e]);
-    double v = z;
-    if (scores && z != -INFINITY && (r.bias || r.best == 2)) {
-      v = r.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - top) / total;
-      if (r.bias) v += r.bias[e];
+  if (!scores || (!r.bias && r.best == 1)) {
+    for (int e = lane; e < r.experts; e += 32) c[e] = (double)Elem<T>::to_f(row[e]);
+  } else {
+    // four at once: an exponential in 64 bits is a chain of some forty steps
+    double total = 0.0;
+#pragma unroll 4
+    for (int e = lane; e < r.experts; e += 32) {
+      const double z = (double)Elem<T>::to_f(row[e]), v = r.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - top);
+      c[e] = v, total += v;
     }
-    c[e] = v;
+    total = r.sigmoid ? 1.0 : team_sum(total, 5);
+#pragma unroll 4
+    for (int e = lane; e < r.experts; e += 32) c[e] = Elem<T>::to_f(row[e]) == -INFINITY ? -INFINITY : (r.sigmoid ? c[e] : c[e] / total) + (r.bias ? (double)r.bias[e] : 0.0);
   }
   __syncwarp();
   // (a, its place) is in front of (b, its place)
@@ -263,9 +266,9 @@ __device__ __noinline__ void route_again(const RouteCall& r, const T* row, doubl
   for (int j = 0; j < r.k; ++j) {
     double best = -INFINITY;
     int at = r.experts;
+#pragma unroll 4
     for (int e = lane; e < r.experts; e += 32)
       if (c[e] != -INFINITY && before(c[e], e, best, at)) best = c[e], at = e;
-#pragma unroll 1
     for (int o = 16; o; o >>= 1) {
       const double b = __shfl_xor_sync(0xffffffffu, best, o);
       const int i = __shfl_xor_sync(0xffffffffu, at, o);
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
       }
     }
     const float by = r.sigmoid ? 1.0f : 1.0f / sum;      // the largest score there can be
-    slack = 0x1p-18f * by;
+    slack = r.sigmoid ? 0x1p-20f : 0x1p-18f * by;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const bool there = z[i] != -INFINITY;

@@ -8,8 +8,9 @@
 //   divided by the sum, p = w / scale:  p_e (g_e - sum_j g_j p_j), times (1 - s_e) for the logistic; 0 where e is not chosen
 //
 // A team of lanes has a row, NV neighbouring experts a lane, in registers; lanes and slots ascend with the experts. The k-th largest of the
-// lanes' own largest (of their two largest each, where lanes are few) is a bound below which nothing is chosen: what is not below it (some ten) goes to shared memory, where
-// every candidate finds its place by counting those in front of it. An expert whose logit is -inf is never chosen: where fewer are left than k, the
+// lanes' own largest (of their two largest each, where lanes are few) is a bound below which nothing is chosen: what is not below it (some ten) goes to
+// shared memory, where every candidate finds its place by counting those in front of it. Where there is no room for as many (very many that are equal, or
+// more wanted than there are lanes) the bound is raised by halves first. An expert whose logit is -inf is never chosen: where fewer are left than k, the
 // others are -1 with weight 0.
 //
 // Ranks are those of the exact scores. Without a bias logits are compared as they are. In 32 bits two logistic scores differ by less than 2^-20.9 from
@@ -17,14 +18,15 @@
 // of a softmax by less than 2^-18.4 of the row's largest: 2^-21.2 each (2^-23 |d| exp(-|d|) for the differences' rounding, 2^-22 and 2^-23 for exponential
 // and product), and the sum of up to 1024 exponentials, 2^-18.9, which all scores share. Their sum with the bias is off by 2^-24 of itself. Where
 // two that are taken one behind the other, or the last one and the next, are nearer than 2^-20 (2^-18 of the largest) and 2^-22 of their size, the row is
-// done again in 64 bits, by a warp for itself (route_again); of rows over 256 experts one in two hundred.
+// done again in 64 bits, by a warp for itself (route_again): of rows over 256 experts one in two hundred. Not where both have the same logit and the same bias,
+// and so the same score: with a bias of zeros and logits of 16 bits that are two rows in five (67584 over 256: 266 us with them, 70 without).
 #include <algorithm>
 
 #include "dense.cuh"
 
 namespace apt {
 
-constexpr int kRouteThreads = 128, kRouteFound = 64;
+constexpr int kRouteThreads = 128, kRouteFound = APT_ROUTE_MAX_CHOSEN + 2;
 
 struct RouteCall {
   const void* logits;
@@ -46,7 +48,7 @@ struct RouteCall {
 // Numbers as unsigned ones of the same order; 0: not to be had. NaN is above all others.
 __device__ __forceinline__ uint32_t rank_of(float v) {
   const uint32_t u = __float_as_uint(v + 0.0f);      // -0 is 0
-  return v != v ? 0xffffffffu : v == -INFINITY ? 0u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return v != v ? 0xfffffffeu : v == -INFINITY ? 0u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float number_of(uint32_t r) { return __uint_as_float(r ^ (r >> 31 ? 0x80000000u : 0xffffffffu)); }
 
@@ -109,17 +111,64 @@ __device__ __forceinline__ bool group_stays(const RouteCall& r, const Team& team
   return stays;
 }
 
+// The sum of the numbers of the team's lanes below, and of all, bit by bit; numbers to 2^BITS - 1.
+template <int BITS>
+__device__ __forceinline__ int lanes_below(const Team& team, int own, int* all) {
+  int below = 0, count = 0;
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
+    const unsigned who = team.votes(own >> b & 1);
+    below += __popc(who & ((1u << team.lane) - 1)) << b, count += __popc(who) << b;
+  }
+  *all = count;
+  return below;
+}
+
+// The bound raised, by halves, until no more keys are not below it than there are places for, and `wanted` still are. Where that many are equal, those
+// behind the first ones that are wanted go below it.
+template <int NV, int BITS>
+__device__ __forceinline__ uint32_t raise_bound(const Team& team, uint32_t (&key)[NV], uint32_t low, bool over, int wanted) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) most = max(most, key[i]);
+  uint32_t high = team_most(most, team.lanes) + 1;
+  const uint32_t least = team_least(most ? most : high, team.lanes);
+  const int have = __popc(team.votes(most != 0));
+  if (over && have >= wanted) low = max(low, least);
+  int above = 0;      // keys that are not below `high`
+  while (__any_sync(0xffffffffu, over && high - low > 1)) {
+    const uint32_t middle = low + (high - low) / 2;
+    int own = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) own += key[i] >= middle;
+    const int count = team_sum(own, team.lanes);
+    if (over && high - low > 1) {
+      if (count >= wanted) low = middle, over = count > kRouteFound;
+      else high = middle, above = count;
+    }
+  }
+  if (__any_sync(0xffffffffu, over)) {
+    int own = 0, all;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) own += key[i] == low;
+    int at = above + lanes_below<BITS>(team, own, &all);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (over && key[i] == low && at++ >= wanted) --key[i];
+  }
+  return low;
+}
+
 // The largest keys, largest first and of equal ones the lowest expert's, to best[0 .. wanted): (key, complement of the expert), 0 where there is none.
-// False: very many that are equal, or more wanted than there are lanes, and so more candidates than there are places.
 template <int NV>
-__device__ __forceinline__ bool take_best(const RouteCall& r, const Team& team, uint32_t (&key)[NV], uint64_t* found, uint64_t* best, int wanted) {
+__device__ __forceinline__ void take_best(const RouteCall& r, const Team& team, uint32_t (&key)[NV], uint64_t* found, uint64_t* best, int wanted) {
   const int base = (team.lane >> r.group_lanes) * r.per + (team.lane & ((1 << r.group_lanes) - 1)) * NV, lanes = 1 << r.team_lanes;
   const auto entry = [&](int i) { return (uint64_t)key[i] << 32 | (uint32_t)~(base + i); };
   uint32_t one = 0, two = 0, bound = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) two = max(two, min(one, key[i])), one = max(one, key[i]);
   if (r.team_lanes == 5) {      // (equal ones go together: the bound is lower then, and holds as well)
-    for (int j = 0; j < wanted; ++j) {
+    for (int j = 0; j < wanted && wanted <= lanes; ++j) {
       bound = __reduce_max_sync(0xffffffffu, one);
       if (one == bound) one = 0;
     }
@@ -142,43 +191,43 @@ __device__ __forceinline__ bool take_best(const RouteCall& r, const Team& team, 
     bound = __shfl_sync(0xffffffffu, first ? one : two, team.first + __ffs(first ? first : second) - 1);
   }
   bound = max(bound, 1u);
-  // where a lane's candidates go: the lanes' numbers of them, bit by bit
-  uint32_t which = 0;
-#pragma unroll
-  for (int i = 0; i < NV && i < 32; ++i) which |= (uint32_t)(key[i] >= bound) << i;
-  int own = __popc(which);
-  if constexpr (NV > 32) {
-#pragma unroll
-    for (int i = 32; i < NV; ++i) own += key[i] >= bound;
-  }
-  int at = 0, count = 0;
+  // where a lane's candidates go
   constexpr int kBits = NV == 8 ? 4 : NV == 16 ? 5 : NV == 32 ? 6 : 7;
+  int own, at, count;
+  const auto tally = [&] {
+    uint32_t which = 0;
 #pragma unroll
-  for (int b = 0; b < kBits; ++b) {
-    const unsigned all = team.votes(own >> b & 1);
-    at += __popc(all & ((1u << team.lane) - 1)) << b, count += __popc(all) << b;
+    for (int i = 0; i < NV && i < 32; ++i) which |= (uint32_t)(key[i] >= bound) << i;
+    own = __popc(which);
+    if constexpr (NV > 32) {
+#pragma unroll
+      for (int i = 32; i < NV; ++i) own += key[i] >= bound;
+    }
+    at = lanes_below<kBits>(team, own, &count);
+  };
+  tally();
+  if (__any_sync(0xffffffffu, count > kRouteFound)) {
+    bound = raise_bound<NV, kBits>(team, key, bound, count > kRouteFound, wanted);
+    tally();
   }
-  if (own && count <= kRouteFound) {
+  if (own) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (key[i] >= bound) found[at++] = entry(i);
   }
   for (int j = team.lane; j < wanted; j += lanes) best[j] = 0;
-  if (team.lane == 0 && count <= kRouteFound) found[count] = 0;      // two are read at once
+  if (team.lane == 0) found[count] = 0;      // two are read at once
   __syncwarp();
-  if (count <= kRouteFound) {
-    for (int p = team.lane; p < count; p += lanes) {
-      const uint64_t me = found[p];
-      int place = 0;
-      for (int q = 0; q < count; q += 2) {
-        const ulonglong2 two = *(const ulonglong2*)(found + q);
-        place += (two.x > me) + (two.y > me);
-      }
-      if (place < wanted) best[place] = me;
+  for (int p = team.lane; p < count; p += lanes) {
+    const uint64_t me = found[p];
+    int place = 0;
+    for (int q = 0; q < count; q += 2) {
+      const ulonglong2 two = *(const ulonglong2*)(found + q);
+      place += (two.x > me) + (two.y > me);
     }
+    if (place < wanted) best[place] = me;
   }
   __syncwarp();
-  return count <= kRouteFound;
 }
 
 // The logits of a lane's experts; -inf for those that are not there.
@@ -216,33 +265,45 @@ __device__ __forceinline__ void row_softmax(const float (&z)[NV], int lanes, flo
   *top = m, *sum = team_sum(s, lanes);
 }
 
+// Of a row whose last pick and the next are ranked by the same logit and bias: whether another is near them, that is not. top, by: of its softmax. A warp's.
+template <typename T>
+__device__ __noinline__ bool others_near(const RouteCall& r, const T* row, uint64_t last, float top, float by, float slack) {
+  bool near = false;
+  const int at = ~(uint32_t)last;
+  const float z = Elem<T>::to_f(row[at]), b = r.bias[at], score = number_of((uint32_t)(last >> 32));
+  for (int e = threadIdx.x % 32; e < r.experts; e += 32) {
+    const float v = Elem<T>::to_f(row[e]), s = (r.sigmoid ? logistic(v) : exp_short(v - top) * by) + r.bias[e];
+    near |= s <= score && too_near(score, s, slack) && !(v == z && r.bias[e] == b);
+  }
+  return __any_sync(0xffffffffu, near);
+}
+
 // A row's picks in 64 bits, by a warp: what experts are ranked by lies in shared memory, 32 neighbours at a time. Few rows come here, and the
 // last of them is what a call waits for.
 template <typename T>
 __device__ __noinline__ void route_again(const RouteCall& r, const T* row, double* c, uint64_t* picks) {
   const int lane = threadIdx.x % 32;
-  const bool scores = r.bias || r.groups > 1;
+  // padding, say: all logits and biases the same, and the picks are right
+  bool equal = true;
+  for (int e = lane; e < r.experts; e += 32) equal &= Elem<T>::to_f(row[e]) == Elem<T>::to_f(row[0]) && (!r.bias || r.bias[e] == r.bias[0]);
+  if (__all_sync(0xffffffffu, equal)) return;
   double top = 0.0;
-  if (!r.sigmoid && scores) {
+  if (!r.sigmoid) {
     float m = -INFINITY;
     for (int e = lane; e < r.experts; e += 32) m = fmaxf(m, Elem<T>::to_f(row[e]));
     m = team_most(m, 5);
     top = m == -INFINITY ? 0.0 : (double)m;
   }
-  if (!scores || (!r.bias && r.best == 1)) {
-    for (int e = lane; e < r.experts; e += 32) c[e] = (double)Elem<T>::to_f(row[e]);
-  } else {
-    // four at once: an exponential in 64 bits is a chain of some forty steps
-    double total = 0.0;
+  // four at once: an exponential in 64 bits is a chain of some forty steps
+  double total = 0.0;
 #pragma unroll 4
-    for (int e = lane; e < r.experts; e += 32) {
-      const double z = (double)Elem<T>::to_f(row[e]), v = r.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - top);
-      c[e] = v, total += v;
-    }
-    total = r.sigmoid ? 1.0 : team_sum(total, 5);
-#pragma unroll 4
-    for (int e = lane; e < r.experts; e += 32) c[e] = Elem<T>::to_f(row[e]) == -INFINITY ? -INFINITY : (r.sigmoid ? c[e] : c[e] / total) + (r.bias ? (double)r.bias[e] : 0.0);
+  for (int e = lane; e < r.experts; e += 32) {
+    const double z = (double)Elem<T>::to_f(row[e]), v = r.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - top);
+    c[e] = v, total += v;
   }
+  total = r.sigmoid ? 1.0 : team_sum(total, 5);
+#pragma unroll 4
+  for (int e = lane; e < r.experts; e += 32) c[e] = Elem<T>::to_f(row[e]) == -INFINITY ? -INFINITY : (r.sigmoid ? c[e] : c[e] / total) + (r.bias ? (double)r.bias[e] : 0.0);
   __syncwarp();
   // (a, its place) is in front of (b, its place)
   const auto before = [](double a, int i, double b, int j) { return b != b ? a != a && i < j : a != a || a > b || (a == b && i < j); };
@@ -295,9 +356,9 @@ __device__ __noinline__ void weights_by_logarithms(const RouteCall& r, const T* 
   for (int j = 0; j < r.k; ++j) to[j] = best[j] ? r.scale * (expf(value(j) - m) / total) : 0.0f;
 }
 
-// 67584 rows over 256 experts in eight groups, logistic with a bias, fp32: 104 us (reading 69 MB: 11), without groups and bias 42; 151552 over 64, softmax,
-// bf16: 39 (6). Instructions bound it, 80 per cent of the issue slots: 1230 a row of the first, 560 of the second. EXACT: ranks are those of scores, not of
-// the logits.
+// 67584 rows over 256 experts in eight groups, logistic with a bias, fp32: 112 us (reading 69 MB: 11), without groups and bias 45; 151552 over 64, softmax,
+// bf16: 37 (6). Instructions bound it, 84 per cent of the issue slots: 1300 a row of the first, 560 of the second. 64 of 256: 177; rows whose logits are all the same,
+// eight of 256: 54. EXACT: ranks are those of scores, not of the logits.
 template <typename T, int NV, bool GROUPS, bool EXACT>
 __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__ RouteCall r) {
   wait_for_previous();
@@ -318,7 +379,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
   if (!r.sigmoid && (EXACT || !r.renorm)) row_softmax(z, r.team_lanes, &top, &sum);
   uint32_t key[NV];
   bool again = false, stays = true;
-  float slack = 0.0f;
+  float slack = 0.0f, by = 1.0f;      // by: the largest score there can be
   if constexpr (EXACT) {
     float s[NV], b[NV];
 #pragma unroll
@@ -333,7 +394,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
         for (int q = 0; q < 4; ++q) b[i + q] = base + i + q < end ? r.bias[base + i + q] : 0.0f;
       }
     }
-    const float by = r.sigmoid ? 1.0f : 1.0f / sum;      // the largest score there can be
+    by = r.sigmoid ? 1.0f : 1.0f / sum;
     slack = r.sigmoid ? 0x1p-20f : 0x1p-18f * by;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -349,21 +410,33 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
     for (int i = 0; i < NV; ++i) key[i] = stays ? rank_of(z[i]) : 0;
   }
   // (one more for what the last one is compared with)
-  again |= !take_best<NV>(r, team, key, found, best, r.k + (EXACT ? 1 : 0));
-  if (EXACT && r.bias)
-    for (int j = team.lane; j < r.k; j += lanes) {
-      const uint32_t mine = (uint32_t)(best[j] >> 32), next = (uint32_t)(best[j + 1] >> 32);
-      again |= next && too_near(number_of(mine), number_of(next), slack);
-    }
-  const unsigned who = __ballot_sync(0xffffffffu, again && alive);
-  if (who)
-    for (int first = 0; first < 32; first += lanes)
-      if (who >> first & (lanes == 32 ? ~0u : (1u << lanes) - 1)) {
-        const int n = (threadIdx.x / 32 * 32 + first) >> r.team_lanes;
-        route_again<T>(r, (const T*)r.logits + ((int64_t)blockIdx.x * teams + n) * r.experts, (double*)(room + teams * (r.found + r.k + 1)) + threadIdx.x / 32 * r.experts,
-                       room + teams * r.found + n * (r.k + 1));
+  take_best<NV>(r, team, key, found, best, r.k + (EXACT ? 1 : 0));
+  if constexpr (EXACT) {
+    bool open = false;
+    if (r.bias) {
+      // what is ranked by the same logit and bias has the same score, and is in its place; if the last one and the next are, what follows may be near both
+      const auto same = [&](int e, int f) { return Elem<T>::to_f(from[e]) == Elem<T>::to_f(from[f]) && r.bias[e] == r.bias[f]; };
+      for (int j = team.lane; j < r.k; j += lanes) {
+        const uint64_t mine = best[j], next = best[j + 1];
+        if (next && too_near(number_of((uint32_t)(mine >> 32)), number_of((uint32_t)(next >> 32)), slack)) {
+          if (!same(~(uint32_t)mine, ~(uint32_t)next)) again = true;
+          else open |= j == r.k - 1;
+        }
       }
-  __syncwarp();
+    }
+    const unsigned redo = __ballot_sync(0xffffffffu, again && alive), ask = __ballot_sync(0xffffffffu, open && alive);
+    if (redo | ask)
+      for (int first = 0; first < 32; first += lanes) {
+        const unsigned team_of = (lanes == 32 ? ~0u : (1u << lanes) - 1) << first;
+        const int n = (threadIdx.x / 32 * 32 + first) >> r.team_lanes;
+        const T* const row = (const T*)r.logits + ((int64_t)blockIdx.x * teams + n) * r.experts;
+        uint64_t* const picks = room + teams * r.found + n * (r.k + 1);
+        const float s = __shfl_sync(0xffffffffu, slack, first), t = __shfl_sync(0xffffffffu, top, first), b = __shfl_sync(0xffffffffu, by, first);
+        if (redo & team_of || (ask & team_of && others_near<T>(r, row, picks[r.k - 1], t, b, s)))
+          route_again<T>(r, row, (double*)(room + teams * (r.found + r.k + 1)) + threadIdx.x / 32 * r.experts, picks);
+      }
+    __syncwarp();
+  }
 
   // Weights: of the picks' own logits, which without a bias are what they were ranked by, the first the largest of them.
   const auto logit = [&](uint64_t pick) { return r.bias ? Elem<T>::to_f(from[~(uint32_t)pick]) : number_of((uint32_t)(pick >> 32)); };
@@ -376,13 +449,14 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
     total = team_sum(total, r.team_lanes) + (sum - sum);      // a row's scores that are NaN (a bias ranked them then) stay so
   }
   if (!alive) return;
-  const float by = r.renorm || !r.sigmoid ? __fdividef(r.scale, total) : r.scale;
+  by = r.renorm || !r.sigmoid ? __fdividef(r.scale, total) : r.scale;
+  const bool few = r.renorm && total < 1e-30f;
   for (int j = team.lane; j < r.k; j += lanes) {
     const uint64_t pick = best[j];
     r.chosen[row * r.k + j] = pick ? (int)~(uint32_t)pick : -1;
-    r.weights[row * r.k + j] = pick ? score(pick) * by : 0.0f;
+    if (!few) r.weights[row * r.k + j] = pick ? score(pick) * by : 0.0f;
   }
-  if (r.renorm && total < 1e-30f && team.lane == 0) weights_by_logarithms<T>(r, from, best, r.weights + row * r.k);
+  if (few && team.lane == 0) weights_by_logarithms<T>(r, from, best, r.weights + row * r.k);
 }
 
 // A team of lanes has a row, which lies in shared memory: gradients of the row's picks are found by a lane each, put to their experts, and leave as
@@ -511,8 +585,8 @@ static int launch_route(const RouteCall& r, cudaStream_t s) {
   const int teams = kRouteThreads >> r.team_lanes;
   const int64_t blocks = ceil_div(r.rows, teams);
   APT_CHECK_ARG(blocks < 1ll << 31, "route_experts: %lld rows are too many", (long long)r.rows);
-  const size_t bytes = ((size_t)teams * (r.found + r.k + 1) + kRouteThreads / 32 * r.experts) * 8;
   const bool exact = r.bias || (r.groups > 1 && r.best == 2);
+  const size_t bytes = ((size_t)teams * (r.found + r.k + 1) + (exact ? kRouteThreads / 32 * r.experts : 0)) * 8;
   if (r.groups > 1) {
     if (exact) APT_FOLLOW((k_route<T, NV, true, true>), blocks, kRouteThreads, bytes, s, r);
     else APT_FOLLOW((k_route<T, NV, true, false>), blocks, kRouteThreads, bytes, s, r);

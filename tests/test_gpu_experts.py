@@ -148,6 +148,29 @@ def test_scores_that_are_one_in_32_bits():
     assert torch.equal(apt_b200.route_experts(logits, *args)[0], _route64(logits, *args)[0])
 
 
+@pytest.mark.parametrize("experts,groups,top_groups,k", [(64, 1, 1, 8), (64, 1, 1, 33), (130, 1, 1, 16), (130, 1, 1, 64), (256, 1, 1, 8), (256, 1, 1, 33), (256, 8, 4, 8),
+                                                         (512, 1, 1, 47), (1000, 1, 1, 64), (1024, 1, 1, 63), (1024, 8, 2, 64), (1020, 17, 5, 31)])
+def test_many_equal_scores(experts, groups, top_groups, k):
+    """Rows of very few values and biases: more equal ones at the last place than there is room for, and neighbours by less than 32 bits tell behind them."""
+    few = torch.randint(0, 3, (40, experts), device="cuda", generator=_gen(experts)).float()
+    few[:4] = 0.0
+    few[4, :] = -1.0
+    few[5, experts // 2:] = -INF
+    round_ = torch.randn((40, experts), device="cuda", generator=_gen(k)).bfloat16()
+    near = few + torch.randint(0, 2, few.shape, device="cuda", generator=_gen(7)) * 2.0 ** -22
+    zeros, two = torch.zeros(experts, device="cuda"), torch.randint(0, 2, (experts,), device="cuda", generator=_gen(8)) * 0.5
+    for logits in (few, round_, near):
+        for best in (1, 2):
+            if groups == 1 and best == 2:
+                continue
+            for score, bias in (("softmax", None), ("softmax", zeros), ("sigmoid", zeros), ("sigmoid", two)):
+                args = (k, score, bias, groups, top_groups, best, True, 1.0)
+                got, weights = apt_b200.route_experts(logits, *args)
+                want, want_weights = _route64(logits, *args)
+                assert torch.equal(got, want)
+                assert float(((weights - want_weights).abs() - 2.0 ** -18 * want_weights.abs()).max()) <= 1e-37
+
+
 def test_wild_logits_stay_in_their_rows():
     logits = torch.randn((64, 32), device="cuda", generator=_gen(1))
     bias = torch.zeros(32, device="cuda")
@@ -367,6 +390,106 @@ def test_a_layer_of_experts(dtype, bound):
     want = (every.gather(1, chosen.unsqueeze(2).expand(-1, -1, 32)) * p.unsqueeze(2)).sum(1)
     for a, b in zip((out,) + got, (want,) + torch.autograd.grad(want, wide, grad.double())):
         assert float((a.detach().double() - b.detach()).norm() / b.detach().norm()) < bound
+    ops.check_status()
+
+
+def _step(x, router, weight, out_weight, out_bias, labels, k, padded=None):
+    logits = x @ router
+    if padded is not None:
+        logits = logits.masked_fill(padded.unsqueeze(1), -INF)
+    experts, weights = apt_b200.RouteExperts.apply(logits, k)
+    rows, offsets, place = apt_b200.ExpertRows.apply(x, experts, weight.shape[0])
+    h = apt_b200.ExpertSum.apply(apt_b200.GroupedLinear.apply(rows, weight, offsets), weights, place)
+    return apt_b200.LinearCrossEntropy.apply(h, out_weight, labels, out_bias)
+
+
+def _step_leaves(rows, dim, hidden, num_experts, classes, dtype, seed=1):
+    gen = _gen(seed)
+    shapes = [(rows, dim), (dim, num_experts), (num_experts, hidden, dim), (classes, hidden), (classes,)]
+    scales = [1.0, 0.2, 0.15, 0.3, 0.5]
+    return [(torch.randn(shape, device="cuda", generator=gen) * scale).to(dtype).requires_grad_() for shape, scale in zip(shapes, scales)]
+
+
+@pytest.mark.parametrize("dtype,bound", [(torch.float32, 1e-4), (torch.bfloat16, 2.0 ** -5)])
+def test_a_layer_of_experts_and_its_loss(dtype, bound):
+    """A padded batch through all of them, against every row times all experts' weights. fp32: logits of the loss of some 18 (their terms'
+    magnitudes and eight more) are (32 2^-23 + 2^-19) of that off, 1e-4, and the slopes with them. bf16: the layer's half steps move the
+    logits by 2^-7, and six roundings of 2^-8 at most follow one another."""
+    leaves = _step_leaves(320, 48, 32, 6, 500, dtype)
+    labels = torch.randint(0, 500, (320,), device="cuda", generator=_gen(9))
+    padded = torch.arange(320, device="cuda") >= 300
+    labels[padded] = -100
+    with torch.no_grad():
+        leaves[0][padded] = 0.0
+    loss = _step(*leaves, labels, 2, padded)
+    got = torch.autograd.grad(loss, leaves)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    x, router, weight, out_weight, out_bias = wide
+    chosen = (leaves[0] @ leaves[1]).detach().topk(2, 1).indices
+    p = torch.softmax(x @ router, 1).gather(1, chosen)
+    p = p / p.sum(1, keepdim=True)
+    every = torch.einsum("rd,eod->reo", x, weight)
+    h = (every.gather(1, chosen.unsqueeze(2).expand(-1, -1, 32)) * p.unsqueeze(2)).sum(1)
+    want = torch.nn.functional.cross_entropy((h @ out_weight.t() + out_bias)[:300], labels[:300])
+    assert abs(loss.item() - want.item()) < bound * want.item()
+    for a, b in zip(got, torch.autograd.grad(want, wide)):
+        assert bool(torch.isfinite(a).all()) and float((a.double() - b).norm() / b.norm()) < bound
+    assert not got[0][300:].any()
+    ops.check_status()
+
+
+def test_calls_at_once():
+    """Steps of two sizes on two streams, none waiting for another's: what each gives alone."""
+    steps, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seed, rows, experts, classes in ((1, 4000, 16, 3001), (2, 2500, 24, 5000)):
+        leaves = _step_leaves(rows, 64, 64, experts, classes, torch.bfloat16, seed)
+        steps.append((leaves, torch.randint(0, classes, (rows,), device="cuda", generator=_gen(seed))))
+
+    def run(n):
+        loss = _step(*steps[n][0], steps[n][1], 3)
+        return [loss.detach()] + list(torch.autograd.grad(loss, steps[n][0]))
+
+    want = [run(0), run(1)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for n in (0, 1):
+            with torch.cuda.stream(streams[n]):
+                got[n].append(run(n))
+    torch.cuda.synchronize()
+    for n in (0, 1):
+        for one in got[n]:
+            assert all(torch.equal(a, b) for a, b in zip(one, want[n]))
+    ops.check_status()
+
+
+def test_more_than_31_bits_of_elements():
+    rows, dim, k, n = 1_100_000, 1024, 2, 500
+    logits = torch.empty((2 * rows, dim), device="cuda", dtype=torch.bfloat16).normal_(generator=_gen(1))
+    assert logits.numel() > 2 ** 31
+    experts, weights = apt_b200.route_experts(logits, k)
+    tail = apt_b200.route_experts(logits[-n:].clone(), k)
+    assert torch.equal(experts[-n:], tail[0]) and torch.equal(weights[-n:], tail[1])
+    grad = torch.randn(weights.shape, device="cuda", generator=_gen(2))
+    for renormalize in (True, False):
+        whole = apt_b200.route_experts_backward(logits, experts, grad, "softmax", renormalize)[-n:].clone()
+        assert torch.equal(whole, apt_b200.route_experts_backward(logits[-n:].clone(), tail[0], grad[-n:].clone(), "softmax", renormalize))
+    x, experts, weights = logits[:rows].clone(), experts[:rows] % 4, weights[:rows].contiguous()
+    del logits, grad
+    y, offsets, place = apt_b200.expert_rows(x, experts, 4)
+    assert y.numel() > 2 ** 31 and int(place.max()) == rows * k - 1 and int(offsets[-1]) == rows * k
+    last = (place == rows * k - 1).nonzero()[0, 0]
+    some = torch.cat([torch.arange(rows - n, rows, device="cuda"), last.view(1)])
+    assert torch.equal(y[place[some]], x[some].unsqueeze(1).expand(-1, k, -1))
+    out = apt_b200.expert_sum(y, weights, place)
+    want = (x[some].double().unsqueeze(1) * weights[some].double().unsqueeze(2)).sum(1)
+    assert bool(((out[some].double() - want).abs() <= (HALF[x.dtype] + 2.0 ** -22) * want.abs() + 1e-37).all())
+    grad_y, grad_weights = apt_b200.expert_sum_backward(y, weights, place, out)
+    want = weights[some].double().unsqueeze(2) * out[some].double().unsqueeze(1)
+    assert bool(((grad_y[place[some]].double() - want).abs() <= (HALF[x.dtype] + 2.0 ** -22) * want.abs() + 1e-37).all())
+    # 1024 terms in fp32: at most 2^-14 of their magnitudes
+    terms = out[some].double().unsqueeze(1) * y[place[some]].double()
+    assert bool(((grad_weights[some].double() - terms.sum(2)).abs() <= 2.0 ** -14 * terms.abs().sum(2)).all())
     ops.check_status()
 
 

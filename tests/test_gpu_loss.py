@@ -314,6 +314,27 @@ def test_again_and_again(dtype):
         assert all(torch.equal(a, b) for a, b in zip(first, step()))
 
 
+def test_more_than_31_bits_of_slopes():
+    """Rows of which the first and the last ones count: what these are alone."""
+    rows, dim, classes, n = 8_500_000, 24, 250, 400
+    x, w, b, _ = _inputs(rows, dim, classes, torch.bfloat16)
+    some = torch.cat([torch.arange(n, device="cuda"), torch.arange(rows - n, rows, device="cuda")])
+    labels = torch.full((rows,), IGNORE, device="cuda")
+    labels[some] = torch.randint(0, classes, (2 * n,), device="cuda", generator=_gen(5))
+    loss, saved = apt_b200.linear_cross_entropy(x, w, labels, b, "sum", return_saved=True)
+    losses, slopes, magnitudes, _ = _plain(x[some], w, b, labels[some])
+    off = (dim * 2.0 ** -23 + 2.0 ** -19) * (float((x[some].double().abs() @ w.double().abs().t()).max()) + float(b.double().abs().max()) + 8)
+    assert abs(float(loss) - float(losses.sum())) <= off * 2 * n + 2.0 ** -23 * float(losses.sum())
+    gx, gw, gb = apt_b200.linear_cross_entropy_backward(x, w, labels, saved, torch.ones((), device="cuda"), b, "sum")
+    near, half = off + HALF[x.dtype] + 3e-5, HALF[x.dtype]
+    for got, want, terms in ((gx[some], slopes @ w.double(), magnitudes @ w.double().abs()), (gw, slopes.t() @ x[some].double(), magnitudes.t() @ x[some].double().abs()),
+                             (gb, slopes.sum(0), magnitudes.sum(0))):
+        assert bool(((got.double() - want).abs() <= near * terms + half * want.abs() + 1e-40).all())
+    gx[some] = 0
+    assert not gx.any()
+    ops.check_status()
+
+
 def test_another_stream_and_a_captured_graph():
     x, w, b, labels = _inputs(600, 64, 900, torch.bfloat16)
     leaves = [t.clone().requires_grad_() for t in (x, w, b)]

@@ -222,7 +222,7 @@ __device__ __forceinline__ Raw<T, VE> load_once(const T* p) {
   }
 }
 
-// 151552 rows of 256 bf16, two of 16 experts: 48 us with weights, 49 without (HBM: 36); four pairs at once of two rows 49 and 51, the next row's
+// 151552 rows of 256 bf16, two of 16 experts: 47 us with weights or without (HBM: 36); four pairs at once of two rows 49 and 51, the next row's
 // places asked for a row ahead, which spilled, 78.
 template <typename T, int VE, int U>
 __global__ void __launch_bounds__(256, U == 4 ? 5 : 6) k_expert_sum(const __grid_constant__ SumCall c) {

@@ -4,7 +4,8 @@
 //   dx[r, k]  = sum_n dy[r, n] w[g, n, k]
 //   dw[g, n, k] = sum_{r in g} dy[r, n] x[r, k],   db[g, n] = sum_{r in g} dy[r, n]
 //
-// One persistent kernel for all three (k_grouped), a block an SM: a thread has boxes of both operands copied to a ring of stages in
+// One persistent kernel for all three (k_grouped), and for the products around a loss whose logits are not kept (loss.cu: the same operands, rows of one
+// group, other ways out of tensor memory), a block an SM: a thread has boxes of both operands copied to a ring of stages in
 // shared memory, one issues the products of a stage into tensor memory, eight warps (fp32: four) bring finished tiles out, from one half of
 // tensor memory while the products of the next go to the other. Where the groups end is on the device only, so every block makes the list of
 // tiles from the ends and its warps walk it. In dw a run of stages, as long for every block, may begin and end within a sum: it leaves
@@ -728,7 +729,7 @@ __device__ __forceinline__ void tile_to_slot(uint32_t acc, int turn, int turns, 
 }
 
 // ---- the kernel ----------------------------------------------------------------------
-// 151552 x 256 -> 256 bf16 in 16 groups, us: out 34, dx 35 (HBM: 24; products: 12), dw and db 45 (24; 12) and their join 11.5. Eight tiles a block,
+// 151552 x 256 -> 256 bf16 in 16 groups, us: out 34, dx 35 (HBM: 24; products: 12), dw and db 43 (24; 12) and their join 9. Eight tiles a block,
 // of which the first waits for the list and the weights and the last is brought out beside nothing: a third of the tensor cores' cycles and 36 to 45 per
 // cent of the DRAM's are in use. 495616 x 1024 -> 256 f16 in 4 groups: 260 (194; 159), at 1.05 to 1.3 GHz under the power cap. 67584 x 128 -> 256 fp32 in
 // 8 groups: out 40, dx 42, dw and db with their join 53 (HBM: 16, 16, 16; products: 16 each): six products of pieces read 208 KB of shared memory a stage, which bounds it.
@@ -1308,7 +1309,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 }
 
 // The partial sums of dw and db that make up one, in the order of the rows. A run that begins within a sum says so in the plan; the first
-// such run of a sum has it joined: blocks (part of the tile, run). 147 runs of 256 x 256: 11.5 us for 38 MB out of L2, of which half is the launch
+// such run of a sum has it joined: blocks (part of the tile, run). 147 runs of 256 x 256: 9 us for 38 MB out of L2, of which half is the launch
 // and the look at the plan.
 template <typename T>
 __global__ void __launch_bounds__(256)

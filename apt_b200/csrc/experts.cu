@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(PairBlock<ONE>::kThreads) k_expert_places(cons
 }
 
 // ---- rows ------------------------------------------------------------------------------
-// A team of lanes has a row. A lane has 16 bytes of it at once: where rows are no whole 16-byte slices, as several narrower ones, each beside the other
+// A team of lanes has a row: at most a warp's, or a block's where few rows leave the GPU empty. A lane has 16 bytes of it at once: where rows are no whole 16-byte slices, as several narrower ones, each beside the other
 // lanes' (100000 x 255 bf16, three experts each, with the gradient: one narrow slice at once 280 us, these 138; 256 wide: 96).
 template <typename W>
 __device__ __forceinline__ W no_bits() {
@@ -261,11 +261,12 @@ __global__ void __launch_bounds__(256, U == 4 ? 5 : 6) k_expert_sum(const __grid
     }
 }
 
-// The same rows: 79 us (HBM: 59).
+// The same rows: 80 us (HBM: 59). A team has at most a warp, or all of a block.
 template <typename T, int VE, int U>
 __global__ void __launch_bounds__(256, U == 4 || VE == 1 ? 4 : 5) k_expert_sum_backward(const __grid_constant__ SumCall c) {
   wait_for_previous();
   constexpr int D = 16 / (int)sizeof(T) / VE;
+  __shared__ float parts[8][U];
   const T *__restrict__ const y = (const T*)c.y, *__restrict__ const grad = (const T*)c.grad;
   T* __restrict__ const grad_y = (T*)c.grad_y;
   const int lane = threadIdx.x & ((1 << c.lanes) - 1), apart = VE << c.lanes;
@@ -309,9 +310,20 @@ __global__ void __launch_bounds__(256, U == 4 || VE == 1 ? 4 : 5) k_expert_sum_b
           }
         }
       if (y) {
-        for (int o = 0; o < c.lanes; ++o)
+        for (int o = 0; o < min(c.lanes, 5); ++o)
 #pragma unroll
           for (int u = 0; u < U; ++u) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], 1 << o);
+        if (c.lanes > 5) {
+          __syncthreads();
+          if (lane % 32 == 0)
+#pragma unroll
+            for (int u = 0; u < U; ++u) parts[lane / 32][u] = dot[u];
+          __syncthreads();
+          if (lane == 0)
+            for (int w = 1; w < 8; ++w)
+#pragma unroll
+              for (int u = 0; u < U; ++u) dot[u] += parts[w][u];
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (lane == 0 && r < c.rows && j0 + u < c.k) c.grad_weights[r * c.k + j0 + u] = dot[u];
@@ -320,9 +332,11 @@ __global__ void __launch_bounds__(256, U == 4 || VE == 1 ? 4 : 5) k_expert_sum_b
 }
 
 // ---- host side -------------------------------------------------------------------------
-static int log2_lanes(int64_t slices) {
+// Lanes for a row of so many slices: a warp's, and up to a block's while all rows' would be a quarter of what the SMs hold. One row of 8192 bf16, eight
+// experts: rows 30 -> 13 us, sums 72 -> 15, their gradients 72 -> 16.
+static int log2_lanes(int64_t slices, int64_t rows) {
   int l = 0;
-  while (l < 5 && (1 << l) < slices) ++l;
+  while (l < 8 && (1 << l) < slices && (l < 5 || rows << l < kNumSMs * 512)) ++l;
   return l;
 }
 
@@ -353,7 +367,7 @@ static int expert_places(PairCall c, cudaStream_t s) {
 template <typename W>
 static int spread(const void* x, int64_t rows, int64_t row_bytes, int k, const int64_t* place, void* out, cudaStream_t s) {
   const int64_t slices = row_bytes / (int64_t)sizeof(W);
-  const int lanes = log2_lanes(ceil_div(row_bytes, 16));
+  const int lanes = log2_lanes(ceil_div(row_bytes, 16), rows);
   APT_FOLLOW((k_expert_spread<W>), wave_grid(ceil_div(rows, 256 >> lanes), 8), 256, 0, s, (const W*)x, rows, (int)slices, k, place, (W*)out, lanes);
   return APT_OK;
 }
@@ -369,7 +383,8 @@ static int launch_pairs(const SumCall& c, bool backward, cudaStream_t s) {
 }
 template <typename T, int VE>
 static int launch_sum(SumCall c, bool backward, cudaStream_t s) {
-  c.lanes = log2_lanes(ceil_div(c.dim, 16 / (int)sizeof(T)));
+  c.lanes = log2_lanes(ceil_div(c.dim, 16 / (int)sizeof(T)), c.rows);
+  if (backward) c.lanes = c.lanes > 6 ? 8 : std::min(c.lanes, 5);
   // pairs at once: eight slices of a lane are on their way at the most (narrow ones take as many registers as wide ones)
   constexpr int kMost = VE * (int)sizeof(T) / 2 < 4 ? VE * (int)sizeof(T) / 2 : 4;
   if constexpr (kMost >= 4)

@@ -331,6 +331,17 @@ def test_sums_over_experts(rows, k, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,dim", [(1, 8, 8192), (1, 3, 5001), (2, 2, 300), (7, 2, 4100), (70, 5, 2500), (150, 1, 3000), (590, 3, 1000), (1200, 2, 600)])
+def test_few_wide_rows(rows, k, dim, dtype):
+    """Rows that several warps share."""
+    x = torch.randn((rows, dim), device="cuda", generator=_gen(dim)).to(dtype)
+    experts = _experts(rows, k, 16, 4)
+    _check_rows(x, experts, 16)
+    y, _, place = apt_b200.expert_rows(x, experts, 16)
+    _check_sum(y, torch.randn((rows, k), device="cuda", generator=_gen(6)), place)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_of_no_expert_count_for_nothing_whatever_they_hold(dtype):
     experts = _experts(200, 3, 6, 1, none=0.4)
     experts[:7] = -1

@@ -314,10 +314,11 @@ def test_again_and_again(dtype):
         assert all(torch.equal(a, b) for a, b in zip(first, step()))
 
 
-def test_more_than_31_bits_of_slopes():
-    """Rows of which the first and the last ones count: what these are alone."""
-    rows, dim, classes, n = 8_500_000, 24, 250, 400
-    x, w, b, _ = _inputs(rows, dim, classes, torch.bfloat16)
+@pytest.mark.parametrize("rows,dim,classes,dtype", [(8_500_000, 24, 250, torch.bfloat16)] + [(200_000, 16, 50_000, dtype) for dtype in DTYPES])
+def test_more_than_31_bits_of_slopes(rows, dim, classes, dtype):
+    """Rows of which the first and the last ones count: what these are alone. Slopes at once, and in many pieces, with statistics in several."""
+    n = 400
+    x, w, b, _ = _inputs(rows, dim, classes, dtype)
     some = torch.cat([torch.arange(n, device="cuda"), torch.arange(rows - n, rows, device="cuda")])
     labels = torch.full((rows,), IGNORE, device="cuda")
     labels[some] = torch.randint(0, classes, (2 * n,), device="cuda", generator=_gen(5))
@@ -326,10 +327,10 @@ def test_more_than_31_bits_of_slopes():
     off = (dim * 2.0 ** -23 + 2.0 ** -19) * (float((x[some].double().abs() @ w.double().abs().t()).max()) + float(b.double().abs().max()) + 8)
     assert abs(float(loss) - float(losses.sum())) <= off * 2 * n + 2.0 ** -23 * float(losses.sum())
     gx, gw, gb = apt_b200.linear_cross_entropy_backward(x, w, labels, saved, torch.ones((), device="cuda"), b, "sum")
-    near, half = off + HALF[x.dtype] + 3e-5, HALF[x.dtype]
+    near, half, tiny = off + HALF[dtype] + 3e-5, HALF[dtype], torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     for got, want, terms in ((gx[some], slopes @ w.double(), magnitudes @ w.double().abs()), (gw, slopes.t() @ x[some].double(), magnitudes.t() @ x[some].double().abs()),
                              (gb, slopes.sum(0), magnitudes.sum(0))):
-        assert bool(((got.double() - want).abs() <= near * terms + half * want.abs() + 1e-40).all())
+        assert bool(((got.double() - want).abs() <= near * terms + half * want.abs() + tiny).all())
     gx[some] = 0
     assert not gx.any()
     ops.check_status()

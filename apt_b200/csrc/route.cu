@@ -265,17 +265,23 @@ __device__ __forceinline__ void row_softmax(const float (&z)[NV], int lanes, flo
   *top = m, *sum = team_sum(s, lanes);
 }
 
-// Of a row whose last pick and the next are ranked by the same logit and bias: whether another is near them, that is not. top, by: of its softmax. A warp's.
+// Whether experts whose scores are near `score` are of different logits or biases: of a row whose last pick and the next are the same, say, whether another
+// is near them. (A pick near the last one that is not the same has the row done again in any case, so that what lies above is not left out.) The
+// scores made here need not be those that were ranked, bit by bit: near is wider than both their errors. top, by: of its softmax. A warp's.
 template <typename T>
-__device__ __noinline__ bool others_near(const RouteCall& r, const T* row, uint64_t last, float top, float by, float slack) {
-  bool near = false;
-  const int at = ~(uint32_t)last;
-  const float z = Elem<T>::to_f(row[at]), b = r.bias[at], score = number_of((uint32_t)(last >> 32));
+__device__ __noinline__ bool others_near(const RouteCall& r, const T* row, float score, float top, float by, float slack) {
+  float z = 0.0f, b = 0.0f;
+  bool found = false, other = false;
   for (int e = threadIdx.x % 32; e < r.experts; e += 32) {
     const float v = Elem<T>::to_f(row[e]), s = (r.sigmoid ? logistic(v) : exp_short(v - top) * by) + r.bias[e];
-    near |= s <= score && too_near(score, s, slack) && !(v == z && r.bias[e] == b);
+    if (v == -INFINITY || fabsf(s - score) >= slack + 0x1p-22f * fabsf(score)) continue;
+    if (!found) found = true, z = v, b = r.bias[e];
+    other |= !(v == z && r.bias[e] == b);
   }
-  return __any_sync(0xffffffffu, near);
+  const unsigned who = __ballot_sync(0xffffffffu, found);
+  const int first = who ? __ffs(who) - 1 : 0;
+  const float one = __shfl_sync(0xffffffffu, z, first), its = __shfl_sync(0xffffffffu, b, first);
+  return __any_sync(0xffffffffu, other || (found && !(z == one && b == its)));
 }
 
 // A row's picks in 64 bits, by a warp: what experts are ranked by lies in shared memory, 32 neighbours at a time. Few rows come here, and the
@@ -432,7 +438,7 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
         const T* const row = (const T*)r.logits + ((int64_t)blockIdx.x * teams + n) * r.experts;
         uint64_t* const picks = room + teams * r.found + n * (r.k + 1);
         const float s = __shfl_sync(0xffffffffu, slack, first), t = __shfl_sync(0xffffffffu, top, first), b = __shfl_sync(0xffffffffu, by, first);
-        if (redo & team_of || (ask & team_of && others_near<T>(r, row, picks[r.k - 1], t, b, s)))
+        if (redo & team_of || (ask & team_of && others_near<T>(r, row, number_of((uint32_t)(picks[r.k - 1] >> 32)), t, b, s)))
           route_again<T>(r, row, (double*)(room + teams * (r.found + r.k + 1)) + threadIdx.x / 32 * r.experts, picks);
       }
     __syncwarp();

@@ -171,6 +171,36 @@ def test_many_equal_scores(experts, groups, top_groups, k):
                 assert float(((weights - want_weights).abs() - 2.0 ** -18 * want_weights.abs()).max()) <= 1e-37
 
 
+def _choice64(logits, k, score, bias, groups=1, top_groups=1, best=1):
+    """_route64's choice for a bias, many rows at once."""
+    s = torch.softmax(logits.double(), 1) if score == "softmax" else torch.sigmoid(logits.double())
+    c = torch.where(logits == -INF, -INF, s + bias.double())
+    if groups > 1:
+        values = c.view(len(c), groups, -1).sort(dim=2, descending=True).values[:, :, :best]
+        values = torch.where(values[:, :, -1] == -INF, values[:, :, 0], values.sum(2))
+        stay = torch.zeros_like(values, dtype=torch.bool).scatter_(1, values.sort(dim=1, descending=True, stable=True).indices[:, :top_groups], True)
+        c = torch.where(stay.repeat_interleave(c.shape[1] // groups, 1), c, -INF)
+    order = c.sort(dim=1, descending=True, stable=True)
+    return torch.where(order.values == -INF, -1, order.indices)[:, :k]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,k", [(6, 1), (16, 2), (64, 3), (256, 8)])
+def test_near_ones_that_are_not_among_the_picks(experts, k, score):
+    """The last pick and the next are one logit and bias; others, of another logit and bias, come to the same 32 bits, and in the exact scores some are above."""
+    gen = _gen(experts)
+    base = torch.rand((1, experts), device="cuda", generator=gen) * 2 - 1
+    table = torch.softmax(base.double(), 1) if score == "softmax" else torch.sigmoid(base.double())
+    bias = (1.0 - table[0]).float()
+    logits = base.repeat(20_000, 1)
+    # half of the experts are the same, the others neighbours by a unit or two
+    logits[:, ::2], bias[::2] = logits[0, 0].clone(), bias[0].clone()
+    step = torch.randint(-3, 4, logits.shape, device="cuda", generator=gen) * 2.0 ** -24
+    step[:, ::2] = 0.0
+    logits += step
+    assert torch.equal(apt_b200.route_experts(logits, k, score, bias)[0], _choice64(logits, k, score, bias))
+
+
 def test_wild_logits_stay_in_their_rows():
     logits = torch.randn((64, 32), device="cuda", generator=_gen(1))
     bias = torch.zeros(32, device="cuda")

@@ -82,10 +82,10 @@ __device__ __forceinline__ float exp_short(float z) { return exp2_short(1.442695
 __device__ __forceinline__ float log_logistic(float z) { return fminf(z, 0.0f) - log1pf(expf(-fabsf(z))); }
 __device__ __forceinline__ bool too_near(float a, float b, float slack) { return !(a - b >= slack + 0x1p-22f * fabsf(a)); }
 
-// Whether the lane's group is one of those that stay: of all groups' values, the same in all lanes of a group. near: the last that stays and the
-// first that does not are too near one another for 32 bits.
-template <int NV>
-__device__ __forceinline__ bool group_stays(const RouteCall& r, const Team& team, const float (&v)[NV], float slack, bool* near) {
+// Whether the lane's group is one of those that stay: of all groups' values, the same in all lanes of a group. EXACT: values are scores in 32 bits, and
+// near: the last that stays and the first that does not are too near one another for those. last: the value of the first of the two.
+template <int NV, bool EXACT>
+__device__ __forceinline__ bool group_stays(const RouteCall& r, const Team& team, const float (&v)[NV], float slack, bool* near, float* last) {
   const int group = team.lane >> r.group_lanes;
   uint32_t one = 0, two = 0;
 #pragma unroll
@@ -104,9 +104,10 @@ __device__ __forceinline__ bool group_stays(const RouteCall& r, const Team& team
     above += other > key || (other == key && g < group);
   }
   const bool stays = above < r.top_groups;
-  if (r.best == 2) {
-    const uint32_t last = team_least(stays && group < r.groups ? key : 0xffffffffu, r.team_lanes), next = team_most(stays ? 0u : key, r.team_lanes);
-    *near = next && too_near(number_of(last), number_of(next), 2.0f * slack);
+  if constexpr (EXACT) {
+    const uint32_t a = team_least(stays && group < r.groups ? key : 0xffffffffu, r.team_lanes), b = team_most(stays ? 0u : key, r.team_lanes);
+    *last = number_of(a);
+    *near = b && too_near(number_of(a), number_of(b), r.best * slack);
   }
   return stays;
 }
@@ -266,7 +267,8 @@ __device__ __forceinline__ void row_softmax(const float (&z)[NV], int lanes, flo
 }
 
 // Whether experts whose scores are near `score` are of different logits or biases: of a row whose last pick and the next are the same, say, whether another
-// is near them. (A pick near the last one that is not the same has the row done again in any case, so that what lies above is not left out.) The
+// is near them. (A pick near the last one that is not the same has the row done again in any case, so that what lies above is not left out.) Or of a row
+// whose groups go by their best, and the last that stays and the first that does not are near: what could make one of them the other lies as near. The
 // scores made here need not be those that were ranked, bit by bit: near is wider than both their errors. top, by: of its softmax. A warp's.
 template <typename T>
 __device__ __noinline__ bool others_near(const RouteCall& r, const T* row, float score, float top, float by, float slack) {
@@ -384,8 +386,8 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
   load_logits<T, NV>(from, base, end, r.whole, z);
   if (!r.sigmoid && (EXACT || !r.renorm)) row_softmax(z, r.team_lanes, &top, &sum);
   uint32_t key[NV];
-  bool again = false, stays = true;
-  float slack = 0.0f, by = 1.0f;      // by: the largest score there can be
+  bool again = false, equal = false, stays = true;      // equal: the groups at the border are near, or have the same best
+  float slack = 0.0f, by = 1.0f, last = 0.0f;           // by: the largest score there can be, last: of the groups that stay
   if constexpr (EXACT) {
     float s[NV], b[NV];
 #pragma unroll
@@ -407,11 +409,15 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
       const bool there = z[i] != -INFINITY;
       s[i] = there ? (r.sigmoid ? logistic(z[i]) : exp_short(z[i] - top) * by) + b[i] : -INFINITY;
     }
-    if constexpr (GROUPS) stays = group_stays<NV>(r, team, s, slack, &again);
+    if constexpr (GROUPS) {
+      stays = group_stays<NV, true>(r, team, s, slack, &again, &last);
+      // (by their best they may be the same, as picks may)
+      if (r.best == 1) equal = again, again = false;
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) key[i] = stays ? rank_of(r.bias ? s[i] : z[i]) : 0;
   } else {
-    if constexpr (GROUPS) stays = group_stays<NV>(r, team, z, 0.0f, &again);
+    if constexpr (GROUPS) stays = group_stays<NV, false>(r, team, z, 0.0f, &again, &last);
 #pragma unroll
     for (int i = 0; i < NV; ++i) key[i] = stays ? rank_of(z[i]) : 0;
   }
@@ -431,14 +437,17 @@ __global__ void __launch_bounds__(kRouteThreads) k_route(const __grid_constant__
       }
     }
     const unsigned redo = __ballot_sync(0xffffffffu, again && alive), ask = __ballot_sync(0xffffffffu, open && alive);
-    if (redo | ask)
+    const unsigned ask_groups = GROUPS ? __ballot_sync(0xffffffffu, equal && alive) : 0u;
+    if (redo | ask | ask_groups)
       for (int first = 0; first < 32; first += lanes) {
         const unsigned team_of = (lanes == 32 ? ~0u : (1u << lanes) - 1) << first;
         const int n = (threadIdx.x / 32 * 32 + first) >> r.team_lanes;
         const T* const row = (const T*)r.logits + ((int64_t)blockIdx.x * teams + n) * r.experts;
         uint64_t* const picks = room + teams * r.found + n * (r.k + 1);
         const float s = __shfl_sync(0xffffffffu, slack, first), t = __shfl_sync(0xffffffffu, top, first), b = __shfl_sync(0xffffffffu, by, first);
-        if (redo & team_of || (ask & team_of && others_near<T>(r, row, number_of((uint32_t)(picks[r.k - 1] >> 32)), t, b, s)))
+        const float l = GROUPS ? __shfl_sync(0xffffffffu, last, first) : 0.0f;
+        if (redo & team_of || (ask & team_of && others_near<T>(r, row, number_of((uint32_t)(picks[r.k - 1] >> 32)), t, b, s)) ||
+            (ask_groups & team_of && others_near<T>(r, row, l, t, b, s)))
           route_again<T>(r, row, (double*)(room + teams * (r.found + r.k + 1)) + threadIdx.x / 32 * r.experts, picks);
       }
     __syncwarp();

@@ -201,6 +201,34 @@ def test_near_ones_that_are_not_among_the_picks(experts, k, score):
     assert torch.equal(apt_b200.route_experts(logits, k, score, bias)[0], _choice64(logits, k, score, bias))
 
 
+def test_groups_by_their_best_that_are_one_in_32_bits():
+    """The best of two groups are one number in 32 bits, logistics next to 1, and not in the exact scores."""
+    zeros = torch.zeros(4, device="cuda")
+    for dtype in DTYPES:
+        logits = torch.tensor([[20.0, -5.0, 25.0, -5.0], [25.0, 1.0, 20.0, 2.0], [-5.0, 21.0, 22.0, 21.0], [22.0, 22.0, 22.0, 22.0]], device="cuda").to(dtype)
+        assert apt_b200.route_experts(logits, 1, "sigmoid", zeros, 2, 1)[0].tolist() == [[2], [0], [2], [0]]
+        assert apt_b200.route_experts(logits, 2, "sigmoid", zeros, 2, 1)[0].tolist() == [[2, 3], [0, 1], [2, 3], [0, 1]]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_groups,k", [(4, 2, 1, 1), (16, 8, 3, 1), (64, 8, 3, 4), (60, 5, 2, 1), (256, 8, 4, 8), (1023, 31, 9, 9), (1020, 17, 5, 1)])
+def test_groups_by_their_best_are_those_of_the_exact_scores(experts, groups, top_groups, k, score):
+    rows = 40_000 if experts < 1000 else 8000
+    gen = _gen(experts + k)
+    # logistics next to 1 in many of the groups
+    wide = (torch.randn((rows, experts), device="cuda", generator=gen) * 6).clamp_(-30, 30)
+    # neighbours by a unit of their last place
+    close = torch.randn((1, experts), device="cuda", generator=gen).clamp_(-2, 2)
+    table = torch.softmax(close.double(), 1) if score == "softmax" else torch.sigmoid(close.double())
+    level = (table.max() - table[0]).float()
+    close = close + torch.randint(-4, 5, (rows, experts), device="cuda", generator=gen) * 2.0 ** -23
+    few = torch.randint(0, 3, (rows, experts), device="cuda", generator=gen).float() + torch.randint(0, 2, (rows, experts), device="cuda", generator=gen) * 2.0 ** -22
+    zeros, constant = torch.zeros(experts, device="cuda"), torch.full((experts,), 0.75, device="cuda")
+    for logits, bias in ((wide, zeros), (wide.bfloat16(), zeros), (wide.half(), constant), (close, level), (few, zeros), (few, constant)):
+        got = apt_b200.route_experts(logits, k, score, bias, groups, top_groups, 1)[0]
+        assert torch.equal(got, _choice64(logits, k, score, bias, groups, top_groups, 1))
+
+
 def test_wild_logits_stay_in_their_rows():
     logits = torch.randn((64, 32), device="cuda", generator=_gen(1))
     bias = torch.zeros(32, device="cuda")

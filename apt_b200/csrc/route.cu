@@ -107,7 +107,15 @@ __device__ __forceinline__ bool group_stays(const RouteCall& r, const Team& team
   if constexpr (EXACT) {
     const uint32_t a = team_least(stays && group < r.groups ? key : 0xffffffffu, r.team_lanes), b = team_most(stays ? 0u : key, r.team_lanes);
     *last = number_of(a);
-    *near = b && too_near(number_of(a), number_of(b), r.best * slack);
+    if (r.best == 1) {
+      *near = b && too_near(number_of(a), number_of(b), slack);
+    } else {
+      // Two scores and their sum are rounded by 2^-24 of themselves each, also where biases take the two away from each other: 2^-23 (|one| + |two|) a group,
+      // of the largest of all. As bits these numbers have their order, and one that is none is above all, which nothing is far enough from.
+      const float size = group < r.groups && key ? fabsf(number_of(one)) + (two ? fabsf(number_of(two)) : 0.0f) : 0.0f;
+      const float most = __uint_as_float(team_most(__float_as_uint(size), r.team_lanes));
+      *near = b && !(number_of(a) - number_of(b) >= 2.0f * slack + 0x1p-22f * most);
+    }
   }
   return stays;
 }

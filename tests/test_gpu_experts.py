@@ -229,6 +229,20 @@ def test_groups_by_their_best_are_those_of_the_exact_scores(experts, groups, top
         assert torch.equal(got, _choice64(logits, k, score, bias, groups, top_groups, 1))
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_groups,k", [(16, 8, 3, 1), (16, 8, 3, 4), (8, 4, 2, 2), (96, 32, 5, 3)])
+def test_groups_whose_two_best_take_each_other_away(experts, groups, top_groups, k, score):
+    """Biases of 64 and more, and minus as much: each sum with one is rounded to steps of 2^-17, the two best together are as little as two scores."""
+    gen = _gen(experts + k)
+    per = experts // groups
+    own = 64.0 + 2.0 * (torch.arange(experts, device="cuda") // per)
+    bias = torch.where(torch.arange(experts, device="cuda") % per == 0, own, -own)
+    logits = torch.randn((1, per), device="cuda", generator=gen).repeat(20_000, groups)
+    logits += torch.randn(logits.shape, device="cuda", generator=gen) * 2e-5
+    got = apt_b200.route_experts(logits, k, score, bias, groups, top_groups, 2)[0]
+    assert torch.equal(got, _choice64(logits, k, score, bias, groups, top_groups, 2))
+
+
 def test_wild_logits_stay_in_their_rows():
     logits = torch.randn((64, 32), device="cuda", generator=_gen(1))
     bias = torch.zeros(32, device="cuda")

@@ -22,6 +22,7 @@ template <bool ONE>
 struct PairBlock {
   static constexpr int kWarps = ONE ? 16 : 8, kThreads = 32 * kWarps, kALane = ONE ? 8 : 4, kPairs = kThreads * kALane;
 };
+constexpr int64_t kMostPairs = (1ll << 31) - 1 - PairBlock<false>::kPairs;      // counts, and the steps of loops beyond the last pair, are numbers of 32 bits
 constexpr int kMostOfOne = 1024;      // experts that a larger block has counts for
 
 struct PairCall {
@@ -411,7 +412,7 @@ static int sum_of(int dtype, const SumCall& c, bool backward, cudaStream_t s) {
 }
 static int sum_check(const char* who, int dtype, int64_t rows, int64_t dim, int64_t k) {
   APT_CHECK_ARG(dtype == APT_F32 || dtype == APT_BF16 || dtype == APT_F16, "%s: unsupported dtype %d", who, dtype);
-  APT_CHECK_ARG(rows >= 0 && dim >= 1 && dim < 1ll << 30 && k >= 1 && k < 1ll << 31 && rows <= ((1ll << 31) - 1) / k, "%s: %lld rows of %lld, %lld experts each", who, (long long)rows,
+  APT_CHECK_ARG(rows >= 0 && dim >= 1 && dim < 1ll << 30 && k >= 1 && k < 1ll << 31 && rows <= kMostPairs / k, "%s: %lld rows of %lld, %lld experts each", who, (long long)rows,
                 (long long)dim, (long long)k);
   return APT_OK;
 }
@@ -426,7 +427,7 @@ extern "C" size_t apt_expert_rows_workspace_bytes(int64_t pairs, int64_t experts
 extern "C" int apt_expert_rows(const void* x, int64_t rows, int64_t row_bytes, const int64_t* experts, int64_t k, int64_t num_experts, void* out,
                                int64_t* offsets, int64_t* place, void* workspace, size_t workspace_bytes, int32_t* status_word, void* stream) {
   using namespace apt;
-  APT_CHECK_ARG(rows >= 0 && k >= 1 && k < 1ll << 31 && rows <= ((1ll << 31) - 1 - PairBlock<false>::kPairs) / k, "apt_expert_rows: %lld rows, %lld experts each", (long long)rows,
+  APT_CHECK_ARG(rows >= 0 && k >= 1 && k < 1ll << 31 && rows <= kMostPairs / k, "apt_expert_rows: %lld rows, %lld experts each", (long long)rows,
                 (long long)k);
   APT_CHECK_ARG(num_experts >= 1 && num_experts <= APT_GROUPED_LINEAR_MAX_GROUPS, "apt_expert_rows: %lld experts (1 to %d are possible)",
                 (long long)num_experts, APT_GROUPED_LINEAR_MAX_GROUPS);

@@ -41,3 +41,11 @@ def test_cpu_tensors_are_refused():
         apt_b200.route_experts(z, 2)
     with pytest.raises(RuntimeError, match="unknown score"):
         apt_b200.route_experts(z, 2, "tanh")
+
+
+def test_more_experts_a_row_than_can_be_counted_are_refused():
+    """Pairs are counted in steps beyond the last one: the same limit as that of expert_rows."""
+    for k in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 1024):
+        for got in (lib.apt_expert_sum(_lib.F32, P, 1, 8, k, P, P, P, P, None), lib.apt_expert_sum_backward(_lib.F32, P, 1, 8, k, P, P, P, P, P, P, None),
+                    lib.apt_expert_rows(P, 1, 64, P, k, 8, P, P, P, P, 2 ** 40, P, None)):
+            assert got == _lib.APT_ERR_BAD_ARG and b"experts each" in lib.apt_last_error()

@@ -95,9 +95,11 @@ struct LossCall {
   int more;                     // dx: there are sums of earlier classes
 };
 
-__device__ __forceinline__ float slope_scale(const LossCall& l) { return l.scale ? l.scale[0] : l.range; }
+// A common gradient that is no number is the slopes' factor, not the sums': rows that do not count have slopes of zero, which stay zeros then.
+__device__ __forceinline__ bool common_in_slopes(const LossCall& l) { return l.common && !(fabsf(*l.common) < INFINITY); }
+__device__ __forceinline__ float slope_scale(const LossCall& l) { return l.scale ? l.scale[0] : common_in_slopes(l) ? *l.common : l.range; }
 __device__ __forceinline__ float sum_scale(const LossCall& l) {
-  return l.scale ? l.scale[1] : l.common ? *l.common / (l.count ? fmaxf(*l.count, 1.0f) : 1.0f) / l.range : 1.0f;
+  return l.scale ? l.scale[1] : l.common && !common_in_slopes(l) ? *l.common / (l.count ? fmaxf(*l.count, 1.0f) : 1.0f) / l.range : 1.0f;
 }
 
 struct GroupedCall {

@@ -106,21 +106,31 @@ __global__ void __launch_bounds__(256) k_loss_rows(const __grid_constant__ RowsC
   if (c.loss) *c.loss = (float)(c.mean ? a / fmax(b, 1.0) : a);
 }
 
-// Rows' own gradients go into their slopes, less the largest of them. scale[0]: what they are multiplied by there, scale[1]: what the sums over slopes
-// are. One block.
+// Rows' own gradients go into their slopes, less the largest of those that are numbers (one that is none is its own row's matter). scale[0]: what they
+// are multiplied by there, scale[1]: what the sums over slopes are. One block.
 __global__ void __launch_bounds__(1024) k_loss_scale(const float* __restrict__ grad, int64_t rows, const float2* __restrict__ stats, float range, float* scale) {
   wait_for_previous();
   __shared__ float part[32];
   float m = 0.0f;
-  for (int64_t i = threadIdx.x; i < rows; i += 1024)
-    if (!(stats[i].y < 0.0f)) m = fmaxf(m, fabsf(grad[i]));
+  // (nothing is asked between the loads of eight rows: a million rows take 155 us, and 630 with a question between the two loads of each)
+  constexpr int kAtOnce = 8;
+  for (int64_t i0 = threadIdx.x; i0 < rows; i0 += kAtOnce * 1024) {
+    float g[kAtOnce], y[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int64_t i = min(i0 + u * 1024, rows - 1);
+      g[u] = fabsf(grad[i]), y[u] = stats[i].y;
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) m = fmaxf(m, !(y[u] < 0.0f) && g[u] < INFINITY ? g[u] : 0.0f);
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
   __syncthreads();
   if (threadIdx.x) return;
   for (int w = 0; w < 32; ++w) m = fmaxf(m, part[w]);
-  m = m > 0.0f && m < INFINITY ? fmaxf(m, 1e-30f) : 1.0f;
+  m = m > 0.0f ? fmaxf(m, 1e-30f) : 1.0f;
   scale[0] = range / m, scale[1] = m / range;
 }
 

@@ -206,6 +206,45 @@ def test_rows_that_do_not_count_may_hold_anything(rows, dim, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim,classes", [(200, 64, 300), (90, 33, 9000)])
+def test_gradients_that_are_no_numbers_stay_in_their_rows(rows, dim, classes, dtype):
+    """A row's own gradient that is infinite, or none: the other rows' dx is what it is without."""
+    x, w, b, labels = _inputs(rows, dim, classes, dtype)
+    labels[5], labels[9] = 3, IGNORE
+    saved = apt_b200.linear_cross_entropy(x, w, labels, b, "none", return_saved=True)[1]
+    fine = torch.arange(rows, device="cuda") != 5
+    for size in (2.0 ** 10, 2.0 ** -12):
+        grad = torch.full((rows,), size, device="cuda")
+        want = apt_b200.linear_cross_entropy_backward(x, w, labels, saved, grad, b, "none")[0]
+        assert torch.isfinite(want).all()
+        for bad in (float("inf"), -float("inf"), float("nan")):
+            grad[5], grad[9] = bad, bad
+            got = apt_b200.linear_cross_entropy_backward(x, w, labels, saved, grad, b, "none")[0]
+            assert torch.equal(got[fine], want[fine]) and not torch.isfinite(got[5]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim,classes", [(200, 64, 300), (300, 128, 9000), (1, 40, 77)])
+def test_rows_that_do_not_count_have_no_gradient_whatever_the_loss_has(rows, dim, classes, dtype):
+    x, w, b, labels = _inputs(rows, dim, classes, dtype, ignored=0.3)
+    labels[0] = IGNORE
+    for none_counts in (False, True):
+        if none_counts:
+            labels = torch.full_like(labels, IGNORE)
+        for reduction in ("mean", "sum", "none"):
+            saved = apt_b200.linear_cross_entropy(x, w, labels, b, reduction, return_saved=True)[1]
+            for bad in (float("inf"), -float("inf"), float("nan")):
+                grad = torch.full((rows,) if reduction == "none" else (), bad, device="cuda")
+                gx, gw, gb = apt_b200.linear_cross_entropy_backward(x, w, labels, saved, grad, b, reduction)
+                counted = labels != IGNORE
+                assert not gx[~counted].any() and not (gx[~counted] != gx[~counted]).any()
+                if counted.any():
+                    assert not torch.isfinite(gx[counted]).all(1).any() and not torch.isfinite(gw).any() and not torch.isfinite(gb).any()
+                else:
+                    assert all(torch.equal(t, torch.zeros_like(t)) for t in (gw, gb))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("polls", [0, 1, 6, 50])
 @pytest.mark.parametrize("rows,dim,classes", [(300, 128, 700), (3000, 64, 1500), (700, 1024, 25_000)])
 def test_the_kernels_end_when_a_wait_runs_out(rows, dim, classes, dtype, polls):

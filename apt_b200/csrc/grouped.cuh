@@ -88,6 +88,10 @@ struct LossCall {
   const float* scale;           // [2]: what the rows' gradients are multiplied by, what dx and dw are; null: range and common over it
   const float *common, *count;  // the gradient that all rows have, and what it is divided by (or null)
   float range;
+  // f16 with rows' own gradients, of which some are much smaller than the largest: the slopes for dx have none of them in, and dx is multiplied by its
+  // row's; those for dW and db are made by themselves. wide: whether it is so (null: it is not); own: these are for dx; again: for dW and db.
+  const int* wide;
+  int own, again;
   int *turn, *dirty;            // statistics: set to 0 for the kernel behind
   // dW: a row that does not count has slopes of zero, and its own elements are no number: there is a copy of the rows with zeros for those
   const int* unclean;
@@ -100,6 +104,16 @@ __device__ __forceinline__ bool common_in_slopes(const LossCall& l) { return l.c
 __device__ __forceinline__ float slope_scale(const LossCall& l) { return l.scale ? l.scale[0] : common_in_slopes(l) ? *l.common : l.range; }
 __device__ __forceinline__ float sum_scale(const LossCall& l) {
   return l.scale ? l.scale[1] : l.common && !common_in_slopes(l) ? *l.common / (l.count ? fmaxf(*l.count, 1.0f) : 1.0f) / l.range : 1.0f;
+}
+
+// A row's slopes are multiplied by this, its dx by that.
+__device__ __forceinline__ float slope_factor(const LossCall& l, float grad) {
+  if (l.own && *l.wide) return grad == 0.0f ? 0.0f : l.range;
+  return grad * slope_scale(l);
+}
+__device__ __forceinline__ float row_scale(const LossCall& l, int64_t row) {
+  if (l.own && *l.wide) return l.stats[row].y < 0.0f ? 0.0f : l.grad[row] / l.range;
+  return sum_scale(l);
 }
 
 struct GroupedCall {
@@ -675,7 +689,7 @@ template <bool SHORT>
 __device__ __forceinline__ Slopes row_slopes(const LossCall& l, const RowFacts& f, int64_t n0) {
   Slopes s = {0.0f, 1.0f, 0.0f, -1};
   if (f.stats.y < 0.0f) return s;      // does not count, or is not there
-  s.factor = f.grad * slope_scale(l);
+  s.factor = slope_factor(l, f.grad);
   s.less = f.stats.x, s.share = s.factor / f.stats.y;
   if (SHORT && fabsf(s.factor) < INFINITY) s.less -= log2f(fabsf(s.factor) / f.stats.y), s.share = s.factor < 0.0f ? -1.0f : 1.0f;
   const int64_t at = f.label - l.class0 - n0;
@@ -823,6 +837,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
   GroupedWalk<T, MODE> walk(c, prefix, begin);
+  // (the slopes that are there already are right for dW and db too)
+  const bool idle = MODE == kSlopes && c.loss.again && !*c.loss.wide;
+  if (idle) walk.next = walk.end;
   if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *c.loss.turn = 0, *c.loss.dirty = 0;
   if (Tr::kOverRows && !Tr::kTall && blockIdx.x == 0 && threadIdx.x == 0) c.plan[0] = walk.runs.units, c.plan[1] = walk.runs.runs;
   GroupedItem item;
@@ -1005,7 +1022,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       uint32_t turns = 0, meetings = 0;
       // the tiles as GroupedWalk has them, with no more of them kept than is needed (t: of rows, n: of classes)
       const int64_t all = (int64_t)c.tiles_m * c.tiles_n;
-      int at = c.keep ? (int)(blockIdx.x * all / gridDim.x) : (int)blockIdx.x, left = c.keep ? (int)((blockIdx.x + 1) * all / gridDim.x) - at : ((int)all - at + gridDim.x - 1) / (int)gridDim.x;
+      int at = c.keep ? (int)(blockIdx.x * all / gridDim.x) : (int)blockIdx.x, left = idle ? 0 : c.keep ? (int)((blockIdx.x + 1) * all / gridDim.x) - at : ((int)all - at + gridDim.x - 1) / (int)gridDim.x;
       int n = at / c.tiles_m, t = at % c.tiles_m - 1, buffer = kBuffers - 1, half = 0, halves = 0;
       // the lane's row, how many of the warp's 32 there are, the tile's columns, their number
       int row = 0, rows = 0, n0 = 0, part = 0, ahead_row = 0, ahead_rows = 0, ahead_n = 0;
@@ -1190,7 +1207,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             if (c.out) {      // whole sums
               if (quarter * 32 < item.rows - half * kTileM)
                 store_tile<T, T, MODE>(acc, empty, mine, lane, quarter, turn, kTurns, (T*)c.out + (item.row + half * kTileM) * c.num_n + item.n0, (int64_t)c.num_n,
-                                       min(item.rows - half * kTileM, c.tile_m), columns, nullptr, 0u, carry, 0, 0, Multiplied{sum_scale(c.loss)});
+                                       min(item.rows - half * kTileM, c.tile_m), columns, nullptr, 0u, carry, 0, 0, Multiplied{there ? row_scale(c.loss, row) : 0.0f});
             } else {
               tile_to_slot<T, MODE>(sums, turn, kTurns, columns, c.carry + ((item.piece * c.halves + half) * 4 + quarter) * 32 * Tr::kMostN + lane * 4, c.loss.more || item.first);
             }

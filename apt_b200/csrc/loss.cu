@@ -11,13 +11,16 @@
 //
 // The slopes' factors g_r are kept out of them as far as they are common to all rows, and multiplied to the sums of dx and dW: in 16 bits the
 // label's slope, p - 1, is then next to a power of two, and f16 has them times 2^14, so that probabilities down to 4e-9 are numbers and not
-// steps of its smallest. Fewer than 2^-11 (f16; bf16 2^-8) of a slope are lost to its rounding.
+// steps of its smallest. Fewer than 2^-11 (f16; bf16 2^-8) of a slope are lost to its rounding. Where every row has a gradient of its own they are in the
+// slopes, next to the largest. f16 has not the range for those of less than 2^-8 of it: then dx goes by slopes without them, and is multiplied by its row's,
+// and dW and db by slopes that are made once more, where a row adds what is more than 2^-39 of the largest gradient.
 #include "grouped.cuh"
 
 namespace apt {
 
 constexpr size_t kMostSlopes = 512ull << 20, kMostParts = 128ull << 20;
 constexpr int kPieceUnit = 256;
+constexpr float kWide = 0x1p-8f;
 constexpr float kLn2 = 0.69314718055994531f;
 
 struct RowsCall {
@@ -107,11 +110,11 @@ __global__ void __launch_bounds__(256) k_loss_rows(const __grid_constant__ RowsC
 }
 
 // Rows' own gradients go into their slopes, less the largest of those that are numbers (one that is none is its own row's matter). scale[0]: what they
-// are multiplied by there, scale[1]: what the sums over slopes are. One block.
-__global__ void __launch_bounds__(1024) k_loss_scale(const float* __restrict__ grad, int64_t rows, const float2* __restrict__ stats, float range, float* scale) {
+// are multiplied by there, scale[1]: what the sums over slopes are. wide: some that are not zero are less than 2^-8 of the largest. One block.
+__global__ void __launch_bounds__(1024) k_loss_scale(const float* __restrict__ grad, int64_t rows, const float2* __restrict__ stats, float range, float* scale, int* wide) {
   wait_for_previous();
-  __shared__ float part[32];
-  float m = 0.0f;
+  __shared__ float part[2][32];
+  float m = 0.0f, least = INFINITY;
   // (nothing is asked between the loads of eight rows: a million rows take 155 us, and 630 with a question between the two loads of each)
   constexpr int kAtOnce = 8;
   for (int64_t i0 = threadIdx.x; i0 < rows; i0 += kAtOnce * 1024) {
@@ -122,14 +125,18 @@ __global__ void __launch_bounds__(1024) k_loss_scale(const float* __restrict__ g
       g[u] = fabsf(grad[i]), y[u] = stats[i].y;
     }
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) m = fmaxf(m, !(y[u] < 0.0f) && g[u] < INFINITY ? g[u] : 0.0f);
+    for (int u = 0; u < kAtOnce; ++u) {
+      const float v = !(y[u] < 0.0f) && g[u] < INFINITY ? g[u] : 0.0f;
+      m = fmaxf(m, v), least = fminf(least, v > 0.0f ? v : INFINITY);
+    }
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o)), least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  if (threadIdx.x % 32 == 0) part[0][threadIdx.x / 32] = m, part[1][threadIdx.x / 32] = least;
   __syncthreads();
   if (threadIdx.x) return;
-  for (int w = 0; w < 32; ++w) m = fmaxf(m, part[w]);
+  for (int w = 0; w < 32; ++w) m = fmaxf(m, part[0][w]), least = fminf(least, part[1][w]);
+  *wide = least < kWide * m;
   m = m > 0.0f ? fmaxf(m, 1e-30f) : 1.0f;
   scale[0] = range / m, scale[1] = m / range;
 }
@@ -143,7 +150,6 @@ __global__ void __launch_bounds__(1024) k_loss_grad_rows(const __grid_constant__
   const int lane = threadIdx.x % 32, quad = threadIdx.x / 32 % 16, team = threadIdx.x / 512, teams = blockDim.x / 512;
   const int64_t row0 = (int64_t)blockIdx.x * 32;
   const int col0 = blockIdx.y * 64;
-  const float scale = sum_scale(c.loss);
   const int tall = c.tile_m * c.halves;
   const int64_t row = row0 + lane;
   const int t = (int)(row / tall), in = (int)(row - (int64_t)t * tall), half = in / kTileM, quarter = in % kTileM / 32;
@@ -164,6 +170,7 @@ __global__ void __launch_bounds__(1024) k_loss_grad_rows(const __grid_constant__
     if (threadIdx.x >= 256) return;
     const int r = threadIdx.x / 8, at = threadIdx.x % 8 * 8;
     if (row0 + r < c.rows && col0 + at < c.num_n) {
+      const float scale = row_scale(c.loss, row0 + r);
       float v[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) v[q] = (tile[0][r][at + q] + (teams > 1 ? tile[1][r][at + q] : 0.0f)) * scale;
@@ -175,7 +182,7 @@ __global__ void __launch_bounds__(1024) k_loss_grad_rows(const __grid_constant__
     for (int i = threadIdx.x; i < 32 * 64; i += blockDim.x) {
       const int64_t r = row0 + i / 64;
       const int at = i % 64;
-      if (r < c.rows && col0 + at < c.num_n) out[r * c.num_n + col0 + at] = Elem<T>::from_f((tile[0][i / 64][at] + (teams > 1 ? tile[1][i / 64][at] : 0.0f)) * scale);
+      if (r < c.rows && col0 + at < c.num_n) out[r * c.num_n + col0 + at] = Elem<T>::from_f((tile[0][i / 64][at] + (teams > 1 ? tile[1][i / 64][at] : 0.0f)) * row_scale(c.loss, r));
     }
   }
 }
@@ -360,6 +367,7 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
   const int64_t pitch = align_up(most, 64);
   T* const slopes = arena->take<T>(q.rows * pitch);
   float* const scale = arena->take<float>(2);
+  int* const wide = arena->take<int>(1);
   float* const carry = carry_of<T>(arena, q.dim);
   void* const clean = arena->take<char>((size_t)q.rows * x.pitch * sizeof(T));
   GroupedCall sum_x = listed_call<T, kSumX>(q.rows, q.dim, most);
@@ -393,23 +401,30 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
   call.labels = q.labels, call.pitch = pitch, call.stats = (const float2*)saved, call.range = range;
   if (each && q.rows > 1) {
     call.grad = grad, call.scale = scale;
-    APT_FOLLOW(k_loss_scale, 1, 1024, 0, s, grad, q.rows, (const float2*)saved, range, scale);
+    APT_FOLLOW(k_loss_scale, 1, 1024, 0, s, grad, q.rows, (const float2*)saved, range, scale, wide);
   } else {
     call.common = grad, call.count = q.reduction == APT_LOSS_MEAN ? saved + 2 * q.rows : nullptr;
   }
+  // dx by its rows' own gradients (where they are wide), and slopes for dW and db by themselves then
+  LossCall call_x = call;
+  if (std::is_same<T, __half>::value && call.scale && grad_x) call_x.wide = wide, call_x.own = 1;
   for (int64_t v0 = 0; v0 < q.classes; v0 += piece) {
     const int64_t n = std::min(piece, q.classes - v0);
     const Operand some = some_rows(w, v0, n, sizeof(T));
     GroupedCall c = listed_call<T, kSlopes>(q.rows, n, q.dim);
     c.bias = q.bias ? (const T*)q.bias + v0 : nullptr, c.carry = carry, c.out = slopes, c.status = q.status;
-    c.loss = call, c.loss.class0 = v0;
+    c.loss = call_x, c.loss.class0 = v0;
     if (const int e = run_listed<T, kSlopes>(c, x, some, s)) return e;
     const Operand dz = {slopes, 0, q.rows, n, pitch};
     if (grad_x) {
       GroupedCall d = sum_x;
       d.num_k = (int)n, d.splits = (int)ceil_div(ceil_div(n, GroupedTraits<T, kSumX>::kBlock * d.deep), d.split_stages);
-      d.status = q.status, d.loss = call, d.loss.more = v0 > 0, d.out = whole_x ? grad_x : nullptr;
+      d.status = q.status, d.loss = call_x, d.loss.more = v0 > 0, d.out = whole_x ? grad_x : nullptr;
       if (const int e = run_listed<T, kSumX>(d, dz, some, s)) return e;
+    }
+    if (call_x.own && (grad_weight || grad_bias)) {
+      c.loss = call, c.loss.class0 = v0, c.loss.wide = wide, c.loss.again = 1;
+      if (const int e = run_listed<T, kSlopes>(c, x, some, s)) return e;
     }
     if (grad_weight && tall_weights<T>(q.dim, most)) {
       if constexpr (sizeof(T) == 2) {
@@ -445,7 +460,7 @@ static int loss_backward(const LossProblem& q, const float* saved, const float* 
     }
   }
   if (grad_x && !whole_x) {
-    sum_x.loss = call;
+    sum_x.loss = call_x;
     const dim3 grid((unsigned)ceil_div(q.rows, 32), (unsigned)ceil_div(q.dim, 64));
     if (q.dim % 8 == 0) APT_FOLLOW((k_loss_grad_rows<T, true>), grid, splits >= 16 ? 1024 : 512, 0, s, sum_x, (T*)grad_x, splits);
     else APT_FOLLOW((k_loss_grad_rows<T, false>), grid, splits >= 16 ? 1024 : 512, 0, s, sum_x, (T*)grad_x, splits);

@@ -245,6 +245,40 @@ def test_rows_that_do_not_count_have_no_gradient_whatever_the_loss_has(rows, dim
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim,classes,bias", [(300, 64, 50_000, True), (200, 32, 6000, False), (257, 33, 8000, True), (20_000, 64, 700, True),
+                                                   (8192, 40, 40_000, False)])
+def test_row_gradients_over_seven_decades(rows, dim, classes, bias, dtype):
+    """dx of every row is right next to its own gradient. In f16 what a row adds to dW has steps of 2^-24 of 2^-14 of the largest gradient."""
+    x, w, b, labels = _inputs(rows, dim, classes, dtype, bias=bias, scale=0.5)
+    w += 1.0      # what probabilities lose as a whole shows in dx then
+    grad = 1e3 * 10.0 ** (-7.0 * torch.arange(rows, device="cuda") / rows)
+    grad[::3] *= -1.0
+    grad[7] = 0.0
+    _, slopes, magnitudes, counted = _plain(x, w, b, labels)
+    size = float((x.double().abs() @ w.double().abs().t()).max()) + (float(b.double().abs().max()) if bias else 0.0)
+    near, half = (dim * 2.0 ** -23 + 2.0 ** -19) * (size + 8) + HALF[dtype] + 3e-5, HALF[dtype]
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    saved = apt_b200.linear_cross_entropy(x, w, labels, b, "none", return_saved=True)[1]
+    g = grad.double().unsqueeze(1)
+    slopes, magnitudes = slopes * g, magnitudes * g.abs()
+    step = 2.0 ** -39 * 1e3 if dtype == torch.float16 else 0.0
+    wants = [(slopes @ w.double(), magnitudes @ w.double().abs(), 0.0), (slopes.t() @ x.double(), magnitudes.t() @ x.double().abs(), step * float(x.double().abs().sum(0).max()))]
+    if bias:
+        wants.append((slopes.sum(0), magnitudes.sum(0), step * rows))
+    every = apt_b200.linear_cross_entropy_backward(x, w, labels, saved, grad, b, "none")
+    for i, (want, terms, least) in enumerate(wants):
+        alone = apt_b200.linear_cross_entropy_backward(x, w, labels, saved, grad, b, "none", i == 0, i == 1, i == 2)[i]
+        for got in (every[i], alone):
+            assert bool(((got.double() - want).abs() <= near * terms + half * want.abs() + tiny + least).all())
+        assert i == 2 or torch.equal(every[i], alone)
+    assert not every[0][~counted].any() and not every[0][7].any()
+    fine = torch.arange(rows, device="cuda") != 11
+    grad[~counted], grad[11] = float("nan"), float("inf")
+    assert torch.equal(apt_b200.linear_cross_entropy_backward(x, w, labels, saved, grad, b, "none", True, False, False)[0][fine], every[0][fine])
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("polls", [0, 1, 6, 50])
 @pytest.mark.parametrize("rows,dim,classes", [(300, 128, 700), (3000, 64, 1500), (700, 1024, 25_000)])
 def test_the_kernels_end_when_a_wait_runs_out(rows, dim, classes, dtype, polls):

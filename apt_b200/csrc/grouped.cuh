@@ -79,7 +79,7 @@ struct GroupedTraits {
 // 2^(log2(e) z - that).
 struct LossCall {
   const int64_t* labels;
-  int64_t class0, ignore;       // the classes' first, the label of rows that do not count
+  int64_t class0;               // the classes' first
   int64_t pitch;                // of the parts and of the slopes
   float2* parts;                // [tiles of classes][pitch]
   float* picked;                // the logit of the row's label
@@ -563,7 +563,7 @@ __device__ __forceinline__ void store_tile(uint32_t acc, bool empty, char* stagi
 }
 
 // ---- logits of linear_cross_entropy ---------------------------------------------------
-// log2(e) is taken as the fp32 number next to it, wherever statistics and probabilities are made: all logits 1e-8 of themselves larger.
+// log2(e) is taken as the fp32 number next to it, wherever statistics and probabilities are made: all logits 1.3e-8 of themselves smaller.
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Of a row: the largest of its logits in these columns, in units of log2(e), and the sum of 2^(what the others are below it). The exponent is one

@@ -779,6 +779,12 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   float* const all_bias = (float*)(staging + Tr::kOutWarps * Tr::kStaging);      // of a tile in out; in dw the sums of db that several threads have
   int *const prefix = (int*)(all_bias + Tr::kBiasFloats), *const begin = prefix + c.groups + 2;
 
+  if constexpr (MODE == kSlopes && std::is_same<T, __half>::value) {
+    if (c.loss.again) {      // nothing is held yet: slopes that are there already are right for dW and db too
+      wait_for_previous();
+      if (!*c.loss.wide) return;
+    }
+  }
   if (warp == 1) tmem_alloc(shared_addr(&tmem_slot), 512);
   if (threadIdx.x == 0) {
     for (int k = 0; k < kMaxStages; ++k) {
@@ -837,9 +843,6 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   tmem_fence_after();
   const uint32_t tmem = tmem_slot;
   GroupedWalk<T, MODE> walk(c, prefix, begin);
-  // (the slopes that are there already are right for dW and db too)
-  const bool idle = MODE == kSlopes && c.loss.again && !*c.loss.wide;
-  if (idle) walk.next = walk.end;
   if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *c.loss.turn = 0, *c.loss.dirty = 0;
   if (Tr::kOverRows && !Tr::kTall && blockIdx.x == 0 && threadIdx.x == 0) c.plan[0] = walk.runs.units, c.plan[1] = walk.runs.runs;
   GroupedItem item;
@@ -1022,7 +1025,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       uint32_t turns = 0, meetings = 0;
       // the tiles as GroupedWalk has them, with no more of them kept than is needed (t: of rows, n: of classes)
       const int64_t all = (int64_t)c.tiles_m * c.tiles_n;
-      int at = c.keep ? (int)(blockIdx.x * all / gridDim.x) : (int)blockIdx.x, left = idle ? 0 : c.keep ? (int)((blockIdx.x + 1) * all / gridDim.x) - at : ((int)all - at + gridDim.x - 1) / (int)gridDim.x;
+      int at = c.keep ? (int)(blockIdx.x * all / gridDim.x) : (int)blockIdx.x, left = c.keep ? (int)((blockIdx.x + 1) * all / gridDim.x) - at : ((int)all - at + gridDim.x - 1) / (int)gridDim.x;
       int n = at / c.tiles_m, t = at % c.tiles_m - 1, buffer = kBuffers - 1, half = 0, halves = 0;
       // the lane's row, how many of the warp's 32 there are, the tile's columns, their number
       int row = 0, rows = 0, n0 = 0, part = 0, ahead_row = 0, ahead_rows = 0, ahead_n = 0;

@@ -1196,13 +1196,15 @@ class ExpertRows:
 
 def expert_sum(y: torch.Tensor, weights: torch.Tensor, place: torch.Tensor) -> torch.Tensor:
     """out[r] = sum_j weights[r, j] y[place[r, j]] over the pairs that have an expert: y [R k, D], weights float32 [R, k] (or [R]), place as
-    expert_rows gave it; out [R, D]. Sums are in fp32 and rounded once."""
+    expert_rows gave it, so that every row of y is one pair's (places beyond y count for nothing and raise at the next host read); out [R, D].
+    Sums are in fp32 and rounded once."""
     return _native.expert_sum(y, weights, place, STATE.words())
 
 
 def expert_sum_backward(y, weights, place, grad_out, want_y: bool = True, want_weights: bool = True):
     """Gradients of expert_sum for grad_out [R, D]: (grad_y, grad_weights), None where not wanted. Rows of pairs without an expert have
-    gradients of zero."""
+    gradients of zero. place has to name every row of y once, as expert_rows' does: a row of grad_y that no place names holds anything, one
+    that two name the gradient of either."""
     return _native.expert_sum_backward(y, weights, place, grad_out, bool(want_y), bool(want_weights), STATE.words())
 
 

@@ -889,7 +889,8 @@ int apt_route_experts_backward(int dtype, const void* logits, int64_t rows, int6
  * operators of ragged groups take them, place [rows, k] where pair (r, j) went. A
  * pair whose expert is -1 goes behind the last group, its row is zeros and its place
  * -1 - the position. Experts beyond those set APT_FLAG_ID_OUT_OF_RANGE and
- * count as -1. num_experts at most APT_GROUPED_LINEAR_MAX_GROUPS. */
+ * count as -1. num_experts at most APT_GROUPED_LINEAR_MAX_GROUPS, rows k below
+ * 2^31 - 1024 (there and in apt_expert_sum). */
 size_t apt_expert_rows_workspace_bytes(int64_t pairs, int64_t num_experts);
 int apt_expert_rows(const void* x, int64_t rows, int64_t row_bytes, const int64_t* experts, int64_t k, int64_t num_experts,
                     void* out, int64_t* offsets, int64_t* place, void* workspace, size_t workspace_bytes,
@@ -897,9 +898,11 @@ int apt_expert_rows(const void* x, int64_t rows, int64_t row_bytes, const int64_
 
 /* out[r] = sum_j weights[r, j] y[place[r, j]] over the pairs with an expert: y
  * [rows k, dim], weights [rows, k] or NULL (ones: the gradient of apt_expert_rows),
- * place as apt_expert_rows gave it (places beyond y set APT_FLAG_ID_OUT_OF_RANGE and
- * count for nothing). Backward: grad_y [rows k, dim], zeros for the pairs without
- * an expert, and grad_weights [rows, k]; each unless NULL. */
+ * place as apt_expert_rows gave it: every row of y is one pair's. (Places beyond y
+ * set APT_FLAG_ID_OUT_OF_RANGE and count for nothing.) Backward: grad_y [rows k,
+ * dim], zeros for the pairs without an expert, and grad_weights [rows, k]; each
+ * unless NULL. A row of grad_y that no place names is not written, of one that two
+ * name either's is kept: such a y has no gradient here. */
 int apt_expert_sum(int dtype, const void* y, int64_t rows, int64_t dim, int64_t k, const float* weights, const int64_t* place,
                    void* out, int32_t* status_word, void* stream);
 int apt_expert_sum_backward(int dtype, const void* y, int64_t rows, int64_t dim, int64_t k, const float* weights, const int64_t* place,
@@ -913,7 +916,7 @@ int apt_expert_sum_backward(int dtype, const void* y, int64_t rows, int64_t dim,
  * where none does). saved [2 rows + 2] is for the backward, which gives grad_x,
  * grad_weight and grad_bias (each unless NULL) for grad_loss [rows] or [1]. Both are
  * NaN where a row that counts has a logit that is NaN or +inf; rows that are out may
- * hold anything. dim at most
+ * hold anything, their own grad_loss too, and have a grad_x of zero. dim at most
  * APT_GROUPED_LINEAR_MAX_DIM. The workspace is aligned to 256 bytes. */
 typedef enum apt_loss_reduction { APT_LOSS_NONE = 0, APT_LOSS_SUM = 1, APT_LOSS_MEAN = 2 } apt_loss_reduction;
 size_t apt_linear_cross_entropy_workspace_bytes(int dtype, int64_t rows, int64_t dim, int64_t classes, int backward);

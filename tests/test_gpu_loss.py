@@ -278,6 +278,36 @@ def test_row_gradients_over_seven_decades(rows, dim, classes, bias, dtype):
     ops.check_status()
 
 
+
+@pytest.mark.parametrize("rows,dim,classes", [(300, 64, 5000), (20_000, 64, 700)])
+def test_a_captured_backward_takes_row_gradients_of_any_range(rows, dim, classes):
+    """f16: whether slopes are made once or twice goes by the gradients that are there at the replay."""
+    x, w, b, labels = _inputs(rows, dim, classes, torch.float16)
+    saved = apt_b200.linear_cross_entropy(x, w, labels, b, "none", return_saved=True)[1]
+    near = torch.rand(rows, device="cuda", generator=_gen(1)) + 0.5
+    far = near * 10.0 ** (-6.0 * torch.arange(rows, device="cuda") / rows)
+    grad = near.clone()
+
+    def call():
+        return apt_b200.linear_cross_entropy_backward(x, w, labels, saved, grad, b, "none")
+
+    call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        captured = call()
+    torch.cuda.current_stream().wait_stream(side)
+    seen = []
+    for now in (far, near, far):
+        grad.copy_(now)
+        graph.replay()
+        seen.append([t.clone() for t in captured])
+        assert all(torch.equal(a, b) for a, b in zip(seen[-1], call()))
+    assert all(torch.equal(a, b) for a, b in zip(seen[0], seen[2])) and not torch.equal(seen[0][0], seen[1][0])
+    ops.check_status()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("polls", [0, 1, 6, 50])
 @pytest.mark.parametrize("rows,dim,classes", [(300, 128, 700), (3000, 64, 1500), (700, 1024, 25_000)])

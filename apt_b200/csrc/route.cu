@@ -13,7 +13,7 @@
 // more wanted than there are lanes) the bound is raised by halves first. An expert whose logit is -inf is never chosen: where fewer are left than k, the
 // others are -1 with weight 0.
 //
-// Ranks are those of the exact scores. Without a bias logits are compared as they are. In 32 bits two logistic scores differ by less than 2^-20.9 from
+// Ranks are those of the scores in 64 bits, which are taken for exact. Without a bias logits are compared as they are. In 32 bits two logistic scores differ by less than 2^-20.9 from
 // what they should: s (1 - s) (2^-24 |z| + 2^-22) for the rounded argument and the exponential, and three quarters of 2^-22 s for sum and reciprocal, twice. Two
 // of a softmax by less than 2^-18.4 of the row's largest: 2^-21.2 each (2^-23 |d| exp(-|d|) for the differences' rounding, 2^-22 and 2^-23 for exponential
 // and product), and the sum of up to 1024 exponentials, 2^-18.9, which all scores share. Their sum with the bias is off by 2^-24 of itself. Where

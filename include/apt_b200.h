@@ -868,7 +868,7 @@ int apt_grouped_linear_backward(int dtype, const void* x, int64_t rows, int64_t 
  * logits) are chosen, ties to the lowest index, largest first; with groups > 1
  * equal runs of experts, only out of the top_groups groups whose best (or whose
  * best two, added up) of s + bias (NULL: of s) are largest. Ranks are those of the
- * exact scores. chosen [rows, k], weights [rows, k] = scale s, divided by the
+ * scores in 64 bits. chosen [rows, k], weights [rows, k] = scale s, divided by the
  * sum of the row's chosen s where renormalize is not 0. An expert whose logit or
  * s + bias is -inf is never chosen; where fewer than k are left the others are -1
  * with weight 0. Rows with a NaN: any experts, NaN weights.
